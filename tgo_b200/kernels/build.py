@@ -48,6 +48,8 @@ LIBRARIES = {
     "gemm_skinny": (["gemm_skinny.cu"], []),
     "gemm_tc": (["gemm_tc.cu"], []),
     "sampling": (["sampling.cu"], []),
+    "beams": (["beams.cu"], []),
+    "adapters": (["adapters.cu"], []),
     # host code only (no kernel): the cache books and the packing of a step
     "host_runtime": (["host_runtime.cpp"], []),
     # calls of the other libraries' entry points (a Python extension; see `entry_points`)

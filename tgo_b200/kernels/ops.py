@@ -7,6 +7,9 @@ nothing falls back to it. A refused size raises with the kernel's name in the me
 from __future__ import annotations
 
 import ctypes
+import itertools
+import math
+from array import array
 from operator import index
 from typing import Optional
 
@@ -2092,6 +2095,110 @@ def logits_adjust(row: torch.Tensor, bias_ids: Optional[torch.Tensor],
                                  _ptr(counts), c_int(ni), c_float(repetition), c_float(presence),
                                  c_float(frequency), c_int(row.numel()), _stream()),
            "logits_adjust")
+
+
+BEAM_MAX_PICKS, BEAM_MAX = 64, 32      # continuations and beams of a request that the kernels take
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, picked: torch.Tensor,
+                parents: torch.Tensor, tokens: torch.Tensor) -> None:
+    """The best continuations of each request over its beams and the vocabulary: with v(w, i) =
+    scores[b, w] + logits[b W + w, i] - logsumexp(logits[b W + w]), the K pairs (w, i) with the
+    largest v, descending, equal ones by (w, i); picked[b] = v, parents[b] = w, tokens[b] = i.
+
+    logits float32 [B W, V] (rows may be strided); scores float32 [B, W]; picked float32, parents
+    and tokens int32, [B, K], K at most 64, W at most 32. A token at -inf is no candidate, nor is
+    any token of a beam whose score is not finite or whose logits hold a NaN, +inf or nothing but
+    -inf; a place that no candidate fills gets (-inf, -1, -1)."""
+    _need_cuda(logits, scores, picked, parents, tokens)
+    B, W = scores.shape
+    K = picked.shape[1]
+    assert logits.dim() == 2 and logits.shape[0] == B * W and logits.dtype == torch.float32 and logits.stride(1) == 1
+    assert scores.dtype == picked.dtype == torch.float32 and parents.dtype == tokens.dtype == torch.int32
+    assert picked.shape == parents.shape == tokens.shape == (B, K)
+    assert scores.is_contiguous() and picked.is_contiguous() and parents.is_contiguous() and tokens.is_contiguous()
+    if not 0 < K <= BEAM_MAX_PICKS or not 0 < W <= BEAM_MAX:
+        raise KernelError(f"beam_select: {W} beams and {K} continuations; at most {BEAM_MAX} and {BEAM_MAX_PICKS}")
+    if B == 0:
+        return
+    V = logits.shape[1]
+    lib = entry_points("beams")
+    parts = lib.tgo_beam_select_parts(c_int(B), c_int(W), c_int(V))
+    work = torch.empty(B * W * parts * (1 + K), dtype=torch.int64, device=logits.device)
+    _check(lib.tgo_beam_select(_ptr(logits), c_ll(logits.stride(0)), _ptr(scores), c_int(B), c_int(W), c_int(V),
+                               c_int(K), _ptr(picked), _ptr(parents), _ptr(tokens), _ptr(work), c_int(parts),
+                               _stream()), "beam_select", f"(B={B}, W={W}, V={V}, K={K})")
+    LAUNCHES[0] += 1
+
+
+def reorder_rows(tensors, index: torch.Tensor, parents: torch.Tensor, axis: int = 0) -> None:
+    """In every tensor, for every group g: row index[g, w] <- old row index[g, parents[g, w]], in
+    place, whatever chains or exchanges the parents make (the rows of a request's beams after a
+    selection). Rows lie along `axis`; a row is everything behind it, contiguous, and what lies
+    before `axis` is gone through row by row. index, parents int32 [groups, W], W at most 32; the
+    rows named by a call are distinct. A row whose parent is itself or outside 0..W-1, or that is
+    or continues a row outside the tensor, stays as it is."""
+    _need_cuda(index, parents, *tensors)
+    G, W = index.shape
+    assert index.dtype == parents.dtype == torch.int32 and parents.shape == index.shape
+    assert index.is_contiguous() and parents.is_contiguous()
+    if not 0 < W <= BEAM_MAX:
+        raise KernelError(f"reorder_rows: groups of {W} rows; at most {BEAM_MAX}")
+    desc = array("q")
+    for t in tensors:
+        if t.numel() == 0:
+            continue
+        assert 0 <= axis < t.dim() and t.element_size() >= 2
+        outer, rows = math.prod(t.shape[:axis]), t.shape[axis]
+        size = t.element_size()
+        row = math.prod(t.shape[axis + 1:]) * size
+        step = t.stride(axis) * size if rows > 1 else row
+        # whole rows, and whatever precedes the rows evenly spaced
+        assert t.is_contiguous() or (axis == 0 and t[0].is_contiguous() and step >= row)
+        desc.extend((t.data_ptr(), outer, rows * step, rows, step, row))
+    if not desc or G == 0:
+        return
+    lib = entry_points("beams")
+    _check(lib.tgo_reorder_rows(c_ll(desc.buffer_info()[0]), c_int(len(desc) // 6), _ptr(index), _ptr(parents),
+                                c_int(G), c_int(W), _stream()), "reorder_rows")
+    LAUNCHES[0] += (len(desc) // 6 - 1) // 64
+
+
+def low_rank_add(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor,
+                 ids: torch.Tensor, widths, interleaved: bool = False,
+                 out: Optional[torch.Tensor] = None) -> None:
+    """out = y + each row's own low-rank product: with i = ids[t], out[t, n] = y[t, n] + scale[i]
+    sum_j (sum_k x[t, k] a[i, s, j, k]) b[i, n, j], s the slice of y's columns that n lies in. A row
+    whose id is outside 0..adapters-1 keeps y. `out` None: in place.
+
+    x [T, K] float32 or bfloat16, y and out [T, N] in x's type or float32, all three with rows that
+    may be strided; a [adapters, slices, rank, K], b [adapters, N, rank] in x's type; scale float32
+    [adapters]; ids int32 [T]. widths: the slices' columns, at most four slices (a joined matrix: q, k
+    and v); `interleaved`: two slices of equal width that take turns, eight columns each."""
+    out = y if out is None else out
+    _need_cuda(x, y, a, b, scale, ids, out)
+    T, K = x.shape
+    n, S, r, _ = a.shape
+    N = y.shape[1]
+    assert y.shape == out.shape == (T, N) and y.dtype == out.dtype and y.dtype in (x.dtype, torch.float32)
+    assert a.dtype == b.dtype == x.dtype and a.shape[3] == K and b.shape == (n, N, r) and S == len(widths)
+    assert a.is_contiguous() and b.is_contiguous() and x.stride(1) == y.stride(1) == out.stride(1) == 1
+    assert scale.dtype == torch.float32 and scale.shape == (n,) and scale.is_contiguous()
+    assert ids.dtype == torch.int32 and ids.shape == (T,) and ids.is_contiguous()
+    if sum(widths) != N or not 0 < S <= 4 or min(widths) <= 0 or \
+            (interleaved and (S != 2 or widths[0] != widths[1] or widths[0] % 8)):
+        raise KernelError(f"low_rank_add: slices {tuple(widths)}{' in eights' if interleaved else ''} of {N} columns")
+    if T == 0:
+        return
+    ends = array("i", itertools.accumulate(widths))
+    work = torch.empty(T * S * r, dtype=torch.float32, device=x.device)
+    lib = entry_points("adapters")
+    _check(lib.tgo_low_rank_add(_ptr(x), c_ll(x.stride(0)), _ptr(y), c_ll(y.stride(0)), _ptr(out), c_ll(out.stride(0)),
+                                _ptr(a), _ptr(b), _ptr(scale), _ptr(ids), c_int(dtype_code(x.dtype)),
+                                c_int(dtype_code(y.dtype)), c_int(T), c_int(K), c_int(N), c_int(n), c_int(r), c_int(S),
+                                c_ll(ends.buffer_info()[0]), c_int(1 if interleaved else 0), _ptr(work), _stream()),
+           "low_rank_add", f"(T={T}, K={K}, N={N}, rank={r}, slices={S})")
+    LAUNCHES[0] += 1
 
 
 _tc_err = {}
