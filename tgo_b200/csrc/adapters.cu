@@ -5,7 +5,7 @@
 // y being the projection's own result and s(n) the slice of its columns that n lies in (q, k and v of a
 // joined matrix; gate and up rows in eights): each slice has an A of its own. A row whose id names no
 // adapter keeps y. u is held in 32 bits.
-#include "common.cuh"
+#include "mma_sync.cuh"
 
 #define LR_MAX_SLICES 4
 
@@ -23,6 +23,351 @@ __device__ __forceinline__ int lr_slice(const LowRankColumns& c, int n) {
     return s;
 }
 
+struct LowRank {
+    const void *x, *y, *a, *b;
+    void* out;
+    long long x_stride, y_stride, out_stride;
+    const float* scale;
+    const int* ids;
+    int T, K, N, adapters, rank;
+    LowRankColumns columns;
+};
+
+// ------------------------------------------------------------------------- the rows of an adapter
+// For many rows: which rows have which adapter, in tiles of up to `tile` rows of one adapter (rows without
+// one come last, as tiles of adapter -1). perm: the rows by tile; info[0]: the number of tiles, a tile is
+// (adapter, first place in perm, rows). One block; the order of an adapter's rows is kept within 32.
+#define LP_THREADS 1024
+#define LP_MAX_ADAPTERS 4095
+
+__global__ void __launch_bounds__(LP_THREADS)
+low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile, int* __restrict__ perm, int* __restrict__ info,
+                     int* __restrict__ tiles) {
+    __shared__ int rows_of[LP_MAX_ADAPTERS + 1];             // rows, then the next free place
+    __shared__ int tiles_before[LP_MAX_ADAPTERS + 1];
+    __shared__ int warp_rows[32], warp_tiles[32];
+    pdl_wait();
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, slots = adapters + 1;
+    for (int i = t; i < slots; i += LP_THREADS) rows_of[i] = 0;
+    __syncthreads();
+    for (int base = warp * 32; base < T; base += LP_THREADS) {
+        const int r = base + lane;
+        const int id = r < T ? ids[r] : -2, slot = r >= T ? -1 : id >= 0 && id < adapters ? id : adapters;
+        const unsigned same = __match_any_sync(0xffffffffu, slot);
+        if (slot >= 0 && lane == __ffs(same) - 1) atomicAdd(&rows_of[slot], __popc(same));
+    }
+    __syncthreads();
+    // exclusive sums of rows and of tiles over the adapters, a thread a run of neighbours
+    const int per = (slots + LP_THREADS - 1) / LP_THREADS, first = min(t * per, slots), last = min(first + per, slots);
+    int my_rows = 0, my_tiles = 0;
+    for (int i = first; i < last; ++i) { my_rows += rows_of[i]; my_tiles += (rows_of[i] + tile - 1) / tile; }
+    int sum_rows = my_rows, sum_tiles = my_tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, sum_rows, o), b = __shfl_up_sync(0xffffffffu, sum_tiles, o);
+        if (lane >= o) { sum_rows += a; sum_tiles += b; }
+    }
+    if (lane == 31) { warp_rows[warp] = sum_rows; warp_tiles[warp] = sum_tiles; }
+    __syncthreads();
+    if (warp == 0) {
+        int a = warp_rows[lane], b = warp_tiles[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int c = __shfl_up_sync(0xffffffffu, a, o), d = __shfl_up_sync(0xffffffffu, b, o);
+            if (lane >= o) { a += c; b += d; }
+        }
+        warp_rows[lane] = a;
+        warp_tiles[lane] = b;
+    }
+    __syncthreads();
+    int at_row = sum_rows - my_rows + (warp ? warp_rows[warp - 1] : 0);
+    int at_tile = sum_tiles - my_tiles + (warp ? warp_tiles[warp - 1] : 0);
+    const int total = warp_tiles[31];
+    for (int i = first; i < last; ++i) {
+        const int n = rows_of[i];
+        rows_of[i] = at_row;
+        tiles_before[i] = at_tile;
+        at_row += n;
+        at_tile += (n + tile - 1) / tile;
+    }
+    __syncthreads();
+    if (t == 0) info[0] = total;
+    for (int q = t; q < total; q += LP_THREADS) {
+        int lo = 0, hi = slots - 1;                          // the last adapter whose tiles begin at q or before
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (tiles_before[mid] <= q) lo = mid; else hi = mid - 1;
+        }
+        const int begin = rows_of[lo] + (q - tiles_before[lo]) * tile;
+        const int end = lo + 1 < slots ? rows_of[lo + 1] : T;
+        tiles[3 * q] = lo < adapters ? lo : -1;
+        tiles[3 * q + 1] = begin;
+        tiles[3 * q + 2] = min(tile, end - begin);
+    }
+    __syncthreads();
+    for (int base = warp * 32; base < T; base += LP_THREADS) {
+        const int r = base + lane;
+        const int id = r < T ? ids[r] : -2, slot = r >= T ? -1 : id >= 0 && id < adapters ? id : adapters;
+        const unsigned same = __match_any_sync(0xffffffffu, slot);
+        const int leader = __ffs(same) - 1;
+        int place = 0;
+        if (slot >= 0 && lane == leader) place = atomicAdd(&rows_of[slot], __popc(same));
+        place = __shfl_sync(0xffffffffu, place, leader);
+        if (slot >= 0) perm[place + __popc(same & ((1u << lane) - 1))] = r;
+    }
+}
+
+// ---------------------------------------------------------------------- few rows of an adapter
+// A cluster of eight blocks takes up to eight rows of one adapter. Each block forms u over an eighth of k,
+// the blocks read each other's sums from shared memory, and each then makes an eighth of the columns: one
+// launch, and every number of A and B is read once for eight rows. Bound by the adapters' way from memory or
+// L2 when many rows have one each, by latency for a handful.
+//
+// bfloat16: the adapter's rows are the 16 rows of mma.sync products, the batch's rows their 8 columns, both
+// straight from memory into the operands' registers: which 16 values of k meet in a product does not
+// matter as long as both sides agree, so a thread takes eight neighbouring ones (16 bytes). For the second
+// product u is two bfloat16 numbers, its value rounded and the rest rounded: 2^-17 of it is lost.
+// float32: plain sums, a warp four values of u for all eight rows, its lanes over k; u's and the result's
+// order of additions depends on K and the rank alone, whatever the batch.
+//
+// Without a plan every row has a cluster, which looks through the ids: the first, ninth, ... row of an
+// adapter takes up to seven further ones, the others leave.
+#define LF_ROWS 8
+#define LF_CTAS 8
+#define LF_THREADS 256
+#define LF_WARPS (LF_THREADS / 32)
+#define LF_PASS 64                // values of u a pass, bfloat16
+
+__device__ __forceinline__ void lf_cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void lf_cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ float4 lf_peer(const float* mine, int rank) {
+    float4 v;
+    asm volatile("{\n\t.reg .u32 p;\n\tmapa.shared::cluster.u32 p, %4, %5;\n\t"
+                 "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [p];\n\t}"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(smem_u32(mine)), "r"(rank) : "memory");
+    return v;
+}
+
+// Floats of shared memory: u of all blocks [8][width + 4], this block's [8][width], then partial sums
+// [8 warps][64][8] (bfloat16) or the block's part of x [8][k] (float32).
+template <typename T> static inline long long lf_floats(int width, int K) {
+    const long long tail = sizeof(T) == 2 ? LF_WARPS * LF_PASS * LF_ROWS : (long long)LF_ROWS * ((((K + LF_CTAS - 1) / LF_CTAS) + 3) / 4 * 4);
+    return (long long)LF_ROWS * (2 * width + 4) + tail;
+}
+
+template <typename T, typename TY>
+__global__ void __launch_bounds__(LF_THREADS)
+low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __restrict__ info, const int* __restrict__ tiles) {
+    extern __shared__ __align__(16) float lf_smem[];
+    __shared__ int rows[LF_ROWS];
+    __shared__ int warp_count[LF_WARPS];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int item = blockIdx.x / LF_CTAS, cta = blockIdx.x % LF_CTAS;
+    pdl_wait();
+    int id, n;
+    if (tiles) {
+        if (item >= info[0]) return;
+        id = tiles[3 * item];
+        n = tiles[3 * item + 2];
+        if (t < n) rows[t] = perm[tiles[3 * item + 1] + t];
+        __syncthreads();
+    } else {
+        id = p.ids[item];
+        n = 1;
+        if (t == 0) rows[0] = item;
+        if (id >= 0 && id < p.adapters) {
+            int before = 0;
+            for (int base = 0; base < item; base += LF_THREADS)
+                before += __syncthreads_count(base + t < item && p.ids[base + t] == id);
+            if (before % LF_ROWS) return;
+            for (int base = item + 1; base < p.T && n < LF_ROWS; base += LF_THREADS) {
+                const bool same = base + t < p.T && p.ids[base + t] == id;
+                const unsigned who = __ballot_sync(0xffffffffu, same);
+                if (lane == 0) warp_count[warp] = __popc(who);
+                __syncthreads();
+                int place = n, all = 0;
+#pragma unroll
+                for (int w = 0; w < LF_WARPS; ++w) {
+                    place += w < warp ? warp_count[w] : 0;
+                    all += warp_count[w];
+                }
+                place += __popc(who & ((1u << lane) - 1));
+                if (same && place < LF_ROWS) rows[place] = base + t;
+                n += all;
+                __syncthreads();
+            }
+            n = min(n, LF_ROWS);
+        }
+        __syncthreads();
+    }
+    const TY* const y = (const TY*)p.y;
+    TY* const out = (TY*)p.out;
+    const int pairs = (p.N + 31) / 32, col0 = min((pairs * cta / LF_CTAS) * 32, p.N), col1 = min((pairs * (cta + 1) / LF_CTAS) * 32, p.N);
+    if (id < 0 || id >= p.adapters) {                        // no adapter: y as it is
+        if (p.out != p.y)
+            for (int i = 0; i < n; ++i)
+                for (int c = col0 + t; c < col1; c += LF_THREADS) out[(size_t)rows[i] * p.out_stride + c] = y[(size_t)rows[i] * p.y_stride + c];
+        return;
+    }
+    const int rank = p.rank, width = p.columns.slices * rank, K = p.K;
+    const T* const a = (const T*)p.a + (size_t)id * width * K;
+    const T* const b = (const T*)p.b + (size_t)id * p.N * rank;
+    float* const u = lf_smem;                                // [8][width + 4]
+    float* const part = u + LF_ROWS * (width + 4);           // [8][width]
+    float* const tail = part + LF_ROWS * width;
+    {   // B's rows and y, which are read last, are asked for now
+        const char* const from = (const char*)(b + (size_t)col0 * rank);
+        const int bytes = (col1 - col0) * rank * (int)sizeof(T);
+        for (int o = t * 128; o < bytes; o += LF_THREADS * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(from + o));
+    }
+
+    if constexpr (sizeof(T) == 2) {
+        const int g = lane >> 2, tig = lane & 3, blocks = (K + 31) / 32;
+        const bf16* const x = (const bf16*)p.x + (size_t)rows[g < n ? g : 0] * p.x_stride;
+        float* const red = tail;                             // [warp][value of u][row]
+        for (int j0 = 0; j0 < width; j0 += LF_PASS) {
+            float acc[LF_PASS / 16][4] = {};
+#pragma unroll 2
+            for (int kb = cta * LF_WARPS + warp; kb < blocks; kb += LF_CTAS * LF_WARPS) {
+                const int k = kb * 32 + tig * 8;
+                const uint4 zero = make_uint4(0, 0, 0, 0);
+                const uint4 xv = g < n && k < K ? *(const uint4*)(x + k) : zero;
+#pragma unroll
+                for (int m = 0; m < LF_PASS / 16; ++m) {
+                    const int j = j0 + m * 16 + g;
+                    if (j0 + m * 16 < width) {
+                        const uint4 lo = k < K && j < width ? *(const uint4*)(a + (size_t)j * K + k) : zero;
+                        const uint4 hi = k < K && j + 8 < width ? *(const uint4*)(a + (size_t)(j + 8) * K + k) : zero;
+                        const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, a1[4] = {lo.z, hi.z, lo.w, hi.w};
+                        mma_bf16(acc[m], a0, xv.x, xv.y);
+                        mma_bf16(acc[m], a1, xv.z, xv.w);
+                    }
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < LF_PASS / 16; ++m) {
+                float* const to = red + (warp * LF_PASS + m * 16 + g) * LF_ROWS + 2 * tig;
+                *(float2*)to = make_float2(acc[m][0], acc[m][1]);
+                *(float2*)(to + 8 * LF_ROWS) = make_float2(acc[m][2], acc[m][3]);
+            }
+            __syncthreads();
+            for (int e = t; e < LF_PASS * LF_ROWS; e += LF_THREADS) {
+                const int j = j0 + e / LF_ROWS;
+                float s = 0.f;
+#pragma unroll
+                for (int w = 0; w < LF_WARPS; ++w) s += red[w * LF_PASS * LF_ROWS + e];
+                if (j < width) part[(e % LF_ROWS) * width + j] = s;
+            }
+            __syncthreads();
+        }
+    } else {
+        const int kc = ((K + LF_CTAS - 1) / LF_CTAS + 3) / 4 * 4, k0 = min(cta * kc, K), k1 = min(k0 + kc, K);
+        float* const xs = tail;                              // [row][k of the block]
+        for (int r = 0; r < LF_ROWS; ++r)
+            for (int k = t * 4; k < k1 - k0; k += LF_THREADS * 4)
+                *(float4*)(xs + r * kc + k) = r < n ? *(const float4*)((const float*)p.x + (size_t)rows[r] * p.x_stride + k0 + k)
+                                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+        __syncthreads();
+        for (int j0 = warp * 4; j0 < width; j0 += 4 * LF_WARPS) {
+            float v[4 * LF_ROWS] = {};
+            for (int k = lane * 4; k < k1 - k0; k += 128) {
+                float4 w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    w[j] = j0 + j < width ? *(const float4*)((const float*)a + (size_t)(j0 + j) * K + k0 + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int r = 0; r < LF_ROWS; ++r) {
+                    const float4 q = *(const float4*)(xs + r * kc + k);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        v[j * LF_ROWS + r] = fmaf(q.w, w[j].w, fmaf(q.z, w[j].z, fmaf(q.y, w[j].y, fmaf(q.x, w[j].x, v[j * LF_ROWS + r]))));
+                }
+            }
+            // 32 sums over the lanes: each step halves the sums a lane has, after five lane l has sum l
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                for (int i = 0; i < o; ++i) {
+                    const float give = lane & o ? v[i] : v[i + o], keep = lane & o ? v[i + o] : v[i];
+                    v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                }
+            if (j0 + lane / LF_ROWS < width) part[(lane % LF_ROWS) * width + j0 + lane / LF_ROWS] = v[0];
+        }
+    }
+    lf_cluster_arrive();
+    lf_cluster_wait();
+    const float scale = p.scale[id];
+    for (int e = t * 4; e < LF_ROWS * width; e += LF_THREADS * 4) {
+        float4 s = lf_peer(part + e, 0);
+#pragma unroll
+        for (int r = 1; r < LF_CTAS; ++r) {
+            const float4 q = lf_peer(part + e, r);
+            s.x += q.x; s.y += q.y; s.z += q.z; s.w += q.w;
+        }
+        *(float4*)(u + (e / width) * (width + 4) + e % width) = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
+    }
+    lf_cluster_arrive();                                     // waited for at the end: a peer may still be reading `part`
+    __syncthreads();
+
+    if constexpr (sizeof(T) == 2) {
+        const int g = lane >> 2, tig = lane & 3;
+        const int r0 = 2 * tig < n ? rows[2 * tig] : -1, r1 = 2 * tig + 1 < n ? rows[2 * tig + 1] : -1;
+#pragma unroll 2
+        for (int q = col0 / 16 + warp; q < col1 / 16; q += LF_WARPS) {
+            // the tile's column of the product's row g, and how much further that of row g + 8 is
+            const int c = p.columns.interleaved ? q / 2 * 32 + (q & 1) * 8 + g : q * 16 + g, far = p.columns.interleaved ? 16 : 8;
+            const int s = p.columns.interleaved ? q & 1 : lr_slice(p.columns, q * 16);
+            const bf16* const w = b + (size_t)c * rank;
+            float v[4];
+            v[0] = r0 >= 0 ? to_f32(y[(size_t)r0 * p.y_stride + c]) : 0.f;
+            v[1] = r1 >= 0 ? to_f32(y[(size_t)r1 * p.y_stride + c]) : 0.f;
+            v[2] = r0 >= 0 ? to_f32(y[(size_t)r0 * p.y_stride + c + far]) : 0.f;
+            v[3] = r1 >= 0 ? to_f32(y[(size_t)r1 * p.y_stride + c + far]) : 0.f;
+            float acc[4] = {};
+            for (int k = 4 * tig; k - 4 * tig < rank; k += 16) {
+                uint2 lo = make_uint2(0, 0), hi = lo;
+                float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (k < rank) {
+                    lo = *(const uint2*)(w + k);
+                    hi = *(const uint2*)(w + (size_t)far * rank + k);
+                    f = *(const float4*)(u + g * (width + 4) + s * rank + k);
+                }
+                const uint32_t m[4] = {lo.x, hi.x, lo.y, hi.y};
+                const float4 h = make_float4(to_f32(from_f32<bf16>(f.x)), to_f32(from_f32<bf16>(f.y)), to_f32(from_f32<bf16>(f.z)), to_f32(from_f32<bf16>(f.w)));
+                mma_bf16(acc, m, pack_bf16(f.x, f.y), pack_bf16(f.z, f.w));
+                mma_bf16(acc, m, pack_bf16(f.x - h.x, f.y - h.y), pack_bf16(f.z - h.z, f.w - h.w));
+            }
+            if (r0 >= 0) {
+                out[(size_t)r0 * p.out_stride + c] = from_f32<TY>(v[0] + acc[0]);
+                out[(size_t)r0 * p.out_stride + c + far] = from_f32<TY>(v[2] + acc[2]);
+            }
+            if (r1 >= 0) {
+                out[(size_t)r1 * p.out_stride + c] = from_f32<TY>(v[1] + acc[1]);
+                out[(size_t)r1 * p.out_stride + c + far] = from_f32<TY>(v[3] + acc[3]);
+            }
+        }
+    } else {
+        for (int c = col0 + t; c < col1; c += LF_THREADS) {
+            const float* const w = (const float*)b + (size_t)c * rank;
+            const float* const us = u + lr_slice(p.columns, c) * rank;
+            float acc[LF_ROWS] = {};
+            for (int k = 0; k < rank; k += 4) {
+                const float4 q = *(const float4*)(w + k);
+#pragma unroll
+                for (int r = 0; r < LF_ROWS; ++r) {
+                    const float4 f = *(const float4*)(us + r * (width + 4) + k);
+                    acc[r] = fmaf(f.w, q.w, fmaf(f.z, q.z, fmaf(f.y, q.y, fmaf(f.x, q.x, acc[r]))));
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < LF_ROWS; ++r)
+                if (r < n) out[(size_t)rows[r] * p.out_stride + c] = from_f32<TY>(to_f32(y[(size_t)rows[r] * p.y_stride + c]) + acc[r]);
+        }
+    }
+    lf_cluster_wait();
+}
+
+// --------------------------------------------------------------------------- any sizes
 // A warp a (row, slice, j): lanes go over k, so the sum's order depends on K alone.
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -62,41 +407,110 @@ low_rank_up_kernel(const float* __restrict__ u, const T* __restrict__ b, const i
     out[(size_t)t * out_stride + n] = from_f32<TY>(v + acc);
 }
 
-template <typename T, typename TY>
-static int low_rank_launch(const void* x, long long x_stride, const void* y, long long y_stride, void* out,
-                           long long out_stride, const void* a, const void* b, const float* scale, const int* ids, int T_,
-                           int K, int N, int adapters, int rank, const LowRankColumns& columns, float* u,
-                           cudaStream_t stream) {
-    const int width = columns.slices * rank;
-    int rc = tgo_launch_pdl(low_rank_down_kernel<T>, dim3(T_, (width + 31) / 32), dim3(256), 0, stream, (const T*)x, x_stride,
-                            (const T*)a, scale, ids, adapters, width, K, u);
+// Whether the vectors of the kernels above find their boundaries: rows of x, A and B on 16 bytes, ranks of whole
+// vectors, slices of whole products.
+template <typename T> static bool lr_vectors(const LowRank& p) {
+    const int v = 16 / (int)sizeof(T);
+    if (p.K % v || p.x_stride % v || p.rank % 4 || ((uintptr_t)p.x | (uintptr_t)p.a | (uintptr_t)p.b) & 15) return false;
+    if (p.columns.interleaved) return p.N % 32 == 0;
+    for (int i = 0; i < p.columns.slices; ++i)
+        if (p.columns.ends[i] % 16) return false;
+    return true;
+}
+
+// Rows from which they are planned: up to here each cluster of the kernel for few rows finds its own.
+#define LR_SCAN_ROWS 256
+
+template <typename T> static bool lr_few_takes(const LowRank& p) {
+    return lr_vectors<T>(p) && lf_floats<T>(p.columns.slices * p.rank, p.K) * 4 <= 200 * 1024 && p.T <= (1 << 24) &&
+           (p.T <= LR_SCAN_ROWS || p.adapters <= LP_MAX_ADAPTERS);
+}
+
+// Tiles there are at most: an adapter leaves one part tile at most.
+static long long lr_tiles(const LowRank& p, int tile) {
+    return (p.T + tile - 1) / tile + (p.T < p.adapters + 1 ? p.T : p.adapters + 1);
+}
+
+template <typename T, typename TY> static int low_rank_few(const LowRank& p, int* plan, cudaStream_t stream) {
+    static bool sized[64] = {};                              // per device
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return (int)err;
+    if (dev < 0 || dev >= 64) return TGO_E_BAD_ARG;
+    if (!sized[dev]) {
+        err = cudaFuncSetAttribute(low_rank_few_kernel<T, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+        if (err != cudaSuccess) return (int)err;
+        sized[dev] = true;
+    }
+    long long items = p.T;
+    int *perm = nullptr, *info = nullptr, *tiles = nullptr;
+    if (p.T > LR_SCAN_ROWS) {
+        items = lr_tiles(p, LF_ROWS);
+        perm = plan;
+        info = perm + p.T;
+        tiles = info + 1;
+        const int rc = tgo_launch_pdl(low_rank_plan_kernel, dim3(1), dim3(LP_THREADS), 0, stream, p.ids, p.T, p.adapters, LF_ROWS, perm, info, tiles);
+        if (rc) return rc;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(items * LF_CTAS));
+    cfg.blockDim = dim3(LF_THREADS);
+    cfg.dynamicSmemBytes = (size_t)lf_floats<T>(p.columns.slices * p.rank, p.K) * 4;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = LF_CTAS;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = tgo_pdl_enabled() ? 2 : 1;
+    return (int)cudaLaunchKernelEx(&cfg, low_rank_few_kernel<T, TY>, p, (const int*)perm, (const int*)info, (const int*)tiles);
+}
+
+template <typename T, typename TY> static int low_rank_any(const LowRank& p, float* u, cudaStream_t stream) {
+    const int width = p.columns.slices * p.rank;
+    const int rc = tgo_launch_pdl(low_rank_down_kernel<T>, dim3(p.T, (width + 31) / 32), dim3(256), 0, stream, (const T*)p.x,
+                                  p.x_stride, (const T*)p.a, p.scale, p.ids, p.adapters, width, p.K, u);
     if (rc) return rc;
-    return tgo_launch_pdl(low_rank_up_kernel<T, TY>, dim3(T_, (N + 255) / 256), dim3(256), 0, stream, (const float*)u,
-                          (const T*)b, ids, adapters, rank, columns, N, (const TY*)y, y_stride, (TY*)out, out_stride);
+    return tgo_launch_pdl(low_rank_up_kernel<T, TY>, dim3(p.T, (p.N + 255) / 256), dim3(256), 0, stream, (const float*)u,
+                          (const T*)p.b, p.ids, p.adapters, p.rank, p.columns, p.N, (const TY*)p.y, p.y_stride, (TY*)p.out,
+                          p.out_stride);
+}
+
+template <typename T, typename TY> static int low_rank_launch(const LowRank& p, void* work, long long work_ints, cudaStream_t stream) {
+    if (lr_few_takes<T>(p)) {
+        if (p.T > LR_SCAN_ROWS && work_ints < p.T + 1 + 3 * lr_tiles(p, LF_ROWS)) return TGO_E_BAD_ARG;
+        return low_rank_few<T, TY>(p, (int*)work, stream);
+    }
+    if (work_ints < (long long)p.T * p.columns.slices * p.rank) return TGO_E_BAD_ARG;
+    return low_rank_any<T, TY>(p, (float*)work, stream);
+}
+
+static bool lr_fill(LowRank& p, int T, int K, int N, int adapters, int rank, int slices, const int* ends, int interleaved) {
+    if (T <= 0 || K <= 0 || N <= 0 || adapters <= 0 || rank <= 0 || slices <= 0 || slices > LR_MAX_SLICES ||
+        (N + 255) / 256 > 65535 || (interleaved && (slices != 2 || N % 16)))
+        return false;
+    p.T = T; p.K = K; p.N = N; p.adapters = adapters; p.rank = rank;
+    p.columns.slices = slices;
+    p.columns.interleaved = interleaved;
+    for (int i = 0; i < slices; ++i) p.columns.ends[i] = ends[i];
+    return true;
 }
 
 // x [T, K] of type dt, y and out [T, N] of type dt_y, rows strided; out may be y. a [adapters, slices, rank, K],
-// b [adapters, N, rank] of type dt; ends: the column after each slice's last. work: T x slices x rank floats.
+// b [adapters, N, rank] of type dt; ends: the column after each slice's last. `work` holds `work_ints` 32-bit
+// numbers: the plan of the rows (T + 1 + 3 tiles), or u (T x slices x rank) where no kernel with vectors takes
+// the call.
 TGO_API int tgo_low_rank_add(const void* x, long long x_stride, const void* y, long long y_stride, void* out,
                              long long out_stride, const void* a, const void* b, const float* scale, const int* ids,
                              int dt, int dt_y, int T, int K, int N, int adapters, int rank, int slices, const int* ends,
-                             int interleaved, float* work, cudaStream_t stream) {
+                             int interleaved, void* work, long long work_ints, cudaStream_t stream) {
     if (T <= 0) return 0;
-    if (K <= 0 || N <= 0 || adapters <= 0 || rank <= 0 || slices <= 0 || slices > LR_MAX_SLICES || (N + 255) / 256 > 65535 ||
-        (interleaved && (slices != 2 || N % 16)))
-        return TGO_E_BAD_ARG;
-    LowRankColumns c = {};
-    c.slices = slices;
-    c.interleaved = interleaved;
-    for (int i = 0; i < slices; ++i) c.ends[i] = ends[i];
-    if (dt == TGO_F32 && dt_y == TGO_F32)
-        return low_rank_launch<float, float>(x, x_stride, y, y_stride, out, out_stride, a, b, scale, ids, T, K, N, adapters,
-                                             rank, c, work, stream);
-    if (dt == TGO_BF16 && dt_y == TGO_BF16)
-        return low_rank_launch<bf16, bf16>(x, x_stride, y, y_stride, out, out_stride, a, b, scale, ids, T, K, N, adapters,
-                                           rank, c, work, stream);
-    if (dt == TGO_BF16 && dt_y == TGO_F32)
-        return low_rank_launch<bf16, float>(x, x_stride, y, y_stride, out, out_stride, a, b, scale, ids, T, K, N, adapters,
-                                            rank, c, work, stream);
+    LowRank p = {x, y, a, b, out, x_stride, y_stride, out_stride, scale, ids};
+    if (!lr_fill(p, T, K, N, adapters, rank, slices, ends, interleaved)) return TGO_E_BAD_ARG;
+    if (dt == TGO_F32 && dt_y == TGO_F32) return low_rank_launch<float, float>(p, work, work_ints, stream);
+    if (dt == TGO_BF16 && dt_y == TGO_BF16) return low_rank_launch<bf16, bf16>(p, work, work_ints, stream);
+    if (dt == TGO_BF16 && dt_y == TGO_F32) return low_rank_launch<bf16, float>(p, work, work_ints, stream);
     return TGO_E_BAD_ARG;
 }

@@ -2191,12 +2191,13 @@ def low_rank_add(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.Ten
     if T == 0:
         return
     ends = array("i", itertools.accumulate(widths))
-    work = torch.empty(T * S * r, dtype=torch.float32, device=x.device)
+    work_ints = max(T * S * r, T + 1 + 3 * (-(-T // 8) + min(T, n + 1)))
+    work = torch.empty(work_ints, dtype=torch.int32, device=x.device)
     lib = entry_points("adapters")
     _check(lib.tgo_low_rank_add(_ptr(x), c_ll(x.stride(0)), _ptr(y), c_ll(y.stride(0)), _ptr(out), c_ll(out.stride(0)),
                                 _ptr(a), _ptr(b), _ptr(scale), _ptr(ids), c_int(dtype_code(x.dtype)),
                                 c_int(dtype_code(y.dtype)), c_int(T), c_int(K), c_int(N), c_int(n), c_int(r), c_int(S),
-                                c_ll(ends.buffer_info()[0]), c_int(1 if interleaved else 0), _ptr(work), _stream()),
+                                c_ll(ends.buffer_info()[0]), c_int(1 if interleaved else 0), _ptr(work), c_ll(work_ints), _stream()),
            "low_rank_add", f"(T={T}, K={K}, N={N}, rank={r}, slices={S})")
     LAUNCHES[0] += 1
 
