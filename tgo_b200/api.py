@@ -113,15 +113,49 @@ class LoadedModel:
         from .engine.session import Session
         return Session(self, context, **kw)
 
+    def load_adapters(self, adapters: dict) -> None:
+        """Low-rank adapters for requests to name: {name: folder, or weights.adapters.Adapter}. All are
+        checked against the model and laid out together, once for a model: the graphs of its engines
+        read them where they lie."""
+        from .weights.adapters import Adapter, AdapterError, bind_adapters, read_adapter
+        if self.model.adapter_names:
+            raise AdapterError("this model's adapters are loaded already; load all of them in one call")
+        if not adapters:
+            raise AdapterError("no adapters to load")
+        read = {str(name): a if isinstance(a, Adapter) else read_adapter(a) for name, a in adapters.items()}
+        self.model.adapter_names = bind_adapters(self.model, read)
+
+    def _adapter_list(self, adapters, n: int) -> list:
+        listed = [adapters] * n if adapters is None or isinstance(adapters, str) else list(adapters)
+        if len(listed) != n:
+            raise ValueError(f"{len(listed)} adapters for {n} prompts")
+        for name in listed:
+            if name is not None and name not in self.model.adapter_names:
+                raise KeyError(f"adapter {name!r} is not loaded; loaded: {self.model.adapter_names}")
+        return listed
+
+    def beam_search(self, prompts, beams: int = 4, max_tokens: int = 32, adapters=None, stop_ids=(),
+                    length_penalty: float = 1.0, chunk: int = 2048, page_size: int = 16):
+        """Every prompt's best hypotheses (engine/beams.py: Hypothesis), the one worth most first, at
+        most `beams` of each; the prompts run together. `adapters` as for `generate`."""
+        from .engine.beams import BeamSearch
+        prompts = [list(map(int, p)) for p in prompts]
+        # a prompt's pages once, and per beam what it generates and the page it shares in part
+        room = sum(-(-len(p) // page_size) + beams * (max_tokens // page_size + 2) for p in prompts)
+        engine = self.new_engine(page_size=page_size, num_pages=max(room, 1), num_slots=max(len(prompts) * beams, 1))
+        search = BeamSearch(engine, beams, max_tokens, stop_ids, length_penalty, chunk)
+        return search.run(prompts, self._adapter_list(adapters, len(prompts)))
+
     def generate(self, prompts, policy=None, slots: Optional[int] = None, chunk: int = 0,
                  pool_tokens: Optional[int] = None, page_size: int = 16, stop_ids=(),
                  max_batched_tokens: Optional[int] = None, scheduler=None,
-                 reserve: Optional[int] = None):
+                 reserve: Optional[int] = None, adapters=None):
         """Run every prompt (lists of token ids) to completion with continuous batching;
         returns the generated ids per prompt, in order. `policy` is one Policy for all or
         one per prompt; its max_tokens must be positive. The requests stay in
         `last_requests`; a policy with logprobs finds a TokenProb per generated token in its
-        request's `.logprobs`."""
+        request's `.logprobs`. `adapters`: the name of a loaded adapter for all prompts, or a list of
+        one name or None per prompt."""
         from .engine.scheduler import Request, Runner
         from .sampling.policy import Policy
         from .sampling.sampler import sample_rows
@@ -142,8 +176,8 @@ class LoadedModel:
                 pol.max_tokens for pol in policies), pool_tokens=pool_tokens,
                 page_size=page_size, max_batched_tokens=max_batched_tokens)
         runner = Runner(scheduler, sample_rows, stop_ids)
-        requests = [Request(p, pol, request_id=i) for i, (p, pol) in
-                    enumerate(zip(prompts, policies))]
+        requests = [Request(p, pol, request_id=i, adapter=ad) for i, (p, pol, ad) in
+                    enumerate(zip(prompts, policies, self._adapter_list(adapters, len(prompts))))]
         for r in requests:
             runner.submit(r)
         runner.run()

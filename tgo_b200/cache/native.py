@@ -131,6 +131,7 @@ class NativeCacheManager:
         self.pools = [_PoolView(self, g) for g in range(len(groups))]
         self.slots = _SlotsView(self, num_slots)
         self.requests: Dict[object, NativeRequest] = {}
+        self._sharing = False                     # whether requests have shared pages (`follow`)
         self._next_handle = 1
         self._meta = np.zeros(64, dtype=np.int32)
         self._rel = np.empty(2 * 4096, dtype=np.int32)
@@ -202,6 +203,23 @@ class NativeCacheManager:
             self._raise(rc, request_id)
         return [(int(buf[2 * i]), int(buf[2 * i + 1])) for i in range(min(n.value, cap))]
 
+    def follow(self, request_ids, parents) -> np.ndarray:
+        """Request i goes on from what request_ids[parents[i]] holds: it gets that request's length
+        and shares its full pages; the page that is still being written stays request i's own. Returns
+        [groups, requests] int32: request i's page at that place, whose rows the caller copies from
+        the parent's, or -1 where there is none. All or nothing."""
+        n = len(request_ids)
+        handles = np.fromiter((self.requests[r].handle for r in request_ids), dtype=np.int64, count=n)
+        par = _ints(parents)
+        if par.shape != (n,):
+            raise ValueError("cache: one parent per request is needed")
+        pages = np.full((len(self.groups), n), -1, dtype=np.int32)
+        rc = self._lib.tgo_cache_follow(self._h, c_int(n), _ptr(handles), _ptr(par), _ptr(pages))
+        if rc:
+            self._raise(rc)
+        self._sharing = True
+        return pages
+
     def finish(self, request_id) -> List[tuple]:
         req = self.requests[request_id]
         tables = req.tables                       # what goes back, read before it is gone
@@ -209,7 +227,10 @@ class NativeCacheManager:
         if rc:
             self._raise(rc, request_id)
         del self.requests[request_id]
-        return [(g, p) for g, t in enumerate(tables) for p in t if p != NULL_PAGE]
+        gone = [(g, p) for g, t in enumerate(tables) for p in t if p != NULL_PAGE]
+        if self._sharing:                         # pages that another request still names have not gone back
+            gone = [(g, p) for g, p in gone if not self.pools[g].is_held(p)]
+        return gone
 
     # ------------------------------------------------------------------ addressing
     def slot_of(self, req: NativeRequest, g: int, position: int) -> int:

@@ -47,7 +47,7 @@ constexpr int KIND_FULL = 0, KIND_WINDOW = 1;
 struct Pool {
     int num_pages = 0;
     std::vector<int> free_;          // back() is the lowest free id
-    std::vector<uint8_t> held;
+    std::vector<int> held;           // per page: the live requests' tables that name it
     long long taken_total = 0, given_total = 0;
 
     void init(int n) {
@@ -66,13 +66,16 @@ struct Pool {
         }
         taken_total += n;
     }
-    // 0, or the page that may not be given
+    // 0, or the page that may not be given. A page goes back to the pool when the last table that names
+    // it gives it; `pages` holds those afterwards.
     int give(std::vector<int>& pages) {
+        size_t n = 0;
         for (int p : pages) {
             if (p < 1 || p > num_pages) return p ? p : -1;
             if (!held[p]) return p;
-            held[p] = 0;            // also catches a page named twice in one call
+            if (--held[p] == 0) pages[n++] = p;      // a page named twice in one call is caught: it is held no more
         }
+        pages.resize(n);
         std::sort(pages.begin(), pages.end(), [](int a, int b) { return a > b; });
         for (int p : pages) free_.push_back(p);
         given_total += (long long)pages.size();
@@ -262,12 +265,13 @@ TGO_HOST_API int tgo_cache_commit(void* p, long long handle, long long new_lengt
         for (long long i = m->pages_for(m->keep[g]); i < std::min<long long>(dead, (long long)t.size()); ++i)
             if (t[i] != NULL_PAGE) { gone.push_back(t[i]); t[i] = NULL_PAGE; }
         if (gone.empty()) continue;
-        for (int pg : gone) {
-            if (released && n < cap) { released[2 * n] = g; released[2 * n + 1] = pg; }
-            ++n;
-        }
         const int bad = m->pools[g].give(gone);
         if (bad) return m->fail(PAGE_MISUSE, "cache: page " + std::to_string(bad) + " cannot be given back", g, bad);
+        // in the order of their ids; a page that another request still names has not gone back
+        for (size_t i = gone.size(); i-- > 0;) {
+            if (released && n < cap) { released[2 * n] = g; released[2 * n + 1] = gone[i]; }
+            ++n;
+        }
         ++r.version;
     }
     if (n_released) *n_released = n;
@@ -287,13 +291,12 @@ TGO_HOST_API int tgo_cache_finish(void* p, long long handle, int* released, int 
         pages.clear();
         for (int pg : r.tables[g])
             if (pg != NULL_PAGE) pages.push_back(pg);
-        for (int pg : pages) {
-            if (released && n < cap) { released[2 * n] = g; released[2 * n + 1] = pg; }
+        if (pages.empty()) continue;
+        const int bad = m->pools[g].give(pages);
+        if (bad) return m->fail(PAGE_MISUSE, "cache: page " + std::to_string(bad) + " cannot be given back", g, bad);
+        for (size_t i = pages.size(); i-- > 0;) {
+            if (released && n < cap) { released[2 * n] = g; released[2 * n + 1] = pages[i]; }
             ++n;
-        }
-        if (!pages.empty()) {
-            const int bad = m->pools[g].give(pages);
-            if (bad) return m->fail(PAGE_MISUSE, "cache: page " + std::to_string(bad) + " cannot be given back", g, bad);
         }
     }
     m->slot_held[r.slot] = 0;
@@ -301,6 +304,87 @@ TGO_HOST_API int tgo_cache_finish(void* p, long long handle, int* released, int 
     std::sort(m->free_slots.begin(), m->free_slots.end(), [](int a, int b) { return a > b; });
     m->requests.erase(it);
     if (n_released) *n_released = n;
+    return OK;
+}
+
+// Of n requests, number i goes on from what number parents[i] holds (itself: it keeps what it has). It gets
+// the parent's length and the parent's full pages, which the two then share: nobody writes them any more.
+// The page that the parent is still writing is not shared: request i's page at that place is its own
+// (taken from the pool if it has none), and the caller copies its rows; so are pages reserved beyond it.
+// pages[g * n + i]: request i's page at that place in group g, or -1 where there is nothing to copy (the
+// parent's length is whole pages, or none). A request may not be longer than its parent, and one that others
+// go on from while it goes on from another has that one's length. All or nothing: on a refusal every request
+// holds what it held.
+TGO_HOST_API int tgo_cache_follow(void* p, int n, const long long* handles, const int* parents, int* pages) {
+    Manager* m = M(p);
+    const int G = (int)m->kind.size(), ps = m->page_size;
+    std::vector<Request*> r(n);
+    for (int i = 0; i < n; ++i) {
+        auto it = m->requests.find(handles[i]);
+        if (it == m->requests.end()) return m->fail(NOT_LIVE, "cache: the request is not live", i);
+        r[i] = &it->second;
+        for (int j = 0; j < i; ++j)
+            if (handles[j] == handles[i]) return m->fail(BAD_ARGUMENT, "cache: a request is named twice", i);
+        if (parents[i] < 0 || parents[i] >= n) return m->fail(BAD_ARGUMENT, "cache: a request to go on from is not among those named", i);
+    }
+    std::vector<int> wanted(G, 0);
+    for (int i = 0; i < n; ++i) {
+        const Request& from = *r[parents[i]];
+        if (r[i]->length > from.length) return m->fail(BAD_ARGUMENT, "cache: a request is longer than the one it would go on from", i);
+        if (r[i]->length != from.length)
+            for (int j = 0; j < n; ++j)
+                if (j != i && parents[j] == i) return m->fail(BAD_ARGUMENT, "cache: a request that others go on from is shorter than the one it would go on from", i);
+        const long long k = from.length / ps;
+        for (int g = 0; g < G; ++g) {
+            const bool part = from.length % ps != 0;
+            pages[g * n + i] = -1;
+            if (parents[i] == i || !part) continue;
+            const std::vector<int>& t = r[i]->tables[g];
+            if (k >= (long long)t.size() || t[k] == NULL_PAGE) ++wanted[g];
+        }
+    }
+    for (int g = 0; g < G; ++g)
+        if (wanted[g] > m->pools[g].free_count())
+            return m->fail(PAGES_EXHAUSTED, "cache: group " + std::to_string(g) + " needs " + std::to_string(wanted[g]) +
+                           " more pages and has " + std::to_string(m->pools[g].free_count()) + " free",
+                           g, wanted[g], m->pools[g].free_count());
+    std::vector<long long> length(n);
+    for (int i = 0; i < n; ++i) length[i] = r[parents[i]]->length;
+    std::vector<std::vector<int>> next(n);
+    std::vector<int> gone, fresh;
+    for (int g = 0; g < G; ++g) {
+        gone.clear();
+        for (int i = 0; i < n; ++i) {
+            next[i] = r[i]->tables[g];
+            if (parents[i] == i) continue;
+            const std::vector<int>& from = r[parents[i]]->tables[g];
+            const size_t k = (size_t)(length[i] / ps);
+            std::vector<int>& t = next[i];
+            for (size_t j = 0; j < k && j < t.size(); ++j)
+                if (t[j] != NULL_PAGE) gone.push_back(t[j]);
+            if (t.size() < k) t.resize(k, NULL_PAGE);
+            for (size_t j = 0; j < k; ++j) {
+                t[j] = j < from.size() ? from[j] : NULL_PAGE;
+                if (t[j] != NULL_PAGE) ++m->pools[g].held[t[j]];
+            }
+            if (length[i] % ps) {
+                if (t.size() <= k) t.resize(k + 1, NULL_PAGE);
+                if (t[k] == NULL_PAGE) {
+                    fresh.clear();
+                    m->pools[g].take(1, fresh);
+                    t[k] = fresh[0];
+                }
+            }
+            ++r[i]->version;
+        }
+        for (int i = 0; i < n; ++i) {
+            r[i]->tables[g] = next[i];
+            if (length[i] % ps) pages[g * n + i] = next[i][(size_t)(length[i] / ps)];
+        }
+        const int bad = m->pools[g].give(gone);
+        if (bad) return m->fail(PAGE_MISUSE, "cache: page " + std::to_string(bad) + " cannot be given back", g, bad);
+    }
+    for (int i = 0; i < n; ++i) r[i]->length = length[i];
     return OK;
 }
 
@@ -340,7 +424,7 @@ TGO_HOST_API long long tgo_cache_pool(void* p, int group, int what) {
 TGO_HOST_API int tgo_cache_page_is_held(void* p, int group, int page) {
     Manager* m = M(p);
     if (group < 0 || group >= (int)m->pools.size()) return 0;
-    return page >= 1 && page <= m->pools[group].num_pages && m->pools[group].held[page];
+    return page >= 1 && page <= m->pools[group].num_pages && m->pools[group].held[page] > 0;
 }
 TGO_HOST_API int tgo_cache_free_slots(void* p) { return (int)M(p)->free_slots.size(); }
 TGO_HOST_API int tgo_cache_live_requests(void* p) { return (int)M(p)->requests.size(); }
@@ -378,24 +462,32 @@ TGO_HOST_API long long tgo_cache_slot_of(void* p, long long handle, int group, l
     return (long long)t[i] * m->page_size + position % m->page_size;
 }
 
-// No page lost, none held twice: every pool's held pages are exactly the pages in the live
-// requests' tables, and no two requests share a slot.
+// No page lost, none held by mistake: every pool's held pages are exactly the pages in the live
+// requests' tables, each counted as often as a table names it, no table names one twice, and no two
+// requests share a slot.
 TGO_HOST_API int tgo_cache_check(void* p) {
     Manager* m = M(p);
     for (int g = 0; g < (int)m->pools.size(); ++g) {
         const Pool& pool = m->pools[g];
-        std::vector<uint8_t> seen(pool.num_pages + 1, 0);
+        std::vector<int> seen(pool.num_pages + 1, 0), last(pool.num_pages + 1, -1);
         long long n = 0;
-        for (const auto& kv : m->requests)
+        int who = 0;
+        for (const auto& kv : m->requests) {
             for (int pg : kv.second.tables[g]) {
                 if (pg == NULL_PAGE) continue;
                 if (pg < 1 || pg > pool.num_pages || !pool.held[pg])
                     return m->fail(BROKEN_BOOKS, "cache: group " + std::to_string(g) + " table names free page " + std::to_string(pg));
-                if (seen[pg])
-                    return m->fail(BROKEN_BOOKS, "cache: group " + std::to_string(g) + " has a page in two tables");
-                seen[pg] = 1;
-                ++n;
+                if (last[pg] == who)
+                    return m->fail(BROKEN_BOOKS, "cache: group " + std::to_string(g) + " has a page twice in one table");
+                last[pg] = who;
+                if (!seen[pg]++) ++n;
             }
+            ++who;
+        }
+        for (int pg = 1; pg <= pool.num_pages; ++pg)
+            if (seen[pg] && seen[pg] != pool.held[pg])
+                return m->fail(BROKEN_BOOKS, "cache: group " + std::to_string(g) + " page " + std::to_string(pg) + " is in " +
+                               std::to_string(seen[pg]) + " tables and counted " + std::to_string(pool.held[pg]) + " times");
         if (n != pool.num_pages - pool.free_count())
             return m->fail(BROKEN_BOOKS, "cache: group " + std::to_string(g) + " holds " +
                            std::to_string(pool.num_pages - pool.free_count()) + " pages and the tables name " + std::to_string(n));

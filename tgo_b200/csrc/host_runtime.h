@@ -38,6 +38,10 @@ int tgo_cache_commit(void* cache, long long handle, long long new_length, int* r
                      int* n_released);
 int tgo_cache_finish(void* cache, long long handle, int* released_pairs, int cap, int* n_released);
 
+/* Request i of n goes on from request parents[i] of them: its length, its full pages (shared from then on),
+   and a page of its own where the parent is still writing one: pages[g * n + i], or -1 (nothing to copy). */
+int tgo_cache_follow(void* cache, int n, const long long* handles, const int* parents, int* pages);
+
 /* what: 0 length, 1 slot, 2 version, 3 live (1 or 0); -1 for a request that is not live */
 long long tgo_cache_request(void* cache, long long handle, int what);
 /* the table's length; its first `cap` entries into `out` */

@@ -41,6 +41,7 @@ class Model:
                              "logits (no fold_scale)")
         self.embedding: Optional[torch.Tensor] = None
         self.head: Optional[torch.Tensor] = None
+        self.adapter_names: List[str] = []       # loaded adapters (weights/adapters.py), by number
         self._layout()
 
     # ------------------------------------------------------------------- weights
@@ -142,6 +143,8 @@ class Model:
     def libraries(self, page_size: int) -> List[str]:
         """Kernel libraries the model's parts say they will call, without repeats."""
         names = ["elementwise", "sgemm" if self.dtype == torch.float32 else "gemm_skinny"]
+        if self.adapter_names:
+            names.append("adapters")
         if self.spec.logit_softcap is not None:
             names.append("layer_ops")
         for b in self.blocks:

@@ -184,7 +184,7 @@ class Scheduler:
         return reserve
 
     # -- lifecycle
-    def admit(self, prompt: Sequence[int], reserve: int = 0, request=None) -> int:
+    def admit(self, prompt: Sequence[int], reserve: int = 0, request=None, adapter: Optional[str] = None) -> int:
         reserve = self._reserve_for(reserve)
         if len(prompt) == 0:
             raise ValueError("scheduler: the prompt is empty")
@@ -194,7 +194,10 @@ class Scheduler:
         self._ids += 1
         rid = ("slot", free, self._ids)
         try:
-            self.engine.admit(rid, len(prompt) + reserve)
+            if adapter is None:
+                self.engine.admit(rid, len(prompt) + reserve)
+            else:
+                self.engine.admit(rid, len(prompt) + reserve, adapter=adapter)
         except SlotsExhausted as e:
             raise NoSlot(str(e)) from None
         self._arrivals += 1
@@ -277,6 +280,7 @@ class Request:
     evictions: int = 0
     sampler: object = None
     logprobs: list = field(default_factory=list)    # TokenProb per sampled token, if asked
+    adapter: Optional[str] = None                   # a loaded adapter's name
 
 
 class Runner:
@@ -307,7 +311,7 @@ class Runner:
             left = req.policy.max_tokens - len(req.output) if req.policy.max_tokens > 0 else 0
             reserve = min(left, self.sched.reserve) if left > 0 else 0
             try:
-                slot = self.sched.admit(req.prompt + req.output, reserve, request=req)
+                slot = self.sched.admit(req.prompt + req.output, reserve, request=req, adapter=req.adapter)
             except PagesExhausted:
                 if not self.by_slot:
                     raise

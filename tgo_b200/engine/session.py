@@ -35,8 +35,10 @@ class Session:
         decode.go:328-345). Valid until the next token is drawn."""
         return self._last_probs
 
-    def complete(self, prompt: Sequence[int], policy: Optional[Policy] = None) -> Iterator[int]:
-        """Yield generated token ids until a stop id, the token budget or the context's end."""
+    def complete(self, prompt: Sequence[int], policy: Optional[Policy] = None,
+                 adapter: Optional[str] = None) -> Iterator[int]:
+        """Yield generated token ids until a stop id, the token budget or the context's end;
+        `adapter`: a loaded adapter's name."""
         policy = policy or Policy()
         policy.check(self.loaded.spec.vocab_size)
         prompt = [int(t) for t in prompt]
@@ -52,7 +54,7 @@ class Session:
         self._n += 1
         rid = ("session", self._n)
         eng = self.engine
-        eng.admit(rid, len(prompt) + budget)
+        eng.admit(rid, len(prompt) + budget, adapter=adapter)
         draws = DrawStream(policy.seed)
         history = list(prompt)
         self.usage = {"prompt_tokens": len(prompt), "completion_tokens": 0}

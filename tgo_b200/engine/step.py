@@ -65,6 +65,7 @@ class Engine:
         self.storage = CacheStorage(model.groups, page_size, pages, num_slots, model.dtype,
                                     model.device, model.state_shapes)
         self.steps_run = 0
+        self._adapter_of = {}         # request -> number of its adapter, for requests that have one
         self.use_graphs = graphs and self.device.type == "cuda"
         self.h2d_bytes_last = 0       # bytes of the last step's inputs copied to the device
         self._graphs = {}
@@ -74,13 +75,65 @@ class Engine:
         self._portion_seen = {}       # key -> times the shape came without a graph
 
     # ------------------------------------------------------------------ requests
-    def admit(self, request_id, reserve_tokens: int = 0):
+    def admit(self, request_id, reserve_tokens: int = 0, adapter: Optional[str] = None):
+        """`adapter`: the name of a loaded adapter that the request's tokens run through."""
+        if adapter is not None and adapter not in self.model.adapter_names:
+            raise KeyError(f"engine: adapter {adapter!r} is not loaded; loaded: {self.model.adapter_names}")
         req = self.cache.admit(request_id, reserve_tokens)
         self.storage.clear_slot(req.slot)
+        if adapter is not None:
+            self._adapter_of[request_id] = self.model.adapter_names.index(adapter)
         return req
 
     def finish(self, request_id):
-        return self.cache.finish(request_id)
+        gone = self.cache.finish(request_id)
+        self._adapter_of.pop(request_id, None)
+        return gone
+
+    def follow(self, groups: Sequence[Sequence], parents: Sequence[Sequence[int]]) -> None:
+        """In every group of requests (equally many in each, at most 32), request i goes on from what the
+        group's request parents[i] holds: the beams of a request after a selection. Full pages are
+        shared; rows of the pages still being written, and fixed-size states, are copied in place by one
+        launch a group of layers. All the groups or, on a refusal, none."""
+        groups = [list(g) for g in groups]
+        if not groups:
+            return
+        W = len(groups[0])
+        if not 0 < W <= ops.BEAM_MAX or any(len(g) != W for g in groups) or len(parents) != len(groups) or \
+                any(len(q) != W for q in parents):
+            raise ValueError(f"follow: groups of one size are needed, of 1 to {ops.BEAM_MAX} requests, and a parent each")
+        for q in parents:
+            if any(not 0 <= int(i) < W for i in q):
+                raise ValueError(f"follow: a parent is a place 0..{W - 1} of its group: {list(q)}")
+        flat = [r for g in groups for r in g]
+        at = [W * g + int(i) for g, q in enumerate(parents) for i in q]
+        pages = self.cache.follow(flat, at)
+        # [groups of layers + 2][groups of requests][W]: pages, slots, parents
+        n, R = len(self.cache.groups), len(groups)
+        host = np.empty((n + 2, R, W), dtype=np.int32)
+        host[:n] = pages.reshape(n, R, W)
+        host[n] = np.asarray([self.cache.requests[r].slot for r in flat], dtype=np.int32).reshape(R, W)
+        host[n + 1] = np.asarray(parents, dtype=np.int32)
+        if (host[n + 1] == np.arange(W)).all():
+            return
+        lists = torch.from_numpy(host)
+        if self.device.type == "cuda":
+            lists = lists.pin_memory()
+        lists = lists.to(self.device, non_blocking=True)
+        for g in range(n):
+            if (host[g] >= 0).any():
+                kv = self.storage.kv[g]
+                if isinstance(kv, tuple):                 # [calls, pages, ...] a plane
+                    ops.reorder_rows(list(kv), lists[g], lists[n + 1], axis=1)
+                else:                                     # [calls, planes, pages, ...]
+                    ops.reorder_rows([kv], lists[g], lists[n + 1], axis=2)
+        if self.storage.state:
+            ops.reorder_rows(list(self.storage.state.values()), lists[n], lists[n + 1])
+        for r, i in zip(flat, at):
+            if flat[i] in self._adapter_of:
+                self._adapter_of[r] = self._adapter_of[flat[i]]
+            else:
+                self._adapter_of.pop(r, None)
 
     def check_kernels(self) -> None:
         """Raise if a kernel gave up one of its bounded waits (its output is then garbage).
@@ -128,25 +181,39 @@ class Engine:
         ids[T] pos[T] seq[T] q_start[B+1] ctx[B] state_slot[B] rows[n] then, per group,
         slots[T] table[B*width]. With pad_to > B, requests that bring nothing fill the batch:
         one token each at position -1 (the kernels read and write nothing for it).
-        Written into `out` if it is given and large enough."""
+        With an adapted request among them, adapter[T] (-1: none) comes last. Written into `out` if
+        it is given and large enough."""
         ids = [e.request_id for e in entries]
         tokens = [e.tokens for e in entries]
         wants = [e.want for e in entries]
         buf = out if out is not None else self._stage
+        adapted = self._adapted(entries)
+        extra = max(sum(len(x) for x in tokens) + max(pad_to - len(ids), 0), 0) if adapted else 0
         begun = self._begun if self._begun is not None and self._begun[0] == ids else None
         begun = begun[1] if begun else None
-        meta, total = self.cache.step_pack(ids, tokens, wants, pad_to, width_quantum, all_rows, buf,
-                                           begun)
+        meta, total = self.cache.step_pack(ids, tokens, wants, pad_to, width_quantum, all_rows,
+                                           buf[:max(buf.size - extra, 0)], begun)
         if meta is None:                         # too small: a buffer of its own
-            buf = np.empty(total, dtype=np.int32)
+            buf = np.empty(total + extra, dtype=np.int32)
             if out is None:
-                self._stage = np.empty(2 * total, dtype=np.int32)
+                self._stage = np.empty(2 * (total + extra), dtype=np.int32)
             meta, total = self.cache.step_pack(ids, tokens, wants, pad_to, width_quantum, all_rows,
-                                               buf, begun)
+                                               buf[:total], begun)
         elif out is None:
-            buf = buf[:total].copy()             # the staging buffer is written again next step
+            buf = buf[:total + extra].copy()     # the staging buffer is written again next step
         meta["extents"] = [len(t) for t in tokens]
+        meta["adapted"] = adapted
+        if adapted:
+            which = np.fromiter((self._adapter_of.get(i, -1) for i in ids), dtype=np.int32, count=len(ids))
+            tail = buf[total:total + extra]
+            tail.fill(-1)
+            flat = np.repeat(which, np.asarray(meta["extents"]))
+            tail[:flat.size] = flat
+            meta["total"] = total + extra
         return buf, meta
+
+    def _adapted(self, entries: List[StepEntry]) -> bool:
+        return bool(self._adapter_of) and any(e.request_id in self._adapter_of for e in entries)
 
     def _views(self, dev: torch.Tensor, meta: dict):
         """Device views into a flat buffer laid out by `_pack`."""
@@ -169,6 +236,8 @@ class Engine:
         for width in widths:
             dev_slots.append(take(T))
             dev_tables.append(take(B * width).view(B, width))
+        if meta.get("adapted"):
+            ctx.adapters = take(T)
         return ctx, dev_tables, dev_slots
 
     def build_context(self, entries: List[StepEntry]):
@@ -253,13 +322,13 @@ class Engine:
         B = len(entries)
         bucket = next((b for b in self.BUCKETS if b >= B), B)
         width = self._graph_width(entries, self.SHORT_WIDTH)
-        key = (bucket, width)
+        key = (bucket, width, self._adapted(entries))
         entry = self._graphs.get(key)
         if entry is None:
             flat, meta = self._pack(entries, pad_to=bucket, width_quantum=width, all_rows=True)
             # a warm-up run only the first time this engine meets a row count that picks other
             # product kernels (few rows, the library's range, many): later captures just record
-            kind = ops.product_regime(bucket)
+            kind = (ops.product_regime(bucket), key[2])
             try:
                 entry = self._capture(flat, meta, warm=kind not in self._warmed)
                 self._warmed.add(kind)
@@ -304,7 +373,7 @@ class Engine:
         Returns None when the step has to run the ordinary way."""
         e = entries[0]
         width = self._graph_width(entries)
-        key = (len(e.tokens), tuple(int(w) for w in e.want), width)
+        key = (len(e.tokens), tuple(int(w) for w in e.want), width, self._adapted(entries))
         entry = self._portion_graphs.get(key)
         if entry is not None:
             self._portion_graphs.move_to_end(key)

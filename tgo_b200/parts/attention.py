@@ -24,7 +24,7 @@ from ..config.spec import MixerSpec, tensor_names
 from ..kernels import ops
 from ..registry import MIXERS, POSITIONS
 from ..weights.binder import WeightSpec
-from .base import CacheNeed, LayerCache, Part
+from .base import AdapterSite, CacheNeed, LayerCache, Part
 
 USE_TC_ATTENTION = True          # prompt portions with head size 128 on the tcgen05 kernel
 SPLIT_MIXED_STEPS = True         # single tokens of a mixed step go through the decode kernel
@@ -179,6 +179,7 @@ class GQAAttention(Part):
         self.names = tensor_names(spec.tensors, prefix, roles, "attention")
         self.w_qkv = self.w_q = self.w_o = None
         self.q_gain = self.k_gain = None
+        self.adapters = {}                   # site -> AdapterBank, once adapters are loaded
 
     # ---- declarations
     def weight_specs(self):
@@ -213,6 +214,23 @@ class GQAAttention(Part):
         if self.qk_norm:
             self.q_gain = weights.pop(n["q_norm"]).contiguous()
             self.k_gain = weights.pop(n["k_norm"]).contiguous()
+
+    # ---- adapters of requests
+    def adapter_sites(self):
+        n, qw, kw = self.names, self.H * self.dh, self.Hkv * self.dh
+        qkv = AdapterSite("qkv", (n["qkv"],), (qw + 2 * kw,), self.hidden) if self.joined else \
+            AdapterSite("qkv", (n["q"], n["k"], n["v"]), (qw, kw, kw), self.hidden)
+        return [qkv, AdapterSite("o", (n["o"],), (self.hidden,), qw)]
+
+    def bind_adapters(self, banks) -> None:
+        self.adapters = banks
+
+    def _output(self, a, ctx, residual):
+        """The output product, and what the rows' adapters add to it."""
+        y = ops.linear(a, self.w_o, residual=residual)
+        if ctx.adapters is not None and "o" in self.adapters:
+            self.adapters["o"].add(a, residual if y is None else y, ctx)
+        return y
 
     # ---- what the engine may ask
     def libraries(self, dtype, page_size) -> List[str]:
@@ -269,7 +287,15 @@ class GQAAttention(Part):
         qw, kw = H * dh, Hkv * dh
         if cache.writable:
             qkv = ops.linear(x, self.w_qkv)           # x may be ops.NormedRows: folded in there
+            if ctx.adapters is not None and "qkv" in self.adapters:
+                self.adapters["qkv"].add(x, qkv, ctx)
             q, k, v = qkv[:, :qw], qkv[:, qw:qw + kw], qkv[:, qw + kw:]
+        elif ctx.adapters is not None and "qkv" in self.adapters:
+            # the queries alone, of an adapter that is laid out for all three
+            qkv = torch.zeros((x.shape[0], qw + 2 * kw), dtype=x.dtype, device=x.device)
+            qkv[:, :qw] = ops.linear(x, self.w_q)
+            self.adapters["qkv"].add(x, qkv, ctx)
+            q, k, v = qkv[:, :qw], None, None
         else:
             q, k, v = ops.linear(x, self.w_q), None, None
         fused = self.position is None or getattr(self.position, "fusable", False)
@@ -284,7 +310,7 @@ class GQAAttention(Part):
                 cache.k, cache.v, cache.page_size, cache.block_tables, ctx.positions, ctx.seq_ids,
                 self.scale, self.window or 0,
                 n_splits=decode_splits(ctx, Hkv, self.window or 0, q.device))
-            return ops.linear(a, self.w_o, residual=residual)
+            return self._output(a, ctx, residual)
         if fused:
             ops.qk_norm_rope_cache(q, k, v, H, Hkv, dh, self.q_gain, self.k_gain, self.eps,
                                    rope, rot, cache.slots if k is not None else None,
@@ -302,7 +328,7 @@ class GQAAttention(Part):
                                        cache.slots, cache.k, cache.v, cache.page_size)
         a = torch.empty((x.shape[0], qw), dtype=q.dtype, device=q.device)
         paged_attention(q, a, H, Hkv, dh, cache, ctx, self.scale, self.window or 0)
-        return ops.linear(a, self.w_o, residual=residual)
+        return self._output(a, ctx, residual)
 
 
 MIXERS.register("gqa_attention", GQAAttention)

@@ -42,6 +42,9 @@ that offers none of them still runs):
   prepare_capture(ctx, cache) -> make, outside a CUDA-graph capture, whatever its forward
                   would otherwise make on the host during the step (lists derived from the
                   step's shape), leaving it in ctx.aux under a key that starts with "tiles";
+  adapter_sites() -> the products whose results a request's low-rank adapter may add to
+                  (`AdapterSite`), and bind_adapters(banks) -> take {site's key: AdapterBank}: the
+                  forward then calls `bank.add(rows, result, ctx)` behind the product;
   flops(extents, first_positions, writes_cache) -> floating-point operations of one forward
                   over requests bringing `extents` tokens from `first_positions` on;
   cache_bytes_read(context_len, width) -> bytes of cache one decoded token at that context
@@ -145,6 +148,8 @@ class StepContext:
     max_extent: int = 0
     max_context: int = 0
     decode_only: bool = False        # every request brings exactly one token
+    adapters: Optional[torch.Tensor] = None   # int32 [T], each token's adapter (-1: none); None: no
+                                              # request of the step has one
     aux: Dict[str, object] = field(default_factory=dict)   # per-step device tensors made once
 
 
@@ -162,7 +167,37 @@ class NormedDelta:
             ops.residual_add(h, self.extra)
 
 
+@dataclass(frozen=True)
+class AdapterSite:
+    """A product of a part, result = rows . W^T, that adapters may add to. W's rows are those of the
+    checkpoint matrices `names`, one after the other or (`interleaved`, two of them) eight rows of each
+    in turn."""
+    key: str
+    names: Tuple[str, ...]
+    widths: Tuple[int, ...]           # rows of each matrix
+    inputs: int
+    interleaved: bool = False
+
+
+@dataclass
+class AdapterBank:
+    """All loaded adapters of one site, laid out for `ops.low_rank_add`."""
+    a: torch.Tensor                  # [adapters, slices, rank, inputs]
+    b: torch.Tensor                  # [adapters, result columns, rank]
+    scale: torch.Tensor              # float32 [adapters]
+    widths: Tuple[int, ...]
+    interleaved: bool = False
+
+    def add(self, x, result: torch.Tensor, ctx: "StepContext") -> None:
+        """result += each row's own adapter's product, where the row has an adapter."""
+        ops.low_rank_add(ops.rows_of(x), result, self.a, self.b, self.scale, ctx.adapters, self.widths,
+                         self.interleaved)
+
+
 class Part:
+    def adapter_sites(self) -> List[AdapterSite]:
+        return []
+
     def weight_specs(self) -> List[WeightSpec]:
         return []
 

@@ -14,7 +14,7 @@ from ..config.spec import FeedForwardSpec, tensor_names
 from ..kernels import ops
 from ..registry import FEED_FORWARDS
 from ..weights.binder import WeightSpec
-from .base import Part
+from .base import AdapterSite, Part
 
 
 class SwiGLU(Part):
@@ -37,6 +37,7 @@ class SwiGLU(Part):
         self.interleaved = False
         self.b_gate_up = None            # float32 [2 ff], in the order of w_gate_up's rows
         self.output_bias = None          # float32 [hidden]: the down product's bias
+        self.adapters = {}               # site -> AdapterBank, once adapters are loaded
 
     def weight_specs(self):
         n = self.names
@@ -79,6 +80,40 @@ class SwiGLU(Part):
                 self.b_gate_up = torch.cat([bg, bu]).contiguous()
             self.output_bias = weights.pop(n["down_bias"]).to(torch.float32).contiguous()
 
+    def adapter_sites(self):
+        n, f, d = self.names, self.inter, self.hidden
+        first = AdapterSite("gate_up", (n["gate_up"],), (2 * f,), d) if self.joined else \
+            AdapterSite("gate_up", (n["gate"], n["up"]), (f, f), d, f % 8 == 0)
+        # a matrix that is shipped joined has one A for both halves: its rows in eights are no two slices
+        return ([] if self.joined and f % 8 == 0 else [first]) + [AdapterSite("down", (n["down"],), (d,), f)]
+
+    def bind_adapters(self, banks) -> None:
+        self.adapters = banks
+
+    def _adapted(self, x, ctx, residual):
+        """The forward of a step with adapted rows: the gate and up rows are written out, so that the
+        adapters add to them before the gate is applied."""
+        x = ops.rows_of(x)
+        if "gate_up" in self.adapters:
+            rows = ops.linear(x, self.w_gate_up)
+            self.adapters["gate_up"].add(x, rows, ctx)
+            act = torch.empty((x.shape[0], self.inter), dtype=x.dtype, device=x.device)
+            if self.activation == "silu" and not self.bias:
+                ops.swiglu(rows, act, self.interleaved)
+            else:
+                ops.gated_act(rows, act, self.interleaved, self.activation, self.b_gate_up)
+        else:
+            act = ops.gated_linear(x, self.w_gate_up, self.interleaved, self.activation, bias=self.b_gate_up)
+        y = ops.linear(act, self.w_down, residual=None if self.bias else residual, out_dtype=self.out_dtype)
+        if "down" in self.adapters:
+            self.adapters["down"].add(act, residual if y is None else y, ctx)
+        if self.bias and not self.defer_output_bias:
+            ops.add_bias(y, self.output_bias)
+        if self.bias and residual is not None:
+            ops.residual_add(residual, y)
+            return None
+        return y
+
     def libraries(self, dtype, page_size) -> List[str]:
         extra = ["layer_ops"] if self.activation != "silu" or self.bias else []
         return (["sgemm"] if dtype == torch.float32 else ["gemm_skinny"]) + extra
@@ -91,6 +126,8 @@ class SwiGLU(Part):
     def forward(self, x, ctx, residual=None):
         """With `residual` (the float32 stream) the result may be added to it, and None is
         then returned; otherwise the result is returned for the caller to add."""
+        if ctx.adapters is not None and self.adapters:
+            return self._adapted(x, ctx, residual)
         if self.bias:
             act = ops.gated_linear(x, self.w_gate_up, self.interleaved, self.activation,
                                    bias=self.b_gate_up)
