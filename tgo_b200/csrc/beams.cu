@@ -16,12 +16,21 @@
 // the slice's K-th best so far. The second kernel has a block a request: it joins the slices' maxima
 // and sums and merges their lists, ordered already, K times the best head. v is formed in 64 bits, so
 // that close candidates of different beams are ordered by their values and not by a rounding.
+#ifndef BS_THREADS
 #define BS_THREADS 256
+#endif
+#ifndef BS_BLOCKS
+#define BS_BLOCKS 4
+#endif
+#ifndef BS_LOOK_K
+#define BS_LOOK_K 3
+#endif
+#ifndef BS_VPT
+#define BS_VPT 4
+#endif
 #define BS_WARPS (BS_THREADS / 32)
 #define BS_MAX_K 64
 #define BS_MAX_BEAMS 32
-#define BS_LISTS 256              // lists of a request: slices of a row x beams; a thread of the merge each
-#define BS_LOOK 192               // candidates in the buffer from which it is cut back to K
 
 // larger float <-> larger unsigned; the value is no NaN
 __device__ __forceinline__ uint32_t bs_order(float x) {
@@ -35,24 +44,31 @@ __device__ __forceinline__ unsigned long long bs_key(float x, int i) {
     return ((unsigned long long)bs_order(x + 0.f) << 32) | (0xffffffffu - (uint32_t)i);
 }
 
-// e^x for x <= 0, as a power of two; results below 2^-126 are 0 (they add nothing to a sum that holds a 1).
-__device__ __forceinline__ float bs_exp(float x) {
+#define BS_LOG2E 1.44269504088896341f
+// 2^x; results below 2^-126 are 0 (they add nothing to a sum that holds a 1).
+__device__ __forceinline__ float bs_exp2(float x) {
     float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504088896341f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+__device__ __forceinline__ float bs_exp(float x) { return bs_exp2(x * BS_LOG2E); }
 
-// The K largest of buf[0..n) to buf[0..K), descending (n may be less than K: then all of them). Every
-// thread calls it; keys are distinct.
-__device__ void bs_cut(unsigned long long* buf, unsigned long long* sorted, unsigned* hist, int n, int K) {
+// The K largest of kept[0..k) and buf[0..n), descending, to `to` (fewer: all of them). Every thread calls it;
+// keys are distinct, buf has room for k more, what is read has been synchronised and what is written has not.
+__device__ void bs_cut(const unsigned long long* kept, int k, unsigned long long* buf, int n, unsigned* hist,
+                       unsigned long long* to, int K) {
+    __shared__ unsigned long long front[BS_MAX_K];
     const int t = threadIdx.x;
-    if (n > BS_THREADS) {
+    if (k + n > BS_THREADS) {
         // the K-th largest by its bits, eight at a time, then the keys from it on to the front
         __shared__ unsigned long long prefix_s;
         __shared__ int left_s, front_s;
+        if (t < k) buf[n + t] = kept[t];
+        n += k;
+        k = 0;
         if (t == 0) { prefix_s = 0; left_s = K; front_s = 0; }
         for (int shift = 56; shift >= 0; shift -= 8) {
-            hist[t] = 0;
+            for (int i = t; i < 256; i += BS_THREADS) hist[i] = 0;
             __syncthreads();
             const unsigned long long prefix = prefix_s;
             for (int i = t; i < n; i += BS_THREADS)
@@ -69,31 +85,33 @@ __device__ void bs_cut(unsigned long long* buf, unsigned long long* sorted, unsi
         }
         const unsigned long long least = prefix_s;
         for (int i = t; i < n; i += BS_THREADS)
-            if (buf[i] >= least) sorted[atomicAdd(&front_s, 1)] = buf[i];
+            if (buf[i] >= least) front[atomicAdd(&front_s, 1)] = buf[i];
         __syncthreads();
-        if (t < K) buf[t] = sorted[t];
+        buf = front;
         n = K;
-        __syncthreads();
     }
-    const unsigned long long mine = t < n ? buf[t] : 0;
+    if ((t & ~31) >= k + n) return;
+    const unsigned long long mine = t < k ? kept[t] : t < k + n ? buf[t - k] : 0;
     int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < k; ++j) rank += kept[j] > mine;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) rank += buf[j] > mine;
-    __syncthreads();
-    if (t < n && rank < K) buf[rank] = mine;
-    __syncthreads();
+    if (t < k + n && rank < K) to[rank] = mine;
 }
 
 // VPT vectors of four values a thread and turn.
 template <int VPT>
-__global__ void __launch_bounds__(BS_THREADS)
+__global__ void __launch_bounds__(BS_THREADS, BS_BLOCKS)
 beam_part_kernel(const float* __restrict__ logits, long long stride, int V, const float* __restrict__ scores, int K,
                  int parts, int turns, float2* __restrict__ sums, unsigned long long* __restrict__ lists) {
     constexpr int TILE = BS_THREADS * VPT;                  // vectors a turn
-    __shared__ unsigned long long buf[4 * TILE + BS_LOOK];
-    __shared__ unsigned long long sorted[BS_MAX_K];
-    __shared__ unsigned hist[BS_THREADS];
+    static_assert(VPT == 4, "the choice of a hit below goes by sixteen values");
+    __shared__ unsigned long long buf[4 * TILE + 4 * BS_MAX_K];
+    __shared__ unsigned long long kept[2][BS_MAX_K];
+    __shared__ unsigned hist[256];
     __shared__ float2 red[BS_WARPS];
-    __shared__ int count;
+    __shared__ int counts[2];         // candidates in buf; the other one is set to 0 meanwhile
     __shared__ unsigned warp_least[BS_WARPS];
     pdl_wait();
     const int row = blockIdx.y, part = blockIdx.x, t = threadIdx.x, warp = t >> 5, lane = t & 31;
@@ -109,22 +127,27 @@ beam_part_kernel(const float* __restrict__ logits, long long stride, int V, cons
     const int off = (int)(((uintptr_t)x >> 2) & 3);
     const int vectors = (V + off + 3) / 4;
     const int v0 = part * turns * TILE, v1 = min(v0 + turns * TILE, vectors);
-    if (t == 0) count = 0;
+    if (t < 2) counts[t] = 0;
 
     float4 next[VPT];
+    const float* const at_v = x - off;                       // where vector 0 would begin; aligned
+    // the vectors before v_head and from v_tail on reach over the row's ends
+    const int v_head = off ? 1 : 0, v_tail = min(v1, (V + off) / 4);
     auto load = [&](int base) {
+        if (base >= v_head && base + TILE <= v_tail) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) next[j] = __ldcs((const float4*)(at_v + 4 * (size_t)(base + t)) + j * BS_THREADS);
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int v = base + j * BS_THREADS + t, e = 4 * v - off;
             float4 q = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
             if (v < v1) {
-                if (e >= 0 && e + 3 < V) q = __ldcs((const float4*)(x + e));
-                else {
-                    if (e >= 0 && e < V) q.x = x[e];
-                    if (e + 1 >= 0 && e + 1 < V) q.y = x[e + 1];
-                    if (e + 2 >= 0 && e + 2 < V) q.z = x[e + 2];
-                    if (e + 3 >= 0 && e + 3 < V) q.w = x[e + 3];
-                }
+                if (e >= 0 && e < V) q.x = x[e];
+                if (e + 1 >= 0 && e + 1 < V) q.y = x[e + 1];
+                if (e + 2 >= 0 && e + 2 < V) q.z = x[e + 2];
+                if (e + 3 >= 0 && e + 3 < V) q.w = x[e + 3];
             }
             next[j] = q;
         }
@@ -133,6 +156,10 @@ beam_part_kernel(const float* __restrict__ logits, long long stride, int V, cons
     float m = -INFINITY, s = 0.f;                            // this thread's running maximum and sum
     unsigned long long least = 0;                            // a later candidate's key is larger than this
     float least_x = -INFINITY;
+    // The buffer is cut back to K whenever it holds this many: the higher the K-th, the fewer threads look closer,
+    // but a cut stops the block for about 1000 cycles.
+    const int look = max(BS_LOOK_K * K, 32);
+    int k = 0, epoch = 0;                                    // kept[epoch & 1][0..k), counts[epoch & 1]
     for (int base = v0; base < v1; base += TILE) {
         float4 cur[VPT];
 #pragma unroll
@@ -141,14 +168,21 @@ beam_part_kernel(const float* __restrict__ logits, long long stride, int V, cons
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) top = fmaxf(top, fmaxf(fmaxf(cur[j].x, cur[j].y), fmaxf(cur[j].z, cur[j].w)));
-        // where everything so far is -inf, 0 stands for the maximum: the exponentials are 0 and not NaN. The
-        // difference is formed before the scaling: rows masked with the type's lowest value stay in range.
+        // where everything so far is -inf, 0 stands for the maximum: the exponentials are 0 and not NaN
         const float now = fmaxf(m, top), at = now > -INFINITY ? now : 0.f;
         s *= m > -INFINITY ? bs_exp(m - at) : 0.f;
         float add = 0.f;
+        if (fabsf(at) < 1e37f) {
+            const float by = -at * BS_LOG2E;
 #pragma unroll
-        for (int j = 0; j < VPT; ++j)
-            add += (bs_exp(cur[j].x - at) + bs_exp(cur[j].y - at)) + (bs_exp(cur[j].z - at) + bs_exp(cur[j].w - at));
+            for (int j = 0; j < VPT; ++j)
+                add += (bs_exp2(fmaf(cur[j].x, BS_LOG2E, by)) + bs_exp2(fmaf(cur[j].y, BS_LOG2E, by))) +
+                       (bs_exp2(fmaf(cur[j].z, BS_LOG2E, by)) + bs_exp2(fmaf(cur[j].w, BS_LOG2E, by)));
+        } else {                                             // rows masked with the type's lowest value: the difference first
+#pragma unroll
+            for (int j = 0; j < VPT; ++j)
+                add += (bs_exp(cur[j].x - at) + bs_exp(cur[j].y - at)) + (bs_exp(cur[j].z - at) + bs_exp(cur[j].w - at));
+        }
         s += add;
         m = now;
         if (base == v0) {
@@ -173,36 +207,48 @@ beam_part_kernel(const float* __restrict__ logits, long long stride, int V, cons
         }
         bool full = false;
         if (top >= least_x && top > -INFINITY) {
+            const float v[4 * VPT] = {cur[0].x, cur[0].y, cur[0].z, cur[0].w, cur[1].x, cur[1].y, cur[1].z, cur[1].w,
+                                      cur[2].x, cur[2].y, cur[2].z, cur[2].w, cur[3].x, cur[3].y, cur[3].z, cur[3].w};
+            unsigned hits = 0;
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                const int e = 4 * (base + j * BS_THREADS + t) - off;
-                const float q[4] = {cur[j].x, cur[j].y, cur[j].z, cur[j].w};
+            for (int i = 0; i < 4 * VPT; ++i) hits |= v[i] >= least_x ? 1u << i : 0u;
+            // a value at a time from each thread that has any: picked from the registers by its number's bits
+            while (hits) {
+                const int i = __ffs(hits) - 1;
+                hits &= hits - 1;
+                float h[8];
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (q[c] >= least_x && q[c] > -INFINITY) {
-                        const unsigned long long key = bs_key(q[c], e + c);
-                        if (key > least) {
-                            const int place = atomicAdd(&count, 1);
-                            buf[place] = key;
-                            full = full || place >= BS_LOOK - 1;
-                        }
-                    }
+                for (int c = 0; c < 8; ++c) h[c] = i & 8 ? v[c + 8] : v[c];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) h[c] = i & 4 ? h[c + 4] : h[c];
+                h[0] = i & 2 ? h[2] : h[0];
+                h[1] = i & 2 ? h[3] : h[1];
+                const float x_i = i & 1 ? h[1] : h[0];
+                const unsigned long long key = bs_key(x_i, 4 * (base + (i >> 2) * BS_THREADS + t) - off + (i & 3));
+                if (key > least && x_i > -INFINITY) {
+                    const int place = atomicAdd(&counts[epoch & 1], 1);
+                    buf[place] = key;
+                    full = full || place >= look - 1;
+                }
             }
         }
         if (__syncthreads_or(full)) {
-            const int n = count;
-            bs_cut(buf, sorted, hist, n, K);
-            if (t == 0) count = min(n, K);
+            const int n = counts[epoch & 1];
+            if (t == 0) counts[~epoch & 1] = 0;
+            bs_cut(kept[epoch & 1], k, buf, n, hist, kept[~epoch & 1], K);
+            k = min(k + n, K);
+            ++epoch;
             __syncthreads();
-            least = buf[K - 1];                              // BS_LOOK > K: there are K of them
-            least_x = bs_value((uint32_t)(least >> 32));
-            __syncthreads();
+            if (k == K) {
+                least = kept[epoch & 1][K - 1];
+                least_x = bs_value((uint32_t)(least >> 32));
+            }
         }
     }
     __syncthreads();
-    const int n = count;
-    bs_cut(buf, sorted, hist, n, K);
-    if (t < K) list[t] = t < n ? buf[t] : 0;
+    const int n = counts[epoch & 1];
+    bs_cut(kept[epoch & 1], k, buf, n, hist, list, K);
+    if (t >= k + n && t < K) list[t] = 0;
     const float wm = warp_max(m);
     const float ws = warp_sum(m > -INFINITY ? s * bs_exp(m - wm) : s);
     if (lane == 0) red[warp] = make_float2(wm, ws);
@@ -217,95 +263,144 @@ beam_part_kernel(const float* __restrict__ logits, long long stride, int V, cons
 }
 
 // One block a request. (m, s) of a slice: its values' exp(x - m) sum to s; a NaN or +inf among them has
-// made s NaN, a slice of -inf alone has m = -inf and s = 0.
-__global__ void __launch_bounds__(BS_LISTS)
+// made s NaN, a slice of -inf alone has m = -inf and s = 0. The slices' lists are sorted: the K-th best of
+// their first candidates (as many of each as make 3 K) bounds what can be among the K best, at most K lists
+// reach it, and what reaches it is ranked by counting.
+#define BM_THREADS 256
+#define BM_LISTS 256
+#define BM_CANDIDATES 4096        // of a request's lists together
+
+// Larger (first, then second) is better: the order of v's bits, the complement of beam and token.
+struct __align__(16) Pick {
+    unsigned long long v, place;
+};
+__device__ __forceinline__ int better(const Pick& a, const Pick& b) { return (int)(a.v > b.v) | ((int)(a.v == b.v) & (int)(a.place > b.place)); }
+__device__ __forceinline__ unsigned long long bm_order(double x) {
+    const unsigned long long b = (unsigned long long)__double_as_longlong(x);
+    return b >> 63 ? ~b : b | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double bm_value(unsigned long long o) {
+    return __longlong_as_double((long long)(o >> 63 ? o & 0x7fffffffffffffffull : ~o));
+}
+// How many of from[0..n) are better than p.
+__device__ __forceinline__ int bm_rank(const Pick* from, int n, const Pick& p) {
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) rank += better(from[j], p);
+    return rank;
+}
+
+__global__ void __launch_bounds__(BM_THREADS)
 beam_merge_kernel(const float* __restrict__ scores, int W, int K, int parts, const float2* __restrict__ sums,
                   const unsigned long long* __restrict__ lists, float* __restrict__ picked, int* __restrict__ parents,
                   int* __restrict__ tokens) {
+    extern __shared__ __align__(16) unsigned char bm_smem[];
     __shared__ double base_s[BS_MAX_BEAMS];                  // score - ln s, or NaN: the beam gives nothing
     __shared__ float max_s[BS_MAX_BEAMS];
-    __shared__ double best_v[BS_LISTS / 32];
-    __shared__ int best_w[BS_LISTS / 32], best_i[BS_LISTS / 32], best_t[BS_LISTS / 32];
+    __shared__ Pick bound_s;
+    __shared__ int count;
     pdl_wait();
-    const int b = blockIdx.x, t = threadIdx.x, warp = t >> 5, lane = t & 31, warps = blockDim.x >> 5;
-    for (int w = warp; w < W; w += warps) {
+    const int b = blockIdx.x, t = threadIdx.x, warp = t >> 5, lane = t & 31, n = W * parts;
+    const int q = min((3 * K + n - 1) / n, K);               // a list's heads
+    Pick* const all = (Pick*)bm_smem;                        // [n][K]
+    Pick* const heads = all + n * K;                         // [n][q]
+    Pick* const found = heads + n * q;                       // [n][K]
+    if (t == 0) { count = 0; bound_s = Pick{0, 0}; }
+    const unsigned long long first = t < n * K ? lists[(size_t)b * n * K + t] : 0;
+    for (int w = warp; w < W; w += BM_THREADS / 32) {
         const float2* row = sums + ((size_t)b * W + w) * parts;
+        const float score = scores[b * W + w];
         float m = -INFINITY;
         for (int p = lane; p < parts; p += 32) m = fmaxf(m, row[p].x);
         m = warp_max(m);
-        double s = 0.0;
-        for (int p = lane; p < parts; p += 32)
-            s += row[p].x > -INFINITY ? (double)row[p].y * exp((double)row[p].x - (double)m) : (double)row[p].y;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        const double base = (double)scores[b * W + w] - log(s);
+        float s = 0.f;
+        for (int p = lane; p < parts; p += 32) s += row[p].x > -INFINITY ? row[p].y * bs_exp(row[p].x - m) : row[p].y;
+        s = warp_sum(s);
+        // ln s = e ln 2 + ln(f), s = 2^e f, 1 <= f < 2: the larger part in 64 bits
+        const int e = (int)(__float_as_uint(s) >> 23) - 127;
+        const float f = __uint_as_float((__float_as_uint(s) & 0x007fffffu) | 0x3f800000u);
+        const double base = (double)score - ((double)e * 0.693147180559945309 + (double)log1pf(f - 1.f));
         if (lane == 0) {
-            base_s[w] = base > -INFINITY && base < INFINITY ? base : __longlong_as_double(0x7ff8000000000000ll);
+            base_s[w] = s > 0.f && s < INFINITY && m < INFINITY ? base : __longlong_as_double(0x7ff8000000000000ll);
             max_s[w] = m;
         }
     }
     __syncthreads();
-    const int w = t / parts;
-    const bool have = w < W;
-    const unsigned long long* list = lists + ((size_t)b * W * parts + t) * K;
-    const double base = have ? base_s[w] : 0.0, top = have ? (double)max_s[w] : 0.0;
-    int at = 0, tok = 0;
-    double v = -INFINITY;
-    auto head = [&]() {                                      // -inf: the list is used up
-        v = -INFINITY;
-        if (have && at < K && base == base) {
-            const unsigned long long key = list[at];
-            if (key) {
-                v = base + ((double)bs_value((uint32_t)(key >> 32)) - top);
-                tok = (int)(0xffffffffu - (uint32_t)key);
-            }
+    for (int e = t; e < n * K; e += BM_THREADS) {
+        const unsigned long long key = e == t ? first : lists[(size_t)b * n * K + e];
+        const int l = e / K, i = e - l * K, w = l / parts;
+        const double base = base_s[w];
+        Pick p = {0, 0};                                     // nothing
+        if (key && base == base) {
+            p.v = bm_order(base + ((double)bs_value((uint32_t)(key >> 32)) - (double)max_s[w]));
+            p.place = ~(((unsigned long long)w << 32) | (0xffffffffu - (uint32_t)key));
         }
-    };
-    head();
-    for (int k = 0; k < K; ++k) {
-        double bv = v;
-        int bw = have ? w : BS_MAX_BEAMS, bi = tok, bt = t;
-        auto take = [&](double ov, int ow, int oi, int ot) {
-            if (ov > bv || (ov == bv && (ow < bw || (ow == bw && oi < bi)))) { bv = ov; bw = ow; bi = oi; bt = ot; }
-        };
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const double ov = __shfl_xor_sync(0xffffffffu, bv, o);
-            const int ow = __shfl_xor_sync(0xffffffffu, bw, o), oi = __shfl_xor_sync(0xffffffffu, bi, o),
-                      ot = __shfl_xor_sync(0xffffffffu, bt, o);
-            take(ov, ow, oi, ot);
+        all[e] = p;
+        if (i < q) heads[l * q + i] = p;
+    }
+    __syncthreads();
+    for (int e = t; e < n * q; e += BM_THREADS) {
+        const Pick p = heads[e];
+        if (p.v && bm_rank(heads, n * q, p) == K - 1) bound_s = p;   // places differ: at most one
+    }
+    __syncthreads();
+    const Pick bound = bound_s;                              // {0, 0}: fewer than K heads, everything reaches it
+    for (int e = t; e < n * K; e += BM_THREADS) {
+        const Pick p = all[e];
+        if (p.v && !better(bound, p)) found[atomicAdd(&count, 1)] = p;
+    }
+    __syncthreads();
+    const int c = count;
+    const size_t out = (size_t)b * K;
+    for (int e = t; e < c; e += BM_THREADS) {
+        const Pick p = found[e];
+        const int rank = bm_rank(found, c, p);
+        if (rank < K) {
+            picked[out + rank] = (float)bm_value(p.v);
+            parents[out + rank] = (int)(~p.place >> 32);
+            tokens[out + rank] = (int)(uint32_t)~p.place;
         }
-        if (lane == 0) { best_v[warp] = bv; best_w[warp] = bw; best_i[warp] = bi; best_t[warp] = bt; }
-        __syncthreads();
-        bv = best_v[0]; bw = best_w[0]; bi = best_i[0]; bt = best_t[0];
-        for (int i = 1; i < warps; ++i) take(best_v[i], best_w[i], best_i[i], best_t[i]);
-        const bool none = !(bv > -INFINITY);
-        if (t == 0) {
-            const size_t o = (size_t)b * K + k;
-            picked[o] = none ? -INFINITY : (float)bv;
-            parents[o] = none ? -1 : bw;
-            tokens[o] = none ? -1 : bi;
-        }
-        if (!none && t == bt) { ++at; head(); }
-        __syncthreads();
+    }
+    for (int k = c + t; k < K; k += BM_THREADS) {
+        picked[out + k] = -INFINITY;
+        parents[out + k] = tokens[out + k] = -1;
     }
 }
 
-static void beam_plan(int rows, int W, int V, int sms, int* vpt, int* turns, int* parts) {
-    *vpt = 4;
-    const int tiles = (V + 3 + 4 * BS_THREADS * 4 - 1) / (4 * BS_THREADS * 4);
-    int p = (4 * sms + rows - 1) / rows;                     // four blocks a multiprocessor
-    p = p < tiles ? p : tiles;
-    p = p < BS_LISTS / W ? p : BS_LISTS / W;
-    *turns = (tiles + p - 1) / p;
+// Bytes of its shared memory: candidates, heads, and those that reach the bound.
+static size_t beam_merge_bytes(int lists, int K) {
+    const int q = (3 * K + lists - 1) / lists < K ? (3 * K + lists - 1) / lists : K;
+    return (size_t)lists * (2 * K + q) * sizeof(Pick);
+}
+
+#ifndef BS_FIXED
+#define BS_FIXED 3
+#endif
+// Slices of a row: the count that is cheapest by a small model. The blocks run in rounds of four a multiprocessor; a
+// block costs a unit a turn and three to begin and end.
+static void beam_plan(int rows, int W, int V, int K, int sms, int* turns, int* parts) {
+    const int tiles = (V + 3 + 4 * BS_THREADS * BS_VPT - 1) / (4 * BS_THREADS * BS_VPT);
+    const int most = BM_CANDIDATES / (W * K) < BM_LISTS / W ? BM_CANDIDATES / (W * K) : BM_LISTS / W;
+    long long best = -1;
+    for (int p = 1; p <= most && p <= tiles; ++p) {
+        const int n = (tiles + p - 1) / p;
+        const long long rounds = ((long long)rows * p + BS_BLOCKS * sms - 1) / (BS_BLOCKS * sms), cost = rounds * (n + BS_FIXED);
+        if (best < 0 || cost < best) { best = cost; *turns = n; }
+    }
     *parts = (tiles + *turns - 1) / *turns;
 }
 
-// Slices of a row that tgo_beam_select works with: it needs rows x slices x (8 + 8 K) bytes of workspace.
-TGO_API int tgo_beam_select_parts(int requests, int beams, int V) {
-    if (requests <= 0 || beams <= 0 || beams > BS_MAX_BEAMS || V <= 0 || V > 0x7fffffff - 8) return 0;
-    int vpt, turns, parts;
-    beam_plan(requests * beams, beams, V, tgo_multiprocessors(), &vpt, &turns, &parts);
+static bool beam_takes(int requests, int beams, int V, int K) {
+    return requests > 0 && beams > 0 && beams <= BS_MAX_BEAMS && K > 0 && K <= BS_MAX_K && V > 0 && V <= 0x7fffffff - 8 &&
+           (long long)requests * beams <= 65535;
+}
+
+// Slices of a row that tgo_beam_select works with (0: it refuses these sizes): it needs rows x slices x (1 + K)
+// 64-bit numbers of workspace.
+TGO_API int tgo_beam_select_parts(int requests, int beams, int V, int K) {
+    if (!beam_takes(requests, beams, V, K)) return 0;
+    int turns, parts;
+    beam_plan(requests * beams, beams, V, K, tgo_multiprocessors(), &turns, &parts);
     return parts;
 }
 
@@ -314,20 +409,28 @@ TGO_API int tgo_beam_select_parts(int requests, int beams, int V) {
 TGO_API int tgo_beam_select(const float* logits, long long stride, const float* scores, int requests, int beams, int V,
                             int K, float* picked, int* parents, int* tokens, void* work, int parts, cudaStream_t stream) {
     if (requests <= 0) return 0;
-    if (beams <= 0 || beams > BS_MAX_BEAMS || K <= 0 || K > BS_MAX_K || V <= 0 || V > 0x7fffffff - 8 ||
-        (long long)requests * beams > 65535)
-        return TGO_E_BAD_ARG;
-    int vpt, turns, mine;
-    beam_plan(requests * beams, beams, V, tgo_multiprocessors(), &vpt, &turns, &mine);
+    if (!beam_takes(requests, beams, V, K)) return TGO_E_BAD_ARG;
+    static bool sized[64] = {};                              // per device
+    int dev = 0, turns, mine;
+    const cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return (int)err;
+    if (dev < 0 || dev >= 64) return TGO_E_BAD_ARG;
+    if (!sized[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   200 * 1024);
+        if (e != cudaSuccess) return (int)e;
+        sized[dev] = true;
+    }
+    beam_plan(requests * beams, beams, V, K, tgo_multiprocessors(), &turns, &mine);
     if (mine != parts) return TGO_E_BAD_ARG;
-    const int rows = requests * beams;
+    const int rows = requests * beams, lists_of = beams * parts;
     float2* sums = (float2*)work;
     unsigned long long* lists = (unsigned long long*)(sums + (size_t)rows * parts);
-    const int rc = tgo_launch_pdl(beam_part_kernel<4>, dim3(parts, rows), dim3(BS_THREADS), 0, stream, logits, stride, V,
+    const int rc = tgo_launch_pdl(beam_part_kernel<BS_VPT>, dim3(parts, rows), dim3(BS_THREADS), 0, stream, logits, stride, V,
                                   scores, K, parts, turns, sums, lists);
     if (rc) return rc;
-    const int threads = (beams * parts + 31) / 32 * 32;
-    return tgo_launch_pdl(beam_merge_kernel, dim3(requests), dim3(threads), 0, stream, scores, beams, K, parts,
+    return tgo_launch_pdl(beam_merge_kernel, dim3(requests), dim3(BM_THREADS),
+                          beam_merge_bytes(lists_of, K), stream, scores, beams, K, parts,
                           (const float2*)sums, (const unsigned long long*)lists, picked, parents, tokens);
 }
 

@@ -2123,7 +2123,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, picked: torch.Tensor
         return
     V = logits.shape[1]
     lib = entry_points("beams")
-    parts = lib.tgo_beam_select_parts(c_int(B), c_int(W), c_int(V))
+    parts = lib.tgo_beam_select_parts(c_int(B), c_int(W), c_int(V), c_int(K))
     work = torch.empty(B * W * parts * (1 + K), dtype=torch.int64, device=logits.device)
     _check(lib.tgo_beam_select(_ptr(logits), c_ll(logits.stride(0)), _ptr(scores), c_int(B), c_int(W), c_int(V),
                                c_int(K), _ptr(picked), _ptr(parents), _ptr(tokens), _ptr(work), c_int(parts),
