@@ -92,6 +92,23 @@ def test_columns_in_eights(x_type, y_type, T, K, f, rank):
     check(inputs(T, K, (f, f), rank, 3, x_type, y_type, seed=f), (f, f), interleaved=True)
 
 
+@pytest.mark.parametrize("y_type", [BF, F32])
+@pytest.mark.parametrize("T,K,widths,rank,adapters,interleaved", [
+    (300, 64, (64,), 8, 1, False), (301, 2048, (2048,), 16, 4, False), (513, 1032, (256, 64, 64), 24, 3, False),
+    (1000, 512, (96, 32), 40, 7, False), (640, 4096, (512, 128, 128), 64, 2, False), (333, 768, (1056,), 128, 3, False),
+    (700, 640, (512, 64, 32, 96), 128, 2, False), (400, 256, (512, 512), 16, 5, True), (777, 1000, (96, 96), 32, 3, True),
+    (450, 512, (160, 160), 128, 2, True), (2500, 192, (64, 64), 8, 30, True)])
+def test_many_rows(y_type, T, K, widths, rank, adapters, interleaved):
+    """Mixed rows, and runs of unlike lengths as prompts of requests leave them."""
+    p = inputs(T, K, widths, rank, adapters, BF, y_type, seed=T + rank)
+    check(p, widths, interleaved)
+    cuts = sorted(torch.randint(0, T, (5,), generator=torch.Generator().manual_seed(T)).tolist())
+    runs = torch.zeros(T, dtype=torch.int32)
+    for i, c in enumerate(cuts):
+        runs[c:] = i % adapters if i % 3 else -1
+    check({**p, "ids": runs.to(DEV)}, widths, interleaved)
+
+
 @pytest.mark.parametrize("x_type,y_type", TYPES)
 @pytest.mark.parametrize("T", [1, 6, 300])
 def test_in_place(x_type, y_type, T):
@@ -99,7 +116,7 @@ def test_in_place(x_type, y_type, T):
 
 
 @pytest.mark.parametrize("x_type,y_type", TYPES)
-@pytest.mark.parametrize("T", [4, 150])
+@pytest.mark.parametrize("T", [4, 150, 333])
 def test_strided_rows(x_type, y_type, T):
     """x and y as columns of wider matrices, at an odd and at an even place."""
     for first in (1, 8):
@@ -137,7 +154,7 @@ def test_float32_rows_do_not_hang_on_their_batch():
 @pytest.mark.parametrize("x_type", [F32, BF])
 def test_values_that_are_not_finite_stay_in_their_row(x_type):
     """A NaN or an infinity in a row of x, or in an adapter that no other row has, reaches that row alone."""
-    for T in (6, 140):
+    for T in (6, 140, 500):
         p = inputs(T, 512, (256,), 16, 4, x_type, x_type, seed=T, ids=(torch.arange(T) % 3).to(torch.int32))
         out = check(p, (256,))
         p["x"][4, 100] = float("nan")

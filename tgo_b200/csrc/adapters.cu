@@ -6,6 +6,7 @@
 // joined matrix; gate and up rows in eights): each slice has an A of its own. A row whose id names no
 // adapter keeps y. u is held in 32 bits.
 #include "mma_sync.cuh"
+#include "tcgen.cuh"
 
 #define LR_MAX_SLICES 4
 
@@ -367,6 +368,349 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
     lf_cluster_wait();
 }
 
+// ---------------------------------------------------------------------- many rows of an adapter
+// Tiles of 128 planned rows, bfloat16. Two kernels, u between them in float32:
+//
+// u (`low_rank_u_kernel`): [128, slices x rank] = X[rows] A^T, a part of k a block, on tcgen05: TMA brings 64
+// columns of the tile's rows (one box where they lie together, else four rows a request) and of A into a ring,
+// a thread issues the products, four warps hand the accumulator on. Bound by x's way from memory.
+//
+// out (`low_rank_out_kernel`): the parts of u are summed and split into two bfloat16 numbers (see above), 64
+// columns of B at a time come into shared memory, mma.sync makes 16 rows x 32 columns a warp, y is read one step
+// ahead and added in registers. Which column of B stands where in a product is chosen so that a thread ends up
+// with eight neighbouring columns: y and out move 16 bytes (float32: 32) at a time. Bound by y's and out's way.
+#define LT_ROWS 128
+#define LT_BK 64
+#define LT_X_BYTES (LT_ROWS * LT_BK * 2)
+#define LT_STAGE_OUT 4096         // per handing-on warp: 32 rows x 128 bytes
+#define LT_THREADS 224
+#ifndef LT_FILL
+#define LT_FILL 1
+#endif
+#define LT_MAX_WIDTH 512          // slices x rank: the columns of tensor memory
+
+__device__ int low_rank_error_flag = 0;
+
+struct LowRankTile {
+    int width, cut, cuts, kbs, splits, stages;    // A's rows come in `cuts` boxes of `cut`
+};
+
+template <int COLS>
+__global__ void __launch_bounds__(LT_THREADS)
+low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_constant__ CUtensorMap map_some,
+                  const __grid_constant__ CUtensorMap map_all, const __grid_constant__ CUtensorMap map_a, const LowRankTile g,
+                  int T, const int* __restrict__ perm, const int* __restrict__ info, const int* __restrict__ tiles,
+                  float* __restrict__ part) {
+    extern __shared__ unsigned char lt_raw[];
+    unsigned char* const base = (unsigned char*)(((uintptr_t)lt_raw + 1023) & ~(uintptr_t)1023);
+    const int stage_bytes = LT_X_BYTES + g.cuts * g.cut * LT_BK * 2;
+    unsigned char* const out_stage = base + (size_t)g.stages * stage_bytes;
+    uint64_t* const full = (uint64_t*)(out_stage + 4 * LT_STAGE_OUT);
+    uint64_t* const empty = full + 8;
+    uint64_t* const done = empty + 8;
+    uint64_t* const settled = done + 1;                      // after a wait ran out
+    uint32_t* const tmem_slot = (uint32_t*)(settled + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tile = blockIdx.y, split = blockIdx.x;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 8; ++i) { tg_init(&full[i], 2); tg_init(&empty[i], 1); }
+        tg_init(done, 1);
+        tg_init(settled, 1);
+        tg_init_done();
+    }
+    pdl_wait();
+    if (tile >= info[0]) return;
+    const int id = tiles[3 * tile], r0 = tiles[3 * tile + 1], rows = tiles[3 * tile + 2];
+    if (id < 0) return;                                      // the same for the whole block
+    if (warp == 1) tg_alloc<COLS>(tmem_slot);
+    tg_before();
+    __syncthreads();
+    tg_after();
+    const uint32_t tmem = *tmem_slot;
+    const int kb0 = g.kbs * split / g.splits, kb1 = g.kbs * (split + 1) / g.splits;
+
+    if (warp == 0 || warp == 6) {
+        // ---- rows (warp 0) and A (warp 6)
+        uint32_t it = 0;
+        bool ok = true;
+        int src[4] = {0, 0, 0, 0}, first = 0;
+        bool together = true;
+        if (warp == 0) {
+            first = perm[r0];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = min(4 * lane + j, rows - 1);
+                src[j] = perm[r0 + i];
+                together = together && src[j] == first + i;
+            }
+            together = __all_sync(0xffffffffu, together);
+        }
+        // more than three boxes of 32 rows come as one of 128: the rows after the tile's give sums that nobody stores
+        const bool whole = together && rows > 96;
+        const int groups = !together ? (rows + 3) / 4 : whole ? 1 : (rows + 31) / 32, group_bytes = !together ? 512 : whole ? LT_X_BYTES : 4096;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int s = it % g.stages;
+            ok = __all_sync(0xffffffffu, tg_wait(&empty[s], ((it / g.stages) & 1) ^ 1, &low_rank_error_flag, 1));
+            if (!ok) break;
+            unsigned char* const st = base + (size_t)s * stage_bytes;
+            if (warp == 6) {
+                if (lane == 0) {
+                    tg_expect(&full[s], (uint32_t)(g.cuts * g.cut * LT_BK * 2));
+                    for (int c = 0; c < g.cuts; ++c)
+                        tg_load_2d(st + LT_X_BYTES + c * g.cut * LT_BK * 2, &map_a, kb * LT_BK, id * g.width + c * g.cut, &full[s]);
+                }
+                __syncwarp();
+                continue;
+            }
+            if (lane == 0) tg_expect(&full[s], (uint32_t)(groups * group_bytes));
+            __syncwarp();
+            if (whole) {
+                if (lane == 0) tg_load_2d(st, &map_all, kb * LT_BK, first, &full[s]);
+            } else if (together) {
+                if (lane < groups) tg_load_2d(st + lane * 4096, &map_some, kb * LT_BK, first + 32 * lane, &full[s]);
+            } else if (lane < groups) {
+                tg_gather4(st + lane * 512, &map_row, kb * LT_BK, src[0], src[1], src[2], src[3], &full[s]);
+            }
+        }
+        if (!ok) tg_settle_copies(full, g.stages, it, &low_rank_error_flag, 1);
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = tg_idesc(g.cut);
+            uint32_t it = 0;
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % g.stages;
+                ok = tg_wait(&full[s], (it / g.stages) & 1, &low_rank_error_flag, 2);
+                if (!ok) break;
+                tg_after();
+                unsigned char* const st = base + (size_t)s * stage_bytes;
+                const uint64_t dx = tg_desc(st);
+                for (int c = 0; c < g.cuts; ++c) {
+                    const uint64_t da = tg_desc(st + LT_X_BYTES + c * g.cut * LT_BK * 2);
+#pragma unroll
+                    for (int k = 0; k < LT_BK / 16; ++k) tg_mma(tmem + c * g.cut, dx + 2 * k, da + 2 * k, idesc, (it > 0 || k > 0) ? 1u : 0u);
+                }
+                tg_commit(&empty[s]);
+            }
+            if (ok) tg_commit(done);
+            else tg_settle_products(settled, &low_rank_error_flag, 2);
+        }
+    } else {
+        const int quarter = warp & 3;                        // tensor-memory lanes this warp may read
+        const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t stage = tg_smem(out_stage + (warp - 2) * LT_STAGE_OUT);
+        const bool ok = __all_sync(0xffffffffu, tg_wait(done, 0, &low_rank_error_flag, 3));
+        tg_after();
+        float* const to = part + ((size_t)split * T + r0 + quarter * 32) * g.width;
+        for (int c = 0; ok && quarter * 32 < rows && c < g.width; c += 32) {
+            uint32_t a[32];
+            tg_ld32(acc + c, a);
+            tg_wait_ld();
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(stage + (uint32_t)(lane * 128 + ((q ^ (lane & 7)) << 4))),
+                             "r"(a[4 * q]), "r"(a[4 * q + 1]), "r"(a[4 * q + 2]), "r"(a[4 * q + 3]) : "memory");
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + (lane >> 3), q = lane & 7;
+                uint4 x;
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                             : "r"(stage + (uint32_t)(r * 128 + ((q ^ (r & 7)) << 4))) : "memory");
+                if (quarter * 32 + r < rows && c + q * 4 < g.width) *(uint4*)(to + (size_t)r * g.width + c + q * 4) = x;
+            }
+            __syncwarp();
+        }
+    }
+    tg_before();
+    __syncthreads();
+    if (warp == 1) {
+        tg_after();
+        tg_free<COLS>(tmem);
+    }
+}
+
+// Columns go through in pieces of 64: two halves of 32 slice columns, the first and the second 32 columns, or, in
+// eights, those of slice 0 and of slice 1. Column j of a half:
+#define LO_THREADS 256
+#ifndef LO_PIECES
+#define LO_PIECES 8               // pieces of a block
+#endif
+#define LO_COLS 64
+
+__device__ __forceinline__ int lo_column(bool eights, int half, int j) { return eights ? (j >> 3) * 16 + half * 8 + (j & 7) : half * 32 + j; }
+// Row pitches (bytes) of u and B in shared memory: 32 more than a multiple of 64, so that the 8-byte reads of four
+// rows by four threads each meet no bank twice.
+static inline int lo_pitch(int values) { return (values * 2 + 31) / 64 * 64 + 32; }
+
+template <int STEPS, typename TY>
+__global__ void __launch_bounds__(LO_THREADS, STEPS <= 4 ? 2 : 1)
+low_rank_out_kernel(const LowRank p, const float* __restrict__ part, int splits, int pieces, int u_pitch, int b_pitch,
+                    const int* __restrict__ perm, const int* __restrict__ info, const int* __restrict__ tiles) {
+    extern __shared__ __align__(16) unsigned char lo_smem[];
+    __shared__ int rows[LT_ROWS];
+    pdl_wait();
+    const int tile = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5, gr = lane >> 2, tig = lane & 3;
+    if (tile >= info[0]) return;
+    const int id = tiles[3 * tile], r0 = tiles[3 * tile + 1], n = tiles[3 * tile + 2];
+    const bool eights = p.columns.interleaved;
+    const int rank = p.rank, width = p.columns.slices * rank;
+    // this block's columns: `pieces` pieces of one slice (in eights: of both)
+    int slice = 0, begin = 0, end = eights ? p.N : p.columns.ends[0], group = blockIdx.x;
+#pragma unroll
+    for (int i = 1; i < LR_MAX_SLICES; ++i) {
+        const int groups = (end - begin + pieces * LO_COLS - 1) / (pieces * LO_COLS);
+        if (slice == i - 1 && group >= groups) {
+            group -= groups;
+            slice = i;
+            begin = end;
+            end = p.columns.ends[i];
+        }
+    }
+    const int col0 = begin + group * pieces * LO_COLS, col1 = min(col0 + pieces * LO_COLS, end);
+    if (t < n) rows[t] = perm[r0 + t];
+    __syncthreads();
+    const TY* const y = (const TY*)p.y;
+    TY* const out = (TY*)p.out;
+    constexpr int PER = 16 / (int)sizeof(TY);
+    if (id < 0) {                                            // no adapter: y as it is
+        if (p.out != p.y) {
+            const int vectors = (col1 - col0) / PER;
+            for (int e = t; e < n * vectors; e += LO_THREADS) {
+                const int r = rows[e / vectors], c = col0 + e % vectors * PER;
+                *(uint4*)(out + (size_t)r * p.out_stride + c) = *(const uint4*)(y + (size_t)r * p.y_stride + c);
+            }
+        }
+        return;
+    }
+    const int halves = eights ? 2 : 1;                       // slices that this block needs
+    unsigned char* const u_hi = lo_smem;                     // [halves][128][u_pitch]
+    unsigned char* const u_lo = u_hi + halves * LT_ROWS * u_pitch;
+    unsigned char* const b_ring = u_lo + halves * LT_ROWS * u_pitch;    // [2][64][b_pitch]
+    const bf16* const b = (const bf16*)p.b + (size_t)id * p.N * rank;
+    const int n_pieces = (col1 - col0 + LO_COLS - 1) / LO_COLS;
+    // B's rows of a piece: a half's column 8 a + 2 q + c stands in row 8 q + 2 a + c, the order in which product q
+    // takes its columns
+    auto fetch = [&](int piece) {
+        unsigned char* const to = b_ring + (piece & 1) * LO_COLS * b_pitch;
+        const int chunks = rank / 8;
+        for (int e = t; e < LO_COLS * chunks; e += LO_THREADS) {
+            const int r = e / chunks, k = e - r * chunks, half = r >> 5, j = r & 31;
+            const int c = col0 + piece * LO_COLS + lo_column(eights, half, j);
+            const int place = half * 32 + ((j >> 1) & 3) * 8 + (j >> 3) * 2 + (j & 1);
+            cp_async16(to + place * b_pitch + k * 16, b + (size_t)(c < col1 ? c : col0) * rank + k * 8, c < col1);
+        }
+        cp_async_commit();
+    };
+    for (int k = rank; k < STEPS * 16; k += 8) {             // the steps beyond the rank: zeros
+        for (int e = t; e < 2 * LO_COLS; e += LO_THREADS) *(uint4*)(b_ring + e * b_pitch + k * 2) = make_uint4(0, 0, 0, 0);
+        for (int e = t; e < 2 * halves * LT_ROWS; e += LO_THREADS) *(uint4*)(u_hi + e * u_pitch + k * 2) = make_uint4(0, 0, 0, 0);
+    }
+    fetch(0);
+    {
+        const float scale = p.scale[id];
+        const int quads = rank / 4;
+        for (int e = t; e < halves * LT_ROWS * quads; e += LO_THREADS) {
+            const int k = e % quads * 4, r = e / quads % LT_ROWS, h = e / quads / LT_ROWS;
+            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < n) {
+                const float* from = part + (size_t)(r0 + r) * width + (slice + h) * rank + k;
+                for (int i = 0; i < splits; ++i) {
+                    const float4 q = *(const float4*)(from + (size_t)i * p.T * width);
+                    s.x += q.x; s.y += q.y; s.z += q.z; s.w += q.w;
+                }
+                s.x *= scale; s.y *= scale; s.z *= scale; s.w *= scale;
+            }
+            const float4 f = make_float4(to_f32(from_f32<bf16>(s.x)), to_f32(from_f32<bf16>(s.y)), to_f32(from_f32<bf16>(s.z)), to_f32(from_f32<bf16>(s.w)));
+            const int at = (h * LT_ROWS + r) * u_pitch + k * 2;
+            *(uint2*)(u_hi + at) = make_uint2(pack_bf16(s.x, s.y), pack_bf16(s.z, s.w));
+            *(uint2*)(u_lo + at) = make_uint2(pack_bf16(s.x - f.x, s.y - f.y), pack_bf16(s.z - f.z, s.w - f.w));
+        }
+    }
+    const int ra = warp * 16 + gr, rb = ra + 8;              // this thread's rows of the tile
+    const TY* const ya = y + (size_t)(ra < n ? rows[ra] : 0) * p.y_stride;
+    const TY* const yb = y + (size_t)(rb < n ? rows[rb] : 0) * p.y_stride;
+    TY* const oa = out + (size_t)(ra < n ? rows[ra] : 0) * p.out_stride;
+    TY* const ob = out + (size_t)(rb < n ? rows[rb] : 0) * p.out_stride;
+    const bool any = warp * 16 < n;                          // the same for the whole warp
+    constexpr int VEC = 8 / PER;                             // 16-byte vectors of a thread's eight columns
+    uint4 next[2][2][VEC];                                   // [half][row]
+    auto read = [&](int piece) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int c = col0 + piece * LO_COLS + lo_column(eights, h, 8 * tig);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                if (c < col1 && ra < n) next[h][0][i] = *(const uint4*)(ya + c + i * PER);
+                if (c < col1 && rb < n) next[h][1][i] = *(const uint4*)(yb + c + i * PER);
+            }
+        }
+    };
+    if (any) read(0);
+    uint32_t fh[STEPS][4], fl[STEPS][4];                     // u's part of the products: kept while the slice stays
+    for (int piece = 0; piece < n_pieces; ++piece) {
+        cp_async_wait<0>();
+        __syncthreads();                                     // this piece's B (and u) is there, the other buffer is read
+        if (piece + 1 < n_pieces) fetch(piece + 1);
+        if (!any) continue;
+        uint4 cur[2][2][VEC];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) { cur[h][0][i] = next[h][0][i]; cur[h][1][i] = next[h][1][i]; }
+        if (piece + 1 < n_pieces) read(piece + 1);
+        const unsigned char* const from = b_ring + (piece & 1) * LO_COLS * b_pitch;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (eights || (piece == 0 && h == 0)) {
+                const unsigned char* const ua = u_hi + ((eights ? h : 0) * LT_ROWS + ra) * u_pitch + tig * 8;
+                const unsigned char* const ul = ua + halves * LT_ROWS * u_pitch;
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) {
+                    const uint2 a = *(const uint2*)(ua + s * 32), c = *(const uint2*)(ua + 8 * u_pitch + s * 32);
+                    const uint2 e = *(const uint2*)(ul + s * 32), f = *(const uint2*)(ul + 8 * u_pitch + s * 32);
+                    fh[s][0] = a.x; fh[s][1] = c.x; fh[s][2] = a.y; fh[s][3] = c.y;
+                    fl[s][0] = e.x; fl[s][1] = f.x; fl[s][2] = e.y; fl[s][3] = f.y;
+                }
+            }
+            float acc[4][4] = {};
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint2 w = *(const uint2*)(from + (h * 32 + q * 8 + gr) * b_pitch + s * 32 + tig * 8);
+                    mma_bf16(acc[q], fh[s], w.x, w.y);
+                    mma_bf16(acc[q], fl[s], w.x, w.y);
+                }
+            const int c = col0 + piece * LO_COLS + lo_column(eights, h, 8 * tig);
+            if (c >= col1) continue;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                uint4 ya4 = cur[h][0][i], yb4 = cur[h][1][i];
+                if constexpr (sizeof(TY) == 2) {
+                    uint32_t* const wa = (uint32_t*)&ya4;
+                    uint32_t* const wb = (uint32_t*)&yb4;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float2 va = __bfloat1622float2(*(const __nv_bfloat162*)&wa[q]), vb = __bfloat1622float2(*(const __nv_bfloat162*)&wb[q]);
+                        wa[q] = pack_bf16(va.x + acc[q][0], va.y + acc[q][1]);
+                        wb[q] = pack_bf16(vb.x + acc[q][2], vb.y + acc[q][3]);
+                    }
+                } else {
+                    float* const wa = (float*)&ya4;
+                    float* const wb = (float*)&yb4;
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        wa[2 * q] += acc[2 * i + q][0]; wa[2 * q + 1] += acc[2 * i + q][1];
+                        wb[2 * q] += acc[2 * i + q][2]; wb[2 * q + 1] += acc[2 * i + q][3];
+                    }
+                }
+                if (ra < n) *(uint4*)(oa + c + i * PER) = ya4;
+                if (rb < n) *(uint4*)(ob + c + i * PER) = yb4;
+            }
+        }
+    }
+}
+
 // --------------------------------------------------------------------------- any sizes
 // A warp a (row, slice, j): lanes go over k, so the sum's order depends on K alone.
 template <typename T>
@@ -468,6 +812,109 @@ template <typename T, typename TY> static int low_rank_few(const LowRank& p, int
     return (int)cudaLaunchKernelEx(&cfg, low_rank_few_kernel<T, TY>, p, (const int*)perm, (const int*)info, (const int*)tiles);
 }
 
+// ---- tiles of 128 rows
+// Whether the kernels for many rows take a call: what they read and write on 16 bytes, A's columns in tensor memory.
+template <typename TY> static bool lr_tile_takes(const LowRank& p) {
+    const int v = 16 / (int)sizeof(TY), width = p.columns.slices * p.rank;
+    if (!lr_vectors<bf16>(p) || p.rank % 8 || p.rank > 128 || width > LT_MAX_WIDTH || p.adapters > LP_MAX_ADAPTERS ||
+        p.T > (1 << 24) || (long long)p.adapters * width > 0x7fffffff || p.y_stride % v || p.out_stride % v ||
+        ((uintptr_t)p.y | (uintptr_t)p.out) & 15)
+        return false;
+    if (p.columns.interleaved) return p.N % 64 == 0;
+    for (int i = 0; i < p.columns.slices; ++i)
+        if (p.columns.ends[i] % 32) return false;
+    return true;
+}
+
+// Parts of k: as many as fill the multiprocessors once with the tiles that there are at least, four blocks of
+// k at the least in each.
+static int lr_splits(const LowRank& p) {
+    const int tiles = (p.T + LT_ROWS - 1) / LT_ROWS, kbs = (p.K + LT_BK - 1) / LT_BK;
+    int s = (LT_FILL * tgo_multiprocessors() + tiles - 1) / tiles;
+    s = s < kbs / 4 ? s : kbs / 4;
+    return s > 1 ? s : 1;
+}
+
+template <int COLS> static int low_rank_u(const LowRank& p, const LowRankTile& g, size_t bytes, const int* perm, const int* info, const int* tiles,
+                                          float* part, cudaStream_t stream) {
+    static bool sized[64] = {};                              // per device
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return (int)err;
+    if (dev < 0 || dev >= 64) return TGO_E_BAD_ARG;
+    if (!sized[dev]) {
+        err = cudaFuncSetAttribute(low_rank_u_kernel<COLS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+        if (err != cudaSuccess) return (int)err;
+        sized[dev] = true;
+    }
+    CUtensorMap row, some, all, a;
+    if (!tg_map(&row, p.x, p.T, p.K, p.x_stride, 1) || !tg_map(&some, p.x, p.T, p.K, p.x_stride, 32) ||
+        !tg_map(&all, p.x, p.T, p.K, p.x_stride, LT_ROWS) || !tg_map(&a, p.a, (long long)p.adapters * g.width, p.K, p.K, g.cut))
+        return TGO_E_BAD_ARG;
+    return tgo_launch_pdl(low_rank_u_kernel<COLS>, dim3(g.splits, (unsigned)lr_tiles(p, LT_ROWS)), dim3(LT_THREADS), bytes, stream, row, some, all, a,
+                          g, p.T, perm, info, tiles, part);
+}
+
+template <int STEPS, typename TY> static int low_rank_out(const LowRank& p, const float* part, int splits, const int* perm, const int* info,
+                                                          const int* tiles, cudaStream_t stream) {
+    static bool sized[64] = {};
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return (int)err;
+    if (dev < 0 || dev >= 64) return TGO_E_BAD_ARG;
+    const int u_pitch = lo_pitch(STEPS * 16), b_pitch = lo_pitch(STEPS * 16), halves = p.columns.interleaved ? 2 : 1;
+    const size_t bytes = (size_t)2 * halves * LT_ROWS * u_pitch + 2 * LO_COLS * b_pitch;
+    if (!sized[dev]) {
+        err = cudaFuncSetAttribute(low_rank_out_kernel<STEPS, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+        if (err != cudaSuccess) return (int)err;
+        sized[dev] = true;
+    }
+    int groups = 0, begin = 0;
+    for (int i = 0; i < (p.columns.interleaved ? 1 : p.columns.slices); ++i) {
+        const int end = p.columns.interleaved ? p.N : p.columns.ends[i];
+        groups += (end - begin + LO_PIECES * LO_COLS - 1) / (LO_PIECES * LO_COLS);
+        begin = end;
+    }
+    return tgo_launch_pdl(low_rank_out_kernel<STEPS, TY>, dim3(groups, (unsigned)lr_tiles(p, LT_ROWS)), dim3(LO_THREADS), bytes, stream, p, part, splits,
+                          (int)LO_PIECES, u_pitch, b_pitch, perm, info, tiles);
+}
+
+template <typename TY> static int low_rank_tiles(const LowRank& p, int* work, cudaStream_t stream) {
+    int* const perm = work;
+    int* const info = perm + p.T;
+    int* const tiles = info + 1;
+    float* const part = (float*)(work + (p.T + 1 + 3 * lr_tiles(p, LT_ROWS) + 3) / 4 * 4);
+    int rc = tgo_launch_pdl(low_rank_plan_kernel, dim3(1), dim3(LP_THREADS), 0, stream, p.ids, p.T, p.adapters, LT_ROWS, perm, info, tiles);
+    if (rc) return rc;
+    LowRankTile g;
+    g.width = p.columns.slices * p.rank;
+    g.cuts = g.width > 256 ? 2 : 1;
+    g.cut = ((g.width + g.cuts - 1) / g.cuts + 15) / 16 * 16;
+    g.kbs = (p.K + LT_BK - 1) / LT_BK;
+    g.splits = lr_splits(p);
+    const int stage = LT_X_BYTES + g.cuts * g.cut * LT_BK * 2, most = 176 * 1024 / stage, wanted = (g.kbs + g.splits - 1) / g.splits;
+    g.stages = most < 4 ? most : 4;
+    g.stages = g.stages < wanted ? g.stages : wanted;
+    const size_t bytes = (size_t)g.stages * stage + 4 * LT_STAGE_OUT + 1024 + 256;
+    const int cols = g.cuts * g.cut;
+    if (cols <= 32) rc = low_rank_u<32>(p, g, bytes, perm, info, tiles, part, stream);
+    else if (cols <= 64) rc = low_rank_u<64>(p, g, bytes, perm, info, tiles, part, stream);
+    else if (cols <= 128) rc = low_rank_u<128>(p, g, bytes, perm, info, tiles, part, stream);
+    else if (cols <= 256) rc = low_rank_u<256>(p, g, bytes, perm, info, tiles, part, stream);
+    else rc = low_rank_u<512>(p, g, bytes, perm, info, tiles, part, stream);
+    if (rc) return rc;
+    const int steps = (p.rank + 15) / 16;
+    if (steps == 1) return low_rank_out<1, TY>(p, part, g.splits, perm, info, tiles, stream);
+    if (steps == 2) return low_rank_out<2, TY>(p, part, g.splits, perm, info, tiles, stream);
+    if (steps <= 4) return low_rank_out<4, TY>(p, part, g.splits, perm, info, tiles, stream);
+    return low_rank_out<8, TY>(p, part, g.splits, perm, info, tiles, stream);
+}
+
+// Rows from which a call goes by tiles of 128.
+#ifndef LR_TILE_ROWS
+#define LR_TILE_ROWS 300
+#endif
+
 template <typename T, typename TY> static int low_rank_any(const LowRank& p, float* u, cudaStream_t stream) {
     const int width = p.columns.slices * p.rank;
     const int rc = tgo_launch_pdl(low_rank_down_kernel<T>, dim3(p.T, (width + 31) / 32), dim3(256), 0, stream, (const T*)p.x,
@@ -478,12 +925,20 @@ template <typename T, typename TY> static int low_rank_any(const LowRank& p, flo
                           p.out_stride);
 }
 
+// 32-bit numbers of workspace that a call needs.
+template <typename T, typename TY> static long long lr_work(const LowRank& p) {
+    const int width = p.columns.slices * p.rank;
+    if constexpr (sizeof(T) == 2)
+        if (p.T >= LR_TILE_ROWS && lr_tile_takes<TY>(p)) return p.T + 1 + 3 * lr_tiles(p, LT_ROWS) + 4 + (long long)lr_splits(p) * p.T * width;
+    if (lr_few_takes<T>(p)) return p.T > LR_SCAN_ROWS ? p.T + 1 + 3 * lr_tiles(p, LF_ROWS) : 0;
+    return (long long)p.T * width;
+}
+
 template <typename T, typename TY> static int low_rank_launch(const LowRank& p, void* work, long long work_ints, cudaStream_t stream) {
-    if (lr_few_takes<T>(p)) {
-        if (p.T > LR_SCAN_ROWS && work_ints < p.T + 1 + 3 * lr_tiles(p, LF_ROWS)) return TGO_E_BAD_ARG;
-        return low_rank_few<T, TY>(p, (int*)work, stream);
-    }
-    if (work_ints < (long long)p.T * p.columns.slices * p.rank) return TGO_E_BAD_ARG;
+    if (work_ints < lr_work<T, TY>(p)) return TGO_E_BAD_ARG;
+    if constexpr (sizeof(T) == 2)
+        if (p.T >= LR_TILE_ROWS && lr_tile_takes<TY>(p)) return low_rank_tiles<TY>(p, (int*)work, stream);
+    if (lr_few_takes<T>(p)) return low_rank_few<T, TY>(p, (int*)work, stream);
     return low_rank_any<T, TY>(p, (float*)work, stream);
 }
 
@@ -498,19 +953,30 @@ static bool lr_fill(LowRank& p, int T, int K, int N, int adapters, int rank, int
     return true;
 }
 
+// The code that a wait of the kernels for many rows left when it ran out, or 0. Synchronises.
+TGO_API int tgo_low_rank_error(int* value) { return (int)cudaMemcpyFromSymbol(value, low_rank_error_flag, sizeof(int)); }
+
 // x [T, K] of type dt, y and out [T, N] of type dt_y, rows strided; out may be y. a [adapters, slices, rank, K],
 // b [adapters, N, rank] of type dt; ends: the column after each slice's last. `work` holds `work_ints` 32-bit
-// numbers: the plan of the rows (T + 1 + 3 tiles), or u (T x slices x rank) where no kernel with vectors takes
-// the call.
+// numbers and lies on 16 bytes; with `needs` given nothing runs, and it gets how many the call needs.
 TGO_API int tgo_low_rank_add(const void* x, long long x_stride, const void* y, long long y_stride, void* out,
                              long long out_stride, const void* a, const void* b, const float* scale, const int* ids,
                              int dt, int dt_y, int T, int K, int N, int adapters, int rank, int slices, const int* ends,
-                             int interleaved, void* work, long long work_ints, cudaStream_t stream) {
+                             int interleaved, void* work, long long work_ints, long long* needs, cudaStream_t stream) {
     if (T <= 0) return 0;
     LowRank p = {x, y, a, b, out, x_stride, y_stride, out_stride, scale, ids};
     if (!lr_fill(p, T, K, N, adapters, rank, slices, ends, interleaved)) return TGO_E_BAD_ARG;
-    if (dt == TGO_F32 && dt_y == TGO_F32) return low_rank_launch<float, float>(p, work, work_ints, stream);
-    if (dt == TGO_BF16 && dt_y == TGO_BF16) return low_rank_launch<bf16, bf16>(p, work, work_ints, stream);
-    if (dt == TGO_BF16 && dt_y == TGO_F32) return low_rank_launch<bf16, float>(p, work, work_ints, stream);
+    if (dt == TGO_F32 && dt_y == TGO_F32) {
+        if (needs) { *needs = lr_work<float, float>(p); return 0; }
+        return low_rank_launch<float, float>(p, work, work_ints, stream);
+    }
+    if (dt == TGO_BF16 && dt_y == TGO_BF16) {
+        if (needs) { *needs = lr_work<bf16, bf16>(p); return 0; }
+        return low_rank_launch<bf16, bf16>(p, work, work_ints, stream);
+    }
+    if (dt == TGO_BF16 && dt_y == TGO_F32) {
+        if (needs) { *needs = lr_work<bf16, float>(p); return 0; }
+        return low_rank_launch<bf16, float>(p, work, work_ints, stream);
+    }
     return TGO_E_BAD_ARG;
 }

@@ -2191,15 +2191,23 @@ def low_rank_add(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.Ten
     if T == 0:
         return
     ends = array("i", itertools.accumulate(widths))
-    work_ints = max(T * S * r, T + 1 + 3 * (-(-T // 8) + min(T, n + 1)))
-    work = torch.empty(work_ints, dtype=torch.int32, device=x.device)
-    lib = entry_points("adapters")
-    _check(lib.tgo_low_rank_add(_ptr(x), c_ll(x.stride(0)), _ptr(y), c_ll(y.stride(0)), _ptr(out), c_ll(out.stride(0)),
-                                _ptr(a), _ptr(b), _ptr(scale), _ptr(ids), c_int(dtype_code(x.dtype)),
-                                c_int(dtype_code(y.dtype)), c_int(T), c_int(K), c_int(N), c_int(n), c_int(r), c_int(S),
-                                c_ll(ends.buffer_info()[0]), c_int(1 if interleaved else 0), _ptr(work), c_ll(work_ints), _stream()),
-           "low_rank_add", f"(T={T}, K={K}, N={N}, rank={r}, slices={S})")
-    LAUNCHES[0] += 1
+    call = entry_points("adapters").tgo_low_rank_add
+    args = (_ptr(x), c_ll(x.stride(0)), _ptr(y), c_ll(y.stride(0)), _ptr(out), c_ll(out.stride(0)), _ptr(a), _ptr(b),
+            _ptr(scale), _ptr(ids), c_int(dtype_code(x.dtype)), c_int(dtype_code(y.dtype)), c_int(T), c_int(K), c_int(N),
+            c_int(n), c_int(r), c_int(S), c_ll(ends.buffer_info()[0]), c_int(1 if interleaved else 0))
+    needs = array("q", (0,))
+    status = call(*args, 0, 0, needs.buffer_info()[0], 0)
+    if status == 0:
+        work = torch.empty(needs[0], dtype=torch.int32, device=x.device) if needs[0] else None
+        status = call(*args, _ptr(work), needs[0], 0, _stream())
+    _check(status, "low_rank_add", f"(T={T}, K={K}, N={N}, rank={r}, slices={S})")
+
+
+def low_rank_error() -> int:
+    """The code a wait of the adapters' kernels left when it ran out, or 0. Synchronises."""
+    value = ctypes.c_int(0)
+    _check(entry_points("adapters").tgo_low_rank_error(ctypes.addressof(value)), "low_rank_error")
+    return int(value.value)
 
 
 _tc_err = {}
@@ -2313,6 +2321,10 @@ def kernel_wait_errors() -> dict:
         code = ssd_error()
         if code:
             out["selective_scan"] = code
+    if "adapters" in _loaded:
+        code = low_rank_error()
+        if code:
+            out["low_rank_add"] = code
     if "retention" in _loaded:
         code = retention_error()
         if code:
