@@ -37,31 +37,73 @@ struct LowRank {
 // ------------------------------------------------------------------------- the rows of an adapter
 // For many rows: which rows have which adapter, in tiles of up to `tile` rows of one adapter (rows without
 // one come last, as tiles of adapter -1). perm: the rows by tile; info[0]: the number of tiles, a tile is
-// (adapter, first place in perm, rows). One block; the order of an adapter's rows is kept within 32.
+// (adapter, first place in perm, rows). One block; a warp has a run of rows. With up to 255 adapters each warp
+// counts for itself, and an adapter's rows keep their order: the rows of a request then lie together, and a tile of them
+// can be fetched as one box. With more, rows take their places as they come, 32 at a time in order.
 #define LP_THREADS 1024
-#define LP_MAX_ADAPTERS 4095
+#define LP_WARPS (LP_THREADS / 32)
+#define LP_MAX_ADAPTERS 3071
+#define LP_ORDERED 255
+#define LP_HELD 8                 // rows a thread holds; more are read twice
+static_assert((LP_WARPS + 2) * (LP_ORDERED + 1) <= 3 * (LP_MAX_ADAPTERS + 1), "the plan's shared memory");
 
 __global__ void __launch_bounds__(LP_THREADS)
 low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile, int* __restrict__ perm, int* __restrict__ info,
                      int* __restrict__ tiles) {
-    __shared__ int rows_of[LP_MAX_ADAPTERS + 1];             // rows, then the next free place
-    __shared__ int tiles_before[LP_MAX_ADAPTERS + 1];
-    __shared__ int warp_rows[32], warp_tiles[32];
+    __shared__ int pool[3 * (LP_MAX_ADAPTERS + 1)];
+    __shared__ int warp_rows[LP_WARPS], warp_tiles[LP_WARPS];
     pdl_wait();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, slots = adapters + 1;
-    for (int i = t; i < slots; i += LP_THREADS) rows_of[i] = 0;
+    const bool ordered = adapters <= LP_ORDERED;
+    int* const rows_before = pool;
+    int* const tiles_before = rows_before + slots;
+    int* const counts = tiles_before + slots;                // [warp][adapter], or [adapter] alone
+    const int run = (T + LP_THREADS - 1) / LP_THREADS * 32, from = min(warp * run, T), to = min(from + run, T);
+    int held[LP_HELD];
+    auto slot_of = [&](int r) {                              // -1: no row
+        const int id = r < to ? ids[r] : 0;
+        return r >= to ? -1 : id >= 0 && id < adapters ? id : adapters;
+    };
+#pragma unroll
+    for (int i = 0; i < LP_HELD; ++i) held[i] = slot_of(from + i * 32 + lane);
+    for (int i = t; i < (ordered ? LP_WARPS * slots : slots); i += LP_THREADS) counts[i] = 0;
     __syncthreads();
-    for (int base = warp * 32; base < T; base += LP_THREADS) {
-        const int r = base + lane;
-        const int id = r < T ? ids[r] : -2, slot = r >= T ? -1 : id >= 0 && id < adapters ? id : adapters;
+    int* const mine = ordered ? counts + warp * slots : counts;
+    auto each = [&](auto&& take) {                           // 32 rows of the run at a time
+#pragma unroll
+        for (int i = 0; i < LP_HELD; ++i)
+            if (from + i * 32 < to) take(from + i * 32 + lane, held[i]);
+        for (int base = from + LP_HELD * 32; base < to; base += 32) take(base + lane, slot_of(base + lane));
+    };
+    each([&](int, int slot) {
         const unsigned same = __match_any_sync(0xffffffffu, slot);
-        if (slot >= 0 && lane == __ffs(same) - 1) atomicAdd(&rows_of[slot], __popc(same));
-    }
+        if (slot >= 0 && lane == __ffs(same) - 1) {
+            if (ordered) mine[slot] += __popc(same);
+            else atomicAdd(&mine[slot], __popc(same));
+        }
+        __syncwarp();
+    });
     __syncthreads();
     // exclusive sums of rows and of tiles over the adapters, a thread a run of neighbours
     const int per = (slots + LP_THREADS - 1) / LP_THREADS, first = min(t * per, slots), last = min(first + per, slots);
     int my_rows = 0, my_tiles = 0;
-    for (int i = first; i < last; ++i) { my_rows += rows_of[i]; my_tiles += (rows_of[i] + tile - 1) / tile; }
+    for (int i = first; i < last; ++i) {
+        int n = 0;
+        if (ordered) {
+#pragma unroll 8
+            for (int w = 0; w < LP_WARPS; ++w) {             // a warp's rows of an adapter come after the earlier warps'
+                const int c = counts[w * slots + i];
+                counts[w * slots + i] = n;
+                n += c;
+            }
+        } else {
+            n = counts[i];
+            counts[i] = 0;
+        }
+        rows_before[i] = n;
+        my_rows += n;
+        my_tiles += (n + tile - 1) / tile;
+    }
     int sum_rows = my_rows, sum_tiles = my_tiles;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -70,23 +112,16 @@ low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile,
     }
     if (lane == 31) { warp_rows[warp] = sum_rows; warp_tiles[warp] = sum_tiles; }
     __syncthreads();
-    if (warp == 0) {
-        int a = warp_rows[lane], b = warp_tiles[lane];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int c = __shfl_up_sync(0xffffffffu, a, o), d = __shfl_up_sync(0xffffffffu, b, o);
-            if (lane >= o) { a += c; b += d; }
-        }
-        warp_rows[lane] = a;
-        warp_tiles[lane] = b;
+    int at_row = sum_rows - my_rows, at_tile = sum_tiles - my_tiles, total = 0;
+    {
+        const int a = warp_rows[lane], b = warp_tiles[lane];
+        at_row += __reduce_add_sync(0xffffffffu, lane < warp ? a : 0);
+        at_tile += __reduce_add_sync(0xffffffffu, lane < warp ? b : 0);
+        total = __reduce_add_sync(0xffffffffu, b);
     }
-    __syncthreads();
-    int at_row = sum_rows - my_rows + (warp ? warp_rows[warp - 1] : 0);
-    int at_tile = sum_tiles - my_tiles + (warp ? warp_tiles[warp - 1] : 0);
-    const int total = warp_tiles[31];
     for (int i = first; i < last; ++i) {
-        const int n = rows_of[i];
-        rows_of[i] = at_row;
+        const int n = rows_before[i];
+        rows_before[i] = at_row;
         tiles_before[i] = at_tile;
         at_row += n;
         at_tile += (n + tile - 1) / tile;
@@ -99,23 +134,24 @@ low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile,
             const int mid = (lo + hi + 1) >> 1;
             if (tiles_before[mid] <= q) lo = mid; else hi = mid - 1;
         }
-        const int begin = rows_of[lo] + (q - tiles_before[lo]) * tile;
-        const int end = lo + 1 < slots ? rows_of[lo + 1] : T;
+        const int begin = rows_before[lo] + (q - tiles_before[lo]) * tile;
+        const int end = lo + 1 < slots ? rows_before[lo + 1] : T;
         tiles[3 * q] = lo < adapters ? lo : -1;
         tiles[3 * q + 1] = begin;
         tiles[3 * q + 2] = min(tile, end - begin);
     }
-    __syncthreads();
-    for (int base = warp * 32; base < T; base += LP_THREADS) {
-        const int r = base + lane;
-        const int id = r < T ? ids[r] : -2, slot = r >= T ? -1 : id >= 0 && id < adapters ? id : adapters;
+    each([&](int r, int slot) {
         const unsigned same = __match_any_sync(0xffffffffu, slot);
         const int leader = __ffs(same) - 1;
         int place = 0;
-        if (slot >= 0 && lane == leader) place = atomicAdd(&rows_of[slot], __popc(same));
+        if (slot >= 0 && lane == leader) {
+            if (ordered) { place = mine[slot]; mine[slot] = place + __popc(same); }
+            else place = atomicAdd(&mine[slot], __popc(same));
+        }
         place = __shfl_sync(0xffffffffu, place, leader);
-        if (slot >= 0) perm[place + __popc(same & ((1u << lane) - 1))] = r;
-    }
+        if (slot >= 0) perm[rows_before[slot] + place + __popc(same & ((1u << lane) - 1))] = r;
+        __syncwarp();
+    });
 }
 
 // ---------------------------------------------------------------------- few rows of an adapter

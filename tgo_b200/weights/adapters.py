@@ -25,7 +25,7 @@ from ..parts.base import AdapterBank, AdapterSite
 from .safetensors import SafetensorsFile
 
 PREFIX = "base_model.model."
-MAX_ADAPTERS = 4095               # one bank's; the kernels' plan of a step's rows holds as many
+MAX_ADAPTERS = 3071               # one bank's; the kernels' plan of a step's rows holds as many
 
 
 class AdapterError(ValueError):
