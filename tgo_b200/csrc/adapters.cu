@@ -574,21 +574,24 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
 #define LO_COLS 64
 
 __device__ __forceinline__ int lo_column(bool eights, int half, int j) { return eights ? (j >> 3) * 16 + half * 8 + (j & 7) : half * 32 + j; }
-// Row pitches (bytes) of u and B in shared memory: 32 more than a multiple of 64, so that the 8-byte reads of four
+// Row pitch (bytes) of u and B in shared memory: 32 more than a multiple of 64, so that the 8-byte reads of four
 // rows by four threads each meet no bank twice.
-static inline int lo_pitch(int values) { return (values * 2 + 31) / 64 * 64 + 32; }
+__host__ __device__ constexpr int lo_pitch(int steps) { return (steps * 32 + 31) / 64 * 64 + 32; }
 
-template <int STEPS, typename TY>
+// STEPS: of 16 values of the rank.
+template <int STEPS, bool EIGHTS, typename TY>
 __global__ void __launch_bounds__(LO_THREADS, STEPS <= 4 ? 2 : 1)
-low_rank_out_kernel(const LowRank p, const float* __restrict__ part, int splits, int pieces, int u_pitch, int b_pitch,
-                    const int* __restrict__ perm, const int* __restrict__ info, const int* __restrict__ tiles) {
+low_rank_out_kernel(const LowRank p, const float* __restrict__ part, int splits, const int* __restrict__ perm,
+                    const int* __restrict__ info, const int* __restrict__ tiles) {
+    constexpr int pitch = lo_pitch(STEPS), pieces = LO_PIECES, halves = EIGHTS ? 2 : 1;    // halves: slices that a block needs
+    constexpr bool KEEP = !EIGHTS || STEPS <= 2;             // u's operands stay in registers
+    constexpr bool eights = EIGHTS;
     extern __shared__ __align__(16) unsigned char lo_smem[];
     __shared__ int rows[LT_ROWS];
     pdl_wait();
     const int tile = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5, gr = lane >> 2, tig = lane & 3;
     if (tile >= info[0]) return;
     const int id = tiles[3 * tile], r0 = tiles[3 * tile + 1], n = tiles[3 * tile + 2];
-    const bool eights = p.columns.interleaved;
     const int rank = p.rank, width = p.columns.slices * rank;
     // this block's columns: `pieces` pieces of one slice (in eights: of both)
     int slice = 0, begin = 0, end = eights ? p.N : p.columns.ends[0], group = blockIdx.x;
@@ -618,107 +621,126 @@ low_rank_out_kernel(const LowRank p, const float* __restrict__ part, int splits,
         }
         return;
     }
-    const int halves = eights ? 2 : 1;                       // slices that this block needs
-    unsigned char* const u_hi = lo_smem;                     // [halves][128][u_pitch]
-    unsigned char* const u_lo = u_hi + halves * LT_ROWS * u_pitch;
-    unsigned char* const b_ring = u_lo + halves * LT_ROWS * u_pitch;    // [2][64][b_pitch]
+    unsigned char* const u_hi = lo_smem;                     // [halves][128][pitch]
+    unsigned char* const u_lo = u_hi + halves * LT_ROWS * pitch;
+    unsigned char* const b_ring = u_lo + halves * LT_ROWS * pitch;      // [2][64][pitch]
     const bf16* const b = (const bf16*)p.b + (size_t)id * p.N * rank;
     const int n_pieces = (col1 - col0 + LO_COLS - 1) / LO_COLS;
     // B's rows of a piece: a half's column 8 a + 2 q + c stands in row 8 q + 2 a + c, the order in which product q
     // takes its columns
+    // Four threads a row. j: the row's column of its half; its own place in the ring and its way through B
+    const int f_half = t >> 7, f_j = (t >> 2) & 31, f_first = lo_column(eights, f_half, f_j);
+    unsigned char* const f_to = b_ring + (f_half * 32 + ((f_j >> 1) & 3) * 8 + (f_j >> 3) * 2 + (f_j & 1)) * pitch + (t & 3) * 16;
+    const bf16* const f_from = b + (size_t)(col0 + f_first) * rank + (t & 3) * 8;
     auto fetch = [&](int piece) {
-        unsigned char* const to = b_ring + (piece & 1) * LO_COLS * b_pitch;
-        const int chunks = rank / 8;
-        for (int e = t; e < LO_COLS * chunks; e += LO_THREADS) {
-            const int r = e / chunks, k = e - r * chunks, half = r >> 5, j = r & 31;
-            const int c = col0 + piece * LO_COLS + lo_column(eights, half, j);
-            const int place = half * 32 + ((j >> 1) & 3) * 8 + (j >> 3) * 2 + (j & 1);
-            cp_async16(to + place * b_pitch + k * 16, b + (size_t)(c < col1 ? c : col0) * rank + k * 8, c < col1);
-        }
+        const bool there = col0 + piece * LO_COLS + f_first < col1;
+        const bf16* const from = there ? f_from + (size_t)piece * LO_COLS * rank : b;
+        unsigned char* const to = f_to + (piece & 1) * LO_COLS * pitch;
+#pragma unroll
+        for (int i = 0; i < (STEPS + 1) / 2; ++i)
+            if (((t & 3) + 4 * i) * 8 < rank) cp_async16(to + i * 64, from + (there ? i * 32 : 0), there);
         cp_async_commit();
     };
-    for (int k = rank; k < STEPS * 16; k += 8) {             // the steps beyond the rank: zeros
-        for (int e = t; e < 2 * LO_COLS; e += LO_THREADS) *(uint4*)(b_ring + e * b_pitch + k * 2) = make_uint4(0, 0, 0, 0);
-        for (int e = t; e < 2 * halves * LT_ROWS; e += LO_THREADS) *(uint4*)(u_hi + e * u_pitch + k * 2) = make_uint4(0, 0, 0, 0);
-    }
+    for (int k = rank; k < STEPS * 16; k += 8)               // the steps beyond the rank: zeros (u's too, below)
+        for (int e = t; e < 2 * LO_COLS; e += LO_THREADS) *(uint4*)(b_ring + e * pitch + k * 2) = make_uint4(0, 0, 0, 0);
     fetch(0);
     {
+        // four threads a row, four neighbouring values each at a time
         const float scale = p.scale[id];
-        const int quads = rank / 4;
-        for (int e = t; e < halves * LT_ROWS * quads; e += LO_THREADS) {
-            const int k = e % quads * 4, r = e / quads % LT_ROWS, h = e / quads / LT_ROWS;
-            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < n) {
-                const float* from = part + (size_t)(r0 + r) * width + (slice + h) * rank + k;
-                for (int i = 0; i < splits; ++i) {
-                    const float4 q = *(const float4*)(from + (size_t)i * p.T * width);
-                    s.x += q.x; s.y += q.y; s.z += q.z; s.w += q.w;
-                }
-                s.x *= scale; s.y *= scale; s.z *= scale; s.w *= scale;
+        for (int r = t >> 2; r < halves * LT_ROWS; r += LO_THREADS / 4) {
+            const int row = r & (LT_ROWS - 1), h = r / LT_ROWS;
+            const float* const from = part + (size_t)(r0 + min(row, n - 1)) * width + (slice + h) * rank + (t & 3) * 4;
+            float4 s[STEPS];
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k)
+                s[k] = row < n && k * 16 + (t & 3) * 4 < rank ? *(const float4*)(from + k * 16) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 1; i < splits; ++i) {
+                const float* const more = from + (size_t)i * p.T * width;
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k)
+                    if (row < n && k * 16 + (t & 3) * 4 < rank) {
+                        const float4 q = *(const float4*)(more + k * 16);
+                        s[k].x += q.x; s[k].y += q.y; s[k].z += q.z; s[k].w += q.w;
+                    }
             }
-            const float4 f = make_float4(to_f32(from_f32<bf16>(s.x)), to_f32(from_f32<bf16>(s.y)), to_f32(from_f32<bf16>(s.z)), to_f32(from_f32<bf16>(s.w)));
-            const int at = (h * LT_ROWS + r) * u_pitch + k * 2;
-            *(uint2*)(u_hi + at) = make_uint2(pack_bf16(s.x, s.y), pack_bf16(s.z, s.w));
-            *(uint2*)(u_lo + at) = make_uint2(pack_bf16(s.x - f.x, s.y - f.y), pack_bf16(s.z - f.z, s.w - f.w));
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) {
+                s[k].x *= scale; s[k].y *= scale; s[k].z *= scale; s[k].w *= scale;
+                const uint32_t h0 = pack_bf16(s[k].x, s[k].y), h1 = pack_bf16(s[k].z, s[k].w);
+                const int at = r * pitch + k * 32 + (t & 3) * 8;
+                *(uint2*)(u_hi + at) = make_uint2(h0, h1);
+                *(uint2*)(u_lo + at) = make_uint2(
+                    pack_bf16(s[k].x - __uint_as_float(h0 << 16), s[k].y - __uint_as_float(h0 & 0xffff0000u)),
+                    pack_bf16(s[k].z - __uint_as_float(h1 << 16), s[k].w - __uint_as_float(h1 & 0xffff0000u)));
+            }
         }
     }
     const int ra = warp * 16 + gr, rb = ra + 8;              // this thread's rows of the tile
-    const TY* const ya = y + (size_t)(ra < n ? rows[ra] : 0) * p.y_stride;
-    const TY* const yb = y + (size_t)(rb < n ? rows[rb] : 0) * p.y_stride;
-    TY* const oa = out + (size_t)(ra < n ? rows[ra] : 0) * p.out_stride;
-    TY* const ob = out + (size_t)(rb < n ? rows[rb] : 0) * p.out_stride;
+    constexpr int VEC = 8 / PER, APART = EIGHTS ? 8 : 32;    // 16-byte vectors of a thread's eight columns; columns between its halves
+    const int c0 = col0 + lo_column(eights, 0, 8 * tig);
+    const TY* ya = y + (size_t)rows[min(ra, n - 1)] * p.y_stride + c0;
+    const TY* yb = y + (size_t)rows[min(rb, n - 1)] * p.y_stride + c0;
+    TY* oa = out + (size_t)rows[min(ra, n - 1)] * p.out_stride + c0;
+    TY* ob = out + (size_t)rows[min(rb, n - 1)] * p.out_stride + c0;
     const bool any = warp * 16 < n;                          // the same for the whole warp
-    constexpr int VEC = 8 / PER;                             // 16-byte vectors of a thread's eight columns
     uint4 next[2][2][VEC];                                   // [half][row]
-    auto read = [&](int piece) {
+    auto read = [&](int piece) {                             // rows past the tile's read its last row, and store nothing
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int c = col0 + piece * LO_COLS + lo_column(eights, h, 8 * tig);
+        for (int h = 0; h < 2; ++h)
+            if (c0 + piece * LO_COLS + h * APART < col1)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                if (c < col1 && ra < n) next[h][0][i] = *(const uint4*)(ya + c + i * PER);
-                if (c < col1 && rb < n) next[h][1][i] = *(const uint4*)(yb + c + i * PER);
-            }
-        }
+                for (int i = 0; i < VEC; ++i) {
+                    next[h][0][i] = *(const uint4*)(ya + h * APART + i * PER);
+                    next[h][1][i] = *(const uint4*)(yb + h * APART + i * PER);
+                }
+        ya += LO_COLS;
+        yb += LO_COLS;
     };
     if (any) read(0);
-    uint32_t fh[STEPS][4], fl[STEPS][4];                     // u's part of the products: kept while the slice stays
+    constexpr int KEPT = KEEP ? halves : 1;
+    uint32_t fh[KEPT][STEPS][4], fl[KEPT][STEPS][4];         // u's part of the products
+    auto operands = [&](int h, int to) {
+        const unsigned char* const ua = u_hi + (h * LT_ROWS + ra) * pitch + tig * 8;
+        const unsigned char* const ul = ua + halves * LT_ROWS * pitch;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const uint2 a = *(const uint2*)(ua + s * 32), c = *(const uint2*)(ua + 8 * pitch + s * 32);
+            const uint2 e = *(const uint2*)(ul + s * 32), f = *(const uint2*)(ul + 8 * pitch + s * 32);
+            fh[to][s][0] = a.x; fh[to][s][1] = c.x; fh[to][s][2] = a.y; fh[to][s][3] = c.y;
+            fl[to][s][0] = e.x; fl[to][s][1] = f.x; fl[to][s][2] = e.y; fl[to][s][3] = f.y;
+        }
+    };
     for (int piece = 0; piece < n_pieces; ++piece) {
         cp_async_wait<0>();
         __syncthreads();                                     // this piece's B (and u) is there, the other buffer is read
         if (piece + 1 < n_pieces) fetch(piece + 1);
         if (!any) continue;
+        if (KEEP && piece == 0) {
+            operands(0, 0);
+            if (EIGHTS) operands(1, KEPT - 1);
+        }
         uint4 cur[2][2][VEC];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) { cur[h][0][i] = next[h][0][i]; cur[h][1][i] = next[h][1][i]; }
         if (piece + 1 < n_pieces) read(piece + 1);
-        const unsigned char* const from = b_ring + (piece & 1) * LO_COLS * b_pitch;
+        const unsigned char* const from = b_ring + (piece & 1) * LO_COLS * pitch + gr * pitch + tig * 8;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            if (eights || (piece == 0 && h == 0)) {
-                const unsigned char* const ua = u_hi + ((eights ? h : 0) * LT_ROWS + ra) * u_pitch + tig * 8;
-                const unsigned char* const ul = ua + halves * LT_ROWS * u_pitch;
-#pragma unroll
-                for (int s = 0; s < STEPS; ++s) {
-                    const uint2 a = *(const uint2*)(ua + s * 32), c = *(const uint2*)(ua + 8 * u_pitch + s * 32);
-                    const uint2 e = *(const uint2*)(ul + s * 32), f = *(const uint2*)(ul + 8 * u_pitch + s * 32);
-                    fh[s][0] = a.x; fh[s][1] = c.x; fh[s][2] = a.y; fh[s][3] = c.y;
-                    fl[s][0] = e.x; fl[s][1] = f.x; fl[s][2] = e.y; fl[s][3] = f.y;
-                }
-            }
+            if (!KEEP) operands(h, 0);
+            constexpr int LAST = KEPT - 1;
+            const int f = KEEP && EIGHTS && h ? LAST : 0;
             float acc[4][4] = {};
 #pragma unroll
             for (int s = 0; s < STEPS; ++s)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const uint2 w = *(const uint2*)(from + (h * 32 + q * 8 + gr) * b_pitch + s * 32 + tig * 8);
-                    mma_bf16(acc[q], fh[s], w.x, w.y);
-                    mma_bf16(acc[q], fl[s], w.x, w.y);
+                    const uint2 w = *(const uint2*)(from + (h * 32 + q * 8) * pitch + s * 32);
+                    mma_bf16(acc[q], fh[f][s], w.x, w.y);
+                    mma_bf16(acc[q], fl[f][s], w.x, w.y);
                 }
-            const int c = col0 + piece * LO_COLS + lo_column(eights, h, 8 * tig);
-            if (c >= col1) continue;
+            if (c0 + piece * LO_COLS + h * APART >= col1) continue;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 uint4 ya4 = cur[h][0][i], yb4 = cur[h][1][i];
@@ -727,9 +749,8 @@ low_rank_out_kernel(const LowRank p, const float* __restrict__ part, int splits,
                     uint32_t* const wb = (uint32_t*)&yb4;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        const float2 va = __bfloat1622float2(*(const __nv_bfloat162*)&wa[q]), vb = __bfloat1622float2(*(const __nv_bfloat162*)&wb[q]);
-                        wa[q] = pack_bf16(va.x + acc[q][0], va.y + acc[q][1]);
-                        wb[q] = pack_bf16(vb.x + acc[q][2], vb.y + acc[q][3]);
+                        wa[q] = pack_bf16(__uint_as_float(wa[q] << 16) + acc[q][0], __uint_as_float(wa[q] & 0xffff0000u) + acc[q][1]);
+                        wb[q] = pack_bf16(__uint_as_float(wb[q] << 16) + acc[q][2], __uint_as_float(wb[q] & 0xffff0000u) + acc[q][3]);
                     }
                 } else {
                     float* const wa = (float*)&ya4;
@@ -740,10 +761,12 @@ low_rank_out_kernel(const LowRank p, const float* __restrict__ part, int splits,
                         wb[2 * q] += acc[2 * i + q][2]; wb[2 * q + 1] += acc[2 * i + q][3];
                     }
                 }
-                if (ra < n) *(uint4*)(oa + c + i * PER) = ya4;
-                if (rb < n) *(uint4*)(ob + c + i * PER) = yb4;
+                if (ra < n) *(uint4*)(oa + h * APART + i * PER) = ya4;
+                if (rb < n) *(uint4*)(ob + h * APART + i * PER) = yb4;
             }
         }
+        oa += LO_COLS;
+        ob += LO_COLS;
     }
 }
 
@@ -891,28 +914,27 @@ template <int COLS> static int low_rank_u(const LowRank& p, const LowRankTile& g
                           g, p.T, perm, info, tiles, part);
 }
 
-template <int STEPS, typename TY> static int low_rank_out(const LowRank& p, const float* part, int splits, const int* perm, const int* info,
+template <int STEPS, bool EIGHTS, typename TY> static int low_rank_out(const LowRank& p, const float* part, int splits, const int* perm, const int* info,
                                                           const int* tiles, cudaStream_t stream) {
     static bool sized[64] = {};
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return (int)err;
     if (dev < 0 || dev >= 64) return TGO_E_BAD_ARG;
-    const int u_pitch = lo_pitch(STEPS * 16), b_pitch = lo_pitch(STEPS * 16), halves = p.columns.interleaved ? 2 : 1;
-    const size_t bytes = (size_t)2 * halves * LT_ROWS * u_pitch + 2 * LO_COLS * b_pitch;
+    const size_t bytes = (size_t)(2 * (EIGHTS ? 2 : 1) * LT_ROWS + 2 * LO_COLS) * lo_pitch(STEPS);
     if (!sized[dev]) {
-        err = cudaFuncSetAttribute(low_rank_out_kernel<STEPS, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+        err = cudaFuncSetAttribute(low_rank_out_kernel<STEPS, EIGHTS, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
         if (err != cudaSuccess) return (int)err;
         sized[dev] = true;
     }
     int groups = 0, begin = 0;
-    for (int i = 0; i < (p.columns.interleaved ? 1 : p.columns.slices); ++i) {
-        const int end = p.columns.interleaved ? p.N : p.columns.ends[i];
+    for (int i = 0; i < (EIGHTS ? 1 : p.columns.slices); ++i) {
+        const int end = EIGHTS ? p.N : p.columns.ends[i];
         groups += (end - begin + LO_PIECES * LO_COLS - 1) / (LO_PIECES * LO_COLS);
         begin = end;
     }
-    return tgo_launch_pdl(low_rank_out_kernel<STEPS, TY>, dim3(groups, (unsigned)lr_tiles(p, LT_ROWS)), dim3(LO_THREADS), bytes, stream, p, part, splits,
-                          (int)LO_PIECES, u_pitch, b_pitch, perm, info, tiles);
+    return tgo_launch_pdl(low_rank_out_kernel<STEPS, EIGHTS, TY>, dim3(groups, (unsigned)lr_tiles(p, LT_ROWS)), dim3(LO_THREADS), bytes, stream, p, part, splits, perm,
+                          info, tiles);
 }
 
 template <typename TY> static int low_rank_tiles(const LowRank& p, int* work, cudaStream_t stream) {
@@ -940,10 +962,16 @@ template <typename TY> static int low_rank_tiles(const LowRank& p, int* work, cu
     else rc = low_rank_u<512>(p, g, bytes, perm, info, tiles, part, stream);
     if (rc) return rc;
     const int steps = (p.rank + 15) / 16;
-    if (steps == 1) return low_rank_out<1, TY>(p, part, g.splits, perm, info, tiles, stream);
-    if (steps == 2) return low_rank_out<2, TY>(p, part, g.splits, perm, info, tiles, stream);
-    if (steps <= 4) return low_rank_out<4, TY>(p, part, g.splits, perm, info, tiles, stream);
-    return low_rank_out<8, TY>(p, part, g.splits, perm, info, tiles, stream);
+    if (p.columns.interleaved) {
+        if (steps == 1) return low_rank_out<1, true, TY>(p, part, g.splits, perm, info, tiles, stream);
+        if (steps == 2) return low_rank_out<2, true, TY>(p, part, g.splits, perm, info, tiles, stream);
+        if (steps <= 4) return low_rank_out<4, true, TY>(p, part, g.splits, perm, info, tiles, stream);
+        return low_rank_out<8, true, TY>(p, part, g.splits, perm, info, tiles, stream);
+    }
+    if (steps == 1) return low_rank_out<1, false, TY>(p, part, g.splits, perm, info, tiles, stream);
+    if (steps == 2) return low_rank_out<2, false, TY>(p, part, g.splits, perm, info, tiles, stream);
+    if (steps <= 4) return low_rank_out<4, false, TY>(p, part, g.splits, perm, info, tiles, stream);
+    return low_rank_out<8, false, TY>(p, part, g.splits, perm, info, tiles, stream);
 }
 
 // Rows from which a call goes by tiles of 128.
