@@ -96,7 +96,7 @@ def test_columns_in_eights(x_type, y_type, T, K, f, rank):
 @pytest.mark.parametrize("T,K,widths,rank,adapters,interleaved", [
     (300, 64, (64,), 8, 1, False), (301, 2048, (2048,), 16, 4, False), (513, 1032, (256, 64, 64), 24, 3, False),
     (1000, 512, (96, 32), 40, 7, False), (640, 4096, (512, 128, 128), 64, 2, False), (333, 768, (1056,), 128, 3, False),
-    (700, 640, (512, 64, 32, 96), 128, 2, False), (400, 256, (512, 512), 16, 5, True), (777, 1000, (96, 96), 32, 3, True),
+    (700, 640, (512, 64, 32, 96), 128, 2, False), (310, 320, (64, 32, 96, 128), 72, 2, False), (400, 256, (512, 512), 16, 5, True), (777, 1000, (96, 96), 32, 3, True),
     (450, 512, (160, 160), 128, 2, True), (2500, 192, (64, 64), 8, 30, True)])
 def test_many_rows(y_type, T, K, widths, rank, adapters, interleaved):
     """Mixed rows, and runs of unlike lengths as prompts of requests leave them."""

@@ -407,41 +407,41 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
 // ---------------------------------------------------------------------- many rows of an adapter
 // Tiles of 128 planned rows, bfloat16. Two kernels, u between them in float32:
 //
-// u (`low_rank_u_kernel`): [128, slices x rank] = X[rows] A^T, a part of k a block, on tcgen05: TMA brings 64
-// columns of the tile's rows (one box where they lie together, else four rows a request) and of A into a ring,
-// a thread issues the products, four warps hand the accumulator on. Bound by x's way from memory.
+// u (`low_rank_u_kernel`): [128, slices x rank] = X[rows] A^T on tcgen05, a cluster a tile, a part of k a block:
+// TMA brings 64 columns of the tile's rows (one box where they lie together, else four rows a request) and of A
+// into a ring, a thread issues the products. The blocks sum their parts through each other's shared memory, scale
+// u and split it into two bfloat16 numbers (see above). Bound by x's way from memory.
 //
-// out (`low_rank_out_kernel`): the parts of u are summed and split into two bfloat16 numbers (see above), 64
-// columns of B at a time come into shared memory, mma.sync makes 16 rows x 32 columns a warp, y is read one step
-// ahead and added in registers. Which column of B stands where in a product is chosen so that a thread ends up
-// with eight neighbouring columns: y and out move 16 bytes (float32: 32) at a time. Bound by y's and out's way.
+// out (`low_rank_out_kernel`): u and 128 columns of B at a time come by TMA, a thread issues the products into two
+// accumulators in turn, eight warps add y, read ahead, and write. Bound by y's and out's way.
 #define LT_ROWS 128
 #define LT_BK 64
 #define LT_X_BYTES (LT_ROWS * LT_BK * 2)
-#define LT_STAGE_OUT 4096         // per handing-on warp: 32 rows x 128 bytes
+#define LT_PASS 256               // columns of u that the blocks of a cluster exchange at a time
 #define LT_THREADS 224
-#ifndef LT_FILL
-#define LT_FILL 1
-#endif
 #define LT_MAX_WIDTH 512          // slices x rank: the columns of tensor memory
 
 __device__ int low_rank_error_flag = 0;
 
 struct LowRankTile {
-    int width, cut, cuts, kbs, splits, stages;    // A's rows come in `cuts` boxes of `cut`
+    int width, cut, cuts, kbs, splits, stages;    // A's rows come in `cuts` boxes of `cut`; `splits` blocks a cluster
 };
+// Bytes of the ring, which later holds a pass of sums.
+__host__ __device__ static inline int lt_ring(const LowRankTile& g) {
+    const int ring = g.stages * (LT_X_BYTES + g.cuts * g.cut * LT_BK * 2), pass = (g.width < LT_PASS ? (g.width + 31) / 32 * 32 : LT_PASS) * LT_ROWS * 4;
+    return ring > pass ? ring : pass;
+}
 
 template <int COLS>
 __global__ void __launch_bounds__(LT_THREADS)
 low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_constant__ CUtensorMap map_some,
                   const __grid_constant__ CUtensorMap map_all, const __grid_constant__ CUtensorMap map_a, const LowRankTile g,
-                  int T, const int* __restrict__ perm, const int* __restrict__ info, const int* __restrict__ tiles,
-                  float* __restrict__ part) {
+                  int rank, const float* __restrict__ scale, const int* __restrict__ perm, const int* __restrict__ info,
+                  const int* __restrict__ tiles, bf16* __restrict__ u) {
     extern __shared__ unsigned char lt_raw[];
     unsigned char* const base = (unsigned char*)(((uintptr_t)lt_raw + 1023) & ~(uintptr_t)1023);
     const int stage_bytes = LT_X_BYTES + g.cuts * g.cut * LT_BK * 2;
-    unsigned char* const out_stage = base + (size_t)g.stages * stage_bytes;
-    uint64_t* const full = (uint64_t*)(out_stage + 4 * LT_STAGE_OUT);
+    uint64_t* const full = (uint64_t*)(base + lt_ring(g));
     uint64_t* const empty = full + 8;
     uint64_t* const done = empty + 8;
     uint64_t* const settled = done + 1;                      // after a wait ran out
@@ -463,6 +463,7 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
     tg_after();
     const uint32_t tmem = *tmem_slot;
     const int kb0 = g.kbs * split / g.splits, kb1 = g.kbs * (split + 1) / g.splits;
+    bool handed = false;                                     // the sums are there
 
     if (warp == 0 || warp == 6) {
         // ---- rows (warp 0) and A (warp 6)
@@ -531,31 +532,66 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
             else tg_settle_products(settled, &low_rank_error_flag, 2);
         }
     } else {
-        const int quarter = warp & 3;                        // tensor-memory lanes this warp may read
-        const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t stage = tg_smem(out_stage + (warp - 2) * LT_STAGE_OUT);
-        const bool ok = __all_sync(0xffffffffu, tg_wait(done, 0, &low_rank_error_flag, 3));
-        tg_after();
-        float* const to = part + ((size_t)split * T + r0 + quarter * 32) * g.width;
-        for (int c = 0; ok && quarter * 32 < rows && c < g.width; c += 32) {
-            uint32_t a[32];
-            tg_ld32(acc + c, a);
-            tg_wait_ld();
+        handed = __all_sync(0xffffffffu, tg_wait(done, 0, &low_rank_error_flag, 3));
+    }
+    __syncwarp();
+    tg_before();
+    __syncthreads();
+    tg_after();
+    // The ring is free: each block of the cluster lays its sums out there, LT_PASS columns a pass (a row's 16-byte pieces
+    // swapped by its place among eight, so that neither side meets a bank twice), and sums an equal share of the rows over
+    // all of them, in the blocks' order. Rank by rank the values are rounded to whole sixteens with zeros.
+    const float by = scale[id];
+    const int padded = (rank + 15) / 16 * 16, slices = g.width / rank, quads = padded / 4;
+    const int share = LT_ROWS / g.splits;
+    for (int c0 = 0; c0 < g.width; c0 += LT_PASS) {
+        const int c1 = min(c0 + LT_PASS, g.width);
+        if (warp >= 2 && warp < 6 && handed) {
+            const int quarter = warp & 3;                    // tensor-memory lanes this warp may read
+            const int row = quarter * 32 + lane;
+            for (int c = c0; quarter * 32 < rows && c < c1; c += 32) {
+                uint32_t a[32];
+                tg_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + c, a);
+                tg_wait_ld();
+                unsigned char* const to = base + (c - c0) * (LT_ROWS * 4) + row * 128;
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(stage + (uint32_t)(lane * 128 + ((q ^ (lane & 7)) << 4))),
-                             "r"(a[4 * q]), "r"(a[4 * q + 1]), "r"(a[4 * q + 2]), "r"(a[4 * q + 3]) : "memory");
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = i * 4 + (lane >> 3), q = lane & 7;
-                uint4 x;
-                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
-                             : "r"(stage + (uint32_t)(r * 128 + ((q ^ (r & 7)) << 4))) : "memory");
-                if (quarter * 32 + r < rows && c + q * 4 < g.width) *(uint4*)(to + (size_t)r * g.width + c + q * 4) = x;
+                for (int q = 0; q < 8; ++q) *(uint4*)(to + ((q ^ (row & 7)) << 4)) = make_uint4(a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]);
             }
-            __syncwarp();
         }
+        lf_cluster_arrive();
+        lf_cluster_wait();
+        // a lane four values of a slice, a warp a row at a time
+        const int s0 = c0 / rank, s1 = (c1 + rank - 1) / rank;   // slices that this pass touches
+        for (int e = lane; e < (s1 - s0) * quads; e += 32) {
+            const int s = s0 + e / quads, k = e % quads * 4, c = s * rank + k;
+            // the zeros behind a slice are written with its last value
+            if (k < rank ? c < c0 || c >= c1 : (s + 1) * rank <= c0 || (s + 1) * rank > c1) continue;
+            const unsigned char* const from = base + (c - c0) / 32 * (32 * LT_ROWS * 4);
+            const int piece = (c - c0) % 32 / 4;
+            bf16* const to = u + ((size_t)r0 * slices + s) * 2 * padded + k;
+#pragma unroll 2
+            for (int row = split * share + warp; row < min((split + 1) * share, rows); row += LT_THREADS / 32) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (k < rank) {
+                    const float* const at = (const float*)(from + row * 128 + ((piece ^ (row & 7)) << 4));
+                    if (g.splits == 1) v = *(const float4*)at;
+                    else
+                        for (int i = 0; i < g.splits; ++i) {
+                            const float4 q = lf_peer(at, i);
+                            v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+                        }
+                    v.x *= by; v.y *= by; v.z *= by; v.w *= by;
+                }
+                const uint32_t h0 = pack_bf16(v.x, v.y), h1 = pack_bf16(v.z, v.w);
+                bf16* const at = to + (size_t)row * slices * 2 * padded;
+                *(uint2*)at = make_uint2(h0, h1);
+                *(uint2*)(at + padded) = make_uint2(
+                    pack_bf16(v.x - __uint_as_float(h0 << 16), v.y - __uint_as_float(h0 & 0xffff0000u)),
+                    pack_bf16(v.z - __uint_as_float(h1 << 16), v.w - __uint_as_float(h1 & 0xffff0000u)));
+            }
+        }
+        lf_cluster_arrive();
+        lf_cluster_wait();                                   // nobody reads this block's sums any more
     }
     tg_before();
     __syncthreads();
@@ -565,39 +601,75 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
     }
 }
 
-// Columns go through in pieces of 64: two halves of 32 slice columns, the first and the second 32 columns, or, in
-// eights, those of slice 0 and of slice 1. Column j of a half:
-#define LO_THREADS 256
-#ifndef LO_PIECES
-#define LO_PIECES 8               // pieces of a block
-#endif
+// 64 columns a turn. In eights the rows of B that a turn brings, eight of slice 0 and eight of slice 1 in turn,
+// are two operands of 32 rows whose groups of eight lie twice as far apart: nothing is moved.
+//
+// y and out go through shared memory, asynchronously: each of four warps has 32 rows (the ones whose sums it can read
+// from tensor memory, a lane a row) and a ring of its own of 32 x 64 tiles; it adds the sums where y lies and has the
+// tile stored from there. Rows that lie together are one box either way; others come four at a time and are written by
+// the warp, as are part tiles. (Reading y into registers two steps ahead and writing from them, through a transposing
+// buffer, took 68 us where this takes XXX: 8192 rows of 6144 columns.)
 #define LO_COLS 64
+#ifndef LO_TURNS
+#define LO_TURNS 8                // of a block
+#endif
+#define LO_THREADS 160
+#define LO_U_BOX (LT_ROWS * 128)  // bytes of 64 values of k: of 128 rows of u,
+#define LO_B_BOX (LO_COLS * 128)  // of a turn's rows of B
 
-__device__ __forceinline__ int lo_column(bool eights, int half, int j) { return eights ? (j >> 3) * 16 + half * 8 + (j & 7) : half * 32 + j; }
-// Row pitch (bytes) of u and B in shared memory: 32 more than a multiple of 64, so that the 8-byte reads of four
-// rows by four threads each meet no bank twice.
-__host__ __device__ constexpr int lo_pitch(int steps) { return (steps * 32 + 31) / 64 * 64 + 32; }
+__device__ __forceinline__ void lo_store_2d(const CUtensorMap* map, int x, int y, const void* src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(tg_smem(src)), "r"(x), "r"(y) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// Operand tile as tg_desc, the groups of eight rows `apart` bytes from each other.
+__device__ __forceinline__ uint64_t lo_desc(const void* tile, uint32_t apart) {
+    return (tg_desc(tile) & ~((uint64_t)0x3fff << 32)) | ((uint64_t)(apart >> 4) << 32);
+}
 
-// STEPS: of 16 values of the rank.
-template <int STEPS, bool EIGHTS, typename TY>
-__global__ void __launch_bounds__(LO_THREADS, STEPS <= 4 ? 2 : 1)
-low_rank_out_kernel(const LowRank p, const float* __restrict__ part, int splits, const int* __restrict__ perm,
+// BOXES: of 64 values of the rank. PAIRED (rank up to 32): a row's rounded values and the rest share a box.
+template <int BOXES, bool PAIRED, bool EIGHTS, typename TY> struct LowRankOut {
+    static constexpr int SLICES = EIGHTS ? 2 : 1, PARTS = PAIRED ? 1 : 2;
+    static constexpr int A_BYTES = SLICES * PARTS * BOXES * LO_U_BOX, B_BYTES = BOXES * LO_B_BOX;
+    static constexpr int Y_BOXES = (int)sizeof(TY) / 2, Y_BYTES = Y_BOXES * 32 * 128;     // a warp's tile: boxes of 128 bytes a row
+    static constexpr int SLOTS = Y_BOXES == 1 ? 3 : 2;
+    static constexpr int BYTES = A_BYTES + 2 * B_BYTES + 4 * SLOTS * Y_BYTES + 1024 + 512;
+    static_assert(BYTES + LT_ROWS * 4 <= 227 * 1024, "shared memory of a block");
+};
+
+template <int BOXES, bool PAIRED, bool EIGHTS, typename TY>
+__global__ void __launch_bounds__(LO_THREADS)
+low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_b,
+                    const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_row,
+                    const __grid_constant__ CUtensorMap map_out, const LowRank p, const int* __restrict__ perm,
                     const int* __restrict__ info, const int* __restrict__ tiles) {
-    constexpr int pitch = lo_pitch(STEPS), pieces = LO_PIECES, halves = EIGHTS ? 2 : 1;    // halves: slices that a block needs
-    constexpr bool KEEP = !EIGHTS || STEPS <= 2;             // u's operands stay in registers
-    constexpr bool eights = EIGHTS;
-    extern __shared__ __align__(16) unsigned char lo_smem[];
+    typedef LowRankOut<BOXES, PAIRED, EIGHTS, TY> L;
+    extern __shared__ unsigned char lo_raw[];
     __shared__ int rows[LT_ROWS];
+    unsigned char* const a_smem = (unsigned char*)(((uintptr_t)lo_raw + 1023) & ~(uintptr_t)1023);   // [slice][part][box][128 rows][128]
+    unsigned char* const b_ring = a_smem + L::A_BYTES;       // [2][box][64 columns][128]
+    unsigned char* const y_ring = b_ring + 2 * L::B_BYTES;   // [warp][slot][box][32 rows][128]
+    uint64_t* const full = (uint64_t*)(y_ring + 4 * L::SLOTS * L::Y_BYTES);   // [2] B's turn is there (the first: u, too)
+    uint64_t* const acc_full = full + 2;                     // [2] its products are done: the accumulator, and the slot free
+    uint64_t* const acc_empty = acc_full + 2;                // [2] the accumulator has been read
+    uint64_t* const y_full = acc_empty + 2;                  // [warp][slot]
+    uint64_t* const settled = y_full + 4 * L::SLOTS;         // after a wait ran out
+    uint32_t* const tmem_slot = (uint32_t*)(settled + 1);
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, tile = blockIdx.y;
+    if (t == 0) {
+        for (int i = 0; i < 2; ++i) { tg_init(&full[i], 1); tg_init(&acc_full[i], 1); tg_init(&acc_empty[i], 4); }
+        for (int i = 0; i < 4 * L::SLOTS; ++i) tg_init(&y_full[i], 1);
+        tg_init(settled, 1);
+        tg_init_done();
+    }
+    __syncthreads();
     pdl_wait();
-    const int tile = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5, gr = lane >> 2, tig = lane & 3;
     if (tile >= info[0]) return;
     const int id = tiles[3 * tile], r0 = tiles[3 * tile + 1], n = tiles[3 * tile + 2];
-    const int rank = p.rank, width = p.columns.slices * rank;
-    // this block's columns: `pieces` pieces of one slice (in eights: of both)
-    int slice = 0, begin = 0, end = eights ? p.N : p.columns.ends[0], group = blockIdx.x;
+    // this block's columns: LO_TURNS turns of one slice (in eights: of both)
+    int slice = 0, begin = 0, end = EIGHTS ? p.N : p.columns.ends[0], group = blockIdx.x;
 #pragma unroll
     for (int i = 1; i < LR_MAX_SLICES; ++i) {
-        const int groups = (end - begin + pieces * LO_COLS - 1) / (pieces * LO_COLS);
+        const int groups = (end - begin + LO_TURNS * LO_COLS - 1) / (LO_TURNS * LO_COLS);
         if (slice == i - 1 && group >= groups) {
             group -= groups;
             slice = i;
@@ -605,168 +677,202 @@ low_rank_out_kernel(const LowRank p, const float* __restrict__ part, int splits,
             end = p.columns.ends[i];
         }
     }
-    const int col0 = begin + group * pieces * LO_COLS, col1 = min(col0 + pieces * LO_COLS, end);
-    if (t < n) rows[t] = perm[r0 + t];
-    __syncthreads();
-    const TY* const y = (const TY*)p.y;
+    const int col0 = begin + group * LO_TURNS * LO_COLS, col1 = min(col0 + LO_TURNS * LO_COLS, end);
+    const int turns = (col1 - col0 + LO_COLS - 1) / LO_COLS;
     TY* const out = (TY*)p.out;
-    constexpr int PER = 16 / (int)sizeof(TY);
+    constexpr int PER = 16 / (int)sizeof(TY);                // columns of a 16-byte piece
     if (id < 0) {                                            // no adapter: y as it is
-        if (p.out != p.y) {
-            const int vectors = (col1 - col0) / PER;
-            for (int e = t; e < n * vectors; e += LO_THREADS) {
-                const int r = rows[e / vectors], c = col0 + e % vectors * PER;
-                *(uint4*)(out + (size_t)r * p.out_stride + c) = *(const uint4*)(y + (size_t)r * p.y_stride + c);
-            }
+        if (p.out == p.y) return;
+        const TY* const y = (const TY*)p.y;
+        if (t < n) rows[t] = perm[r0 + t];
+        __syncthreads();
+        const int vectors = (col1 - col0) / PER;
+        for (int e = t; e < n * vectors; e += LO_THREADS) {
+            const int r = rows[e / vectors], c = col0 + e % vectors * PER;
+            *(uint4*)(out + (size_t)r * p.out_stride + c) = *(const uint4*)(y + (size_t)r * p.y_stride + c);
         }
         return;
     }
-    unsigned char* const u_hi = lo_smem;                     // [halves][128][pitch]
-    unsigned char* const u_lo = u_hi + halves * LT_ROWS * pitch;
-    unsigned char* const b_ring = u_lo + halves * LT_ROWS * pitch;      // [2][64][pitch]
-    const bf16* const b = (const bf16*)p.b + (size_t)id * p.N * rank;
-    const int n_pieces = (col1 - col0 + LO_COLS - 1) / LO_COLS;
-    // B's rows of a piece: a half's column 8 a + 2 q + c stands in row 8 q + 2 a + c, the order in which product q
-    // takes its columns
-    // Four threads a row. j: the row's column of its half; its own place in the ring and its way through B
-    const int f_half = t >> 7, f_j = (t >> 2) & 31, f_first = lo_column(eights, f_half, f_j);
-    unsigned char* const f_to = b_ring + (f_half * 32 + ((f_j >> 1) & 3) * 8 + (f_j >> 3) * 2 + (f_j & 1)) * pitch + (t & 3) * 16;
-    const bf16* const f_from = b + (size_t)(col0 + f_first) * rank + (t & 3) * 8;
-    auto fetch = [&](int piece) {
-        const bool there = col0 + piece * LO_COLS + f_first < col1;
-        const bf16* const from = there ? f_from + (size_t)piece * LO_COLS * rank : b;
-        unsigned char* const to = f_to + (piece & 1) * LO_COLS * pitch;
+    const int steps_all = (p.rank + 15) / 16;
+    auto fetch = [&](int turn) {                             // one thread
 #pragma unroll
-        for (int i = 0; i < (STEPS + 1) / 2; ++i)
-            if (((t & 3) + 4 * i) * 8 < rank) cp_async16(to + i * 64, from + (there ? i * 32 : 0), there);
-        cp_async_commit();
+        for (int x = 0; x < BOXES; ++x)
+            tg_load_2d(b_ring + (turn & 1) * L::B_BYTES + x * LO_B_BOX, &map_b, x * 64, id * p.N + col0 + turn * LO_COLS, &full[turn & 1]);
     };
-    for (int k = rank; k < STEPS * 16; k += 8)               // the steps beyond the rank: zeros (u's too, below)
-        for (int e = t; e < 2 * LO_COLS; e += LO_THREADS) *(uint4*)(b_ring + e * pitch + k * 2) = make_uint4(0, 0, 0, 0);
-    fetch(0);
-    {
-        // four threads a row, four neighbouring values each at a time
-        const float scale = p.scale[id];
-        for (int r = t >> 2; r < halves * LT_ROWS; r += LO_THREADS / 4) {
-            const int row = r & (LT_ROWS - 1), h = r / LT_ROWS;
-            const float* const from = part + (size_t)(r0 + min(row, n - 1)) * width + (slice + h) * rank + (t & 3) * 4;
-            float4 s[STEPS];
+    if (warp == 4) {
+        if (lane == 0) {
+            // the rows after the tile's come along: their sums are never stored
+            tg_expect(&full[0], L::A_BYTES + L::B_BYTES);
 #pragma unroll
-            for (int k = 0; k < STEPS; ++k)
-                s[k] = row < n && k * 16 + (t & 3) * 4 < rank ? *(const float4*)(from + k * 16) : make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int i = 1; i < splits; ++i) {
-                const float* const more = from + (size_t)i * p.T * width;
+            for (int i = 0; i < L::SLICES * L::PARTS * BOXES; ++i) {
+                const int x = i % BOXES, rest = i / BOXES % L::PARTS, h = i / BOXES / L::PARTS;
+                tg_load_2d(a_smem + i * LO_U_BOX, &map_u, ((slice + h) * 2 + rest) * steps_all * 16 + x * 64, r0, &full[0]);
+            }
+            fetch(0);
+            if (turns > 1) {
+                tg_expect(&full[1], L::B_BYTES);
+                fetch(1);
+            }
+        }
+        __syncwarp();
+        tg_alloc<2 * LO_COLS>(tmem_slot);
+        tg_before();
+        __syncthreads();
+        tg_after();
+        const uint32_t tmem = *tmem_slot;
+        if (lane == 0) {
+            const uint32_t idesc = tg_idesc(EIGHTS ? LO_COLS / 2 : LO_COLS);
+            uint32_t sent = min(turns, 2);
+            bool ok = true;
+            for (int i = 0; i < turns; ++i) {
+                const int s = i & 1;
+                ok = tg_wait(&full[s], (i >> 1) & 1, &low_rank_error_flag, 4);
+                if (ok) ok = tg_wait(&acc_empty[s], ((i >> 1) & 1) ^ 1, &low_rank_error_flag, 5);
+                if (!ok) break;
+                tg_after();
 #pragma unroll
-                for (int k = 0; k < STEPS; ++k)
-                    if (row < n && k * 16 + (t & 3) * 4 < rank) {
-                        const float4 q = *(const float4*)(more + k * 16);
-                        s[k].x += q.x; s[k].y += q.y; s[k].z += q.z; s[k].w += q.w;
+                for (int h = 0; h < L::SLICES; ++h) {
+                    const uint32_t d = tmem + s * LO_COLS + h * (LO_COLS / 2);
+                    bool first = true;
+#pragma unroll
+                    for (int x = 0; x < BOXES; ++x) {
+                        const unsigned char* const bx = b_ring + s * L::B_BYTES + x * LO_B_BOX + (EIGHTS ? h * 1024 : 0);
+                        const uint64_t db = lo_desc(bx, EIGHTS ? 2048 : 1024);
+                        const uint64_t da = tg_desc(a_smem + (h * L::PARTS * BOXES + x) * LO_U_BOX);
+                        const uint64_t dr = PAIRED ? da + 2 * steps_all : da + BOXES * (LO_U_BOX >> 4);
+                        const int steps = min(steps_all - 4 * x, 4);
+                        for (int k = 0; k < steps; ++k) {
+                            tg_mma(d, da + 2 * k, db + 2 * k, idesc, first ? 0u : 1u);
+                            tg_mma(d, dr + 2 * k, db + 2 * k, idesc, 1u);
+                            first = false;
+                        }
                     }
-            }
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k) {
-                s[k].x *= scale; s[k].y *= scale; s[k].z *= scale; s[k].w *= scale;
-                const uint32_t h0 = pack_bf16(s[k].x, s[k].y), h1 = pack_bf16(s[k].z, s[k].w);
-                const int at = r * pitch + k * 32 + (t & 3) * 8;
-                *(uint2*)(u_hi + at) = make_uint2(h0, h1);
-                *(uint2*)(u_lo + at) = make_uint2(
-                    pack_bf16(s[k].x - __uint_as_float(h0 << 16), s[k].y - __uint_as_float(h0 & 0xffff0000u)),
-                    pack_bf16(s[k].z - __uint_as_float(h1 << 16), s[k].w - __uint_as_float(h1 & 0xffff0000u)));
-            }
-        }
-    }
-    const int ra = warp * 16 + gr, rb = ra + 8;              // this thread's rows of the tile
-    constexpr int VEC = 8 / PER, APART = EIGHTS ? 8 : 32;    // 16-byte vectors of a thread's eight columns; columns between its halves
-    const int c0 = col0 + lo_column(eights, 0, 8 * tig);
-    const TY* ya = y + (size_t)rows[min(ra, n - 1)] * p.y_stride + c0;
-    const TY* yb = y + (size_t)rows[min(rb, n - 1)] * p.y_stride + c0;
-    TY* oa = out + (size_t)rows[min(ra, n - 1)] * p.out_stride + c0;
-    TY* ob = out + (size_t)rows[min(rb, n - 1)] * p.out_stride + c0;
-    const bool any = warp * 16 < n;                          // the same for the whole warp
-    uint4 next[2][2][VEC];                                   // [half][row]
-    auto read = [&](int piece) {                             // rows past the tile's read its last row, and store nothing
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            if (c0 + piece * LO_COLS + h * APART < col1)
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    next[h][0][i] = *(const uint4*)(ya + h * APART + i * PER);
-                    next[h][1][i] = *(const uint4*)(yb + h * APART + i * PER);
                 }
-        ya += LO_COLS;
-        yb += LO_COLS;
-    };
-    if (any) read(0);
-    constexpr int KEPT = KEEP ? halves : 1;
-    uint32_t fh[KEPT][STEPS][4], fl[KEPT][STEPS][4];         // u's part of the products
-    auto operands = [&](int h, int to) {
-        const unsigned char* const ua = u_hi + (h * LT_ROWS + ra) * pitch + tig * 8;
-        const unsigned char* const ul = ua + halves * LT_ROWS * pitch;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            const uint2 a = *(const uint2*)(ua + s * 32), c = *(const uint2*)(ua + 8 * pitch + s * 32);
-            const uint2 e = *(const uint2*)(ul + s * 32), f = *(const uint2*)(ul + 8 * pitch + s * 32);
-            fh[to][s][0] = a.x; fh[to][s][1] = c.x; fh[to][s][2] = a.y; fh[to][s][3] = c.y;
-            fl[to][s][0] = e.x; fl[to][s][1] = f.x; fl[to][s][2] = e.y; fl[to][s][3] = f.y;
-        }
-    };
-    for (int piece = 0; piece < n_pieces; ++piece) {
-        cp_async_wait<0>();
-        __syncthreads();                                     // this piece's B (and u) is there, the other buffer is read
-        if (piece + 1 < n_pieces) fetch(piece + 1);
-        if (!any) continue;
-        if (KEEP && piece == 0) {
-            operands(0, 0);
-            if (EIGHTS) operands(1, KEPT - 1);
-        }
-        uint4 cur[2][2][VEC];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) { cur[h][0][i] = next[h][0][i]; cur[h][1][i] = next[h][1][i]; }
-        if (piece + 1 < n_pieces) read(piece + 1);
-        const unsigned char* const from = b_ring + (piece & 1) * LO_COLS * pitch + gr * pitch + tig * 8;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (!KEEP) operands(h, 0);
-            constexpr int LAST = KEPT - 1;
-            const int f = KEEP && EIGHTS && h ? LAST : 0;
-            float acc[4][4] = {};
-#pragma unroll
-            for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const uint2 w = *(const uint2*)(from + (h * 32 + q * 8) * pitch + s * 32);
-                    mma_bf16(acc[q], fh[f][s], w.x, w.y);
-                    mma_bf16(acc[q], fl[f][s], w.x, w.y);
+                tg_commit(&acc_full[s]);
+                if (i + 2 < turns) {                         // the slot again, once its products are done
+                    ok = tg_wait(&acc_full[s], (i >> 1) & 1, &low_rank_error_flag, 6);
+                    if (!ok) break;
+                    tg_expect(&full[s], L::B_BYTES);
+                    fetch(i + 2);
+                    ++sent;
                 }
-            if (c0 + piece * LO_COLS + h * APART >= col1) continue;
+            }
+            if (!ok) {
+                tg_settle_copies(full, 2, sent, &low_rank_error_flag, 4);
+                tg_settle_products(settled, &low_rank_error_flag, 6);
+            }
+        }
+        __syncwarp();
+    } else {
+        const int q0 = warp * 32, mine = min(n - q0, 32);    // this warp's rows of the tile, none or fewer perhaps
+        const int row = perm[r0 + min(q0 + lane, n - 1)];
+        rows[q0 + lane] = row;
+        __syncwarp();
+        const int first = __shfl_sync(0xffffffffu, row, 0);
+        const bool together = __all_sync(0xffffffffu, lane >= mine || row == first + lane);
+        unsigned char* const ring = y_ring + warp * L::SLOTS * L::Y_BYTES;
+        uint64_t* const there = y_full + warp * L::SLOTS;
+        auto load = [&](int turn) {                          // the whole warp
+            const int s = turn % L::SLOTS, c = col0 + turn * LO_COLS;
+            if (lane == 0) tg_expect(&there[s], together ? L::Y_BYTES : (mine + 3) / 4 * 4 * 128 * L::Y_BOXES);
+            __syncwarp();
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                uint4 ya4 = cur[h][0][i], yb4 = cur[h][1][i];
-                if constexpr (sizeof(TY) == 2) {
-                    uint32_t* const wa = (uint32_t*)&ya4;
-                    uint32_t* const wb = (uint32_t*)&yb4;
+            for (int x = 0; x < L::Y_BOXES; ++x) {
+                unsigned char* const to = ring + s * L::Y_BYTES + x * 4096;
+                if (together) {
+                    if (lane == 0) tg_load_2d(to, &map_y, c + x * 32, first, &there[s]);
+                } else if (4 * lane < mine) {
+                    const int* const r = rows + q0 + 4 * lane;
+                    tg_gather4(to + lane * 512, &map_row, c + x * 32, r[0], r[1], r[2], r[3], &there[s]);
+                }
+            }
+        };
+        if (mine > 0)
+            for (int i = 0; i < min(turns, L::SLOTS); ++i) load(i);
+        tg_before();
+        __syncthreads();
+        tg_after();
+        const uint32_t sums = *tmem_slot + ((uint32_t)q0 << 16);
+        bool ok = true;
+        uint32_t sent = min(turns, L::SLOTS);
+        for (int turn = 0; turn < turns && ok; ++turn) {
+            const int s = turn & 1, slot = turn % L::SLOTS, c = col0 + turn * LO_COLS;
+            ok = __all_sync(0xffffffffu, tg_wait(&acc_full[s], (turn >> 1) & 1, &low_rank_error_flag, 7));
+            if (ok && mine > 0) ok = __all_sync(0xffffffffu, tg_wait(&there[slot], (turn / L::SLOTS) & 1, &low_rank_error_flag, 8));
+            if (!ok) break;
+            tg_after();
+            unsigned char* const at = ring + slot * L::Y_BYTES;
+            // a row of 128 bytes a lane, its 16-byte pieces swapped by the row's place among eight
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        wa[q] = pack_bf16(__uint_as_float(wa[q] << 16) + acc[q][0], __uint_as_float(wa[q] & 0xffff0000u) + acc[q][1]);
-                        wb[q] = pack_bf16(__uint_as_float(wb[q] << 16) + acc[q][2], __uint_as_float(wb[q] & 0xffff0000u) + acc[q][3]);
+            for (int v = 0; v < 2 && mine > 0; ++v) {        // 32 columns
+                uint32_t acc[32];
+                if constexpr (EIGHTS) {                      // 16 of each slice
+                    uint32_t a0[16], a1[16];
+                    tg_ld16(sums + s * LO_COLS + v * 16, a0);
+                    tg_ld16(sums + s * LO_COLS + LO_COLS / 2 + v * 16, a1);
+                    tg_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        acc[i / 8 * 16 + i % 8] = a0[i];
+                        acc[i / 8 * 16 + 8 + i % 8] = a1[i];
                     }
                 } else {
-                    float* const wa = (float*)&ya4;
-                    float* const wb = (float*)&yb4;
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        wa[2 * q] += acc[2 * i + q][0]; wa[2 * q + 1] += acc[2 * i + q][1];
-                        wb[2 * q] += acc[2 * i + q][2]; wb[2 * q + 1] += acc[2 * i + q][3];
-                    }
+                    tg_ld32(sums + s * LO_COLS + v * 32, acc);
+                    tg_wait_ld();
                 }
-                if (ra < n) *(uint4*)(oa + h * APART + i * PER) = ya4;
-                if (rb < n) *(uint4*)(ob + h * APART + i * PER) = yb4;
+                unsigned char* const line = at + lane * 128 + (L::Y_BOXES == 2 ? v * 4096 : 0);
+#pragma unroll
+                for (int i = 0; i < 32 / PER; ++i) {
+                    uint4* const piece = (uint4*)(line + (((i + (L::Y_BOXES == 1 ? v * 4 : 0)) ^ (lane & 7)) << 4));
+                    uint4 w = *piece;
+                    uint32_t* const e = (uint32_t*)&w;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if constexpr (sizeof(TY) == 2)
+                            e[k] = pack_bf16(__uint_as_float(e[k] << 16) + __uint_as_float(acc[i * 8 + 2 * k]),
+                                             __uint_as_float(e[k] & 0xffff0000u) + __uint_as_float(acc[i * 8 + 2 * k + 1]));
+                        else
+                            e[k] = __float_as_uint(__uint_as_float(e[k]) + __uint_as_float(acc[i * 4 + k]));
+                    }
+                    *piece = w;
+                }
+            }
+            tg_before();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tg_arrive(&acc_empty[s]);
+            if (mine <= 0) continue;
+            if (together && mine == 32 && c + LO_COLS <= col1) {
+                if (lane == 0)
+#pragma unroll
+                    for (int x = 0; x < L::Y_BOXES; ++x) lo_store_2d(&map_out, c + x * 32, first, at + x * 4096);
+            } else {
+#pragma unroll
+                for (int x = 0; x < L::Y_BOXES; ++x)
+                    for (int r = lane >> 3; r < mine; r += 4) {
+                        const int col = c + x * 32 + (lane & 7) * PER;
+                        if (col < col1)
+                            *(uint4*)(out + (size_t)rows[q0 + r] * p.out_stride + col) = *(const uint4*)(at + x * 4096 + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+                    }
+            }
+            // the slot of the turn before: its store has been read once only this turn's is under way (a block's last turn
+            // alone may be written otherwise, and nothing is loaded after it)
+            if (turn > 0 && turn - 1 + L::SLOTS < turns) {
+                asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(L::Y_BOXES) : "memory");
+                __syncwarp();
+                load(turn - 1 + L::SLOTS);
+                ++sent;
             }
         }
-        oa += LO_COLS;
-        ob += LO_COLS;
+        if (!ok && lane == 0 && mine > 0) tg_settle_copies(there, L::SLOTS, sent, &low_rank_error_flag, 8);
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
+    }
+    tg_before();
+    __syncthreads();
+    if (warp == 4) {
+        tg_after();
+        tg_free<2 * LO_COLS>(*tmem_slot);
     }
 }
 
@@ -876,26 +982,38 @@ template <typename T, typename TY> static int low_rank_few(const LowRank& p, int
 template <typename TY> static bool lr_tile_takes(const LowRank& p) {
     const int v = 16 / (int)sizeof(TY), width = p.columns.slices * p.rank;
     if (!lr_vectors<bf16>(p) || p.rank % 8 || p.rank > 128 || width > LT_MAX_WIDTH || p.adapters > LP_MAX_ADAPTERS ||
-        p.T > (1 << 24) || (long long)p.adapters * width > 0x7fffffff || p.y_stride % v || p.out_stride % v ||
+        p.T > (1 << 24) || (long long)p.adapters * width > 0x7fffffff || (long long)p.adapters * p.N > 0x7fffffff || p.y_stride % v || p.out_stride % v ||
         ((uintptr_t)p.y | (uintptr_t)p.out) & 15)
         return false;
-    if (p.columns.interleaved) return p.N % 64 == 0;
+    if (p.columns.interleaved) return p.N % 32 == 0;
     for (int i = 0; i < p.columns.slices; ++i)
         if (p.columns.ends[i] % 32) return false;
     return true;
 }
 
-// Parts of k: as many as fill the multiprocessors once with the tiles that there are at least, four blocks of
-// k at the least in each.
-static int lr_splits(const LowRank& p) {
-    const int tiles = (p.T + LT_ROWS - 1) / LT_ROWS, kbs = (p.K + LT_BK - 1) / LT_BK;
-    int s = (LT_FILL * tgo_multiprocessors() + tiles - 1) / tiles;
-    s = s < kbs / 4 ? s : kbs / 4;
-    return s > 1 ? s : 1;
+// How A's rows are fetched, the ring, and the parts of k (blocks of a cluster): the count that is cheapest by a small
+// model. The blocks run in rounds of as many as the multiprocessors hold; a block costs a unit a block of k and eight to
+// begin and end. The tiles that the rows make at least, and one, are counted with (how many more is the device's to know).
+static int lt_bytes(const LowRankTile& g) { return lt_ring(g) + 1024 + 256; }
+static LowRankTile lr_plan(const LowRank& p) {
+    LowRankTile g;
+    g.width = p.columns.slices * p.rank;
+    g.cuts = g.width > 256 ? 2 : 1;
+    g.cut = ((g.width + g.cuts - 1) / g.cuts + 15) / 16 * 16;
+    g.kbs = (p.K + LT_BK - 1) / LT_BK;
+    const int stage = LT_X_BYTES + g.cuts * g.cut * LT_BK * 2, most = 176 * 1024 / stage, tiles = (p.T + LT_ROWS - 1) / LT_ROWS + 1;
+    g.stages = most < 4 ? most : 4;
+    const int slots = tgo_multiprocessors() * (2 * lt_bytes(g) <= 226 * 1024 && g.cuts * g.cut <= 256 ? 2 : 1);
+    long long best = -1;
+    for (int s = 1; s <= 8 && (s == 1 || s * 4 <= g.kbs); s *= 2) {
+        const long long cost = ((long long)tiles * s + slots - 1) / slots * ((g.kbs + s - 1) / s + 8);
+        if (best < 0 || cost < best) { best = cost; g.splits = s; }
+    }
+    return g;
 }
 
-template <int COLS> static int low_rank_u(const LowRank& p, const LowRankTile& g, size_t bytes, const int* perm, const int* info, const int* tiles,
-                                          float* part, cudaStream_t stream) {
+template <int COLS> static int low_rank_u(const LowRank& p, const LowRankTile& g, const int* perm, const int* info, const int* tiles, bf16* u,
+                                          cudaStream_t stream) {
     static bool sized[64] = {};                              // per device
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
@@ -910,68 +1028,83 @@ template <int COLS> static int low_rank_u(const LowRank& p, const LowRankTile& g
     if (!tg_map(&row, p.x, p.T, p.K, p.x_stride, 1) || !tg_map(&some, p.x, p.T, p.K, p.x_stride, 32) ||
         !tg_map(&all, p.x, p.T, p.K, p.x_stride, LT_ROWS) || !tg_map(&a, p.a, (long long)p.adapters * g.width, p.K, p.K, g.cut))
         return TGO_E_BAD_ARG;
-    return tgo_launch_pdl(low_rank_u_kernel<COLS>, dim3(g.splits, (unsigned)lr_tiles(p, LT_ROWS)), dim3(LT_THREADS), bytes, stream, row, some, all, a,
-                          g, p.T, perm, info, tiles, part);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(g.splits, (unsigned)lr_tiles(p, LT_ROWS));
+    cfg.blockDim = dim3(LT_THREADS);
+    cfg.dynamicSmemBytes = (size_t)lt_bytes(g);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = g.splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = tgo_pdl_enabled() ? 2 : 1;
+    return (int)cudaLaunchKernelEx(&cfg, low_rank_u_kernel<COLS>, row, some, all, a, g, p.rank, p.scale, perm, info, tiles, u);
 }
 
-template <int STEPS, bool EIGHTS, typename TY> static int low_rank_out(const LowRank& p, const float* part, int splits, const int* perm, const int* info,
-                                                          const int* tiles, cudaStream_t stream) {
-    static bool sized[64] = {};
+template <int BOXES, bool PAIRED, bool EIGHTS, typename TY>
+static int low_rank_out(const LowRank& p, const bf16* u, const int* perm, const int* info, const int* tiles, cudaStream_t stream) {
+    static bool sized[64] = {};                              // per device
+    constexpr int bytes = LowRankOut<BOXES, PAIRED, EIGHTS, TY>::BYTES;
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return (int)err;
     if (dev < 0 || dev >= 64) return TGO_E_BAD_ARG;
-    const size_t bytes = (size_t)(2 * (EIGHTS ? 2 : 1) * LT_ROWS + 2 * LO_COLS) * lo_pitch(STEPS);
     if (!sized[dev]) {
-        err = cudaFuncSetAttribute(low_rank_out_kernel<STEPS, EIGHTS, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+        err = cudaFuncSetAttribute(low_rank_out_kernel<BOXES, PAIRED, EIGHTS, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
         if (err != cudaSuccess) return (int)err;
         sized[dev] = true;
     }
     int groups = 0, begin = 0;
     for (int i = 0; i < (EIGHTS ? 1 : p.columns.slices); ++i) {
         const int end = EIGHTS ? p.N : p.columns.ends[i];
-        groups += (end - begin + LO_PIECES * LO_COLS - 1) / (LO_PIECES * LO_COLS);
+        groups += (end - begin + LO_TURNS * LO_COLS - 1) / (LO_TURNS * LO_COLS);
         begin = end;
     }
-    return tgo_launch_pdl(low_rank_out_kernel<STEPS, EIGHTS, TY>, dim3(groups, (unsigned)lr_tiles(p, LT_ROWS)), dim3(LO_THREADS), bytes, stream, p, part, splits, perm,
-                          info, tiles);
+    const int width = 2 * ((p.rank + 15) / 16 * 16) * p.columns.slices;
+    auto map_of = [](CUtensorMap* map, const void* ptr, long long rows, long long cols, long long stride, int box_rows) {
+        return sizeof(TY) == 2 ? tg_map(map, ptr, rows, cols, stride, box_rows) : tg_map_f32(map, ptr, rows, cols, stride, box_rows);
+    };
+    CUtensorMap map_u, map_b, map_y, map_row, map_out;
+    if (!tg_map(&map_u, u, p.T, width, width, LT_ROWS) || !tg_map(&map_b, p.b, (long long)p.adapters * p.N, p.rank, p.rank, LO_COLS) ||
+        !map_of(&map_y, p.y, p.T, p.N, p.y_stride, 32) || !map_of(&map_row, p.y, p.T, p.N, p.y_stride, 1) ||
+        !map_of(&map_out, p.out, p.T, p.N, p.out_stride, 32))
+        return TGO_E_BAD_ARG;
+    return tgo_launch_pdl(low_rank_out_kernel<BOXES, PAIRED, EIGHTS, TY>, dim3(groups, (unsigned)lr_tiles(p, LT_ROWS)), dim3(LO_THREADS), bytes, stream,
+                          map_u, map_b, map_y, map_row, map_out, p, perm, info, tiles);
+}
+
+template <bool EIGHTS, typename TY>
+static int low_rank_out_of(const LowRank& p, const bf16* u, const int* perm, const int* info, const int* tiles, cudaStream_t stream) {
+    if (p.rank <= 32) return low_rank_out<1, true, EIGHTS, TY>(p, u, perm, info, tiles, stream);
+    if (p.rank <= 64) return low_rank_out<1, false, EIGHTS, TY>(p, u, perm, info, tiles, stream);
+    return low_rank_out<2, false, EIGHTS, TY>(p, u, perm, info, tiles, stream);
+}
+
+// 32-bit numbers of workspace: the plan, and u twice in bfloat16.
+static long long lr_tile_work(const LowRank& p) {
+    return (p.T + 1 + 3 * lr_tiles(p, LT_ROWS) + 3) / 4 * 4 + (long long)p.T * ((p.rank + 15) / 16 * 16) * p.columns.slices;
 }
 
 template <typename TY> static int low_rank_tiles(const LowRank& p, int* work, cudaStream_t stream) {
     int* const perm = work;
     int* const info = perm + p.T;
     int* const tiles = info + 1;
-    float* const part = (float*)(work + (p.T + 1 + 3 * lr_tiles(p, LT_ROWS) + 3) / 4 * 4);
+    bf16* const u = (bf16*)(work + (p.T + 1 + 3 * lr_tiles(p, LT_ROWS) + 3) / 4 * 4);
     int rc = tgo_launch_pdl(low_rank_plan_kernel, dim3(1), dim3(LP_THREADS), 0, stream, p.ids, p.T, p.adapters, LT_ROWS, perm, info, tiles);
     if (rc) return rc;
-    LowRankTile g;
-    g.width = p.columns.slices * p.rank;
-    g.cuts = g.width > 256 ? 2 : 1;
-    g.cut = ((g.width + g.cuts - 1) / g.cuts + 15) / 16 * 16;
-    g.kbs = (p.K + LT_BK - 1) / LT_BK;
-    g.splits = lr_splits(p);
-    const int stage = LT_X_BYTES + g.cuts * g.cut * LT_BK * 2, most = 176 * 1024 / stage, wanted = (g.kbs + g.splits - 1) / g.splits;
-    g.stages = most < 4 ? most : 4;
-    g.stages = g.stages < wanted ? g.stages : wanted;
-    const size_t bytes = (size_t)g.stages * stage + 4 * LT_STAGE_OUT + 1024 + 256;
+    const LowRankTile g = lr_plan(p);
     const int cols = g.cuts * g.cut;
-    if (cols <= 32) rc = low_rank_u<32>(p, g, bytes, perm, info, tiles, part, stream);
-    else if (cols <= 64) rc = low_rank_u<64>(p, g, bytes, perm, info, tiles, part, stream);
-    else if (cols <= 128) rc = low_rank_u<128>(p, g, bytes, perm, info, tiles, part, stream);
-    else if (cols <= 256) rc = low_rank_u<256>(p, g, bytes, perm, info, tiles, part, stream);
-    else rc = low_rank_u<512>(p, g, bytes, perm, info, tiles, part, stream);
+    if (cols <= 32) rc = low_rank_u<32>(p, g, perm, info, tiles, u, stream);
+    else if (cols <= 64) rc = low_rank_u<64>(p, g, perm, info, tiles, u, stream);
+    else if (cols <= 128) rc = low_rank_u<128>(p, g, perm, info, tiles, u, stream);
+    else if (cols <= 256) rc = low_rank_u<256>(p, g, perm, info, tiles, u, stream);
+    else rc = low_rank_u<512>(p, g, perm, info, tiles, u, stream);
     if (rc) return rc;
-    const int steps = (p.rank + 15) / 16;
-    if (p.columns.interleaved) {
-        if (steps == 1) return low_rank_out<1, true, TY>(p, part, g.splits, perm, info, tiles, stream);
-        if (steps == 2) return low_rank_out<2, true, TY>(p, part, g.splits, perm, info, tiles, stream);
-        if (steps <= 4) return low_rank_out<4, true, TY>(p, part, g.splits, perm, info, tiles, stream);
-        return low_rank_out<8, true, TY>(p, part, g.splits, perm, info, tiles, stream);
-    }
-    if (steps == 1) return low_rank_out<1, false, TY>(p, part, g.splits, perm, info, tiles, stream);
-    if (steps == 2) return low_rank_out<2, false, TY>(p, part, g.splits, perm, info, tiles, stream);
-    if (steps <= 4) return low_rank_out<4, false, TY>(p, part, g.splits, perm, info, tiles, stream);
-    return low_rank_out<8, false, TY>(p, part, g.splits, perm, info, tiles, stream);
+    return p.columns.interleaved ? low_rank_out_of<true, TY>(p, u, perm, info, tiles, stream)
+                                 : low_rank_out_of<false, TY>(p, u, perm, info, tiles, stream);
 }
 
 // Rows from which a call goes by tiles of 128.
@@ -993,7 +1126,7 @@ template <typename T, typename TY> static int low_rank_any(const LowRank& p, flo
 template <typename T, typename TY> static long long lr_work(const LowRank& p) {
     const int width = p.columns.slices * p.rank;
     if constexpr (sizeof(T) == 2)
-        if (p.T >= LR_TILE_ROWS && lr_tile_takes<TY>(p)) return p.T + 1 + 3 * lr_tiles(p, LT_ROWS) + 4 + (long long)lr_splits(p) * p.T * width;
+        if (p.T >= LR_TILE_ROWS && lr_tile_takes<TY>(p)) return lr_tile_work(p);
     if (lr_few_takes<T>(p)) return p.T > LR_SCAN_ROWS ? p.T + 1 + 3 * lr_tiles(p, LF_ROWS) : 0;
     return (long long)p.T * width;
 }
