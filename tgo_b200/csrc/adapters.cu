@@ -75,8 +75,12 @@ low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile,
             if (from + i * 32 < to) take(from + i * 32 + lane, held[i]);
         for (int base = from + LP_HELD * 32; base < to; base += 32) take(base + lane, slot_of(base + lane));
     };
+    // the lanes with a lane's adapter; a request's rows lie together: mostly all of them
+    auto alike = [&](int slot) {
+        return __all_sync(0xffffffffu, slot == __shfl_sync(0xffffffffu, slot, 0)) ? 0xffffffffu : __match_any_sync(0xffffffffu, slot);
+    };
     each([&](int, int slot) {
-        const unsigned same = __match_any_sync(0xffffffffu, slot);
+        const unsigned same = alike(slot);
         if (slot >= 0 && lane == __ffs(same) - 1) {
             if (ordered) mine[slot] += __popc(same);
             else atomicAdd(&mine[slot], __popc(same));
@@ -84,25 +88,31 @@ low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile,
         __syncwarp();
     });
     __syncthreads();
+    // a warp's rows of an adapter come after the earlier warps'
+    if (ordered) {
+        for (int i = warp; i < slots; i += LP_WARPS) {
+            const int c = counts[lane * slots + i];
+            int n = c;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int a = __shfl_up_sync(0xffffffffu, n, o);
+                if (lane >= o) n += a;
+            }
+            counts[lane * slots + i] = n - c;
+            if (lane == 31) rows_before[i] = n;
+        }
+        __syncthreads();
+    }
     // exclusive sums of rows and of tiles over the adapters, a thread a run of neighbours
     const int per = (slots + LP_THREADS - 1) / LP_THREADS, first = min(t * per, slots), last = min(first + per, slots);
     int my_rows = 0, my_tiles = 0;
     for (int i = first; i < last; ++i) {
-        int n = 0;
-        if (ordered) {
-#pragma unroll 8
-            for (int w = 0; w < LP_WARPS; ++w) {             // a warp's rows of an adapter come after the earlier warps'
-                const int c = counts[w * slots + i];
-                counts[w * slots + i] = n;
-                n += c;
-            }
-        } else {
-            n = counts[i];
+        if (!ordered) {
+            rows_before[i] = counts[i];
             counts[i] = 0;
         }
-        rows_before[i] = n;
-        my_rows += n;
-        my_tiles += (n + tile - 1) / tile;
+        my_rows += rows_before[i];
+        my_tiles += (rows_before[i] + tile - 1) / tile;
     }
     int sum_rows = my_rows, sum_tiles = my_tiles;
 #pragma unroll
@@ -141,7 +151,7 @@ low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile,
         tiles[3 * q + 2] = min(tile, end - begin);
     }
     each([&](int r, int slot) {
-        const unsigned same = __match_any_sync(0xffffffffu, slot);
+        const unsigned same = alike(slot);
         const int leader = __ffs(same) - 1;
         int place = 0;
         if (slot >= 0 && lane == leader) {
@@ -417,6 +427,9 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
 #define LT_ROWS 128
 #define LT_BK 64
 #define LT_X_BYTES (LT_ROWS * LT_BK * 2)
+#ifndef LT_STAGES
+#define LT_STAGES 4               // of the ring, at most 8
+#endif
 #define LT_PASS 256               // columns of u that the blocks of a cluster exchange at a time
 #define LT_THREADS 224
 #define LT_MAX_WIDTH 512          // slices x rank: the columns of tensor memory
@@ -454,9 +467,8 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
         tg_init_done();
     }
     pdl_wait();
-    if (tile >= info[0]) return;
     const int id = tiles[3 * tile], r0 = tiles[3 * tile + 1], rows = tiles[3 * tile + 2];
-    if (id < 0) return;                                      // the same for the whole block
+    if (tile >= info[0] || id < 0) return;                   // the same for the whole cluster
     if (warp == 1) tg_alloc<COLS>(tmem_slot);
     tg_before();
     __syncthreads();
@@ -484,49 +496,63 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
         // more than three boxes of 32 rows come as one of 128: the rows after the tile's give sums that nobody stores
         const bool whole = together && rows > 96;
         const int groups = !together ? (rows + 3) / 4 : whole ? 1 : (rows + 31) / 32, group_bytes = !together ? 512 : whole ? LT_X_BYTES : 4096;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-            const int s = it % g.stages;
-            ok = __all_sync(0xffffffffu, tg_wait(&empty[s], ((it / g.stages) & 1) ^ 1, &low_rank_error_flag, 1));
-            if (!ok) break;
-            unsigned char* const st = base + (size_t)s * stage_bytes;
-            if (warp == 6) {
-                if (lane == 0) {
-                    tg_expect(&full[s], (uint32_t)(g.cuts * g.cut * LT_BK * 2));
-                    for (int c = 0; c < g.cuts; ++c)
-                        tg_load_2d(st + LT_X_BYTES + c * g.cut * LT_BK * 2, &map_a, kb * LT_BK, id * g.width + c * g.cut, &full[s]);
+        int s = 0;
+        uint32_t phase = 1;
+        if (warp == 6 || whole) {                            // one thread asks for everything
+            if (tg_elect()) {
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    ok = tg_wait(&empty[s], phase, &low_rank_error_flag, 1);
+                    if (!ok) break;
+                    unsigned char* const st = base + (size_t)s * stage_bytes;
+                    if (warp == 6) {
+                        tg_expect(&full[s], (uint32_t)(g.cuts * g.cut * LT_BK * 2));
+                        tg_load_2d(st + LT_X_BYTES, &map_a, kb * LT_BK, id * g.width, &full[s]);
+                        if (g.cuts == 2) tg_load_2d(st + LT_X_BYTES + g.cut * LT_BK * 2, &map_a, kb * LT_BK, id * g.width + g.cut, &full[s]);
+                    } else {
+                        tg_expect(&full[s], LT_X_BYTES);
+                        tg_load_2d(st, &map_all, kb * LT_BK, first, &full[s]);
+                    }
+                    if (++s == g.stages) { s = 0; phase ^= 1; }
                 }
-                __syncwarp();
-                continue;
+                if (!ok) tg_settle_copies(full, g.stages, it, &low_rank_error_flag, 1);
             }
-            if (lane == 0) tg_expect(&full[s], (uint32_t)(groups * group_bytes));
-            __syncwarp();
-            if (whole) {
-                if (lane == 0) tg_load_2d(st, &map_all, kb * LT_BK, first, &full[s]);
-            } else if (together) {
-                if (lane < groups) tg_load_2d(st + lane * 4096, &map_some, kb * LT_BK, first + 32 * lane, &full[s]);
-            } else if (lane < groups) {
-                tg_gather4(st + lane * 512, &map_row, kb * LT_BK, src[0], src[1], src[2], src[3], &full[s]);
-            }
-        }
-        if (!ok) tg_settle_copies(full, g.stages, it, &low_rank_error_flag, 1);
-    } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = tg_idesc(g.cut);
-            uint32_t it = 0;
-            bool ok = true;
+        } else {
             for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const int s = it % g.stages;
-                ok = tg_wait(&full[s], (it / g.stages) & 1, &low_rank_error_flag, 2);
+                ok = __all_sync(0xffffffffu, tg_wait(&empty[s], phase, &low_rank_error_flag, 1));
+                if (!ok) break;
+                unsigned char* const st = base + (size_t)s * stage_bytes;
+                if (lane == 0) tg_expect(&full[s], (uint32_t)(groups * group_bytes));
+                __syncwarp();
+                if (together) {
+                    if (lane < groups) tg_load_2d(st + lane * 4096, &map_some, kb * LT_BK, first + 32 * lane, &full[s]);
+                } else if (lane < groups) {
+                    tg_gather4(st + lane * 512, &map_row, kb * LT_BK, src[0], src[1], src[2], src[3], &full[s]);
+                }
+                if (++s == g.stages) { s = 0; phase ^= 1; }
+            }
+            if (!ok) tg_settle_copies(full, g.stages, it, &low_rank_error_flag, 1);
+        }
+    } else if (warp == 1) {
+        if (tg_elect()) {
+            const uint32_t idesc = tg_idesc(g.cut);
+            int s = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                ok = tg_wait(&full[s], phase, &low_rank_error_flag, 2);
                 if (!ok) break;
                 tg_after();
                 unsigned char* const st = base + (size_t)s * stage_bytes;
-                const uint64_t dx = tg_desc(st);
-                for (int c = 0; c < g.cuts; ++c) {
-                    const uint64_t da = tg_desc(st + LT_X_BYTES + c * g.cut * LT_BK * 2);
+                const uint64_t dx = tg_desc(st), da = tg_desc(st + LT_X_BYTES);
 #pragma unroll
-                    for (int k = 0; k < LT_BK / 16; ++k) tg_mma(tmem + c * g.cut, dx + 2 * k, da + 2 * k, idesc, (it > 0 || k > 0) ? 1u : 0u);
+                for (int k = 0; k < LT_BK / 16; ++k) tg_mma(tmem, dx + 2 * k, da + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+                if (g.cuts == 2) {
+                    const uint64_t db = da + (uint64_t)(g.cut * LT_BK * 2 >> 4);
+#pragma unroll
+                    for (int k = 0; k < LT_BK / 16; ++k) tg_mma(tmem + g.cut, dx + 2 * k, db + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
                 }
                 tg_commit(&empty[s]);
+                if (++s == g.stages) { s = 0; phase ^= 1; }
             }
             if (ok) tg_commit(done);
             else tg_settle_products(settled, &low_rank_error_flag, 2);
@@ -538,24 +564,29 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
     tg_before();
     __syncthreads();
     tg_after();
-    // The ring is free: each block of the cluster lays its sums out there, LT_PASS columns a pass (a row's 16-byte pieces
-    // swapped by its place among eight, so that neither side meets a bank twice), and sums an equal share of the rows over
-    // all of them, in the blocks' order. Rank by rank the values are rounded to whole sixteens with zeros.
+    // The rings are free: each block of the cluster has an equal share of the rows, and is handed all blocks' sums of
+    // those, LT_PASS columns a pass ([block][32 columns][row of the share], a row's 16-byte pieces swapped by its place
+    // among eight). It adds them in the blocks' order. Rank by rank the values are filled up to whole sixteens with zeros.
     const float by = scale[id];
     const int padded = (rank + 15) / 16 * 16, slices = g.width / rank, quads = padded / 4;
-    const int share = LT_ROWS / g.splits;
+    const int share = LT_ROWS / g.splits, blocks = (min(g.width, LT_PASS) + 31) / 32;
     for (int c0 = 0; c0 < g.width; c0 += LT_PASS) {
         const int c1 = min(c0 + LT_PASS, g.width);
+        lf_cluster_arrive();
+        lf_cluster_wait();
         if (warp >= 2 && warp < 6 && handed) {
             const int quarter = warp & 3;                    // tensor-memory lanes this warp may read
-            const int row = quarter * 32 + lane;
-            for (int c = c0; quarter * 32 < rows && c < c1; c += 32) {
+            const int row = quarter * 32 + lane, in = row % share;
+            uint32_t to;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(tg_smem(base) + (uint32_t)(split * blocks * share * 128 + in * 128)), "r"(row / share));
+            for (int c = c0; quarter * 32 < rows && c < c1; c += 32, to += share * 128) {
                 uint32_t a[32];
                 tg_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + c, a);
                 tg_wait_ld();
-                unsigned char* const to = base + (c - c0) * (LT_ROWS * 4) + row * 128;
 #pragma unroll
-                for (int q = 0; q < 8; ++q) *(uint4*)(to + ((q ^ (row & 7)) << 4)) = make_uint4(a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]);
+                for (int q = 0; q < 8; ++q)
+                    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + ((q ^ (in & 7)) << 4)), "r"(a[4 * q]), "r"(a[4 * q + 1]),
+                                 "r"(a[4 * q + 2]), "r"(a[4 * q + 3]) : "memory");
             }
         }
         lf_cluster_arrive();
@@ -566,20 +597,20 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
             const int s = s0 + e / quads, k = e % quads * 4, c = s * rank + k;
             // the zeros behind a slice are written with its last value
             if (k < rank ? c < c0 || c >= c1 : (s + 1) * rank <= c0 || (s + 1) * rank > c1) continue;
-            const unsigned char* const from = base + (c - c0) / 32 * (32 * LT_ROWS * 4);
+            const unsigned char* const from = base + (c - c0) / 32 * (share * 128);
             const int piece = (c - c0) % 32 / 4;
-            bf16* const to = u + ((size_t)r0 * slices + s) * 2 * padded + k;
-#pragma unroll 2
-            for (int row = split * share + warp; row < min((split + 1) * share, rows); row += LT_THREADS / 32) {
+            bf16* const to = u + ((size_t)(r0 + split * share) * slices + s) * 2 * padded + k;
+#pragma unroll 4
+            for (int row = warp; row < min(share, rows - split * share); row += LT_THREADS / 32) {
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (k < rank) {
-                    const float* const at = (const float*)(from + row * 128 + ((piece ^ (row & 7)) << 4));
-                    if (g.splits == 1) v = *(const float4*)at;
-                    else
-                        for (int i = 0; i < g.splits; ++i) {
-                            const float4 q = lf_peer(at, i);
-                            v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
-                        }
+                    const unsigned char* at = from + row * 128 + ((piece ^ (row & 7)) << 4);
+                    v = *(const float4*)at;
+                    for (int i = 1; i < g.splits; ++i) {
+                        at += blocks * share * 128;
+                        const float4 q = *(const float4*)at;
+                        v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+                    }
                     v.x *= by; v.y *= by; v.z *= by; v.w *= by;
                 }
                 const uint32_t h0 = pack_bf16(v.x, v.y), h1 = pack_bf16(v.z, v.w);
@@ -590,8 +621,6 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
                     pack_bf16(v.z - __uint_as_float(h1 << 16), v.w - __uint_as_float(h1 & 0xffff0000u)));
             }
         }
-        lf_cluster_arrive();
-        lf_cluster_wait();                                   // nobody reads this block's sums any more
     }
     tg_before();
     __syncthreads();
@@ -604,22 +633,22 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
 // 64 columns a turn. In eights the rows of B that a turn brings, eight of slice 0 and eight of slice 1 in turn,
 // are two operands of 32 rows whose groups of eight lie twice as far apart: nothing is moved.
 //
-// y and out go through shared memory, asynchronously: each of four warps has 32 rows (the ones whose sums it can read
-// from tensor memory, a lane a row) and a ring of its own of 32 x 64 tiles; it adds the sums where y lies and has the
-// tile stored from there. Rows that lie together are one box either way; others come four at a time and are written by
+// y and out go through shared memory, asynchronously: each of eight warps has 32 rows (the ones whose sums it can read
+// from tensor memory, a lane a row) of every other turn and a ring of its own of 32 x 64 tiles; it adds the sums where
+// y lies and has the tile stored from there. Rows that lie together are one box either way; others come four at a time and are written by
 // the warp, as are part tiles. (Reading y into registers two steps ahead and writing from them, through a transposing
 // buffer, took 68 us where this takes XXX: 8192 rows of 6144 columns.)
 #define LO_COLS 64
 #ifndef LO_TURNS
 #define LO_TURNS 8                // of a block
 #endif
-#define LO_THREADS 160
+#define LO_HANDS 8                // warps that hand on; the one after them asks for copies and products
+#define LO_THREADS (LO_HANDS * 32 + 32)
 #define LO_U_BOX (LT_ROWS * 128)  // bytes of 64 values of k: of 128 rows of u,
 #define LO_B_BOX (LO_COLS * 128)  // of a turn's rows of B
 
 __device__ __forceinline__ void lo_store_2d(const CUtensorMap* map, int x, int y, const void* src) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(tg_smem(src)), "r"(x), "r"(y) : "memory");
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 // Operand tile as tg_desc, the groups of eight rows `apart` bytes from each other.
 __device__ __forceinline__ uint64_t lo_desc(const void* tile, uint32_t apart) {
@@ -631,9 +660,9 @@ template <int BOXES, bool PAIRED, bool EIGHTS, typename TY> struct LowRankOut {
     static constexpr int SLICES = EIGHTS ? 2 : 1, PARTS = PAIRED ? 1 : 2;
     static constexpr int A_BYTES = SLICES * PARTS * BOXES * LO_U_BOX, B_BYTES = BOXES * LO_B_BOX;
     static constexpr int Y_BOXES = (int)sizeof(TY) / 2, Y_BYTES = Y_BOXES * 32 * 128;     // a warp's tile: boxes of 128 bytes a row
-    static constexpr int SLOTS = Y_BOXES == 1 ? 3 : 2;
-    static constexpr int BYTES = A_BYTES + 2 * B_BYTES + 4 * SLOTS * Y_BYTES + 1024 + 512;
-    static_assert(BYTES + LT_ROWS * 4 <= 227 * 1024, "shared memory of a block");
+    static constexpr int SLOTS = A_BYTES + 2 * B_BYTES + LO_HANDS * 2 * Y_BYTES <= 224 * 1024 ? 2 : 1;
+    static constexpr int BYTES = A_BYTES + 2 * B_BYTES + LO_HANDS * SLOTS * Y_BYTES + 512 + LT_ROWS * 4;
+    static_assert(BYTES <= 227 * 1024, "shared memory of a block");
 };
 
 template <int BOXES, bool PAIRED, bool EIGHTS, typename TY>
@@ -643,28 +672,28 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
                     const __grid_constant__ CUtensorMap map_out, const LowRank p, const int* __restrict__ perm,
                     const int* __restrict__ info, const int* __restrict__ tiles) {
     typedef LowRankOut<BOXES, PAIRED, EIGHTS, TY> L;
-    extern __shared__ unsigned char lo_raw[];
-    __shared__ int rows[LT_ROWS];
-    unsigned char* const a_smem = (unsigned char*)(((uintptr_t)lo_raw + 1023) & ~(uintptr_t)1023);   // [slice][part][box][128 rows][128]
+    extern __shared__ __align__(1024) unsigned char lo_raw[];
+    unsigned char* const a_smem = lo_raw;                    // [slice][part][box][128 rows][128]
     unsigned char* const b_ring = a_smem + L::A_BYTES;       // [2][box][64 columns][128]
     unsigned char* const y_ring = b_ring + 2 * L::B_BYTES;   // [warp][slot][box][32 rows][128]
-    uint64_t* const full = (uint64_t*)(y_ring + 4 * L::SLOTS * L::Y_BYTES);   // [2] B's turn is there (the first: u, too)
+    int* const rows = (int*)(y_ring + LO_HANDS * L::SLOTS * L::Y_BYTES);
+    uint64_t* const full = (uint64_t*)(rows + LT_ROWS);      // [2] B's turn is there (the first: u, too)
     uint64_t* const acc_full = full + 2;                     // [2] its products are done: the accumulator, and the slot free
     uint64_t* const acc_empty = acc_full + 2;                // [2] the accumulator has been read
     uint64_t* const y_full = acc_empty + 2;                  // [warp][slot]
-    uint64_t* const settled = y_full + 4 * L::SLOTS;         // after a wait ran out
+    uint64_t* const settled = y_full + LO_HANDS * L::SLOTS;         // after a wait ran out
     uint32_t* const tmem_slot = (uint32_t*)(settled + 1);
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, tile = blockIdx.y;
     if (t == 0) {
         for (int i = 0; i < 2; ++i) { tg_init(&full[i], 1); tg_init(&acc_full[i], 1); tg_init(&acc_empty[i], 4); }
-        for (int i = 0; i < 4 * L::SLOTS; ++i) tg_init(&y_full[i], 1);
+        for (int i = 0; i < LO_HANDS * L::SLOTS; ++i) tg_init(&y_full[i], 1);
         tg_init(settled, 1);
         tg_init_done();
     }
     __syncthreads();
     pdl_wait();
-    if (tile >= info[0]) return;
     const int id = tiles[3 * tile], r0 = tiles[3 * tile + 1], n = tiles[3 * tile + 2];
+    if (tile >= info[0]) return;                             // what was read of it is nothing
     // this block's columns: LO_TURNS turns of one slice (in eights: of both)
     int slice = 0, begin = 0, end = EIGHTS ? p.N : p.columns.ends[0], group = blockIdx.x;
 #pragma unroll
@@ -699,7 +728,7 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
         for (int x = 0; x < BOXES; ++x)
             tg_load_2d(b_ring + (turn & 1) * L::B_BYTES + x * LO_B_BOX, &map_b, x * 64, id * p.N + col0 + turn * LO_COLS, &full[turn & 1]);
     };
-    if (warp == 4) {
+    if (warp == LO_HANDS) {
         if (lane == 0) {
             // the rows after the tile's come along: their sums are never stored
             tg_expect(&full[0], L::A_BYTES + L::B_BYTES);
@@ -720,7 +749,7 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
         __syncthreads();
         tg_after();
         const uint32_t tmem = *tmem_slot;
-        if (lane == 0) {
+        if (tg_elect()) {
             const uint32_t idesc = tg_idesc(EIGHTS ? LO_COLS / 2 : LO_COLS);
             uint32_t sent = min(turns, 2);
             bool ok = true;
@@ -764,16 +793,19 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
         }
         __syncwarp();
     } else {
-        const int q0 = warp * 32, mine = min(n - q0, 32);    // this warp's rows of the tile, none or fewer perhaps
+        const int q0 = (warp & 3) * 32, mine = min(n - q0, 32), set = warp >> 2;   // its rows of the tile, none or fewer
+                                                                                   // perhaps; its turns are set, set + 2, ...
         const int row = perm[r0 + min(q0 + lane, n - 1)];
-        rows[q0 + lane] = row;
-        __syncwarp();
-        const int first = __shfl_sync(0xffffffffu, row, 0);
+        if (set == 0) rows[q0 + lane] = row;
+        const int first = __shfl_sync(0xffffffffu, row, 0), turns_mine = (turns - set + 1) / 2;
         const bool together = __all_sync(0xffffffffu, lane >= mine || row == first + lane);
+        int gather[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) gather[i] = __shfl_sync(0xffffffffu, row, (4 * lane + i) & 31);
         unsigned char* const ring = y_ring + warp * L::SLOTS * L::Y_BYTES;
         uint64_t* const there = y_full + warp * L::SLOTS;
-        auto load = [&](int turn) {                          // the whole warp
-            const int s = turn % L::SLOTS, c = col0 + turn * LO_COLS;
+        auto load = [&](int i) {                             // of this warp's turns; the whole warp
+            const int s = i % L::SLOTS, c = col0 + (2 * i + set) * LO_COLS;
             if (lane == 0) tg_expect(&there[s], together ? L::Y_BYTES : (mine + 3) / 4 * 4 * 128 * L::Y_BOXES);
             __syncwarp();
 #pragma unroll
@@ -782,23 +814,22 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
                 if (together) {
                     if (lane == 0) tg_load_2d(to, &map_y, c + x * 32, first, &there[s]);
                 } else if (4 * lane < mine) {
-                    const int* const r = rows + q0 + 4 * lane;
-                    tg_gather4(to + lane * 512, &map_row, c + x * 32, r[0], r[1], r[2], r[3], &there[s]);
+                    tg_gather4(to + lane * 512, &map_row, c + x * 32, gather[0], gather[1], gather[2], gather[3], &there[s]);
                 }
             }
         };
+        uint32_t sent = 0;
         if (mine > 0)
-            for (int i = 0; i < min(turns, L::SLOTS); ++i) load(i);
+            for (; sent < min(turns_mine, L::SLOTS); ++sent) load(sent);
         tg_before();
         __syncthreads();
         tg_after();
-        const uint32_t sums = *tmem_slot + ((uint32_t)q0 << 16);
+        const uint32_t sums = *tmem_slot + ((uint32_t)q0 << 16) + set * LO_COLS;
         bool ok = true;
-        uint32_t sent = min(turns, L::SLOTS);
-        for (int turn = 0; turn < turns && ok; ++turn) {
-            const int s = turn & 1, slot = turn % L::SLOTS, c = col0 + turn * LO_COLS;
-            ok = __all_sync(0xffffffffu, tg_wait(&acc_full[s], (turn >> 1) & 1, &low_rank_error_flag, 7));
-            if (ok && mine > 0) ok = __all_sync(0xffffffffu, tg_wait(&there[slot], (turn / L::SLOTS) & 1, &low_rank_error_flag, 8));
+        for (int i = 0; i < turns_mine && ok; ++i) {
+            const int slot = i % L::SLOTS, c = col0 + (2 * i + set) * LO_COLS;
+            ok = __all_sync(0xffffffffu, tg_wait(&acc_full[set], i & 1, &low_rank_error_flag, 7));
+            if (ok && mine > 0) ok = __all_sync(0xffffffffu, tg_wait(&there[slot], (i / L::SLOTS) & 1, &low_rank_error_flag, 8));
             if (!ok) break;
             tg_after();
             unsigned char* const at = ring + slot * L::Y_BYTES;
@@ -808,31 +839,31 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
                 uint32_t acc[32];
                 if constexpr (EIGHTS) {                      // 16 of each slice
                     uint32_t a0[16], a1[16];
-                    tg_ld16(sums + s * LO_COLS + v * 16, a0);
-                    tg_ld16(sums + s * LO_COLS + LO_COLS / 2 + v * 16, a1);
+                    tg_ld16(sums + v * 16, a0);
+                    tg_ld16(sums + LO_COLS / 2 + v * 16, a1);
                     tg_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        acc[i / 8 * 16 + i % 8] = a0[i];
-                        acc[i / 8 * 16 + 8 + i % 8] = a1[i];
+                    for (int j = 0; j < 16; ++j) {
+                        acc[j / 8 * 16 + j % 8] = a0[j];
+                        acc[j / 8 * 16 + 8 + j % 8] = a1[j];
                     }
                 } else {
-                    tg_ld32(sums + s * LO_COLS + v * 32, acc);
+                    tg_ld32(sums + v * 32, acc);
                     tg_wait_ld();
                 }
                 unsigned char* const line = at + lane * 128 + (L::Y_BOXES == 2 ? v * 4096 : 0);
 #pragma unroll
-                for (int i = 0; i < 32 / PER; ++i) {
-                    uint4* const piece = (uint4*)(line + (((i + (L::Y_BOXES == 1 ? v * 4 : 0)) ^ (lane & 7)) << 4));
+                for (int j = 0; j < 32 / PER; ++j) {
+                    uint4* const piece = (uint4*)(line + (((j + (L::Y_BOXES == 1 ? v * 4 : 0)) ^ (lane & 7)) << 4));
                     uint4 w = *piece;
                     uint32_t* const e = (uint32_t*)&w;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         if constexpr (sizeof(TY) == 2)
-                            e[k] = pack_bf16(__uint_as_float(e[k] << 16) + __uint_as_float(acc[i * 8 + 2 * k]),
-                                             __uint_as_float(e[k] & 0xffff0000u) + __uint_as_float(acc[i * 8 + 2 * k + 1]));
+                            e[k] = pack_bf16(__uint_as_float(e[k] << 16) + __uint_as_float(acc[j * 8 + 2 * k]),
+                                             __uint_as_float(e[k] & 0xffff0000u) + __uint_as_float(acc[j * 8 + 2 * k + 1]));
                         else
-                            e[k] = __float_as_uint(__uint_as_float(e[k]) + __uint_as_float(acc[i * 4 + k]));
+                            e[k] = __float_as_uint(__uint_as_float(e[k]) + __uint_as_float(acc[j * 4 + k]));
                     }
                     *piece = w;
                 }
@@ -840,12 +871,14 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
             tg_before();
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) tg_arrive(&acc_empty[s]);
+            if (lane == 0) tg_arrive(&acc_empty[set]);
             if (mine <= 0) continue;
             if (together && mine == 32 && c + LO_COLS <= col1) {
-                if (lane == 0)
+                if (lane == 0) {
 #pragma unroll
                     for (int x = 0; x < L::Y_BOXES; ++x) lo_store_2d(&map_out, c + x * 32, first, at + x * 4096);
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
             } else {
 #pragma unroll
                 for (int x = 0; x < L::Y_BOXES; ++x)
@@ -855,13 +888,15 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
                             *(uint4*)(out + (size_t)rows[q0 + r] * p.out_stride + col) = *(const uint4*)(at + x * 4096 + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
                     }
             }
-            // the slot of the turn before: its store has been read once only this turn's is under way (a block's last turn
-            // alone may be written otherwise, and nothing is loaded after it)
-            if (turn > 0 && turn - 1 + L::SLOTS < turns) {
-                asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(L::Y_BOXES) : "memory");
-                __syncwarp();
-                load(turn - 1 + L::SLOTS);
-                ++sent;
+            // The next load goes where the turn before lay (with one slot: this turn), once its store has been read: this
+            // turn's may still be. (A block's last turn alone may be written otherwise, and nothing is loaded after it.)
+            if (L::SLOTS == 1 || i > 0) {
+                if (sent < turns_mine) {
+                    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(L::SLOTS - 1) : "memory");
+                    __syncwarp();
+                    load(sent);
+                    ++sent;
+                }
             }
         }
         if (!ok && lane == 0 && mine > 0) tg_settle_copies(there, L::SLOTS, sent, &low_rank_error_flag, 8);
@@ -870,7 +905,7 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
     }
     tg_before();
     __syncthreads();
-    if (warp == 4) {
+    if (warp == LO_HANDS) {
         tg_after();
         tg_free<2 * LO_COLS>(*tmem_slot);
     }
@@ -1002,7 +1037,7 @@ static LowRankTile lr_plan(const LowRank& p) {
     g.cut = ((g.width + g.cuts - 1) / g.cuts + 15) / 16 * 16;
     g.kbs = (p.K + LT_BK - 1) / LT_BK;
     const int stage = LT_X_BYTES + g.cuts * g.cut * LT_BK * 2, most = 176 * 1024 / stage, tiles = (p.T + LT_ROWS - 1) / LT_ROWS + 1;
-    g.stages = most < 4 ? most : 4;
+    g.stages = most < LT_STAGES ? most : LT_STAGES;
     const int slots = tgo_multiprocessors() * (2 * lt_bytes(g) <= 226 * 1024 && g.cuts * g.cut <= 256 ? 2 : 1);
     long long best = -1;
     for (int s = 1; s <= 8 && (s == 1 || s * 4 <= g.kbs); s *= 2) {
