@@ -79,7 +79,18 @@ low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile,
     auto alike = [&](int slot) {
         return __all_sync(0xffffffffu, slot == __shfl_sync(0xffffffffu, slot, 0)) ? 0xffffffffu : __match_any_sync(0xffffffffu, slot);
     };
-    each([&](int, int slot) {
+    // a run of one adapter alone needs no looking at its parts
+    const int lead = __shfl_sync(0xffffffffu, held[0], 0);
+    bool one = run <= LP_HELD * 32 && from < to;
+#pragma unroll
+    for (int i = 0; i < LP_HELD; ++i) one = one && (held[i] == lead || held[i] < 0);
+    one = __all_sync(0xffffffffu, one);
+    if (one) {
+        if (lane == 0) {
+            if (ordered) mine[lead] = to - from;
+            else atomicAdd(&mine[lead], to - from);
+        }
+    } else each([&](int, int slot) {
         const unsigned same = alike(slot);
         if (slot >= 0 && lane == __ffs(same) - 1) {
             if (ordered) mine[slot] += __popc(same);
@@ -150,7 +161,12 @@ low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile,
         tiles[3 * q + 1] = begin;
         tiles[3 * q + 2] = min(tile, end - begin);
     }
-    each([&](int r, int slot) {
+    if (one) {
+        int place = 0;
+        if (lane == 0) place = ordered ? mine[lead] : atomicAdd(&mine[lead], to - from);
+        place = rows_before[lead] + __shfl_sync(0xffffffffu, place, 0);
+        for (int r = lane; r < to - from; r += 32) perm[place + r] = from + r;
+    } else each([&](int r, int slot) {
         const unsigned same = alike(slot);
         const int leader = __ffs(same) - 1;
         int place = 0;
@@ -474,6 +490,7 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
     __syncthreads();
     tg_after();
     const uint32_t tmem = *tmem_slot;
+    const float by = scale[id];
     const int kb0 = g.kbs * split / g.splits, kb1 = g.kbs * (split + 1) / g.splits;
     bool handed = false;                                     // the sums are there
 
@@ -567,7 +584,6 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
     // The rings are free: each block of the cluster has an equal share of the rows, and is handed all blocks' sums of
     // those, LT_PASS columns a pass ([block][32 columns][row of the share], a row's 16-byte pieces swapped by its place
     // among eight). It adds them in the blocks' order. Rank by rank the values are filled up to whole sixteens with zeros.
-    const float by = scale[id];
     const int padded = (rank + 15) / 16 * 16, slices = g.width / rank, quads = padded / 4;
     const int share = LT_ROWS / g.splits, blocks = (min(g.width, LT_PASS) + 31) / 32;
     for (int c0 = 0; c0 < g.width; c0 += LT_PASS) {
@@ -600,19 +616,17 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
             const unsigned char* const from = base + (c - c0) / 32 * (share * 128);
             const int piece = (c - c0) % 32 / 4;
             bf16* const to = u + ((size_t)(r0 + split * share) * slices + s) * 2 * padded + k;
-#pragma unroll 4
+#pragma unroll 2
             for (int row = warp; row < min(share, rows - split * share); row += LT_THREADS / 32) {
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (k < rank) {
-                    const unsigned char* at = from + row * 128 + ((piece ^ (row & 7)) << 4);
-                    v = *(const float4*)at;
-                    for (int i = 1; i < g.splits; ++i) {
-                        at += blocks * share * 128;
-                        const float4 q = *(const float4*)at;
-                        v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
-                    }
-                    v.x *= by; v.y *= by; v.z *= by; v.w *= by;
-                }
+                const unsigned char* const at_row = from + row * 128 + ((piece ^ (row & 7)) << 4);
+                float4 q[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    q[i] = i < g.splits && k < rank ? *(const float4*)(at_row + i * blocks * share * 128) : make_float4(0.f, 0.f, 0.f, 0.f);
+                float4 v = q[0];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) { v.x += q[i].x; v.y += q[i].y; v.z += q[i].z; v.w += q[i].w; }
+                v.x *= by; v.y *= by; v.z *= by; v.w *= by;
                 const uint32_t h0 = pack_bf16(v.x, v.y), h1 = pack_bf16(v.z, v.w);
                 bf16* const at = to + (size_t)row * slices * 2 * padded;
                 *(uint2*)at = make_uint2(h0, h1);
@@ -678,14 +692,15 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
     unsigned char* const y_ring = b_ring + 2 * L::B_BYTES;   // [warp][slot][box][32 rows][128]
     int* const rows = (int*)(y_ring + LO_HANDS * L::SLOTS * L::Y_BYTES);
     uint64_t* const full = (uint64_t*)(rows + LT_ROWS);      // [2] B's turn is there (the first: u, too)
-    uint64_t* const acc_full = full + 2;                     // [2] its products are done: the accumulator, and the slot free
-    uint64_t* const acc_empty = acc_full + 2;                // [2] the accumulator has been read
-    uint64_t* const y_full = acc_empty + 2;                  // [warp][slot]
+    uint64_t* const acc_full = full + 2;                     // [4] a turn's products are done: the accumulator, and B's slot free
+    uint64_t* const acc_empty = acc_full + 4;                // [4] the accumulator has been read
+    uint64_t* const y_full = acc_empty + 4;                  // [warp][slot]
     uint64_t* const settled = y_full + LO_HANDS * L::SLOTS;         // after a wait ran out
     uint32_t* const tmem_slot = (uint32_t*)(settled + 1);
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, tile = blockIdx.y;
     if (t == 0) {
-        for (int i = 0; i < 2; ++i) { tg_init(&full[i], 1); tg_init(&acc_full[i], 1); tg_init(&acc_empty[i], 4); }
+        for (int i = 0; i < 2; ++i) tg_init(&full[i], 1);
+        for (int i = 0; i < 4; ++i) { tg_init(&acc_full[i], 1); tg_init(&acc_empty[i], 4); }
         for (int i = 0; i < LO_HANDS * L::SLOTS; ++i) tg_init(&y_full[i], 1);
         tg_init(settled, 1);
         tg_init_done();
@@ -744,7 +759,7 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
             }
         }
         __syncwarp();
-        tg_alloc<2 * LO_COLS>(tmem_slot);
+        tg_alloc<4 * LO_COLS>(tmem_slot);
         tg_before();
         __syncthreads();
         tg_after();
@@ -754,14 +769,14 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
             uint32_t sent = min(turns, 2);
             bool ok = true;
             for (int i = 0; i < turns; ++i) {
-                const int s = i & 1;
+                const int s = i & 1, acc = i & 3;
                 ok = tg_wait(&full[s], (i >> 1) & 1, &low_rank_error_flag, 4);
-                if (ok) ok = tg_wait(&acc_empty[s], ((i >> 1) & 1) ^ 1, &low_rank_error_flag, 5);
+                if (ok) ok = tg_wait(&acc_empty[acc], ((i >> 2) & 1) ^ 1, &low_rank_error_flag, 5);
                 if (!ok) break;
                 tg_after();
 #pragma unroll
                 for (int h = 0; h < L::SLICES; ++h) {
-                    const uint32_t d = tmem + s * LO_COLS + h * (LO_COLS / 2);
+                    const uint32_t d = tmem + acc * LO_COLS + h * (LO_COLS / 2);
                     bool first = true;
 #pragma unroll
                     for (int x = 0; x < BOXES; ++x) {
@@ -777,9 +792,9 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
                         }
                     }
                 }
-                tg_commit(&acc_full[s]);
+                tg_commit(&acc_full[acc]);
                 if (i + 2 < turns) {                         // the slot again, once its products are done
-                    ok = tg_wait(&acc_full[s], (i >> 1) & 1, &low_rank_error_flag, 6);
+                    ok = tg_wait(&acc_full[acc], (i >> 2) & 1, &low_rank_error_flag, 6);
                     if (!ok) break;
                     tg_expect(&full[s], L::B_BYTES);
                     fetch(i + 2);
@@ -824,11 +839,12 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
         tg_before();
         __syncthreads();
         tg_after();
-        const uint32_t sums = *tmem_slot + ((uint32_t)q0 << 16) + set * LO_COLS;
+        const uint32_t lanes = *tmem_slot + ((uint32_t)q0 << 16);
         bool ok = true;
         for (int i = 0; i < turns_mine && ok; ++i) {
-            const int slot = i % L::SLOTS, c = col0 + (2 * i + set) * LO_COLS;
-            ok = __all_sync(0xffffffffu, tg_wait(&acc_full[set], i & 1, &low_rank_error_flag, 7));
+            const int slot = i % L::SLOTS, c = col0 + (2 * i + set) * LO_COLS, buf = (2 * i + set) & 3;
+            const uint32_t sums = lanes + buf * LO_COLS;
+            ok = __all_sync(0xffffffffu, tg_wait(&acc_full[buf], (i >> 1) & 1, &low_rank_error_flag, 7));
             if (ok && mine > 0) ok = __all_sync(0xffffffffu, tg_wait(&there[slot], (i / L::SLOTS) & 1, &low_rank_error_flag, 8));
             if (!ok) break;
             tg_after();
@@ -871,7 +887,7 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
             tg_before();
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) tg_arrive(&acc_empty[set]);
+            if (lane == 0) tg_arrive(&acc_empty[buf]);
             if (mine <= 0) continue;
             if (together && mine == 32 && c + LO_COLS <= col1) {
                 if (lane == 0) {
@@ -907,7 +923,7 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
     __syncthreads();
     if (warp == LO_HANDS) {
         tg_after();
-        tg_free<2 * LO_COLS>(*tmem_slot);
+        tg_free<4 * LO_COLS>(*tmem_slot);
     }
 }
 
