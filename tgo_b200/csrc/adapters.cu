@@ -442,9 +442,8 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
 // accumulators in turn, eight warps add y, read ahead, and write. Bound by y's and out's way.
 #define LT_ROWS 128
 #define LT_BK 64
-#define LT_X_BYTES (LT_ROWS * LT_BK * 2)
 #ifndef LT_STAGES
-#define LT_STAGES 4               // of the ring, at most 8
+#define LT_STAGES 6               // of the ring, at most 8
 #endif
 #define LT_PASS 256               // columns of u that the blocks of a cluster exchange at a time
 #define LT_THREADS 224
@@ -454,12 +453,16 @@ __device__ int low_rank_error_flag = 0;
 
 struct LowRankTile {
     int width, cut, cuts, kbs, splits, stages;    // A's rows come in `cuts` boxes of `cut`; `splits` blocks a cluster
+    int rows;                                     // of a cluster: 128, or 64 and two clusters a tile
 };
 // Bytes of the ring, which later holds a pass of sums.
 __host__ __device__ static inline int lt_ring(const LowRankTile& g) {
-    const int ring = g.stages * (LT_X_BYTES + g.cuts * g.cut * LT_BK * 2), pass = (g.width < LT_PASS ? (g.width + 31) / 32 * 32 : LT_PASS) * LT_ROWS * 4;
+    // with 64 rows the products read on for 64 more, into whatever lies there
+    const int ring = g.stages * (g.rows * LT_BK * 2 + g.cuts * g.cut * LT_BK * 2) + (LT_ROWS - g.rows) * LT_BK * 2, pass = (g.width < LT_PASS ? (g.width + 31) / 32 * 32 : LT_PASS) * g.rows * 4;
     return ring > pass ? ring : pass;
 }
+
+template <int N> struct LtParts { static constexpr int value = N; };
 
 template <int COLS>
 __global__ void __launch_bounds__(LT_THREADS)
@@ -469,13 +472,13 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
                   const int* __restrict__ tiles, bf16* __restrict__ u) {
     extern __shared__ unsigned char lt_raw[];
     unsigned char* const base = (unsigned char*)(((uintptr_t)lt_raw + 1023) & ~(uintptr_t)1023);
-    const int stage_bytes = LT_X_BYTES + g.cuts * g.cut * LT_BK * 2;
+    const int x_bytes = g.rows * LT_BK * 2, stage_bytes = x_bytes + g.cuts * g.cut * LT_BK * 2;
     uint64_t* const full = (uint64_t*)(base + lt_ring(g));
     uint64_t* const empty = full + 8;
     uint64_t* const done = empty + 8;
     uint64_t* const settled = done + 1;                      // after a wait ran out
     uint32_t* const tmem_slot = (uint32_t*)(settled + 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tile = blockIdx.y, split = blockIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tile = blockIdx.y, split = blockIdx.x % g.splits, skip = blockIdx.x / g.splits * g.rows;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 8; ++i) { tg_init(&full[i], 2); tg_init(&empty[i], 1); }
         tg_init(done, 1);
@@ -483,8 +486,8 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
         tg_init_done();
     }
     pdl_wait();
-    const int id = tiles[3 * tile], r0 = tiles[3 * tile + 1], rows = tiles[3 * tile + 2];
-    if (tile >= info[0] || id < 0) return;                   // the same for the whole cluster
+    const int id = tiles[3 * tile], r0 = tiles[3 * tile + 1] + skip, rows = min(tiles[3 * tile + 2] - skip, g.rows);
+    if (tile >= info[0] || id < 0 || rows <= 0) return;      // the same for the whole cluster
     if (warp == 1) tg_alloc<COLS>(tmem_slot);
     tg_before();
     __syncthreads();
@@ -510,9 +513,9 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
             }
             together = __all_sync(0xffffffffu, together);
         }
-        // more than three boxes of 32 rows come as one of 128: the rows after the tile's give sums that nobody stores
-        const bool whole = together && rows > 96;
-        const int groups = !together ? (rows + 3) / 4 : whole ? 1 : (rows + 31) / 32, group_bytes = !together ? 512 : whole ? LT_X_BYTES : 4096;
+        // three quarters and more come as one box: the rows after the tile's give sums that nobody stores
+        const bool whole = together && 4 * rows > 3 * g.rows;
+        const int groups = !together ? (rows + 3) / 4 : (rows + 31) / 32, group_bytes = !together ? 512 : 4096;
         int s = 0;
         uint32_t phase = 1;
         if (warp == 6 || whole) {                            // one thread asks for everything
@@ -523,10 +526,10 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
                     unsigned char* const st = base + (size_t)s * stage_bytes;
                     if (warp == 6) {
                         tg_expect(&full[s], (uint32_t)(g.cuts * g.cut * LT_BK * 2));
-                        tg_load_2d(st + LT_X_BYTES, &map_a, kb * LT_BK, id * g.width, &full[s]);
-                        if (g.cuts == 2) tg_load_2d(st + LT_X_BYTES + g.cut * LT_BK * 2, &map_a, kb * LT_BK, id * g.width + g.cut, &full[s]);
+                        tg_load_2d(st + x_bytes, &map_a, kb * LT_BK, id * g.width, &full[s]);
+                        if (g.cuts == 2) tg_load_2d(st + x_bytes + g.cut * LT_BK * 2, &map_a, kb * LT_BK, id * g.width + g.cut, &full[s]);
                     } else {
-                        tg_expect(&full[s], LT_X_BYTES);
+                        tg_expect(&full[s], (uint32_t)x_bytes);
                         tg_load_2d(st, &map_all, kb * LT_BK, first, &full[s]);
                     }
                     if (++s == g.stages) { s = 0; phase ^= 1; }
@@ -560,7 +563,7 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
                 if (!ok) break;
                 tg_after();
                 unsigned char* const st = base + (size_t)s * stage_bytes;
-                const uint64_t dx = tg_desc(st), da = tg_desc(st + LT_X_BYTES);
+                const uint64_t dx = tg_desc(st), da = tg_desc(st + x_bytes);
 #pragma unroll
                 for (int k = 0; k < LT_BK / 16; ++k) tg_mma(tmem, dx + 2 * k, da + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
                 if (g.cuts == 2) {
@@ -585,17 +588,17 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
     // those, LT_PASS columns a pass ([block][32 columns][row of the share], a row's 16-byte pieces swapped by its place
     // among eight). It adds them in the blocks' order. Rank by rank the values are filled up to whole sixteens with zeros.
     const int padded = (rank + 15) / 16 * 16, slices = g.width / rank, quads = padded / 4;
-    const int share = LT_ROWS / g.splits, blocks = (min(g.width, LT_PASS) + 31) / 32;
+    const int share = g.rows / g.splits, blocks = (min(g.width, LT_PASS) + 31) / 32;
     for (int c0 = 0; c0 < g.width; c0 += LT_PASS) {
         const int c1 = min(c0 + LT_PASS, g.width);
         lf_cluster_arrive();
         lf_cluster_wait();
-        if (warp >= 2 && warp < 6 && handed) {
+        if (warp >= 2 && warp < 6 && handed && (warp & 3) * 32 < rows) {
             const int quarter = warp & 3;                    // tensor-memory lanes this warp may read
             const int row = quarter * 32 + lane, in = row % share;
             uint32_t to;
             asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(tg_smem(base) + (uint32_t)(split * blocks * share * 128 + in * 128)), "r"(row / share));
-            for (int c = c0; quarter * 32 < rows && c < c1; c += 32, to += share * 128) {
+            for (int c = c0; c < c1; c += 32, to += share * 128) {
                 uint32_t a[32];
                 tg_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + c, a);
                 tg_wait_ld();
@@ -609,32 +612,38 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
         lf_cluster_wait();
         // a lane four values of a slice, a warp a row at a time
         const int s0 = c0 / rank, s1 = (c1 + rank - 1) / rank;   // slices that this pass touches
-        for (int e = lane; e < (s1 - s0) * quads; e += 32) {
-            const int s = s0 + e / quads, k = e % quads * 4, c = s * rank + k;
-            // the zeros behind a slice are written with its last value
-            if (k < rank ? c < c0 || c >= c1 : (s + 1) * rank <= c0 || (s + 1) * rank > c1) continue;
-            const unsigned char* const from = base + (c - c0) / 32 * (share * 128);
-            const int piece = (c - c0) % 32 / 4;
-            bf16* const to = u + ((size_t)(r0 + split * share) * slices + s) * 2 * padded + k;
-#pragma unroll 2
-            for (int row = warp; row < min(share, rows - split * share); row += LT_THREADS / 32) {
-                const unsigned char* const at_row = from + row * 128 + ((piece ^ (row & 7)) << 4);
-                float4 q[8];
+        auto add = [&](auto parts) {
+            constexpr int PARTS = decltype(parts)::value;
+            for (int e = lane; e < (s1 - s0) * quads; e += 32) {
+                const int s = s0 + e / quads, k = e % quads * 4, c = s * rank + k;
+                // the zeros behind a slice are written with its last value
+                if (k < rank ? c < c0 || c >= c1 : (s + 1) * rank <= c0 || (s + 1) * rank > c1) continue;
+                const unsigned char* const from = base + (c - c0) / 32 * (share * 128);
+                const int piece = (c - c0) % 32 / 4, step = blocks * share * 128;
+                bf16* to = u + ((size_t)(r0 + split * share + warp) * slices + s) * 2 * padded + k;
+#pragma unroll 4
+                for (int row = warp; row < min(share, rows - split * share); row += LT_THREADS / 32, to += (size_t)(LT_THREADS / 32) * slices * 2 * padded) {
+                    const unsigned char* const at = from + row * 128 + ((piece ^ (row & 7)) << 4);
+                    float4 v = *(const float4*)at;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    q[i] = i < g.splits && k < rank ? *(const float4*)(at_row + i * blocks * share * 128) : make_float4(0.f, 0.f, 0.f, 0.f);
-                float4 v = q[0];
-#pragma unroll
-                for (int i = 1; i < 8; ++i) { v.x += q[i].x; v.y += q[i].y; v.z += q[i].z; v.w += q[i].w; }
-                v.x *= by; v.y *= by; v.z *= by; v.w *= by;
-                const uint32_t h0 = pack_bf16(v.x, v.y), h1 = pack_bf16(v.z, v.w);
-                bf16* const at = to + (size_t)row * slices * 2 * padded;
-                *(uint2*)at = make_uint2(h0, h1);
-                *(uint2*)(at + padded) = make_uint2(
-                    pack_bf16(v.x - __uint_as_float(h0 << 16), v.y - __uint_as_float(h0 & 0xffff0000u)),
-                    pack_bf16(v.z - __uint_as_float(h1 << 16), v.w - __uint_as_float(h1 & 0xffff0000u)));
+                    for (int i = 1; i < PARTS; ++i) {
+                        const float4 q = *(const float4*)(at + i * step);
+                        v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+                    }
+                    if (k >= rank) v = make_float4(0.f, 0.f, 0.f, 0.f);     // what lies behind a slice is the next one's
+                    v.x *= by; v.y *= by; v.z *= by; v.w *= by;
+                    const uint32_t h0 = pack_bf16(v.x, v.y), h1 = pack_bf16(v.z, v.w);
+                    *(uint2*)to = make_uint2(h0, h1);
+                    *(uint2*)(to + padded) = make_uint2(
+                        pack_bf16(v.x - __uint_as_float(h0 << 16), v.y - __uint_as_float(h0 & 0xffff0000u)),
+                        pack_bf16(v.z - __uint_as_float(h1 << 16), v.w - __uint_as_float(h1 & 0xffff0000u)));
+                }
             }
-        }
+        };
+        if (g.splits == 1) add(LtParts<1>());
+        else if (g.splits == 2) add(LtParts<2>());
+        else if (g.splits == 4) add(LtParts<4>());
+        else add(LtParts<8>());
     }
     tg_before();
     __syncthreads();
@@ -1042,25 +1051,34 @@ template <typename TY> static bool lr_tile_takes(const LowRank& p) {
     return true;
 }
 
-// How A's rows are fetched, the ring, and the parts of k (blocks of a cluster): the count that is cheapest by a small
-// model. The blocks run in rounds of as many as the multiprocessors hold; a block costs a unit a block of k and eight to
-// begin and end. The tiles that the rows make at least, and one, are counted with (how many more is the device's to know).
 static int lt_bytes(const LowRankTile& g) { return lt_ring(g) + 1024 + 256; }
+// How a tile's u is made: the rows of a cluster and the parts of k, its blocks, that are cheapest by a small model in
+// cycles. The blocks run in rounds of as many as the multiprocessors hold. 64 columns cost a block their way into the
+// multiprocessor (70 bytes a cycle) or its part of the way of all blocks' rows from memory (3400); to begin and end
+// takes 6000, to exchange sums 3000 and 50 a column. (The tiles that the rows make at least, and one: how many more is the
+// device's to know.) MEASURED: XXX
 static LowRankTile lr_plan(const LowRank& p) {
-    LowRankTile g;
-    g.width = p.columns.slices * p.rank;
-    g.cuts = g.width > 256 ? 2 : 1;
-    g.cut = ((g.width + g.cuts - 1) / g.cuts + 15) / 16 * 16;
-    g.kbs = (p.K + LT_BK - 1) / LT_BK;
-    const int stage = LT_X_BYTES + g.cuts * g.cut * LT_BK * 2, most = 176 * 1024 / stage, tiles = (p.T + LT_ROWS - 1) / LT_ROWS + 1;
-    g.stages = most < LT_STAGES ? most : LT_STAGES;
-    const int slots = tgo_multiprocessors() * (2 * lt_bytes(g) <= 226 * 1024 && g.cuts * g.cut <= 256 ? 2 : 1);
-    long long best = -1;
-    for (int s = 1; s <= 8 && (s == 1 || s * 4 <= g.kbs); s *= 2) {
-        const long long cost = ((long long)tiles * s + slots - 1) / slots * ((g.kbs + s - 1) / s + 8);
-        if (best < 0 || cost < best) { best = cost; g.splits = s; }
-    }
-    return g;
+    LowRankTile best = {};
+    long long least = -1;
+    for (int rows = LT_ROWS; rows >= LT_ROWS / 2; rows /= 2)
+        for (int s = 1; s <= 8; s *= 2) {
+            LowRankTile g;
+            g.rows = rows;
+            g.splits = s;
+            g.width = p.columns.slices * p.rank;
+            g.cuts = g.width > 256 ? 2 : 1;
+            g.cut = ((g.width + g.cuts - 1) / g.cuts + 15) / 16 * 16;
+            g.kbs = (p.K + LT_BK - 1) / LT_BK;
+            if (s > 1 && s * 4 > g.kbs) break;
+            const int x = rows * LT_BK * 2, stage = x + g.cuts * g.cut * LT_BK * 2, most = 168 * 1024 / stage;
+            g.stages = most < LT_STAGES ? most : LT_STAGES;
+            const int slots = tgo_multiprocessors() * (2 * lt_bytes(g) <= 226 * 1024 && g.cuts * g.cut <= 256 ? 2 : 1);
+            const long long blocks = ((p.T + LT_ROWS - 1) / LT_ROWS + 1ll) * (LT_ROWS / rows) * s;
+            const long long feed = stage / 70, memory = (blocks < slots ? blocks : slots) * x / 3400, each = feed > memory ? feed : memory;
+            const long long cost = (blocks + slots - 1) / slots * ((g.kbs + s - 1) / s * each + 6000 + (s > 1 ? 3000 + 50 * g.width : 0));
+            if (least < 0 || cost < least) { least = cost; best = g; }
+        }
+    return best;
 }
 
 template <int COLS> static int low_rank_u(const LowRank& p, const LowRankTile& g, const int* perm, const int* info, const int* tiles, bf16* u,
@@ -1077,10 +1095,10 @@ template <int COLS> static int low_rank_u(const LowRank& p, const LowRankTile& g
     }
     CUtensorMap row, some, all, a;
     if (!tg_map(&row, p.x, p.T, p.K, p.x_stride, 1) || !tg_map(&some, p.x, p.T, p.K, p.x_stride, 32) ||
-        !tg_map(&all, p.x, p.T, p.K, p.x_stride, LT_ROWS) || !tg_map(&a, p.a, (long long)p.adapters * g.width, p.K, p.K, g.cut))
+        !tg_map(&all, p.x, p.T, p.K, p.x_stride, g.rows) || !tg_map(&a, p.a, (long long)p.adapters * g.width, p.K, p.K, g.cut))
         return TGO_E_BAD_ARG;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(g.splits, (unsigned)lr_tiles(p, LT_ROWS));
+    cfg.gridDim = dim3(LT_ROWS / g.rows * g.splits, (unsigned)lr_tiles(p, LT_ROWS));
     cfg.blockDim = dim3(LT_THREADS);
     cfg.dynamicSmemBytes = (size_t)lt_bytes(g);
     cfg.stream = stream;
