@@ -14,6 +14,14 @@ def ops():
     return o
 
 
+@pytest.fixture(params=["chosen", "tiles"], autouse=True)
+def way(request):
+    """Every test goes the way that the framework chooses, and by tiles of 128 rows wherever they take its call."""
+    ops().low_rank_force_way(2 if request.param == "tiles" else 0)
+    yield request.param
+    ops().low_rank_force_way(0)
+
+
 def columns_of(widths, interleaved):
     if interleaved:
         return (torch.arange(sum(widths)) // 8) % 2
@@ -165,6 +173,28 @@ def test_values_that_are_not_finite_stay_in_their_row(x_type):
         rest = [t for t in range(T) if t not in (4, 5)]
         assert torch.equal(bad[rest], out[rest])
         assert torch.isnan(bad[4]).all() and not torch.isfinite(bad[5]).any()
+
+
+@pytest.mark.parametrize("x_type", [F32, BF])
+@pytest.mark.parametrize("T", [3, 140, 333])
+def test_infinite_products(x_type, T):
+    """An infinity in x gives infinities of B's signs, not NaN."""
+    p = inputs(T, 64, (32,), 8, 1, x_type, x_type, seed=T, ids=torch.zeros(T, dtype=torch.int32))
+    p["a"].fill_(1.0)
+    p["x"][1] = 0.0
+    p["x"][1, 7] = float("inf")
+    out = torch.empty_like(p["y"])
+    p["b"].copy_(p["b"].abs())
+    p["b"][0, 3] *= -1.0
+    ops().low_rank_add(p["x"], p["y"], p["a"], p["b"], p["scale"], p["ids"], (32,), out=out)
+    want = torch.full((32,), float("inf"), device=DEV)
+    want[3] = -float("inf")
+    assert torch.equal(out[1].float(), want) and torch.isfinite(out[torch.arange(T) != 1]).all()
+
+
+@pytest.mark.parametrize("T,K,widths,rank", [(1210, 2048, (2048,), 64), (700, 1024, (1536, 512, 512), 72)])
+def test_sizes_that_go_by_tiles(T, K, widths, rank):
+    check(inputs(T, K, widths, rank, 3, BF, BF, seed=T), widths)
 
 
 def test_no_rows_and_other_streams():

@@ -16,6 +16,14 @@ struct LowRankColumns {
     int interleaved;              // eight columns of slice 0, eight of slice 1, and so on
 };
 
+// Four values of u as the second product takes them: each rounded to bfloat16 (x, y) and what that left out, rounded
+// too (z, w). An infinity leaves nothing out.
+__device__ __forceinline__ uint4 lr_split(float4 v) {
+    auto rest = [](float f, uint32_t rounded) { const float h = __uint_as_float(rounded); return f == h ? 0.f : f - h; };
+    const uint32_t a = pack_bf16(v.x, v.y), b = pack_bf16(v.z, v.w);
+    return make_uint4(a, b, pack_bf16(rest(v.x, a << 16), rest(v.y, a & 0xffff0000u)), pack_bf16(rest(v.z, b << 16), rest(v.w, b & 0xffff0000u)));
+}
+
 __device__ __forceinline__ int lr_slice(const LowRankColumns& c, int n) {
     if (c.interleaved) return (n >> 3) & 1;
     int s = 0;
@@ -193,13 +201,16 @@ low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile,
 // float32: plain sums, a warp four values of u for all eight rows, its lanes over k; u's and the result's
 // order of additions depends on K and the rank alone, whatever the batch.
 //
-// Without a plan every row has a cluster, which looks through the ids: the first, ninth, ... row of an
-// adapter takes up to seven further ones, the others leave.
+// Without a plan (up to 256 rows) each cluster finds its rows by itself: a thread a row counts the rows of the same
+// adapter before it, every eighth begins a group, and the cluster takes the group of its number. Half a microsecond,
+// where a plan of its own takes four. (A single row has nothing to look for: 4.2 us, 4.5 with it.)
 #define LF_ROWS 8
 #define LF_CTAS 8
 #define LF_THREADS 256
 #define LF_WARPS (LF_THREADS / 32)
 #define LF_PASS 64                // values of u a pass, bfloat16
+#define LF_TILES 2                // tiles of 16 columns a warp has under way, bfloat16
+static_assert(LF_ROWS == LF_WARPS, "a warp a row");
 
 __device__ __forceinline__ void lf_cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void lf_cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
@@ -219,11 +230,12 @@ template <typename T> static inline long long lf_floats(int width, int K) {
 }
 
 template <typename T, typename TY>
-__global__ void __launch_bounds__(LF_THREADS)
+__global__ void __launch_bounds__(LF_THREADS, 3)
 low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __restrict__ info, const int* __restrict__ tiles) {
     extern __shared__ __align__(16) float lf_smem[];
     __shared__ int rows[LF_ROWS];
-    __shared__ int warp_count[LF_WARPS];
+    __shared__ __align__(16) int ids[LF_THREADS];
+    __shared__ int warp_count[LF_WARPS], group[2];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int item = blockIdx.x / LF_CTAS, cta = blockIdx.x % LF_CTAS;
     pdl_wait();
@@ -234,42 +246,58 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
         n = tiles[3 * item + 2];
         if (t < n) rows[t] = perm[tiles[3 * item + 1] + t];
         __syncthreads();
-    } else {
-        id = p.ids[item];
+    } else if (p.T == 1) {
+        id = p.ids[0];
         n = 1;
-        if (t == 0) rows[0] = item;
-        if (id >= 0 && id < p.adapters) {
-            int before = 0;
-            for (int base = 0; base < item; base += LF_THREADS)
-                before += __syncthreads_count(base + t < item && p.ids[base + t] == id);
-            if (before % LF_ROWS) return;
-            for (int base = item + 1; base < p.T && n < LF_ROWS; base += LF_THREADS) {
-                const bool same = base + t < p.T && p.ids[base + t] == id;
-                const unsigned who = __ballot_sync(0xffffffffu, same);
-                if (lane == 0) warp_count[warp] = __popc(who);
-                __syncthreads();
-                int place = n, all = 0;
-#pragma unroll
-                for (int w = 0; w < LF_WARPS; ++w) {
-                    place += w < warp ? warp_count[w] : 0;
-                    all += warp_count[w];
-                }
-                place += __popc(who & ((1u << lane) - 1));
-                if (same && place < LF_ROWS) rows[place] = base + t;
-                n += all;
-                __syncthreads();
-            }
-            n = min(n, LF_ROWS);
-        }
+        if (t == 0) rows[0] = 0;
         __syncthreads();
+    } else {
+        int mine = -2;
+        if (t < p.T) {
+            mine = p.ids[t];
+            if (mine < 0 || mine >= p.adapters) mine = -1;
+        }
+        ids[t] = mine;
+        __syncthreads();
+        int before = 0, place = 0, all = 0;                  // rows of this one's adapter before it; groups before this one's, and all
+        for (int j = 0; j < min(t | 31, p.T); j += 4) {
+            const int4 q = *(const int4*)(ids + j);
+            before += (q.x == mine && j < t) + (q.y == mine && j + 1 < t) + (q.z == mine && j + 2 < t) + (q.w == mine && j + 3 < t);
+        }
+        const bool begins = t < p.T && before % LF_ROWS == 0;
+        const unsigned who = __ballot_sync(0xffffffffu, begins);
+        if (lane == 0) warp_count[warp] = __popc(who);
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < LF_WARPS; ++w) {
+            place += w < warp ? warp_count[w] : 0;
+            all += warp_count[w];
+        }
+        if (item >= all) return;
+        if (begins && place + __popc(who & ((1u << lane) - 1)) == item) { group[0] = mine; group[1] = before; }
+        __syncthreads();
+        id = group[0];
+        const bool in = mine == id && before >= group[1] && before < group[1] + LF_ROWS;
+        if (in) rows[before - group[1]] = t;
+        n = __syncthreads_count(in);
     }
     const TY* const y = (const TY*)p.y;
     TY* const out = (TY*)p.out;
     const int pairs = (p.N + 31) / 32, col0 = min((pairs * cta / LF_CTAS) * 32, p.N), col1 = min((pairs * (cta + 1) / LF_CTAS) * 32, p.N);
     if (id < 0 || id >= p.adapters) {                        // no adapter: y as it is
-        if (p.out != p.y)
-            for (int i = 0; i < n; ++i)
-                for (int c = col0 + t; c < col1; c += LF_THREADS) out[(size_t)rows[i] * p.out_stride + c] = y[(size_t)rows[i] * p.y_stride + c];
+        if (p.out != p.y && warp < n) {
+            const TY* const from = y + (size_t)rows[warp] * p.y_stride;
+            TY* const to = out + (size_t)rows[warp] * p.out_stride;
+            for (int c = col0 + lane; c < col1; c += 8 * 32) {
+                TY v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (c + i * 32 < col1) v[i] = from[c + i * 32];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (c + i * 32 < col1) to[c + i * 32] = v[i];
+            }
+        }
         return;
     }
     const int rank = p.rank, width = p.columns.slices * rank, K = p.K;
@@ -324,12 +352,14 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
             __syncthreads();
         }
     } else {
+        // x in shared memory, a warp a row. Three blocks a multiprocessor are asked for: 347 rows of three adapters, width
+        // 2048, 3072 columns, rank 8 14.0 us, with two 18.8.
         const int kc = ((K + LF_CTAS - 1) / LF_CTAS + 3) / 4 * 4, k0 = min(cta * kc, K), k1 = min(k0 + kc, K);
         float* const xs = tail;                              // [row][k of the block]
-        for (int r = 0; r < LF_ROWS; ++r)
-            for (int k = t * 4; k < k1 - k0; k += LF_THREADS * 4)
-                *(float4*)(xs + r * kc + k) = r < n ? *(const float4*)((const float*)p.x + (size_t)rows[r] * p.x_stride + k0 + k)
-                                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int k = lane * 4; k < k1 - k0; k += 128)
+            *(float4*)(xs + warp * kc + k) = warp < n ? *(const float4*)((const float*)p.x + (size_t)rows[warp] * p.x_stride + k0 + k)
+                                                      : make_float4(0.f, 0.f, 0.f, 0.f);
         __syncthreads();
         for (int j0 = warp * 4; j0 < width; j0 += 4 * LF_WARPS) {
             float v[4 * LF_ROWS] = {};
@@ -367,7 +397,10 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
             const float4 q = lf_peer(part + e, r);
             s.x += q.x; s.y += q.y; s.z += q.z; s.w += q.w;
         }
-        *(float4*)(u + (e / width) * (width + 4) + e % width) = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
+        s = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
+        float* const to = u + (e / width) * (width + 4) + e % width;
+        if constexpr (sizeof(T) == 2) *(uint4*)to = lr_split(s);
+        else *(float4*)to = s;
     }
     lf_cluster_arrive();                                     // waited for at the end: a peer may still be reading `part`
     __syncthreads();
@@ -375,45 +408,66 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
     if constexpr (sizeof(T) == 2) {
         const int g = lane >> 2, tig = lane & 3;
         const int r0 = 2 * tig < n ? rows[2 * tig] : -1, r1 = 2 * tig + 1 < n ? rows[2 * tig + 1] : -1;
-#pragma unroll 2
-        for (int q = col0 / 16 + warp; q < col1 / 16; q += LF_WARPS) {
-            // the tile's column of the product's row g, and how much further that of row g + 8 is
-            const int c = p.columns.interleaved ? q / 2 * 32 + (q & 1) * 8 + g : q * 16 + g, far = p.columns.interleaved ? 16 : 8;
-            const int s = p.columns.interleaved ? q & 1 : lr_slice(p.columns, q * 16);
-            const bf16* const w = b + (size_t)c * rank;
-            float v[4];
-            v[0] = r0 >= 0 ? to_f32(y[(size_t)r0 * p.y_stride + c]) : 0.f;
-            v[1] = r1 >= 0 ? to_f32(y[(size_t)r1 * p.y_stride + c]) : 0.f;
-            v[2] = r0 >= 0 ? to_f32(y[(size_t)r0 * p.y_stride + c + far]) : 0.f;
-            v[3] = r1 >= 0 ? to_f32(y[(size_t)r1 * p.y_stride + c + far]) : 0.f;
-            float acc[4] = {};
+        // LF_TILES tiles of 16 columns at a time: what is read of y and B is under way before the first is made (out may be
+        // y, so no load passes a store by itself). MEASURED: 96 rows of 24 adapters, width 4096, 6144 columns, rank 16: one at a time 12.7 us, two 11.6,
+        // four 12.6: the code is run once, and its fetching shows.
+        const int far = p.columns.interleaved ? 16 : 8;      // columns from a product's row g to row g + 8
+#pragma unroll 1
+        for (int q0 = col0 / 16 + warp; q0 < col1 / 16; q0 += LF_TILES * LF_WARPS) {
+            int c[LF_TILES], at_u[LF_TILES];
+            TY v[LF_TILES][4];
+            float acc[LF_TILES][4] = {};
+#pragma unroll
+            for (int i = 0; i < LF_TILES; ++i) {
+                const int q = min(q0 + i * LF_WARPS, col1 / 16 - 1);     // past the end: the last one, and not stored
+                c[i] = p.columns.interleaved ? q / 2 * 32 + (q & 1) * 8 + g : q * 16 + g;
+                at_u[i] = g * (width + 4) + (p.columns.interleaved ? q & 1 : lr_slice(p.columns, q * 16)) * rank;
+                const TY* const ya = y + (size_t)max(r0, 0) * p.y_stride + c[i];
+                const TY* const yb = y + (size_t)max(r1, 0) * p.y_stride + c[i];
+                if (r0 >= 0) { v[i][0] = ya[0]; v[i][2] = ya[far]; }
+                if (r1 >= 0) { v[i][1] = yb[0]; v[i][3] = yb[far]; }
+            }
+#pragma unroll 1
             for (int k = 4 * tig; k - 4 * tig < rank; k += 16) {
-                uint2 lo = make_uint2(0, 0), hi = lo;
-                float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (k < rank) {
-                    lo = *(const uint2*)(w + k);
-                    hi = *(const uint2*)(w + (size_t)far * rank + k);
-                    f = *(const float4*)(u + g * (width + 4) + s * rank + k);
+                uint2 lo[LF_TILES], hi[LF_TILES];
+#pragma unroll
+                for (int i = 0; i < LF_TILES; ++i) {
+                    lo[i] = hi[i] = make_uint2(0, 0);
+                    if (k < rank) {
+                        lo[i] = *(const uint2*)(b + (size_t)c[i] * rank + k);
+                        hi[i] = *(const uint2*)(b + (size_t)(c[i] + far) * rank + k);
+                    }
                 }
-                const uint32_t m[4] = {lo.x, hi.x, lo.y, hi.y};
-                const float4 h = make_float4(to_f32(from_f32<bf16>(f.x)), to_f32(from_f32<bf16>(f.y)), to_f32(from_f32<bf16>(f.z)), to_f32(from_f32<bf16>(f.w)));
-                mma_bf16(acc, m, pack_bf16(f.x, f.y), pack_bf16(f.z, f.w));
-                mma_bf16(acc, m, pack_bf16(f.x - h.x, f.y - h.y), pack_bf16(f.z - h.z, f.w - h.w));
+#pragma unroll
+                for (int i = 0; i < LF_TILES; ++i) {
+                    const uint4 f = k < rank ? *(const uint4*)(u + at_u[i] + k) : make_uint4(0, 0, 0, 0);
+                    const uint32_t m[4] = {lo[i].x, hi[i].x, lo[i].y, hi[i].y};
+                    mma_bf16(acc[i], m, f.x, f.y);
+                    mma_bf16(acc[i], m, f.z, f.w);
+                }
             }
-            if (r0 >= 0) {
-                out[(size_t)r0 * p.out_stride + c] = from_f32<TY>(v[0] + acc[0]);
-                out[(size_t)r0 * p.out_stride + c + far] = from_f32<TY>(v[2] + acc[2]);
-            }
-            if (r1 >= 0) {
-                out[(size_t)r1 * p.out_stride + c] = from_f32<TY>(v[1] + acc[1]);
-                out[(size_t)r1 * p.out_stride + c + far] = from_f32<TY>(v[3] + acc[3]);
+#pragma unroll
+            for (int i = 0; i < LF_TILES; ++i) {
+                if (q0 + i * LF_WARPS >= col1 / 16) break;
+                if (r0 >= 0) {
+                    out[(size_t)r0 * p.out_stride + c[i]] = from_f32<TY>(to_f32(v[i][0]) + acc[i][0]);
+                    out[(size_t)r0 * p.out_stride + c[i] + far] = from_f32<TY>(to_f32(v[i][2]) + acc[i][2]);
+                }
+                if (r1 >= 0) {
+                    out[(size_t)r1 * p.out_stride + c[i]] = from_f32<TY>(to_f32(v[i][1]) + acc[i][1]);
+                    out[(size_t)r1 * p.out_stride + c[i] + far] = from_f32<TY>(to_f32(v[i][3]) + acc[i][3]);
+                }
             }
         }
     } else {
         for (int c = col0 + t; c < col1; c += LF_THREADS) {
             const float* const w = (const float*)b + (size_t)c * rank;
             const float* const us = u + lr_slice(p.columns, c) * rank;
-            float acc[LF_ROWS] = {};
+            float acc[LF_ROWS] = {}, v[LF_ROWS];             // y first: out may be y, and no load passes a store
+#pragma unroll
+            for (int r = 0; r < LF_ROWS; ++r)
+                if (r < n) v[r] = to_f32(y[(size_t)rows[r] * p.y_stride + c]);
+#pragma unroll 2
             for (int k = 0; k < rank; k += 4) {
                 const float4 q = *(const float4*)(w + k);
 #pragma unroll
@@ -424,27 +478,26 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
             }
 #pragma unroll
             for (int r = 0; r < LF_ROWS; ++r)
-                if (r < n) out[(size_t)rows[r] * p.out_stride + c] = from_f32<TY>(to_f32(y[(size_t)rows[r] * p.y_stride + c]) + acc[r]);
+                if (r < n) out[(size_t)rows[r] * p.out_stride + c] = from_f32<TY>(v[r] + acc[r]);
         }
     }
     lf_cluster_wait();
 }
 
 // ---------------------------------------------------------------------- many rows of an adapter
-// Tiles of 128 planned rows, bfloat16. Two kernels, u between them in float32:
+// Tiles of 128 planned rows, bfloat16. Two kernels, u between them as two bfloat16 numbers a value (see above):
 //
-// u (`low_rank_u_kernel`): [128, slices x rank] = X[rows] A^T on tcgen05, a cluster a tile, a part of k a block:
-// TMA brings 64 columns of the tile's rows (one box where they lie together, else four rows a request) and of A
-// into a ring, a thread issues the products. The blocks sum their parts through each other's shared memory, scale
-// u and split it into two bfloat16 numbers (see above). Bound by x's way from memory.
+// u (`low_rank_u_kernel`): X[rows] A^T on tcgen05, a cluster 64 or 128 rows, a part of k a block: TMA brings 64 columns of
+// the rows (one box where they lie together, else four rows a request) and of A into a ring, a thread issues the products.
+// Each block sends its sums to the blocks that add them, by rows, through their shared memory; these scale u and split it.
+// Bound by x's way into the multiprocessors: 28 of the 72 us of 8192 rows, width 4096, rank 64, q, k and v.
 //
-// out (`low_rank_out_kernel`): u and 128 columns of B at a time come by TMA, a thread issues the products into two
-// accumulators in turn, eight warps add y, read ahead, and write. Bound by y's and out's way.
+// out (`low_rank_out_kernel`): u and 64 columns of B at a time come by TMA, a thread issues the products into four
+// accumulators in turn, eight warps add them to y in shared memory, from where TMA stores it. Bound by y's and out's way:
+// 40 of the 72 us, 5 TB/s.
 #define LT_ROWS 128
 #define LT_BK 64
-#ifndef LT_STAGES
 #define LT_STAGES 6               // of the ring, at most 8
-#endif
 #define LT_PASS 256               // columns of u that the blocks of a cluster exchange at a time
 #define LT_THREADS 224
 #define LT_MAX_WIDTH 512          // slices x rank: the columns of tensor memory
@@ -632,11 +685,9 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
                     }
                     if (k >= rank) v = make_float4(0.f, 0.f, 0.f, 0.f);     // what lies behind a slice is the next one's
                     v.x *= by; v.y *= by; v.z *= by; v.w *= by;
-                    const uint32_t h0 = pack_bf16(v.x, v.y), h1 = pack_bf16(v.z, v.w);
-                    *(uint2*)to = make_uint2(h0, h1);
-                    *(uint2*)(to + padded) = make_uint2(
-                        pack_bf16(v.x - __uint_as_float(h0 << 16), v.y - __uint_as_float(h0 & 0xffff0000u)),
-                        pack_bf16(v.z - __uint_as_float(h1 << 16), v.w - __uint_as_float(h1 & 0xffff0000u)));
+                    const uint4 two = lr_split(v);
+                    *(uint2*)to = make_uint2(two.x, two.y);
+                    *(uint2*)(to + padded) = make_uint2(two.z, two.w);
                 }
             }
         };
@@ -660,11 +711,9 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
 // from tensor memory, a lane a row) of every other turn and a ring of its own of 32 x 64 tiles; it adds the sums where
 // y lies and has the tile stored from there. Rows that lie together are one box either way; others come four at a time and are written by
 // the warp, as are part tiles. (Reading y into registers two steps ahead and writing from them, through a transposing
-// buffer, took 68 us where this takes XXX: 8192 rows of 6144 columns.)
+// buffer, took 68 us where this takes 40: 8192 rows of 6144 columns, rank 64.)
 #define LO_COLS 64
-#ifndef LO_TURNS
 #define LO_TURNS 8                // of a block
-#endif
 #define LO_HANDS 8                // warps that hand on; the one after them asks for copies and products
 #define LO_THREADS (LO_HANDS * 32 + 32)
 #define LO_U_BOX (LT_ROWS * 128)  // bytes of 64 values of k: of 128 rows of u,
@@ -988,16 +1037,17 @@ template <typename T> static bool lr_vectors(const LowRank& p) {
 }
 
 // Rows from which they are planned: up to here each cluster of the kernel for few rows finds its own.
-#define LR_SCAN_ROWS 256
+#define LR_SCAN_ROWS LF_THREADS
 
 template <typename T> static bool lr_few_takes(const LowRank& p) {
     return lr_vectors<T>(p) && lf_floats<T>(p.columns.slices * p.rank, p.K) * 4 <= 200 * 1024 && p.T <= (1 << 24) &&
            (p.T <= LR_SCAN_ROWS || p.adapters <= LP_MAX_ADAPTERS);
 }
 
-// Tiles there are at most: an adapter leaves one part tile at most.
+// Tiles there are at most: with an adapter's first row comes one, with every `tile` further ones another.
 static long long lr_tiles(const LowRank& p, int tile) {
-    return (p.T + tile - 1) / tile + (p.T < p.adapters + 1 ? p.T : p.adapters + 1);
+    const long long adapters = p.T < p.adapters + 1 ? p.T : p.adapters + 1;
+    return adapters + (p.T - adapters) / tile;
 }
 
 template <typename T, typename TY> static int low_rank_few(const LowRank& p, int* plan, cudaStream_t stream) {
@@ -1011,10 +1061,9 @@ template <typename T, typename TY> static int low_rank_few(const LowRank& p, int
         if (err != cudaSuccess) return (int)err;
         sized[dev] = true;
     }
-    long long items = p.T;
+    const long long items = lr_tiles(p, LF_ROWS);
     int *perm = nullptr, *info = nullptr, *tiles = nullptr;
     if (p.T > LR_SCAN_ROWS) {
-        items = lr_tiles(p, LF_ROWS);
         perm = plan;
         info = perm + p.T;
         tiles = info + 1;
@@ -1055,8 +1104,10 @@ static int lt_bytes(const LowRankTile& g) { return lt_ring(g) + 1024 + 256; }
 // How a tile's u is made: the rows of a cluster and the parts of k, its blocks, that are cheapest by a small model in
 // cycles. The blocks run in rounds of as many as the multiprocessors hold. 64 columns cost a block their way into the
 // multiprocessor (70 bytes a cycle) or its part of the way of all blocks' rows from memory (3400); to begin and end
-// takes 6000, to exchange sums 3000 and 50 a column. (The tiles that the rows make at least, and one: how many more is the
-// device's to know.) MEASURED: XXX
+// takes 6000, to exchange sums 1500 and a cycle for four. (The tiles that the rows make at least, and one: how many more is
+// the device's to know.) MEASURED, all three kernels, us, 1, 2, 4 and 8 parts: 8192 rows, rank 64, q, k and v, clusters of
+// 128 rows 80, 72 (taken), 83, 118, of 64 74, 81, 98, 140; 1833 rows, rank 32, gate and up, 128 rows 73, 68, 65, 70, 64 rows
+// 72, 66, 64 (taken), 64.
 static LowRankTile lr_plan(const LowRank& p) {
     LowRankTile best = {};
     long long least = -1;
@@ -1075,7 +1126,7 @@ static LowRankTile lr_plan(const LowRank& p) {
             const int slots = tgo_multiprocessors() * (2 * lt_bytes(g) <= 226 * 1024 && g.cuts * g.cut <= 256 ? 2 : 1);
             const long long blocks = ((p.T + LT_ROWS - 1) / LT_ROWS + 1ll) * (LT_ROWS / rows) * s;
             const long long feed = stage / 70, memory = (blocks < slots ? blocks : slots) * x / 3400, each = feed > memory ? feed : memory;
-            const long long cost = (blocks + slots - 1) / slots * ((g.kbs + s - 1) / s * each + 6000 + (s > 1 ? 3000 + 50 * g.width : 0));
+            const long long cost = (blocks + slots - 1) / slots * ((g.kbs + s - 1) / s * each + 6000 + (s > 1 ? 1500 + rows * g.width / 4 : 0));
             if (least < 0 || cost < least) { least = cost; best = g; }
         }
     return best;
@@ -1176,10 +1227,18 @@ template <typename TY> static int low_rank_tiles(const LowRank& p, int* work, cu
                                  : low_rank_out_of<false, TY>(p, u, perm, info, tiles, stream);
 }
 
-// Rows from which a call goes by tiles of 128.
-#ifndef LR_TILE_ROWS
-#define LR_TILE_ROWS 300
-#endif
+#define LR_TILE_BYTES 40000000ll
+// Whether a call goes by tiles of 128 rows: three kernels take 17 us however few the rows are; the clusters read an
+// adapter again for every eight rows, at about 3 TB/s. So from 40 MB of such reading on. MEASURED (us, clusters / tiles;
+// rows in four runs, then of 24 adapters at random): width 4096, q, k and v, rank 16, 384 rows 18 / 19 and 21 / 26, 768
+// 31 / 20 and 33 / 29; rank 64, 128 rows 31 / 21 and 31 / 34, 384 36 / 23 and 44 / 36; gate and up of 12288, rank 32, 128
+// rows 39 / 21 and 40 / 50, 512 53 / 24 and 100 / 59; 2048 x 2048, rank 16, 1024 rows 18 / 22 and 20 / 39.
+static int lr_forced = 0;                                    // for tests: 1 clusters, 2 tiles; 0: by the rule
+TGO_API void tgo_low_rank_force_way(int way) { lr_forced = way; }
+static bool lr_many(const LowRank& p) {
+    if (lr_forced) return lr_forced == 2;
+    return (long long)p.T * p.rank * ((long long)p.columns.slices * p.K + p.N) * 2 / LF_ROWS >= LR_TILE_BYTES;
+}
 
 template <typename T, typename TY> static int low_rank_any(const LowRank& p, float* u, cudaStream_t stream) {
     const int width = p.columns.slices * p.rank;
@@ -1191,19 +1250,20 @@ template <typename T, typename TY> static int low_rank_any(const LowRank& p, flo
                           p.out_stride);
 }
 
+#define LR_E_WORK 1001            // returned, nothing done: the workspace is too small
 // 32-bit numbers of workspace that a call needs.
 template <typename T, typename TY> static long long lr_work(const LowRank& p) {
     const int width = p.columns.slices * p.rank;
     if constexpr (sizeof(T) == 2)
-        if (p.T >= LR_TILE_ROWS && lr_tile_takes<TY>(p)) return lr_tile_work(p);
+        if (lr_many(p) && lr_tile_takes<TY>(p)) return lr_tile_work(p);
     if (lr_few_takes<T>(p)) return p.T > LR_SCAN_ROWS ? p.T + 1 + 3 * lr_tiles(p, LF_ROWS) : 0;
     return (long long)p.T * width;
 }
 
 template <typename T, typename TY> static int low_rank_launch(const LowRank& p, void* work, long long work_ints, cudaStream_t stream) {
-    if (work_ints < lr_work<T, TY>(p)) return TGO_E_BAD_ARG;
+    if (work_ints < lr_work<T, TY>(p)) return LR_E_WORK;
     if constexpr (sizeof(T) == 2)
-        if (p.T >= LR_TILE_ROWS && lr_tile_takes<TY>(p)) return low_rank_tiles<TY>(p, (int*)work, stream);
+        if (lr_many(p) && lr_tile_takes<TY>(p)) return low_rank_tiles<TY>(p, (int*)work, stream);
     if (lr_few_takes<T>(p)) return low_rank_few<T, TY>(p, (int*)work, stream);
     return low_rank_any<T, TY>(p, (float*)work, stream);
 }
@@ -1224,7 +1284,8 @@ TGO_API int tgo_low_rank_error(int* value) { return (int)cudaMemcpyFromSymbol(va
 
 // x [T, K] of type dt, y and out [T, N] of type dt_y, rows strided; out may be y. a [adapters, slices, rank, K],
 // b [adapters, N, rank] of type dt; ends: the column after each slice's last. `work` holds `work_ints` 32-bit
-// numbers and lies on 16 bytes; with `needs` given nothing runs, and it gets how many the call needs.
+// numbers and lies on 16 bytes; LR_E_WORK: too few (for up to 256 rows most calls need none). With `needs` given
+// nothing runs, and it gets how many the call needs.
 TGO_API int tgo_low_rank_add(const void* x, long long x_stride, const void* y, long long y_stride, void* out,
                              long long out_stride, const void* a, const void* b, const float* scale, const int* ids,
                              int dt, int dt_y, int T, int K, int N, int adapters, int rank, int slices, const int* ends,

@@ -20,6 +20,7 @@ from .build import entry_points, load_library
 F32, BF16 = 0, 1
 _CODES = {torch.float32: F32, torch.bfloat16: BF16}
 E_BAD_ARG = 1000
+E_WORK = 1001            # low_rank_add: the workspace is too small, nothing was done
 
 # What an entry point is handed (`entry_points`): whole numbers as they are (anything else refused),
 # single-precision numbers as floats, addresses as whole numbers.
@@ -2175,16 +2176,20 @@ def low_rank_add(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.Ten
     may be strided; a [adapters, slices, rank, K], b [adapters, N, rank] in x's type; scale float32
     [adapters]; ids int32 [T]. widths: the slices' columns, at most four slices (a joined matrix: q, k
     and v); `interleaved`: two slices of equal width that take turns, eight columns each."""
-    out = y if out is None else out
-    _need_cuda(x, y, a, b, scale, ids, out)
+    if out is None:
+        out = y
+    if not (x.is_cuda and y.is_cuda and a.is_cuda and b.is_cuda and scale.is_cuda and ids.is_cuda and out.is_cuda):
+        _need_cuda(x, y, a, b, scale, ids, out)
     T, K = x.shape
-    n, S, r, _ = a.shape
-    N = y.shape[1]
-    assert y.shape == out.shape == (T, N) and y.dtype == out.dtype and y.dtype in (x.dtype, torch.float32)
-    assert a.dtype == b.dtype == x.dtype and a.shape[3] == K and b.shape == (n, N, r) and S == len(widths)
-    assert a.is_contiguous() and b.is_contiguous() and x.stride(1) == y.stride(1) == out.stride(1) == 1
-    assert scale.dtype == torch.float32 and scale.shape == (n,) and scale.is_contiguous()
-    assert ids.dtype == torch.int32 and ids.shape == (T,) and ids.is_contiguous()
+    n, S, r, wide = a.shape
+    shape, kind, kind_y = y.shape, x.dtype, y.dtype
+    N = shape[1]
+    assert shape[0] == T and out.shape == shape and out.dtype == kind_y and (kind_y == kind or kind_y == torch.float32)
+    assert a.dtype == kind and b.dtype == kind and wide == K and b.shape == (n, N, r) and S == len(widths)
+    assert a.is_contiguous() and b.is_contiguous() and scale.is_contiguous() and ids.is_contiguous()
+    (xs, x1), (ys, y1), (os, o1) = x.stride(), y.stride(), out.stride()
+    assert x1 == y1 == o1 == 1 and scale.dtype == torch.float32 and scale.shape == (n,)
+    assert ids.dtype == torch.int32 and ids.shape == (T,)
     if sum(widths) != N or not 0 < S <= 4 or min(widths) <= 0 or \
             (interleaved and (S != 2 or widths[0] != widths[1] or widths[0] % 8)):
         raise KernelError(f"low_rank_add: slices {tuple(widths)}{' in eights' if interleaved else ''} of {N} columns")
@@ -2192,15 +2197,24 @@ def low_rank_add(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.Ten
         return
     ends = array("i", itertools.accumulate(widths))
     call = entry_points("adapters").tgo_low_rank_add
-    args = (_ptr(x), c_ll(x.stride(0)), _ptr(y), c_ll(y.stride(0)), _ptr(out), c_ll(out.stride(0)), _ptr(a), _ptr(b),
-            _ptr(scale), _ptr(ids), c_int(dtype_code(x.dtype)), c_int(dtype_code(y.dtype)), c_int(T), c_int(K), c_int(N),
-            c_int(n), c_int(r), c_int(S), c_ll(ends.buffer_info()[0]), c_int(1 if interleaved else 0))
-    needs = array("q", (0,))
-    status = call(*args, 0, 0, needs.buffer_info()[0], 0)
-    if status == 0:
-        work = torch.empty(needs[0], dtype=torch.int32, device=x.device) if needs[0] else None
-        status = call(*args, _ptr(work), needs[0], 0, _stream())
-    _check(status, "low_rank_add", f"(T={T}, K={K}, N={N}, rank={r}, slices={S})")
+    args = (x.data_ptr(), xs, y.data_ptr(), ys, out.data_ptr(), os, a.data_ptr(), b.data_ptr(), scale.data_ptr(),
+            ids.data_ptr(), dtype_code(kind), dtype_code(kind_y), T, K, N, n, r, S, ends.buffer_info()[0],
+            1 if interleaved else 0)
+    status = call(*args, 0, 0, 0, _stream())
+    if status == E_WORK:                    # a call that plans its rows: the workspace, and again
+        needs = array("q", (0,))
+        call(*args, 0, 0, needs.buffer_info()[0], 0)
+        work = torch.empty(needs[0], dtype=torch.int32, device=x.device)
+        status = call(*args, work.data_ptr(), needs[0], 0, _stream())
+    if status:
+        _check(status, "low_rank_add", f"(T={T}, K={K}, N={N}, rank={r}, slices={S})")
+    LAUNCHES[0] += 1
+
+
+def low_rank_force_way(way: int = 0) -> None:
+    """For tests and tuning: `low_rank_add` goes by clusters of eight rows (1) or, where they take the
+    call, by tiles of 128 (2) instead of choosing; 0 gives the choice back."""
+    load_library("adapters").tgo_low_rank_force_way(c_int(way))
 
 
 def low_rank_error() -> int:
