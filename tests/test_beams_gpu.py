@@ -16,6 +16,14 @@ def ops():
     return o
 
 
+@pytest.fixture(params=["chosen", "two kernels", "clusters"], autouse=True)
+def way(request):
+    """Every test goes the way that the framework chooses, and both of them wherever they take its call."""
+    ops().beam_force_way(["chosen", "two kernels", "clusters"].index(request.param))
+    yield request.param
+    ops().beam_force_way(0)
+
+
 def plain_values(logits, scores):
     """[B, W, V] in 64 bits on the CPU; -inf where the pair is no candidate."""
     B, W = scores.shape

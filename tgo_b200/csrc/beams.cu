@@ -10,17 +10,18 @@
 // a candidate get (-inf, -1, -1).
 //
 // Inside a row the order is that of x itself, so one pass over a row gives both what the normaliser
-// needs (a maximum and a sum per thread) and the row's K best. Blocks of the first kernel take a slice of a
-// row each: sixteen values a thread and turn, the next turn's already under way; a thread looks closer at
-// its values only when their largest, which the sum needs anyway, reaches the slice's K-th best so far. The
-// second kernel has a block a request: it joins the slices' maxima and sums and ranks what can be among the
-// K best. v is formed in 64 bits, so that close candidates of different beams are ordered by their values and
-// not by a rounding.
+// needs (a maximum and a sum per thread) and the row's K best. A request's blocks are shared out evenly among its beams
+// that live, a slice of a row each: sixteen values a thread and turn, the next turn's already under way; a thread looks
+// closer at its values only when their largest, which the sum needs anyway, reaches the slice's K-th best so far. Then one
+// block a request joins the slices' maxima and sums and ranks what can be among the K best: in a second kernel, or, for
+// few rows, in the first block of a cluster. v is formed in 64 bits, so that close candidates of different beams are ordered
+// by their values and not by a rounding.
 //
-// MEASURED (B200): 512 rows of 151936 and 16 picks 58 us, 5.4 TB/s; without looking for candidates the same
+// MEASURED (B200): 512 rows of 151936 and 16 picks 57 us, 5.4 TB/s; without looking for candidates the same
 // pass takes 50, with a look only every fourth turn, at values read again, 64, from a ring filled by bulk
-// copies 66, with warps that meet only when one has found enough 65. 64 rows of it 15.7 us, 4 rows of 32768 8.0: there
-// the two kernels' latencies, about 4 and 3 us, and the first turns' many candidates.
+// copies 66, with warps that meet only when one has found enough 65. 64 rows of it 15.6 us; one live beam of five in 12
+// requests 10.4 (13.8 where the others' blocks find nothing to do); 4 rows of 32768 7.8. There the kernels' latencies
+// show, about 4 and 3 us, and the first turns' many candidates.
 #define BS_THREADS 256
 #define BS_VPT 4                  // vectors of four values a thread and turn
 #define BS_TILE (BS_THREADS * BS_VPT)       // vectors a turn
@@ -78,23 +79,36 @@ __device__ void bs_cut(const unsigned long long* kept, int k, unsigned long long
         // the K-th largest by its bits, eight at a time, then the keys from it on to the front
         __shared__ unsigned long long prefix_s;
         __shared__ int left_s, front_s;
+        __shared__ int warp_sums[BS_WARPS];
+        static_assert(BS_THREADS == 256, "a thread a bin");
         if (t < k) buf[n + t] = kept[t];
         n += k;
         k = 0;
         if (t == 0) { prefix_s = 0; left_s = K; front_s = 0; }
         for (int shift = 56; shift >= 0; shift -= 8) {
-            for (int i = t; i < 256; i += BS_THREADS) hist[i] = 0;
+            hist[t] = 0;
             __syncthreads();
             const unsigned long long prefix = prefix_s;
+            const int left = left_s;
             for (int i = t; i < n; i += BS_THREADS)
                 if (shift == 56 || (buf[i] >> (shift + 8)) == (prefix >> (shift + 8)))
                     atomicAdd(&hist[(unsigned)(buf[i] >> shift) & 255u], 1u);
             __syncthreads();
-            if (t == 0) {
-                int left = left_s, b = 255;
-                for (; b > 0 && (int)hist[b] < left; --b) left -= hist[b];
-                prefix_s = prefix | ((unsigned long long)b << shift);
-                left_s = left;
+            // keys in this thread's bin, the bins above it and this one, counted from the top
+            const int bin = 255 - t, mine = (int)hist[bin];
+            int sum = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int below = __shfl_up_sync(0xffffffffu, sum, o);
+                sum += (t & 31) >= o ? below : 0;
+            }
+            if ((t & 31) == 31) warp_sums[t >> 5] = sum;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < BS_WARPS; ++w) sum += w < t >> 5 ? warp_sums[w] : 0;
+            if (sum >= left && sum - mine < left) {          // one thread's
+                prefix_s = prefix | ((unsigned long long)bin << shift);
+                left_s = left - (sum - mine);
             }
             __syncthreads();
         }
@@ -115,29 +129,21 @@ __device__ void bs_cut(const unsigned long long* kept, int k, unsigned long long
     if (t < k + n && rank < K) to[rank] = mine;
 }
 
-__global__ void __launch_bounds__(BS_THREADS, BS_BLOCKS)
-beam_part_kernel(const float* __restrict__ logits, long long stride, int V, const float* __restrict__ scores, int K,
-                 int parts, int turns, float2* __restrict__ sums, unsigned long long* __restrict__ lists) {
-    __shared__ unsigned long long buf[4 * BS_TILE + 4 * BS_MAX_K];
+// The block's slice `part` of `parts` even ones of a row x of V values: its K best to `list`, descending (0: none), its maximum and sum to `sum`.
+// buf has BS_BUF numbers of shared memory.
+#define BS_BUF (4 * BS_TILE + 4 * BS_MAX_K)
+__device__ __forceinline__ void bs_scan(const float* __restrict__ x, int V, int K, int part, int parts, unsigned long long* buf,
+                                        float2* sum, unsigned long long* list) {
     __shared__ unsigned long long kept[2][BS_MAX_K];
     __shared__ unsigned hist[256];
     __shared__ float2 red[BS_WARPS];
     __shared__ int counts[2];         // candidates in buf; the other one is set to 0 meanwhile
     __shared__ unsigned warp_least[BS_WARPS];
-    pdl_wait();
-    const int row = blockIdx.y, part = blockIdx.x, t = threadIdx.x, warp = t >> 5, lane = t & 31;
-    unsigned long long* const list = lists + ((size_t)row * parts + part) * K;
-    const float score = scores[row];
-    if (!(score > -INFINITY && score < INFINITY)) {          // the same for the whole block
-        if (t < K) list[t] = 0;
-        if (t == 0) sums[(size_t)row * parts + part] = make_float2(-INFINITY, 0.f);
-        return;
-    }
-    const float* const x = logits + (size_t)row * stride;
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
     // vectors lie on 16-byte boundaries: vector v holds the row's values 4 v - off .. 4 v - off + 3
     const int off = (int)(((uintptr_t)x >> 2) & 3);
     const int vectors = (V + off + 3) / 4;
-    const int v0 = part * turns * BS_TILE, v1 = min(v0 + turns * BS_TILE, vectors);
+    const int share = (int)((unsigned)(vectors + parts - 1) / (unsigned)parts), v0 = min(part * share, vectors), v1 = min(v0 + share, vectors);
     if (t < 2) counts[t] = 0;
 
     float4 next[BS_VPT];
@@ -154,7 +160,8 @@ beam_part_kernel(const float* __restrict__ logits, long long stride, int V, cons
         for (int j = 0; j < BS_VPT; ++j) {
             const int v = base + j * BS_THREADS + t, e = 4 * v - off;
             float4 q = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-            if (v < v1) {
+            if (v >= v_head && v < v_tail) q = __ldcs((const float4*)(at_v + 4 * (size_t)v));
+            else if (v < v1) {
                 if (e >= 0 && e < V) q.x = x[e];
                 if (e + 1 >= 0 && e + 1 < V) q.y = x[e + 1];
                 if (e + 2 >= 0 && e + 2 < V) q.z = x[e + 2];
@@ -274,13 +281,53 @@ beam_part_kernel(const float* __restrict__ logits, long long stride, int V, cons
     if (t == 0) {
         float bm = red[0].x;
         for (int i = 1; i < BS_WARPS; ++i) bm = fmaxf(bm, red[i].x);
-        float sum = 0.f;
-        for (int i = 0; i < BS_WARPS; ++i) sum += red[i].x > -INFINITY ? red[i].y * bs_exp(red[i].x - bm) : red[i].y;
-        sums[(size_t)row * parts + part] = make_float2(bm, sum);
+        float all = 0.f;
+        for (int i = 0; i < BS_WARPS; ++i) all += red[i].x > -INFINITY ? red[i].y * bs_exp(red[i].x - bm) : red[i].y;
+        *sum = make_float2(bm, all);
     }
 }
 
-// One block a request. (m, s) of a slice: its values' exp(x - m) sum to s; a NaN or +inf among them has
+// How a request's blocks are shared out: evenly among the beams that live, those whose score is finite, and no finer than
+// a turn a block. (A search's first step has one beam of each request.)
+struct BeamShare {
+    unsigned lives;                                          // a bit a beam
+    int live, parts;
+    float score;                                             // of the beam of this lane's number (any for a lane past them)
+    // a / b for both up to 256: the quotient of a + 1/2 is 1/512 or more from a whole number
+    __device__ __forceinline__ static int divide(int a, int b) { return (int)__fdividef((float)a + 0.5f, (float)b); }
+    __device__ __forceinline__ BeamShare(float mine, int W, int V, int blocks) : score(mine) {
+        const int lane = threadIdx.x & 31, turns = (V + 3 + 4 * BS_TILE - 1) / (4 * BS_TILE);
+        lives = __ballot_sync(0xffffffffu, lane < W && score > -INFINITY && score < INFINITY);
+        live = __popc(lives);
+        parts = live ? min(divide(blocks, live), turns) : 0;
+    }
+    // The j-th beam that lives.
+    __device__ __forceinline__ int beam(int j) const {
+        const int lane = threadIdx.x & 31;
+        return __ffs(__ballot_sync(0xffffffffu, (lives >> lane & 1) && __popc(lives & ((1u << lane) - 1)) == j)) - 1;
+    }
+    // Block `block` of the request does its part, if it has one.
+    __device__ __forceinline__ void scan(const float* logits, long long stride, size_t row, int V, int K, int block, unsigned long long* buf,
+                                         float2* sum, unsigned long long* list) const {
+        if (block >= live * parts) return;
+        const int j = divide(block, parts);
+        const float* const x = logits + (row + beam(j)) * stride;
+        bs_scan(x, V, K, block - j * parts, parts, buf, sum, list);
+    }
+};
+__device__ __forceinline__ float bs_score(const float* scores, int W) { return (threadIdx.x & 31) < W ? scores[threadIdx.x & 31] : 0.f; }
+
+__global__ void __launch_bounds__(BS_THREADS, BS_BLOCKS)
+beam_part_kernel(const float* __restrict__ logits, long long stride, int V, const float* __restrict__ scores, int W, int K,
+                 float2* __restrict__ sums, unsigned long long* __restrict__ lists) {
+    __shared__ unsigned long long buf[BS_BUF];
+    pdl_wait();
+    const int block = blockIdx.x, blocks = gridDim.x;
+    const size_t b = blockIdx.y, at = b * blocks + block;
+    BeamShare(bs_score(scores + b * W, W), W, V, blocks).scan(logits, stride, b * W, V, K, block, buf, sums + at, lists + at * K);
+}
+
+// The block joins a request's slices. (m, s) of a slice: its values' exp(x - m) sum to s; a NaN or +inf among them has
 // made s NaN, a slice of -inf alone has m = -inf and s = 0. The slices' lists are sorted: the K-th best of
 // their first candidates (as many of each as make 3 K) bounds what can be among the K best, at most K lists
 // reach it, and what reaches it is ranked by counting.
@@ -308,26 +355,26 @@ __device__ __forceinline__ int bm_rank(const Pick* from, int n, const Pick& p) {
     return rank;
 }
 
-__global__ void __launch_bounds__(BM_THREADS)
-beam_merge_kernel(const float* __restrict__ scores, int W, int K, int parts, const float2* __restrict__ sums,
-                  const unsigned long long* __restrict__ lists, float* __restrict__ picked, int* __restrict__ parents,
-                  int* __restrict__ tokens) {
-    extern __shared__ __align__(16) unsigned char bm_smem[];
+// lists [live * parts][K] and sums [live * parts]; `first`: the lists' number of this thread; `room`: as much shared memory as beam_merge_bytes says.
+__device__ __forceinline__ void bm_join(const BeamShare& share, int K, const float2* sums,
+                                        const unsigned long long* lists, unsigned long long first,
+                                        unsigned char* room, float* picked, int* parents, int* tokens) {
     __shared__ double base_s[BS_MAX_BEAMS];                  // score - ln s, or NaN: the beam gives nothing
     __shared__ float max_s[BS_MAX_BEAMS];
+    __shared__ int beam_s[BS_MAX_BEAMS];
     __shared__ Pick bound_s;
     __shared__ int count;
-    pdl_wait();
-    const int b = blockIdx.x, t = threadIdx.x, warp = t >> 5, lane = t & 31, n = W * parts;
-    const int q = min((3 * K + n - 1) / n, K);               // a list's heads
-    Pick* const all = (Pick*)bm_smem;                        // [n][K]
+    const int W = share.live, parts = share.parts;
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, n = W * parts;
+    const int q = n ? min((3 * K + n - 1) / n, K) : 0;       // a list's heads
+    Pick* const all = (Pick*)room;                           // [n][K]
     Pick* const heads = all + n * K;                         // [n][q]
     Pick* const found = heads + n * q;                       // [n][K]
     if (t == 0) { count = 0; bound_s = Pick{0, 0}; }
-    const unsigned long long first = t < n * K ? lists[(size_t)b * n * K + t] : 0;
     for (int w = warp; w < W; w += BM_THREADS / 32) {
-        const float2* row = sums + ((size_t)b * W + w) * parts;
-        const float score = scores[b * W + w];
+        const float2* row = sums + w * parts;
+        const int beam = share.beam(w);
+        const float score = __shfl_sync(0xffffffffu, share.score, beam);
         float m = -INFINITY;
         for (int p = lane; p < parts; p += 32) m = fmaxf(m, row[p].x);
         m = warp_max(m);
@@ -341,17 +388,18 @@ beam_merge_kernel(const float* __restrict__ scores, int W, int K, int parts, con
         if (lane == 0) {
             base_s[w] = s > 0.f && s < INFINITY && m < INFINITY ? base : __longlong_as_double(0x7ff8000000000000ll);
             max_s[w] = m;
+            beam_s[w] = beam;
         }
     }
     __syncthreads();
     for (int e = t; e < n * K; e += BM_THREADS) {
-        const unsigned long long key = e == t ? first : lists[(size_t)b * n * K + e];
+        const unsigned long long key = e == t ? first : lists[e];
         const int l = e / K, i = e - l * K, w = l / parts;
         const double base = base_s[w];
         Pick p = {0, 0};                                     // nothing
         if (key && base == base) {
             p.v = bm_order(base + ((double)bs_value((uint32_t)(key >> 32)) - (double)max_s[w]));
-            p.place = ~(((unsigned long long)w << 32) | (0xffffffffu - (uint32_t)key));
+            p.place = ~(((unsigned long long)beam_s[w] << 32) | (0xffffffffu - (uint32_t)key));
         }
         all[e] = p;
         if (i < q) heads[l * q + i] = p;
@@ -369,40 +417,88 @@ beam_merge_kernel(const float* __restrict__ scores, int W, int K, int parts, con
     }
     __syncthreads();
     const int c = count;
-    const size_t out = (size_t)b * K;
     for (int e = t; e < c; e += BM_THREADS) {
         const Pick p = found[e];
         const int rank = bm_rank(found, c, p);
         if (rank < K) {
-            picked[out + rank] = (float)bm_value(p.v);
-            parents[out + rank] = (int)(~p.place >> 32);
-            tokens[out + rank] = (int)(uint32_t)~p.place;
+            picked[rank] = (float)bm_value(p.v);
+            parents[rank] = (int)(~p.place >> 32);
+            tokens[rank] = (int)(uint32_t)~p.place;
         }
     }
     for (int k = c + t; k < K; k += BM_THREADS) {
-        picked[out + k] = -INFINITY;
-        parents[out + k] = tokens[out + k] = -1;
+        picked[k] = -INFINITY;
+        parents[k] = tokens[k] = -1;
     }
 }
 
-// Bytes of its shared memory: candidates, heads, and those that reach the bound.
-static size_t beam_merge_bytes(int lists, int K) {
-    const int q = (3 * K + lists - 1) / lists < K ? (3 * K + lists - 1) / lists : K;
-    return (size_t)lists * (2 * K + q) * sizeof(Pick);
+__global__ void __launch_bounds__(BM_THREADS)
+beam_merge_kernel(const float* __restrict__ scores, int V, int W, int K, int blocks, const float2* __restrict__ sums,
+                  const unsigned long long* __restrict__ lists, float* __restrict__ picked, int* __restrict__ parents,
+                  int* __restrict__ tokens) {
+    extern __shared__ __align__(16) unsigned char bm_smem[];
+    __shared__ float2 sum_s[BM_LISTS];
+    pdl_wait();
+    const size_t b = blockIdx.x;
+    lists += b * blocks * K;
+    const int t = threadIdx.x;
+    static_assert(BM_LISTS == BM_THREADS, "a thread a sum");
+    const float score = bs_score(scores + b * W, W);         // these three at once
+    const unsigned long long first = t < blocks * K ? lists[t] : 0;
+    if (t < blocks) sum_s[t] = sums[b * blocks + t];
+    const BeamShare share(score, W, V, blocks);
+    __syncthreads();
+    bm_join(share, K, sum_s, lists, first, bm_smem, picked + b * K, parents + b * K, tokens + b * K);
+}
+
+// Bytes of shared memory to join up to so many lists: candidates, heads (at most 3 K - 1 and one a list), and those that
+// reach the bound.
+__host__ __device__ static constexpr size_t beam_merge_bytes(int lists, int K) {
+    return ((size_t)lists * (2 * K + 1) + 3 * K - 1) * sizeof(Pick);
+}
+
+// Both at once: a cluster of sixteen blocks a request; the slices' sums and lists go to the first block's shared memory,
+// which joins them.
+#define BC_BLOCKS 16
+#define BC_ROOM (beam_merge_bytes(BC_BLOCKS, BS_MAX_K) > BS_BUF * 8 ? beam_merge_bytes(BC_BLOCKS, BS_MAX_K) : BS_BUF * 8)
+
+template <typename T> __device__ __forceinline__ T* bc_first(T* mine) {      // the first block's
+    T* theirs;
+    asm("mapa.u64 %0, %1, 0;" : "=l"(theirs) : "l"(mine));
+    return theirs;
+}
+
+__global__ void __launch_bounds__(BS_THREADS, BS_BLOCKS)
+beam_cluster_kernel(const float* __restrict__ logits, long long stride, int V, const float* __restrict__ scores, int W, int K,
+                    float* __restrict__ picked, int* __restrict__ parents, int* __restrict__ tokens) {
+    __shared__ __align__(16) unsigned char room[BC_ROOM];    // the scan's buffer, then what joining takes
+    __shared__ unsigned long long lists[BC_BLOCKS * BS_MAX_K];
+    __shared__ float2 sums[BC_BLOCKS];
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+    pdl_wait();
+    const int block = blockIdx.x % BC_BLOCKS;
+    const size_t b = blockIdx.x / BC_BLOCKS;
+    const BeamShare share(bs_score(scores + b * W, W), W, V, BC_BLOCKS);
+    asm volatile("barrier.cluster.wait;" ::: "memory");      // the first block is there
+    share.scan(logits, stride, b * W, V, K, block, (unsigned long long*)room, bc_first(sums + block), bc_first(lists + block * K));
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    if (block == 0) bm_join(share, K, sums, lists, threadIdx.x < BC_BLOCKS * BS_MAX_K ? lists[threadIdx.x] : 0, room, picked + b * K, parents + b * K, tokens + b * K);
 }
 
 // Slices of a row: the count that is cheapest by a small model. The blocks run in rounds of four a multiprocessor; a
 // block costs a unit a turn and three to begin and end.
-static void beam_plan(int rows, int W, int V, int K, int sms, int* turns, int* parts) {
+static int beam_parts(int rows, int W, int V, int K, int sms) {
     const int tiles = (V + 3 + 4 * BS_TILE - 1) / (4 * BS_TILE);
     const int most = BM_CANDIDATES / (W * K) < BM_LISTS / W ? BM_CANDIDATES / (W * K) : BM_LISTS / W;
     long long best = -1;
+    int turns = tiles;
     for (int p = 1; p <= most && p <= tiles; ++p) {
         const int n = (tiles + p - 1) / p;
         const long long rounds = ((long long)rows * p + BS_BLOCKS * sms - 1) / (BS_BLOCKS * sms), cost = rounds * (n + 3);
-        if (best < 0 || cost < best) { best = cost; *turns = n; }
+        if (best < 0 || cost < best) { best = cost; turns = n; }
     }
-    *parts = (tiles + *turns - 1) / *turns;
+    return (tiles + turns - 1) / turns;
 }
 
 static bool beam_takes(int requests, int beams, int V, int K) {
@@ -410,43 +506,78 @@ static bool beam_takes(int requests, int beams, int V, int K) {
            (long long)requests * beams <= 65535;
 }
 
-// Slices of a row that tgo_beam_select works with (0: it refuses these sizes): it needs rows x slices x (1 + K)
-// 64-bit numbers of workspace.
-TGO_API int tgo_beam_select_parts(int requests, int beams, int V, int K) {
-    if (!beam_takes(requests, beams, V, K)) return 0;
-    int turns, parts;
-    beam_plan(requests * beams, beams, V, K, tgo_multiprocessors(), &turns, &parts);
-    return parts;
+static int beam_cluster(const float* logits, long long stride, const float* scores, int requests, int beams, int V, int K, float* picked,
+                        int* parents, int* tokens, int dev, cudaStream_t stream) {
+    static bool sized[64] = {};                              // per device
+    if (!sized[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(beam_cluster_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return (int)e;
+        sized[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)requests * BC_BLOCKS);
+    cfg.blockDim = dim3(BS_THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = BC_BLOCKS;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = tgo_pdl_enabled() ? 2 : 1;
+    return (int)cudaLaunchKernelEx(&cfg, beam_cluster_kernel, logits, stride, V, scores, beams, K, picked, parents, tokens);
+}
+
+static int beam_forced = 0;                                  // for tests: 1 two kernels, 2 clusters; 0: by the rule
+TGO_API void tgo_beam_force_way(int way) { beam_forced = way; }
+// Whether a call goes by clusters: one launch and no workspace, 5.5 us of the host's time where two kernels take 10, but only
+// sixteen blocks a request. So where two turns of each are enough and no multiprocessor has more than two blocks. MEASURED
+// (us on the device, clusters / two kernels), 32768 tokens: 1 x 1 beams 6.1 / 6.6, 1 x 4 7.7 / 8.1, 16 x 4 9.0 / 9.8, 32 x 4 13.5 /
+// 11.5, 16 x 5 (three turns) 10.9 / 10.6, 1 x 8 10.6 / 10.4; 151936 tokens: 1 x 1 (three turns) 8.2 / 7.4, 1 x 4 13.9 / 11.3.
+static bool beam_by_clusters(int requests, int beams, int V) {
+    if (beams > BC_BLOCKS) return false;
+    if (beam_forced) return beam_forced == 2;
+    const int parts = BC_BLOCKS / beams, tiles = (V + 4 * BS_TILE - 1) / (4 * BS_TILE);
+    return requests * BC_BLOCKS <= 2 * tgo_multiprocessors() && (tiles + parts - 1) / parts <= 2;
+}
+
+// 64-bit numbers of workspace that a call needs (a call by clusters none); a refused one 0.
+TGO_API int tgo_beam_select_work(int requests, int beams, int V, int K) {
+    if (!beam_takes(requests, beams, V, K) || beam_by_clusters(requests, beams, V)) return 0;
+    const long long n = (long long)requests * beams * beam_parts(requests * beams, beams, V, K, tgo_multiprocessors()) * (1 + K);
+    return n > 0x7fffffff ? 0 : (int)n;
 }
 
 // picked, parents, tokens [requests, K]; scores [requests, beams]; logits rows `stride` floats apart, beams of
-// a request one after the other. `work` has `parts` slices' room for each row, parts as above.
+// a request one after the other. `work`: as above, `work_longs` of them.
 TGO_API int tgo_beam_select(const float* logits, long long stride, const float* scores, int requests, int beams, int V,
-                            int K, float* picked, int* parents, int* tokens, void* work, int parts, cudaStream_t stream) {
+                            int K, float* picked, int* parents, int* tokens, void* work, int work_longs,
+                            cudaStream_t stream) {
     if (requests <= 0) return 0;
     if (!beam_takes(requests, beams, V, K)) return TGO_E_BAD_ARG;
     static bool sized[64] = {};                              // per device
-    int dev = 0, turns, mine;
+    int dev = 0;
     const cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return (int)err;
     if (dev < 0 || dev >= 64) return TGO_E_BAD_ARG;
+    if (beam_by_clusters(requests, beams, V))
+        return beam_cluster(logits, stride, scores, requests, beams, V, K, picked, parents, tokens, dev, stream);
+    const int blocks = beams * beam_parts(requests * beams, beams, V, K, tgo_multiprocessors());       // of a request
+    if (work_longs < (long long)requests * blocks * (1 + K)) return TGO_E_BAD_ARG;
     if (!sized[dev]) {
         const cudaError_t e = cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                    200 * 1024);
         if (e != cudaSuccess) return (int)e;
         sized[dev] = true;
     }
-    beam_plan(requests * beams, beams, V, K, tgo_multiprocessors(), &turns, &mine);
-    if (mine != parts) return TGO_E_BAD_ARG;
-    const int rows = requests * beams, lists_of = beams * parts;
     float2* sums = (float2*)work;
-    unsigned long long* lists = (unsigned long long*)(sums + (size_t)rows * parts);
-    const int rc = tgo_launch_pdl(beam_part_kernel, dim3(parts, rows), dim3(BS_THREADS), 0, stream, logits, stride, V,
-                                  scores, K, parts, turns, sums, lists);
+    unsigned long long* lists = (unsigned long long*)(sums + (size_t)requests * blocks);
+    const int rc = tgo_launch_pdl(beam_part_kernel, dim3(blocks, requests), dim3(BS_THREADS), 0, stream, logits, stride, V,
+                                  scores, beams, K, sums, lists);
     if (rc) return rc;
-    return tgo_launch_pdl(beam_merge_kernel, dim3(requests), dim3(BM_THREADS),
-                          beam_merge_bytes(lists_of, K), stream, scores, beams, K, parts,
-                          (const float2*)sums, (const unsigned long long*)lists, picked, parents, tokens);
+    return tgo_launch_pdl(beam_merge_kernel, dim3(requests), dim3(BM_THREADS), beam_merge_bytes(blocks, K), stream, scores, V, beams, K,
+                          blocks, (const float2*)sums, (const unsigned long long*)lists, picked, parents, tokens);
 }
 
 // ------------------------------------------------------------------------ reorder_rows

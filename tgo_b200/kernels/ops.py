@@ -20,7 +20,8 @@ from .build import entry_points, load_library
 F32, BF16 = 0, 1
 _CODES = {torch.float32: F32, torch.bfloat16: BF16}
 E_BAD_ARG = 1000
-E_WORK = 1001            # low_rank_add: the workspace is too small, nothing was done
+E_WORK = 1001            # the workspace is too small, nothing was done
+LOW_RANK_SCANNED = 256   # rows up to which low_rank_add's kernels find each adapter's rows themselves
 
 # What an entry point is handed (`entry_points`): whole numbers as they are (anything else refused),
 # single-precision numbers as floats, addresses as whole numbers.
@@ -2111,25 +2112,35 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, picked: torch.Tensor
     and tokens int32, [B, K], K at most 64, W at most 32. A token at -inf is no candidate, nor is
     any token of a beam whose score is not finite or whose logits hold a NaN, +inf or nothing but
     -inf; a place that no candidate fills gets (-inf, -1, -1)."""
-    _need_cuda(logits, scores, picked, parents, tokens)
+    if not (logits.is_cuda and scores.is_cuda and picked.is_cuda and parents.is_cuda and tokens.is_cuda):
+        _need_cuda(logits, scores, picked, parents, tokens)
     B, W = scores.shape
-    K = picked.shape[1]
-    assert logits.dim() == 2 and logits.shape[0] == B * W and logits.dtype == torch.float32 and logits.stride(1) == 1
+    shape = picked.shape
+    K = shape[1]
+    rows, V = logits.shape
+    stride, step = logits.stride()
+    assert rows == B * W and logits.dtype == torch.float32 and step == 1
     assert scores.dtype == picked.dtype == torch.float32 and parents.dtype == tokens.dtype == torch.int32
-    assert picked.shape == parents.shape == tokens.shape == (B, K)
+    assert shape[0] == B and parents.shape == shape and tokens.shape == shape
     assert scores.is_contiguous() and picked.is_contiguous() and parents.is_contiguous() and tokens.is_contiguous()
     if not 0 < K <= BEAM_MAX_PICKS or not 0 < W <= BEAM_MAX:
         raise KernelError(f"beam_select: {W} beams and {K} continuations; at most {BEAM_MAX} and {BEAM_MAX_PICKS}")
     if B == 0:
         return
-    V = logits.shape[1]
     lib = entry_points("beams")
-    parts = lib.tgo_beam_select_parts(c_int(B), c_int(W), c_int(V), c_int(K))
-    work = torch.empty(B * W * parts * (1 + K), dtype=torch.int64, device=logits.device)
-    _check(lib.tgo_beam_select(_ptr(logits), c_ll(logits.stride(0)), _ptr(scores), c_int(B), c_int(W), c_int(V),
-                               c_int(K), _ptr(picked), _ptr(parents), _ptr(tokens), _ptr(work), c_int(parts),
-                               _stream()), "beam_select", f"(B={B}, W={W}, V={V}, K={K})")
-    LAUNCHES[0] += 1
+    needs = lib.tgo_beam_select_work(B, W, V, K)
+    work = logits.new_empty(needs, dtype=torch.int64) if needs else None     # between two kernels
+    _check(lib.tgo_beam_select(logits.data_ptr(), stride, scores.data_ptr(), B, W, V, K, picked.data_ptr(), parents.data_ptr(),
+                               tokens.data_ptr(), work.data_ptr() if needs else 0, needs, _stream()), "beam_select",
+           f"(B={B}, W={W}, V={V}, K={K})")
+    if needs:
+        LAUNCHES[0] += 1
+
+
+def beam_force_way(way: int = 0) -> None:
+    """For tests and tuning: `beam_select` runs its two kernels (1) or, for up to 16 beams, a cluster a
+    request (2) instead of choosing; 0 gives the choice back."""
+    load_library("beams").tgo_beam_force_way(c_int(way))
 
 
 def reorder_rows(tensors, index: torch.Tensor, parents: torch.Tensor, axis: int = 0) -> None:
@@ -2139,29 +2150,32 @@ def reorder_rows(tensors, index: torch.Tensor, parents: torch.Tensor, axis: int 
     before `axis` is gone through row by row. index, parents int32 [groups, W], W at most 32; the
     rows named by a call are distinct. A row whose parent is itself or outside 0..W-1, or that is
     or continues a row outside the tensor, stays as it is."""
-    _need_cuda(index, parents, *tensors)
-    G, W = index.shape
-    assert index.dtype == parents.dtype == torch.int32 and parents.shape == index.shape
+    if not (index.is_cuda and parents.is_cuda):
+        _need_cuda(index, parents)
+    shape = index.shape
+    G, W = shape
+    assert index.dtype == parents.dtype == torch.int32 and parents.shape == shape
     assert index.is_contiguous() and parents.is_contiguous()
     if not 0 < W <= BEAM_MAX:
         raise KernelError(f"reorder_rows: groups of {W} rows; at most {BEAM_MAX}")
     desc = array("q")
     for t in tensors:
-        if t.numel() == 0:
+        if not t.is_cuda:
+            _need_cuda(t)
+        shape, size = t.shape, t.element_size()
+        assert 0 <= axis < len(shape) and size >= 2
+        outer, rows = math.prod(shape[:axis]), shape[axis]
+        row = math.prod(shape[axis + 1:]) * size
+        if outer == 0 or rows == 0 or row == 0:
             continue
-        assert 0 <= axis < t.dim() and t.element_size() >= 2
-        outer, rows = math.prod(t.shape[:axis]), t.shape[axis]
-        size = t.element_size()
-        row = math.prod(t.shape[axis + 1:]) * size
-        step = t.stride(axis) * size if rows > 1 else row
+        step = t.stride()[axis] * size if rows > 1 else row
         # whole rows, and whatever precedes the rows evenly spaced
         assert t.is_contiguous() or (axis == 0 and t[0].is_contiguous() and step >= row)
         desc.extend((t.data_ptr(), outer, rows * step, rows, step, row))
     if not desc or G == 0:
         return
-    lib = entry_points("beams")
-    _check(lib.tgo_reorder_rows(c_ll(desc.buffer_info()[0]), c_int(len(desc) // 6), _ptr(index), _ptr(parents),
-                                c_int(G), c_int(W), _stream()), "reorder_rows")
+    _check(entry_points("beams").tgo_reorder_rows(desc.buffer_info()[0], len(desc) // 6, index.data_ptr(), parents.data_ptr(),
+                                                  G, W, _stream()), "reorder_rows")
     LAUNCHES[0] += (len(desc) // 6 - 1) // 64
 
 
@@ -2200,15 +2214,19 @@ def low_rank_add(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.Ten
     args = (x.data_ptr(), xs, y.data_ptr(), ys, out.data_ptr(), os, a.data_ptr(), b.data_ptr(), scale.data_ptr(),
             ids.data_ptr(), dtype_code(kind), dtype_code(kind_y), T, K, N, n, r, S, ends.buffer_info()[0],
             1 if interleaved else 0)
-    status = call(*args, 0, 0, 0, _stream())
-    if status == E_WORK:                    # a call that plans its rows: the workspace, and again
-        needs = array("q", (0,))
-        call(*args, 0, 0, needs.buffer_info()[0], 0)
-        work = torch.empty(needs[0], dtype=torch.int32, device=x.device)
-        status = call(*args, work.data_ptr(), needs[0], 0, _stream())
-    if status:
-        _check(status, "low_rank_add", f"(T={T}, K={K}, N={N}, rank={r}, slices={S})")
-    LAUNCHES[0] += 1
+    if T <= LOW_RANK_SCANNED:               # most such calls need no workspace
+        status = call(*args, 0, 0, 0, _stream())
+        if status == E_WORK:
+            needs = array("q", (0,))
+            call(*args, 0, 0, needs.buffer_info()[0], 0)
+            work = x.new_empty(needs[0], dtype=torch.int32)
+            status = call(*args, work.data_ptr(), needs[0], 0, _stream())
+    else:                                   # a plan of the rows (four numbers a row and a few) and at most u
+        needs = T * (S * ((r + 15) // 16 * 16) + 4) + 8
+        work = x.new_empty(needs, dtype=torch.int32)
+        status = call(*args, work.data_ptr(), needs, 0, _stream())
+        LAUNCHES[0] += 1
+    _check(status, "low_rank_add", f"(T={T}, K={K}, N={N}, rank={r}, slices={S})" if status else "")
 
 
 def low_rank_force_way(way: int = 0) -> None:
