@@ -249,6 +249,17 @@ def test_reorder(dtype, W, row):
     run_reorder([t], index, some_parents(G, W, seed=row), 0)
 
 
+@pytest.mark.parametrize("dtype,W,row", [(torch.float32, 4, 75004), (torch.float32, 3, 74001), (torch.bfloat16, 16, 4999),
+                                         (torch.bfloat16, 4, 140002)])
+def test_reorder_of_large_rows(dtype, W, row):
+    """So many rows, and so large, that a block goes through several pieces of them."""
+    g = torch.Generator().manual_seed(row)
+    groups, outer = (64 if W == 16 else 16), 4
+    t = torch.randn(outer, groups * W + 3, row, generator=g).to(dtype).to(DEV)
+    index = torch.randperm(groups * W + 3, generator=g)[:groups * W].view(groups, W).to(torch.int32)
+    run_reorder([t], index, some_parents(groups, W, row), axis=1)
+
+
 def test_reorder_of_many_tensors_of_unlike_rows():
     g = torch.Generator().manual_seed(5)
     tensors = [torch.randn(9, 1 + 37 * i % 211, generator=g).to(torch.float32 if i % 3 else torch.bfloat16).to(DEV)

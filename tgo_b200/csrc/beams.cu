@@ -596,15 +596,18 @@ struct ReorderRows {
     int outer[RR_MAX_TENSORS];
 };
 
-template <typename VEC, int W>
+template <typename VEC, int W, bool AHEAD>
 __global__ void __launch_bounds__(RR_THREADS)
 reorder_rows_kernel(const __grid_constant__ ReorderRows d, const int* __restrict__ index, const int* __restrict__ parents,
-                    int beams) {
+                    int beams, int run) {
     __shared__ long long to[RR_MAX_BEAMS], from[RR_MAX_BEAMS];       // byte offsets; from < 0: the row stays
     pdl_wait();
     const int k = blockIdx.z, g = blockIdx.y, t = threadIdx.x;
-    const long long vectors = d.row_bytes[k] / (long long)sizeof(VEC), chunks = (vectors + RR_THREADS - 1) / RR_THREADS;
-    if (blockIdx.x >= chunks * d.outer[k]) return;
+    const long long vectors = d.row_bytes[k] / (long long)sizeof(VEC);
+    // pieces of RR_THREADS vectors of a row of every outer block, one after the other
+    const int pieces = (int)((vectors + RR_THREADS - 1) / RR_THREADS), last = min((int)blockIdx.x * run + run, pieces * d.outer[k]);
+    int i = blockIdx.x * run;
+    if (i >= last) return;
     bool moves = false;
     if (t < beams) {
         const int p = parents[(size_t)g * beams + t];
@@ -615,27 +618,65 @@ reorder_rows_kernel(const __grid_constant__ ReorderRows d, const int* __restrict
         from[t] = moves ? q * d.row_stride[k] : -1;
     }
     if (!__syncthreads_or(moves)) return;
-    const int o = (int)(blockIdx.x / chunks);
-    const long long v = (blockIdx.x - o * chunks) * RR_THREADS + t;
-    if (v >= vectors) return;
-    char* const base = d.base[k] + o * d.outer_stride[k] + v * (long long)sizeof(VEC);
-    VEC got[W];
+    int o = i / pieces, c = i - o * pieces;
+    VEC got[AHEAD ? 2 : 1][W];
+    char* base;
+    bool mine;
+    auto load = [&](VEC* into) {
+        const long long v = (long long)c * RR_THREADS + t;
+        base = d.base[k] + o * d.outer_stride[k] + v * (long long)sizeof(VEC);
+        mine = v < vectors;
 #pragma unroll
-    for (int w = 0; w < W; ++w)
-        if (w < beams && from[w] >= 0) got[w] = *(const VEC*)(base + from[w]);
+        for (int w = 0; w < W; ++w)
+            if (mine && w < beams && from[w] >= 0) into[w] = *(const VEC*)(base + from[w]);
+    };
+    auto store = [&](const VEC* what, char* at, bool had) {
 #pragma unroll
-    for (int w = 0; w < W; ++w)
-        if (w < beams && from[w] >= 0) *(VEC*)(base + to[w]) = got[w];
+        for (int w = 0; w < W; ++w)
+            if (had && w < beams && from[w] >= 0) *(VEC*)(at + to[w]) = what[w];
+    };
+    load(got[0]);
+    if constexpr (!AHEAD) store(got[0], base, mine);         // run is 1
+    else {
+        // the next piece is read before this one is written
+        auto step = [&](VEC* now, VEC* next) {
+            char* const at = base;
+            const bool had = mine;
+            if (++c == pieces) { c = 0; ++o; }
+            if (++i < last) load(next);
+            store(now, at, had);
+        };
+        while (true) {
+            step(got[0], got[1]);
+            if (i >= last) break;
+            step(got[1], got[0]);
+            if (i >= last) break;
+        }
+    }
+}
+
+// Two pieces a block where that still leaves every multiprocessor two rounds of blocks, and up to 64 bytes of a piece a
+// thread: finding the rows costs a block two reads that wait for each other. MEASURED (us, one piece, two, four): 16 groups of 4
+// pages of 36 layers, three of each moved, 33.4, 32.4 (5.8 TB/s), 32.9; 8 groups of 4 states of 8 MB, three moved, 107.5, 101.8 (6.6 TB/s), 104.4; 1
+// group of 4 pages of 8 layers 2.0, 2.3, 2.9.
+template <typename VEC, int W>
+static int reorder_of(const ReorderRows& d, int tensors, int groups, int beams, long long blocks, const int* index,
+                      const int* parents, cudaStream_t stream) {
+    if constexpr (W * sizeof(VEC) <= 64)
+        if (blocks * groups * tensors >= 2ll * 2 * 8 * tgo_multiprocessors())
+            return tgo_launch_pdl(reorder_rows_kernel<VEC, W, true>, dim3((unsigned)((blocks + 1) / 2), groups, tensors), dim3(RR_THREADS), 0, stream, d,
+                                  index, parents, beams, 2);
+    return tgo_launch_pdl(reorder_rows_kernel<VEC, W, false>, dim3((unsigned)blocks, groups, tensors), dim3(RR_THREADS), 0, stream, d, index,
+                          parents, beams, 1);
 }
 
 template <typename VEC>
 static int reorder_launch(const ReorderRows& d, int tensors, int groups, int beams, long long blocks, const int* index,
                           const int* parents, cudaStream_t stream) {
-    const dim3 grid((unsigned)blocks, groups, tensors), block(RR_THREADS);
-    if (beams <= 4) return tgo_launch_pdl(reorder_rows_kernel<VEC, 4>, grid, block, 0, stream, d, index, parents, beams);
-    if (beams <= 8) return tgo_launch_pdl(reorder_rows_kernel<VEC, 8>, grid, block, 0, stream, d, index, parents, beams);
-    if (beams <= 16) return tgo_launch_pdl(reorder_rows_kernel<VEC, 16>, grid, block, 0, stream, d, index, parents, beams);
-    return tgo_launch_pdl(reorder_rows_kernel<VEC, 32>, grid, block, 0, stream, d, index, parents, beams);
+    if (beams <= 4) return reorder_of<VEC, 4>(d, tensors, groups, beams, blocks, index, parents, stream);
+    if (beams <= 8) return reorder_of<VEC, 8>(d, tensors, groups, beams, blocks, index, parents, stream);
+    if (beams <= 16) return reorder_of<VEC, 16>(d, tensors, groups, beams, blocks, index, parents, stream);
+    return reorder_of<VEC, 32>(d, tensors, groups, beams, blocks, index, parents, stream);
 }
 
 // desc: per tensor six numbers: address, outer count, bytes from one outer block to the next, rows, bytes
@@ -665,7 +706,7 @@ TGO_API int tgo_reorder_rows(const long long* desc, int tensors, const int* inde
             const long long c = (d.row_bytes[i] / width + RR_THREADS - 1) / RR_THREADS * d.outer[i];
             blocks = c > blocks ? c : blocks;
         }
-        if (blocks > 0x7fffffff) return TGO_E_BAD_ARG;
+        if (blocks > 0x7fffff00) return TGO_E_BAD_ARG;
         int rc;
         if (width == 16) rc = reorder_launch<uint4>(d, n, groups, beams, blocks, index, parents, stream);
         else if (width == 8) rc = reorder_launch<uint2>(d, n, groups, beams, blocks, index, parents, stream);
