@@ -61,6 +61,7 @@ low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile,
     __shared__ int pool[3 * (LP_MAX_ADAPTERS + 1)];
     __shared__ int warp_rows[LP_WARPS], warp_tiles[LP_WARPS];
     pdl_wait();
+    pdl_launch_late();                                       // the next kernel's blocks may come and wait: 0.8 us
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, slots = adapters + 1;
     const bool ordered = adapters <= LP_ORDERED;
     int* const rows_before = pool;
@@ -210,6 +211,8 @@ low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile,
 #define LF_WARPS (LF_THREADS / 32)
 #define LF_PASS 64                // values of u a pass, bfloat16
 #define LF_TILES 2                // tiles of 16 columns a warp has under way, bfloat16
+#define LR_SCAN_TURNS 2           // rows a thread looks at
+#define LR_SCAN_ROWS (LR_SCAN_TURNS * LF_THREADS)
 static_assert(LF_ROWS == LF_WARPS, "a warp a row");
 
 __device__ __forceinline__ void lf_cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
@@ -234,8 +237,8 @@ __global__ void __launch_bounds__(LF_THREADS, 3)
 low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __restrict__ info, const int* __restrict__ tiles) {
     extern __shared__ __align__(16) float lf_smem[];
     __shared__ int rows[LF_ROWS];
-    __shared__ __align__(16) int ids[LF_THREADS];
-    __shared__ int warp_count[LF_WARPS], group[2];
+    __shared__ __align__(16) int ids[LR_SCAN_ROWS];
+    __shared__ int warp_count[LR_SCAN_TURNS * LF_WARPS], group[2];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int item = blockIdx.x / LF_CTAS, cta = blockIdx.x % LF_CTAS;
     pdl_wait();
@@ -252,34 +255,53 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
         if (t == 0) rows[0] = 0;
         __syncthreads();
     } else {
-        int mine = -2;
-        if (t < p.T) {
-            mine = p.ids[t];
-            if (mine < 0 || mine >= p.adapters) mine = -1;
+        // up to LR_SCAN_TURNS rows a thread: which adapter, how many rows of it before, and whether it begins a group
+        int mine[LR_SCAN_TURNS], before[LR_SCAN_TURNS], all = 0;
+        unsigned who[LR_SCAN_TURNS];
+#pragma unroll
+        for (int h = 0; h < LR_SCAN_TURNS; ++h) {
+            const int r = h * LF_THREADS + t;
+            mine[h] = r < p.T ? p.ids[r] : -2;
+            if (r < p.T && (mine[h] < 0 || mine[h] >= p.adapters)) mine[h] = -1;
+            ids[r] = mine[h];
         }
-        ids[t] = mine;
-        __syncthreads();
-        int before = 0, place = 0, all = 0;                  // rows of this one's adapter before it; groups before this one's, and all
-        for (int j = 0; j < min(t | 31, p.T); j += 4) {
-            const int4 q = *(const int4*)(ids + j);
-            before += (q.x == mine && j < t) + (q.y == mine && j + 1 < t) + (q.z == mine && j + 2 < t) + (q.w == mine && j + 3 < t);
-        }
-        const bool begins = t < p.T && before % LF_ROWS == 0;
-        const unsigned who = __ballot_sync(0xffffffffu, begins);
-        if (lane == 0) warp_count[warp] = __popc(who);
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < LF_WARPS; ++w) {
-            place += w < warp ? warp_count[w] : 0;
-            all += warp_count[w];
+        for (int h = 0; h < LR_SCAN_TURNS; ++h) {
+            const int r = h * LF_THREADS + t;
+            before[h] = 0;
+            if (r - lane < p.T) {                            // the warps before, then this one
+#pragma unroll 8
+                for (int j = 0; j < r - lane; j += 4) {
+                    const int4 q = *(const int4*)(ids + j);
+                    before[h] += (q.x == mine[h]) + (q.y == mine[h]) + (q.z == mine[h]) + (q.w == mine[h]);
+                }
+                before[h] += __popc(__match_any_sync(0xffffffffu, mine[h]) & ((1u << lane) - 1));
+            }
+            who[h] = __ballot_sync(0xffffffffu, r < p.T && before[h] % LF_ROWS == 0);
+            if (lane == 0) warp_count[h * LF_WARPS + warp] = __popc(who[h]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < LR_SCAN_TURNS; ++h) {
+            int place = __popc(who[h] & ((1u << lane) - 1)) + all;
+#pragma unroll
+            for (int w = 0; w < LF_WARPS; ++w) {
+                place += w < warp ? warp_count[h * LF_WARPS + w] : 0;
+                all += warp_count[h * LF_WARPS + w];
+            }
+            if ((who[h] >> lane & 1) && place == item) { group[0] = mine[h]; group[1] = before[h]; }
         }
         if (item >= all) return;
-        if (begins && place + __popc(who & ((1u << lane) - 1)) == item) { group[0] = mine; group[1] = before; }
         __syncthreads();
         id = group[0];
-        const bool in = mine == id && before >= group[1] && before < group[1] + LF_ROWS;
-        if (in) rows[before - group[1]] = t;
-        n = __syncthreads_count(in);
+        n = 0;
+#pragma unroll
+        for (int h = 0; h < LR_SCAN_TURNS; ++h) {
+            const bool in = mine[h] == id && before[h] >= group[1] && before[h] < group[1] + LF_ROWS;
+            if (in) rows[before[h] - group[1]] = h * LF_THREADS + t;
+            n += __syncthreads_count(in);
+        }
     }
     const TY* const y = (const TY*)p.y;
     TY* const out = (TY*)p.out;
@@ -539,6 +561,7 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
         tg_init_done();
     }
     pdl_wait();
+    pdl_launch_late();                                       // out's blocks come as these leave: 0.7 us of 64
     const int id = tiles[3 * tile], r0 = tiles[3 * tile + 1] + skip, rows = min(tiles[3 * tile + 2] - skip, g.rows);
     if (tile >= info[0] || id < 0 || rows <= 0) return;      // the same for the whole cluster
     if (warp == 1) tg_alloc<COLS>(tmem_slot);
@@ -1037,7 +1060,6 @@ template <typename T> static bool lr_vectors(const LowRank& p) {
 }
 
 // Rows from which they are planned: up to here each cluster of the kernel for few rows finds its own.
-#define LR_SCAN_ROWS LF_THREADS
 
 template <typename T> static bool lr_few_takes(const LowRank& p) {
     return lr_vectors<T>(p) && lf_floats<T>(p.columns.slices * p.rank, p.K) * 4 <= 200 * 1024 && p.T <= (1 << 24) &&

@@ -21,7 +21,7 @@ F32, BF16 = 0, 1
 _CODES = {torch.float32: F32, torch.bfloat16: BF16}
 E_BAD_ARG = 1000
 E_WORK = 1001            # the workspace is too small, nothing was done
-LOW_RANK_SCANNED = 256   # rows up to which low_rank_add's kernels find each adapter's rows themselves
+LOW_RANK_SCANNED = 512   # rows up to which low_rank_add's kernels find each adapter's rows themselves
 
 # What an entry point is handed (`entry_points`): whole numbers as they are (anything else refused),
 # single-precision numbers as floats, addresses as whole numbers.
