@@ -44,10 +44,11 @@ struct LowRank {
 
 // ------------------------------------------------------------------------- the rows of an adapter
 // For many rows: which rows have which adapter, in tiles of up to `tile` rows of one adapter (rows without
-// one come last, as tiles of adapter -1). perm: the rows by tile; info[0]: the number of tiles, a tile is
-// (adapter, first place in perm, rows). One block; a warp has a run of rows. With up to 255 adapters each warp
+// one come last, as tiles of adapter -1). perm: the rows by tile; info: the number of tiles, of those with an adapter, and the first
+// place in perm of a row without; a tile is (adapter, first place in perm, rows). One block; a warp has a run of rows. With up to 255 adapters each warp
 // counts for itself, and an adapter's rows keep their order: the rows of a request then lie together, and a tile of them
 // can be fetched as one box. With more, rows take their places as they come, 32 at a time in order.
+#define LP_INFO 3
 #define LP_THREADS 1024
 #define LP_WARPS (LP_THREADS / 32)
 #define LP_MAX_ADAPTERS 3071
@@ -157,7 +158,11 @@ low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile,
         at_tile += (n + tile - 1) / tile;
     }
     __syncthreads();
-    if (t == 0) info[0] = total;
+    if (t == 0) {
+        info[0] = total;
+        info[1] = tiles_before[adapters];
+        info[2] = rows_before[adapters];
+    }
     for (int q = t; q < total; q += LP_THREADS) {
         int lo = 0, hi = slots - 1;                          // the last adapter whose tiles begin at q or before
         while (lo < hi) {
@@ -733,10 +738,10 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
 // y and out go through shared memory, asynchronously: each of eight warps has 32 rows (the ones whose sums it can read
 // from tensor memory, a lane a row) of every other turn and a ring of its own of 32 x 64 tiles; it adds the sums where
 // y lies and has the tile stored from there. Rows that lie together are one box either way; others come four at a time and are written by
-// the warp, as are part tiles. (Reading y into registers two steps ahead and writing from them, through a transposing
+// the warp, as are part tiles. As many blocks as fit share all tiles' turns out evenly, so that a block's first reads are waited
+// for once. (Blocks of eight turns each: the call took 63 us where it takes 57, 1833 rows, gate and up of 12288, rank 32. Reading y into registers two steps ahead and writing from them, through a transposing
 // buffer, took 68 us where this takes 40: 8192 rows of 6144 columns, rank 64.)
 #define LO_COLS 64
-#define LO_TURNS 8                // of a block
 #define LO_HANDS 8                // warps that hand on; the one after them asks for copies and products
 #define LO_THREADS (LO_HANDS * 32 + 32)
 #define LO_U_BOX (LT_ROWS * 128)  // bytes of 64 values of k: of 128 rows of u,
@@ -756,31 +761,33 @@ template <int BOXES, bool PAIRED, bool EIGHTS, typename TY> struct LowRankOut {
     static constexpr int A_BYTES = SLICES * PARTS * BOXES * LO_U_BOX, B_BYTES = BOXES * LO_B_BOX;
     static constexpr int Y_BOXES = (int)sizeof(TY) / 2, Y_BYTES = Y_BOXES * 32 * 128;     // a warp's tile: boxes of 128 bytes a row
     static constexpr int SLOTS = A_BYTES + 2 * B_BYTES + LO_HANDS * 2 * Y_BYTES <= 224 * 1024 ? 2 : 1;
-    static constexpr int BYTES = A_BYTES + 2 * B_BYTES + LO_HANDS * SLOTS * Y_BYTES + 512 + LT_ROWS * 4;
+    static constexpr int BYTES = A_BYTES + 2 * B_BYTES + LO_HANDS * SLOTS * Y_BYTES + 512;
+    static constexpr int BLOCKS = 2 * (BYTES + 1024) <= 228 * 1024 ? 2 : 1;      // of a multiprocessor
     static_assert(BYTES <= 227 * 1024, "shared memory of a block");
 };
 
 template <int BOXES, bool PAIRED, bool EIGHTS, typename TY>
-__global__ void __launch_bounds__(LO_THREADS)
+__global__ void __launch_bounds__(LO_THREADS, (LowRankOut<BOXES, PAIRED, EIGHTS, TY>::BLOCKS))
 low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_b,
                     const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_row,
-                    const __grid_constant__ CUtensorMap map_out, const LowRank p, const int* __restrict__ perm,
+                    const __grid_constant__ CUtensorMap map_out, const LowRank p, const int tile_turns, const int* __restrict__ perm,
                     const int* __restrict__ info, const int* __restrict__ tiles) {
     typedef LowRankOut<BOXES, PAIRED, EIGHTS, TY> L;
     extern __shared__ __align__(1024) unsigned char lo_raw[];
     unsigned char* const a_smem = lo_raw;                    // [slice][part][box][128 rows][128]
     unsigned char* const b_ring = a_smem + L::A_BYTES;       // [2][box][64 columns][128]
     unsigned char* const y_ring = b_ring + 2 * L::B_BYTES;   // [warp][slot][box][32 rows][128]
-    int* const rows = (int*)(y_ring + LO_HANDS * L::SLOTS * L::Y_BYTES);
-    uint64_t* const full = (uint64_t*)(rows + LT_ROWS);      // [2] B's turn is there (the first: u, too)
-    uint64_t* const acc_full = full + 2;                     // [4] a turn's products are done: the accumulator, and B's slot free
+    uint64_t* const full = (uint64_t*)(y_ring + LO_HANDS * L::SLOTS * L::Y_BYTES);       // [2] B's turn is there
+    uint64_t* const u_full = full + 2;
+    uint64_t* const acc_full = u_full + 1;                   // [4] a turn's products are done: the accumulator, and B's slot free
     uint64_t* const acc_empty = acc_full + 4;                // [4] the accumulator has been read
     uint64_t* const y_full = acc_empty + 4;                  // [warp][slot]
     uint64_t* const settled = y_full + LO_HANDS * L::SLOTS;         // after a wait ran out
     uint32_t* const tmem_slot = (uint32_t*)(settled + 1);
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, tile = blockIdx.y;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     if (t == 0) {
         for (int i = 0; i < 2; ++i) tg_init(&full[i], 1);
+        tg_init(u_full, 1);
         for (int i = 0; i < 4; ++i) { tg_init(&acc_full[i], 1); tg_init(&acc_empty[i], 4); }
         for (int i = 0; i < LO_HANDS * L::SLOTS; ++i) tg_init(&y_full[i], 1);
         tg_init(settled, 1);
@@ -788,56 +795,79 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
     }
     __syncthreads();
     pdl_wait();
-    const int id = tiles[3 * tile], r0 = tiles[3 * tile + 1], n = tiles[3 * tile + 2];
-    if (tile >= info[0]) return;                             // what was read of it is nothing
-    // this block's columns: LO_TURNS turns of one slice (in eights: of both)
-    int slice = 0, begin = 0, end = EIGHTS ? p.N : p.columns.ends[0], group = blockIdx.x;
+    // this block's turns: an even share of those of all tiles with an adapter, one after the other
+    const int all = info[1] * tile_turns, least = all / (int)gridDim.x, more = all - least * (int)gridDim.x;
+    const int begin = blockIdx.x * least + min((int)blockIdx.x, more), turns = least + ((int)blockIdx.x < more);
+    // where the w-th turn of a tile lies
+    auto columns = [&](int w, int& slice, int& col, int& end) {
+        int from = 0;
+        slice = 0;
+        end = EIGHTS ? p.N : p.columns.ends[0];
+        if constexpr (!EIGHTS) {
 #pragma unroll
-    for (int i = 1; i < LR_MAX_SLICES; ++i) {
-        const int groups = (end - begin + LO_TURNS * LO_COLS - 1) / (LO_TURNS * LO_COLS);
-        if (slice == i - 1 && group >= groups) {
-            group -= groups;
-            slice = i;
-            begin = end;
-            end = p.columns.ends[i];
+            for (int i = 1; i < LR_MAX_SLICES; ++i) {
+                const int n = (end - from + LO_COLS - 1) / LO_COLS;
+                if (slice == i - 1 && w >= n) {
+                    w -= n;
+                    slice = i;
+                    from = end;
+                    end = p.columns.ends[i];
+                }
+            }
         }
-    }
-    const int col0 = begin + group * LO_TURNS * LO_COLS, col1 = min(col0 + LO_TURNS * LO_COLS, end);
-    const int turns = (col1 - col0 + LO_COLS - 1) / LO_COLS;
+        col = from + w * LO_COLS;
+    };
     TY* const out = (TY*)p.out;
     constexpr int PER = 16 / (int)sizeof(TY);                // columns of a 16-byte piece
-    if (id < 0) {                                            // no adapter: y as it is
-        if (p.out == p.y) return;
-        const TY* const y = (const TY*)p.y;
-        if (t < n) rows[t] = perm[r0 + t];
-        __syncthreads();
-        const int vectors = (col1 - col0) / PER;
-        for (int e = t; e < n * vectors; e += LO_THREADS) {
-            const int r = rows[e / vectors], c = col0 + e % vectors * PER;
-            *(uint4*)(out + (size_t)r * p.out_stride + c) = *(const uint4*)(y + (size_t)r * p.y_stride + c);
-        }
-        return;
-    }
     const int steps_all = (p.rank + 15) / 16;
-    auto fetch = [&](int turn) {                             // one thread
-#pragma unroll
-        for (int x = 0; x < BOXES; ++x)
-            tg_load_2d(b_ring + (turn & 1) * L::B_BYTES + x * LO_B_BOX, &map_b, x * 64, id * p.N + col0 + turn * LO_COLS, &full[turn & 1]);
-    };
     if (warp == LO_HANDS) {
-        if (lane == 0) {
-            // the rows after the tile's come along: their sums are never stored
-            tg_expect(&full[0], L::A_BYTES + L::B_BYTES);
+        struct Turn {
+            int row, r0, slice;                              // of B; of u
+            bool fresh;                                      // another u than the turn before
+        };
+        int tile = begin / tile_turns, w = begin - tile * tile_turns, id = 0, r0 = 0, last = 0;
+        bool moved = true;
+        auto look = [&]() {                                  // the next turn
+            Turn q;
+            int col, end;
+            if (moved) {
+                id = tiles[3 * tile];
+                r0 = tiles[3 * tile + 1];
+            }
+            columns(w, q.slice, col, end);
+            q.row = id * p.N + col;
+            q.r0 = r0;
+            q.fresh = moved || q.slice != last;
+            last = q.slice;
+            moved = ++w == tile_turns;
+            if (moved) {
+                w = 0;
+                ++tile;
+            }
+            return q;
+        };
+        auto fetch_u = [&](const Turn& q) {                  // one thread; the rows after the tile's come along: their sums are never stored
+            tg_expect(u_full, L::A_BYTES);
 #pragma unroll
             for (int i = 0; i < L::SLICES * L::PARTS * BOXES; ++i) {
                 const int x = i % BOXES, rest = i / BOXES % L::PARTS, h = i / BOXES / L::PARTS;
-                tg_load_2d(a_smem + i * LO_U_BOX, &map_u, ((slice + h) * 2 + rest) * steps_all * 16 + x * 64, r0, &full[0]);
+                tg_load_2d(a_smem + i * LO_U_BOX, &map_u, ((q.slice + h) * 2 + rest) * steps_all * 16 + x * 64, q.r0, u_full);
             }
-            fetch(0);
-            if (turns > 1) {
-                tg_expect(&full[1], L::B_BYTES);
-                fetch(1);
+        };
+        auto fetch = [&](const Turn& q, int s) {             // one thread
+            tg_expect(&full[s], L::B_BYTES);
+#pragma unroll
+            for (int x = 0; x < BOXES; ++x) tg_load_2d(b_ring + s * L::B_BYTES + x * LO_B_BOX, &map_b, x * 64, q.row, &full[s]);
+        };
+        Turn two[2] = {};                                    // a turn and the next
+        if (turns > 0) two[0] = look();
+        if (turns > 1) two[1] = look();
+        if (lane == 0) {
+            if (turns > 0) {
+                fetch_u(two[0]);
+                fetch(two[0], 0);
             }
+            if (turns > 1) fetch(two[1], 1);
         }
         __syncwarp();
         tg_alloc<4 * LO_COLS>(tmem_slot);
@@ -847,11 +877,21 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
         const uint32_t tmem = *tmem_slot;
         if (tg_elect()) {
             const uint32_t idesc = tg_idesc(EIGHTS ? LO_COLS / 2 : LO_COLS);
-            uint32_t sent = min(turns, 2);
+            uint32_t sent = min(turns, 2), u_sent = min(turns, 1);
             bool ok = true;
             for (int i = 0; i < turns; ++i) {
                 const int s = i & 1, acc = i & 3;
-                ok = tg_wait(&full[s], (i >> 1) & 1, &low_rank_error_flag, 4);
+                const Turn q = s ? two[1] : two[0];
+                if (q.fresh) {
+                    if (i > 0) {                             // u's place again, once the products before are done
+                        ok = tg_wait(&acc_full[(i - 1) & 3], ((i - 1) >> 2) & 1, &low_rank_error_flag, 6);
+                        if (!ok) break;
+                        fetch_u(q);
+                        ++u_sent;
+                    }
+                    ok = tg_wait(u_full, (u_sent - 1) & 1, &low_rank_error_flag, 4);
+                }
+                if (ok) ok = tg_wait(&full[s], (i >> 1) & 1, &low_rank_error_flag, 4);
                 if (ok) ok = tg_wait(&acc_empty[acc], ((i >> 2) & 1) ^ 1, &low_rank_error_flag, 5);
                 if (!ok) break;
                 tg_after();
@@ -875,58 +915,87 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
                 }
                 tg_commit(&acc_full[acc]);
                 if (i + 2 < turns) {                         // the slot again, once its products are done
+                    const Turn next = look();
+                    if (s) two[1] = next;
+                    else two[0] = next;
                     ok = tg_wait(&acc_full[acc], (i >> 2) & 1, &low_rank_error_flag, 6);
                     if (!ok) break;
-                    tg_expect(&full[s], L::B_BYTES);
-                    fetch(i + 2);
+                    fetch(next, s);
                     ++sent;
                 }
             }
             if (!ok) {
                 tg_settle_copies(full, 2, sent, &low_rank_error_flag, 4);
+                tg_settle_copies(u_full, 1, u_sent, &low_rank_error_flag, 4);
                 tg_settle_products(settled, &low_rank_error_flag, 6);
             }
         }
         __syncwarp();
     } else {
-        const int q0 = (warp & 3) * 32, mine = min(n - q0, 32), set = warp >> 2;   // its rows of the tile, none or fewer
-                                                                                   // perhaps; its turns are set, set + 2, ...
-        const int row = perm[r0 + min(q0 + lane, n - 1)];
-        if (set == 0) rows[q0 + lane] = row;
-        const int first = __shfl_sync(0xffffffffu, row, 0), turns_mine = (turns - set + 1) / 2;
-        const bool together = __all_sync(0xffffffffu, lane >= mine || row == first + lane);
-        int gather[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) gather[i] = __shfl_sync(0xffffffffu, row, (4 * lane + i) & 31);
+        // its rows of a tile, from q0 on, none or fewer than 32 perhaps; its turns are set, set + 2, ... of the block's
+        const int q0 = (warp & 3) * 32, set = warp >> 2, turns_mine = (turns - set + 1) / 2;
+        struct Rows {
+            int place, first, count, col, end;               // in perm; in y; columns
+            bool together;
+        };
+        int tile = (begin + set) / tile_turns, w = begin + set - tile * tile_turns, gather[4] = {};
+        Rows next = {};
+        bool moved = true;
         unsigned char* const ring = y_ring + warp * L::SLOTS * L::Y_BYTES;
         uint64_t* const there = y_full + warp * L::SLOTS;
         auto load = [&](int i) {                             // of this warp's turns; the whole warp
-            const int s = i % L::SLOTS, c = col0 + (2 * i + set) * LO_COLS;
-            if (lane == 0) tg_expect(&there[s], together ? L::Y_BYTES : (mine + 3) / 4 * 4 * 128 * L::Y_BOXES);
+            if (moved) {
+                const int r0 = tiles[3 * tile + 1], n = tiles[3 * tile + 2], row = perm[r0 + min(q0 + lane, n - 1)];
+                next.place = r0 + q0;
+                next.count = min(n - q0, 32);
+                next.first = __shfl_sync(0xffffffffu, row, 0);
+                next.together = __all_sync(0xffffffffu, lane >= next.count || row == next.first + lane);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) gather[j] = __shfl_sync(0xffffffffu, row, (4 * lane + j) & 31);
+            }
+            int slice;
+            columns(w, slice, next.col, next.end);
+            const int s = i % L::SLOTS;
+            if (lane == 0) {
+                if (next.count > 0) tg_expect(&there[s], next.together ? L::Y_BYTES : (next.count + 3) / 4 * 4 * 128 * L::Y_BOXES);
+                else tg_arrive(&there[s]);
+            }
             __syncwarp();
 #pragma unroll
             for (int x = 0; x < L::Y_BOXES; ++x) {
                 unsigned char* const to = ring + s * L::Y_BYTES + x * 4096;
-                if (together) {
-                    if (lane == 0) tg_load_2d(to, &map_y, c + x * 32, first, &there[s]);
-                } else if (4 * lane < mine) {
-                    tg_gather4(to + lane * 512, &map_row, c + x * 32, gather[0], gather[1], gather[2], gather[3], &there[s]);
+                if (next.together) {
+                    if (lane == 0 && next.count > 0) tg_load_2d(to, &map_y, next.col + x * 32, next.first, &there[s]);
+                } else if (4 * lane < next.count) {
+                    tg_gather4(to + lane * 512, &map_row, next.col + x * 32, gather[0], gather[1], gather[2], gather[3], &there[s]);
                 }
+            }
+            w += 2;
+            moved = w >= tile_turns;
+            while (w >= tile_turns) {
+                w -= tile_turns;
+                ++tile;
             }
         };
         uint32_t sent = 0;
-        if (mine > 0)
-            for (; sent < min(turns_mine, L::SLOTS); ++sent) load(sent);
+        Rows slots[2] = {};
+        for (; sent < min(turns_mine, L::SLOTS); ++sent) {
+            load(sent);
+            if (sent) slots[1] = next;
+            else slots[0] = next;
+        }
         tg_before();
         __syncthreads();
         tg_after();
         const uint32_t lanes = *tmem_slot + ((uint32_t)q0 << 16);
         bool ok = true;
         for (int i = 0; i < turns_mine && ok; ++i) {
-            const int slot = i % L::SLOTS, c = col0 + (2 * i + set) * LO_COLS, buf = (2 * i + set) & 3;
+            const int slot = i % L::SLOTS, buf = (2 * i + set) & 3;
+            const Rows now = slot ? slots[1] : slots[0];
+            const int mine = now.count, c = now.col;
             const uint32_t sums = lanes + buf * LO_COLS;
             ok = __all_sync(0xffffffffu, tg_wait(&acc_full[buf], (i >> 1) & 1, &low_rank_error_flag, 7));
-            if (ok && mine > 0) ok = __all_sync(0xffffffffu, tg_wait(&there[slot], (i / L::SLOTS) & 1, &low_rank_error_flag, 8));
+            if (ok) ok = __all_sync(0xffffffffu, tg_wait(&there[slot], (i / L::SLOTS) & 1, &low_rank_error_flag, 8));
             if (!ok) break;
             tg_after();
             unsigned char* const at = ring + slot * L::Y_BYTES;
@@ -969,34 +1038,49 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) tg_arrive(&acc_empty[buf]);
-            if (mine <= 0) continue;
-            if (together && mine == 32 && c + LO_COLS <= col1) {
+            if (now.together && mine == 32 && c + LO_COLS <= now.end) {
                 if (lane == 0) {
 #pragma unroll
-                    for (int x = 0; x < L::Y_BOXES; ++x) lo_store_2d(&map_out, c + x * 32, first, at + x * 4096);
-                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    for (int x = 0; x < L::Y_BOXES; ++x) lo_store_2d(&map_out, c + x * 32, now.first, at + x * 4096);
                 }
             } else {
 #pragma unroll
                 for (int x = 0; x < L::Y_BOXES; ++x)
                     for (int r = lane >> 3; r < mine; r += 4) {
-                        const int col = c + x * 32 + (lane & 7) * PER;
-                        if (col < col1)
-                            *(uint4*)(out + (size_t)rows[q0 + r] * p.out_stride + col) = *(const uint4*)(at + x * 4096 + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+                        const int col = c + x * 32 + (lane & 7) * PER, row = now.together ? now.first + r : perm[now.place + r];
+                        if (col < now.end)
+                            *(uint4*)(out + (size_t)row * p.out_stride + col) = *(const uint4*)(at + x * 4096 + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
                     }
             }
+            if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");     // with or without a store: a group a turn
             // The next load goes where the turn before lay (with one slot: this turn), once its store has been read: this
-            // turn's may still be. (A block's last turn alone may be written otherwise, and nothing is loaded after it.)
-            if (L::SLOTS == 1 || i > 0) {
-                if (sent < turns_mine) {
-                    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(L::SLOTS - 1) : "memory");
-                    __syncwarp();
-                    load(sent);
-                    ++sent;
-                }
+            // turn's may still be.
+            if ((L::SLOTS == 1 || i > 0) && sent < turns_mine) {
+                asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(L::SLOTS - 1) : "memory");
+                __syncwarp();
+                load(sent);
+                if (sent % L::SLOTS) slots[1] = next;
+                else slots[0] = next;
+                ++sent;
             }
         }
-        if (!ok && lane == 0 && mine > 0) tg_settle_copies(there, L::SLOTS, sent, &low_rank_error_flag, 8);
+        if (!ok && lane == 0) tg_settle_copies(there, L::SLOTS, sent, &low_rank_error_flag, 8);
+        // rows without an adapter: y as it is, 128 vectors of a row a warp and turn
+        if (p.out != p.y) {
+            const int vectors = p.N / PER, pieces = (vectors + 127) / 128, place = info[2];
+            for (long long e = (long long)blockIdx.x * LO_HANDS + warp; e < (long long)(p.T - place) * pieces; e += (long long)gridDim.x * LO_HANDS) {
+                const int r = (int)(e / pieces), row = perm[place + r], v = (int)(e - (long long)r * pieces) * 128 + lane;
+                const uint4* const from = (const uint4*)((const TY*)p.y + (size_t)row * p.y_stride);
+                uint4* const to = (uint4*)(out + (size_t)row * p.out_stride);
+                uint4 held[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (v + 32 * j < vectors) held[j] = from[v + 32 * j];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (v + 32 * j < vectors) to[v + 32 * j] = held[j];
+            }
+        }
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         __syncwarp();
     }
@@ -1088,7 +1172,7 @@ template <typename T, typename TY> static int low_rank_few(const LowRank& p, int
     if (p.T > LR_SCAN_ROWS) {
         perm = plan;
         info = perm + p.T;
-        tiles = info + 1;
+        tiles = info + LP_INFO;
         const int rc = tgo_launch_pdl(low_rank_plan_kernel, dim3(1), dim3(LP_THREADS), 0, stream, p.ids, p.T, p.adapters, LF_ROWS, perm, info, tiles);
         if (rc) return rc;
     }
@@ -1199,12 +1283,14 @@ static int low_rank_out(const LowRank& p, const bf16* u, const int* perm, const 
         if (err != cudaSuccess) return (int)err;
         sized[dev] = true;
     }
-    int groups = 0, begin = 0;
+    int turns = 0, begin = 0;                                // of a tile
     for (int i = 0; i < (EIGHTS ? 1 : p.columns.slices); ++i) {
         const int end = EIGHTS ? p.N : p.columns.ends[i];
-        groups += (end - begin + LO_TURNS * LO_COLS - 1) / (LO_TURNS * LO_COLS);
+        turns += (end - begin + LO_COLS - 1) / LO_COLS;
         begin = end;
     }
+    const long long most = (lr_tiles(p, LT_ROWS) * turns + 1) / 2, slots = (long long)tgo_multiprocessors() * LowRankOut<BOXES, PAIRED, EIGHTS, TY>::BLOCKS;
+    if (most > 0x3fffffff) return TGO_E_BAD_ARG;
     const int width = 2 * ((p.rank + 15) / 16 * 16) * p.columns.slices;
     auto map_of = [](CUtensorMap* map, const void* ptr, long long rows, long long cols, long long stride, int box_rows) {
         return sizeof(TY) == 2 ? tg_map(map, ptr, rows, cols, stride, box_rows) : tg_map_f32(map, ptr, rows, cols, stride, box_rows);
@@ -1214,8 +1300,8 @@ static int low_rank_out(const LowRank& p, const bf16* u, const int* perm, const 
         !map_of(&map_y, p.y, p.T, p.N, p.y_stride, 32) || !map_of(&map_row, p.y, p.T, p.N, p.y_stride, 1) ||
         !map_of(&map_out, p.out, p.T, p.N, p.out_stride, 32))
         return TGO_E_BAD_ARG;
-    return tgo_launch_pdl(low_rank_out_kernel<BOXES, PAIRED, EIGHTS, TY>, dim3(groups, (unsigned)lr_tiles(p, LT_ROWS)), dim3(LO_THREADS), bytes, stream,
-                          map_u, map_b, map_y, map_row, map_out, p, perm, info, tiles);
+    return tgo_launch_pdl(low_rank_out_kernel<BOXES, PAIRED, EIGHTS, TY>, dim3((unsigned)(most < slots ? most : slots)), dim3(LO_THREADS), bytes, stream,
+                          map_u, map_b, map_y, map_row, map_out, p, turns, perm, info, tiles);
 }
 
 template <bool EIGHTS, typename TY>
@@ -1227,14 +1313,14 @@ static int low_rank_out_of(const LowRank& p, const bf16* u, const int* perm, con
 
 // 32-bit numbers of workspace: the plan, and u twice in bfloat16.
 static long long lr_tile_work(const LowRank& p) {
-    return (p.T + 1 + 3 * lr_tiles(p, LT_ROWS) + 3) / 4 * 4 + (long long)p.T * ((p.rank + 15) / 16 * 16) * p.columns.slices;
+    return (p.T + LP_INFO + 3 * lr_tiles(p, LT_ROWS) + 3) / 4 * 4 + (long long)p.T * ((p.rank + 15) / 16 * 16) * p.columns.slices;
 }
 
 template <typename TY> static int low_rank_tiles(const LowRank& p, int* work, cudaStream_t stream) {
     int* const perm = work;
     int* const info = perm + p.T;
-    int* const tiles = info + 1;
-    bf16* const u = (bf16*)(work + (p.T + 1 + 3 * lr_tiles(p, LT_ROWS) + 3) / 4 * 4);
+    int* const tiles = info + LP_INFO;
+    bf16* const u = (bf16*)(work + (p.T + LP_INFO + 3 * lr_tiles(p, LT_ROWS) + 3) / 4 * 4);
     int rc = tgo_launch_pdl(low_rank_plan_kernel, dim3(1), dim3(LP_THREADS), 0, stream, p.ids, p.T, p.adapters, LT_ROWS, perm, info, tiles);
     if (rc) return rc;
     const LowRankTile g = lr_plan(p);
@@ -1278,7 +1364,7 @@ template <typename T, typename TY> static long long lr_work(const LowRank& p) {
     const int width = p.columns.slices * p.rank;
     if constexpr (sizeof(T) == 2)
         if (lr_many(p) && lr_tile_takes<TY>(p)) return lr_tile_work(p);
-    if (lr_few_takes<T>(p)) return p.T > LR_SCAN_ROWS ? p.T + 1 + 3 * lr_tiles(p, LF_ROWS) : 0;
+    if (lr_few_takes<T>(p)) return p.T > LR_SCAN_ROWS ? p.T + LP_INFO + 3 * lr_tiles(p, LF_ROWS) : 0;
     return (long long)p.T * width;
 }
 
