@@ -984,6 +984,15 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
             if (sent) slots[1] = next;
             else slots[0] = next;
         }
+        auto load_next = [&]() {                             // once what was stored has been read
+            if (sent >= turns_mine) return;
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+            load(sent);
+            if (sent % L::SLOTS) slots[1] = next;
+            else slots[0] = next;
+            ++sent;
+        };
         tg_before();
         __syncthreads();
         tg_after();
@@ -997,6 +1006,7 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
             ok = __all_sync(0xffffffffu, tg_wait(&acc_full[buf], (i >> 1) & 1, &low_rank_error_flag, 7));
             if (ok) ok = __all_sync(0xffffffffu, tg_wait(&there[slot], (i / L::SLOTS) & 1, &low_rank_error_flag, 8));
             if (!ok) break;
+            if (L::SLOTS == 2 && i > 0) load_next();         // where the turn before lay
             tg_after();
             unsigned char* const at = ring + slot * L::Y_BYTES;
             // a row of 128 bytes a lane, its 16-byte pieces swapped by the row's place among eight
@@ -1053,16 +1063,7 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
                     }
             }
             if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");     // with or without a store: a group a turn
-            // The next load goes where the turn before lay (with one slot: this turn), once its store has been read: this
-            // turn's may still be.
-            if ((L::SLOTS == 1 || i > 0) && sent < turns_mine) {
-                asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(L::SLOTS - 1) : "memory");
-                __syncwarp();
-                load(sent);
-                if (sent % L::SLOTS) slots[1] = next;
-                else slots[0] = next;
-                ++sent;
-            }
+            if (L::SLOTS == 1) load_next();
         }
         if (!ok && lane == 0) tg_settle_copies(there, L::SLOTS, sent, &low_rank_error_flag, 8);
         // rows without an adapter: y as it is, 128 vectors of a row a warp and turn
