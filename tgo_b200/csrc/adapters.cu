@@ -56,13 +56,38 @@ struct LowRank {
 #define LP_HELD 8                 // rows a thread holds; more are read twice
 static_assert((LP_WARPS + 2) * (LP_ORDERED + 1) <= 3 * (LP_MAX_ADAPTERS + 1), "the plan's shared memory");
 
+// Rows that the kernels after the plan read, for the blocks after the first to ask for into L2 while the first plans and u,
+// which does not fill the memory's time, is made: the first `many` of each matrix, x before y. MEASURED (us, without, 32 MB, 64
+// MB, 96 MB): 1833 rows, rank 32, gate and up of 12288 53.0, 50.8, 51.3, 51.6; 8192 rows, rank 64, q, k and v 68.8, 67.1, 66.9, 67.5.
+#define LP_AHEAD 48000000
+#define LP_PIECE 4096             // bytes asked for at once, at most
+struct LowRankAhead {
+    const char* from[2];
+    long long stride[2];          // bytes
+    int bytes[2], many[2];        // of a row; rows
+    int all;                      // rows without an adapter, too
+};
+
 __global__ void __launch_bounds__(LP_THREADS)
 low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile, int* __restrict__ perm, int* __restrict__ info,
-                     int* __restrict__ tiles) {
+                     int* __restrict__ tiles, const LowRankAhead ahead) {
     __shared__ int pool[3 * (LP_MAX_ADAPTERS + 1)];
     __shared__ int warp_rows[LP_WARPS], warp_tiles[LP_WARPS];
     pdl_wait();
     pdl_launch_late();                                       // the next kernel's blocks may come and wait: 0.8 us
+    if (blockIdx.x > 0) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const int pieces = (ahead.bytes[m] + LP_PIECE - 1) / LP_PIECE;
+            for (int e = threadIdx.x * (gridDim.x - 1) + blockIdx.x - 1; e < ahead.many[m] * pieces; e += (gridDim.x - 1) * LP_THREADS) {
+                const int r = e / pieces, at = (e - r * pieces) * LP_PIECE, id = ids[r];
+                if (ahead.all || (id >= 0 && id < adapters))
+                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(ahead.from[m] + r * ahead.stride[m] + at),
+                                 "r"(min(LP_PIECE, ahead.bytes[m] - at)));
+            }
+        }
+        return;
+    }
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, slots = adapters + 1;
     const bool ordered = adapters <= LP_ORDERED;
     int* const rows_before = pool;
@@ -517,11 +542,11 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
 // u (`low_rank_u_kernel`): X[rows] A^T on tcgen05, a cluster 64 or 128 rows, a part of k a block: TMA brings 64 columns of
 // the rows (one box where they lie together, else four rows a request) and of A into a ring, a thread issues the products.
 // Each block sends its sums to the blocks that add them, by rows, through their shared memory; these scale u and split it.
-// Bound by x's way into the multiprocessors: 28 of the 72 us of 8192 rows, width 4096, rank 64, q, k and v.
+// Bound by x's way into the multiprocessors: 26 of the 67 us of 8192 rows, width 4096, rank 64, q, k and v.
 //
 // out (`low_rank_out_kernel`): u and 64 columns of B at a time come by TMA, a thread issues the products into four
 // accumulators in turn, eight warps add them to y in shared memory, from where TMA stores it. Bound by y's and out's way:
-// 40 of the 72 us, 5 TB/s.
+// 36 of the 67 us, 5.6 TB/s.
 #define LT_ROWS 128
 #define LT_BK 64
 #define LT_STAGES 6               // of the ring, at most 8
@@ -739,8 +764,9 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
 // from tensor memory, a lane a row) of every other turn and a ring of its own of 32 x 64 tiles; it adds the sums where
 // y lies and has the tile stored from there. Rows that lie together are one box either way; others come four at a time and are written by
 // the warp, as are part tiles. As many blocks as fit share all tiles' turns out evenly, so that a block's first reads are waited
-// for once. (Blocks of eight turns each: the call took 63 us where it takes 57, 1833 rows, gate and up of 12288, rank 32. Reading y into registers two steps ahead and writing from them, through a transposing
-// buffer, took 68 us where this takes 40: 8192 rows of 6144 columns, rank 64.)
+// for once. MEASURED (the call, us): 1833 rows, rank 32, gate and up of 12288, blocks of eight turns each 63, these 57, with the next
+// tile of y asked for before this one is made, not after, 53. Reading y into registers two steps ahead and writing from them, through
+// a transposing buffer, took 68 us for 8192 rows of 6144 columns, rank 64, where this takes 36.
 #define LO_COLS 64
 #define LO_HANDS 8                // warps that hand on; the one after them asks for copies and products
 #define LO_THREADS (LO_HANDS * 32 + 32)
@@ -1174,7 +1200,7 @@ template <typename T, typename TY> static int low_rank_few(const LowRank& p, int
         perm = plan;
         info = perm + p.T;
         tiles = info + LP_INFO;
-        const int rc = tgo_launch_pdl(low_rank_plan_kernel, dim3(1), dim3(LP_THREADS), 0, stream, p.ids, p.T, p.adapters, LF_ROWS, perm, info, tiles);
+        const int rc = tgo_launch_pdl(low_rank_plan_kernel, dim3(1), dim3(LP_THREADS), 0, stream, p.ids, p.T, p.adapters, LF_ROWS, perm, info, tiles, LowRankAhead{});
         if (rc) return rc;
     }
     cudaLaunchConfig_t cfg = {};
@@ -1322,7 +1348,15 @@ template <typename TY> static int low_rank_tiles(const LowRank& p, int* work, cu
     int* const info = perm + p.T;
     int* const tiles = info + LP_INFO;
     bf16* const u = (bf16*)(work + (p.T + LP_INFO + 3 * lr_tiles(p, LT_ROWS) + 3) / 4 * 4);
-    int rc = tgo_launch_pdl(low_rank_plan_kernel, dim3(1), dim3(LP_THREADS), 0, stream, p.ids, p.T, p.adapters, LT_ROWS, perm, info, tiles);
+    LowRankAhead ahead = {{(const char*)p.x, (const char*)p.y}, {p.x_stride * 2, p.y_stride * (long long)sizeof(TY)},
+                          {p.K * 2, p.N * (int)sizeof(TY)}, {}, p.out != p.y};
+    long long left = LP_AHEAD;
+    for (int m = 0; m < 2; ++m) {
+        ahead.many[m] = (int)(left / ahead.bytes[m] < p.T ? left / ahead.bytes[m] : p.T);
+        left -= (long long)ahead.many[m] * ahead.bytes[m];
+    }
+    int rc = tgo_launch_pdl(low_rank_plan_kernel, dim3(1 + 2 * tgo_multiprocessors()), dim3(LP_THREADS), 0, stream, p.ids, p.T, p.adapters,
+                            LT_ROWS, perm, info, tiles, ahead);
     if (rc) return rc;
     const LowRankTile g = lr_plan(p);
     const int cols = g.cuts * g.cut;
