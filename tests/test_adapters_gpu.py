@@ -192,6 +192,15 @@ def test_infinite_products(x_type, T):
     assert torch.equal(out[1].float(), want) and torch.isfinite(out[torch.arange(T) != 1]).all()
 
 
+@pytest.mark.parametrize("x_type", [F32, BF])
+@pytest.mark.parametrize("T", [255, 257, 511, 512, 513])
+@pytest.mark.parametrize("adapters", [1, 255, 256])
+def test_rows_found_and_planned(x_type, T, adapters):
+    """Both sides of the numbers of rows and adapters up to which a call needs no plan."""
+    ids = torch.randint(-2, adapters + 1, (T,), generator=torch.Generator().manual_seed(T + adapters)).to(torch.int32)
+    check(inputs(T, 64, (32,), 8, adapters, x_type, x_type, seed=T, ids=ids), (32,))
+
+
 @pytest.mark.parametrize("T,K,widths,rank", [(1210, 2048, (2048,), 64), (700, 1024, (1536, 512, 512), 72)])
 def test_sizes_that_go_by_tiles(T, K, widths, rank):
     check(inputs(T, K, widths, rank, 3, BF, BF, seed=T), widths)

@@ -232,8 +232,8 @@ low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile,
 // float32: plain sums, a warp four values of u for all eight rows, its lanes over k; u's and the result's
 // order of additions depends on K and the rank alone, whatever the batch.
 //
-// Without a plan (up to 256 rows) each cluster finds its rows by itself: a thread a row counts the rows of the same
-// adapter before it, every eighth begins a group, and the cluster takes the group of its number. Half a microsecond,
+// Without a plan (up to 512 rows and 255 adapters) each cluster finds its rows by itself: a thread a row counts the rows of the
+// same adapter before it, every eighth begins a group, and the cluster takes the group of its number. Under a microsecond,
 // where a plan of its own takes four. (A single row has nothing to look for: 4.2 us, 4.5 with it.)
 #define LF_ROWS 8
 #define LF_CTAS 8
@@ -243,6 +243,8 @@ low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile,
 #define LF_TILES 2                // tiles of 16 columns a warp has under way, bfloat16
 #define LR_SCAN_TURNS 2           // rows a thread looks at
 #define LR_SCAN_ROWS (LR_SCAN_TURNS * LF_THREADS)
+#define LR_SCAN_ADAPTERS 255      // their counts' places, and one for none
+static_assert(LR_SCAN_ADAPTERS + 1 == LF_THREADS && LR_SCAN_TURNS * LF_WARPS == 16, "sixteen counts of 32 rows a thread's adapter");
 static_assert(LF_ROWS == LF_WARPS, "a warp a row");
 
 __device__ __forceinline__ void lf_cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(LF_THREADS, 3)
 low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __restrict__ info, const int* __restrict__ tiles) {
     extern __shared__ __align__(16) float lf_smem[];
     __shared__ int rows[LF_ROWS];
-    __shared__ __align__(16) int ids[LR_SCAN_ROWS];
+    __shared__ __align__(16) unsigned char counts[LF_THREADS][LR_SCAN_TURNS * LF_WARPS];
     __shared__ int warp_count[LR_SCAN_TURNS * LF_WARPS], group[2];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int item = blockIdx.x / LF_CTAS, cta = blockIdx.x % LF_CTAS;
@@ -285,30 +287,35 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
         if (t == 0) rows[0] = 0;
         __syncthreads();
     } else {
-        // up to LR_SCAN_TURNS rows a thread: which adapter, how many rows of it before, and whether it begins a group
+        // LR_SCAN_TURNS rows a thread: which adapter, how many rows of it before (counted by the 32 rows of a warp), and
+        // whether it begins a group
         int mine[LR_SCAN_TURNS], before[LR_SCAN_TURNS], all = 0;
         unsigned who[LR_SCAN_TURNS];
+        *(uint4*)counts[t] = make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int h = 0; h < LR_SCAN_TURNS; ++h) {
             const int r = h * LF_THREADS + t;
             mine[h] = r < p.T ? p.ids[r] : -2;
             if (r < p.T && (mine[h] < 0 || mine[h] >= p.adapters)) mine[h] = -1;
-            ids[r] = mine[h];
         }
         __syncthreads();
 #pragma unroll
         for (int h = 0; h < LR_SCAN_TURNS; ++h) {
-            const int r = h * LF_THREADS + t;
-            before[h] = 0;
-            if (r - lane < p.T) {                            // the warps before, then this one
-#pragma unroll 8
-                for (int j = 0; j < r - lane; j += 4) {
-                    const int4 q = *(const int4*)(ids + j);
-                    before[h] += (q.x == mine[h]) + (q.y == mine[h]) + (q.z == mine[h]) + (q.w == mine[h]);
-                }
-                before[h] += __popc(__match_any_sync(0xffffffffu, mine[h]) & ((1u << lane) - 1));
+            const unsigned same = __match_any_sync(0xffffffffu, mine[h]);
+            before[h] = __popc(same & ((1u << lane) - 1));
+            if (mine[h] >= -1 && before[h] == 0) counts[mine[h] & 255][h * LF_WARPS + warp] = (unsigned char)__popc(same);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < LR_SCAN_TURNS; ++h) {
+            const uint4 q = *(const uint4*)counts[mine[h] & 255];
+            const unsigned word[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int k = h * LF_WARPS + warp - 4 * i;   // bytes of it that count
+                before[h] = (int)__dp4a(k >= 4 ? word[i] : k > 0 ? word[i] & ((1u << 8 * k) - 1) : 0u, 0x01010101u, (unsigned)before[h]);
             }
-            who[h] = __ballot_sync(0xffffffffu, r < p.T && before[h] % LF_ROWS == 0);
+            who[h] = __ballot_sync(0xffffffffu, mine[h] >= -1 && before[h] % LF_ROWS == 0);
             if (lane == 0) warp_count[h * LF_WARPS + warp] = __popc(who[h]);
         }
         __syncthreads();
@@ -405,7 +412,7 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
         }
     } else {
         // x in shared memory, a warp a row. Three blocks a multiprocessor are asked for: 347 rows of three adapters, width
-        // 2048, 3072 columns, rank 8 14.0 us, with two 18.8.
+        // 2048, 3072 columns, rank 8 14.0 us, with two 18.8 (10.6 since the clusters find their rows).
         const int kc = ((K + LF_CTAS - 1) / LF_CTAS + 3) / 4 * 4, k0 = min(cta * kc, K), k1 = min(k0 + kc, K);
         float* const xs = tail;                              // [row][k of the block]
 #pragma unroll 4
@@ -1172,9 +1179,10 @@ template <typename T> static bool lr_vectors(const LowRank& p) {
 
 // Rows from which they are planned: up to here each cluster of the kernel for few rows finds its own.
 
+static bool lr_scanned(const LowRank& p) { return p.T <= LR_SCAN_ROWS && p.adapters <= LR_SCAN_ADAPTERS; }
 template <typename T> static bool lr_few_takes(const LowRank& p) {
     return lr_vectors<T>(p) && lf_floats<T>(p.columns.slices * p.rank, p.K) * 4 <= 200 * 1024 && p.T <= (1 << 24) &&
-           (p.T <= LR_SCAN_ROWS || p.adapters <= LP_MAX_ADAPTERS);
+           (lr_scanned(p) || p.adapters <= LP_MAX_ADAPTERS);
 }
 
 // Tiles there are at most: with an adapter's first row comes one, with every `tile` further ones another.
@@ -1196,7 +1204,7 @@ template <typename T, typename TY> static int low_rank_few(const LowRank& p, int
     }
     const long long items = lr_tiles(p, LF_ROWS);
     int *perm = nullptr, *info = nullptr, *tiles = nullptr;
-    if (p.T > LR_SCAN_ROWS) {
+    if (!lr_scanned(p)) {
         perm = plan;
         info = perm + p.T;
         tiles = info + LP_INFO;
@@ -1371,16 +1379,18 @@ template <typename TY> static int low_rank_tiles(const LowRank& p, int* work, cu
 }
 
 #define LR_TILE_BYTES 40000000ll
-// Whether a call goes by tiles of 128 rows: three kernels take 17 us however few the rows are; the clusters read an
-// adapter again for every eight rows, at about 3 TB/s. So from 40 MB of such reading on. MEASURED (us, clusters / tiles;
-// rows in four runs, then of 24 adapters at random): width 4096, q, k and v, rank 16, 384 rows 18 / 19 and 21 / 26, 768
-// 31 / 20 and 33 / 29; rank 64, 128 rows 31 / 21 and 31 / 34, 384 36 / 23 and 44 / 36; gate and up of 12288, rank 32, 128
-// rows 39 / 21 and 40 / 50, 512 53 / 24 and 100 / 59; 2048 x 2048, rank 16, 1024 rows 18 / 22 and 20 / 39.
+#define LR_TILE_ROWS 1024
+// Whether a call goes by tiles of 128 rows: three kernels take 15 us however few the rows are, and each further adapter a
+// part tile; the clusters read an adapter again for every eight rows, at about 3 TB/s, and come in rounds of 444 blocks. So
+// from 40 MB of such reading or 1024 rows on. MEASURED (us, clusters / tiles; rows in four runs, then of 24 adapters at
+// random): width 4096, q, k and v, rank 16, 384 rows 13 / 17 and 23 / 28, 768 28 / 19 and 36 / 33; rank 64, 96 rows 19 / 19 and
+// 24 / 35, 256 25 / 19 and 30 / 37, 384 32 / 19 and 53 / 39; gate and up of 12288, rank 32, 128 rows 27 / 21 and 27 / 45, 384
+// 38 / 21 and 69 / 54; 2048 x 2048, rank 16, 768 rows 15 / 15 and 20 / 24, 1536 25 / 17 and 31 / 27.
 static int lr_forced = 0;                                    // for tests: 1 clusters, 2 tiles; 0: by the rule
 TGO_API void tgo_low_rank_force_way(int way) { lr_forced = way; }
 static bool lr_many(const LowRank& p) {
     if (lr_forced) return lr_forced == 2;
-    return (long long)p.T * p.rank * ((long long)p.columns.slices * p.K + p.N) * 2 / LF_ROWS >= LR_TILE_BYTES;
+    return p.T >= LR_TILE_ROWS || (long long)p.T * p.rank * ((long long)p.columns.slices * p.K + p.N) * 2 / LF_ROWS >= LR_TILE_BYTES;
 }
 
 template <typename T, typename TY> static int low_rank_any(const LowRank& p, float* u, cudaStream_t stream) {
@@ -1399,7 +1409,7 @@ template <typename T, typename TY> static long long lr_work(const LowRank& p) {
     const int width = p.columns.slices * p.rank;
     if constexpr (sizeof(T) == 2)
         if (lr_many(p) && lr_tile_takes<TY>(p)) return lr_tile_work(p);
-    if (lr_few_takes<T>(p)) return p.T > LR_SCAN_ROWS ? p.T + LP_INFO + 3 * lr_tiles(p, LF_ROWS) : 0;
+    if (lr_few_takes<T>(p)) return !lr_scanned(p) ? p.T + LP_INFO + 3 * lr_tiles(p, LF_ROWS) : 0;
     return (long long)p.T * width;
 }
 
@@ -1427,7 +1437,7 @@ TGO_API int tgo_low_rank_error(int* value) { return (int)cudaMemcpyFromSymbol(va
 
 // x [T, K] of type dt, y and out [T, N] of type dt_y, rows strided; out may be y. a [adapters, slices, rank, K],
 // b [adapters, N, rank] of type dt; ends: the column after each slice's last. `work` holds `work_ints` 32-bit
-// numbers and lies on 16 bytes; LR_E_WORK: too few (for up to 256 rows most calls need none). With `needs` given
+// numbers and lies on 16 bytes; LR_E_WORK: too few (for up to 512 rows most calls need none). With `needs` given
 // nothing runs, and it gets how many the call needs.
 TGO_API int tgo_low_rank_add(const void* x, long long x_stride, const void* y, long long y_stride, void* out,
                              long long out_stride, const void* a, const void* b, const float* scale, const int* ids,
