@@ -412,7 +412,7 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
         }
     } else {
         // x in shared memory, a warp a row. Three blocks a multiprocessor are asked for: 347 rows of three adapters, width
-        // 2048, 3072 columns, rank 8 14.0 us, with two 18.8 (10.6 since the clusters find their rows).
+        // 2048, 2048 + 512 + 512 columns, rank 8 14.0 us, with two 18.8 (10.6 since the clusters find their rows).
         const int kc = ((K + LF_CTAS - 1) / LF_CTAS + 3) / 4 * 4, k0 = min(cta * kc, K), k1 = min(k0 + kc, K);
         float* const xs = tail;                              // [row][k of the block]
 #pragma unroll 4
@@ -570,7 +570,8 @@ struct LowRankTile {
 // Bytes of the ring, which later holds a pass of sums.
 __host__ __device__ static inline int lt_ring(const LowRankTile& g) {
     // with 64 rows the products read on for 64 more, into whatever lies there
-    const int ring = g.stages * (g.rows * LT_BK * 2 + g.cuts * g.cut * LT_BK * 2) + (LT_ROWS - g.rows) * LT_BK * 2, pass = (g.width < LT_PASS ? (g.width + 31) / 32 * 32 : LT_PASS) * g.rows * 4;
+    const int ring = g.stages * (g.rows * LT_BK * 2 + g.cuts * g.cut * LT_BK * 2) + (LT_ROWS - g.rows) * LT_BK * 2;
+    const int pass = (g.width < LT_PASS ? (g.width + 31) / 32 * 32 : LT_PASS) * g.rows * 4;
     return ring > pass ? ring : pass;
 }
 

@@ -2162,15 +2162,15 @@ def reorder_rows(tensors, index: torch.Tensor, parents: torch.Tensor, axis: int 
     for t in tensors:
         if not t.is_cuda:
             _need_cuda(t)
-        shape, size = t.shape, t.element_size()
+        shape, size, numel = t.shape, t.element_size(), t.numel()
         assert 0 <= axis < len(shape) and size >= 2
-        outer, rows = math.prod(shape[:axis]), shape[axis]
-        row = math.prod(shape[axis + 1:]) * size
-        if outer == 0 or rows == 0 or row == 0:
+        if numel == 0:
             continue
-        step = t.stride()[axis] * size if rows > 1 else row
-        # whole rows, and whatever precedes the rows evenly spaced
-        assert t.is_contiguous() or (axis == 0 and t[0].is_contiguous() and step >= row)
+        outer, rows = math.prod(shape[:axis]), shape[axis]
+        row = step = numel // (outer * rows) * size
+        if not t.is_contiguous():            # whole rows, and whatever precedes the rows evenly spaced
+            step = t.stride()[axis] * size if rows > 1 else row
+            assert axis == 0 and t[0].is_contiguous() and step >= row
         desc.extend((t.data_ptr(), outer, rows * step, rows, step, row))
     if not desc or G == 0:
         return
@@ -2209,10 +2209,11 @@ def low_rank_add(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.Ten
         raise KernelError(f"low_rank_add: slices {tuple(widths)}{' in eights' if interleaved else ''} of {N} columns")
     if T == 0:
         return
+    code = dtype_code(kind)
     ends = array("i", itertools.accumulate(widths))
     call = entry_points("adapters").tgo_low_rank_add
     args = (x.data_ptr(), xs, y.data_ptr(), ys, out.data_ptr(), os, a.data_ptr(), b.data_ptr(), scale.data_ptr(),
-            ids.data_ptr(), dtype_code(kind), dtype_code(kind_y), T, K, N, n, r, S, ends.buffer_info()[0],
+            ids.data_ptr(), code, code if kind_y is kind else F32, T, K, N, n, r, S, ends.buffer_info()[0],
             1 if interleaved else 0)
     if T <= LOW_RANK_SCANNED:               # most such calls need no workspace
         status = call(*args, 0, 0, 0, _stream())

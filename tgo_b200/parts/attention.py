@@ -228,7 +228,7 @@ class GQAAttention(Part):
     def _output(self, a, ctx, residual):
         """The output product, and what the rows' adapters add to it."""
         y = ops.linear(a, self.w_o, residual=residual)
-        if ctx.adapters is not None and "o" in self.adapters:
+        if "o" in self.adapters and ctx.adapters is not None:
             self.adapters["o"].add(a, residual if y is None else y, ctx)
         return y
 
@@ -287,10 +287,10 @@ class GQAAttention(Part):
         qw, kw = H * dh, Hkv * dh
         if cache.writable:
             qkv = ops.linear(x, self.w_qkv)           # x may be ops.NormedRows: folded in there
-            if ctx.adapters is not None and "qkv" in self.adapters:
+            if "qkv" in self.adapters and ctx.adapters is not None:
                 self.adapters["qkv"].add(x, qkv, ctx)
             q, k, v = qkv[:, :qw], qkv[:, qw:qw + kw], qkv[:, qw + kw:]
-        elif ctx.adapters is not None and "qkv" in self.adapters:
+        elif "qkv" in self.adapters and ctx.adapters is not None:
             # the queries alone, of an adapter that is laid out for all three
             qkv = torch.zeros((x.shape[0], qw + 2 * kw), dtype=x.dtype, device=x.device)
             qkv[:, :qw] = ops.linear(x, self.w_q)

@@ -126,7 +126,7 @@ class SwiGLU(Part):
     def forward(self, x, ctx, residual=None):
         """With `residual` (the float32 stream) the result may be added to it, and None is
         then returned; otherwise the result is returned for the caller to add."""
-        if ctx.adapters is not None and self.adapters:
+        if self.adapters and ctx.adapters is not None:
             return self._adapted(x, ctx, residual)
         if self.bias:
             act = ops.gated_linear(x, self.w_gate_up, self.interleaved, self.activation,
