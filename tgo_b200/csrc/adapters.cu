@@ -774,7 +774,7 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
 // the warp, as are part tiles. As many blocks as fit share all tiles' turns out evenly, so that a block's first reads are waited
 // for once. MEASURED (the call, us): 1833 rows, rank 32, gate and up of 12288, blocks of eight turns each 63, these 57, with the next
 // tile of y asked for before this one is made, not after, 53. Reading y into registers two steps ahead and writing from them, through
-// a transposing buffer, took 68 us for 8192 rows of 6144 columns, rank 64, where this takes 36.
+// a transposing buffer, took 68 us for 8192 rows of 6144 columns, rank 64, where the kernel takes 36.
 #define LO_COLS 64
 #define LO_HANDS 8                // warps that hand on; the one after them asks for copies and products
 #define LO_THREADS (LO_HANDS * 32 + 32)
@@ -1248,8 +1248,8 @@ static int lt_bytes(const LowRankTile& g) { return lt_ring(g) + 1024 + 256; }
 // multiprocessor (70 bytes a cycle) or its part of the way of all blocks' rows from memory (3400); to begin and end
 // takes 6000, to exchange sums 1500 and a cycle for four. (The tiles that the rows make at least, and one: how many more is
 // the device's to know.) MEASURED, all three kernels, us, 1, 2, 4 and 8 parts: 8192 rows, rank 64, q, k and v, clusters of
-// 128 rows 80, 72 (taken), 83, 118, of 64 74, 81, 98, 140; 1833 rows, rank 32, gate and up, 128 rows 73, 68, 65, 70, 64 rows
-// 72, 66, 64 (taken), 64.
+// 128 rows 74, 67 (taken), 78, 112, of 64 69, 76, 93, 135; 1833 rows, rank 32, gate and up, 128 rows 60, 54, 51, 56, 64 rows
+// 60, 53, 51 (taken), 51.
 static LowRankTile lr_plan(const LowRank& p) {
     LowRankTile best = {};
     long long least = -1;
