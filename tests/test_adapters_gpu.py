@@ -138,6 +138,15 @@ def test_strided_rows(x_type, y_type, T):
 
 
 @pytest.mark.parametrize("x_type", [F32, BF])
+@pytest.mark.parametrize("T", [1, 40, 700])
+def test_one_row_for_all(x_type, T):
+    """x expanded from a single row."""
+    p = inputs(T, 256, (128, 64), 16, 3, x_type, x_type, seed=T)
+    p["x"] = p["x"][:1].expand(T, 256)
+    check(p, (128, 64))
+
+
+@pytest.mark.parametrize("x_type", [F32, BF])
 @pytest.mark.parametrize("kind", ["none", "one", "all different", "runs", "outside"])
 @pytest.mark.parametrize("T", [1, 9, 96, 700])
 def test_mixtures_of_adapters(x_type, kind, T):
@@ -236,6 +245,11 @@ def test_refusals():
                   dict(b=p["b"][:, :40]), dict(scale=p["scale"][:1]), dict(x=p["x"][:2])):
         with pytest.raises(AssertionError):
             call(**wrong)
+    for widths in ((32, 16, 0), (64, -16)):
+        with pytest.raises((o.KernelError, AssertionError)):
+            call(widths=widths)
+    with pytest.raises(AssertionError):
+        call(y=torch.zeros(1, 48, dtype=BF, device=DEV).expand(3, 48))
     with pytest.raises(o.KernelError, match="CUDA device"):
         call(x=p["x"].cpu())
     with pytest.raises(o.KernelError):

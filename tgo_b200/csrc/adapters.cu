@@ -1232,6 +1232,7 @@ template <typename T, typename TY> static int low_rank_few(const LowRank& p, int
 // Whether the kernels for many rows take a call: what they read and write on 16 bytes, A's columns in tensor memory.
 template <typename TY> static bool lr_tile_takes(const LowRank& p) {
     const int v = 16 / (int)sizeof(TY), width = p.columns.slices * p.rank;
+    if (p.x_stride < p.K || p.y_stride < p.N || p.out_stride < p.N) return false;      // rows over each other (an expanded x)
     if (!lr_vectors<bf16>(p) || p.rank % 8 || p.rank > 128 || width > LT_MAX_WIDTH || p.adapters > LP_MAX_ADAPTERS ||
         p.T > (1 << 24) || (long long)p.adapters * width > 0x7fffffff || (long long)p.adapters * p.N > 0x7fffffff || p.y_stride % v || p.out_stride % v ||
         ((uintptr_t)p.y | (uintptr_t)p.out) & 15)
@@ -1422,31 +1423,36 @@ template <typename T, typename TY> static int low_rank_launch(const LowRank& p, 
     return low_rank_any<T, TY>(p, (float*)work, stream);
 }
 
-static bool lr_fill(LowRank& p, int T, int K, int N, int adapters, int rank, int slices, const int* ends, int interleaved) {
+static bool lr_fill(LowRank& p, int T, int K, int N, int adapters, int rank, int slices, const int* widths, int interleaved) {
     if (T <= 0 || K <= 0 || N <= 0 || adapters <= 0 || rank <= 0 || slices <= 0 || slices > LR_MAX_SLICES ||
-        (N + 255) / 256 > 65535 || (interleaved && (slices != 2 || N % 16)))
+        (N + 255) / 256 > 65535 || (interleaved && (slices != 2 || widths[0] != widths[1] || widths[0] % 8)))
         return false;
     p.T = T; p.K = K; p.N = N; p.adapters = adapters; p.rank = rank;
     p.columns.slices = slices;
     p.columns.interleaved = interleaved;
-    for (int i = 0; i < slices; ++i) p.columns.ends[i] = ends[i];
-    return true;
+    long long end = 0;
+    for (int i = 0; i < slices; ++i) {
+        end += widths[i];
+        if (widths[i] <= 0 || end > N) return false;
+        p.columns.ends[i] = (int)end;
+    }
+    return end == N;
 }
 
 // The code that a wait of the kernels for many rows left when it ran out, or 0. Synchronises.
 TGO_API int tgo_low_rank_error(int* value) { return (int)cudaMemcpyFromSymbol(value, low_rank_error_flag, sizeof(int)); }
 
 // x [T, K] of type dt, y and out [T, N] of type dt_y, rows strided; out may be y. a [adapters, slices, rank, K],
-// b [adapters, N, rank] of type dt; ends: the column after each slice's last. `work` holds `work_ints` 32-bit
+// b [adapters, N, rank] of type dt; widths: each slice's columns. `work` holds `work_ints` 32-bit
 // numbers and lies on 16 bytes; LR_E_WORK: too few (for up to 512 rows most calls need none). With `needs` given
 // nothing runs, and it gets how many the call needs.
 TGO_API int tgo_low_rank_add(const void* x, long long x_stride, const void* y, long long y_stride, void* out,
                              long long out_stride, const void* a, const void* b, const float* scale, const int* ids,
-                             int dt, int dt_y, int T, int K, int N, int adapters, int rank, int slices, const int* ends,
+                             int dt, int dt_y, int T, int K, int N, int adapters, int rank, int slices, const int* widths,
                              int interleaved, void* work, long long work_ints, long long* needs, cudaStream_t stream) {
     if (T <= 0) return 0;
     LowRank p = {x, y, a, b, out, x_stride, y_stride, out_stride, scale, ids};
-    if (!lr_fill(p, T, K, N, adapters, rank, slices, ends, interleaved)) return TGO_E_BAD_ARG;
+    if (!lr_fill(p, T, K, N, adapters, rank, slices, widths, interleaved)) return TGO_E_BAD_ARG;
     if (dt == TGO_F32 && dt_y == TGO_F32) {
         if (needs) { *needs = lr_work<float, float>(p); return 0; }
         return low_rank_launch<float, float>(p, work, work_ints, stream);

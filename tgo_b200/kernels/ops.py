@@ -7,7 +7,6 @@ nothing falls back to it. A refused size raises with the kernel's name in the me
 from __future__ import annotations
 
 import ctypes
-import itertools
 import math
 from array import array
 from operator import index
@@ -2204,16 +2203,13 @@ def low_rank_add(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.Ten
     (xs, x1), (ys, y1), (os, o1) = x.stride(), y.stride(), out.stride()
     assert x1 == y1 == o1 == 1 and scale.dtype == torch.float32 and scale.shape == (n,)
     assert ids.dtype == torch.int32 and ids.shape == (T,)
-    if sum(widths) != N or not 0 < S <= 4 or min(widths) <= 0 or \
-            (interleaved and (S != 2 or widths[0] != widths[1] or widths[0] % 8)):
-        raise KernelError(f"low_rank_add: slices {tuple(widths)}{' in eights' if interleaved else ''} of {N} columns")
+    assert T <= 1 or os >= N
     if T == 0:
         return
-    code = dtype_code(kind)
-    ends = array("i", itertools.accumulate(widths))
+    code, columns = dtype_code(kind), array("i", widths)
     call = entry_points("adapters").tgo_low_rank_add
     args = (x.data_ptr(), xs, y.data_ptr(), ys, out.data_ptr(), os, a.data_ptr(), b.data_ptr(), scale.data_ptr(),
-            ids.data_ptr(), code, code if kind_y is kind else F32, T, K, N, n, r, S, ends.buffer_info()[0],
+            ids.data_ptr(), code, code if kind_y is kind else F32, T, K, N, n, r, S, columns.buffer_info()[0],
             1 if interleaved else 0)
     if T <= LOW_RANK_SCANNED:               # most such calls need no workspace
         status = call(*args, 0, 0, 0, _stream())
@@ -2227,7 +2223,8 @@ def low_rank_add(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.Ten
         work = x.new_empty(needs, dtype=torch.int32)
         status = call(*args, work.data_ptr(), needs, 0, _stream())
         LAUNCHES[0] += 1
-    _check(status, "low_rank_add", f"(T={T}, K={K}, N={N}, rank={r}, slices={S})" if status else "")
+    _check(status, "low_rank_add", f"(T={T}, K={K}, rank={r}, slices {tuple(widths)}{' in eights' if interleaved else ''} "
+                                   f"of {N} columns)" if status else "")
 
 
 def low_rank_force_way(way: int = 0) -> None:
