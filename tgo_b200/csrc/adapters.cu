@@ -223,7 +223,9 @@ low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile,
 // A cluster of eight blocks takes up to eight rows of one adapter. Each block forms u over an eighth of k,
 // the blocks read each other's sums from shared memory, and each then makes an eighth of the columns: one
 // launch, and every number of A and B is read once for eight rows. Bound by the adapters' way from memory or
-// L2 when many rows have one each, by latency for a handful.
+// L2 when many rows have one each, by latency for a handful. MEASURED (us, clusters of 4, 8, 16): one row, rank 16, 2048 x 2048
+// 5.1, 4.1, 4.4; 96 rows of 24 adapters, rank 16, q, k and v of width 4096 12.5, 10.0, 18.0; 347 float32 rows of three adapters,
+// rank 8, q, k and v of width 2048 12.4, 10.6, 19.1.
 //
 // bfloat16: the adapter's rows are the 16 rows of mma.sync products, the batch's rows their 8 columns, both
 // straight from memory into the operands' registers: which 16 values of k meet in a product does not
