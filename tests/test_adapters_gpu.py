@@ -215,6 +215,20 @@ def test_sizes_that_go_by_tiles(T, K, widths, rank):
     check(inputs(T, K, widths, rank, 3, BF, BF, seed=T), widths)
 
 
+@pytest.mark.parametrize("T,widths,rank,interleaved", [
+    (1, (64,), 16, False), (40, (96, 64), 32, False), (300, (64,), 8, False), (333, (128, 32), 16, False), (700, (256,), 64, False),
+    (520, (96,), 128, False), (400, (64, 64), 16, True), (260, (160, 160), 64, True), (300, (64, 64), 128, True)])
+def test_float32_rows_of_bfloat16_products(T, widths, rank, interleaved):
+    """What is added to float32 rows is as exact as 32 bits make it: the errors of 64 + rank additions of random signs come to
+    sqrt(64 + rank) 2^-24 of the sum, below 2^-20; two bfloat16 parts of u alone would be off by 2^-18."""
+    p = inputs(T, 64, widths, rank, 3, BF, F32, seed=rank, ids=(torch.arange(T) // 50 % 3).to(torch.int32))
+    p["y"].zero_()
+    want, _ = plain(p["x"], p["y"], p["a"], p["b"], p["scale"], p["ids"], widths, interleaved)
+    ops().low_rank_add(p["x"], p["y"], p["a"], p["b"], p["scale"], p["ids"], widths, interleaved)
+    off = (p["y"].double().cpu() - want).norm() / want.norm()
+    assert off < 2.0 ** -20, float(off) * 2 ** 20
+
+
 def test_no_rows_and_other_streams():
     p = inputs(0, 64, (32,), 8, 2, BF, BF, seed=1)
     ops().low_rank_add(p["x"], p["y"], p["a"], p["b"], p["scale"], p["ids"], (32,))

@@ -16,13 +16,17 @@ struct LowRankColumns {
     int interleaved;              // eight columns of slice 0, eight of slice 1, and so on
 };
 
-// Four values of u as the second product takes them: each rounded to bfloat16 (x, y) and what that left out, rounded
-// too (z, w). An infinity leaves nothing out.
-__device__ __forceinline__ uint4 lr_split(float4 v) {
-    auto rest = [](float f, uint32_t rounded) { const float h = __uint_as_float(rounded); return f == h ? 0.f : f - h; };
-    const uint32_t a = pack_bf16(v.x, v.y), b = pack_bf16(v.z, v.w);
-    return make_uint4(a, b, pack_bf16(rest(v.x, a << 16), rest(v.y, a & 0xffff0000u)), pack_bf16(rest(v.z, b << 16), rest(v.w, b & 0xffff0000u)));
+// Four values of u as the second product takes them: each rounded to bfloat16, what that left out rounded too, and, where y
+// is float32, what that left out. An infinity leaves nothing out.
+__device__ __forceinline__ float lr_rest(float f, float rounded) { return f == rounded ? 0.f : f - rounded; }
+__device__ __forceinline__ uint2 lr_round(float4& v) {      // v gets what is left out
+    const uint2 r = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+    v = make_float4(lr_rest(v.x, __uint_as_float(r.x << 16)), lr_rest(v.y, __uint_as_float(r.x & 0xffff0000u)),
+                    lr_rest(v.z, __uint_as_float(r.y << 16)), lr_rest(v.w, __uint_as_float(r.y & 0xffff0000u)));
+    return r;
 }
+// Parts of u: 2^-17 of it is lost with two (a bfloat16 y's own rounding is 2^-9), 2^-25 with three.
+template <typename TY> struct LowRankParts { static constexpr int N = sizeof(TY) == 4 ? 3 : 2; };
 
 __device__ __forceinline__ int lr_slice(const LowRankColumns& c, int n) {
     if (c.interleaved) return (n >> 3) & 1;
@@ -230,7 +234,7 @@ low_rank_plan_kernel(const int* __restrict__ ids, int T, int adapters, int tile,
 // bfloat16: the adapter's rows are the 16 rows of mma.sync products, the batch's rows their 8 columns, both
 // straight from memory into the operands' registers: which 16 values of k meet in a product does not
 // matter as long as both sides agree, so a thread takes eight neighbouring ones (16 bytes). For the second
-// product u is two bfloat16 numbers, its value rounded and the rest rounded: 2^-17 of it is lost.
+// product u is two bfloat16 numbers, its value rounded and the rest rounded, or three where y is float32.
 // float32: plain sums, a warp four values of u for all eight rows, its lanes over k; u's and the result's
 // order of additions depends on K and the rank alone, whatever the batch.
 //
@@ -260,9 +264,10 @@ __device__ __forceinline__ float4 lf_peer(const float* mine, int rank) {
 }
 
 // Floats of shared memory: u of all blocks [8][width + 4], this block's [8][width], then partial sums
-// [8 warps][64][8] (bfloat16) or the block's part of x [8][k] (float32).
+// [8 warps][64][8], later u's third parts [8][width / 2 + 4] (bfloat16), or the block's part of x [8][k] (float32).
 template <typename T> static inline long long lf_floats(int width, int K) {
-    const long long tail = sizeof(T) == 2 ? LF_WARPS * LF_PASS * LF_ROWS : (long long)LF_ROWS * ((((K + LF_CTAS - 1) / LF_CTAS) + 3) / 4 * 4);
+    const long long third = (long long)LF_ROWS * (width / 2 + 4), sums = LF_WARPS * LF_PASS * LF_ROWS;
+    const long long tail = sizeof(T) == 2 ? (third > sums ? third : sums) : (long long)LF_ROWS * ((((K + LF_CTAS - 1) / LF_CTAS) + 3) / 4 * 4);
     return (long long)LF_ROWS * (2 * width + 4) + tail;
 }
 
@@ -460,8 +465,11 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
         }
         s = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
         float* const to = u + (e / width) * (width + 4) + e % width;
-        if constexpr (sizeof(T) == 2) *(uint4*)to = lr_split(s);
-        else *(float4*)to = s;
+        if constexpr (sizeof(T) == 2) {
+            const uint2 first = lr_round(s), second = lr_round(s);
+            *(uint4*)to = make_uint4(first.x, first.y, second.x, second.y);
+            if constexpr (LowRankParts<TY>::N == 3) *(uint2*)(tail + (e / width) * (width / 2 + 4) + e % width / 2) = lr_round(s);
+        } else *(float4*)to = s;
     }
     lf_cluster_arrive();                                     // waited for at the end: a peer may still be reading `part`
     __syncthreads();
@@ -475,14 +483,16 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
         const int far = p.columns.interleaved ? 16 : 8;      // columns from a product's row g to row g + 8
 #pragma unroll 1
         for (int q0 = col0 / 16 + warp; q0 < col1 / 16; q0 += LF_TILES * LF_WARPS) {
-            int c[LF_TILES], at_u[LF_TILES];
+            int c[LF_TILES], at_u[LF_TILES], at_third[LF_TILES];
             TY v[LF_TILES][4];
             float acc[LF_TILES][4] = {};
 #pragma unroll
             for (int i = 0; i < LF_TILES; ++i) {
                 const int q = min(q0 + i * LF_WARPS, col1 / 16 - 1);     // past the end: the last one, and not stored
                 c[i] = p.columns.interleaved ? q / 2 * 32 + (q & 1) * 8 + g : q * 16 + g;
-                at_u[i] = g * (width + 4) + (p.columns.interleaved ? q & 1 : lr_slice(p.columns, q * 16)) * rank;
+                const int first = (p.columns.interleaved ? q & 1 : lr_slice(p.columns, q * 16)) * rank;
+                at_u[i] = g * (width + 4) + first;
+                at_third[i] = g * (width / 2 + 4) + first / 2;
                 const TY* const ya = y + (size_t)max(r0, 0) * p.y_stride + c[i];
                 const TY* const yb = y + (size_t)max(r1, 0) * p.y_stride + c[i];
                 if (r0 >= 0) { v[i][0] = ya[0]; v[i][2] = ya[far]; }
@@ -505,6 +515,10 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
                     const uint32_t m[4] = {lo[i].x, hi[i].x, lo[i].y, hi[i].y};
                     mma_bf16(acc[i], m, f.x, f.y);
                     mma_bf16(acc[i], m, f.z, f.w);
+                    if constexpr (LowRankParts<TY>::N == 3) {
+                        const uint2 third = k < rank ? *(const uint2*)(tail + at_third[i] + k / 2) : make_uint2(0, 0);
+                        mma_bf16(acc[i], m, third.x, third.y);
+                    }
                 }
             }
 #pragma unroll
@@ -546,7 +560,7 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
 }
 
 // ---------------------------------------------------------------------- many rows of an adapter
-// Tiles of 128 planned rows, bfloat16. Two kernels, u between them as two bfloat16 numbers a value (see above):
+// Tiles of 128 planned rows, bfloat16. Two kernels, u between them as two or three bfloat16 numbers a value (see above):
 //
 // u (`low_rank_u_kernel`): X[rows] A^T on tcgen05, a cluster 64 or 128 rows, a part of k a block: TMA brings 64 columns of
 // the rows (one box where they lie together, else four rows a request) and of A into a ring, a thread issues the products.
@@ -583,7 +597,7 @@ template <int COLS>
 __global__ void __launch_bounds__(LT_THREADS)
 low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_constant__ CUtensorMap map_some,
                   const __grid_constant__ CUtensorMap map_all, const __grid_constant__ CUtensorMap map_a, const LowRankTile g,
-                  int rank, const float* __restrict__ scale, const int* __restrict__ perm, const int* __restrict__ info,
+                  int rank, int parts, const float* __restrict__ scale, const int* __restrict__ perm, const int* __restrict__ info,
                   const int* __restrict__ tiles, bf16* __restrict__ u) {
     extern __shared__ unsigned char lt_raw[];
     unsigned char* const base = (unsigned char*)(((uintptr_t)lt_raw + 1023) & ~(uintptr_t)1023);
@@ -728,36 +742,40 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
         lf_cluster_wait();
         // a lane four values of a slice, a warp a row at a time
         const int s0 = c0 / rank, s1 = (c1 + rank - 1) / rank;   // slices that this pass touches
-        auto add = [&](auto parts) {
-            constexpr int PARTS = decltype(parts)::value;
+        auto add = [&](auto blocks_of, auto parts_of) {
+            constexpr int BLOCKS = decltype(blocks_of)::value, PARTS = decltype(parts_of)::value;
             for (int e = lane; e < (s1 - s0) * quads; e += 32) {
                 const int s = s0 + e / quads, k = e % quads * 4, c = s * rank + k;
                 // the zeros behind a slice are written with its last value
                 if (k < rank ? c < c0 || c >= c1 : (s + 1) * rank <= c0 || (s + 1) * rank > c1) continue;
                 const unsigned char* const from = base + (c - c0) / 32 * (share * 128);
                 const int piece = (c - c0) % 32 / 4, step = blocks * share * 128;
-                bf16* to = u + ((size_t)(r0 + split * share + warp) * slices + s) * 2 * padded + k;
+                bf16* to = u + ((size_t)(r0 + split * share + warp) * slices + s) * PARTS * padded + k;
 #pragma unroll 4
-                for (int row = warp; row < min(share, rows - split * share); row += LT_THREADS / 32, to += (size_t)(LT_THREADS / 32) * slices * 2 * padded) {
+                for (int row = warp; row < min(share, rows - split * share); row += LT_THREADS / 32, to += (size_t)(LT_THREADS / 32) * slices * PARTS * padded) {
                     const unsigned char* const at = from + row * 128 + ((piece ^ (row & 7)) << 4);
                     float4 v = *(const float4*)at;
 #pragma unroll
-                    for (int i = 1; i < PARTS; ++i) {
+                    for (int i = 1; i < BLOCKS; ++i) {
                         const float4 q = *(const float4*)(at + i * step);
                         v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
                     }
                     if (k >= rank) v = make_float4(0.f, 0.f, 0.f, 0.f);     // what lies behind a slice is the next one's
                     v.x *= by; v.y *= by; v.z *= by; v.w *= by;
-                    const uint4 two = lr_split(v);
-                    *(uint2*)to = make_uint2(two.x, two.y);
-                    *(uint2*)(to + padded) = make_uint2(two.z, two.w);
+                    *(uint2*)to = lr_round(v);
+                    *(uint2*)(to + padded) = lr_round(v);
+                    if constexpr (PARTS == 3) *(uint2*)(to + 2 * padded) = lr_round(v);
                 }
             }
         };
-        if (g.splits == 1) add(LtParts<1>());
-        else if (g.splits == 2) add(LtParts<2>());
-        else if (g.splits == 4) add(LtParts<4>());
-        else add(LtParts<8>());
+        auto add_of = [&](auto parts_of) {
+            if (g.splits == 1) add(LtParts<1>(), parts_of);
+            else if (g.splits == 2) add(LtParts<2>(), parts_of);
+            else if (g.splits == 4) add(LtParts<4>(), parts_of);
+            else add(LtParts<8>(), parts_of);
+        };
+        if (parts == 2) add_of(LtParts<2>());
+        else add_of(LtParts<3>());
     }
     tg_before();
     __syncthreads();
@@ -791,9 +809,9 @@ __device__ __forceinline__ uint64_t lo_desc(const void* tile, uint32_t apart) {
     return (tg_desc(tile) & ~((uint64_t)0x3fff << 32)) | ((uint64_t)(apart >> 4) << 32);
 }
 
-// BOXES: of 64 values of the rank. PAIRED (rank up to 32): a row's rounded values and the rest share a box.
+// BOXES: of 64 values of the rank. PAIRED (rank up to 32, for a float32 y up to 16): all parts of a row share a box.
 template <int BOXES, bool PAIRED, bool EIGHTS, typename TY> struct LowRankOut {
-    static constexpr int SLICES = EIGHTS ? 2 : 1, PARTS = PAIRED ? 1 : 2;
+    static constexpr int SLICES = EIGHTS ? 2 : 1, PARTS = PAIRED ? 1 : LowRankParts<TY>::N;
     static constexpr int A_BYTES = SLICES * PARTS * BOXES * LO_U_BOX, B_BYTES = BOXES * LO_B_BOX;
     static constexpr int Y_BOXES = (int)sizeof(TY) / 2, Y_BYTES = Y_BOXES * 32 * 128;     // a warp's tile: boxes of 128 bytes a row
     static constexpr int SLOTS = A_BYTES + 2 * B_BYTES + LO_HANDS * 2 * Y_BYTES <= 224 * 1024 ? 2 : 1;
@@ -887,7 +905,7 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
 #pragma unroll
             for (int i = 0; i < L::SLICES * L::PARTS * BOXES; ++i) {
                 const int x = i % BOXES, rest = i / BOXES % L::PARTS, h = i / BOXES / L::PARTS;
-                tg_load_2d(a_smem + i * LO_U_BOX, &map_u, ((q.slice + h) * 2 + rest) * steps_all * 16 + x * 64, q.r0, u_full);
+                tg_load_2d(a_smem + i * LO_U_BOX, &map_u, ((q.slice + h) * LowRankParts<TY>::N + rest) * steps_all * 16 + x * 64, q.r0, u_full);
             }
         };
         auto fetch = [&](const Turn& q, int s) {             // one thread
@@ -940,11 +958,12 @@ low_rank_out_kernel(const __grid_constant__ CUtensorMap map_u, const __grid_cons
                         const unsigned char* const bx = b_ring + s * L::B_BYTES + x * LO_B_BOX + (EIGHTS ? h * 1024 : 0);
                         const uint64_t db = lo_desc(bx, EIGHTS ? 2048 : 1024);
                         const uint64_t da = tg_desc(a_smem + (h * L::PARTS * BOXES + x) * LO_U_BOX);
-                        const uint64_t dr = PAIRED ? da + 2 * steps_all : da + BOXES * (LO_U_BOX >> 4);
+                        const uint64_t part = PAIRED ? 2 * steps_all : BOXES * (LO_U_BOX >> 4);      // from a part to the next
                         const int steps = min(steps_all - 4 * x, 4);
                         for (int k = 0; k < steps; ++k) {
                             tg_mma(d, da + 2 * k, db + 2 * k, idesc, first ? 0u : 1u);
-                            tg_mma(d, dr + 2 * k, db + 2 * k, idesc, 1u);
+#pragma unroll
+                            for (int r = 1; r < LowRankParts<TY>::N; ++r) tg_mma(d, da + r * part + 2 * k, db + 2 * k, idesc, 1u);
                             first = false;
                         }
                     }
@@ -1239,7 +1258,7 @@ template <typename TY> static bool lr_tile_takes(const LowRank& p) {
         p.T > (1 << 24) || (long long)p.adapters * width > 0x7fffffff || (long long)p.adapters * p.N > 0x7fffffff || p.y_stride % v || p.out_stride % v ||
         ((uintptr_t)p.y | (uintptr_t)p.out) & 15)
         return false;
-    if (p.columns.interleaved) return p.N % 32 == 0;
+    if (p.columns.interleaved) return p.N % 32 == 0 && (sizeof(TY) == 2 || p.rank <= 64);       // u's parts in shared memory
     for (int i = 0; i < p.columns.slices; ++i)
         if (p.columns.ends[i] % 32) return false;
     return true;
@@ -1277,7 +1296,7 @@ static LowRankTile lr_plan(const LowRank& p) {
     return best;
 }
 
-template <int COLS> static int low_rank_u(const LowRank& p, const LowRankTile& g, const int* perm, const int* info, const int* tiles, bf16* u,
+template <int COLS> static int low_rank_u(const LowRank& p, const LowRankTile& g, int parts, const int* perm, const int* info, const int* tiles, bf16* u,
                                           cudaStream_t stream) {
     static bool sized[64] = {};                              // per device
     int dev = 0;
@@ -1306,7 +1325,7 @@ template <int COLS> static int low_rank_u(const LowRank& p, const LowRankTile& g
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = tgo_pdl_enabled() ? 2 : 1;
-    return (int)cudaLaunchKernelEx(&cfg, low_rank_u_kernel<COLS>, row, some, all, a, g, p.rank, p.scale, perm, info, tiles, u);
+    return (int)cudaLaunchKernelEx(&cfg, low_rank_u_kernel<COLS>, row, some, all, a, g, p.rank, parts, p.scale, perm, info, tiles, u);
 }
 
 template <int BOXES, bool PAIRED, bool EIGHTS, typename TY>
@@ -1330,7 +1349,7 @@ static int low_rank_out(const LowRank& p, const bf16* u, const int* perm, const 
     }
     const long long most = (lr_tiles(p, LT_ROWS) * turns + 1) / 2, slots = (long long)tgo_multiprocessors() * LowRankOut<BOXES, PAIRED, EIGHTS, TY>::BLOCKS;
     if (most > 0x3fffffff) return TGO_E_BAD_ARG;
-    const int width = 2 * ((p.rank + 15) / 16 * 16) * p.columns.slices;
+    const int width = LowRankParts<TY>::N * ((p.rank + 15) / 16 * 16) * p.columns.slices;
     auto map_of = [](CUtensorMap* map, const void* ptr, long long rows, long long cols, long long stride, int box_rows) {
         return sizeof(TY) == 2 ? tg_map(map, ptr, rows, cols, stride, box_rows) : tg_map_f32(map, ptr, rows, cols, stride, box_rows);
     };
@@ -1345,14 +1364,15 @@ static int low_rank_out(const LowRank& p, const bf16* u, const int* perm, const 
 
 template <bool EIGHTS, typename TY>
 static int low_rank_out_of(const LowRank& p, const bf16* u, const int* perm, const int* info, const int* tiles, cudaStream_t stream) {
-    if (p.rank <= 32) return low_rank_out<1, true, EIGHTS, TY>(p, u, perm, info, tiles, stream);
+    if (LowRankParts<TY>::N * ((p.rank + 15) / 16 * 16) <= 64) return low_rank_out<1, true, EIGHTS, TY>(p, u, perm, info, tiles, stream);
     if (p.rank <= 64) return low_rank_out<1, false, EIGHTS, TY>(p, u, perm, info, tiles, stream);
-    return low_rank_out<2, false, EIGHTS, TY>(p, u, perm, info, tiles, stream);
+    if constexpr (!EIGHTS || sizeof(TY) == 2) return low_rank_out<2, false, EIGHTS, TY>(p, u, perm, info, tiles, stream);
+    return TGO_E_BAD_ARG;                                    // three parts of two slices: lr_tile_takes refuses them
 }
 
-// 32-bit numbers of workspace: the plan, and u twice in bfloat16.
-static long long lr_tile_work(const LowRank& p) {
-    return (p.T + LP_INFO + 3 * lr_tiles(p, LT_ROWS) + 3) / 4 * 4 + (long long)p.T * ((p.rank + 15) / 16 * 16) * p.columns.slices;
+// 32-bit numbers of workspace: the plan, and u's parts in bfloat16.
+template <typename TY> static long long lr_tile_work(const LowRank& p) {
+    return (p.T + LP_INFO + 3 * lr_tiles(p, LT_ROWS) + 3) / 4 * 4 + (long long)p.T * ((p.rank + 15) / 16 * 16) * p.columns.slices * LowRankParts<TY>::N / 2;
 }
 
 template <typename TY> static int low_rank_tiles(const LowRank& p, int* work, cudaStream_t stream) {
@@ -1372,11 +1392,11 @@ template <typename TY> static int low_rank_tiles(const LowRank& p, int* work, cu
     if (rc) return rc;
     const LowRankTile g = lr_plan(p);
     const int cols = g.cuts * g.cut;
-    if (cols <= 32) rc = low_rank_u<32>(p, g, perm, info, tiles, u, stream);
-    else if (cols <= 64) rc = low_rank_u<64>(p, g, perm, info, tiles, u, stream);
-    else if (cols <= 128) rc = low_rank_u<128>(p, g, perm, info, tiles, u, stream);
-    else if (cols <= 256) rc = low_rank_u<256>(p, g, perm, info, tiles, u, stream);
-    else rc = low_rank_u<512>(p, g, perm, info, tiles, u, stream);
+    if (cols <= 32) rc = low_rank_u<32>(p, g, LowRankParts<TY>::N, perm, info, tiles, u, stream);
+    else if (cols <= 64) rc = low_rank_u<64>(p, g, LowRankParts<TY>::N, perm, info, tiles, u, stream);
+    else if (cols <= 128) rc = low_rank_u<128>(p, g, LowRankParts<TY>::N, perm, info, tiles, u, stream);
+    else if (cols <= 256) rc = low_rank_u<256>(p, g, LowRankParts<TY>::N, perm, info, tiles, u, stream);
+    else rc = low_rank_u<512>(p, g, LowRankParts<TY>::N, perm, info, tiles, u, stream);
     if (rc) return rc;
     return p.columns.interleaved ? low_rank_out_of<true, TY>(p, u, perm, info, tiles, stream)
                                  : low_rank_out_of<false, TY>(p, u, perm, info, tiles, stream);
@@ -1412,7 +1432,7 @@ template <typename T, typename TY> static int low_rank_any(const LowRank& p, flo
 template <typename T, typename TY> static long long lr_work(const LowRank& p) {
     const int width = p.columns.slices * p.rank;
     if constexpr (sizeof(T) == 2)
-        if (lr_many(p) && lr_tile_takes<TY>(p)) return lr_tile_work(p);
+        if (lr_many(p) && lr_tile_takes<TY>(p)) return lr_tile_work<TY>(p);
     if (lr_few_takes<T>(p)) return !lr_scanned(p) ? p.T + LP_INFO + 3 * lr_tiles(p, LF_ROWS) : 0;
     return (long long)p.T * width;
 }

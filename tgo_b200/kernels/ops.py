@@ -2218,8 +2218,8 @@ def low_rank_add(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.Ten
             call(*args, 0, 0, needs.buffer_info()[0], 0)
             work = x.new_empty(needs[0], dtype=torch.int32)
             status = call(*args, work.data_ptr(), needs[0], 0, _stream())
-    else:                                   # a plan of the rows (four numbers a row and a few) and at most u
-        needs = T * (S * ((r + 15) // 16 * 16) + 4) + 8
+    else:                                   # a plan of the rows (four numbers a row and a few) and at most u in parts
+        needs = T * (S * ((r + 15) // 16 * 24) + 4) + 8
         work = x.new_empty(needs, dtype=torch.int32)
         status = call(*args, work.data_ptr(), needs, 0, _stream())
         LAUNCHES[0] += 1
