@@ -138,6 +138,17 @@ def test_strided_rows(x_type, y_type, T):
 
 
 @pytest.mark.parametrize("x_type", [F32, BF])
+def test_rows_further_apart_than_31_bits(x_type):
+    """Rows of x and y whose offsets pass 2^31 numbers."""
+    T, apart = 300, 1 << 23
+    p = inputs(T, 128, (64, 32), 16, 3, x_type, x_type, seed=9)
+    for name in ("x", "y"):
+        wide = torch.empty(T, apart, dtype=x_type, device=DEV)[:, :p[name].shape[1]]
+        p[name] = wide.copy_(p[name])
+    check(p, (64, 32), in_place=True)
+
+
+@pytest.mark.parametrize("x_type", [F32, BF])
 @pytest.mark.parametrize("T", [1, 40, 700])
 def test_one_row_for_all(x_type, T):
     """x expanded from a single row."""
