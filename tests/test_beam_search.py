@@ -193,6 +193,47 @@ def test_searches_match_plain(emulated, tmp_path, name, beams, length_penalty):
         same(g, plain_beam_search(lambda t: plain.forward(pcfg, w, t)[-1], p, beams, 9, set(stop), length_penalty), 1e-3)
 
 
+def search_over_everything(last_logits, prompt, beams, max_tokens, stop_ids, length_penalty):
+    """A search whose turns put every continuation of every beam in order, none left out. [(tokens, score, stopped)]."""
+    def worth(s, n):
+        return s / max(n, 1) ** length_penalty
+    live, done = [([], 0.0)], []
+    for _ in range(max_tokens):
+        found = []
+        for w, (t, s) in enumerate(live):
+            x = np.asarray(last_logits(prompt + t), dtype=np.float64)
+            lp = x - x.max() - np.log(np.exp(x - x.max()).sum())
+            found += [(-(s + v), w, i) for i, v in enumerate(lp)]
+        found.sort()
+        ends = [(worth(-v, len(live[w][0])), live[w][0], -v, True) for v, w, i in found[:beams] if i in stop_ids]
+        done = sorted(done + ends, key=lambda h: -h[0])[:beams]
+        live = [(live[w][0] + [i], -v) for v, w, i in found if i not in stop_ids][:beams]
+        assert len(live) == beams                # the vocabulary has enough of them
+        if len(done) == beams and worth(live[0][1], len(live[0][0])) <= done[-1][0]:
+            return [h[1:] for h in done]
+    return [h[1:] for h in sorted(done + [(worth(s, len(t)), t, s, False) for t, s in live], key=lambda h: -h[0])[:beams]]
+
+
+@pytest.mark.parametrize("stops,beams", [(1, 4), (2, 1), (2, 3), (3, 2), (3, 4), (5, 8), (2, 32), (13, 5), (40, 4)])
+def test_stop_ids_leave_no_beam_without_continuations(emulated, tmp_path, stops, beams):
+    """However many of the best continuations end in one of the stop ids, `beams` others go on."""
+    from tgo_b200.engine.beams import BeamSearch
+    d, cfg, run = tiny_model(tmp_path, "A")
+    pcfg, w = plain.load_model_dir(d)
+    V = cfg["vocab_size"]
+    stop = np.random.default_rng(stops).choice(V, stops, replace=False).tolist()
+    more = np.zeros(V, dtype=np.float32)
+    more[stop] = 4.0
+    eng = cpu_model(d, cfg).new_engine(page_size=4, max_tokens=4000, num_slots=2 * beams)
+    step = eng.step
+    eng.step = lambda entries: step(entries) + torch.from_numpy(more)
+    prompts = list(tiny.random_requests(V, [5, 9], seed=7).values())
+    got = BeamSearch(eng, beams, 5, stop + [V + 7], length_penalty=2.0).run(prompts)
+    for g, p in zip(got, prompts):
+        same(g, search_over_everything(lambda t: plain.forward(pcfg, w, t)[-1] + more, p, beams, 5, set(stop), 2.0), 1e-3)
+        assert len(g) == beams
+
+
 def test_one_beam_is_greedy(emulated, tmp_path):
     d, cfg, run = tiny_model(tmp_path, "B")
     pcfg, w = plain.load_model_dir(d)

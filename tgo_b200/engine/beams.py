@@ -2,9 +2,11 @@
 them as one decode batch.
 
 A prompt is run once; its other beams then share its pages (`Engine.follow`). Each turn selects, on the
-device, the 2 x beams best continuations over a request's beams and the vocabulary
-(`ops.beam_select`: summed log probabilities, equal ones by beam and token) and reads back those few
-numbers. In their order, a continuation that ends in a stop id becomes a finished hypothesis (if it is
+device, the best continuations over a request's beams and the vocabulary
+(`ops.beam_select`: summed log probabilities, equal ones by beam and token), (1 + stop ids) x beams of them,
+so that `beams` remain however many of the others end in a stop id, and reads back those few numbers. Where
+these are more than a selection gives, it is made for each beam alone, beams + stop ids of each, and the host
+puts them in order. In their order, a continuation that ends in a stop id becomes a finished hypothesis (if it is
 among the first `beams`: a worse one would not be kept), any other the next live beam, until there are
 `beams` of them; the beams then take over the pages and states of the ones they continue, in place.
 
@@ -54,7 +56,7 @@ class BeamSearch:
         if chunk <= 0:
             raise ValueError(f"beam search: the prompt chunk is {chunk}")
         self.engine, self.beams, self.max_tokens = engine, beams, max_tokens
-        self.stop_ids = set(int(t) for t in stop_ids)
+        self.stop_ids = set(int(t) for t in stop_ids if 0 <= int(t) < engine.model.spec.vocab_size)
         self.length_penalty, self.chunk = float(length_penalty), chunk
         self._runs = 0
 
@@ -116,21 +118,35 @@ class BeamSearch:
             logits[q * self.beams] = got[0]
         return logits
 
-    def _advance(self, searches, logits) -> List[List[int]]:
-        """Select, and bring every search a token further; the parents of its beams."""
-        B, W, K = len(searches), self.beams, 2 * self.beams
+    def _select(self, searches, logits) -> List[list]:
+        """Every search's continuations (value, parent, token), the best first: `beams` that end in no stop id
+        are among them if there are as many. (A selection for one beam holds 64: with more than 64 - beams stop
+        ids, continuations are missed of a beam whose 64 best are nearly all of them stop ids.)"""
+        B, W, n = len(searches), self.beams, len(self.stop_ids)
+        groups, beams, K = B, W, (1 + n) * W
+        if K > ops.BEAM_MAX_PICKS:
+            groups, beams, K = B * W, 1, min(W + n, ops.BEAM_MAX_PICKS)
         scores = torch.tensor([s.scores for s in searches], dtype=torch.float32).to(logits.device)
-        picks = torch.empty((3, B, K), dtype=torch.int32, device=logits.device)
-        ops.beam_select(logits, scores, picks[0].view(torch.float32), picks[1], picks[2])
+        picks = torch.empty((3, groups, K), dtype=torch.int32, device=logits.device)
+        ops.beam_select(logits, scores.view(groups, beams), picks[0].view(torch.float32), picks[1], picks[2])
         host = picks.cpu().numpy()
         values = host[0].view(np.float32).tolist()
         from_beam, token = host[1].tolist(), host[2].tolist()
+        found = []
+        for q in range(B):
+            own = [q] if groups == B else range(q * W, (q + 1) * W)
+            one = [(v, p + g - own[0], t) for g in own for v, p, t in zip(values[g], from_beam[g], token[g]) if p >= 0]
+            found.append(one if groups == B else sorted(one, key=lambda c: -c[0]))      # equal ones stay by beam and token
+        return found
+
+    def _advance(self, searches, logits) -> List[List[int]]:
+        """Select, and bring every search a token further; the parents of its beams."""
+        W = self.beams
         parents = []
-        for q, s in enumerate(searches):
+        for s, found in zip(searches, self._select(searches, logits)):
             parent, tokens, scores = [], [], []
-            for k in range(K):
-                p, t, v = from_beam[q][k], token[q][k], values[q][k]
-                if p < 0 or len(parent) == W:
+            for k, (v, p, t) in enumerate(found):
+                if len(parent) == W:
                     break
                 if t in self.stop_ids:
                     if k < W:
