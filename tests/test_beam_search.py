@@ -319,6 +319,26 @@ def test_adapted_requests_beside_plain_ones(emulated, tmp_path, name):
     assert not eng._adapter_of
 
 
+@pytest.mark.parametrize("parents", [[1, 0, 2], [0, 0, 1], [2, 0, 1], [1, 2, 2], [2, 2, 0]])
+def test_adapters_follow_what_the_parents_held(emulated, tmp_path, parents):
+    """Requests of one group with unlike adapters: exchanges and chains take the parents' old ones, as they take their rows."""
+    from tgo_b200.engine.step import StepEntry
+    d, cfg, run = tiny_model(tmp_path, "A")
+    pcfg, w = plain.load_model_dir(d)
+    loaded, adapters = cpu_model(d, cfg), some_adapters(w)
+    loaded.load_adapters(adapters)
+    which, text = ["all", None, "first layer"], [[3, 1, 4, 1, 5], [9, 2, 6, 5, 3], [5, 8, 9, 7, 9]]
+    eng = loaded.new_engine(page_size=4, max_tokens=96, num_slots=3)
+    for r, name in enumerate(which):
+        eng.admit(r, adapter=name)
+    eng.step([StepEntry(r, text[r], []) for r in range(3)])
+    eng.follow([[0, 1, 2]], [parents])
+    got = eng.step([StepEntry(r, [7], [0]) for r in range(3)]).numpy()
+    for r, p in enumerate(parents):
+        ww = w if which[p] is None else with_adapter(w, adapters[which[p]].matrices, adapters[which[p]].scale)
+        assert np.allclose(got[r], plain.forward(pcfg, ww, text[p] + [7])[-1], rtol=0, atol=1e-3), r
+
+
 def write_folder(path, config, tensors):
     from tgo_b200.weights.safetensors import write_safetensors
     os.makedirs(path)

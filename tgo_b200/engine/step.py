@@ -129,9 +129,10 @@ class Engine:
                     ops.reorder_rows([kv], lists[g], lists[n + 1], axis=2)
         if self.storage.state:
             ops.reorder_rows(list(self.storage.state.values()), lists[n], lists[n + 1])
+        held = [self._adapter_of.get(r) for r in flat]        # before any of them changes
         for r, i in zip(flat, at):
-            if flat[i] in self._adapter_of:
-                self._adapter_of[r] = self._adapter_of[flat[i]]
+            if held[i] is not None:
+                self._adapter_of[r] = held[i]
             else:
                 self._adapter_of.pop(r, None)
 
