@@ -404,3 +404,20 @@ def test_adapters_are_checked(emulated, tmp_path):
         loaded.generate([[1]], adapters=["other"])
     with pytest.raises(ValueError, match="2 adapters for 1"):
         loaded.beam_search([[1]], adapters=["good", "good"])
+
+
+@pytest.mark.parametrize("dtype,number", [("float32", 1e39), ("bfloat16", 3.4e38)])
+def test_adapters_that_the_engine_cannot_hold(emulated, tmp_path, dtype, number):
+    """Numbers that are finite on disk and would be infinite in the bank, and a scale that would be."""
+    d, cfg, run = tiny_model(tmp_path, "A")
+    _, w = plain.load_model_dir(d)
+    loaded = cpu_model(d, cfg)
+    loaded.model.dtype = getattr(torch, dtype)
+    n = "model.layers.0.self_attn.q_proj.weight"
+    out, inp = w[n].shape
+    a, b = torch.ones(2, inp, dtype=torch.float64), torch.ones(out, 2, dtype=torch.float64)
+    for big_a, big_b, scale, text in [(number, 1.0, 1.0, "not finite"), (1.0, -number, 1.0, "not finite"), (1.0, 1.0, 1e39, "scale")]:
+        with pytest.raises(AdapterError, match=text):
+            loaded.load_adapters({"big": Adapter({n: (a * big_a, b * big_b)}, scale)})
+    assert loaded.model.adapter_names == []
+    loaded.load_adapters({"large": Adapter({n: (a * number / 1e3, b)}, 1e30)})

@@ -76,12 +76,13 @@ def read_adapter(folder: str) -> Adapter:
     return Adapter({m: (h["A"], h["B"]) for m, h in halves.items()}, scale)
 
 
-def _check(name: str, adapter: Adapter, sites: Dict[str, Tuple[AdapterSite, int]]) -> None:
-    """One error that lists everything an adapter and the model disagree on."""
+def _check(name: str, adapter: Adapter, sites: Dict[str, Tuple[AdapterSite, int]], dtype) -> None:
+    """One error that lists everything an adapter and the model disagree on. Its numbers have to be finite as the
+    engine holds them: the matrices in `dtype`, the scale in float32."""
     wrong = []
     if not adapter.matrices:
         wrong.append("it holds no matrices")
-    if not math.isfinite(adapter.scale):
+    if not bool(torch.isfinite(torch.tensor(adapter.scale, dtype=torch.float64).float())):
         wrong.append(f"its scale is {adapter.scale}")
     for matrix, (a, b) in sorted(adapter.matrices.items()):
         if matrix not in sites:
@@ -94,8 +95,8 @@ def _check(name: str, adapter: Adapter, sites: Dict[str, Tuple[AdapterSite, int]
                          f"[{site.widths[i]}, {site.inputs}]")
         elif not (a.is_floating_point() and b.is_floating_point()):
             wrong.append(f"{matrix}: A and B hold whole numbers")
-        elif not (bool(torch.isfinite(a).all()) and bool(torch.isfinite(b).all())):
-            wrong.append(f"{matrix}: A or B holds a number that is not finite")
+        elif not (bool(torch.isfinite(a.to(dtype)).all()) and bool(torch.isfinite(b.to(dtype)).all())):
+            wrong.append(f"{matrix}: A or B holds a number that is not finite in {dtype}")
     if wrong:
         raise AdapterError(f"adapter {name!r}: " + "; ".join(wrong[:8]) + ("; ..." if len(wrong) > 8 else ""))
 
@@ -133,7 +134,7 @@ def bind_adapters(model, adapters: Dict[str, Adapter]) -> List[str]:
     parts = [(p, p.adapter_sites()) for p in parts if hasattr(p, "adapter_sites") and hasattr(p, "bind_adapters")]
     sites = {m: (s, i) for _, own in parts for s in own for i, m in enumerate(s.names)}
     for name, adapter in adapters.items():
-        _check(name, adapter, sites)
+        _check(name, adapter, sites, model.dtype)
     every = list(adapters.values())
     for part, own in parts:
         part.bind_adapters({s.key: _bank(s, every, model.dtype, model.device) for s in own
