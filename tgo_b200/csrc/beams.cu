@@ -14,8 +14,8 @@
 // that live, a slice of a row each: sixteen values a thread and turn, the next turn's already under way; a thread looks
 // closer at its values only when their largest, which the sum needs anyway, reaches the slice's K-th best so far. Then one
 // block a request joins the slices' maxima and sums and ranks what can be among the K best: in a second kernel, or, for
-// few rows, in the first block of a cluster. v is formed in 64 bits, so that close candidates of different beams are ordered
-// by their values and not by a rounding.
+// few rows, in the first block of a cluster. v is formed in 64 bits: candidates of one beam are ordered as their logits are, those of
+// different beams but for the error of the sums under the logarithms, which are 32-bit sums of approximate exponentials.
 //
 // MEASURED (B200): 512 rows of 151936 and 16 picks 57 us, 5.4 TB/s; without looking for candidates the same
 // pass takes 50, with a look only every fourth turn, at values read again, 64, from a ring filled by bulk
@@ -58,9 +58,9 @@ __device__ __forceinline__ unsigned long long bs_pair(float a, float b) {
     return r;
 }
 __device__ __forceinline__ void bs_unpair(unsigned long long p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
-__device__ __forceinline__ unsigned long long bs_fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+__device__ __forceinline__ unsigned long long bs_mul2(unsigned long long a, unsigned long long b) {
     unsigned long long r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 __device__ __forceinline__ unsigned long long bs_add2(unsigned long long a, unsigned long long b) {
@@ -195,23 +195,20 @@ __device__ __forceinline__ void bs_scan(const float* __restrict__ x, int V, int 
             s *= m > -INFINITY ? bs_exp(m - top) : 0.f;
             m = top;
         }
+        // The difference comes first, then the factor: its rounding goes by its own size. A difference of two products with
+        // log2 e is off by 2^-24 of the maximum's, whatever the difference: by hundreds where tokens are masked with -1e10.
         const float at = m > -INFINITY ? m : 0.f;
-        if (fabsf(at) < 1e37f) {
-            const unsigned long long by = bs_pair(-at * BS_LOG2E, -at * BS_LOG2E), scale = bs_pair(BS_LOG2E, BS_LOG2E);
-            unsigned long long sum[2] = {bs_pair(s, 0.f), 0ull};
+        const unsigned long long by = bs_pair(-at, -at), scale = bs_pair(BS_LOG2E, BS_LOG2E);
+        unsigned long long sum[2] = {bs_pair(s, 0.f), 0ull};
 #pragma unroll
-            for (int i = 0; i < 16 / 2; ++i) {
-                float a, b;
-                bs_unpair(bs_fma2(bs_pair(v[2 * i], v[2 * i + 1]), scale, by), a, b);
-                sum[i & 1] = bs_add2(sum[i & 1], bs_pair(bs_exp2(a), bs_exp2(b)));
-            }
+        for (int i = 0; i < 16 / 2; ++i) {
             float a, b;
-            bs_unpair(bs_add2(sum[0], sum[1]), a, b);
-            s = a + b;
-        } else {                                     // rows masked with the type's lowest value: the difference first
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s += bs_exp(v[i] - at);
+            bs_unpair(bs_mul2(bs_add2(bs_pair(v[2 * i], v[2 * i + 1]), by), scale), a, b);
+            sum[i & 1] = bs_add2(sum[i & 1], bs_pair(bs_exp2(a), bs_exp2(b)));
         }
+        float a, b;
+        bs_unpair(bs_add2(sum[0], sum[1]), a, b);
+        s = a + b;
         if (base == v0) {
             // before anything is kept: of each warp's threads' maxima the ceil(K / 8)-th, and the least of
             // those over the warps, is reached by K values at least
