@@ -17,12 +17,15 @@ struct LowRankColumns {
 };
 
 // Four values of u as the second product takes them: each rounded to bfloat16, what that left out rounded too, and, where y
-// is float32, what that left out. An infinity leaves nothing out.
-__device__ __forceinline__ float lr_rest(float f, float rounded) { return f == rounded ? 0.f : f - rounded; }
-__device__ __forceinline__ uint2 lr_round(float4& v) {      // v gets what is left out
-    const uint2 r = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
-    v = make_float4(lr_rest(v.x, __uint_as_float(r.x << 16)), lr_rest(v.y, __uint_as_float(r.x & 0xffff0000u)),
-                    lr_rest(v.z, __uint_as_float(r.y << 16)), lr_rest(v.w, __uint_as_float(r.y & 0xffff0000u)));
+// is float32, what that left out. All parts but the last stay finite: the largest bfloat16 number stands for a value that would round
+// to infinity, and an infinity is left for the last part.
+template <bool LAST> __device__ __forceinline__ uint2 lr_round(float4& v) {      // v gets what is left out
+    if constexpr (LAST) return make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+    uint2 r;
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r.x) : "f"(v.y), "f"(v.x));
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r.y) : "f"(v.w), "f"(v.z));
+    v = make_float4(v.x - __uint_as_float(r.x << 16), v.y - __uint_as_float(r.x & 0xffff0000u),
+                    v.z - __uint_as_float(r.y << 16), v.w - __uint_as_float(r.y & 0xffff0000u));
     return r;
 }
 // Parts of u: 2^-17 of it is lost with two (a bfloat16 y's own rounding is 2^-9), 2^-25 with three.
@@ -466,9 +469,9 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
         s = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
         float* const to = u + (e / width) * (width + 4) + e % width;
         if constexpr (sizeof(T) == 2) {
-            const uint2 first = lr_round(s), second = lr_round(s);
+            const uint2 first = lr_round<false>(s), second = lr_round<LowRankParts<TY>::N == 2>(s);
             *(uint4*)to = make_uint4(first.x, first.y, second.x, second.y);
-            if constexpr (LowRankParts<TY>::N == 3) *(uint2*)(tail + (e / width) * (width / 2 + 4) + e % width / 2) = lr_round(s);
+            if constexpr (LowRankParts<TY>::N == 3) *(uint2*)(tail + (e / width) * (width / 2 + 4) + e % width / 2) = lr_round<true>(s);
         } else *(float4*)to = s;
     }
     lf_cluster_arrive();                                     // waited for at the end: a peer may still be reading `part`
@@ -762,9 +765,9 @@ low_rank_u_kernel(const __grid_constant__ CUtensorMap map_row, const __grid_cons
                     }
                     if (k >= rank) v = make_float4(0.f, 0.f, 0.f, 0.f);     // what lies behind a slice is the next one's
                     v.x *= by; v.y *= by; v.z *= by; v.w *= by;
-                    *(uint2*)to = lr_round(v);
-                    *(uint2*)(to + padded) = lr_round(v);
-                    if constexpr (PARTS == 3) *(uint2*)(to + 2 * padded) = lr_round(v);
+                    *(uint2*)to = lr_round<false>(v);
+                    *(uint2*)(to + padded) = lr_round<PARTS == 2>(v);
+                    if constexpr (PARTS == 3) *(uint2*)(to + 2 * padded) = lr_round<true>(v);
                 }
             }
         };

@@ -2187,7 +2187,8 @@ def low_rank_add(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.Ten
 
     x [T, K] float32 or bfloat16, y and out [T, N] in x's type or float32, all three with rows that
     may be strided; a [adapters, slices, rank, K], b [adapters, N, rank] in x's type; scale float32
-    [adapters]; ids int32 [T]. widths: the slices' columns, at most four slices (a joined matrix: q, k
+    [adapters]; ids int32 [T]; a, b and scale hold finite numbers (beside an
+    infinity in b, u's parts give NaN). widths: the slices' columns, at most four slices (a joined matrix: q, k
     and v); `interleaved`: two slices of equal width that take turns, eight columns each."""
     if out is None:
         out = y
