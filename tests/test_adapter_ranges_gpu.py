@@ -1,9 +1,9 @@
-"""The low-rank product of every row's own adapter at the ends of its ranges: numbers that round to
-infinity. Statement and bounds of test_adapters_gpu.py, each test by the ways it names."""
+"""The low-rank product of every row's own adapter at the ends of its ranges: numbers that round to infinity, more rows than a
+grid holds. Statement and bounds of test_adapters_gpu.py, each test by the ways it names."""
 import pytest
 import torch
 
-from test_adapters_gpu import DEV, TYPES, check, inputs, ops
+from test_adapters_gpu import BF, DEV, TYPES, bound, check, inputs, ops, plain
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +30,20 @@ def test_products_near_the_end_of_the_range(by, way, x_type, y_type):
         p["x"][2, :2] = -p["x"][1, :2]
         p["b"].mul_(2.0 ** -100)
         check(p, (32,))
+
+
+@pytest.mark.parametrize("way", [CHOSEN, TILES])
+def test_more_rows_than_a_grid_has_tiles(by, way):
+    """8.4 million rows, 65536 tiles of 128: more than a launch's second extent takes."""
+    by(way)
+    T, g = 65536 * 128, torch.Generator(device=DEV).manual_seed(6)
+    p = inputs(1, 32, (32,), 8, 2, BF, BF, seed=6)
+    p["x"], p["y"] = (torch.randn(T, 32, generator=g, device=DEV, dtype=BF) for _ in range(2))
+    p["ids"] = (torch.arange(T, device=DEV) // 4999 % 3 - 1).to(torch.int32)
+    out = torch.empty_like(p["y"])
+    ops().low_rank_add(p["x"], p["y"], p["a"], p["b"], p["scale"], p["ids"], (32,), out=out)
+    at = torch.cat([torch.arange(0, T, 4001), torch.arange(T - 300, T)]).to(DEV)
+    x, y, ids = p["x"][at], p["y"][at], p["ids"][at]
+    want, size = plain(x, y, p["a"], p["b"], p["scale"], ids, (32,), False)
+    off = (out[at].double().cpu() - want).abs()
+    assert (off <= bound(want, size, 32, 8, BF, BF)).all()

@@ -1256,6 +1256,7 @@ template <typename T, typename TY> static int low_rank_few(const LowRank& p, int
 // Whether the kernels for many rows take a call: what they read and write on 16 bytes, A's columns in tensor memory.
 template <typename TY> static bool lr_tile_takes(const LowRank& p) {
     const int v = 16 / (int)sizeof(TY), width = p.columns.slices * p.rank;
+    if (lr_tiles(p, LT_ROWS) > 65535) return false;          // u's grid has a tile a place of its second extent
     if (p.x_stride < p.K || p.y_stride < p.N || p.out_stride < p.N) return false;      // rows over each other (an expanded x)
     if (!lr_vectors<bf16>(p) || p.rank % 8 || p.rank > 128 || width > LT_MAX_WIDTH || p.adapters > LP_MAX_ADAPTERS ||
         p.T > (1 << 24) || (long long)p.adapters * width > 0x7fffffff || (long long)p.adapters * p.N > 0x7fffffff || p.y_stride % v || p.out_stride % v ||
