@@ -1268,7 +1268,31 @@ template <typename TY> static bool lr_tile_takes(const LowRank& p) {
     return true;
 }
 
-static int lt_bytes(const LowRankTile& g) { return lt_ring(g) + 1024 + 256; }
+static int lt_stage(const LowRankTile& g) { return (g.rows + g.cuts * g.cut) * LT_BK * 2; }
+static LowRankTile lt_tile(int width, int K, int rows, int splits) {
+    LowRankTile g;
+    g.rows = rows;
+    g.splits = splits;
+    g.width = width;
+    g.cuts = width > 256 ? 2 : 1;
+    g.cut = ((width + g.cuts - 1) / g.cuts + 15) / 16 * 16;
+    g.kbs = (K + LT_BK - 1) / LT_BK;
+    const int most = 168 * 1024 / lt_stage(g);
+    g.stages = most < LT_STAGES ? most : LT_STAGES;
+    return g;
+}
+static int lt_columns(const LowRankTile& g) {               // of tensor memory
+    const int cols = g.cuts * g.cut;
+    return cols <= 32 ? 32 : cols <= 64 ? 64 : cols <= 128 ? 128 : cols <= 256 ? 256 : 512;
+}
+// Shared memory of a block, and no less than its part of the multiprocessor's 228 KB (1 KB a block is the system's) as it has a part of
+// the 512 columns: clusters of two calls, on two streams, could otherwise each hold tensor memory on one multiprocessor that the
+// other waits for there, and neither would end. (Only the blocks with 512 columns have to be enlarged for it: their clusters ran one block a
+// multiprocessor anyway.)
+static int lt_bytes(const LowRankTile& g) {
+    const int needed = lt_ring(g) + 1024 + 256, part = lt_columns(g) * (228 * 1024 / 512) - 1024;
+    return needed > part ? needed : part;
+}
 // How a tile's u is made: the rows of a cluster and the parts of k, its blocks, that are cheapest by a small model in
 // cycles. The blocks run in rounds of as many as the multiprocessors hold. 64 columns cost a block their way into the
 // multiprocessor (70 bytes a cycle) or its part of the way of all blocks' rows from memory (3400); to begin and end
@@ -1281,16 +1305,9 @@ static LowRankTile lr_plan(const LowRank& p) {
     long long least = -1;
     for (int rows = LT_ROWS; rows >= LT_ROWS / 2; rows /= 2)
         for (int s = 1; s <= 8; s *= 2) {
-            LowRankTile g;
-            g.rows = rows;
-            g.splits = s;
-            g.width = p.columns.slices * p.rank;
-            g.cuts = g.width > 256 ? 2 : 1;
-            g.cut = ((g.width + g.cuts - 1) / g.cuts + 15) / 16 * 16;
-            g.kbs = (p.K + LT_BK - 1) / LT_BK;
+            const LowRankTile g = lt_tile(p.columns.slices * p.rank, p.K, rows, s);
             if (s > 1 && s * 4 > g.kbs) break;
-            const int x = rows * LT_BK * 2, stage = x + g.cuts * g.cut * LT_BK * 2, most = 168 * 1024 / stage;
-            g.stages = most < LT_STAGES ? most : LT_STAGES;
+            const int x = rows * LT_BK * 2, stage = lt_stage(g);
             const int slots = tgo_multiprocessors() * (2 * lt_bytes(g) <= 226 * 1024 && g.cuts * g.cut <= 256 ? 2 : 1);
             const long long blocks = ((p.T + LT_ROWS - 1) / LT_ROWS + 1ll) * (LT_ROWS / rows) * s;
             const long long feed = stage / 70, memory = (blocks < slots ? blocks : slots) * x / 3400, each = feed > memory ? feed : memory;
@@ -1308,7 +1325,7 @@ template <int COLS> static int low_rank_u(const LowRank& p, const LowRankTile& g
     if (err != cudaSuccess) return (int)err;
     if (dev < 0 || dev >= 64) return TGO_E_BAD_ARG;
     if (!sized[dev]) {
-        err = cudaFuncSetAttribute(low_rank_u_kernel<COLS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+        err = cudaFuncSetAttribute(low_rank_u_kernel<COLS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
         if (err != cudaSuccess) return (int)err;
         sized[dev] = true;
     }
@@ -1395,11 +1412,11 @@ template <typename TY> static int low_rank_tiles(const LowRank& p, int* work, cu
                             LT_ROWS, perm, info, tiles, ahead);
     if (rc) return rc;
     const LowRankTile g = lr_plan(p);
-    const int cols = g.cuts * g.cut;
-    if (cols <= 32) rc = low_rank_u<32>(p, g, LowRankParts<TY>::N, perm, info, tiles, u, stream);
-    else if (cols <= 64) rc = low_rank_u<64>(p, g, LowRankParts<TY>::N, perm, info, tiles, u, stream);
-    else if (cols <= 128) rc = low_rank_u<128>(p, g, LowRankParts<TY>::N, perm, info, tiles, u, stream);
-    else if (cols <= 256) rc = low_rank_u<256>(p, g, LowRankParts<TY>::N, perm, info, tiles, u, stream);
+    const int cols = lt_columns(g);
+    if (cols == 32) rc = low_rank_u<32>(p, g, LowRankParts<TY>::N, perm, info, tiles, u, stream);
+    else if (cols == 64) rc = low_rank_u<64>(p, g, LowRankParts<TY>::N, perm, info, tiles, u, stream);
+    else if (cols == 128) rc = low_rank_u<128>(p, g, LowRankParts<TY>::N, perm, info, tiles, u, stream);
+    else if (cols == 256) rc = low_rank_u<256>(p, g, LowRankParts<TY>::N, perm, info, tiles, u, stream);
     else rc = low_rank_u<512>(p, g, LowRankParts<TY>::N, perm, info, tiles, u, stream);
     if (rc) return rc;
     return p.columns.interleaved ? low_rank_out_of<true, TY>(p, u, perm, info, tiles, stream)
@@ -1467,6 +1484,14 @@ static bool lr_fill(LowRank& p, int T, int K, int N, int adapters, int rank, int
 
 // The code that a wait of the kernels for many rows left when it ran out, or 0. Synchronises.
 TGO_API int tgo_low_rank_error(int* value) { return (int)cudaMemcpyFromSymbol(value, low_rank_error_flag, sizeof(int)); }
+
+// What a block of u's kernel takes of its multiprocessor for slices x rank values a row and clusters of `rows` rows: columns of tensor
+// memory; *bytes gets the shared memory.
+TGO_API int tgo_low_rank_tile_needs(int width, int rows, int* bytes) {
+    const LowRankTile g = lt_tile(width, 4096, rows, 1);
+    *bytes = lt_bytes(g);
+    return lt_columns(g);
+}
 
 // x [T, K] of type dt, y and out [T, N] of type dt_y, rows strided; out may be y. a [adapters, slices, rank, K],
 // b [adapters, N, rank] of type dt; widths: each slice's columns. `work` holds `work_ints` 32-bit
