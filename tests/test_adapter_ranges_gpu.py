@@ -1,5 +1,5 @@
 """The low-rank product of every row's own adapter at the ends of its ranges: numbers that round to infinity, more rows than a
-grid holds. Statement and bounds of test_adapters_gpu.py, each test by the ways it names."""
+grid holds; and the launches it counts. Statement and bounds of test_adapters_gpu.py, each test by the ways it names."""
 import pytest
 import torch
 
@@ -47,3 +47,21 @@ def test_more_rows_than_a_grid_has_tiles(by, way):
     want, size = plain(x, y, p["a"], p["b"], p["scale"], ids, (32,), False)
     off = (out[at].double().cpu() - want).abs()
     assert (off <= bound(want, size, 32, 8, BF, BF)).all()
+
+
+@pytest.mark.parametrize("T,K,counts", [(1, 64, (1, 1, 3)), (300, 64, (1, 1, 3)), (600, 64, (2, 2, 3)), (1024, 64, (3, 2, 3)),
+                                        (20, 60, (2, 2, 2)), (600, 60, (2, 2, 2))])
+def test_launches_are_counted(by, T, K, counts):
+    """One kernel where the clusters find their rows, two with a plan or by the general kernels, three by tiles."""
+    o = ops()
+    p = inputs(T, K, (32,), 8, 2, BF, BF, seed=T)
+    for way in (CHOSEN, CLUSTERS, TILES):
+        by(way)
+        before = o.LAUNCHES[0]
+        o.low_rank_add(p["x"], p["y"], p["a"], p["b"], p["scale"], p["ids"], (32,))
+        assert o.LAUNCHES[0] - before == counts[way]
+
+
+def test_rows_that_need_no_workspace():
+    """The number of rows up to which a call is tried without a workspace is the library's own."""
+    assert ops().LOW_RANK_SCANNED == ops().entry_points("adapters").tgo_low_rank_scanned_rows()

@@ -1202,8 +1202,7 @@ template <typename T> static bool lr_vectors(const LowRank& p) {
     return true;
 }
 
-// Rows from which they are planned: up to here each cluster of the kernel for few rows finds its own.
-
+// Whether each cluster of the kernel for few rows finds its rows by itself; a call with more rows or more adapters is planned.
 static bool lr_scanned(const LowRank& p) { return p.T <= LR_SCAN_ROWS && p.adapters <= LR_SCAN_ADAPTERS; }
 template <typename T> static bool lr_few_takes(const LowRank& p) {
     return lr_vectors<T>(p) && lf_floats<T>(p.columns.slices * p.rank, p.K) * 4 <= 200 * 1024 && p.T <= (1 << 24) &&
@@ -1458,12 +1457,15 @@ template <typename T, typename TY> static long long lr_work(const LowRank& p) {
     return (long long)p.T * width;
 }
 
+// What a call returns: an error, 0 for one kernel launched, or minus the number of them.
+static int lr_done(int rc, int kernels) { return rc || kernels == 1 ? rc : -kernels; }
+
 template <typename T, typename TY> static int low_rank_launch(const LowRank& p, void* work, long long work_ints, cudaStream_t stream) {
     if (work_ints < lr_work<T, TY>(p)) return LR_E_WORK;
     if constexpr (sizeof(T) == 2)
-        if (lr_many(p) && lr_tile_takes<TY>(p)) return low_rank_tiles<TY>(p, (int*)work, stream);
-    if (lr_few_takes<T>(p)) return low_rank_few<T, TY>(p, (int*)work, stream);
-    return low_rank_any<T, TY>(p, (float*)work, stream);
+        if (lr_many(p) && lr_tile_takes<TY>(p)) return lr_done(low_rank_tiles<TY>(p, (int*)work, stream), 3);
+    if (lr_few_takes<T>(p)) return lr_done(low_rank_few<T, TY>(p, (int*)work, stream), lr_scanned(p) ? 1 : 2);
+    return lr_done(low_rank_any<T, TY>(p, (float*)work, stream), 2);
 }
 
 static bool lr_fill(LowRank& p, int T, int K, int N, int adapters, int rank, int slices, const int* widths, int interleaved) {
@@ -1493,10 +1495,13 @@ TGO_API int tgo_low_rank_tile_needs(int width, int rows, int* bytes) {
     return lt_columns(g);
 }
 
+// Rows up to which a call of up to LR_SCAN_ADAPTERS adapters needs no workspace, if the kernel for few rows takes it.
+TGO_API int tgo_low_rank_scanned_rows() { return LR_SCAN_ROWS; }
+
 // x [T, K] of type dt, y and out [T, N] of type dt_y, rows strided; out may be y. a [adapters, slices, rank, K],
 // b [adapters, N, rank] of type dt; widths: each slice's columns. `work` holds `work_ints` 32-bit
 // numbers and lies on 16 bytes; LR_E_WORK: too few (for up to 512 rows most calls need none). With `needs` given
-// nothing runs, and it gets how many the call needs.
+// nothing runs, and it gets how many the call needs. Returns an error, 0 for one kernel launched, or minus the number of them.
 TGO_API int tgo_low_rank_add(const void* x, long long x_stride, const void* y, long long y_stride, void* out,
                              long long out_stride, const void* a, const void* b, const float* scale, const int* ids,
                              int dt, int dt_y, int T, int K, int N, int adapters, int rank, int slices, const int* widths,

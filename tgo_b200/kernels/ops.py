@@ -2223,7 +2223,9 @@ def low_rank_add(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.Ten
         needs = T * (S * ((r + 15) // 16 * 24) + 4) + 8
         work = x.new_empty(needs, dtype=torch.int32)
         status = call(*args, work.data_ptr(), needs, 0, _stream())
-        LAUNCHES[0] += 1
+    if status < 0:                          # minus the number of kernels, where there are several
+        LAUNCHES[0] -= status + 1
+        status = 0
     _check(status, "low_rank_add", f"(T={T}, K={K}, rank={r}, slices {tuple(widths)}{' in eights' if interleaved else ''} "
                                    f"of {N} columns)" if status else "")
 
