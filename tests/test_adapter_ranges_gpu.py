@@ -1,9 +1,9 @@
 """The low-rank product of every row's own adapter at the ends of its ranges: numbers that round to infinity, more rows than a
-grid holds; and the launches it counts. Statement and bounds of test_adapters_gpu.py, each test by the ways it names."""
+plan or a grid holds, the widest product. Statement and bounds of test_adapters_gpu.py, each test by the ways it names."""
 import pytest
 import torch
 
-from test_adapters_gpu import BF, DEV, TYPES, bound, check, inputs, ops, plain
+from test_adapters_gpu import BF, DEV, F32, TYPES, bound, check, inputs, ops, plain
 
 pytestmark = pytest.mark.gpu
 
@@ -47,6 +47,26 @@ def test_more_rows_than_a_grid_has_tiles(by, way):
     want, size = plain(x, y, p["a"], p["b"], p["scale"], ids, (32,), False)
     off = (out[at].double().cpu() - want).abs()
     assert (off <= bound(want, size, 32, 8, BF, BF)).all()
+
+
+@pytest.mark.parametrize("T,adapters", [(8192, 3), (8193, 255), (20001, 3), (20001, 255), (20001, 300)])
+@pytest.mark.parametrize("way,x_type", [(CLUSTERS, F32), (CLUSTERS, BF), (TILES, BF)])
+def test_more_rows_than_the_plan_holds(by, way, x_type, T, adapters):
+    """From 8193 rows on the plan reads some of their adapters a second time; from 256 adapters on it counts another way.
+    Rows in any order, then in runs of one adapter."""
+    by(way)
+    ids = torch.randint(-1, adapters, (T,), generator=torch.Generator().manual_seed(T + adapters))
+    p = inputs(T, 32, (32,), 8, adapters, x_type, x_type, seed=T, ids=ids.to(torch.int32))
+    check(p, (32,))
+    check({**p, "ids": ids.sort().values.roll(77).to(torch.int32).to(DEV)}, (32,))
+
+
+@pytest.mark.parametrize("T", [1, 96, 1100])
+@pytest.mark.parametrize("way,rank", [(CLUSTERS, 4), (CLUSTERS, 16), (TILES, 16)])
+def test_the_widest_product(by, way, rank, T):
+    """A feed-forward's last product, 12288 wide, into the float32 stream: one token, a batch of tokens, a prompt."""
+    by(way)
+    check(inputs(T, 12288, (256,), rank, 3, BF, F32, seed=T + rank), (256,), in_place=True)
 
 
 @pytest.mark.parametrize("T,K,counts", [(1, 64, (1, 1, 3)), (300, 64, (1, 1, 3)), (600, 64, (2, 2, 3)), (1024, 64, (3, 2, 3)),

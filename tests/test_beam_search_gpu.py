@@ -147,3 +147,42 @@ def test_plain_requests_keep_their_bits_when_adapters_are_loaded(tmp_path):
     model.load_adapters(adapters_for(w))
     assert torch.equal(logits_of(model), before)
     assert model.generate(prompts, Policy(max_tokens=5)) == text
+
+
+@pytest.mark.parametrize("name,adapter", [("B", None), ("C", "all")])
+def test_searches_in_bfloat16_read_their_own_pages(tmp_path, name, adapter):
+    """What every beam of a bfloat16 search sees behind each prefix of its hypothesis, through pages that the beams share,
+    copy and give up, is what a whole forward over that text gives."""
+    import tgo_b200
+    from tgo_b200.engine.beams import BeamSearch
+    cfg, run = tiny.TINIES[name]
+    d = tiny.make_model_dir(tmp_path / name, cfg, run["seed"], run["sigma"])
+    pcfg, w = plain.load_model_dir(d)
+    model = tgo_b200.open(d, dtype="bfloat16", device=DEV)
+    if adapter:
+        adapters = adapters_for(w, rank=16)
+        model.load_adapters(adapters)
+        w = with_adapter(w, adapters[adapter].matrices, adapters[adapter].scale)
+    prompts = list(tiny.random_requests(cfg["vocab_size"], [13, 40], seed=9).values())
+    seen = {}
+
+    class Watched(BeamSearch):
+        def _advance(self, searches, logits):
+            rows = logits.cpu().numpy()
+            for i, s in enumerate(searches):
+                for k, (t, score) in enumerate(zip(s.tokens, s.scores)):
+                    if score > -np.inf:
+                        seen[(s.rids[0][2], tuple(t))] = rows[i * self.beams + k]
+            return super()._advance(searches, logits)
+    eng = model.new_engine(page_size=4, max_tokens=600, num_slots=8)
+    found = Watched(eng, 4, 22).run(prompts, [adapter] * 2)
+    assert all(len(q) == 4 and all(len(h.tokens) == 22 for h in q) for q in found)
+    got, want, rounded = {}, {}, {}
+    for q, p in enumerate(prompts):
+        for i, h in enumerate(found[q]):
+            text = p + h.tokens
+            want[(q, i)], rounded[(q, i)] = plain.forward(pcfg, w, text), plain.forward_rounded(pcfg, w, text)
+            for n in range(22):
+                got[((q, i), len(p) - 1 + n)] = seen[(q, tuple(h.tokens[:n]))]
+    worst, where, allowed = tiny.compare(got, want, cfg, "bfloat16", f"bfloat16 search/{name}", rounded)
+    assert worst <= allowed, (worst, where, allowed)
