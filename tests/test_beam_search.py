@@ -421,3 +421,16 @@ def test_adapters_that_the_engine_cannot_hold(emulated, tmp_path, dtype, number)
             loaded.load_adapters({"big": Adapter({n: (a * big_a, b * big_b)}, scale)})
     assert loaded.model.adapter_names == []
     loaded.load_adapters({"large": Adapter({n: (a * number / 1e3, b)}, 1e30)})
+
+
+@pytest.mark.parametrize("begun,fine", [(True, True), (False, True), ("gaussian", True), ("pissa", False), ("pissa_niter_4", False),
+                                        ("olora", False), ("loftq", False)])
+def test_adapters_of_changed_matrices_are_refused(tmp_path, begun, fine):
+    """Halves that were begun from parts of the model's matrices are added to what was left of those."""
+    halves = {"x.lora_A.weight": torch.ones(2, 4), "x.lora_B.weight": torch.ones(4, 2)}
+    folder = write_folder(tmp_path / "a", {"r": 2, "lora_alpha": 2, "init_lora_weights": begun}, halves)
+    if fine:
+        assert set(read_adapter(folder).matrices) == {"x.weight"}
+    else:
+        with pytest.raises(AdapterError, match="init_lora_weights"):
+            read_adapter(folder)

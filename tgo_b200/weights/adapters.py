@@ -52,6 +52,10 @@ def read_adapter(folder: str) -> Adapter:
                        ("rank_pattern", (None, {})), ("alpha_pattern", (None, {})), ("fan_in_fan_out", (None, False))):
         if config.get(key) not in plain:
             raise AdapterError(f"adapter {folder}: adapter_config.json: {key} = {config[key]!r} is not supported")
+    # how the halves were begun matters only where the model's own matrices were changed for it
+    if config.get("init_lora_weights") not in (None, True, False, "gaussian", "eva", "orthogonal"):
+        raise AdapterError(f"adapter {folder}: adapter_config.json: init_lora_weights = {config['init_lora_weights']!r}: the halves "
+                           "may belong to matrices that were changed when they were begun")
     scale = alpha / math.sqrt(rank) if config.get("use_rslora") else alpha / rank
     file = SafetensorsFile(os.path.join(folder, "adapter_model.safetensors"))
     halves: Dict[str, Dict[str, torch.Tensor]] = {}
