@@ -137,7 +137,9 @@ class LoadedModel:
     def beam_search(self, prompts, beams: int = 4, max_tokens: int = 32, adapters=None, stop_ids=(),
                     length_penalty: float = 1.0, chunk: int = 2048, page_size: int = 16):
         """Every prompt's best hypotheses (engine/beams.py: Hypothesis), the one worth most first, at
-        most `beams` of each; the prompts run together. `adapters` as for `generate`."""
+        most `beams` of each. The prompts are run one after the other, then all beams of all of them as
+        one decode batch. `adapters` as for `generate`. Each call makes an engine, with its pools and decode
+        graphs; for many searches make one (`new_engine`) and hand it to engine/beams.py: BeamSearch."""
         from .engine.beams import BeamSearch
         prompts = [list(map(int, p)) for p in prompts]
         # a prompt's pages once, and per beam what it generates and the page it shares in part

@@ -568,11 +568,12 @@ low_rank_few_kernel(const LowRank p, const int* __restrict__ perm, const int* __
 // u (`low_rank_u_kernel`): X[rows] A^T on tcgen05, a cluster 64 or 128 rows, a part of k a block: TMA brings 64 columns of
 // the rows (one box where they lie together, else four rows a request) and of A into a ring, a thread issues the products.
 // Each block sends its sums to the blocks that add them, by rows, through their shared memory; these scale u and split it.
-// Bound by x's way into the multiprocessors: 26 of the 67 us of 8192 rows, width 4096, rank 64, q, k and v.
+// Bound by x's way into the multiprocessors: 26 of the 66 us of 8192 rows, width 4096, rank 64, q, k and v (calls in a graph; 70
+// where the host makes each call).
 //
 // out (`low_rank_out_kernel`): u and 64 columns of B at a time come by TMA, a thread issues the products into four
 // accumulators in turn, eight warps add them to y in shared memory, from where TMA stores it. Bound by y's and out's way:
-// 36 of the 67 us, 5.6 TB/s.
+// 36 of the 66 us, 5.6 TB/s.
 #define LT_ROWS 128
 #define LT_BK 64
 #define LT_STAGES 6               // of the ring, at most 8

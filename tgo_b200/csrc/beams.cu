@@ -17,10 +17,10 @@
 // few rows, in the first block of a cluster. v is formed in 64 bits: candidates of one beam are ordered as their logits are, those of
 // different beams but for the error of the sums under the logarithms, which are 32-bit sums of approximate exponentials.
 //
-// MEASURED (B200): 512 rows of 151936 and 16 picks 57 us, 5.4 TB/s; without looking for candidates the same
-// pass takes 50, with a look only every fourth turn, at values read again, 64, from a ring filled by bulk
-// copies 66, with warps that meet only when one has found enough 65. 64 rows of it 15.6 us; one live beam of five in 12
-// requests 10.4 (13.8 where the others' blocks find nothing to do); 4 rows of 32768 7.8. There the kernels' latencies
+// MEASURED (B200, calls in a graph): 512 rows of 151936 and 16 picks 57.4 us, 5.4 TB/s (59.7 where the host makes each call);
+// without looking for candidates the same pass takes 50, with a look only every fourth turn, at values read again, 64, from a ring filled by bulk
+// copies 66, with warps that meet only when one has found enough 65. 64 rows of it 15.4 us; one live beam of five in 12
+// requests 10.3 (13.8 where the others' blocks find nothing to do); 4 rows of 32768 7.6. There the kernels' latencies
 // show, about 4 and 3 us, and the first turns' many candidates.
 #define BS_THREADS 256
 #define BS_VPT 4                  // vectors of four values a thread and turn

@@ -92,7 +92,10 @@ class SwiGLU(Part):
 
     def _adapted(self, x, ctx, residual):
         """The forward of a step with adapted rows: the gate and up rows are written out, so that the
-        adapters add to them before the gate is applied."""
+        adapters add to them before the gate is applied. They are written in the activations' type, as
+        where the gate is a kernel of its own anyway (`ops.gated_linear`): half the bytes of float32 rows,
+        and a rounding more than where the product's own kernel applies the gate. So the last bits of a
+        request without an adapter may differ beside one that has one."""
         x = ops.rows_of(x)
         if "gate_up" in self.adapters:
             rows = ops.linear(x, self.w_gate_up)
