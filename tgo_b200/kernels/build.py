@@ -50,6 +50,8 @@ LIBRARIES = {
     "sampling": (["sampling.cu"], []),
     "beams": (["beams.cu"], []),
     "adapters": (["adapters.cu"], []),
+    "attention_tree": (["attention_tree.cu"], []),
+    "drafts": (["drafts.cu"], []),
     # host code only (no kernel): the cache books and the packing of a step
     "host_runtime": (["host_runtime.cpp"], []),
     # calls of the other libraries' entry points (a Python extension; see `entry_points`)

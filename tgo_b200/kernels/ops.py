@@ -2246,6 +2246,177 @@ def low_rank_error() -> int:
 _tc_err = {}
 
 
+TREE_NODES = 64          # drafted tokens of a request that the kernels take: what a node sees is a 64-bit number
+
+
+def attention_tree(q: torch.Tensor, out: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int,
+                   k_cache: torch.Tensor, v_cache: torch.Tensor, page_size: int, block_tables: torch.Tensor,
+                   context_lens: torch.Tensor, q_start: torch.Tensor, seen: torch.Tensor, scale: float, window: int,
+                   max_nodes: int, max_context: int) -> None:
+    """Attention of trees of drafted tokens over the paged cache: request b's tokens q_start[b] .. q_start[b + 1] - 1
+    are its nodes, at most 64, whose keys and values are stored at the last places of its cache,
+    base .. context_lens[b] - 1, in their order. Bit j of seen[t]: token t sees its request's node j. With its position
+    base + (bits set) - 1, it sees every cached key before base too, or those less than `window` before its position.
+    A token that sees nothing gets zeros, and so do those of a request whose context is shorter than its nodes (a padded
+    one). Rows that no request has are left as they are. What lies in places that a token does not see does not reach it.
+
+    q, out [T, >= heads * head_dim] float32 or bfloat16, rows may be strided; k_cache, v_cache [pages, kv heads, page_size,
+    head_dim] of that type; block_tables int32 [B, width], context_lens int32 [B], q_start int32 [B + 1], seen int64
+    [T]. head_dim at most 256. max_nodes, max_context: the most that any request of the call has."""
+    if not (q.is_cuda and out.is_cuda and k_cache.is_cuda and v_cache.is_cuda and block_tables.is_cuda and
+            context_lens.is_cuda and q_start.is_cuda and seen.is_cuda):
+        _need_cuda(q, out, k_cache, v_cache, block_tables, context_lens, q_start, seen)
+    T, kind, shape = q.shape[0], q.dtype, k_cache.shape
+    B, width = block_tables.shape
+    code = dtype_code(kind)
+    (qs, q1), (os, o1) = q.stride(), out.stride()
+    assert out.dtype == k_cache.dtype == v_cache.dtype == kind and q1 == o1 == 1 and out.shape[0] == T
+    assert q.shape[1] >= num_heads * head_dim and out.shape[1] >= num_heads * head_dim
+    assert shape[1:] == (num_kv_heads, page_size, head_dim) and v_cache.shape == shape
+    assert k_cache.is_contiguous() and v_cache.is_contiguous()
+    assert block_tables.dtype == context_lens.dtype == q_start.dtype == torch.int32 and seen.dtype == torch.int64
+    assert block_tables.is_contiguous() and context_lens.is_contiguous() and q_start.is_contiguous() and seen.is_contiguous()
+    assert context_lens.shape == (B,) and q_start.shape == (B + 1,) and seen.shape == (T,)
+    if not 0 <= max_nodes <= TREE_NODES:
+        raise KernelError(f"attention_tree: {max_nodes} drafted tokens of a request; at most {TREE_NODES}")
+    if T == 0 or B == 0:
+        return
+    lib = entry_points("attention_tree")
+    work = q.new_empty(lib.tgo_attention_tree_work(code, head_dim), dtype=torch.float32)
+    _check(lib.tgo_attention_tree(q.data_ptr(), qs, out.data_ptr(), os, code, k_cache.data_ptr(), v_cache.data_ptr(), shape[0],
+                                  page_size, block_tables.data_ptr(), width, context_lens.data_ptr(), q_start.data_ptr(),
+                                  seen.data_ptr(), B, num_heads, num_kv_heads, head_dim, window, work.data_ptr(), _stream(),
+                                  float(scale)), "attention_tree",
+           f"(head_dim={head_dim}, heads={num_heads}/{num_kv_heads}, page_size={page_size}, window={window})")
+    LAUNCHES[0] += 1
+
+
+def logits_constrain(logits: torch.Tensor, owner: Optional[torch.Tensor] = None, bias=None, history=None,
+                     penalties: Optional[torch.Tensor] = None, windows: Optional[torch.Tensor] = None, drafts=None,
+                     allowed: Optional[torch.Tensor] = None, allowed_rows: Optional[torch.Tensor] = None,
+                     out: Optional[torch.Tensor] = None) -> None:
+    """Biases, penalties for repeated tokens and masks of allowed tokens on all rows of logits, into `out` or in place.
+    Row r of request q = owner[r] (None: q = r; outside 0..Q-1: no biases or penalties): first the request's biases are
+    added; then, for a token that stands c > 0 times in the last windows[q] tokens (0 or None: all) of its history, and a
+    repetition penalty that is neither 0 nor 1, a positive logit is divided by it and another multiplied, and
+    presence + frequency * c is taken off; then tokens that row allowed_rows[r] (None: r; outside: no mask) of `allowed`
+    does not name become -inf.
+
+    logits, out float32 [R, V], rows may be strided; owner int32 [R]. bias: (int32 starts [Q + 1], int32 ids, float32
+    values), a request's ids distinct. history: (int32 starts [Q + 1], int32 tokens). penalties float32 [Q, 3]: repetition,
+    presence, frequency; windows int32 [Q]. drafts: (q_start int32 [Q + 1], drafted tokens int32, seen int64 [R]): behind
+    the history of row r come the drafted tokens of its request that the bits of seen[r] name. allowed int32
+    [M, words >= V / 32]: bit i % 32 of word i / 32 allows token i; allowed_rows int32 [R]. Token ids outside the
+    vocabulary are passed over."""
+    if out is None:
+        out = logits
+    if not (logits.is_cuda and out.is_cuda):
+        _need_cuda(logits, out)
+    R, V = logits.shape
+    (s_in, s1), (s_out, s2) = logits.stride(), out.stride()
+    assert logits.dtype == out.dtype == torch.float32 and out.shape == (R, V) and (V <= 1 or s1 == s2 == 1)
+    assert R <= 1 or (s_in >= V and s_out >= V)
+    at, to = logits.data_ptr(), out.data_ptr()
+    if R and V and (s_in != s_out if at == to else
+                    at < to + 4 * ((R - 1) * s_out + V) and to < at + 4 * ((R - 1) * s_in + V)):
+        raise KernelError("logits_constrain: `out` lies over other rows of the logits; the same rows, or rows of its own")
+    Q = R
+
+    def take(t, kind, shape=None):
+        if not t.is_cuda:
+            _need_cuda(t)
+        assert t.dtype == kind and t.is_contiguous() and (shape is None or t.shape == shape)
+        return t.data_ptr()
+
+    for t in (penalties, windows):
+        if t is not None:
+            Q = t.shape[0]
+    for t in (bias, history, drafts):
+        if t is not None:
+            Q = t[0].shape[0] - 1
+    i32, f32 = torch.int32, torch.float32
+    p_owner = take(owner, i32, (R,)) if owner is not None else 0
+    b0 = b1 = b2 = h0 = h1 = d0 = d1 = d2 = words = m = width = 0
+    if bias is not None:
+        b0, b1, b2 = take(bias[0], i32, (Q + 1,)), take(bias[1], i32), take(bias[2], f32, bias[1].shape)
+    if history is not None:
+        h0, h1 = take(history[0], i32, (Q + 1,)), take(history[1], i32)
+    if drafts is not None:
+        d0, d1, d2 = take(drafts[0], i32, (Q + 1,)), take(drafts[1], i32), take(drafts[2], torch.int64, (R,))
+    p_pen = take(penalties, f32, (Q, 3)) if penalties is not None else 0
+    p_win = take(windows, i32, (Q,)) if windows is not None else 0
+    if allowed is not None:
+        m, width = allowed.shape
+        words = take(allowed, i32)
+        if width * 32 < V:
+            raise KernelError(f"logits_constrain: masks of {width} words for {V} tokens")
+    p_rows = take(allowed_rows, i32, (R,)) if allowed_rows is not None else 0
+    if R == 0 or V == 0:
+        return
+    _check(entry_points("drafts").tgo_logits_constrain(
+        at, s_in, to, s_out, R, V, Q, p_owner, b0, b1, b2, h0, h1, p_pen, p_win, d0, d1, d2, words, width, m, p_rows,
+        _stream()), "logits_constrain", f"(R={R}, V={V})")
+
+
+def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, chosen: torch.Tensor, q_start: torch.Tensor, path: torch.Tensor,
+                counts: torch.Tensor, following: torch.Tensor) -> None:
+    """The path through each request's tree of drafted tokens that the tokens chosen at its nodes confirm: node 0 (the token
+    that is certain), then from every node the first later one whose parent it is and whose token is the one chosen at it.
+    path[q_start[b] + j] = the path's node j (-1 behind its end), counts[b] = its length, following[b] = the token
+    chosen at its last node: the one that comes next. A request without nodes gets 0 and -1.
+
+    tokens, parents (a node's place in its request; below its own, or -1), chosen, path int32 [T]; q_start int32 [B + 1], at
+    most 64 nodes a request; counts, following int32 [B]."""
+    if not (tokens.is_cuda and parents.is_cuda and chosen.is_cuda and q_start.is_cuda and path.is_cuda and counts.is_cuda and
+            following.is_cuda):
+        _need_cuda(tokens, parents, chosen, q_start, path, counts, following)
+    shape, each = tokens.shape, counts.shape
+    assert len(shape) == len(each) == 1 and parents.shape == chosen.shape == path.shape == shape and following.shape == each
+    assert q_start.shape == (each[0] + 1,)
+    for t in (tokens, parents, chosen, q_start, path, counts, following):
+        assert t.dtype == torch.int32 and t.is_contiguous()
+    if each[0] == 0:
+        return
+    _check(entry_points("drafts").tgo_tree_accept(tokens.data_ptr(), parents.data_ptr(), chosen.data_ptr(), q_start.data_ptr(),
+                                                  each[0], path.data_ptr(), counts.data_ptr(), following.data_ptr(), _stream()),
+           "tree_accept", f"(B={each[0]})")
+
+
+def tree_keep(tensors, slots: torch.Tensor, q_start: torch.Tensor, path: torch.Tensor, counts: torch.Tensor, axis: int = 0) -> None:
+    """The rows of the accepted nodes moved together: for every request b and j < counts[b], in every tensor, the row of
+    place slots[q_start[b] + j] <- that of place slots[q_start[b] + path[q_start[b] + j]], in place, each as it was
+    before the call. Pages lie along `axis`; a page is [heads, page_size, width] (or [page_size, width]), a place is
+    page * page_size + offset, and what lies before `axis` is gone through page by page. A path ascends
+    (`tree_accept`'s do); an entry of it outside its request or below j, or a place outside the tensor, is passed over.
+
+    tensors contiguous, all with pages of one size; slots, path int32 [T] (a request's slots distinct), q_start int32
+    [B + 1], counts int32 [B]."""
+    if not (slots.is_cuda and q_start.is_cuda and path.is_cuda and counts.is_cuda):
+        _need_cuda(slots, q_start, path, counts)
+    shape, (B,) = slots.shape, counts.shape
+    assert path.shape == shape and q_start.shape == (B + 1,)
+    assert slots.dtype == q_start.dtype == path.dtype == counts.dtype == torch.int32
+    assert slots.is_contiguous() and q_start.is_contiguous() and path.is_contiguous() and counts.is_contiguous()
+    desc, page_size = array("q"), 0
+    for t in tensors:
+        if not t.is_cuda:
+            _need_cuda(t)
+        one, size = t.shape, t.element_size()
+        rest = len(one) - axis
+        assert 0 <= axis and rest in (3, 4) and t.is_contiguous() and size >= 2
+        if page_size and one[-2] != page_size:
+            raise KernelError(f"tree_keep: pages of {one[-2]} places beside pages of {page_size}")
+        page_size = one[-2]
+        if t.numel():
+            desc.extend((t.data_ptr(), math.prod(one[:axis]), one[axis], one[axis + 1] if rest == 4 else 1, one[-1] * size))
+    if not desc or B == 0:
+        return
+    _check(entry_points("drafts").tgo_tree_keep(desc.buffer_info()[0], len(desc) // 5, page_size, slots.data_ptr(),
+                                                q_start.data_ptr(), B, path.data_ptr(), counts.data_ptr(), _stream()),
+           "tree_keep", f"(B={B}, page_size={page_size})")
+    LAUNCHES[0] += (len(desc) // 5 - 1) // 64
+
+
 def gemm_tc_error_flag(device) -> torch.Tensor:
     """The int32 flag a tensor-core product sets if one of its waits ran out (0: none;
     1 producer, 2 issuer, 3 epilogue). One per device, made at first use."""
