@@ -36,6 +36,15 @@ def paths_of(parents):
     return bits
 
 
+@pytest.fixture(params=["chosen", "FMA units"])
+def way(request):
+    """The attention goes the way that the framework chooses, and by the kernel that takes every call."""
+    ops().attention_tree_force_way(["chosen", "FMA units"].index(request.param))
+    yield request.param
+    ops().attention_tree_force_way(0)
+    assert ops().attention_tree_error() == 0
+
+
 # ------------------------------------------------------------------------------ attention
 
 
@@ -136,31 +145,31 @@ LAYOUTS = [(16, 4, 128), (32, 8, 128), (8, 2, 64), (5, 5, 64), (10, 2, 128), (16
 
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("heads,kv_heads,dim", LAYOUTS)
-def test_layouts(dtype, heads, kv_heads, dim):
+def test_layouts(way, dtype, heads, kv_heads, dim):
     Trees(dtype, heads, kv_heads, dim, [0, 37, 300, 128], [3, 13, 1, 64], seed=dim + heads).check()
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("page", [1, 3, 8, 16, 32, 64, 128, 256])
-def test_page_sizes(dtype, page):
+def test_page_sizes(way, dtype, page):
     Trees(dtype, 8, 2, 128, [page - 1, 2 * page, 127], [2, 7, 33], page=page, seed=page).check()
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("window", [1, 2, 15, 64, 129, 300])
-def test_windows(dtype, dim, window):
+def test_windows(way, dtype, dim, window):
     Trees(dtype, 8, 2, dim, [0, 5, 63, 64, 500], [9, 30, 1, 17, 64], window=window, seed=window).check()
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("base", [0, 1, 62, 63, 64, 65, 126, 127, 128, 129, 255, 256])
-def test_tile_edges(dtype, base):
+def test_tile_edges(way, dtype, base):
     Trees(dtype, 4, 2, 128, [base], [5], seed=base).check()
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
-def test_one_node_is_a_decode_step(dtype):
+def test_one_node_is_a_decode_step(way, dtype):
     """The same keys through the decode attention: a node alone sees its whole request."""
     c = Trees(dtype, 16, 4, 128, [700, 15, 0, 129], [1, 1, 1, 1], seed=4, spare=0)
     mine = c.check()[:, :16 * 128].float()
@@ -178,7 +187,7 @@ def test_one_node_is_a_decode_step(dtype):
 
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("dim", [64, 128])
-def test_many_requests_of_unlike_lengths(dtype, dim):
+def test_many_requests_of_unlike_lengths(way, dtype, dim):
     """Requests without nodes and padded ones among them, items that several workers share."""
     rng = random.Random(dim)
     lens = [rng.choice([0, 1, 17, 130, 900, 2500]) for _ in range(41)]
@@ -197,13 +206,13 @@ def test_many_requests_of_unlike_lengths(dtype, dim):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
-def test_one_long_request(dtype):
+def test_one_long_request(way, dtype):
     Trees(dtype, 4, 1, 128, [33000], [3], seed=9).check()
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("dim", [64, 128])
-def test_empty_rows_and_masks_that_are_no_tree(dtype, dim):
+def test_empty_rows_and_masks_that_are_no_tree(way, dtype, dim):
     c = Trees(dtype, 8, 2, dim, [0, 0, 40], [4, 64, 20], seed=1)
     rng = random.Random(5)
     c.bits = [0, 1 << 3, 0b1011, 0] + [rng.getrandbits(64) & rng.getrandbits(64) & rng.getrandbits(64) for _ in range(64)] + \
@@ -219,7 +228,7 @@ def test_empty_rows_and_masks_that_are_no_tree(dtype, dim):
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("what", [INF, -INF, NAN])
 @pytest.mark.parametrize("where", ["k", "v"])
-def test_what_is_masked_does_not_show(dtype, dim, what, where):
+def test_what_is_masked_does_not_show(way, dtype, dim, what, where):
     """A node whose key or value is no finite number is nothing to the nodes that do not see it; to those that do it is
     what the formula makes of it."""
     for base, window in ((0, 0), (100, 0), (120, 33), (127, 0)):
@@ -242,7 +251,7 @@ def test_what_is_masked_does_not_show(dtype, dim, what, where):
 
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("dim", [64, 128])
-def test_values_behind_the_window_do_not_show(dtype, dim):
+def test_values_behind_the_window_do_not_show(way, dtype, dim):
     """Cached keys that the first nodes see and deeper ones no more."""
     c = Trees(dtype, 8, 2, dim, [200], [20], window=50, seed=3)
     c.bits = paths_of([i - 1 for i in range(20)])              # a chain: node i at 200 + i sees keys from 151 + i on
@@ -253,7 +262,7 @@ def test_values_behind_the_window_do_not_show(dtype, dim):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
-def test_scores_of_any_size(dtype):
+def test_scores_of_any_size(way, dtype):
     """Scores up to a few hundred apart, and all alike."""
     Trees(dtype, 8, 2, 128, [500, 20], [16, 5], seed=2, size=5.0).check()
     c = Trees(dtype, 8, 2, 128, [500, 20], [16, 5], seed=2)
@@ -262,7 +271,7 @@ def test_scores_of_any_size(dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
-def test_pages_that_nobody_has(dtype):
+def test_pages_that_nobody_has(way, dtype):
     """Numbers outside the pages behind a request's end are not looked at; inside it they are no fault."""
     c = Trees(dtype, 8, 2, 128, [100, 33], [4, 4], seed=6)
     want = c.check().clone()
@@ -274,7 +283,7 @@ def test_pages_that_nobody_has(dtype):
     assert torch.equal(c.run(bad)[:4], want[:4])
 
 
-def test_attention_captured_beside_another_stream():
+def test_attention_captured_beside_another_stream(way):
     """A captured call follows what its inputs hold; two graphs and an eager call on another stream share nothing."""
     cases = [Trees(BF, 16, 4, 128, [2000, 77], [16, 5], seed=s) for s in range(3)]
     want = [c.run().clone() for c in cases]

@@ -2279,16 +2279,31 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, num_heads: int, num_kv_he
     assert context_lens.shape == (B,) and q_start.shape == (B + 1,) and seen.shape == (T,)
     if not 0 <= max_nodes <= TREE_NODES:
         raise KernelError(f"attention_tree: {max_nodes} drafted tokens of a request; at most {TREE_NODES}")
-    if T == 0 or B == 0:
+    if T == 0 or B == 0 or max_nodes == 0:
         return
     lib = entry_points("attention_tree")
-    work = q.new_empty(lib.tgo_attention_tree_work(code, head_dim), dtype=torch.float32)
-    _check(lib.tgo_attention_tree(q.data_ptr(), qs, out.data_ptr(), os, code, k_cache.data_ptr(), v_cache.data_ptr(), shape[0],
+    work = q.new_empty(lib.tgo_attention_tree_work(code, head_dim, num_heads // num_kv_heads, page_size, max_nodes),
+                       dtype=torch.float32)
+    _check(lib.tgo_attention_tree(q.data_ptr(), qs, out.data_ptr(), os, code, T, k_cache.data_ptr(), v_cache.data_ptr(), shape[0],
                                   page_size, block_tables.data_ptr(), width, context_lens.data_ptr(), q_start.data_ptr(),
-                                  seen.data_ptr(), B, num_heads, num_kv_heads, head_dim, window, work.data_ptr(), _stream(),
-                                  float(scale)), "attention_tree",
+                                  seen.data_ptr(), B, num_heads, num_kv_heads, head_dim, window, max_nodes, work.data_ptr(),
+                                  _stream(), float(scale)), "attention_tree",
            f"(head_dim={head_dim}, heads={num_heads}/{num_kv_heads}, page_size={page_size}, window={window})")
     LAUNCHES[0] += 1
+
+
+def attention_tree_force_way(way: int = 0) -> None:
+    """For tests and tuning: `attention_tree` takes the FMA units (1) or, where they take the call, the tensor cores (2)
+    instead of choosing; 0 gives the choice back."""
+    load_library("attention_tree").tgo_attention_tree_force(c_int(way))
+
+
+def attention_tree_error() -> int:
+    """The code a wait of the trees' tcgen05 kernel left when it ran out (1 copies, 2 products, 3 softmax), or 0.
+    Synchronises with the device."""
+    value = ctypes.c_int(0)
+    _check(entry_points("attention_tree").tgo_attention_tree_error(ctypes.addressof(value)), "attention_tree_error")
+    return int(value.value)
 
 
 def logits_constrain(logits: torch.Tensor, owner: Optional[torch.Tensor] = None, bias=None, history=None,
@@ -2505,6 +2520,10 @@ def kernel_wait_errors() -> dict:
         code = attention_tc_error()
         if code:
             out["attention_tc"] = code
+    if "attention_tree" in _loaded:
+        code = attention_tree_error()
+        if code:
+            out["attention_tree"] = code
     if "attention_decode_tma" in _loaded:
         code = attention_decode_tma_error()
         if code:
