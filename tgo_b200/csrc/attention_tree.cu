@@ -26,16 +26,16 @@ struct TreeWork {
     const int *context_lens, *q_start;
     int B, T, H, Hkv, window, max_nodes, max_keys;      // max_keys: what a block table can name
     int rows_per_tile, tokens_per_tile;       // a tile holds so many rows, or (if not 0) so many whole tokens
-    int key_tile, min_units;
-    int workers;                              // at most
+    int min_units, workers;                   // of a piece at least, in all at most
 };
 
 struct TreeRequest {
     int tok0, n, base, len, t_lo, tiles, row_tiles;
-    long long units;                          // of all its items
+    int units;                                // of all its items
 };
 
-__device__ __forceinline__ TreeRequest tree_request(const TreeWork& w, int b) {
+// KT: keys of a tile.
+template <int KT> __device__ __forceinline__ TreeRequest tree_request(const TreeWork& w, int b) {
     TreeRequest r;
     r.tok0 = w.q_start[b];
     r.n = min(min(max(w.q_start[b + 1] - r.tok0, 0), w.max_nodes), r.tok0 < 0 ? 0 : max(w.T - r.tok0, 0));
@@ -44,89 +44,113 @@ __device__ __forceinline__ TreeRequest tree_request(const TreeWork& w, int b) {
     const bool none = r.base < 0;             // a padded request: its rows get zeros
     const int hi = none ? 0 : min(r.len, w.max_keys);
     const int lo = w.window > 0 && r.base - w.window > 0 ? r.base - w.window : 0;
-    r.t_lo = none ? 0 : lo / w.key_tile;
-    r.tiles = max((hi + w.key_tile - 1) / w.key_tile - r.t_lo, 1);
-    const int G = w.H / w.Hkv;
+    r.t_lo = none ? 0 : lo / KT;
+    r.tiles = max((hi + KT - 1) / KT - r.t_lo, 1);
     r.row_tiles = w.tokens_per_tile ? (r.n + w.tokens_per_tile - 1) / w.tokens_per_tile
-                                    : (r.n * G + w.rows_per_tile - 1) / w.rows_per_tile;
-    r.units = (long long)r.row_tiles * w.Hkv * (r.tiles + TREE_OVERHEAD);
+                                    : (r.n * (w.H / w.Hkv) + w.rows_per_tile - 1) / w.rows_per_tile;
+    r.units = r.row_tiles * w.Hkv * (r.tiles + TREE_OVERHEAD);
     return r;
 }
 
-// All units, by one warp.
-__device__ __forceinline__ long long tree_total(const TreeWork& w) {
-    long long sum = 0;
-    for (int b = threadIdx.x & 31; b < w.B; b += 32) sum += tree_request(w, b).units;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum;
-}
-__device__ __forceinline__ int tree_workers(const TreeWork& w, long long total) {
-    const long long most = total / w.min_units;
-    return most < 1 ? 1 : most < w.workers ? (int)most : w.workers;
-}
-__device__ __forceinline__ long long tree_begin(long long total, int workers, int i) {
-    return total / workers * i + (total % workers) * i / workers;
-}
-// The request that unit u lies in and its first unit, by one warp; u < the total.
-__device__ __forceinline__ int tree_find(const TreeWork& w, long long u, long long& first) {
-    const int lane = threadIdx.x & 31;
-    long long before = 0;
-    for (int b0 = 0; b0 < w.B; b0 += 32) {
-        const long long mine = b0 + lane < w.B ? tree_request(w, b0 + lane).units : 0;
-        long long upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long other = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += other;
-        }
-        const uint32_t in = __ballot_sync(0xffffffffu, u < before + upto);
-        if (in) {
-            const int l = __ffs(in) - 1;
-            first = before + __shfl_sync(0xffffffffu, upto - mine, l);
-            return b0 + l;
-        }
-        before += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    first = before;
-    return w.B;
-}
+// How all units are cut: worker i begins at i * each + min(i, more).
+struct TreeCut {
+    int workers, each, more;
+    __device__ __forceinline__ int begin(int i) const { return i * each + min(i, more); }
+};
 
 // A worker's walk over its pieces: `next` gives them one after the other.
-struct TreeWalk {
-    long long u, end, first;                  // where it stands, where its piece ends, where request b begins
+template <int KT> struct TreeWalk {
+    TreeCut cut;
+    int u, end, first;                        // where it stands, where its piece ends, where request b begins
     int b;
     TreeRequest r;
     // of the piece
     int kvh, row_tile, from, to;              // key tiles from .. to - 1 of the item
+    // Worker i's, by one warp; no pieces if there are fewer workers.
+    __device__ __forceinline__ void find(const TreeWork& w, int i) {
+        const int lane = threadIdx.x & 31;
+        TreeRequest mine;
+        mine.units = 0;
+        if (lane < w.B) mine = tree_request<KT>(w, lane);
+        const int first_units = mine.units;
+        int total = first_units;
+        for (int c = lane + 32; c < w.B; c += 32) total += tree_request<KT>(w, c).units;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        const int most = total / w.min_units;
+        cut.workers = total == 0 ? 0 : most < 1 ? 1 : min(most, w.workers);
+        u = end = first = b = 0;
+        if (i >= cut.workers) return;
+        cut.each = total / cut.workers;
+        cut.more = total - cut.each * cut.workers;
+        u = cut.begin(i);
+        end = cut.begin(i + 1);
+        int before = 0;
+        for (int b0 = 0; b0 < w.B; b0 += 32) {
+            if (b0) {
+                mine.units = 0;
+                if (b0 + lane < w.B) mine = tree_request<KT>(w, b0 + lane);
+            }
+            int upto = mine.units;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += other;
+            }
+            const uint32_t in = __ballot_sync(0xffffffffu, u < before + upto);
+            if (in) {
+                const int l = __ffs(in) - 1;
+                b = b0 + l;
+                first = before + __shfl_sync(0xffffffffu, upto - mine.units, l);
+                r.tok0 = __shfl_sync(0xffffffffu, mine.tok0, l);
+                r.n = __shfl_sync(0xffffffffu, mine.n, l);
+                r.base = __shfl_sync(0xffffffffu, mine.base, l);
+                r.len = __shfl_sync(0xffffffffu, mine.len, l);
+                r.t_lo = __shfl_sync(0xffffffffu, mine.t_lo, l);
+                r.tiles = __shfl_sync(0xffffffffu, mine.tiles, l);
+                r.row_tiles = __shfl_sync(0xffffffffu, mine.row_tiles, l);
+                r.units = __shfl_sync(0xffffffffu, mine.units, l);
+                return;
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+    }
     __device__ __forceinline__ bool next(const TreeWork& w) {
         while (u < end) {
             while (u >= first + r.units) {
                 first += r.units;
                 if (++b >= w.B) return false;
-                r = tree_request(w, b);
+                r = tree_request<KT>(w, b);
             }
             const int item_units = r.tiles + TREE_OVERHEAD;
-            const int item = (int)((u - first) / item_units);
-            const long long s = first + (long long)item * item_units;
-            from = max((int)(u - s) - TREE_OVERHEAD, 0);
-            to = end - s >= item_units ? r.tiles : max((int)(end - s) - TREE_OVERHEAD, 0);
-            kvh = item / r.row_tiles;
-            row_tile = item % r.row_tiles;
+            const int item = (u - first) / item_units;
+            const int s = first + item * item_units;
+            from = max(u - s - TREE_OVERHEAD, 0);
+            to = end - s >= item_units ? r.tiles : max(end - s - TREE_OVERHEAD, 0);
+            kvh = r.row_tiles == 1 ? item : item / r.row_tiles;
+            row_tile = item - kvh * r.row_tiles;
             u = s + item_units;
             if (to > from) return true;
         }
         return false;
     }
 };
-// The walk of worker i, found by one warp.
-__device__ __forceinline__ TreeWalk tree_walk(const TreeWork& w, long long total, int workers, int i) {
-    TreeWalk k;
-    k.u = tree_begin(total, workers, i);
-    k.end = tree_begin(total, workers, i + 1);
-    k.b = tree_find(w, k.u, k.first);
-    k.r = tree_request(w, min(k.b, w.B - 1));
-    return k;
+
+// What worker i leaves for the join about an item that it begins and does not end; n_rows is 0 where there is none.
+struct TreeNote {
+    int parts, n_rows, row0, tok0, kvh;       // workers with a part; rows row0 .. of the request that begins at token tok0
+};
+template <int KT> __device__ __forceinline__ TreeNote tree_note(const TreeWork& w, const TreeWalk<KT>& k, int i) {
+    TreeNote t = {0, 0, 0, 0, 0};
+    if (k.from > 0 || k.to == k.r.tiles) return t;
+    t.parts = 2;
+    while (k.cut.begin(i + t.parts) < k.u) ++t.parts;          // u is where the item ends
+    const int G = w.H / w.Hkv, per_tile = w.tokens_per_tile ? w.tokens_per_tile * G : w.rows_per_tile;
+    t.row0 = k.row_tile * per_tile;
+    t.n_rows = min(k.r.n * G - t.row0, per_tile);
+    t.tok0 = k.r.tok0;
+    t.kvh = k.kvh;
+    return t;
 }
 
 // What a row may see of its request's keys.
@@ -169,32 +193,32 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
     const T* __restrict__ q, long long q_stride, T* __restrict__ out, long long out_stride, const T* __restrict__ k_cache,
     const T* __restrict__ v_cache, int n_pages, int page_size, const int* __restrict__ block_tables, int max_blocks,
     const unsigned long long* __restrict__ seen, int dh, float scale, const TreeWork w, float* __restrict__ part_o,
-    float* __restrict__ part_ml) {
+    float* __restrict__ part_ml, TreeNote* __restrict__ notes) {
     constexpr int LD = DP + 4, LS = TP_KEYS + 4, J = DP / 64;
     extern __shared__ __align__(16) float tp_smem[];
     float* sq = tp_smem;                          // [TP_ROWS][LD]
     float* sk = sq + TP_ROWS * LD;                // [TP_KEYS][LD]
     float* sv = sk + TP_KEYS * LD;                // [TP_KEYS][LD]
     float* ss = sv + TP_KEYS * LD;                // [TP_ROWS][LS]
-    __shared__ TreeWalk s_walk;
-    __shared__ int s_workers;
+    __shared__ TreeWalk<TP_KEYS> s_walk;
     pdl_wait();
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     if (tid < 32) {
-        const long long total = tree_total(w);
-        const int workers = total > 0 ? tree_workers(w, total) : 0;
-        TreeWalk k;
-        if ((int)blockIdx.x < workers) k = tree_walk(w, total, workers, blockIdx.x);
-        if (tid == 0) { s_workers = workers; if ((int)blockIdx.x < workers) s_walk = k; }
+        TreeWalk<TP_KEYS> k;
+        k.find(w, blockIdx.x);
+        if (tid == 0) {
+            s_walk = k;
+            notes[blockIdx.x].n_rows = 0;
+        }
     }
     __syncthreads();
-    if ((int)blockIdx.x >= s_workers) return;
-    TreeWalk walk = s_walk;
+    TreeWalk<TP_KEYS> walk = s_walk;
     const int G = w.H / w.Hkv;
     const float c = scale * TREE_LOG2E;
     const bool vectors = dh % 4 == 0 && ((uintptr_t)k_cache | (uintptr_t)v_cache) % (4 * sizeof(T)) == 0;
     while (walk.next(w)) {
         const TreeRequest r = walk.r;
+        if (tid == 0 && walk.from == 0 && walk.to < r.tiles) notes[blockIdx.x] = tree_note(w, walk, blockIdx.x);
         const int row0 = walk.row_tile * TP_ROWS, n_rows = min(r.n * G - row0, TP_ROWS);
         const int kvh = walk.kvh;
         __syncthreads();                          // the last piece's rows have been read
@@ -342,12 +366,11 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
                     if (col < dh) dst[col] = from_f32<T>(o[i][d] * inv);
                 }
             } else {
-                float* dst = part_o + (slot * TP_ROWS + row) * dh;
+                const int fours = (dh + 3) / 4;
+                float4* dst = (float4*)part_o + slot * fours * TP_ROWS + row;
 #pragma unroll
-                for (int d = 0; d < J * 4; ++d) {
-                    const int col = tx * 4 + 64 * (d >> 2) + (d & 3);
-                    if (col < dh) dst[col] = o[i][d];
-                }
+                for (int j = 0; j < J; ++j)
+                    if (tx + 16 * j < fours) dst[(tx + 16 * j) * TP_ROWS] = make_float4(o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]);
                 if (tx == 0) {
                     part_ml[(slot * TP_ROWS + row) * 2] = m[i];
                     part_ml[(slot * TP_ROWS + row) * 2 + 1] = sum;
@@ -358,51 +381,64 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
 }
 
 // -------------------------------------------------------------------------- tensor cores
-// bfloat16, heads of 64 or 128, pages of 8 to 128 places: tcgen05. A tile is 128 query rows (128 / G whole nodes, row r =
-// node r / G, head r % G; rows that a short tree leaves empty cost their warps nothing) and 128 keys. One CTA an SM walks its
-// pieces with everything double-buffered: tensor memory holds S0, S1 (P lies over S) and O0, O1, shared memory two Q, two K
-// and two V tiles.
-//   warp 0        walks, asks TMA for an item's Q rows and publishes a record of the item in a ring of four;
-//   warps 12, 10  follow the records and ask TMA for the K and for the V pages;
-//   warps 1, 11   issue S = Q K^T and O += P V, a thread each;
-//   warps 2-9     softmax, two threads a row, a half of the tile's keys each.
-// The running maximum moves only when a row has outgrown it by 2^8: then the rows of O are rescaled. P is rounded to
-// bfloat16, at most 2^-8 of a weight, as the storage's own rounding is; its sum is not.
+// bfloat16, heads of 64 or 128, pages of 8 to 128 places: tcgen05, tiles of 128 keys. An item's query rows (row r = node
+// r / G, head r % G) make one tile of 128 rows or, for wide trees, two, which share the item's K and V. One persistent CTA an
+// SM walks its pieces.
+//
+// The softmax of a tile takes longer than its two products, most of it in the special-function unit, which idles while
+// scores are read, maxima found and products waited for. So there are two streams, each with scores S, sums O, a running
+// maximum and a sum of exponentials of its own, and four softmax warps, a thread a row, that need nothing of each other:
+// two row tiles, or, where there is one, the first and the second half of every key tile, put together at the item's end. A
+// step of a stream is 64 keys, and its scores have two buffers: the next step's are made while this one's exponentials run.
+//   warp 0        walks, publishes a record of every item in a ring and asks TMA for its Q rows;
+//   warp 1        issues S = Q K^T, warp 2 O += P V, a thread each;
+//   warp 3        walks too, and asks TMA for the K and the V pages, two tiles of each in flight, K one ahead;
+//   warps 4-7, 8-11   softmax of stream 0 and of stream 1; P lies over its scores;
+//   warps 12-15   clean V's tiles where that is needed, and take an item's result out of tensor memory.
+// The running maximum moves only when a row has outgrown it by 2^8: then, when the product before has run, O is rescaled. P
+// is rounded to bfloat16, at most 2^-8 of a weight, as the storage's own rounding is; its sum is not.
 // Rows of V that nobody sees are zeroed before the product, the cache may hold anything there. Where only some rows see
 // a key (the nodes, and the cached keys at the windows' edges), a value that is no finite number is zeroed too, and its
-// key noted: at the item's end the rows that see it get it added (rows are read from the cache again then).
+// key noted: at the item's end the rows that see it get it added (it is read from the cache again then).
 // Waits have a limit of about two seconds, after which a code is left, what is under way is waited for, and the CTA ends.
 #define TT_ROWS 128
 #define TT_KEYS 128
-#define TT_THREADS 416
+#define TT_THREADS 512
 #define TT_BLOCK (128 * 64 * 2)               // 128 rows x 64 columns of bfloat16
 #define TT_TILE (2 * TT_BLOCK)
-#define TT_PAGES 1024                         // pages of a piece whose numbers are kept in shared memory
 
 __device__ int tree_error_flag = 0;
 
 struct TreeItem {
     int valid;                                // 0: no more
-    int tok0, n_rows, kvh, seq;               // its tile's first token
-    int first_token;                          // its request's
+    int tok0, n_rows, kvh, seq;               // its first token
     int key_tile, n_it;                       // key tiles from .. on, 0: zeros out
     int base, n, lo, hi;                      // of the request; keys lo .. hi - 1 are somebody's
     int whole, slot;                          // the item's result, or a part of it
-    int pad[2];
+    int pad[3];
 };
 
-// Both warps of a quarter of the rows; everyone gets the OR.
-__device__ __forceinline__ bool tt_both(int quarter, bool pred) {
-    uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-                 "bar.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                 : "=r"(r) : "r"((uint32_t)pred), "r"(quarter + 1) : "memory");
-    return r != 0;
-}
 __device__ __forceinline__ float tt_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// Two numbers at a time.
+__device__ __forceinline__ unsigned long long tt_pair(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void tt_unpair(unsigned long long p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ unsigned long long tt_fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long tt_add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 __device__ __forceinline__ void tt_load_3d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
@@ -424,14 +460,20 @@ __device__ __forceinline__ uint32_t tt_finite(uint32_t x) {
     if ((x & 0x7f800000u) == 0x7f800000u) x &= 0x0000ffffu;
     return x;
 }
+__device__ __forceinline__ int tt_low(const TreeWork& w, int base) { return w.window > 0 && base > w.window ? base - w.window : 0; }
+// Whether V's tile that begins at this key holds places that not every row sees.
+__device__ __forceinline__ bool tt_mixed(int key, int base, int lo, int hi, int window) {
+    return key + TT_KEYS > min(base, hi) || (window > 0 && key < lo + TREE_NODES);
+}
 
-template <int DH>
+// DH: head size. RT: row tiles of an item (at most).
+template <int DH, int RT>
 __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q,
     const bf16* __restrict__ v_cache, int n_pages, bf16* __restrict__ out, long long out_stride, int page_size, int page_shift,
     const int* __restrict__ block_tables, int max_blocks, const unsigned long long* __restrict__ seen, float scale_log2,
-    const TreeWork w, float* __restrict__ part_o, float* __restrict__ part_ml) {
-    constexpr int NH = DH / 64, OC = DH / 2;
+    const TreeWork w, float* __restrict__ part_o, float* __restrict__ part_ml, TreeNote* __restrict__ notes) {
+    constexpr int NH = DH / 64;
     extern __shared__ unsigned char tt_raw[];
     unsigned char* base = (unsigned char*)(((uintptr_t)tt_raw + 1023) & ~(uintptr_t)1023);
     unsigned char* sQ = base;                                   // [2][2 column halves][128 rows][128 bytes]
@@ -439,33 +481,39 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
     unsigned char* sV = sK + 2 * TT_TILE;
     uint64_t* bars = (uint64_t*)(sV + 2 * TT_TILE);
     uint64_t *q_full = bars, *q_empty = bars + 2, *k_full = bars + 4, *k_empty = bars + 6, *v_full = bars + 8, *v_empty = bars + 10,
-             *s_full = bars + 12, *p_full = bars + 14, *o_free = bars + 16, *p_free = bars + 18, *o_done = bars + 20, *settled = bars + 21;
-    unsigned long long* odd_nodes = (unsigned long long*)(bars + 23);       // [4 items]: nodes, and keys lo + i, whose values
-    unsigned long long* odd_edge = odd_nodes + 4;                           // are not all finite
-    uint32_t* tmem_slot = (uint32_t*)(bars + 31);
-    TreeItem* ring = (TreeItem*)(bars + 32);                    // [4]
-    float* s_m = (float*)(ring + 4);                            // [2][2 halves][128 rows]
-    float* s_l = s_m + 512;                                     // [2 halves][128 rows]
-    int* s_pages_k = (int*)(s_l + 256);
-    int* s_pages_v = s_pages_k + TT_PAGES;
+             *told = bars + 12, *bits_told = bars + 14,         // an item's record, what its nodes see
+             *v_raw = bars + 16, *v_clean = bars + 18,          // mixed tiles: landed, cleaned
+             *o_full = bars + 20, *l_full = bars + 22, *o_free = bars + 24,         // of an item
+             *settled = bars + 26, *s_full = bars + 28, *p_full = bars + 32, *p_free = bars + 36;       // [stream][buffer]
+    unsigned long long* odd_nodes = (unsigned long long*)(bars + 40);       // [8 items]: nodes, and keys lo + i, whose values
+    unsigned long long* odd_edge = odd_nodes + 8;                           // are not all finite
+    unsigned long long* s_bits = odd_edge + 8;                  // [2][64 nodes of the item]
+    TreeItem* ring = (TreeItem*)(s_bits + 128);                 // [4]
+    float* s_m = (float*)(ring + 4);                            // [2 items][2 streams][128 rows]
+    float* s_l = s_m + 512;
+    uint4* s_stage = (uint4*)(s_l + 512);                       // [4 warps][32 rows][64 bytes]
+    uint32_t* tmem_slot = (uint32_t*)(s_stage + 512);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = w.H / w.Hkv;
+    const int tile_tokens = TT_ROWS / G, tile_rows = tile_tokens * G;       // of a row tile
     const int pages_per_tile = TT_KEYS >> page_shift;
     int* const err = &tree_error_flag;
     // rows of the Q tiles that no box writes must not hold NaN by chance
-    for (int i = tid; i < 2 * TT_TILE / 16; i += TT_THREADS) ((uint4*)sQ)[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (tid < 8) odd_nodes[tid] = 0;
+    if (tile_rows != TT_ROWS) for (int i = tid; i < 2 * TT_TILE / 16; i += TT_THREADS) ((uint4*)sQ)[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (tid < 16) odd_nodes[tid] = 0;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            tg_init(&q_full[i], 1); tg_init(&q_empty[i], 12);
+            tg_init(&q_full[i], 1); tg_init(&q_empty[i], 14);   // products 1 + 1, softmax 8, results 4
             tg_init(&k_full[i], 1); tg_init(&k_empty[i], 1);
             tg_init(&v_full[i], 1); tg_init(&v_empty[i], 1);
-            tg_init(&s_full[i], 1); tg_init(&p_full[i], 8);
-            tg_init(&o_free[i], 8); tg_init(&p_free[i], 1);
+            tg_init(&told[i], 1); tg_init(&bits_told[i], 1);
+            tg_init(&v_raw[i], 1); tg_init(&v_clean[i], 4);
+            tg_init(&s_full[i], 1); tg_init(&p_full[i], 4); tg_init(&p_free[i], 1);
+            tg_init(&s_full[2 + i], 1); tg_init(&p_full[2 + i], 4); tg_init(&p_free[2 + i], 1);
+            tg_init(&o_full[i], 1); tg_init(&l_full[i], 8); tg_init(&o_free[i], 4);
             tg_init(&settled[i], 1);
         }
-        tg_init(o_done, 1);
     }
     tg_init_done();
     if (warp == 1) tg_alloc512(tmem_slot);
@@ -476,217 +524,282 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
     pdl_wait();
 
     if (warp == 0) {
-        // ------------------------------------------------------------- pieces and Q
-        const long long total = tree_total(w);
-        const int workers = total > 0 ? tree_workers(w, total) : 0;
-        TreeWalk walk;
-        bool more = (int)blockIdx.x < workers;
-        if (more) walk = tree_walk(w, total, workers, blockIdx.x);
-        const int box_rows = w.tokens_per_tile * G;
+        // ------------------------------------------------------------- records and Q
+        TreeWalk<TT_KEYS> walk;
+        walk.find(w, blockIdx.x);
+        TreeNote note = {0, 0, 0, 0, 0};
+        if (lane == 0) notes[blockIdx.x] = note;
+        uint32_t sent = 0;                                      // items whose Q was asked for
         for (uint32_t n = 0;; ++n) {
+            // A record lies in n % 4; a buffer of Q and of what nodes see is item n's if n is even, and the other one's
+            // otherwise, or both tiles of Q are the item's.
             TreeItem* rec = &ring[n & 3];
             const uint32_t qb = n & 1u, qph = (n >> 1) & 1u;
-            if (more) more = walk.next(w);
-            if (!__all_sync(0xffffffffu, tg_wait(&q_empty[qb], qph ^ 1u, err, 1))) {
-                tg_settle_copies(q_full, 2, n, err, 1);
+            const bool more = walk.next(w);
+            const TreeRequest& r = walk.r;
+            const int token = walk.row_tile * w.tokens_per_tile;
+            // what its nodes see, read while the buffers come free
+            unsigned long long bits[2] = {0, 0};
+            if (more)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (lane + 32 * h < w.tokens_per_tile && token + lane + 32 * h < r.n)
+                        bits[h] = seen[r.tok0 + token + lane + 32 * h] & (r.n >= 64 ? ~0ull : (1ull << r.n) - 1ull);
+            bool ok = __all_sync(0xffffffffu, tg_wait(&q_empty[qb], qph ^ 1u, err, 1));
+            if (RT == 2 && ok && n > 0) ok = __all_sync(0xffffffffu, tg_wait(&q_empty[qb ^ 1u], ((n - 1u) >> 1) & 1u, err, 1));
+            if (!ok) {
+                tg_settle_copies(q_full, 2, sent, err, 1);
                 break;
             }
             if (!more) {
-                if (lane == 0) { rec->valid = 0; tg_arrive(&q_full[qb]); }
+                if (lane == 0) {
+                    rec->valid = 0;
+                    tg_arrive(&told[qb]);
+                    tg_arrive(&bits_told[qb]);
+                    notes[blockIdx.x] = note;
+                }
                 break;
             }
             if (lane == 0) {
-                const TreeRequest& r = walk.r;
-                const int token = walk.row_tile * w.tokens_per_tile;
+                const int tok0 = r.tok0 + token, lo = tt_low(w, r.base), hi = min(r.len, w.max_keys);
+                const int n_it = r.base < 0 || hi <= lo ? 0 : walk.to - walk.from;
+                const int n_rows = min(r.n - token, w.tokens_per_tile) * G;
                 rec->valid = 1;
-                rec->tok0 = r.tok0 + token;
-                rec->n_rows = min(r.n - token, w.tokens_per_tile) * G;
-                rec->kvh = walk.kvh; rec->seq = walk.b; rec->first_token = r.tok0;
+                rec->tok0 = tok0;
+                rec->n_rows = n_rows;
+                rec->kvh = walk.kvh; rec->seq = walk.b;
                 rec->key_tile = r.t_lo + walk.from;
+                rec->n_it = n_it;
                 rec->base = r.base; rec->n = r.n;
-                rec->hi = min(r.len, w.max_keys);
-                rec->lo = w.window > 0 && r.base > w.window ? r.base - w.window : 0;
-                rec->n_it = r.base < 0 || rec->hi <= rec->lo ? 0 : walk.to - walk.from;
+                rec->lo = lo; rec->hi = hi;
                 rec->whole = walk.from == 0 && walk.to == r.tiles;
                 rec->slot = (int)blockIdx.x * 2 + (walk.from == 0 ? 1 : 0);
-                if (rec->n_it > 0) {
+                tg_arrive(&told[qb]);
+                if (n_it > 0) {
                     // the G heads of a full tile's tokens: tokens behind this tile's are others' rows, whose results are
                     // not stored, tokens behind the last zeros
-                    unsigned char* dq = sQ + qb * TT_TILE;
-                    tg_expect(&q_full[qb], (uint32_t)(NH * box_rows) * 128u);
-                    tt_load_3d(dq, &map_q, 0, walk.kvh * G, rec->tok0, &q_full[qb]);
-                    if (NH > 1) tt_load_3d(dq + TT_BLOCK, &map_q, 64, walk.kvh * G, rec->tok0, &q_full[qb]);
+                    const int tiles = RT == 2 && n_rows > tile_rows ? 2 : 1;
+                    tg_expect(&q_full[qb], (uint32_t)(tiles * NH * tile_rows) * 128u);
+                    for (int t = 0; t < tiles; ++t) {
+                        unsigned char* dq = sQ + (RT == 2 ? (uint32_t)t : qb) * TT_TILE;
+                        tt_load_3d(dq, &map_q, 0, walk.kvh * G, tok0 + t * tile_tokens, &q_full[qb]);
+                        if (NH > 1) tt_load_3d(dq + TT_BLOCK, &map_q, 64, walk.kvh * G, tok0 + t * tile_tokens, &q_full[qb]);
+                    }
                 } else {
                     tg_arrive(&q_full[qb]);
                 }
             }
+            ++sent;
+            s_bits[qb * 64 + lane] = bits[0];
+            s_bits[qb * 64 + lane + 32] = bits[1];
             __syncwarp();
+            if (lane == 0) tg_arrive(&bits_told[qb]);
+            if (walk.from == 0 && walk.to < r.tiles) note = tree_note(w, walk, blockIdx.x);
         }
-    } else if (warp == 10 || warp == 12) {
-        // ------------------------------------------------------------- V (warp 10), K (warp 12)
-        const bool is_k = warp == 12;
-        int* s_pages = is_k ? s_pages_k : s_pages_v;
-        unsigned char* tiles = is_k ? sK : sV;
-        uint64_t *full = is_k ? k_full : v_full, *empty = is_k ? k_empty : v_empty;
-        const CUtensorMap* map = is_k ? &map_k : &map_v;
+    } else if (warp == 3) {
+        // ------------------------------------------------------------- K and V
         bool ok = true;
-        uint32_t g = 0;
-        for (uint32_t n = 0; ok; ++n) {
-            const uint32_t qb = n & 1u;
-            ok = __all_sync(0xffffffffu, tg_wait(&q_full[qb], (n >> 1) & 1u, err, 1));
-            if (!ok) break;
-            const TreeItem rec = ring[n & 3];
-            if (!rec.valid) break;
-            __syncwarp();
-            if (lane == 0) tg_arrive(&q_empty[qb]);
-            const int* bt = block_tables + (size_t)rec.seq * max_blocks;
-            const int pg_lo = rec.key_tile * pages_per_tile;
-            const int pg_hi = min(min(pg_lo + rec.n_it * pages_per_tile, max_blocks), pg_lo + TT_PAGES);
-            for (int i = pg_lo + lane; i < pg_hi; i += 32) s_pages[i - pg_lo] = bt[i];
-            __syncwarp();
-            for (int it = 0; it < rec.n_it; ++it, ++g) {
-                const uint32_t s = g & 1u, ph = (g >> 1) & 1u;
+        uint32_t gk = 0, gv = 0, mixed = 0, plain0 = 0, plain1 = 0;      // tiles of K, of V; V's mixed and other ones by stage
+        TreeWalk<TT_KEYS> walk;
+        walk.find(w, blockIdx.x);
+        while (ok && walk.next(w)) {
+            const TreeRequest& r = walk.r;
+            const int lo = tt_low(w, r.base), hi = min(r.len, w.max_keys);
+            const int n_it = r.base < 0 || hi <= lo ? 0 : walk.to - walk.from;
+            // a lane asks for the pages whose place in the piece is its number, 32 pages at a time, the next 32 already read
+            const int* bt = block_tables + (size_t)walk.b * max_blocks;
+            const int pg_lo = (r.t_lo + walk.from) * pages_per_tile, pg_end = min(pg_lo + n_it * pages_per_tile, max_blocks);
+            int page = pg_lo + lane < pg_end ? bt[pg_lo + lane] : -1, next_page = -1, last_page = -1;
+            int group = pg_lo;
+            auto load = [&](const CUtensorMap* map, unsigned char* tile, uint64_t* bar, int p0, int my_group, int my_page) {
                 // the tile's pages that hold a key of somebody's
-                const int p0 = (rec.key_tile + it) * pages_per_tile;
-                const int first = max(p0, rec.lo >> page_shift), last = min(p0 + pages_per_tile, ((rec.hi - 1) >> page_shift) + 1);
-                ok = __all_sync(0xffffffffu, tg_wait(&empty[s], ph ^ 1u, err, 1));
-                if (!ok) break;
-                if (lane == 0) tg_expect(&full[s], (uint32_t)max(last - first, 0) * (uint32_t)page_size * (uint32_t)(DH * 2));
+                const int first = max(p0, lo >> page_shift), last = min(p0 + pages_per_tile, ((hi - 1) >> page_shift) + 1);
+                if (lane == 0) tg_expect(bar, (uint32_t)max(last - first, 0) * (uint32_t)page_size * (uint32_t)(DH * 2));
                 __syncwarp();
-                for (int pi = first + lane; pi < last; pi += 32) {
-                    const int page = pi - pg_lo < TT_PAGES ? s_pages[pi - pg_lo] : bt[pi];
+                const int pi = my_group + lane;
+                if (pi >= first && pi < last) {
                     // a number that names no page reads zeros: rows behind the last
-                    const int row = page >= 0 && page < n_pages ? (page * w.Hkv + rec.kvh) * page_size : n_pages * w.Hkv * page_size;
-                    unsigned char* dst = tiles + s * TT_TILE + (pi - p0) * page_size * 128;
-                    tg_load_2d(dst, map, 0, row, &full[s]);
-                    if (NH > 1) tg_load_2d(dst + TT_BLOCK, map, 64, row, &full[s]);
+                    const int row = my_page >= 0 && my_page < n_pages ? (my_page * w.Hkv + walk.kvh) * page_size : n_pages * w.Hkv * page_size;
+                    unsigned char* dst = tile + (pi - p0) * page_size * 128;
+                    tg_load_2d(dst, map, 0, row, bar);
+                    if (NH > 1) tg_load_2d(dst + TT_BLOCK, map, 64, row, bar);
+                }
+            };
+            for (int it = 0; it <= n_it && ok && n_it > 0; ++it) {
+                int v_group = group, v_page = page;             // V's tile is the one before
+                if (it < n_it) {
+                    const int p0 = pg_lo + it * pages_per_tile;
+                    if (p0 >= group + 32) {
+                        last_page = page;
+                        group += 32;
+                        page = next_page;
+                        v_group = group - 32;
+                        v_page = last_page;
+                    }
+                    if (p0 == group) next_page = group + 32 + lane < pg_end ? bt[group + 32 + lane] : -1;
+                    ok = __all_sync(0xffffffffu, tg_wait(&k_empty[gk & 1u], ((gk >> 1) & 1u) ^ 1u, err, 1));
+                    if (!ok) break;
+                    load(&map_k, sK + (gk & 1u) * TT_TILE, &k_full[gk & 1u], p0, group, page);
+                    ++gk;
+                }
+                if (it > 0) {
+                    const int p0 = pg_lo + (it - 1) * pages_per_tile;
+                    const uint32_t s = gv & 1u;
+                    ok = __all_sync(0xffffffffu, tg_wait(&v_empty[s], ((gv >> 1) & 1u) ^ 1u, err, 1));
+                    if (!ok) break;
+                    uint64_t* bar = &v_full[s];
+                    if (tt_mixed(p0 << page_shift, r.base, lo, hi, w.window)) bar = &v_raw[mixed++ & 1u];
+                    else if (s) ++plain1;
+                    else ++plain0;
+                    load(&map_v, sV + s * TT_TILE, bar, p0, v_group, v_page);
+                    ++gv;
                 }
             }
             __syncwarp();
         }
-        if (!ok) tg_settle_copies(full, 2, g, err, 1);
+        if (!ok) {                                              // the copies under way
+            tg_settle_copies(k_full, 2, gk, err, 1);
+            tg_settle_copies(v_raw, 2, mixed, err, 1);
+            if (plain0) tg_wait(&v_full[0], (plain0 - 1u) & 1u, err, 1);
+            if (plain1) tg_wait(&v_full[1], (plain1 - 1u) & 1u, err, 1);
+        }
     } else if (warp == 1) {
         // ------------------------------------------------------------- S = Q K^T
         if (lane == 0) {
-            const uint32_t idesc = tg_idesc(128);
-            uint32_t g = 0;
+            const uint32_t idesc = tg_idesc(64);
+            uint32_t g = 0, steps[2] = {0, 0};                  // key tiles, steps of each stream
             bool ok = true;
             for (uint32_t n = 0; ok; ++n) {
                 const uint32_t qb = n & 1u;
-                ok = tg_wait(&q_full[qb], (n >> 1) & 1u, err, 2);
+                ok = tg_wait(&told[qb], (n >> 1) & 1u, err, 2);
                 if (!ok) break;
                 const TreeItem* rec = &ring[n & 3];
                 if (!rec->valid) break;
                 const int n_it = rec->n_it;
-                const unsigned char* qt = sQ + qb * TT_TILE;
-                const uint64_t dq0 = tg_desc(qt), dq1 = tg_desc(qt + TT_BLOCK);
-                for (int it = 0; it < n_it; ++it, ++g) {
+                const bool two = RT == 2 && rec->n_rows > tile_rows;
+                ok = tg_wait(&q_full[qb], (n >> 1) & 1u, err, 2);
+                if (!ok) break;
+                for (int it = 0; it < n_it && ok; ++it, ++g) {
                     const uint32_t s = g & 1u, ph = (g >> 1) & 1u;
-                    ok = tg_wait(&k_full[s], ph, err, 2) && tg_wait(&p_free[s], ph ^ 1u, err, 2);
-                    if (!ok) break;
-                    tg_after();
-                    const uint64_t dk0 = tg_desc(sK + s * TT_TILE), dk1 = tg_desc(sK + s * TT_TILE + TT_BLOCK);
+                    ok = tg_wait(&k_full[s], ph, err, 2);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tg_mma(tmem + 128u * s, dq0 + 2 * k, dk0 + 2 * k, idesc, k > 0 ? 1u : 0u);
-                    if (NH > 1)
+                    for (int u = 0; u < 2 * RT; ++u) {
+                        const int x = u & 1, half = RT == 2 ? u >> 1 : u;          // the stream, and the tile's half
+                        if (RT == 2 && x == 1 && !two) continue;
+                        const uint32_t step = steps[x]++, b = step & 1u;
+                        ok = ok && tg_wait(&p_free[2 * x + b], ((step >> 1) & 1u) ^ 1u, err, 2);     // the product with what lay there has run
+                        if (!ok) break;
+                        tg_after();
+                        const unsigned char* qt = sQ + (RT == 2 ? (uint32_t)x : qb) * TT_TILE;
+                        const unsigned char* kt = sK + s * TT_TILE + half * (TT_BLOCK / 2);
+                        const uint64_t dq0 = tg_desc(qt), dq1 = tg_desc(qt + TT_BLOCK), dk0 = tg_desc(kt), dk1 = tg_desc(kt + TT_BLOCK);
+                        const uint32_t d = tmem + 128u * x + 64u * b;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) tg_mma(tmem + 128u * s, dq1 + 2 * k, dk1 + 2 * k, idesc, 1u);
-                    tg_commit(&k_empty[s]);
-                    tg_commit(&s_full[s]);
+                        for (int k = 0; k < 4; ++k) tg_mma(d, dq0 + 2 * k, dk0 + 2 * k, idesc, k > 0 ? 1u : 0u);
+                        if (NH > 1)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) tg_mma(d, dq1 + 2 * k, dk1 + 2 * k, idesc, 1u);
+                        tg_commit(&s_full[2 * x + b]);
+                    }
+                    if (ok) tg_commit(&k_empty[s]);
                 }
-                tg_commit(&q_empty[qb]);
+                if (ok) tg_commit(&q_empty[qb]);
             }
             if (!ok) tg_settle_products(&settled[0], err, 2);
         }
-    } else if (warp == 11) {
+    } else if (warp == 2) {
         // ------------------------------------------------------------- O += P V
         if (lane == 0) {
             const uint32_t idesc = tg_idesc(DH, true);
-            uint32_t g = 0;
+            uint32_t g = 0, mixed = 0, plain0 = 0, plain1 = 0, steps[2] = {0, 0}, walked = 0;
             bool ok = true;
             for (uint32_t n = 0; ok; ++n) {
-                ok = tg_wait(&q_full[n & 1u], (n >> 1) & 1u, err, 2);
+                ok = tg_wait(&told[n & 1u], (n >> 1) & 1u, err, 2);
                 if (!ok) break;
                 const TreeItem* rec = &ring[n & 3];
                 if (!rec->valid) break;
-                const int n_it = rec->n_it;
+                const int n_it = rec->n_it, key_tile = rec->key_tile, r_base = rec->base, lo = rec->lo, hi = rec->hi;
+                const bool two = RT == 2 && rec->n_rows > tile_rows;
                 tg_arrive(&q_empty[n & 1u]);
-                const uint32_t ob = n & 1u, tm_o = tmem + 256u + 128u * ob;
+                if (n_it == 0) continue;
+                // the last item's O is out
+                if (walked > 0) ok = tg_wait(&o_free[(walked - 1u) & 1u], ((walked - 1u) >> 1) & 1u, err, 2);
                 for (int it = 0; it < n_it && ok; ++it, ++g) {
-                    const uint32_t s = g & 1u, ph = (g >> 1) & 1u;
-                    if (it == 0) ok = tg_wait(&o_free[ob], ((n >> 1) & 1u) ^ 1u, err, 2);
-                    ok = ok && tg_wait(&p_full[s], ph, err, 2) && tg_wait(&v_full[s], ph, err, 2);
-                    if (!ok) break;
-                    tg_after();
-                    const uint64_t dv = NH > 1 ? tg_desc_mn(sV + s * TT_TILE, TT_BLOCK) : tg_desc(sV + s * TT_TILE);
+                    const uint32_t s = g & 1u;
+                    if (tt_mixed((key_tile + it) * TT_KEYS, r_base, lo, hi, w.window)) {
+                        ok = tg_wait(&v_clean[mixed & 1u], (mixed >> 1) & 1u, err, 2);
+                        ++mixed;
+                    } else {
+                        ok = tg_wait(&v_full[s], (s ? plain1++ : plain0++) & 1u, err, 2);
+                    }
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        tg_mma_ts(tm_o, tmem + 128u * s + 8u * k, dv + (uint64_t)(128 * k), idesc, (it > 0 || k > 0) ? 1u : 0u);
-                    tg_commit(&v_empty[s]);
-                    tg_commit(&p_free[s]);
-                    tg_commit(o_done);
+                    for (int u = 0; u < 2 * RT; ++u) {
+                        const int x = u & 1, half = RT == 2 ? u >> 1 : u;
+                        if (RT == 2 && x == 1 && !two) continue;
+                        const uint32_t step = steps[x]++, b = step & 1u;
+                        ok = ok && tg_wait(&p_full[2 * x + b], (step >> 1) & 1u, err, 2);
+                        if (!ok) break;
+                        tg_after();
+                        const unsigned char* vt = sV + s * TT_TILE + half * (TT_BLOCK / 2);
+                        const uint64_t dv = NH > 1 ? tg_desc_mn(vt, TT_BLOCK) : tg_desc(vt);
+                        const uint32_t more = it > 0 || (RT == 2 && half > 0);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            tg_mma_ts(tmem + 256u + 128u * x, tmem + 128u * x + 64u * b + 8u * k, dv + (uint64_t)(128 * k), idesc, k > 0 ? 1u : more);
+                        tg_commit(&p_free[2 * x + b]);
+                    }
+                    if (ok) tg_commit(&v_empty[s]);
                 }
+                if (ok) tg_commit(&o_full[walked & 1u]);
+                ++walked;
             }
             if (!ok) tg_settle_products(&settled[1], err, 2);
         }
-    } else {
+    } else if (warp < 12) {
         // ------------------------------------------------------------- softmax
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const int quarter = warp & 3, x = (warp - 4) >> 2;
         const int row = quarter * 32 + lane;
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+        const uint32_t tm_x = tmem + 128u * x + lane_base, tm_o = tmem + 256u + 128u * x + lane_base;
+        const int row_lo = RT == 2 ? x * tile_rows : 0;         // the item's row that is row 0 here
         bool ok = true;
-        uint32_t g = 0, walked = 0;                             // key tiles, items with any
+        uint32_t step = 0, walked = 0;                          // this stream's, items with any
         for (uint32_t n = 0;; ++n) {
-            if (ok) ok = tg_wait(&q_full[n & 1u], (n >> 1) & 1u, err, 3);
-            if (tt_both(quarter, !ok)) break;                   // both warps of the rows leave together
+            ok = __all_sync(0xffffffffu, tg_wait(&bits_told[n & 1u], (n >> 1) & 1u, err, 3));
+            if (!ok) break;
             const TreeItem rec = ring[n & 3];
+            const int n_rows = min(rec.n_rows - row_lo, tile_rows);
+            const bool row_ok = row < n_rows;
+            const unsigned long long bits = rec.valid && row_ok ? s_bits[(n & 1u) * 64 + (row_lo + row) / G] : 0ull;
             if (!rec.valid) break;
             __syncwarp();
             if (lane == 0) tg_arrive(&q_empty[n & 1u]);
-            const uint32_t ob = n & 1u, tm_o = tmem + 256u + 128u * ob;
-            const bool row_ok = row < rec.n_rows;
-            const bool live = quarter * 32 < rec.n_rows;        // a row of the warp's is somebody's
-            const int token = (row_ok ? row : 0) / G, head = rec.kvh * G + (row_ok ? row : 0) % G;
-            bf16* dst = out + (size_t)(rec.tok0 + token) * out_stride + (size_t)head * DH + OC * half;
-            if (rec.n_it == 0) {
-                if (row_ok)
-#pragma unroll
-                    for (int i = 0; i < OC / 8; ++i) *(uint4*)(dst + i * 8) = make_uint4(0u, 0u, 0u, 0u);
-                __syncwarp();
-                if (lane == 0) tg_arrive(&o_free[ob]);
-                continue;
-            }
-            unsigned long long bits = 0;
-            int lo = 0x7fffffff;
-            if (row_ok) {
-                bits = seen[rec.tok0 + token] & (rec.n >= 64 ? ~0ull : (1ull << rec.n) - 1ull);
-                lo = w.window > 0 ? max(rec.base + __popcll(bits) - w.window, 0) : 0;
-            }
-            const bool warp_rows_ok = quarter * 32 + 31 < rec.n_rows;
+            if (rec.n_it == 0) continue;
+            const bool live = quarter * 32 < n_rows;            // a row of the warp's is somebody's
+            const int lo = !row_ok ? 0x7fffffff : w.window > 0 ? max(rec.base + __popcll(bits) - w.window, 0) : 0;
+            const bool warp_rows_ok = quarter * 32 + 31 < n_rows;
             // keys whole_lo .. base - 1 are seen by every row
             const int whole_lo = w.window > 0 ? rec.base + rec.n - w.window : 0;
             float m_used = -INFINITY, l = 0.f;
-            bool left = false;                                  // decided at a barrier: the same for both warps
-            for (int it = 0; it < rec.n_it; ++it, ++g) {
-                const uint32_t s = g & 1u, ph = (g >> 1) & 1u;
-                const uint32_t tm_s = tmem + 128u * s;
-                const int tile_lo = (rec.key_tile + it) * TT_KEYS, kbase = tile_lo + 64 * half;
-                float corr = 1.f;
-                bool rescale = false;
+            const int n_steps = n_rows <= 0 ? 0 : RT * rec.n_it;
+            for (int i_step = 0; i_step < n_steps; ++i_step, ++step) {
+                const uint32_t b = step & 1u;
+                ok = __all_sync(0xffffffffu, tg_wait(&s_full[2 * x + b], (step >> 1) & 1u, err, 3));
+                if (!ok) break;
                 if (live) {
-                    if (ok) ok = tg_wait(&s_full[s], ph, err, 3);
                     tg_after();
+                    const uint32_t tm_s = tm_x + 64u * b;
+                    const int kbase = rec.key_tile * TT_KEYS + (RT == 2 ? 64 * i_step : TT_KEYS * i_step + 64 * x);
                     float sc[64];
                     {
                         uint32_t r0[32], r1[32];
-                        tg_ld32(tm_s + lane_base + 64u * half, r0);
-                        tg_ld32(tm_s + lane_base + 64u * half + 32u, r1);
+                        tg_ld32(tm_s, r0);
+                        tg_ld32(tm_s + 32u, r1);
                         tg_wait_ld();
 #pragma unroll
                         for (int i = 0; i < 32; ++i) { sc[i] = __uint_as_float(r0[i]); sc[32 + i] = __uint_as_float(r1[i]); }
                     }
-                    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    if (!(warp_rows_ok && kbase + 64 <= rec.base && kbase >= whole_lo && kbase + 64 <= rec.hi)) {
+                    if (!(warp_rows_ok && kbase + 64 <= min(rec.base, rec.hi) && kbase >= whole_lo)) {
                         const unsigned long long see = (tt_range(lo - kbase, rec.base - kbase) | tt_shift(bits, rec.base - kbase)) &
                                                        tt_range(0, rec.hi - kbase);
                         const uint32_t see0 = (uint32_t)see, see1 = (uint32_t)(see >> 32);
@@ -696,142 +809,219 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
                             sc[32 + i] = see1 >> i & 1u ? sc[32 + i] : -INFINITY;
                         }
                     }
+                    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], sc[i]);
-                    float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;
-                    float* xm = s_m + (g & 1u) * 256;
-                    xm[half * 128 + row] = mx;
-                    // both halves have read their S (P is written over it)
-                    if (tt_both(quarter, !ok)) { left = true; break; }
-                    mx = fmaxf(mx, xm[(half ^ 1) * 128 + row]);
+                    for (int i = 0; i < 32; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], fmaxf(sc[2 * i], sc[2 * i + 1]));
+                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;
                     const float m_new = fmaxf(m_used, mx);
                     const bool grow = m_new > m_used + 8.f || (m_used == -INFINITY && m_new != -INFINITY);
-                    rescale = __any_sync(0xffffffffu, grow);
-                    if (rescale) {
-                        corr = m_new == -INFINITY ? 1.f : exp2f(m_used - m_new);
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float corr = m_new == -INFINITY ? 1.f : exp2f(m_used - m_new);
                         m_used = m_new;
-                    }
-                    const float ref = m_used == -INFINITY ? 0.f : m_used;
-                    float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-                    uint32_t r[32];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float a = tt_exp2(fmaf(sc[2 * i], scale_log2, -ref));
-                        const float b = tt_exp2(fmaf(sc[2 * i + 1], scale_log2, -ref));
-                        sum4[i & 3] += a + b;
-                        r[i] = tg_pack(a, b);
-                    }
-                    tg_st32(tm_s + lane_base + 32u * half, r);
-                    l = l * corr + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
-                }
-                if (tile_lo + TT_KEYS > min(rec.base, rec.hi) || (w.window > 0 && tile_lo < rec.lo + 64)) {
-                    // places that nobody sees, and values that are no numbers where only some rows see them
-                    if (ok) ok = tg_wait(&v_full[s], ph, err, 3);
-                    const int key = tile_lo + row;
-                    unsigned char* vrow = sV + s * TT_TILE + row * 128 + (NH > 1 ? half * TT_BLOCK : half * 64);
-                    const bool nobody = key >= rec.hi || key < rec.lo;
-                    if (nobody || key >= rec.base || key < whole_lo) {
-#pragma unroll
-                        for (int c = 0; c < 4 * NH; ++c) {
-                            uint4* at = (uint4*)(vrow + c * 16);
-                            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                            if (!nobody) {
-                                const uint4 u = *at;
-                                v = make_uint4(tt_finite(u.x), tt_finite(u.y), tt_finite(u.z), tt_finite(u.w));
-                                if (v.x == u.x && v.y == u.y && v.z == u.z && v.w == u.w) continue;
-                                if (key >= rec.base) atomicOr(&odd_nodes[walked & 3u], 1ull << (key - rec.base));
-                                else atomicOr(&odd_edge[walked & 3u], 1ull << (key - rec.lo));
-                            }
-                            *at = v;
-                        }
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                }
-                if (live) {
-                    if (it > 0) {
-                        if (ok) ok = tg_wait(o_done, (g - 1u) & 1u, err, 3);
-                        tg_after();
-                        if (rescale) {
-                            uint32_t r[32];
-#pragma unroll
-                            for (int c = 0; c < NH; ++c) {
-                                tg_ld32(tm_o + lane_base + (uint32_t)(OC * half) + 32u * c, r);
+                        l *= corr;
+                        if (i_step > 0) {
+                            // when the product before has run
+                            ok = __all_sync(0xffffffffu, tg_wait(&p_free[2 * x + (b ^ 1u)], ((step - 1u) >> 1) & 1u, err, 3));
+                            if (!ok) break;
+                            tg_after();
+#pragma unroll 1
+                            for (int c = 0; c < 2 * NH; ++c) {
+                                uint32_t r[32];
+                                tg_ld32(tm_o + 32u * c, r);
                                 tg_wait_ld();
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
-                                tg_st32(tm_o + lane_base + (uint32_t)(OC * half) + 32u * c, r);
+                                tg_st32(tm_o + 32u * c, r);
                             }
                         }
                     }
+                    const float ref = m_used == -INFINITY ? 0.f : m_used;
+                    const unsigned long long scale2 = tt_pair(scale_log2, scale_log2), ref2 = tt_pair(-ref, -ref);
+                    unsigned long long sum2[2] = {0ull, 0ull};
+                    uint32_t r[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        float y0, y1;
+                        tt_unpair(tt_fma2(tt_pair(sc[2 * i], sc[2 * i + 1]), scale2, ref2), y0, y1);
+                        y0 = tt_exp2(y0);
+                        y1 = tt_exp2(y1);
+                        sum2[i & 1] = tt_add2(sum2[i & 1], tt_pair(y0, y1));
+                        r[i] = tg_pack(y0, y1);
+                    }
+                    tg_st32(tm_s, r);
+                    float s0, s1;
+                    tt_unpair(tt_add2(sum2[0], sum2[1]), s0, s1);
+                    l += s0 + s1;
                     tg_wait_st();
                     tg_before();
-                } else if (it > 0) {
-                    // not a phase further than the others: an arrival for this tile may not run into the last one's
-                    if (ok) ok = tg_wait(o_done, (g - 1u) & 1u, err, 3);
                 }
-                const bool warp_ok = __all_sync(0xffffffffu, ok);
-                if (lane == 0 && warp_ok) tg_arrive(&p_full[s]);
-                if (!live && tt_both(quarter, !warp_ok)) { left = true; break; }
+                __syncwarp();
+                if (lane == 0) tg_arrive(&p_full[2 * x + b]);
             }
-            if (left) break;
-            if (ok) ok = tg_wait(o_done, (g - 1u) & 1u, err, 3);
-            tg_after();
-            s_l[half * 128 + row] = l;
-            if (tt_both(quarter, !ok)) break;
-            l += s_l[(half ^ 1) * 128 + row];
-            const unsigned long long nodes = odd_nodes[walked & 3u] & bits;
-            const unsigned long long edge = odd_edge[walked & 3u] & tt_range(lo - rec.lo, rec.base - rec.lo);
-            // for the item after the next: nobody is past that one, which wants this thread's arrivals, or before this one
-            if (tid == 64) odd_nodes[(walked + 2u) & 3u] = odd_edge[(walked + 2u) & 3u] = 0;
+            if (!ok) break;
+            // the row's sums to the warps that take the result out, when they have read those of the item before the last
+            if (walked > 1) ok = __all_sync(0xffffffffu, tg_wait(&o_free[walked & 1u], ((walked >> 1) - 1u) & 1u, err, 3));
+            if (!ok) break;
+            s_m[(walked & 1u) * 256 + x * 128 + row] = m_used;
+            s_l[(walked & 1u) * 256 + x * 128 + row] = l;
+            __syncwarp();
+            if (lane == 0) tg_arrive(&l_full[walked & 1u]);
             ++walked;
-            if (live) {
-                const float factor = rec.whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-                const size_t at = (size_t)rec.slot * w.rows_per_tile + row;
-                if (!rec.whole && row_ok && half == 0) {
-                    part_ml[at * 2] = m_used;
-                    part_ml[at * 2 + 1] = l;
+        }
+    } else {
+        // ------------------------------------------------------------- V cleaned, results out
+        const int quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+        uint4* const stage = s_stage + quarter * 128;
+        uint32_t g = 0, mixed = 0, walked = 0;                  // key tiles, mixed ones, items with any
+        bool ok = true;
+        for (uint32_t n = 0;; ++n) {
+            ok = __all_sync(0xffffffffu, tg_wait(&bits_told[n & 1u], (n >> 1) & 1u, err, 4));
+            if (!ok) break;
+            const TreeItem rec = ring[n & 3];
+            if (!rec.valid) break;
+            unsigned long long bits[RT];
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+                bits[t] = row < min(rec.n_rows - t * tile_rows, tile_rows) ? s_bits[(n & 1u) * 64 + (t * tile_rows + row) / G] : 0ull;
+            __syncwarp();
+            if (lane == 0) tg_arrive(&q_empty[n & 1u]);
+            auto result = [&](int r) { return out + (size_t)(rec.tok0 + r / G) * out_stride + (size_t)(rec.kvh * G + r % G) * DH; };
+            if (rec.n_it == 0) {
+                for (int r = row; r < rec.n_rows; r += TT_ROWS) {
+                    bf16* dst = result(r);
+                    for (int i = 0; i < DH / 8; ++i) *(uint4*)(dst + i * 8) = make_uint4(0u, 0u, 0u, 0u);
                 }
+                continue;
+            }
+            const int whole_lo = w.window > 0 ? rec.base + rec.n - w.window : 0;
+            for (int it = 0; it < rec.n_it; ++it, ++g) {
+                const int tile_lo = (rec.key_tile + it) * TT_KEYS;
+                if (!tt_mixed(tile_lo, rec.base, rec.lo, rec.hi, w.window)) continue;
+                ok = __all_sync(0xffffffffu, tg_wait(&v_raw[mixed & 1u], (mixed >> 1) & 1u, err, 4));
+                if (!ok) break;
+                const int key = tile_lo + row;
+                const bool nobody = key >= rec.hi || key < rec.lo;
+                if (nobody || key >= rec.base || key < whole_lo) {
+                    unsigned char* vrow = sV + (g & 1u) * TT_TILE + row * 128;
+                    bool odd = false;
 #pragma unroll
-                for (int c = 0; c < NH; ++c) {
-                    uint32_t r[32];
-                    tg_ld32(tm_o + lane_base + (uint32_t)(OC * half) + 32u * c, r);
-                    tg_wait_ld();
-                    if (row_ok) {
-                        float o[32];
+                    for (int c = 0; c < 8 * NH; ++c) {
+                        // eight lanes' rows lie 128 bytes apart: each begins at another sixteen of them
+                        uint4* at = (uint4*)(vrow + (c >> 3) * TT_BLOCK + ((c ^ lane) & 7) * 16);
+                        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                        if (!nobody) {
+                            const uint4 u = *at;
+                            v = make_uint4(tt_finite(u.x), tt_finite(u.y), tt_finite(u.z), tt_finite(u.w));
+                            if (v.x == u.x && v.y == u.y && v.z == u.z && v.w == u.w) continue;
+                            odd = true;
+                        }
+                        *at = v;
+                    }
+                    if (odd && key >= rec.base) atomicOr(&odd_nodes[walked & 7u], 1ull << (key - rec.base));
+                    else if (odd) atomicOr(&odd_edge[walked & 7u], 1ull << (key - rec.lo));
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) tg_arrive(&v_clean[mixed & 1u]);
+                ++mixed;
+            }
+            if (!ok) break;
+            const uint32_t wb = walked & 1u, turn = (walked >> 1) & 1u;
+            ok = __all_sync(0xffffffffu, tg_wait(&l_full[wb], turn, err, 4) && tg_wait(&o_full[wb], turn, err, 4));
+            if (!ok) break;
+            tg_after();
+#pragma unroll 1
+            for (int t = 0; t < RT; ++t) {
+                const int n_rows = min(rec.n_rows - t * tile_rows, tile_rows);
+                if (quarter * 32 >= n_rows) break;
+                const bool row_ok = row < n_rows;
+                const unsigned long long mine = RT == 2 && t == 1 ? bits[RT - 1] : bits[0];
+                const int lo = w.window > 0 ? max(rec.base + __popcll(mine) - w.window, 0) : 0;
+                const unsigned long long nodes = odd_nodes[walked & 7u] & mine;
+                const unsigned long long edge = row_ok ? odd_edge[walked & 7u] & tt_range(lo - rec.lo, rec.base - rec.lo) : 0ull;
+                const float* sm = s_m + wb * 256 + (RT == 2 ? t * 128 : 0) + row;
+                const float* sl = s_l + wb * 256 + (RT == 2 ? t * 128 : 0) + row;
+                float m = sm[0], l = sl[0], f0 = 1.f, f1 = 0.f;
+                if (RT == 1) {
+                    const float m0 = m, m1 = sm[128];
+                    m = fmaxf(m0, m1);
+                    const float ref = m == -INFINITY ? 0.f : m;
+                    f0 = exp2f(m0 - ref);
+                    f1 = exp2f(m1 - ref);
+                    l = l * f0 + sl[128] * f1;
+                }
+                if (rec.whole) {
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+                    f0 *= inv;
+                    f1 *= inv;
+                }
+                const int item_row = t * tile_rows + row;
+                if (!rec.whole && row_ok)
+                    *(float2*)(part_ml + ((size_t)rec.slot * w.rows_per_tile + item_row) * 2) = make_float2(m, l);
+                float4* po = (float4*)part_o + (size_t)rec.slot * (DH / 4) * w.rows_per_tile + item_row;
+                const uint32_t tm_o = tmem + 256u + (RT == 2 ? 128u * t : 0u) + lane_base;
+#pragma unroll 1
+                for (int c = 0; c < DH / 32; ++c) {
+                    float o[32];
+                    if (RT == 2) {
+                        uint32_t r[32];
+                        tg_ld32(tm_o + 32u * c, r);
+                        tg_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(r[i]) * factor;
-                        if (nodes | edge) {
-                            for (int k = 0; k < 128; ++k) {
-                                if (!((k < 64 ? nodes >> k : edge >> (k - 64)) & 1ull)) continue;
-                                const int key = k < 64 ? rec.base + k : rec.lo + k - 64;
-                                const int page = block_tables[(size_t)rec.seq * max_blocks + (key >> page_shift)];
-                                const bf16* v = v_cache + (((size_t)page * w.Hkv + rec.kvh) * page_size + (key & (page_size - 1))) * DH +
-                                                OC * half + 32 * c;
+                        for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(r[i]) * f0;
+                    } else {
+                        uint32_t r[32], u[32];
+                        tg_ld32(tm_o + 32u * c, r);
+                        tg_ld32(tm_o + 128u + 32u * c, u);
+                        tg_wait_ld();
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) {
-                                    const float x = __bfloat162float(v[i]);
-                                    if (!isfinite(x)) o[i] += x;
-                                }
+                        for (int i = 0; i < 32; ++i)
+                            o[i] = fmaf(__uint_as_float(r[i]), f0, __uint_as_float(u[i]) * f1);
+                    }
+                    if (nodes | edge) {
+                        for (int k = 0; k < 128; ++k) {
+                            if (!((k < 64 ? nodes >> k : edge >> (k - 64)) & 1ull)) continue;
+                            const int key = k < 64 ? rec.base + k : rec.lo + k - 64;
+                            const int page = block_tables[(size_t)rec.seq * max_blocks + (key >> page_shift)];
+                            const bf16* v = v_cache + (((size_t)page * w.Hkv + rec.kvh) * page_size + (key & (page_size - 1))) * DH + 32 * c;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const float y = __bfloat162float(v[i]);
+                                if (!isfinite(y)) o[i] += y;
                             }
                         }
-                        if (rec.whole) {
+                    }
+                    if (rec.whole) {
+                        // by way of shared memory, so that four lanes store a row's 64 bytes
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                *(uint4*)(dst + c * 32 + i * 8) = make_uint4(tg_pack(o[8 * i], o[8 * i + 1]), tg_pack(o[8 * i + 2], o[8 * i + 3]),
-                                                                             tg_pack(o[8 * i + 4], o[8 * i + 5]), tg_pack(o[8 * i + 6], o[8 * i + 7]));
-                        } else {
-                            float* po = part_o + at * DH + OC * half + 32 * c;
+                        for (int i = 0; i < 4; ++i)
+                            stage[lane * 4 + ((i ^ (lane >> 1)) & 3)] = make_uint4(tg_pack(o[8 * i], o[8 * i + 1]), tg_pack(o[8 * i + 2], o[8 * i + 3]),
+                                                                         tg_pack(o[8 * i + 4], o[8 * i + 5]), tg_pack(o[8 * i + 6], o[8 * i + 7]));
+                        __syncwarp();
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) *(float4*)(po + i * 4) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        for (int k = 0; k < 4; ++k) {
+                            const int line = 8 * k + (lane >> 2), r_out = quarter * 32 + line;
+                            if (r_out < n_rows)
+                                *(uint4*)(result(t * tile_rows + r_out) + 32 * c + (lane & 3) * 8) = stage[line * 4 + ((lane ^ (line >> 1)) & 3)];
                         }
+                        __syncwarp();
+                    } else if (row_ok) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            po[(8 * c + i) * w.rows_per_tile] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
                 }
             }
+            // these warps are at most two items apart: nobody reads the last item's but three any more, or writes them yet
+            if (quarter == 0 && lane == 0) odd_nodes[(walked + 4u) & 7u] = odd_edge[(walked + 4u) & 7u] = 0;
             tg_before();
             __syncwarp();
-            if (lane == 0) tg_arrive(&o_free[ob]);
+            if (lane == 0) tg_arrive(&o_free[wb]);
+            ++walked;
         }
     }
+    pdl_launch_late();
     tg_before();
     __syncthreads();
     if (warp == 1) {
@@ -841,63 +1031,62 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
 }
 
 // ------------------------------------------------------------------------------- the join
-// Block (j, y): the item that the boundary between workers j and j + 1 is the first to cut, eight of its rows, a warp a
-// row. Its parts are worker j's second slot and the following workers' first ones.
-#define TJ_WARPS 8
-template <typename T>
-__global__ void __launch_bounds__(TJ_WARPS * 32) tree_join_kernel(T* __restrict__ out, long long out_stride, int dh, const TreeWork w,
+// A part's sums lie four columns of all its rows after the other, as the workers' threads (a row each) store them. A warp
+// joins eight rows of the item that worker j began and others ended, as its note says: its parts are worker j's second
+// slot and the following workers' first ones. The first two, most often all, are read before the note is known.
+#define TJ_WARPS 4
+#define TJ_ROWS (8 * TJ_WARPS)
+template <typename T, int DP>                 // DP: columns, rounded up to 64, 128 or 256
+__global__ void __launch_bounds__(TJ_WARPS * 32) tree_join_kernel(T* __restrict__ out, long long out_stride, int dh, int G,
+                                                                  int rows_per_part, const TreeNote* __restrict__ notes,
                                                                   const float* __restrict__ part_o, const float* __restrict__ part_ml) {
+    constexpr int C = DP / 16;                // fours a lane
     pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = blockIdx.x;
-    const long long total = tree_total(w);
-    const int workers = total > 0 ? tree_workers(w, total) : 0;
-    if (j + 1 >= workers) return;
-    const long long u = tree_begin(total, workers, j + 1);
-    long long first;
-    const int b = tree_find(w, u, first);
-    if (b >= w.B) return;
-    const TreeRequest r = tree_request(w, b);
-    const int item_units = r.tiles + TREE_OVERHEAD;
-    const int item = (int)((u - first) / item_units);
-    const long long s = first + (long long)item * item_units;
-    if (u - s <= TREE_OVERHEAD) return;                                       // between items
-    if (tree_begin(total, workers, j) - s > TREE_OVERHEAD) return;            // cut before
-    int parts = 2;
-    while (tree_begin(total, workers, j + parts) < s + item_units) ++parts;
-    const int G = w.H / w.Hkv, kvh = item / r.row_tiles, row_tile = item % r.row_tiles;
-    const int per_tile = w.tokens_per_tile ? w.tokens_per_tile * G : w.rows_per_tile;
-    const int row0 = row_tile * per_tile, n_rows = min(r.n * G - row0, per_tile);
-    const int row = blockIdx.y * TJ_WARPS + warp, f = row0 + row;
-    if (row >= n_rows) return;
-    auto at = [&](int p) { return (size_t)(p == 0 ? 2 * j + 1 : 2 * (j + p)) * w.rows_per_tile + row; };
-    float m = -INFINITY;
-    for (int p = lane; p < parts; p += 32) m = fmaxf(m, part_ml[at(p) * 2]);
-    m = warp_max(m);
-    float sum = 0.f, o[8] = {};
-    const float ref = m == -INFINITY ? 0.f : m;
-    for (int p0 = 0; p0 < parts; p0 += 32) {
-        float weight = 0.f, l = 0.f;
-        if (p0 + lane < parts) {
-            weight = exp2f(part_ml[at(p0 + lane) * 2] - ref);
-            l = part_ml[at(p0 + lane) * 2 + 1];
-        }
-        sum += weight * l;
-        const int n = min(32, parts - p0);
-#pragma unroll 4
-        for (int p = 0; p < n; ++p) {
-            const float f_p = __shfl_sync(0xffffffffu, weight, p);
-            const float* src = part_o + at(p0 + p) * dh;
+    const int lane = threadIdx.x & 31, j = blockIdx.x;
+    const int row = blockIdx.y * TJ_ROWS + (threadIdx.x >> 5) * 8 + (lane & 7), c0 = lane >> 3, fours = (dh + 3) / 4;
+    if (row >= rows_per_part) return;
+    const TreeNote note = notes[j];
+    auto slot = [&](int p) { return (size_t)(p == 0 ? 2 * j + 1 : 2 * (j + p)); };
+    auto ml = [&](int p) { return *(const float2*)(part_ml + (slot(p) * rows_per_part + row) * 2); };
+    auto sums = [&](int p, float4 (&v)[C]) {
+        const float4* src = (const float4*)part_o + slot(p) * fours * rows_per_part + row;
 #pragma unroll
-            for (int d = 0; d < 8; ++d)
-                if (lane + 32 * d < dh) o[d] = fmaf(f_p, src[lane + 32 * d], o[d]);
+        for (int i = 0; i < C; ++i)
+            if (c0 + 4 * i < fours) v[i] = src[(size_t)(c0 + 4 * i) * rows_per_part];
+    };
+    float4 o[C], v[C];
+    float2 a = ml(0), b = ml(1);
+    sums(0, o);
+    sums(1, v);
+    if (row >= note.n_rows) return;
+    float m = a.x, l = a.y;
+    for (int p = 1; p < note.parts; ++p) {
+        const float m_new = fmaxf(m, b.x), ref = m_new == -INFINITY ? 0.f : m_new;
+        const float fa = exp2f(m - ref), fb = exp2f(b.x - ref);
+        l = l * fa + b.y * fb;
+        m = m_new;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            o[i].x = o[i].x * fa + v[i].x * fb;
+            o[i].y = o[i].y * fa + v[i].y * fb;
+            o[i].z = o[i].z * fa + v[i].z * fb;
+            o[i].w = o[i].w * fa + v[i].w * fb;
+        }
+        if (p + 1 < note.parts) {
+            b = ml(p + 1);
+            sums(p + 1, v);
         }
     }
-    sum = warp_sum(sum);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    T* dst = out + (size_t)(r.tok0 + f / G) * out_stride + (size_t)(kvh * G + f % G) * dh;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int f = note.row0 + row;
+    T* dst = out + (size_t)(note.tok0 + f / G) * out_stride + (size_t)(note.kvh * G + f % G) * dh;
 #pragma unroll
-    for (int d = 0; d < 8; ++d)
-        if (lane + 32 * d < dh) dst[lane + 32 * d] = from_f32<T>(o[d] * inv);
+    for (int i = 0; i < C; ++i) {
+        const float x[4] = {o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if ((c0 + 4 * i) * 4 + e < dh) dst[(c0 + 4 * i) * 4 + e] = from_f32<T>(x[e]);
+    }
 }
 
 // ------------------------------------------------------------------------------------ host
@@ -906,7 +1095,7 @@ TGO_API int tgo_attention_tree_tc_supports(int dh, int group, int page_size) {
     return (dh == 64 || dh == 128) && group >= 1 && group <= TT_ROWS && page_size >= 8 && page_size <= TT_KEYS &&
            (page_size & (page_size - 1)) == 0;
 }
-// The code that a wait of that kernel left when it ran out (1 copies, 2 products, 3 softmax), or 0. Synchronises.
+// The code that a wait of that kernel left when it ran out (1 copies, 2 products, 3 softmax, 4 results), or 0. Synchronises.
 TGO_API int tgo_attention_tree_error(int* value) { return (int)cudaMemcpyFromSymbol(value, tree_error_flag, sizeof(int)); }
 
 static int tree_force = 0;                    // for tests: 1 plain products, 2 tensor cores where they take the call
@@ -917,10 +1106,10 @@ TGO_API int tgo_attention_tree_work(int dtype, int dh, int group, int page_size,
     const int sms = tgo_multiprocessors();
     int rows = 2 * TP_ROWS;
     if (dtype == TGO_BF16 && tgo_attention_tree_tc_supports(dh, group, page_size)) {
-        const int mine = max_nodes * group < TT_ROWS ? max_nodes * group : TT_ROWS;
+        const int mine = max_nodes * group < 2 * TT_ROWS ? max_nodes * group : 2 * TT_ROWS;
         rows = mine > rows ? mine : rows;
     }
-    return sms * 2 * rows * (dh + 2);
+    return sms * 2 * rows * ((dh + 3) / 4 * 4 + 2) + 2 * sms * (int)(sizeof(TreeNote) / sizeof(float));
 }
 
 // The tensor map of a layer's K or V pages, kept by address, rows, page size and width.
@@ -980,39 +1169,43 @@ static const CUtensorMap* tree_map_q(const void* q, long long stride, int tokens
 
 template <typename T>
 static int tree_join_go(void* out, long long out_stride, int dh, const TreeWork& w, const float* part_o, const float* part_ml,
-                        cudaStream_t stream) {
+                        const TreeNote* notes, cudaStream_t stream) {
     if (w.workers == 1) return 0;
-    return tgo_launch_pdl(tree_join_kernel<T>, dim3(w.workers - 1, (w.rows_per_tile + TJ_WARPS - 1) / TJ_WARPS), dim3(TJ_WARPS * 32), 0,
-                          stream, (T*)out, out_stride, dh, w, part_o, part_ml);
+    return tgo_launch_pdl(dh <= 64 ? tree_join_kernel<T, 64> : dh <= 128 ? tree_join_kernel<T, 128> : tree_join_kernel<T, 256>,
+                          dim3(w.workers - 1, (w.rows_per_tile + TJ_ROWS - 1) / TJ_ROWS), dim3(TJ_WARPS * 32), 0, stream, (T*)out,
+                          out_stride, dh, w.H / w.Hkv, w.rows_per_tile, notes, part_o, part_ml);
 }
+// The workspace's parts: sums, (maximum, sum of exponentials) pairs, notes.
+static float* tree_ml(float* work, const TreeWork& w, int dh) { return work + (size_t)w.workers * 2 * w.rows_per_tile * ((dh + 3) / 4 * 4); }
+static TreeNote* tree_notes(float* work, const TreeWork& w, int dh) { return (TreeNote*)(tree_ml(work, w, dh) + (size_t)w.workers * 4 * w.rows_per_tile); }
 
-template <int DH>
+template <int DH, int RT>
 static int tree_tc_go(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, const void* v, int n_pages, void* out,
                       long long out_stride, int page_size, const int* tables, int max_blocks, const void* seen, float scale,
-                      const TreeWork& w, float* part_o, float* part_ml, cudaStream_t stream) {
-    constexpr size_t smem = 1024 + 6 * (size_t)TT_TILE + 32 * 8 + 4 * sizeof(TreeItem) + 768 * sizeof(float) + 2 * TT_PAGES * sizeof(int);
+                      const TreeWork& w, float* work, cudaStream_t stream) {
+    constexpr size_t smem = 1024 + 6 * (size_t)TT_TILE + 184 * 8 + 4 * sizeof(TreeItem) + 1024 * sizeof(float) + 512 * 16 + 16;
     static bool set[64] = {};
     int dev = 0, shift = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
     if (dev < 0 || dev >= 64) return TGO_E_BAD_ARG;
     if (!set[dev]) {
-        e = cudaFuncSetAttribute(tree_tc_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        e = cudaFuncSetAttribute(tree_tc_kernel<DH, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return (int)e;
         set[dev] = true;
     }
     while ((1 << shift) < page_size) ++shift;
-    const int rc = tgo_launch_pdl(tree_tc_kernel<DH>, dim3(w.workers), dim3(TT_THREADS), smem, stream, mk, mv, mq, (const bf16*)v, n_pages,
+    const int rc = tgo_launch_pdl(tree_tc_kernel<DH, RT>, dim3(w.workers), dim3(TT_THREADS), smem, stream, mk, mv, mq, (const bf16*)v, n_pages,
                                   (bf16*)out, out_stride, page_size, shift, tables, max_blocks, (const unsigned long long*)seen,
-                                  scale * TREE_LOG2E, w, part_o, part_ml);
+                                  scale * TREE_LOG2E, w, work, tree_ml(work, w, DH), tree_notes(work, w, DH));
     if (rc) return rc;
-    return tree_join_go<bf16>(out, out_stride, DH, w, part_o, part_ml, stream);
+    return tree_join_go<bf16>(out, out_stride, DH, w, work, tree_ml(work, w, DH), tree_notes(work, w, DH), stream);
 }
 
 template <typename T, int DP>
 static int tree_plain_go(const void* q, long long q_stride, void* out, long long out_stride, const void* k, const void* v,
                          int n_pages, int page_size, const int* tables, int max_blocks, const void* seen, int dh, float scale,
-                         const TreeWork& w, float* part_o, float* part_ml, cudaStream_t stream) {
+                         const TreeWork& w, float* work, cudaStream_t stream) {
     constexpr size_t smem = (size_t)((TP_ROWS + 2 * TP_KEYS) * (DP + 4) + TP_ROWS * (TP_KEYS + 4)) * sizeof(float);
     static bool set[64] = {};
     int dev = 0;
@@ -1026,9 +1219,9 @@ static int tree_plain_go(const void* q, long long q_stride, void* out, long long
     }
     int rc = tgo_launch_pdl(tree_plain_kernel<T, DP>, dim3(w.workers), dim3(TP_THREADS), smem, stream, (const T*)q, q_stride, (T*)out,
                             out_stride, (const T*)k, (const T*)v, n_pages, page_size, tables, max_blocks,
-                            (const unsigned long long*)seen, dh, scale, w, part_o, part_ml);
+                            (const unsigned long long*)seen, dh, scale, w, work, tree_ml(work, w, dh), tree_notes(work, w, dh));
     if (rc) return rc;
-    return tree_join_go<T>(out, out_stride, dh, w, part_o, part_ml, stream);
+    return tree_join_go<T>(out, out_stride, dh, w, work, tree_ml(work, w, dh), tree_notes(work, w, dh), stream);
 }
 
 // work: tgo_attention_tree_work() floats. scale > 0.
@@ -1042,28 +1235,31 @@ TGO_API int tgo_attention_tree(const void* q, long long q_stride, void* out, lon
         return TGO_E_BAD_ARG;
     const int sms = tgo_multiprocessors(), G = H / Hkv;
     const long long rows = (long long)n_pages * Hkv * page_size;
-    TreeWork w = {context_lens, q_start, B, T, H, Hkv, window, max_nodes, max_blocks * page_size, 0, 0, 0, 2, 0};
+    TreeWork w = {context_lens, q_start, B, T, H, Hkv, window, max_nodes, max_blocks * page_size, 0, 0, 2, 0};
+    // units are counted in 32 bits
+    if ((double)B * Hkv * ((double)max_nodes * G / TP_ROWS + 1) * ((double)max_blocks * page_size / TP_KEYS + 2 + TREE_OVERHEAD) > 2e9) return TGO_E_BAD_ARG;
     if (dtype == TGO_BF16 && tree_force != 1 && tgo_attention_tree_tc_supports(dh, G, page_size) && q_stride % 8 == 0 && out_stride % 8 == 0 &&
         (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)k_cache % 128 == 0 && (uintptr_t)v_cache % 128 == 0 &&
         rows + page_size <= 0x7fffffffll) {
-        w.tokens_per_tile = TT_ROWS / G;
-        w.rows_per_tile = max_nodes * G < TT_ROWS ? max_nodes * G : TT_ROWS;      // of a part
-        w.key_tile = TT_KEYS;
+        // trees of more rows than a tile's: two tiles an item
+        const bool two = max_nodes > TT_ROWS / G;
+        w.tokens_per_tile = (two ? 2 : 1) * (TT_ROWS / G);
+        w.rows_per_tile = (max_nodes < w.tokens_per_tile ? max_nodes : w.tokens_per_tile) * G;      // of a part
         w.workers = sms;
         const CUtensorMap* mk = tree_map_kv(k_cache, rows, page_size, dh);
         const CUtensorMap* mv = tree_map_kv(v_cache, rows, page_size, dh);
         const CUtensorMap* mq = tree_map_q(q, q_stride, T, H, G, dh);
         if (!mk || !mv || !mq) return TGO_E_BAD_ARG;
-        float* part_ml = work + (size_t)w.workers * 2 * w.rows_per_tile * dh;
-        if (dh == 128) return tree_tc_go<128>(*mk, *mv, *mq, v_cache, n_pages, out, out_stride, page_size, block_tables, max_blocks, seen, scale, w, work, part_ml, stream);
-        return tree_tc_go<64>(*mk, *mv, *mq, v_cache, n_pages, out, out_stride, page_size, block_tables, max_blocks, seen, scale, w, work, part_ml, stream);
+#define TT_GO(DH, RT) return tree_tc_go<DH, RT>(*mk, *mv, *mq, v_cache, n_pages, out, out_stride, page_size, block_tables, max_blocks, seen, scale, w, work, stream)
+        if (dh == 128) { if (two) TT_GO(128, 2); TT_GO(128, 1); }
+        if (two) TT_GO(64, 2);
+        TT_GO(64, 1);
+#undef TT_GO
     }
     w.rows_per_tile = TP_ROWS;
-    w.key_tile = TP_KEYS;
     w.workers = 2 * sms;
-    float* part_ml = work + (size_t)w.workers * 2 * TP_ROWS * dh;
 #define TP_GO(T, DP) return tree_plain_go<T, DP>(q, q_stride, out, out_stride, k_cache, v_cache, n_pages, page_size, block_tables, \
-                                                 max_blocks, seen, dh, scale, w, work, part_ml, stream)
+                                                 max_blocks, seen, dh, scale, w, work, stream)
     if (dtype == TGO_F32) { if (dh <= 64) TP_GO(float, 64); if (dh <= 128) TP_GO(float, 128); TP_GO(float, 256); }
     if (dh <= 64) TP_GO(bf16, 64);
     if (dh <= 128) TP_GO(bf16, 128);

@@ -2299,8 +2299,8 @@ def attention_tree_force_way(way: int = 0) -> None:
 
 
 def attention_tree_error() -> int:
-    """The code a wait of the trees' tcgen05 kernel left when it ran out (1 copies, 2 products, 3 softmax), or 0.
-    Synchronises with the device."""
+    """The code a wait of the trees' tcgen05 kernel left when it ran out (1 copies, 2 products, 3 softmax,
+    4 results), or 0. Synchronises with the device."""
     value = ctypes.c_int(0)
     _check(entry_points("attention_tree").tgo_attention_tree_error(ctypes.addressof(value)), "attention_tree_error")
     return int(value.value)
