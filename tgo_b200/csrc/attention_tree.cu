@@ -27,6 +27,7 @@ struct TreeWork {
     int B, T, H, Hkv, window, max_nodes, max_keys;      // max_keys: what a block table can name
     int rows_per_tile, tokens_per_tile;       // a tile holds so many rows, or (if not 0) so many whole tokens
     int min_units, workers;                   // of a piece at least, in all at most
+    int whole;                                // items are not cut: each is a unit
 };
 
 struct TreeRequest {
@@ -48,7 +49,7 @@ template <int KT> __device__ __forceinline__ TreeRequest tree_request(const Tree
     r.tiles = max((hi + KT - 1) / KT - r.t_lo, 1);
     r.row_tiles = w.tokens_per_tile ? (r.n + w.tokens_per_tile - 1) / w.tokens_per_tile
                                     : (r.n * (w.H / w.Hkv) + w.rows_per_tile - 1) / w.rows_per_tile;
-    r.units = r.row_tiles * w.Hkv * (r.tiles + TREE_OVERHEAD);
+    r.units = r.row_tiles * w.Hkv * (w.whole ? 1 : r.tiles + TREE_OVERHEAD);
     return r;
 }
 
@@ -122,8 +123,8 @@ template <int KT> struct TreeWalk {
                 if (++b >= w.B) return false;
                 r = tree_request<KT>(w, b);
             }
-            const int item_units = r.tiles + TREE_OVERHEAD;
-            const int item = (u - first) / item_units;
+            const int item_units = w.whole ? 1 : r.tiles + TREE_OVERHEAD;
+            const int item = w.whole ? u - first : (u - first) / item_units;
             const int s = first + item * item_units;
             from = max(u - s - TREE_OVERHEAD, 0);
             to = end - s >= item_units ? r.tiles : max(end - s - TREE_OVERHEAD, 0);
@@ -390,9 +391,10 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
 // maximum and a sum of exponentials of its own, and four softmax warps, a thread a row, that need nothing of each other:
 // two row tiles, or, where there is one, the first and the second half of every key tile, put together at the item's end. A
 // step of a stream is 64 keys, and its scores have two buffers: the next step's are made while this one's exponentials run.
-//   warp 0        walks, publishes a record of every item in a ring and asks TMA for its Q rows;
+//   warp 0        walks, publishes a record of every item in a ring and asks TMA for its Q rows and its K pages;
+//   warp 3        walks too, and asks for the V pages (two tiles of each are in flight; a warp starts a copy about every
+//                 80 cycles, 16 copies a tile of 16-place pages);
 //   warp 1        issues S = Q K^T, warp 2 O += P V, a thread each;
-//   warp 3        walks too, and asks TMA for the K and the V pages, two tiles of each in flight, K one ahead;
 //   warps 4-7, 8-11   softmax of stream 0 and of stream 1; P lies over its scores;
 //   warps 12-15   clean V's tiles where that is needed, and take an item's result out of tensor memory.
 // The running maximum moves only when a row has outgrown it by 2^8: then, when the product before has run, O is rescaled. P
@@ -440,6 +442,22 @@ __device__ __forceinline__ unsigned long long tt_add2(unsigned long long a, unsi
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+// 2^x of two numbers, at most 2^127 and not below 2^-126, on the FMA units: x = n + f with n whole and f in [-1/2, 1/2], a
+// cubic for 2^f (least largest relative error there, found by reweighted least squares: 7.5e-5), n added to the exponent.
+__device__ __forceinline__ void tt_exp2_fma(unsigned long long x2, float& y0, float& y1) {
+    float x0, x1, n0, n1;
+    tt_unpair(x2, x0, x1);
+    x2 = tt_pair(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+    const unsigned long long n2 = tt_add2(x2, tt_pair(12582912.f, 12582912.f));        // 1.5 * 2^23: the last bits are n's
+    const unsigned long long f2 = tt_fma2(tt_add2(n2, tt_pair(-12582912.f, -12582912.f)), tt_pair(-1.f, -1.f), x2);
+    unsigned long long p2 = tt_fma2(tt_pair(0.05517166876f, 0.05517166876f), f2, tt_pair(0.24261113279f, 0.24261113279f));
+    p2 = tt_fma2(p2, f2, tt_pair(0.69326098644f, 0.69326098644f));
+    p2 = tt_fma2(p2, f2, tt_pair(0.99992807292f, 0.99992807292f));
+    tt_unpair(n2, n0, n1);
+    tt_unpair(p2, y0, y1);
+    y0 = __int_as_float(__float_as_int(y0) + (__float_as_int(n0) << 23));
+    y1 = __int_as_float(__float_as_int(y1) + (__float_as_int(n1) << 23));
+}
 __device__ __forceinline__ void tt_load_3d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                  ::"r"(tg_smem(dst)), "l"(map), "r"(tg_smem(bar)), "r"(c0), "r"(c1), "r"(c2) : "memory");
@@ -465,6 +483,53 @@ __device__ __forceinline__ int tt_low(const TreeWork& w, int base) { return w.wi
 __device__ __forceinline__ bool tt_mixed(int key, int base, int lo, int hi, int window) {
     return key + TT_KEYS > min(base, hi) || (window > 0 && key < lo + TREE_NODES);
 }
+
+// The pages of a piece's key tiles: a lane asks for those whose place in the piece is its number, 32 at a time; the next 32
+// numbers are read meanwhile.
+struct TreePages {
+    const int* table;
+    int lo, hi, n_it;                         // keys of somebody's, key tiles
+    int first, end, per_tile, shift;          // of the piece: its first page, behind its last
+    int group, page, next_page;
+    __device__ __forceinline__ TreePages() { n_it = 0; }
+    __device__ __forceinline__ TreePages(const TreeWork& w, const TreeWalk<TT_KEYS>& k, const int* tables, int max_blocks, int page_shift) {
+        lo = tt_low(w, k.r.base);
+        hi = min(k.r.len, w.max_keys);
+        n_it = k.r.base < 0 || hi <= lo ? 0 : k.to - k.from;
+        shift = page_shift;
+        per_tile = TT_KEYS >> page_shift;
+        table = tables + (size_t)k.b * max_blocks;
+        first = group = (k.r.t_lo + k.from) * per_tile;
+        end = min(first + n_it * per_tile, max_blocks);
+        const int mine = group + (int)(threadIdx.x & 31);
+        page = mine < end ? table[mine] : -1;
+        next_page = -1;
+    }
+    __device__ __forceinline__ void turn(int it) {
+        const int p0 = first + it * per_tile;
+        if (p0 >= group + 32) {
+            group += 32;
+            page = next_page;
+        }
+        const int mine = group + 32 + (int)(threadIdx.x & 31);
+        if (p0 == group) next_page = mine < end ? table[mine] : -1;
+    }
+    // tile `it`, of which only pages that hold a key of somebody's; a page is two boxes of 64 columns, or one
+    template <int NH>
+    __device__ __forceinline__ void load(const CUtensorMap* map, unsigned char* tile, uint64_t* bar, int it, int Hkv, int kvh, int n_pages) {
+        const int p0 = first + it * per_tile, from = max(p0, lo >> shift), to = min(p0 + per_tile, ((hi - 1) >> shift) + 1);
+        const int lane = threadIdx.x & 31, mine = group + lane;
+        if (lane == 0) tg_expect(bar, (uint32_t)max(to - from, 0) << (shift + 7) << (NH - 1));
+        __syncwarp();
+        if (mine >= from && mine < to) {
+            // a number that names no page reads zeros: rows behind the last
+            const int row = (page >= 0 && page < n_pages ? page * Hkv + kvh : n_pages * Hkv) << shift;
+            unsigned char* dst = tile + ((mine - p0) << (shift + 7));
+            tg_load_2d(dst, map, 0, row, bar);
+            if (NH > 1) tg_load_2d(dst + TT_BLOCK, map, 64, row, bar);
+        }
+    }
+};
 
 // DH: head size. RT: row tiles of an item (at most).
 template <int DH, int RT>
@@ -497,7 +562,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = w.H / w.Hkv;
     const int tile_tokens = TT_ROWS / G, tile_rows = tile_tokens * G;       // of a row tile
-    const int pages_per_tile = TT_KEYS >> page_shift;
     int* const err = &tree_error_flag;
     // rows of the Q tiles that no box writes must not hold NaN by chance
     if (tile_rows != TT_ROWS) for (int i = tid; i < 2 * TT_TILE / 16; i += TT_THREADS) ((uint4*)sQ)[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -529,7 +593,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
         walk.find(w, blockIdx.x);
         TreeNote note = {0, 0, 0, 0, 0};
         if (lane == 0) notes[blockIdx.x] = note;
-        uint32_t sent = 0;                                      // items whose Q was asked for
+        uint32_t sent = 0, g = 0;                               // items whose Q was asked for, key tiles
+        bool ok = true;
         for (uint32_t n = 0;; ++n) {
             // A record lies in n % 4; a buffer of Q and of what nodes see is item n's if n is even, and the other one's
             // otherwise, or both tiles of Q are the item's.
@@ -538,6 +603,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
             const bool more = walk.next(w);
             const TreeRequest& r = walk.r;
             const int token = walk.row_tile * w.tokens_per_tile;
+            TreePages pages;
+            if (more) pages = TreePages(w, walk, block_tables, max_blocks, page_shift);
             // what its nodes see, read while the buffers come free
             unsigned long long bits[2] = {0, 0};
             if (more)
@@ -545,12 +612,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
                 for (int h = 0; h < 2; ++h)
                     if (lane + 32 * h < w.tokens_per_tile && token + lane + 32 * h < r.n)
                         bits[h] = seen[r.tok0 + token + lane + 32 * h] & (r.n >= 64 ? ~0ull : (1ull << r.n) - 1ull);
-            bool ok = __all_sync(0xffffffffu, tg_wait(&q_empty[qb], qph ^ 1u, err, 1));
+            ok = __all_sync(0xffffffffu, tg_wait(&q_empty[qb], qph ^ 1u, err, 1));
             if (RT == 2 && ok && n > 0) ok = __all_sync(0xffffffffu, tg_wait(&q_empty[qb ^ 1u], ((n - 1u) >> 1) & 1u, err, 1));
-            if (!ok) {
-                tg_settle_copies(q_full, 2, sent, err, 1);
-                break;
-            }
+            if (!ok) break;
             if (!more) {
                 if (lane == 0) {
                     rec->valid = 0;
@@ -561,8 +625,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
                 break;
             }
             if (lane == 0) {
-                const int tok0 = r.tok0 + token, lo = tt_low(w, r.base), hi = min(r.len, w.max_keys);
-                const int n_it = r.base < 0 || hi <= lo ? 0 : walk.to - walk.from;
+                const int tok0 = r.tok0 + token, n_it = pages.n_it;
                 const int n_rows = min(r.n - token, w.tokens_per_tile) * G;
                 rec->valid = 1;
                 rec->tok0 = tok0;
@@ -571,7 +634,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
                 rec->key_tile = r.t_lo + walk.from;
                 rec->n_it = n_it;
                 rec->base = r.base; rec->n = r.n;
-                rec->lo = lo; rec->hi = hi;
+                rec->lo = pages.lo; rec->hi = pages.hi;
                 rec->whole = walk.from == 0 && walk.to == r.tiles;
                 rec->slot = (int)blockIdx.x * 2 + (walk.from == 0 ? 1 : 0);
                 tg_arrive(&told[qb]);
@@ -595,77 +658,49 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
             __syncwarp();
             if (lane == 0) tg_arrive(&bits_told[qb]);
             if (walk.from == 0 && walk.to < r.tiles) note = tree_note(w, walk, blockIdx.x);
+            for (int it = 0; it < pages.n_it; ++it, ++g) {
+                const uint32_t s = g & 1u;
+                pages.turn(it);
+                ok = __all_sync(0xffffffffu, tg_wait(&k_empty[s], ((g >> 1) & 1u) ^ 1u, err, 1));
+                if (!ok) break;
+                pages.load<NH>(&map_k, sK + s * TT_TILE, &k_full[s], it, w.Hkv, walk.kvh, n_pages);
+            }
+            if (!ok) break;
+            __syncwarp();
+        }
+        if (!ok) {                                              // the copies under way
+            tg_settle_copies(q_full, 2, sent, err, 1);
+            tg_settle_copies(k_full, 2, g, err, 1);
         }
     } else if (warp == 3) {
-        // ------------------------------------------------------------- K and V
+        // ------------------------------------------------------------- V
         bool ok = true;
-        uint32_t gk = 0, gv = 0, mixed = 0, plain0 = 0, plain1 = 0;      // tiles of K, of V; V's mixed and other ones by stage
+        uint32_t g = 0, mixed = 0, plain0 = 0, plain1 = 0;      // tiles; mixed ones, the others by stage
         TreeWalk<TT_KEYS> walk;
         walk.find(w, blockIdx.x);
         while (ok && walk.next(w)) {
-            const TreeRequest& r = walk.r;
-            const int lo = tt_low(w, r.base), hi = min(r.len, w.max_keys);
-            const int n_it = r.base < 0 || hi <= lo ? 0 : walk.to - walk.from;
-            // a lane asks for the pages whose place in the piece is its number, 32 pages at a time, the next 32 already read
-            const int* bt = block_tables + (size_t)walk.b * max_blocks;
-            const int pg_lo = (r.t_lo + walk.from) * pages_per_tile, pg_end = min(pg_lo + n_it * pages_per_tile, max_blocks);
-            int page = pg_lo + lane < pg_end ? bt[pg_lo + lane] : -1, next_page = -1, last_page = -1;
-            int group = pg_lo;
-            auto load = [&](const CUtensorMap* map, unsigned char* tile, uint64_t* bar, int p0, int my_group, int my_page) {
-                // the tile's pages that hold a key of somebody's
-                const int first = max(p0, lo >> page_shift), last = min(p0 + pages_per_tile, ((hi - 1) >> page_shift) + 1);
-                if (lane == 0) tg_expect(bar, (uint32_t)max(last - first, 0) * (uint32_t)page_size * (uint32_t)(DH * 2));
-                __syncwarp();
-                const int pi = my_group + lane;
-                if (pi >= first && pi < last) {
-                    // a number that names no page reads zeros: rows behind the last
-                    const int row = my_page >= 0 && my_page < n_pages ? (my_page * w.Hkv + walk.kvh) * page_size : n_pages * w.Hkv * page_size;
-                    unsigned char* dst = tile + (pi - p0) * page_size * 128;
-                    tg_load_2d(dst, map, 0, row, bar);
-                    if (NH > 1) tg_load_2d(dst + TT_BLOCK, map, 64, row, bar);
-                }
-            };
-            for (int it = 0; it <= n_it && ok && n_it > 0; ++it) {
-                int v_group = group, v_page = page;             // V's tile is the one before
-                if (it < n_it) {
-                    const int p0 = pg_lo + it * pages_per_tile;
-                    if (p0 >= group + 32) {
-                        last_page = page;
-                        group += 32;
-                        page = next_page;
-                        v_group = group - 32;
-                        v_page = last_page;
-                    }
-                    if (p0 == group) next_page = group + 32 + lane < pg_end ? bt[group + 32 + lane] : -1;
-                    ok = __all_sync(0xffffffffu, tg_wait(&k_empty[gk & 1u], ((gk >> 1) & 1u) ^ 1u, err, 1));
-                    if (!ok) break;
-                    load(&map_k, sK + (gk & 1u) * TT_TILE, &k_full[gk & 1u], p0, group, page);
-                    ++gk;
-                }
-                if (it > 0) {
-                    const int p0 = pg_lo + (it - 1) * pages_per_tile;
-                    const uint32_t s = gv & 1u;
-                    ok = __all_sync(0xffffffffu, tg_wait(&v_empty[s], ((gv >> 1) & 1u) ^ 1u, err, 1));
-                    if (!ok) break;
-                    uint64_t* bar = &v_full[s];
-                    if (tt_mixed(p0 << page_shift, r.base, lo, hi, w.window)) bar = &v_raw[mixed++ & 1u];
-                    else if (s) ++plain1;
-                    else ++plain0;
-                    load(&map_v, sV + s * TT_TILE, bar, p0, v_group, v_page);
-                    ++gv;
-                }
+            TreePages pages(w, walk, block_tables, max_blocks, page_shift);
+            for (int it = 0; it < pages.n_it; ++it, ++g) {
+                const uint32_t s = g & 1u;
+                pages.turn(it);
+                ok = __all_sync(0xffffffffu, tg_wait(&v_empty[s], ((g >> 1) & 1u) ^ 1u, err, 1));
+                if (!ok) break;
+                uint64_t* bar = &v_full[s];
+                if (tt_mixed((walk.r.t_lo + walk.from + it) * TT_KEYS, walk.r.base, pages.lo, pages.hi, w.window)) bar = &v_raw[mixed++ & 1u];
+                else if (s) ++plain1;
+                else ++plain0;
+                pages.load<NH>(&map_v, sV + s * TT_TILE, bar, it, w.Hkv, walk.kvh, n_pages);
             }
             __syncwarp();
         }
         if (!ok) {                                              // the copies under way
-            tg_settle_copies(k_full, 2, gk, err, 1);
             tg_settle_copies(v_raw, 2, mixed, err, 1);
             if (plain0) tg_wait(&v_full[0], (plain0 - 1u) & 1u, err, 1);
             if (plain1) tg_wait(&v_full[1], (plain1 - 1u) & 1u, err, 1);
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------- S = Q K^T
-        if (lane == 0) {
+        if (tg_elect()) {
             const uint32_t idesc = tg_idesc(64);
             uint32_t g = 0, steps[2] = {0, 0};                  // key tiles, steps of each stream
             bool ok = true;
@@ -709,7 +744,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
         }
     } else if (warp == 2) {
         // ------------------------------------------------------------- O += P V
-        if (lane == 0) {
+        if (tg_elect()) {
             const uint32_t idesc = tg_idesc(DH, true);
             uint32_t g = 0, mixed = 0, plain0 = 0, plain1 = 0, steps[2] = {0, 0}, walked = 0;
             bool ok = true;
@@ -799,7 +834,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
 #pragma unroll
                         for (int i = 0; i < 32; ++i) { sc[i] = __uint_as_float(r0[i]); sc[32 + i] = __uint_as_float(r1[i]); }
                     }
-                    if (!(warp_rows_ok && kbase + 64 <= min(rec.base, rec.hi) && kbase >= whole_lo)) {
+                    const bool all = warp_rows_ok && kbase + 64 <= min(rec.base, rec.hi) && kbase >= whole_lo;
+                    if (!all) {
                         const unsigned long long see = (tt_range(lo - kbase, rec.base - kbase) | tt_shift(bits, rec.base - kbase)) &
                                                        tt_range(0, rec.hi - kbase);
                         const uint32_t see0 = (uint32_t)see, see1 = (uint32_t)(see >> 32);
@@ -839,15 +875,23 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
                     const unsigned long long scale2 = tt_pair(scale_log2, scale_log2), ref2 = tt_pair(-ref, -ref);
                     unsigned long long sum2[2] = {0ull, 0ull};
                     uint32_t r[32];
+                    auto weigh = [&](bool fma) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        float y0, y1;
-                        tt_unpair(tt_fma2(tt_pair(sc[2 * i], sc[2 * i + 1]), scale2, ref2), y0, y1);
-                        y0 = tt_exp2(y0);
-                        y1 = tt_exp2(y1);
-                        sum2[i & 1] = tt_add2(sum2[i & 1], tt_pair(y0, y1));
-                        r[i] = tg_pack(y0, y1);
-                    }
+                        for (int i = 0; i < 32; ++i) {
+                            float y0, y1;
+                            const unsigned long long y2 = tt_fma2(tt_pair(sc[2 * i], sc[2 * i + 1]), scale2, ref2);
+                            if (fma && i % 8 % 3 == 2) {        // some on the FMA units, beside the special-function unit
+                                tt_exp2_fma(y2, y0, y1);
+                            } else {
+                                tt_unpair(y2, y0, y1);
+                                y0 = tt_exp2(y0);
+                                y1 = tt_exp2(y1);
+                            }
+                            sum2[i & 1] = tt_add2(sum2[i & 1], tt_pair(y0, y1));
+                            r[i] = tg_pack(y0, y1);
+                        }
+                    };
+                    if (all) weigh(true); else weigh(false);
                     tg_st32(tm_s, r);
                     float s0, s1;
                     tt_unpair(tt_add2(sum2[0], sum2[1]), s0, s1);
@@ -1032,56 +1076,62 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
 
 // ------------------------------------------------------------------------------- the join
 // A part's sums lie four columns of all its rows after the other, as the workers' threads (a row each) store them. A warp
-// joins eight rows of the item that worker j began and others ended, as its note says: its parts are worker j's second
-// slot and the following workers' first ones. The first two, most often all, are read before the note is known.
-#define TJ_WARPS 4
-#define TJ_ROWS (8 * TJ_WARPS)
-template <typename T, int DP>                 // DP: columns, rounded up to 64, 128 or 256
+// joins 32 columns of eight rows of the item that worker j began and others ended, as its note says: its parts are worker
+// j's second slot and the following workers' first ones, taken eight at a time.
+#define TJ_WARPS 8
+#define TJ_AHEAD 8
+template <typename T>
 __global__ void __launch_bounds__(TJ_WARPS * 32) tree_join_kernel(T* __restrict__ out, long long out_stride, int dh, int G,
-                                                                  int rows_per_part, const TreeNote* __restrict__ notes,
+                                                                  int rows_per_part, int strips, const TreeNote* __restrict__ notes,
                                                                   const float* __restrict__ part_o, const float* __restrict__ part_ml) {
-    constexpr int C = DP / 16;                // fours a lane
     pdl_wait();
-    const int lane = threadIdx.x & 31, j = blockIdx.x;
-    const int row = blockIdx.y * TJ_ROWS + (threadIdx.x >> 5) * 8 + (lane & 7), c0 = lane >> 3, fours = (dh + 3) / 4;
-    if (row >= rows_per_part) return;
+    const int lane = threadIdx.x & 31, j = blockIdx.x, unit = blockIdx.y * TJ_WARPS + (threadIdx.x >> 5);
     const TreeNote note = notes[j];
-    auto slot = [&](int p) { return (size_t)(p == 0 ? 2 * j + 1 : 2 * (j + p)); };
-    auto ml = [&](int p) { return *(const float2*)(part_ml + (slot(p) * rows_per_part + row) * 2); };
-    auto sums = [&](int p, float4 (&v)[C]) {
-        const float4* src = (const float4*)part_o + slot(p) * fours * rows_per_part + row;
-#pragma unroll
-        for (int i = 0; i < C; ++i)
-            if (c0 + 4 * i < fours) v[i] = src[(size_t)(c0 + 4 * i) * rows_per_part];
-    };
-    float4 o[C], v[C];
-    float2 a = ml(0), b = ml(1);
-    sums(0, o);
-    sums(1, v);
+    const int row = unit / strips * 8 + (lane & 7), c0 = unit % strips * 8 + (lane >> 3), fours = (dh + 3) / 4;
     if (row >= note.n_rows) return;
-    float m = a.x, l = a.y;
-    for (int p = 1; p < note.parts; ++p) {
-        const float m_new = fmaxf(m, b.x), ref = m_new == -INFINITY ? 0.f : m_new;
-        const float fa = exp2f(m - ref), fb = exp2f(b.x - ref);
-        l = l * fa + b.y * fb;
-        m = m_new;
+    float m = -INFINITY, l = 0.f;
+    float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+    for (int p0 = 0; p0 < note.parts; p0 += TJ_AHEAD) {
+        float2 ml[TJ_AHEAD];
+        float4 v[TJ_AHEAD][2];
 #pragma unroll
-        for (int i = 0; i < C; ++i) {
-            o[i].x = o[i].x * fa + v[i].x * fb;
-            o[i].y = o[i].y * fa + v[i].y * fb;
-            o[i].z = o[i].z * fa + v[i].z * fb;
-            o[i].w = o[i].w * fa + v[i].w * fb;
+        for (int p = 0; p < TJ_AHEAD; ++p) {
+            ml[p] = make_float2(-INFINITY, 0.f);
+            if (p0 + p >= note.parts) continue;
+            const size_t slot = p0 + p == 0 ? 2 * j + 1 : 2 * (j + p0 + p);
+            ml[p] = *(const float2*)(part_ml + (slot * rows_per_part + row) * 2);
+            const float4* src = (const float4*)part_o + slot * fours * rows_per_part + row;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (c0 + 4 * i < fours) v[p][i] = src[(size_t)(c0 + 4 * i) * rows_per_part];
         }
-        if (p + 1 < note.parts) {
-            b = ml(p + 1);
-            sums(p + 1, v);
+        float m_new = m;
+#pragma unroll
+        for (int p = 0; p < TJ_AHEAD; ++p) m_new = fmaxf(m_new, ml[p].x);
+        const float ref = m_new == -INFINITY ? 0.f : m_new, f = exp2f(m - ref);
+        m = m_new;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) { o[i].x *= f; o[i].y *= f; o[i].z *= f; o[i].w *= f; }
+#pragma unroll
+        for (int p = 0; p < TJ_AHEAD; ++p) {
+            if (p0 + p >= note.parts) continue;
+            const float f_p = exp2f(ml[p].x - ref);
+            l = fmaf(f_p, ml[p].y, l);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                o[i].x = fmaf(f_p, v[p][i].x, o[i].x);
+                o[i].y = fmaf(f_p, v[p][i].y, o[i].y);
+                o[i].z = fmaf(f_p, v[p][i].z, o[i].z);
+                o[i].w = fmaf(f_p, v[p][i].w, o[i].w);
+            }
         }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int f = note.row0 + row;
     T* dst = out + (size_t)(note.tok0 + f / G) * out_stride + (size_t)(note.kvh * G + f % G) * dh;
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
+    for (int i = 0; i < 2; ++i) {
         const float x[4] = {o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -1170,10 +1220,10 @@ static const CUtensorMap* tree_map_q(const void* q, long long stride, int tokens
 template <typename T>
 static int tree_join_go(void* out, long long out_stride, int dh, const TreeWork& w, const float* part_o, const float* part_ml,
                         const TreeNote* notes, cudaStream_t stream) {
-    if (w.workers == 1) return 0;
-    return tgo_launch_pdl(dh <= 64 ? tree_join_kernel<T, 64> : dh <= 128 ? tree_join_kernel<T, 128> : tree_join_kernel<T, 256>,
-                          dim3(w.workers - 1, (w.rows_per_tile + TJ_ROWS - 1) / TJ_ROWS), dim3(TJ_WARPS * 32), 0, stream, (T*)out,
-                          out_stride, dh, w.H / w.Hkv, w.rows_per_tile, notes, part_o, part_ml);
+    if (w.workers == 1 || w.whole) return 0;
+    const int strips = (dh + 31) / 32, units = (w.rows_per_tile + 7) / 8 * strips;
+    return tgo_launch_pdl(tree_join_kernel<T>, dim3(w.workers - 1, (units + TJ_WARPS - 1) / TJ_WARPS), dim3(TJ_WARPS * 32), 0, stream,
+                          (T*)out, out_stride, dh, w.H / w.Hkv, w.rows_per_tile, strips, notes, part_o, part_ml);
 }
 // The workspace's parts: sums, (maximum, sum of exponentials) pairs, notes.
 static float* tree_ml(float* work, const TreeWork& w, int dh) { return work + (size_t)w.workers * 2 * w.rows_per_tile * ((dh + 3) / 4 * 4); }
@@ -1224,18 +1274,25 @@ static int tree_plain_go(const void* q, long long q_stride, void* out, long long
     return tree_join_go<T>(out, out_stride, dh, w, work, tree_ml(work, w, dh), tree_notes(work, w, dh), stream);
 }
 
+// Whether a call's items stay whole: where none has more than so many key tiles.
+static int tree_whole(const TreeWork& w, int max_context, int keys, int tiles) {
+    const int reach = w.window > 0 && max_context > w.window + w.max_nodes ? w.window + w.max_nodes + keys - 1 : max_context;
+    return (reach + keys - 1) / keys <= tiles;
+}
+
 // work: tgo_attention_tree_work() floats. scale > 0.
 TGO_API int tgo_attention_tree(const void* q, long long q_stride, void* out, long long out_stride, int dtype, int T, const void* k_cache,
                                const void* v_cache, int n_pages, int page_size, const int* block_tables, int max_blocks,
                                const int* context_lens, const int* q_start, const void* seen, int B, int H, int Hkv, int dh,
-                               int window, int max_nodes, float* work, cudaStream_t stream, float scale) {
+                               int window, int max_nodes, int max_context, float* work, cudaStream_t stream,
+                               float scale) {
     if (B <= 0 || T <= 0 || max_nodes <= 0) return 0;
     if (H <= 0 || Hkv <= 0 || H % Hkv || dh <= 0 || dh > 256 || n_pages <= 0 || page_size <= 0 || max_blocks <= 0 || window < 0 ||
         max_nodes > TREE_NODES || (long long)max_blocks * page_size > 0x7fffff00ll || (dtype != TGO_F32 && dtype != TGO_BF16) || !(scale > 0.f))
         return TGO_E_BAD_ARG;
     const int sms = tgo_multiprocessors(), G = H / Hkv;
     const long long rows = (long long)n_pages * Hkv * page_size;
-    TreeWork w = {context_lens, q_start, B, T, H, Hkv, window, max_nodes, max_blocks * page_size, 0, 0, 2, 0};
+    TreeWork w = {context_lens, q_start, B, T, H, Hkv, window, max_nodes, max_blocks * page_size, 0, 0, 2, 0, 0};
     // units are counted in 32 bits
     if ((double)B * Hkv * ((double)max_nodes * G / TP_ROWS + 1) * ((double)max_blocks * page_size / TP_KEYS + 2 + TREE_OVERHEAD) > 2e9) return TGO_E_BAD_ARG;
     if (dtype == TGO_BF16 && tree_force != 1 && tgo_attention_tree_tc_supports(dh, G, page_size) && q_stride % 8 == 0 && out_stride % 8 == 0 &&
@@ -1246,6 +1303,8 @@ TGO_API int tgo_attention_tree(const void* q, long long q_stride, void* out, lon
         w.tokens_per_tile = (two ? 2 : 1) * (TT_ROWS / G);
         w.rows_per_tile = (max_nodes < w.tokens_per_tile ? max_nodes : w.tokens_per_tile) * G;      // of a part
         w.workers = sms;
+        w.whole = tree_whole(w, max_context, TT_KEYS, two ? 8 : 12);
+        if (w.whole) w.min_units = 1;
         const CUtensorMap* mk = tree_map_kv(k_cache, rows, page_size, dh);
         const CUtensorMap* mv = tree_map_kv(v_cache, rows, page_size, dh);
         const CUtensorMap* mq = tree_map_q(q, q_stride, T, H, G, dh);
@@ -1258,6 +1317,8 @@ TGO_API int tgo_attention_tree(const void* q, long long q_stride, void* out, lon
     }
     w.rows_per_tile = TP_ROWS;
     w.workers = 2 * sms;
+    w.whole = tree_whole(w, max_context, TP_KEYS, 2);
+    if (w.whole) w.min_units = 1;
 #define TP_GO(T, DP) return tree_plain_go<T, DP>(q, q_stride, out, out_stride, k_cache, v_cache, n_pages, page_size, block_tables, \
                                                  max_blocks, seen, dh, scale, w, work, stream)
     if (dtype == TGO_F32) { if (dh <= 64) TP_GO(float, 64); if (dh <= 128) TP_GO(float, 128); TP_GO(float, 256); }

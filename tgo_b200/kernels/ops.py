@@ -2286,8 +2286,8 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, num_heads: int, num_kv_he
                        dtype=torch.float32)
     _check(lib.tgo_attention_tree(q.data_ptr(), qs, out.data_ptr(), os, code, T, k_cache.data_ptr(), v_cache.data_ptr(), shape[0],
                                   page_size, block_tables.data_ptr(), width, context_lens.data_ptr(), q_start.data_ptr(),
-                                  seen.data_ptr(), B, num_heads, num_kv_heads, head_dim, window, max_nodes, work.data_ptr(),
-                                  _stream(), float(scale)), "attention_tree",
+                                  seen.data_ptr(), B, num_heads, num_kv_heads, head_dim, window, max_nodes, max_context,
+                                  work.data_ptr(), _stream(), float(scale)), "attention_tree",
            f"(head_dim={head_dim}, heads={num_heads}/{num_kv_heads}, page_size={page_size}, window={window})")
     LAUNCHES[0] += 1
 
