@@ -442,22 +442,6 @@ __device__ __forceinline__ unsigned long long tt_add2(unsigned long long a, unsi
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// 2^x of two numbers, at most 2^127 and not below 2^-126, on the FMA units: x = n + f with n whole and f in [-1/2, 1/2], a
-// cubic for 2^f (least largest relative error there, found by reweighted least squares: 7.5e-5), n added to the exponent.
-__device__ __forceinline__ void tt_exp2_fma(unsigned long long x2, float& y0, float& y1) {
-    float x0, x1, n0, n1;
-    tt_unpair(x2, x0, x1);
-    x2 = tt_pair(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-    const unsigned long long n2 = tt_add2(x2, tt_pair(12582912.f, 12582912.f));        // 1.5 * 2^23: the last bits are n's
-    const unsigned long long f2 = tt_fma2(tt_add2(n2, tt_pair(-12582912.f, -12582912.f)), tt_pair(-1.f, -1.f), x2);
-    unsigned long long p2 = tt_fma2(tt_pair(0.05517166876f, 0.05517166876f), f2, tt_pair(0.24261113279f, 0.24261113279f));
-    p2 = tt_fma2(p2, f2, tt_pair(0.69326098644f, 0.69326098644f));
-    p2 = tt_fma2(p2, f2, tt_pair(0.99992807292f, 0.99992807292f));
-    tt_unpair(n2, n0, n1);
-    tt_unpair(p2, y0, y1);
-    y0 = __int_as_float(__float_as_int(y0) + (__float_as_int(n0) << 23));
-    y1 = __int_as_float(__float_as_int(y1) + (__float_as_int(n1) << 23));
-}
 __device__ __forceinline__ void tt_load_3d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                  ::"r"(tg_smem(dst)), "l"(map), "r"(tg_smem(bar)), "r"(c0), "r"(c1), "r"(c2) : "memory");
@@ -834,8 +818,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
 #pragma unroll
                         for (int i = 0; i < 32; ++i) { sc[i] = __uint_as_float(r0[i]); sc[32 + i] = __uint_as_float(r1[i]); }
                     }
-                    const bool all = warp_rows_ok && kbase + 64 <= min(rec.base, rec.hi) && kbase >= whole_lo;
-                    if (!all) {
+                    if (!(warp_rows_ok && kbase + 64 <= min(rec.base, rec.hi) && kbase >= whole_lo)) {
                         const unsigned long long see = (tt_range(lo - kbase, rec.base - kbase) | tt_shift(bits, rec.base - kbase)) &
                                                        tt_range(0, rec.hi - kbase);
                         const uint32_t see0 = (uint32_t)see, see1 = (uint32_t)(see >> 32);
@@ -875,23 +858,15 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
                     const unsigned long long scale2 = tt_pair(scale_log2, scale_log2), ref2 = tt_pair(-ref, -ref);
                     unsigned long long sum2[2] = {0ull, 0ull};
                     uint32_t r[32];
-                    auto weigh = [&](bool fma) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            float y0, y1;
-                            const unsigned long long y2 = tt_fma2(tt_pair(sc[2 * i], sc[2 * i + 1]), scale2, ref2);
-                            if (fma && i % 8 % 3 == 2) {        // some on the FMA units, beside the special-function unit
-                                tt_exp2_fma(y2, y0, y1);
-                            } else {
-                                tt_unpair(y2, y0, y1);
-                                y0 = tt_exp2(y0);
-                                y1 = tt_exp2(y1);
-                            }
-                            sum2[i & 1] = tt_add2(sum2[i & 1], tt_pair(y0, y1));
-                            r[i] = tg_pack(y0, y1);
-                        }
-                    };
-                    if (all) weigh(true); else weigh(false);
+                    for (int i = 0; i < 32; ++i) {
+                        float y0, y1;
+                        tt_unpair(tt_fma2(tt_pair(sc[2 * i], sc[2 * i + 1]), scale2, ref2), y0, y1);
+                        y0 = tt_exp2(y0);
+                        y1 = tt_exp2(y1);
+                        sum2[i & 1] = tt_add2(sum2[i & 1], tt_pair(y0, y1));
+                        r[i] = tg_pack(y0, y1);
+                    }
                     tg_st32(tm_s, r);
                     float s0, s1;
                     tt_unpair(tt_add2(sum2[0], sum2[1]), s0, s1);
