@@ -173,34 +173,40 @@ __device__ __forceinline__ TreeRow tree_row(const TreeWork& w, const TreeRequest
 #define TREE_LOG2E 1.44269504088896341f
 
 // ------------------------------------------------------------------------- plain products
-// float32, and bfloat16 where the tensor cores' kernel has no instance: 32 rows and 64 keys a tile on the FMA units, sixteen
-// threads a pair of rows. A thread makes 2 x 4 scores, then 2 x (width / 16) outputs; rows lie in shared memory 4 floats
-// further apart than they are wide, so that eight threads' 16-byte reads meet no bank twice.
-// A masked score becomes the weight -0, which no exponential gives: in tiles that not every row sees whole, such
-// a weight is left out of the sum, so that what lies in a masked place (an infinity, a NaN) does not reach it.
-#define TP_ROWS 32
+// float32, and bfloat16 where the tensor cores' kernel has no instance: 16, 32 or 64 rows (R = 1, 2, 4 a thread) and 64 keys a
+// tile on the FMA units, sixteen threads R rows. A thread makes R x 4 scores, then R x (width / 16) outputs; rows lie in
+// shared memory 4 floats further apart than they are wide, so that eight threads' 16-byte reads meet no bank twice. Four rows a
+// thread read 12 times 128 bytes for 64 products of a warp and are bound by these, fewer by the reads. The next K is
+// copied while this tile's weights and sums are made, the next V while its scores are.
+// A masked score becomes the weight -0, which no exponential gives: in tiles that not every row sees whole and that hold an
+// infinity or a NaN, such a weight is left out of the sum, so that what lies in a masked place does not reach it.
 #define TP_KEYS 64
 #define TP_THREADS 256
 
-__device__ __forceinline__ float4 tp_load4(const float* p) { return *(const float4*)p; }
-__device__ __forceinline__ float4 tp_load4(const bf16* p) {
-    const uint2 u = *(const uint2*)p;
-    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                       __uint_as_float(u.y & 0xffff0000u));
+// Four numbers of the cache into shared memory, or zeros; bfloat16 by way of registers.
+__device__ __forceinline__ void tp_copy4(float* dst, const float* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tg_smem(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void tp_copy4(float* dst, const bf16* src, bool there) {
+    uint2 u = make_uint2(0u, 0u);
+    if (there) u = *(const uint2*)src;
+    *(float4*)dst = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                                __uint_as_float(u.y & 0xffff0000u));
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int R>
 __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
     const T* __restrict__ q, long long q_stride, T* __restrict__ out, long long out_stride, const T* __restrict__ k_cache,
-    const T* __restrict__ v_cache, int n_pages, int page_size, const int* __restrict__ block_tables, int max_blocks,
+    const T* __restrict__ v_cache, int n_pages, int page_size, int page_shift, const int* __restrict__ block_tables, int max_blocks,
     const unsigned long long* __restrict__ seen, int dh, float scale, const TreeWork w, float* __restrict__ part_o,
     float* __restrict__ part_ml, TreeNote* __restrict__ notes) {
-    constexpr int LD = DP + 4, LS = TP_KEYS + 4, J = DP / 64;
+    constexpr int ROWS = 16 * R, LD = DP + 4, LS = TP_KEYS + 4, J = DP / 64;
+    constexpr int FOURS = DP / 4, EACH = TP_THREADS / FOURS, PASSES = TP_KEYS / EACH;
     extern __shared__ __align__(16) float tp_smem[];
-    float* sq = tp_smem;                          // [TP_ROWS][LD]
-    float* sk = sq + TP_ROWS * LD;                // [TP_KEYS][LD]
+    float* sq = tp_smem;                          // [ROWS][LD]
+    float* sk = sq + ROWS * LD;                   // [TP_KEYS][LD]
     float* sv = sk + TP_KEYS * LD;                // [TP_KEYS][LD]
-    float* ss = sv + TP_KEYS * LD;                // [TP_ROWS][LS]
+    float* ss = sv + TP_KEYS * LD;                // [ROWS][LS]
     __shared__ TreeWalk<TP_KEYS> s_walk;
     pdl_wait();
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
@@ -217,67 +223,77 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
     const int G = w.H / w.Hkv;
     const float c = scale * TREE_LOG2E;
     const bool vectors = dh % 4 == 0 && ((uintptr_t)k_cache | (uintptr_t)v_cache) % (4 * sizeof(T)) == 0;
+    const bool q_vectors = dh % 4 == 0 && q_stride % 4 == 0 && (uintptr_t)q % (4 * sizeof(T)) == 0;
+    const int my_d = tid % FOURS * 4, my_row = tid / FOURS;
     while (walk.next(w)) {
         const TreeRequest r = walk.r;
-        if (tid == 0 && walk.from == 0 && walk.to < r.tiles) notes[blockIdx.x] = tree_note(w, walk, blockIdx.x);
-        const int row0 = walk.row_tile * TP_ROWS, n_rows = min(r.n * G - row0, TP_ROWS);
+        const int row0 = walk.row_tile * ROWS, n_rows = min(r.n * G - row0, ROWS);
         const int kvh = walk.kvh;
-        __syncthreads();                          // the last piece's rows have been read
-        for (int i = tid; i < TP_ROWS * DP; i += TP_THREADS) {
-            const int row = i / DP, d = i % DP, f = row0 + row;
-            sq[row * LD + d] = row < n_rows && d < dh
-                ? to_f32(q[(size_t)(r.tok0 + f / G) * q_stride + (size_t)(kvh * G + f % G) * dh + d]) : 0.f;
-        }
-        TreeRow see[2];
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-        float o[2][J * 4];
+        const int hi = r.base < 0 ? 0 : min(r.len, w.max_keys);
+        const int* bt = block_tables + (size_t)walk.b * max_blocks;
+        // A tile of K or V, a thread the same four columns of every EACH-th row. 32-bit numbers are copied past the registers.
+        auto fill = [&](float* dst, const T* cache, int t) {
+            const int key0 = (r.t_lo + t) * TP_KEYS;
+            int page[PASSES], place[PASSES];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int row = ty * 2 + i;
+            for (int i = 0; i < PASSES; ++i) {
+                const int key = key0 + my_row + i * EACH, nth = page_shift >= 0 ? key >> page_shift : key / page_size;
+                place[i] = key - nth * page_size;
+                page[i] = key < hi ? bt[nth] : -1;
+            }
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) {
+                const bool there = page[i] >= 0 && page[i] < n_pages && my_d < dh;
+                const T* at = cache + (there ? (((size_t)page[i] * w.Hkv + kvh) * page_size + place[i]) * dh + my_d : 0);
+                float* to = dst + (my_row + i * EACH) * LD + my_d;
+                if (vectors) tp_copy4(to, at, there);
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) to[e] = there && my_d + e < dh ? to_f32(at[e]) : 0.f;
+            }
+        };
+        __syncthreads();                          // the last piece's rows have been read
+#pragma unroll
+        for (int row = my_row; row < ROWS; row += EACH) {
+            const int f = row0 + row;
+            const bool there = row < n_rows && my_d < dh;
+            const T* at = q + (there ? (size_t)(r.tok0 + f / G) * q_stride + (size_t)(kvh * G + f % G) * dh + my_d : 0);
+            float* to = sq + row * LD + my_d;
+            if (q_vectors) tp_copy4(to, at, there);
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) to[e] = there && my_d + e < dh ? to_f32(at[e]) : 0.f;
+        }
+        fill(sk, k_cache, walk.from);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        fill(sv, v_cache, walk.from);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        TreeRow see[R];
+        float m[R], l[R], o[R][J * 4];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int row = ty * R + i;
             if (row < n_rows) see[i] = tree_row(w, r, seen, (row0 + row) / G);
             else { see[i].lo = 0x7fffffff; see[i].bits = 0; }
+            m[i] = -INFINITY;
+            l[i] = 0.f;
 #pragma unroll
             for (int d = 0; d < J * 4; ++d) o[i][d] = 0.f;
         }
-        const int hi = r.base < 0 ? 0 : min(r.len, w.max_keys);
-        const int* bt = block_tables + (size_t)walk.b * max_blocks;
         for (int t = walk.from; t < walk.to; ++t) {
             const int key0 = (r.t_lo + t) * TP_KEYS;
-            __syncthreads();                      // the last tile's K and V have been read
-            for (int i = tid; i < TP_KEYS * (DP / 4); i += TP_THREADS) {
-                const int row = i / (DP / 4), d = i % (DP / 4) * 4, key = key0 + row;
-                float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-                const int page = key < hi ? bt[key / page_size] : -1;
-                if (page >= 0 && page < n_pages && d < dh) {
-                    const size_t at = (((size_t)page * w.Hkv + kvh) * page_size + key % page_size) * dh + d;
-                    if (vectors) {
-                        a = tp_load4(k_cache + at);
-                        b = tp_load4(v_cache + at);
-                    } else {
-                        float ka[4], va[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            ka[e] = d + e < dh ? to_f32(k_cache[at + e]) : 0.f;
-                            va[e] = d + e < dh ? to_f32(v_cache[at + e]) : 0.f;
-                        }
-                        a = make_float4(ka[0], ka[1], ka[2], ka[3]);
-                        b = make_float4(va[0], va[1], va[2], va[3]);
-                    }
-                }
-                *(float4*)(sk + row * LD + d) = a;
-                *(float4*)(sv + row * LD + d) = b;
-            }
+            asm volatile("cp.async.wait_group 1;" ::: "memory");         // K is there
             __syncthreads();
-            float x[2][4] = {};
-#pragma unroll 8
+            float x[R][4] = {};
+#pragma unroll 4
             for (int d = 0; d < DP; d += 4) {
-                float4 a[2], b[4];
+                float4 a[R], b[4];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) a[i] = *(const float4*)(sq + (ty * 2 + i) * LD + d);
+                for (int i = 0; i < R; ++i) a[i] = *(const float4*)(sq + (ty * R + i) * LD + d);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) b[j] = *(const float4*)(sk + (tx + 16 * j) * LD + d);
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < R; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         x[i][j] = fmaf(a[i].x, b[j].x, x[i][j]);
@@ -286,16 +302,24 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
                         x[i][j] = fmaf(a[i].w, b[j].w, x[i][j]);
                     }
             }
-            bool ok[2][4];
+            __syncthreads();                      // K has been read
+            if (t + 1 < walk.to) fill(sk, k_cache, t + 1);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            // all of the tile's keys are seen by every row: cached, behind every window's beginning
+            const bool whole = key0 + TP_KEYS <= min(hi, r.base) && (w.window <= 0 || key0 >= r.base + r.n - w.window);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < R; ++i) {
+                uint32_t ok = ty * R + i < n_rows ? 15u : 0u;
+                if (!whole)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int key = key0 + tx + 16 * j;
+                        if (!(key < hi && see[i].sees(key, r.base, r.n))) ok &= ~(1u << j);
+                    }
                 float mx = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int key = key0 + tx + 16 * j;
-                    ok[i][j] = key < hi && see[i].sees(key, r.base, r.n);
-                    if (ok[i][j]) mx = fmaxf(mx, x[i][j]);
-                }
+                for (int j = 0; j < 4; ++j)
+                    if (ok >> j & 1u) mx = fmaxf(mx, x[i][j]);
 #pragma unroll
                 for (int s = 8; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
                 const float m_new = fmaxf(m[i], mx * c);
@@ -305,39 +329,51 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
                 float sum = 0.f;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float p = ok[i][j] ? exp2f(fmaf(x[i][j], c, -ref)) : -0.f;
+                    const float p = ok >> j & 1u ? exp2f(fmaf(x[i][j], c, -ref)) : -0.f;
                     sum += p;
-                    ss[(ty * 2 + i) * LS + tx + 16 * j] = p;
+                    ss[(ty * R + i) * LS + tx + 16 * j] = p;
                 }
                 l[i] = l[i] * corr + sum;
 #pragma unroll
                 for (int d = 0; d < J * 4; ++d) o[i][d] *= corr;
             }
-            __syncwarp();                         // a pair of rows belongs to half a warp
-            // all of the tile's keys are seen by every row: cached, behind every window's beginning
-            const bool whole = key0 + TP_KEYS <= min(hi, r.base) && (w.window <= 0 || key0 >= r.base + r.n - w.window);
-            if (whole) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");         // V is there
+            bool odd = false;                     // values that are no finite numbers where not every row sees them
+            if (!whole)
+#pragma unroll
+                for (int i = 0; i < PASSES; ++i) {
+                    const float4 v = *(const float4*)(sv + (my_row + i * EACH) * LD + my_d);
+                    odd |= !(isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w));
+                }
+            if (!__syncthreads_or(odd)) {
 #pragma unroll 2
                 for (int k = 0; k < TP_KEYS; k += 4) {
-                    const float4 p0 = *(const float4*)(ss + (ty * 2) * LS + k), p1 = *(const float4*)(ss + (ty * 2 + 1) * LS + k);
-                    const float pa[4] = {p0.x, p0.y, p0.z, p0.w}, pb[4] = {p1.x, p1.y, p1.z, p1.w};
+                    float p[R][4];
+#pragma unroll
+                    for (int i = 0; i < R; ++i) {
+                        const float4 u = *(const float4*)(ss + (ty * R + i) * LS + k);
+                        p[i][0] = u.x; p[i][1] = u.y; p[i][2] = u.z; p[i][3] = u.w;
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
                         for (int j = 0; j < J; ++j) {
                             const float4 v = *(const float4*)(sv + (k + e) * LD + tx * 4 + 64 * j);
-                            o[0][4 * j] = fmaf(pa[e], v.x, o[0][4 * j]); o[0][4 * j + 1] = fmaf(pa[e], v.y, o[0][4 * j + 1]);
-                            o[0][4 * j + 2] = fmaf(pa[e], v.z, o[0][4 * j + 2]); o[0][4 * j + 3] = fmaf(pa[e], v.w, o[0][4 * j + 3]);
-                            o[1][4 * j] = fmaf(pb[e], v.x, o[1][4 * j]); o[1][4 * j + 1] = fmaf(pb[e], v.y, o[1][4 * j + 1]);
-                            o[1][4 * j + 2] = fmaf(pb[e], v.z, o[1][4 * j + 2]); o[1][4 * j + 3] = fmaf(pb[e], v.w, o[1][4 * j + 3]);
+#pragma unroll
+                            for (int i = 0; i < R; ++i) {
+                                o[i][4 * j] = fmaf(p[i][e], v.x, o[i][4 * j]);
+                                o[i][4 * j + 1] = fmaf(p[i][e], v.y, o[i][4 * j + 1]);
+                                o[i][4 * j + 2] = fmaf(p[i][e], v.z, o[i][4 * j + 2]);
+                                o[i][4 * j + 3] = fmaf(p[i][e], v.w, o[i][4 * j + 3]);
+                            }
                         }
                 }
             } else {
-#pragma unroll 2
+#pragma unroll 1
                 for (int k = 0; k < TP_KEYS; ++k) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float p = ss[(ty * 2 + i) * LS + k];
+                    for (int i = 0; i < R; ++i) {
+                        const float p = ss[(ty * R + i) * LS + k];
                         if (__float_as_uint(p) == 0x80000000u) continue;
 #pragma unroll
                         for (int j = 0; j < J; ++j) {
@@ -348,15 +384,20 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
                     }
                 }
             }
+            __syncthreads();                      // V has been read
+            if (t + 1 < walk.to) fill(sv, v_cache, t + 1);
+            asm volatile("cp.async.commit_group;" ::: "memory");
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
         const bool whole_item = walk.from == 0 && walk.to == r.tiles;
+        if (tid == 0 && walk.from == 0 && !whole_item) notes[blockIdx.x] = tree_note(w, walk, blockIdx.x);
         const size_t slot = (size_t)blockIdx.x * 2 + (walk.from == 0 ? 1 : 0);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < R; ++i) {
             float sum = l[i];
 #pragma unroll
             for (int s = 8; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-            const int row = ty * 2 + i, f = row0 + row;
+            const int row = ty * R + i, f = row0 + row;
             if (row >= n_rows) continue;
             if (whole_item) {
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -368,17 +409,15 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
                 }
             } else {
                 const int fours = (dh + 3) / 4;
-                float4* dst = (float4*)part_o + slot * fours * TP_ROWS + row;
+                float4* dst = (float4*)part_o + slot * fours * w.rows_per_tile + row;
 #pragma unroll
                 for (int j = 0; j < J; ++j)
-                    if (tx + 16 * j < fours) dst[(tx + 16 * j) * TP_ROWS] = make_float4(o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]);
-                if (tx == 0) {
-                    part_ml[(slot * TP_ROWS + row) * 2] = m[i];
-                    part_ml[(slot * TP_ROWS + row) * 2 + 1] = sum;
-                }
+                    if (tx + 16 * j < fours) dst[(tx + 16 * j) * w.rows_per_tile] = make_float4(o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]);
+                if (tx == 0) *(float2*)(part_ml + (slot * w.rows_per_tile + row) * 2) = make_float2(m[i], sum);
             }
         }
     }
+    pdl_launch_late();
 }
 
 // -------------------------------------------------------------------------- tensor cores
@@ -1129,7 +1168,7 @@ TGO_API int tgo_attention_tree_force(int way) { tree_force = way; return 0; }
 // Floats of workspace that a call wants.
 TGO_API int tgo_attention_tree_work(int dtype, int dh, int group, int page_size, int max_nodes) {
     const int sms = tgo_multiprocessors();
-    int rows = 2 * TP_ROWS;
+    int rows = 2 * 64;                        // two blocks an SM with 64 rows a tile
     if (dtype == TGO_BF16 && tgo_attention_tree_tc_supports(dh, group, page_size)) {
         const int mine = max_nodes * group < 2 * TT_ROWS ? max_nodes * group : 2 * TT_ROWS;
         rows = mine > rows ? mine : rows;
@@ -1227,32 +1266,43 @@ static int tree_tc_go(const CUtensorMap& mk, const CUtensorMap& mv, const CUtens
     return tree_join_go<bf16>(out, out_stride, DH, w, work, tree_ml(work, w, DH), tree_notes(work, w, DH), stream);
 }
 
-template <typename T, int DP>
-static int tree_plain_go(const void* q, long long q_stride, void* out, long long out_stride, const void* k, const void* v,
-                         int n_pages, int page_size, const int* tables, int max_blocks, const void* seen, int dh, float scale,
-                         const TreeWork& w, float* work, cudaStream_t stream) {
-    constexpr size_t smem = (size_t)((TP_ROWS + 2 * TP_KEYS) * (DP + 4) + TP_ROWS * (TP_KEYS + 4)) * sizeof(float);
-    static bool set[64] = {};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return (int)e;
-    if (dev < 0 || dev >= 64) return TGO_E_BAD_ARG;
-    if (!set[dev]) {
-        e = cudaFuncSetAttribute(tree_plain_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return (int)e;
-        set[dev] = true;
-    }
-    int rc = tgo_launch_pdl(tree_plain_kernel<T, DP>, dim3(w.workers), dim3(TP_THREADS), smem, stream, (const T*)q, q_stride, (T*)out,
-                            out_stride, (const T*)k, (const T*)v, n_pages, page_size, tables, max_blocks,
-                            (const unsigned long long*)seen, dh, scale, w, work, tree_ml(work, w, dh), tree_notes(work, w, dh));
-    if (rc) return rc;
-    return tree_join_go<T>(out, out_stride, dh, w, work, tree_ml(work, w, dh), tree_notes(work, w, dh), stream);
-}
-
 // Whether a call's items stay whole: where none has more than so many key tiles.
 static int tree_whole(const TreeWork& w, int max_context, int keys, int tiles) {
     const int reach = w.window > 0 && max_context > w.window + w.max_nodes ? w.window + w.max_nodes + keys - 1 : max_context;
     return (reach + keys - 1) / keys <= tiles;
+}
+
+template <typename T, int DP, int R>
+static int tree_plain_go(const void* q, long long q_stride, void* out, long long out_stride, const void* k, const void* v,
+                         int n_pages, int page_size, const int* tables, int max_blocks, const void* seen, int dh, float scale,
+                         TreeWork w, int max_context, float* work, cudaStream_t stream) {
+    constexpr int ROWS = 16 * R;
+    constexpr size_t smem = (size_t)((ROWS + 2 * TP_KEYS) * (DP + 4) + ROWS * (TP_KEYS + 4)) * sizeof(float);
+    // per device: how many of its blocks an SM holds
+    static int held[64] = {};
+    int dev = 0, shift = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < 0 || dev >= 64) return TGO_E_BAD_ARG;
+    if (!held[dev]) {
+        e = cudaFuncSetAttribute(tree_plain_kernel<T, DP, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return (int)e;
+        int n = 0;
+        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, tree_plain_kernel<T, DP, R>, TP_THREADS, smem);
+        if (e != cudaSuccess) return (int)e;
+        held[dev] = n < 1 ? 1 : n > 2 ? 2 : n;
+    }
+    while ((1 << shift) < page_size) ++shift;
+    if ((1 << shift) != page_size) shift = -1;
+    w.rows_per_tile = ROWS;
+    w.workers = held[dev] * tgo_multiprocessors();
+    w.whole = tree_whole(w, max_context, TP_KEYS, 2);
+    if (w.whole) w.min_units = 1;
+    int rc = tgo_launch_pdl(tree_plain_kernel<T, DP, R>, dim3(w.workers), dim3(TP_THREADS), smem, stream, (const T*)q, q_stride, (T*)out,
+                            out_stride, (const T*)k, (const T*)v, n_pages, page_size, shift, tables, max_blocks,
+                            (const unsigned long long*)seen, dh, scale, w, work, tree_ml(work, w, dh), tree_notes(work, w, dh));
+    if (rc) return rc;
+    return tree_join_go<T>(out, out_stride, dh, w, work, tree_ml(work, w, dh), tree_notes(work, w, dh), stream);
 }
 
 // work: tgo_attention_tree_work() floats. scale > 0.
@@ -1269,7 +1319,7 @@ TGO_API int tgo_attention_tree(const void* q, long long q_stride, void* out, lon
     const long long rows = (long long)n_pages * Hkv * page_size;
     TreeWork w = {context_lens, q_start, B, T, H, Hkv, window, max_nodes, max_blocks * page_size, 0, 0, 2, 0, 0};
     // units are counted in 32 bits
-    if ((double)B * Hkv * ((double)max_nodes * G / TP_ROWS + 1) * ((double)max_blocks * page_size / TP_KEYS + 2 + TREE_OVERHEAD) > 2e9) return TGO_E_BAD_ARG;
+    if ((double)B * Hkv * ((double)max_nodes * G / 16 + 1) * ((double)max_blocks * page_size / TP_KEYS + 2 + TREE_OVERHEAD) > 2e9) return TGO_E_BAD_ARG;
     if (dtype == TGO_BF16 && tree_force != 1 && tgo_attention_tree_tc_supports(dh, G, page_size) && q_stride % 8 == 0 && out_stride % 8 == 0 &&
         (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)k_cache % 128 == 0 && (uintptr_t)v_cache % 128 == 0 &&
         rows + page_size <= 0x7fffffffll) {
@@ -1290,15 +1340,18 @@ TGO_API int tgo_attention_tree(const void* q, long long q_stride, void* out, lon
         TT_GO(64, 1);
 #undef TT_GO
     }
-    w.rows_per_tile = TP_ROWS;
-    w.workers = 2 * sms;
-    w.whole = tree_whole(w, max_context, TP_KEYS, 2);
-    if (w.whole) w.min_units = 1;
-#define TP_GO(T, DP) return tree_plain_go<T, DP>(q, q_stride, out, out_stride, k_cache, v_cache, n_pages, page_size, block_tables, \
-                                                 max_blocks, seen, dh, scale, w, work, stream)
-    if (dtype == TGO_F32) { if (dh <= 64) TP_GO(float, 64); if (dh <= 128) TP_GO(float, 128); TP_GO(float, 256); }
-    if (dh <= 64) TP_GO(bf16, 64);
-    if (dh <= 128) TP_GO(bf16, 128);
-    TP_GO(bf16, 256);
+#define TP_GO(T, DP, R) return tree_plain_go<T, DP, R>(q, q_stride, out, out_stride, k_cache, v_cache, n_pages, page_size, block_tables, \
+                                                       max_blocks, seen, dh, scale, w, max_context, work, stream)
+    if (dtype == TGO_F32) {
+        // as many rows a thread as the widest tree fills
+        const int rows = max_nodes * G;
+        if (dh <= 64) { if (rows <= 16) TP_GO(float, 64, 1); if (rows <= 32) TP_GO(float, 64, 2); TP_GO(float, 64, 4); }
+        if (dh <= 128) { if (rows <= 16) TP_GO(float, 128, 1); if (rows <= 32) TP_GO(float, 128, 2); TP_GO(float, 128, 4); }
+        if (rows <= 16) TP_GO(float, 256, 1);
+        TP_GO(float, 256, 2);
+    }
+    if (dh <= 64) TP_GO(bf16, 64, 2);
+    if (dh <= 128) TP_GO(bf16, 128, 2);
+    TP_GO(bf16, 256, 2);
 #undef TP_GO
 }

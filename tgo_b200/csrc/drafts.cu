@@ -1,7 +1,7 @@
 // What a step of drafted tokens needs beside its attention: rows of logits constrained (biases, penalties for repeated
 // tokens, masks of allowed ones), the path through a tree of drafts that the chosen tokens confirm, and the accepted
 // nodes' rows of the cache moved together.
-#include "common.cuh"
+#include "tcgen.cuh"
 
 #define DR_NODES 64               // most drafted tokens of a request: a path is a 64-bit number
 
@@ -13,13 +13,16 @@
 //   not allowed: x = -inf
 // the order and the arithmetic of the sampler's single rows (adjust_kernel of sampling.cu), so that both give the same bits.
 //
-// A block takes a slice of 8192 columns of a row. It asks for the slice's logits first, counts the history's tokens that fall
-// into its slice in shared memory while they come (integers: the order of the additions changes nothing), and then edits
-// and stores. A biased token is left to a second look, when everything else of the slice is done. In place, a
-// group of four columns without a counted or a forbidden token is neither read nor written.
+// In place, or for rows that lie on no 16-byte boundaries, a block takes a slice of 8192 columns of a row: it counts the history's
+// tokens that fall into its slice in shared memory (integers: the order of the additions changes nothing), and then edits and
+// stores. A biased token is left to a second look, when everything else of the slice is done. In place, a group of
+// four columns (VECTORS; or a column) without a counted or a forbidden token is neither read nor written.
 #define LC_THREADS 256
 #define LC_VPT 8                  // groups of four columns a thread
 #define LC_COLUMNS (LC_THREADS * LC_VPT * 4)
+#ifndef LC_AHEAD
+#define LC_AHEAD 8                // tokens of the history that a thread reads at once
+#endif
 #define LC_BIASED 0x80000000u
 
 struct Constrain {
@@ -57,54 +60,51 @@ __global__ void __launch_bounds__(LC_THREADS) constrain_kernel(const Constrain a
     float* dst = a.out + (size_t)r * a.out_stride + col0;
     const bool in_place = a.logits == a.out;
     const int q = a.owner ? a.owner[r] : r;
-    const bool owned = q >= 0 && q < a.requests;
-    float4 x[LC_VPT];
-    if (VECTORS && !in_place) {
-#pragma unroll
-        for (int i = 0; i < LC_VPT; ++i) {
-            const int c = (i * LC_THREADS + tid) * 4;
-            if (c + 3 < n_cols) x[i] = __ldcs((const float4*)(src + c));
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < LC_VPT; ++i) ((uint4*)count)[i * LC_THREADS + tid] = make_uint4(0u, 0u, 0u, 0u);
     const uint32_t* words = nullptr;
     if (a.allowed) {
         const int w = a.allowed_rows ? a.allowed_rows[r] : r;
         if (w >= 0 && w < a.allowed_rows_n) words = a.allowed + (size_t)w * a.allowed_stride + (col0 >> 5);
     }
+    const bool owned = q >= 0 && q < a.requests;
     float rep = 1.f, presence = 0.f, frequency = 0.f;
-    int b_lo = 0, b_hi = 0;
-    bool counts = false;
+    int b_lo = 0, b_hi = 0, h_lo = 0, h_hi = 0, room = 0, d_lo = 0, d_n = 0;
+    unsigned long long path = 0;
     if (owned && a.bias_start) { b_lo = a.bias_start[q]; b_hi = a.bias_start[q + 1]; }
     if (owned && a.penalties) {
         rep = a.penalties[3 * q]; presence = a.penalties[3 * q + 1]; frequency = a.penalties[3 * q + 2];
-        counts = (rep != 0.f && rep != 1.f) || presence != 0.f || frequency != 0.f;
-    }
-    __syncthreads();
-    if (counts) {
-        int room = a.windows ? a.windows[q] : 0;
-        if (room <= 0) room = 0x7fffffff;
+        if (a.history_start) { h_lo = a.history_start[q]; h_hi = a.history_start[q + 1]; }
+        if (a.windows) room = a.windows[q];
         if (a.seen) {
-            unsigned long long path = a.seen[r];
-            const int t0 = a.draft_start[q], n = min(a.draft_start[q + 1] - t0, DR_NODES);
-            path &= n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull;
-            const int length = __popcll(path);
-            if (tid < DR_NODES && path >> tid & 1ull && __popcll(path >> tid) <= room) {
-                const int c = a.draft_tokens[t0 + tid] - col0;
-                if (c >= 0 && c < n_cols) atomicAdd(&count[c], 1u);
-            }
-            room -= min(room, length);
+            path = a.seen[r];
+            d_lo = a.draft_start[q];
+            d_n = min(a.draft_start[q + 1] - d_lo, DR_NODES);
         }
-        if (a.history_start) {
-            int lo = a.history_start[q];
-            const int hi = a.history_start[q + 1];
-            if (hi - lo > room) lo = hi - room;
-#pragma unroll 4
-            for (int i = lo + tid; i < hi; i += LC_THREADS) {
-                const int c = a.history[i] - col0;
-                if (c >= 0 && c < n_cols) atomicAdd(&count[c], 1u);
-            }
+    }
+    uint32_t allowed[LC_VPT];                 // of the vectors' columns
+#pragma unroll
+    for (int i = 0; i < LC_VPT; ++i) {
+        const int c = (i * LC_THREADS + tid) * 4;
+        allowed[i] = VECTORS && words && c < n_cols ? words[c >> 5] : 0xffffffffu;
+    }
+#pragma unroll
+    for (int i = 0; i < LC_VPT; ++i) ((uint4*)count)[i * LC_THREADS + tid] = make_uint4(0u, 0u, 0u, 0u);
+    __syncthreads();
+    if ((rep != 0.f && rep != 1.f) || presence != 0.f || frequency != 0.f) {
+        if (room <= 0) room = 0x7fffffff;
+        path &= d_n >= 64 ? ~0ull : d_n <= 0 ? 0ull : (1ull << d_n) - 1ull;
+        if (tid < DR_NODES && path >> tid & 1ull && __popcll(path >> tid) <= room) {
+            const int c = a.draft_tokens[d_lo + tid] - col0;
+            if (c >= 0 && c < n_cols) atomicAdd(&count[c], 1u);
+        }
+        room -= min(room, __popcll(path));
+        if (h_hi - h_lo > room) h_lo = h_hi - room;
+        for (int i = h_lo + tid; i < h_hi; i += LC_AHEAD * LC_THREADS) {
+            int c[LC_AHEAD];
+#pragma unroll
+            for (int k = 0; k < LC_AHEAD; ++k) c[k] = i + k * LC_THREADS < h_hi ? a.history[i + k * LC_THREADS] - col0 : -1;
+#pragma unroll
+            for (int k = 0; k < LC_AHEAD; ++k)
+                if (c[k] >= 0 && c[k] < n_cols) atomicAdd(&count[c[k]], 1u);
         }
     }
     for (int i = b_lo + tid; i < b_hi; i += LC_THREADS) {
@@ -112,9 +112,9 @@ __global__ void __launch_bounds__(LC_THREADS) constrain_kernel(const Constrain a
         if (c >= 0 && c < n_cols) atomicOr(&count[c], LC_BIASED);
     }
     __syncthreads();
-    auto value = [&](float v, uint32_t n, uint32_t allowed) {
+    auto value = [&](float v, uint32_t n, uint32_t ok) {
         if (n & LC_BIASED) return v;
-        if (!(allowed & 1u)) return -INFINITY;
+        if (!(ok & 1u)) return -INFINITY;
         return lc_edit(v, n, rep, presence, frequency);
     };
     if (VECTORS) {
@@ -123,14 +123,13 @@ __global__ void __launch_bounds__(LC_THREADS) constrain_kernel(const Constrain a
             const int g = i * LC_THREADS + tid, c = g * 4;
             if (c >= n_cols) break;
             const uint4 n = ((const uint4*)count)[g];
-            const uint32_t bits = words ? words[c >> 5] >> (c & 31) : 0xfu;
-            if (in_place && (bits & 0xfu) == 0xfu && !((n.x | n.y | n.z | n.w) & ~LC_BIASED)) continue;
+            const uint32_t bits = allowed[i] >> (c & 31);
+            if ((bits & 0xfu) == 0xfu && !((n.x | n.y | n.z | n.w) & ~LC_BIASED)) continue;
             if (c + 3 < n_cols) {
-                float4 v;
-                if (in_place) v = *(const float4*)(src + c); else v = x[i];
+                float4 v = *(const float4*)(src + c);
                 v.x = value(v.x, n.x, bits); v.y = value(v.y, n.y, bits >> 1);
                 v.z = value(v.z, n.z, bits >> 2); v.w = value(v.w, n.w, bits >> 3);
-                __stcs((float4*)(dst + c), v);
+                *(float4*)(dst + c) = v;
             } else {
                 for (int k = 0; c + k < n_cols; ++k) dst[c + k] = value(src[c + k], count[c + k], bits >> k);
             }
@@ -153,6 +152,194 @@ __global__ void __launch_bounds__(LC_THREADS) constrain_kernel(const Constrain a
     }
 }
 
+// Out of place, rows on 16-byte boundaries: persistent blocks take slices one after the other, each a run of them, mostly of one row,
+// whose numbers then stay in registers. A slice comes into shared memory by one bulk copy, asked for while the slice
+// before it is edited, is edited there where there is something to edit, and leaves by another: the copies wait for nothing
+// but each other.
+#ifndef LS_THREADS
+#define LS_THREADS 512
+#endif
+#ifndef LS_BLOCKS
+#define LS_BLOCKS 2                  // of an SM
+#endif
+#ifndef LS_RING
+#define LS_RING 3
+#endif
+#ifndef LS_COLUMNS
+#define LS_COLUMNS 6144              // a slice: a whole number of four columns a thread
+#endif
+#ifndef LS_AHEAD
+#define LS_AHEAD 8                   // tokens of the history that a thread keeps for all the slices of a row
+#endif
+
+__device__ int drafts_error_flag = 0;
+
+__device__ __forceinline__ void ls_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(tg_smem(dst)), "l"(src), "r"(bytes), "r"(tg_smem(bar)) : "memory");
+}
+__device__ __forceinline__ void ls_store(void* dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(tg_smem(src)), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+__global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel(const Constrain a, int slices) {
+    constexpr int GROUPS = LS_COLUMNS / 4 / LS_THREADS;         // of four columns a thread
+    extern __shared__ __align__(128) unsigned char ls_raw[];
+    float* ring = (float*)ls_raw;                              // [LS_RING][LS_COLUMNS]
+    uint32_t* count = (uint32_t*)(ring + LS_RING * LS_COLUMNS);
+    uint64_t* full = (uint64_t*)(count + LS_COLUMNS);          // [LS_RING]
+    const int tid = threadIdx.x;
+    if (tid == 0) {
+        for (int i = 0; i < LS_RING; ++i) tg_init(&full[i], 1);
+        tg_init_done();
+    }
+    for (int i = tid; i < LS_COLUMNS / 4; i += LS_THREADS) ((uint4*)count)[i] = make_uint4(0u, 0u, 0u, 0u);
+    pdl_wait();
+    // this block's slices: `todo` from slice `part` of row `r` on
+    const int units = a.rows * slices, each = units / (int)gridDim.x, more = units - each * (int)gridDim.x;
+    const int u0 = (int)blockIdx.x * each + min((int)blockIdx.x, more), todo = each + ((int)blockIdx.x < more ? 1 : 0);
+    int r = u0 / slices, part = u0 - r * slices;
+    int ask_r = r, ask_part = part, asked = 0;                 // the slice that is asked for next, by one thread
+    auto ask = [&]() {
+        const int b = asked % LS_RING, n = min(LS_COLUMNS, a.vocab - ask_part * LS_COLUMNS);
+        const uint32_t bytes = (uint32_t)(n & ~3) * 4u;
+        tg_expect(&full[b], bytes);
+        if (bytes) ls_load(ring + b * LS_COLUMNS, a.logits + ask_r * a.in_stride + ask_part * LS_COLUMNS, bytes, &full[b]);
+        ++asked;
+        if (++ask_part == slices) { ask_part = 0; ++ask_r; }
+    };
+    if (tid == 0)
+        while (asked < todo && asked < LS_RING - 2) ask();
+    __syncthreads();
+    int b_lo = 0, b_hi = 0, h_lo = 0, h_hi = 0;
+    float rep = 1.f, presence = 0.f, frequency = 0.f;
+    bool counts = false, ok = true;
+    const uint32_t* mask = nullptr;
+    int said[LS_AHEAD], drafted = -1, bias_id = -1;            // this thread's first tokens of the history, its drafted one, its
+    float bias_of = 0.f;                                       // first biased one
+    uint32_t next_word[GROUPS];                                // of the mask, for the next slice
+    auto read_mask = [&](int first) {                          // the words of the columns from there on
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            const int c = first + (i * LS_THREADS + tid) * 4;
+            next_word[i] = mask && c < a.vocab ? mask[c >> 5] : 0xffffffffu;
+        }
+    };
+    for (int k = 0, b = 0, phase = 0; k < todo; ++k) {
+        float* buf = ring + b * LS_COLUMNS;
+        if (tid == 0 && asked < todo) {
+            // the buffer of a slice to come: what lay there has been read out, but for the last slice's
+            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            ask();
+        }
+        const int col0 = part * LS_COLUMNS, n_cols = min(LS_COLUMNS, a.vocab - col0);
+        if (k == 0 || part == 0) {                             // another row
+            const int q = a.owner ? a.owner[r] : r;
+            mask = nullptr;
+            if (a.allowed) {
+                const int w = a.allowed_rows ? a.allowed_rows[r] : r;
+                if (w >= 0 && w < a.allowed_rows_n) mask = a.allowed + (size_t)w * a.allowed_stride;
+            }
+            read_mask(col0);
+            b_lo = b_hi = h_lo = h_hi = 0;
+            counts = false;
+            unsigned long long path = 0;                       // drafted tokens of the row's history
+            int d_lo = 0;
+            if (q >= 0 && q < a.requests) {
+                int room = 0;
+                if (a.bias_start) { b_lo = a.bias_start[q]; b_hi = a.bias_start[q + 1]; }
+                if (a.penalties) {
+                    rep = a.penalties[3 * q]; presence = a.penalties[3 * q + 1]; frequency = a.penalties[3 * q + 2];
+                    counts = (rep != 0.f && rep != 1.f) || presence != 0.f || frequency != 0.f;
+                    if (a.history_start) { h_lo = a.history_start[q]; h_hi = a.history_start[q + 1]; }
+                    if (a.windows) room = a.windows[q];
+                    if (room <= 0) room = 0x7fffffff;
+                    if (a.seen) {
+                        d_lo = a.draft_start[q];
+                        const int n = min(a.draft_start[q + 1] - d_lo, DR_NODES);
+                        path = a.seen[r] & (n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull);
+                        const int length = __popcll(path);
+                        while (__popcll(path) > room) path &= path - 1;         // the last ones
+                        room -= min(room, length);
+                    }
+                    if (h_hi - h_lo > room) h_lo = h_hi - room;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < LS_AHEAD; ++j) said[j] = h_lo + j * LS_THREADS + tid < h_hi ? a.history[h_lo + j * LS_THREADS + tid] : -1;
+            drafted = tid < DR_NODES && path >> tid & 1ull ? a.draft_tokens[d_lo + tid] : -1;
+            bias_id = b_lo + tid < b_hi ? a.bias_ids[b_lo + tid] : -1;
+            bias_of = b_lo + tid < b_hi ? a.bias[b_lo + tid] : 0.f;
+        }
+        uint32_t word[GROUPS];
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) word[i] = next_word[i];
+        if (part + 1 < slices) read_mask(col0 + LS_COLUMNS);
+        if (counts) {
+            auto count_in = [&](int token) {
+                const uint32_t c = (uint32_t)(token - col0);
+                if (token >= 0 && c < (uint32_t)n_cols) atomicAdd(&count[c], 1u);
+            };
+            count_in(drafted);
+#pragma unroll
+            for (int j = 0; j < LS_AHEAD; ++j)
+                if (h_lo + j * LS_THREADS < h_hi) count_in(said[j]);
+            for (int i = h_lo + LS_AHEAD * LS_THREADS + tid; i < h_hi; i += LS_THREADS) count_in(a.history[i]);
+        }
+        if (ok) ok = tg_wait(&full[b], phase, &drafts_error_flag, 1);
+        if (tid < (n_cols & 3)) {                              // behind the last whole 16 bytes
+            const int c = (n_cols & ~3) + tid;
+            buf[c] = a.logits[(long long)r * a.in_stride + col0 + c];
+        }
+        if (__syncthreads_or(!ok)) break;
+        if (b_hi > b_lo) {
+            const uint32_t mine = (uint32_t)(bias_id - col0);
+            if (bias_id >= 0 && mine < (uint32_t)n_cols) buf[mine] += bias_of;
+            for (int i = b_lo + LS_THREADS + tid; i < b_hi; i += LS_THREADS) {
+                const int id = a.bias_ids[i];
+                const uint32_t c = (uint32_t)(id - col0);
+                if (id >= 0 && c < (uint32_t)n_cols) buf[c] += a.bias[i];
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            const int g = i * LS_THREADS + tid;
+            const uint32_t bits = word[i] >> (4 * g & 31);
+            const uint4 n = ((const uint4*)count)[g];
+            if ((bits & 0xfu) == 0xfu && !(n.x | n.y | n.z | n.w)) continue;
+            float4 v = ((const float4*)buf)[g];
+            if (n.x | n.y | n.z | n.w) {
+                ((uint4*)count)[g] = make_uint4(0u, 0u, 0u, 0u);
+                v.x = lc_edit(v.x, n.x, rep, presence, frequency);
+                v.y = lc_edit(v.y, n.y, rep, presence, frequency);
+                v.z = lc_edit(v.z, n.z, rep, presence, frequency);
+                v.w = lc_edit(v.w, n.w, rep, presence, frequency);
+            }
+            if (!(bits & 1u)) v.x = -INFINITY;
+            if (!(bits & 2u)) v.y = -INFINITY;
+            if (!(bits & 4u)) v.z = -INFINITY;
+            if (!(bits & 8u)) v.w = -INFINITY;
+            ((float4*)buf)[g] = v;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
+        float* dst = a.out + (long long)r * a.out_stride + col0;
+        if (tid < (n_cols & 3)) dst[(n_cols & ~3) + tid] = buf[(n_cols & ~3) + tid];
+        if (tid == 0) {
+            if (n_cols >= 4) ls_store(dst, buf, (uint32_t)(n_cols & ~3) * 4u);
+            else asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+        if (++part == slices) { part = 0; ++r; }
+        if (++b == LS_RING) { b = 0; phase ^= 1; }
+    }
+    if (tid == 0) {
+        if (!ok) tg_settle_copies(full, LS_RING, asked, &drafts_error_flag, 1);        // not left with copies under way
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+}
+
 // Addresses that are null leave their stage out. strides in elements (words for `allowed`).
 TGO_API int tgo_logits_constrain(const float* logits, long long in_stride, float* out, long long out_stride, int rows, int vocab,
                                  int requests, const int* owner, const int* bias_start, const int* bias_ids, const float* bias,
@@ -168,6 +355,22 @@ TGO_API int tgo_logits_constrain(const float* logits, long long in_stride, float
                    penalties, windows, draft_start, draft_tokens, (const unsigned long long*)seen, (const uint32_t*)allowed,
                    allowed_stride, allowed_rows_n, allowed_rows};
     const bool vectors = ((uintptr_t)logits % 16 == 0 && (uintptr_t)out % 16 == 0) && (rows == 1 || (in_stride % 4 == 0 && out_stride % 4 == 0));
+    if (vectors && logits != out) {
+        constexpr size_t smem = (LS_RING + 1) * LS_COLUMNS * sizeof(float) + LS_RING * 8;
+        static bool set[64] = {};
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return (int)e;
+        if (dev < 0 || dev >= 64) return TGO_E_BAD_ARG;
+        if (!set[dev]) {
+            e = cudaFuncSetAttribute(constrain_stream_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e != cudaSuccess) return (int)e;
+            set[dev] = true;
+        }
+        const int cuts = (vocab + LS_COLUMNS - 1) / LS_COLUMNS;
+        const long long units = (long long)rows * cuts, blocks = (long long)LS_BLOCKS * tgo_multiprocessors();
+        return tgo_launch_pdl(constrain_stream_kernel, dim3((unsigned)(units < blocks ? units : blocks)), dim3(LS_THREADS), smem, stream, a, cuts);
+    }
     if (vectors) return tgo_launch_pdl(constrain_kernel<true>, dim3(slices, rows), dim3(LC_THREADS), 0, stream, a);
     return tgo_launch_pdl(constrain_kernel<false>, dim3(slices, rows), dim3(LC_THREADS), 0, stream, a);
 }
