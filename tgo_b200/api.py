@@ -148,6 +148,34 @@ class LoadedModel:
         search = BeamSearch(engine, beams, max_tokens, stop_ids, length_penalty, chunk)
         return search.run(prompts, self._adapter_list(adapters, len(prompts)))
 
+    def generate_drafted(self, prompts, policy=None, nodes: int = 16, drafter=None, slots: Optional[int] = None,
+                         chunk: int = 2048, pool_tokens: Optional[int] = None, page_size: int = 16, stop_ids=(), adapters=None):
+        """`generate`, several tokens a step where a drafter guesses them (engine/drafts.py): every step verifies a tree of at
+        most `nodes` tokens (64 at most) of each request. `drafter`: an object with `propose(tokens, nodes)` as
+        NgramDrafter, which is the default and looks into the request's own tokens. The requests stay in `last_requests`,
+        the counts of steps, drafted and accepted tokens in `last_drafts`."""
+        from .engine.drafts import DraftedGeneration
+        from .engine.scheduler import Request
+        from .sampling.policy import Policy
+        prompts = [list(map(int, p)) for p in prompts]
+        policies = policy if isinstance(policy, (list, tuple)) else [policy or Policy(max_tokens=16)] * len(prompts)
+        if len(policies) != len(prompts):
+            raise ValueError(f"{len(policies)} policies for {len(prompts)} prompts")
+        if not prompts:
+            return []
+        slots = slots or min(len(prompts), 64)
+        need = max(len(p) + max(pol.max_tokens, 0) for p, pol in zip(prompts, policies)) + nodes
+        if pool_tokens is None:
+            pool_tokens = slots * ((need + 63) // 64 * 64)
+        engine = self.new_engine(page_size=page_size, max_tokens=pool_tokens, num_slots=slots)
+        runner = DraftedGeneration(engine, drafter, nodes, chunk, stop_ids)
+        requests = [Request(p, pol, request_id=i, adapter=ad) for i, (p, pol, ad) in
+                    enumerate(zip(prompts, policies, self._adapter_list(adapters, len(prompts))))]
+        runner.run(requests)
+        self.last_drafts = runner
+        self.last_requests = requests
+        return [r.output for r in requests]
+
     def generate(self, prompts, policy=None, slots: Optional[int] = None, chunk: int = 0,
                  pool_tokens: Optional[int] = None, page_size: int = 16, stop_ids=(),
                  max_batched_tokens: Optional[int] = None, scheduler=None,

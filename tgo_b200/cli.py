@@ -68,6 +68,9 @@ def run_parser():
                          "(default): eos_token_id of the model folder; none: no stop ids")
     ap.add_argument("--kv-pages", type=int, default=0,
                     help="pages in the cache pool (default: enough for --context per prompt)")
+    ap.add_argument("--drafts", type=int, default=0, metavar="N",
+                    help="verify up to N tokens a step and request, drafted from its own earlier tokens "
+                         "(0, the default: one token a step; at most 64)")
     ap.add_argument("--raw", action="store_true",
                     help="accepted for compatibility; prompts are always token ids")
     ap.add_argument("--max-tokens", type=int, default=128,
@@ -170,6 +173,8 @@ def cmd_run(argv, out=sys.stdout, err=sys.stderr, opener=None):
         raise UsageError("--prompt-len N stands in place of --prompt and is positive")
     if args.kv_pages < 0:
         raise UsageError(f"--kv-pages {args.kv_pages}: it cannot be negative")
+    if not 0 <= args.drafts <= 64:
+        raise UsageError(f"--drafts {args.drafts}: 0 to 64 tokens a step")
     prompts = [_ids(p) for p in (args.prompt or ([] if args.prompt_len else ["1 2 3 4 5 6 7 8"]))]
     from .sampling.policy import Policy
     policy = Policy(temperature=args.temp, top_k=args.top_k, top_p=args.top_p,
@@ -187,6 +192,8 @@ def cmd_run(argv, out=sys.stdout, err=sys.stderr, opener=None):
     print(f"tgo: {model.info['architecture']} {dtype} context={args.context} "
           f"temp={args.temp} seed={args.seed} prompt={' + '.join(str(len(p)) for p in prompts)} "
           f"tokens stop_ids={stop_ids}", file=err)
+    if args.drafts:
+        return _run_drafted(args, model, prompts, policy, stop_ids, out, err)
     if len(prompts) > 1:
         return _run_together(args, model, prompts, policy, stop_ids, out, err)
     prompt = prompts[0]
@@ -210,6 +217,33 @@ def cmd_run(argv, out=sys.stdout, err=sys.stderr, opener=None):
     if n:
         print(f"tgo: {len(prompt)} prompt tokens, {n} generated, first token after "
               f"{first * 1e3:.1f} ms, {n / dt:.2f} tokens/s overall", file=err)
+    return 0
+
+
+def _run_drafted(args, model, prompts, policy, stop_ids, out, err):
+    """Several tokens a step where drafts are right; one line of ids per prompt."""
+    import copy
+    need = max(len(p) for p in prompts) + args.max_tokens
+    if need > args.context:
+        raise UsageError(f"a prompt of {need - args.max_tokens} tokens and --max-tokens "
+                         f"{args.max_tokens} exceed the --context {args.context}")
+    policies = []
+    for i in range(len(prompts)):           # each request draws from a stream of its own
+        pol = copy.copy(policy)
+        pol.seed = policy.seed + i
+        policies.append(pol)
+    t0 = time.perf_counter()
+    try:
+        outs = model.generate_drafted(prompts, policies, nodes=args.drafts, page_size=args.page_size, stop_ids=stop_ids,
+                                      pool_tokens=args.kv_pages * args.page_size if args.kv_pages else None)
+    except ValueError as e:
+        raise UsageError(str(e)) from None
+    dt = time.perf_counter() - t0
+    for o in outs:
+        print(" ".join(str(t) for t in o), file=out)
+    n, d = sum(len(o) for o in outs), model.last_drafts
+    print(f"tgo: {len(prompts)} prompts, {sum(len(p) for p in prompts)} prompt tokens, {n} generated in {d.steps} steps "
+          f"({d.accepted} of {d.drafted} drafts accepted), {n / dt:.2f} tokens/s overall", file=err)
     return 0
 
 

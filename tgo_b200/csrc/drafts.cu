@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(LC_THREADS) constrain_kernel(const Constrain a
         if (w >= 0 && w < a.allowed_rows_n) words = a.allowed + (size_t)w * a.allowed_stride + (col0 >> 5);
     }
     const bool owned = q >= 0 && q < a.requests;
+    if (in_place && !owned && !words) return;
     float rep = 1.f, presence = 0.f, frequency = 0.f;
     int b_lo = 0, b_hi = 0, h_lo = 0, h_hi = 0, room = 0, d_lo = 0, d_n = 0;
     unsigned long long path = 0;

@@ -66,8 +66,9 @@ class Session:
                 logits = eng.step([StepEntry(rid, part, [len(part) - 1] if last else [])])
             for _ in range(budget):
                 reports: list = []
+                mask = policy.allowed_words(history[len(prompt):], logits.shape[1])
                 tok = int(sample_batch(logits, [policy], [draws.next()], [history],
-                                       reports).item())
+                                       reports, [mask]).item())
                 self._last_probs = [r for r in reports if r is not None]
                 if tok in self.stop_ids:
                     self._last_probs = []

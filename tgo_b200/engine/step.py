@@ -34,6 +34,23 @@ class StepEntry:
     want: Sequence[int] = field(default_factory=list)
 
 
+@dataclass
+class DraftEntry:
+    """One request's share of a step of drafted tokens: a tree. `tokens[0]` is the token that comes next for certain,
+    every other one continues the one at place `parents[i]`, an earlier place (parents[0]: -1)."""
+    request_id: object
+    tokens: Sequence[int]
+    parents: Sequence[int]
+
+
+@dataclass
+class Accepted:
+    """What a step of drafted tokens confirmed of one request's tree: the places of the tokens that now belong to the
+    request, and the token that comes after them."""
+    path: List[int]
+    following: int
+
+
 class Engine:
     """Model + cache storage + cache bookkeeping on one device."""
 
@@ -288,6 +305,101 @@ class Engine:
         self._begun = None
         self.steps_run += 1
         return logits
+
+    # ------------------------------------------------------------- drafted tokens
+    def takes_drafts(self) -> Optional[str]:
+        """None, or why this model runs no steps of drafted tokens."""
+        for call in self.model.spec.run_order:
+            mixer = self.model.blocks[call.layer].mixer
+            if not getattr(mixer, "takes_drafts", False):
+                return f"its mixer {type(mixer).__name__} takes no trees of tokens"
+        if self.storage.state:
+            return "it keeps a state per request, which cannot go back to the token before a draft"
+        return None
+
+    def _longest_path(self) -> int:
+        """Most tokens of a path through a tree: no node may be behind another's window."""
+        windows = [getattr(self.model.blocks[call.layer].mixer, "window", None) for call in self.model.spec.run_order]
+        return min([ops.TREE_NODES] + [w for w in windows if w])
+
+    def _validate_drafts(self, entries: List[DraftEntry]) -> List[List[int]]:
+        """Every entry's paths, as bits per token."""
+        why = self.takes_drafts()
+        if why:
+            raise ValueError(f"draft_step: this model runs no drafted tokens: {why}")
+        if any(len(e.parents) != len(e.tokens) for e in entries):
+            raise ValueError("draft_step: a parent per token is needed")
+        self._validate([StepEntry(e.request_id, e.tokens) for e in entries])
+        longest, paths = self._longest_path(), []
+        for e in entries:
+            if len(e.tokens) > ops.TREE_NODES:
+                raise ValueError(f"draft_step: request {e.request_id!r} brings {len(e.tokens)} tokens; at most {ops.TREE_NODES}")
+            bits = []
+            for i, p in enumerate(e.parents):
+                if p != -1 if i == 0 else not 0 <= p < i:
+                    raise ValueError(f"draft_step: token {i} of request {e.request_id!r} continues place {p}; the first token "
+                                     "continues none (-1), every other one an earlier place")
+                bits.append((bits[p] if i else 0) | 1 << i)
+                if bin(bits[i]).count("1") > longest:
+                    raise ValueError(f"draft_step: a path of request {e.request_id!r} is longer than {longest} tokens")
+            paths.append(bits)
+        return paths
+
+    def draft_step(self, entries: List[DraftEntry], choose) -> List[Accepted]:
+        """Run every request's tree of drafted tokens as one batch, choose a token behind each of them, and keep what
+        the choice confirms. `choose(logits, ctx)` gets float32 logits [tokens of the step, vocabulary], the entries' one
+        after the other, and returns int32 token ids [tokens] on the device. From its first token on, a request then goes
+        along the drafts that were chosen: their cache rows are moved together, its length grows by the
+        path's. A step that fails leaves every request where it was."""
+        entries = [e if isinstance(e, DraftEntry) else DraftEntry(*e) for e in entries]
+        if not entries:
+            raise ValueError("draft_step: an empty batch carries nothing")
+        paths = self._validate_drafts(entries)
+        if self.device.type == "cuda":
+            compile_together(["attention_tree", "drafts"])
+        ids = [e.request_id for e in entries]
+        begun = self.cache.step_begin(ids, [len(e.tokens) for e in entries])
+        self._begun = (ids, begun)
+        try:
+            buf, meta = self._pack([StepEntry(e.request_id, e.tokens, range(len(e.tokens))) for e in entries])
+        finally:
+            self._begun = None
+        T, total = meta["T"], meta["total"]
+        even = total + total % 2                          # what follows are 64-bit numbers
+        host = np.empty(even + 3 * T, dtype=np.int32)
+        host[:total] = buf[:total]
+        bits = np.array([b for p in paths for b in p], dtype=np.uint64)
+        depth = np.array([bin(b).count("1") - 1 for p in paths for b in p], dtype=np.int32)
+        host[T:2 * T] = np.repeat(np.asarray(meta["firsts"], dtype=np.int32), meta["extents"]) + depth
+        host[even:even + 2 * T] = bits.view(np.int32)
+        host[even + 2 * T:] = [p for e in entries for p in e.parents]
+        dev = torch.from_numpy(host)
+        if self.device.type == "cuda":
+            dev = dev.pin_memory()
+        dev = dev.to(self.device, non_blocking=True)
+        self.h2d_bytes_last = host.nbytes
+        ctx, tables, slots = self._views(dev[:total], meta)
+        ctx.seen, ctx.decode_only = dev[even:even + 2 * T].view(torch.int64), False
+        logits = self.model.forward(ctx, self.storage, tables, slots)
+        chosen = choose(logits, ctx)
+        B = len(entries)
+        found = torch.empty(T + 2 * B, dtype=torch.int32, device=self.device)
+        path, counts, following = found[:T], found[T:T + B], found[T + B:]
+        ops.tree_accept(ctx.token_ids, dev[even + 2 * T:], chosen, ctx.q_start, path, counts, following)
+        for g, kv in enumerate(self.storage.kv):
+            if isinstance(kv, tuple):                     # [calls, pages, ...] a plane
+                ops.tree_keep(list(kv), slots[g], ctx.q_start, path, counts, axis=1)
+            else:                                         # [calls, planes, pages, ...]
+                ops.tree_keep([kv], slots[g], ctx.q_start, path, counts, axis=2)
+        got = found.cpu().numpy()
+        handles, _, widest = begun
+        self.cache.step_commit((handles, np.ascontiguousarray(got[T:T + B]), widest))
+        self.steps_run += 1
+        out, at = [], 0
+        for e, n, f in zip(entries, got[T:T + B].tolist(), got[T + B:].tolist()):
+            out.append(Accepted(got[at:at + n].tolist(), f))
+            at += len(e.tokens)
+        return out
 
     # ------------------------------------------------------------- decode graphs
     BUCKETS = (1, 2, 4, 8, 16, 24, 32, 48, 64, 96, 128, 192, 256)

@@ -279,6 +279,7 @@ class GQAAttention(Part):
 
     # ---- compute
     lazy_rows = True        # x may come as ops.NormedRows; its first product folds the norm in
+    takes_drafts = True     # steps whose tokens are trees of drafts
 
     def forward(self, x, ctx, cache: LayerCache, residual=None):
         """With `residual` (the float32 stream) the result may be added to it, and None is
@@ -327,7 +328,11 @@ class GQAAttention(Part):
                 ops.qk_norm_rope_cache(q, k, v, H, Hkv, dh, None, None, 0.0, None, 0,
                                        cache.slots, cache.k, cache.v, cache.page_size)
         a = torch.empty((x.shape[0], qw), dtype=q.dtype, device=q.device)
-        paged_attention(q, a, H, Hkv, dh, cache, ctx, self.scale, self.window or 0)
+        if ctx.seen is not None:
+            ops.attention_tree(q, a, H, Hkv, dh, cache.k, cache.v, cache.page_size, cache.block_tables, ctx.context_lens,
+                               ctx.q_start, ctx.seen, self.scale, self.window or 0, ctx.max_extent, ctx.max_context)
+        else:
+            paged_attention(q, a, H, Hkv, dh, cache, ctx, self.scale, self.window or 0)
         return self._output(a, ctx, residual)
 
 

@@ -42,6 +42,8 @@ that offers none of them still runs):
   prepare_capture(ctx, cache) -> make, outside a CUDA-graph capture, whatever its forward
                   would otherwise make on the host during the step (lists derived from the
                   step's shape), leaving it in ctx.aux under a key that starts with "tiles";
+  takes_drafts = True (a mixer's class): its forward takes a step of drafted tokens (`ctx.seen`), whose
+                  requests' tokens are trees; an engine refuses drafted steps of a model with other mixers;
   adapter_sites() -> the products whose results a request's low-rank adapter may add to
                   (`AdapterSite`), and bind_adapters(banks) -> take {site's key: AdapterBank}: the
                   forward then calls `bank.add(rows, result, ctx)` behind the product;
@@ -150,6 +152,9 @@ class StepContext:
     decode_only: bool = False        # every request brings exactly one token
     adapters: Optional[torch.Tensor] = None   # int32 [T], each token's adapter (-1: none); None: no
                                               # request of the step has one
+    seen: Optional[torch.Tensor] = None       # int64 [T], a step of drafted tokens: which of its request's
+                                              # tokens of this step each one sees, by bits (itself among
+                                              # them); positions are then those along each one's path
     aux: Dict[str, object] = field(default_factory=dict)   # per-step device tensors made once
 
 

@@ -11,7 +11,9 @@ from __future__ import annotations
 import math
 import struct
 from dataclasses import dataclass, field
-from typing import Dict, List
+from typing import Callable, Dict, List, Optional
+
+import numpy as np
 
 TOP_MAX = 128                 # most candidates either truncation keeps (sample/sample.go:47)
 MAX_DRAW = 0.99999994         # the largest float32 below one (sample/sample.go:194)
@@ -31,6 +33,10 @@ class Policy:
     max_tokens: int = 0               # 0: until the context is full
     logprobs: bool = False            # report each drawn token's log probability
     top_logprobs: int = 0             # and this many alternatives a step (needs logprobs)
+    # A grammar: called with the tokens generated so far, it returns the ids that may come next (any that ends
+    # the request among them), or None: any. Or one number of 32 bits per 32 ids, as an array of uint32 or int32 (bit
+    # i % 32 of number i / 32 allows id i).
+    allowed: Optional[Callable[[List[int]], object]] = None
 
     def check(self, vocab: int) -> None:
         t = self.temperature
@@ -64,6 +70,31 @@ class Policy:
                 raise ValueError(f"policy: logit bias id {i} is outside the vocabulary of {vocab}")
             if b != b or b == math.inf:
                 raise ValueError(f"policy: logit bias for id {i} is {b}")
+        if self.allowed is not None and not callable(self.allowed):
+            raise ValueError("policy: `allowed` is called with the tokens generated so far; it cannot be "
+                             f"a {type(self.allowed).__name__}")
+
+    def allowed_words(self, generated: List[int], vocab: int):
+        """The mask of the tokens that may follow `generated`, uint32 [vocab / 32, rounded up], or None: any may."""
+        got = self.allowed(list(generated)) if self.allowed is not None else None
+        if got is None:
+            return None
+        n = (vocab + 31) // 32
+        if isinstance(got, np.ndarray) and got.dtype in (np.uint32, np.int32) and got.ndim == 1:
+            if got.size < n:
+                raise ValueError(f"policy: a mask of {got.size} words for {vocab} tokens")
+            words = np.array(got[:n]).view(np.uint32)
+            if vocab % 32:
+                words[-1] &= np.uint32((1 << vocab % 32) - 1)
+        else:
+            ids = np.fromiter((int(i) for i in got), dtype=np.int64)
+            if ids.size and (ids.min() < 0 or ids.max() >= vocab):
+                raise ValueError(f"policy: an allowed id is outside the vocabulary of {vocab}")
+            words = np.zeros(n, dtype=np.uint32)
+            np.bitwise_or.at(words, ids // 32, np.uint32(1) << (ids % 32).astype(np.uint32))
+        if not words.any():
+            raise ValueError("policy: no token is allowed to come next")
+        return words
 
     @property
     def greedy(self) -> bool:
@@ -71,8 +102,11 @@ class Policy:
 
     @property
     def edits_logits(self) -> bool:
-        return bool(self.logit_bias) or self.repetition_penalty not in (0.0, 1.0) or \
-            self.presence_penalty != 0 or self.frequency_penalty != 0
+        return bool(self.logit_bias) or self.penalises
+
+    @property
+    def penalises(self) -> bool:
+        return self.repetition_penalty not in (0.0, 1.0) or self.presence_penalty != 0 or self.frequency_penalty != 0
 
 
 @dataclass
@@ -105,8 +139,13 @@ class DrawStream:
         self.index = 0
 
     def next(self) -> float:
-        bits = _splitmix64(_splitmix64(self.seed) ^ self.index)
+        u = self.ahead(0)
         self.index += 1
+        return u
+
+    def ahead(self, n: int) -> float:
+        """The draw that `next` would give after n others."""
+        bits = _splitmix64(_splitmix64(self.seed) ^ (self.index + n))
         u = (bits >> 11) / float(1 << 53)
         u = struct.unpack("<f", struct.pack("<f", u))[0]
         return min(u, MAX_DRAW)

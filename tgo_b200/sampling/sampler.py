@@ -1,7 +1,7 @@
 """From rows of logits on the device to token ids, with one small read-back.
 
-`sample_rows(logits, requests)` applies each request's Policy: bias and penalties edit
-the request's row in place (only for policies that ask for them), then one kernel launch
+`sample_rows(logits, requests)` applies each request's Policy: biases, penalties and masks of allowed
+tokens edit the rows in place, one launch for all that ask for them, then one kernel launch
 samples every row (greedy rows take the argmax branch inside it), and the ids come back
 as one int32 copy. Every row consumes one draw of its request's stream, greedy or not.
 A policy that asks for log probabilities gets them from the same launch: the kernel that
@@ -13,6 +13,7 @@ from __future__ import annotations
 from collections import Counter
 from typing import List, Optional, Sequence
 
+import numpy as np
 import torch
 
 from ..kernels import ops
@@ -46,16 +47,59 @@ def adjust_row(row: torch.Tensor, policy: Policy, history: Sequence[int]) -> Non
                       policy.presence_penalty, policy.frequency_penalty)
 
 
+def constrain(logits: torch.Tensor, policies: Sequence[Policy], histories: Sequence[Sequence[int]], masks: Sequence = (),
+              owner: Optional[Sequence[int]] = None, drafts: Optional[tuple] = None) -> None:
+    """Edit rows of logits in place as the policies ask: row r is the request's owner[r] (None: r), masks[r] an array of
+    uint32 (Policy.allowed_words) or None. `drafts` as for `ops.logits_constrain`: what a row's request has
+    drafted up to it comes behind its history."""
+    Q, R = len(policies), logits.shape[0]
+    masks = list(masks) or [None] * R
+    edits = [p.edits_logits for p in policies]
+    if not any(edits) and all(m is None for m in masks):
+        return
+    biases = [sorted(p.logit_bias.items()) for p in policies]
+    said = []
+    for p, h in zip(policies, histories or [()] * Q):
+        if not p.penalises:
+            h = ()
+        elif p.penalty_window > 0:
+            h = h[-p.penalty_window:]
+        said.append(np.asarray(h, dtype=np.int32))
+    # one buffer of 32-bit numbers, one copy: starts, owners and ids, then what is no whole number
+    first_bias = np.concatenate([[0], np.cumsum([len(b) for b in biases])]).astype(np.int32)
+    first_said = np.concatenate([[0], np.cumsum([s.size for s in said])]).astype(np.int32)
+    kept = [m for m in masks if m is not None]
+    which = np.cumsum([m is not None for m in masks]) - 1
+    parts = [np.array([q if edits[q] else -1 for q in (owner if owner is not None else range(R))], dtype=np.int32),
+             np.array([-1 if m is None else w for m, w in zip(masks, which)], dtype=np.int32),
+             np.array([p.penalty_window for p in policies], dtype=np.int32), first_bias, first_said, np.concatenate(said),
+             np.array([i for b in biases for i, _ in b], dtype=np.int32),
+             np.array([v for b in biases for _, v in b], dtype=np.float32),
+             np.array([[p.repetition_penalty, p.presence_penalty, p.frequency_penalty] for p in policies], dtype=np.float32),
+             np.stack(kept) if kept else np.empty((0, 0), dtype=np.uint32)]
+    host = torch.from_numpy(np.concatenate([x.ravel().view(np.int32) for x in parts]))
+    dev, at = host.to(logits.device), 0
+    views = []
+    for x in parts:
+        views.append(dev[at:at + x.size].view(x.shape))
+        at += x.size
+    owners, rows, windows, b0, h0, tokens, b_ids, b_values, penalties, words = views
+    floats = [t.view(torch.float32) for t in (b_values, penalties)]
+    ops.logits_constrain(logits, owners, bias=(b0, b_ids, floats[0]) if b_ids.numel() else None,
+                         history=(h0, tokens), penalties=floats[1], windows=windows, drafts=drafts,
+                         allowed=words if kept else None, allowed_rows=rows if kept else None)
+
+
 def sample_batch(logits: torch.Tensor, policies: Sequence[Policy], draws: Sequence[float],
                  histories: Sequence[Sequence[int]] = (),
-                 reports: Optional[list] = None) -> torch.Tensor:
+                 reports: Optional[list] = None, masks: Sequence = (), edited: bool = False) -> torch.Tensor:
     """Token ids (int32, on the device) for each row. With `reports` (a list), it is
-    filled with one entry per row: a TokenProb for a policy with logprobs, else None."""
+    filled with one entry per row: a TokenProb for a policy with logprobs, else None. `masks`: each row's
+    Policy.allowed_words. `edited`: the rows have been through `constrain` already."""
     n = logits.shape[0]
     assert len(policies) == n and len(draws) == n
-    for r, pol in enumerate(policies):
-        if pol.edits_logits:
-            adjust_row(logits[r], pol, histories[r] if histories else ())
+    if not edited:
+        constrain(logits, policies, histories, masks)
     out = torch.empty(n, dtype=torch.int32, device=logits.device)
     asked = reports is not None and any(p.logprobs for p in policies)
     if reports is not None:
@@ -93,15 +137,16 @@ def sample_rows(logits: torch.Tensor, requests) -> List[int]:
     """The Runner's sampling hook: requests carry `.policy`, `.sampler` (a DrawStream),
     `.prompt`, `.output` and `.logprobs` (a TokenProb is appended for every sampled token of a
     policy that asks; the Runner drops a stop token's)."""
-    policies, draws, histories = [], [], []
+    policies, draws, histories, masks = [], [], [], []
     for req in requests:
         if req.sampler is None:
             req.sampler = DrawStream(req.policy.seed)
         policies.append(req.policy)
         draws.append(req.sampler.next())
         histories.append(req.prompt + req.output if req.policy.edits_logits else ())
+        masks.append(req.policy.allowed_words(req.output, logits.shape[1]))
     reports: list = []
-    ids = sample_batch(logits, policies, draws, histories, reports).tolist()
+    ids = sample_batch(logits, policies, draws, histories, reports, masks).tolist()
     for req, rep in zip(requests, reports):
         if rep is not None:
             req.logprobs.append(rep)
