@@ -462,6 +462,27 @@ def test_constrain_single_stages(stage):
     check_constrain(x, c)
 
 
+@pytest.mark.parametrize("V", [1, 3, 6143, 6145, 12289, 30002])
+@pytest.mark.parametrize("first,stride", [(0, 0), (1, 0), (2, 3), (3, 1), (0, 4)])
+def test_constrain_rows_anywhere_to_boundaries(V, first, stride):
+    """Rows that begin at any place of 16 bytes, in both matrices alike or not; nothing beside them is written."""
+    x, c = constrained(5, V, 3, seed=V + first, bias=7, history=200, windows=[0, 9], nodes=5, allowed=4)
+    want = plain_constrain(x, **c).to(DEV)
+    size = x.abs().double() * 2 + 4 * 6 + 50
+    for out_first in (first, (first + 1) % 4):
+        src, dst = (torch.full((5 * (V + stride) + 8,), 9.0, device=DEV) for _ in range(2))
+        rows = src[first:].as_strided((5, V), (V + stride, 1), first)
+        rows.copy_(x)
+        held = src.clone()
+        to = dst.as_strided((5, V), (V + stride, 1), out_first)
+        ops().logits_constrain(rows, out=to, **c)
+        gone = want == -INF
+        assert torch.equal(to == -INF, gone) and torch.equal(src, held)
+        assert bool(((to.double() - want).abs()[~gone] <= 5 * 2.0 ** -24 * size[~gone]).all())
+        to.fill_(9.0)
+        assert bool((dst == 9).all())
+
+
 def test_constrain_odd_values():
     """Infinities and NaN in the logits pass through; -inf stays; a token said a thousand times; ids outside."""
     x, c = constrained(3, 5000, 3, seed=5, history=3000, allowed=3)

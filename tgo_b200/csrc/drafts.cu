@@ -13,13 +13,12 @@
 //   not allowed: x = -inf
 // the order and the arithmetic of the sampler's single rows (adjust_kernel of sampling.cu), so that both give the same bits.
 //
-// In place, or for rows that lie on no 16-byte boundaries, a block takes a slice of 8192 columns of a row: it counts the history's
-// tokens that fall into its slice in shared memory (integers: the order of the additions changes nothing), and then edits and
-// stores. A biased token is left to a second look, when everything else of the slice is done. In place, a group of
-// four columns (VECTORS; or a column) without a counted or a forbidden token is neither read nor written.
+// In place, and where the two matrices' rows lie differently to 16-byte boundaries, a block takes a slice of 8192 columns of a
+// row: it counts the history's tokens that fall into its slice in shared memory (integers: the order of the additions
+// changes nothing), and then edits and stores, a thread a column at a time, in place only what changes. A biased token is left
+// to a second look, when everything else of the slice is done.
 #define LC_THREADS 256
-#define LC_VPT 8                  // groups of four columns a thread
-#define LC_COLUMNS (LC_THREADS * LC_VPT * 4)
+#define LC_COLUMNS 8192
 #ifndef LC_AHEAD
 #define LC_AHEAD 8                // tokens of the history that a thread reads at once
 #endif
@@ -49,7 +48,6 @@ __device__ __forceinline__ float lc_edit(float x, uint32_t count, float rep, flo
     return x;
 }
 
-template <bool VECTORS>
 __global__ void __launch_bounds__(LC_THREADS) constrain_kernel(const Constrain a) {
     __shared__ __align__(16) uint32_t count[LC_COLUMNS];
     pdl_wait();
@@ -81,16 +79,11 @@ __global__ void __launch_bounds__(LC_THREADS) constrain_kernel(const Constrain a
             d_n = min(a.draft_start[q + 1] - d_lo, DR_NODES);
         }
     }
-    uint32_t allowed[LC_VPT];                 // of the vectors' columns
-#pragma unroll
-    for (int i = 0; i < LC_VPT; ++i) {
-        const int c = (i * LC_THREADS + tid) * 4;
-        allowed[i] = VECTORS && words && c < n_cols ? words[c >> 5] : 0xffffffffu;
-    }
-#pragma unroll
-    for (int i = 0; i < LC_VPT; ++i) ((uint4*)count)[i * LC_THREADS + tid] = make_uint4(0u, 0u, 0u, 0u);
+    const bool counts = (rep != 0.f && rep != 1.f) || presence != 0.f || frequency != 0.f;
+    if (in_place && !counts && !words && b_hi <= b_lo) return;
+    for (int i = tid; i < LC_COLUMNS / 4; i += LC_THREADS) ((uint4*)count)[i] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
-    if ((rep != 0.f && rep != 1.f) || presence != 0.f || frequency != 0.f) {
+    if (counts) {
         if (room <= 0) room = 0x7fffffff;
         path &= d_n >= 64 ? ~0ull : d_n <= 0 ? 0ull : (1ull << d_n) - 1ull;
         if (tid < DR_NODES && path >> tid & 1ull && __popcll(path >> tid) <= room) {
@@ -113,50 +106,27 @@ __global__ void __launch_bounds__(LC_THREADS) constrain_kernel(const Constrain a
         if (c >= 0 && c < n_cols) atomicOr(&count[c], LC_BIASED);
     }
     __syncthreads();
-    auto value = [&](float v, uint32_t n, uint32_t ok) {
-        if (n & LC_BIASED) return v;
-        if (!(ok & 1u)) return -INFINITY;
-        return lc_edit(v, n, rep, presence, frequency);
-    };
-    if (VECTORS) {
-#pragma unroll
-        for (int i = 0; i < LC_VPT; ++i) {
-            const int g = i * LC_THREADS + tid, c = g * 4;
-            if (c >= n_cols) break;
-            const uint4 n = ((const uint4*)count)[g];
-            const uint32_t bits = allowed[i] >> (c & 31);
-            if ((bits & 0xfu) == 0xfu && !((n.x | n.y | n.z | n.w) & ~LC_BIASED)) continue;
-            if (c + 3 < n_cols) {
-                float4 v = *(const float4*)(src + c);
-                v.x = value(v.x, n.x, bits); v.y = value(v.y, n.y, bits >> 1);
-                v.z = value(v.z, n.z, bits >> 2); v.w = value(v.w, n.w, bits >> 3);
-                *(float4*)(dst + c) = v;
-            } else {
-                for (int k = 0; c + k < n_cols; ++k) dst[c + k] = value(src[c + k], count[c + k], bits >> k);
-            }
-        }
-    } else {
-        for (int c = tid; c < n_cols; c += LC_THREADS) {
-            const uint32_t bits = words ? words[c >> 5] >> (c & 31) : 1u;
-            if (in_place && (bits & 1u) && !(count[c] & ~LC_BIASED)) continue;
-            dst[c] = value(src[c], count[c], bits);
-        }
+#pragma unroll 4
+    for (int c = tid; c < n_cols; c += LC_THREADS) {
+        const bool ok = !words || words[c >> 5] >> (c & 31) & 1u;
+        const uint32_t n = count[c];
+        if (n & LC_BIASED) continue;
+        if (!ok) dst[c] = -INFINITY;
+        else if (n || !in_place) dst[c] = lc_edit(src[c], n, rep, presence, frequency);
     }
-    if (b_hi > b_lo) {
-        __syncthreads();
-        for (int i = b_lo + tid; i < b_hi; i += LC_THREADS) {
-            const int c = a.bias_ids[i] - col0;
-            if (c < 0 || c >= n_cols) continue;
-            const bool ok = !words || words[c >> 5] >> (c & 31) & 1u;
-            dst[c] = ok ? lc_edit(src[c] + a.bias[i], count[c] & ~LC_BIASED, rep, presence, frequency) : -INFINITY;
-        }
+    for (int i = b_lo + tid; i < b_hi; i += LC_THREADS) {
+        const int c = a.bias_ids[i] - col0;
+        if (c < 0 || c >= n_cols) continue;
+        const bool ok = !words || words[c >> 5] >> (c & 31) & 1u;
+        dst[c] = ok ? lc_edit(src[c] + a.bias[i], count[c] & ~LC_BIASED, rep, presence, frequency) : -INFINITY;
     }
 }
 
-// Out of place, rows on 16-byte boundaries: persistent blocks take slices one after the other, each a run of them, mostly of one row,
-// whose numbers then stay in registers. A slice comes into shared memory by one bulk copy, asked for while the slice
-// before it is edited, is edited there where there is something to edit, and leaves by another: the copies wait for nothing
-// but each other.
+// Out of place: persistent blocks take slices one after the other, each a run of them, mostly of one row, whose numbers then
+// stay in registers. A slice comes into shared memory by one bulk copy, asked for while the slices before it are edited, is
+// edited there where there is something to edit, and leaves by another: the copies wait for nothing but each other. They go
+// by 16 bytes: a slice begins at a boundary, and what of a first or last 16 bytes belongs to another row is read but not
+// stored. (Both matrices' rows lie alike to the boundaries.)
 #ifndef LS_THREADS
 #define LS_THREADS 512
 #endif
@@ -197,16 +167,19 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
     }
     for (int i = tid; i < LS_COLUMNS / 4; i += LS_THREADS) ((uint4*)count)[i] = make_uint4(0u, 0u, 0u, 0u);
     pdl_wait();
+    // A row's places are its columns and, before them, the `skip` numbers from the boundary on.
     // this block's slices: `todo` from slice `part` of row `r` on
     const int units = a.rows * slices, each = units / (int)gridDim.x, more = units - each * (int)gridDim.x;
     const int u0 = (int)blockIdx.x * each + min((int)blockIdx.x, more), todo = each + ((int)blockIdx.x < more ? 1 : 0);
     int r = u0 / slices, part = u0 - r * slices;
     int ask_r = r, ask_part = part, asked = 0;                 // the slice that is asked for next, by one thread
     auto ask = [&]() {
-        const int b = asked % LS_RING, n = min(LS_COLUMNS, a.vocab - ask_part * LS_COLUMNS);
-        const uint32_t bytes = (uint32_t)(n & ~3) * 4u;
+        const float* from = a.logits + ask_r * a.in_stride;
+        const int b = asked % LS_RING, skip = (int)((uintptr_t)from >> 2 & 3);
+        const int n = min(LS_COLUMNS, skip + a.vocab - ask_part * LS_COLUMNS);
+        const uint32_t bytes = n > 0 ? (uint32_t)(n + 3 & ~3) * 4u : 0u;
         tg_expect(&full[b], bytes);
-        if (bytes) ls_load(ring + b * LS_COLUMNS, a.logits + ask_r * a.in_stride + ask_part * LS_COLUMNS, bytes, &full[b]);
+        if (bytes) ls_load(ring + b * LS_COLUMNS, from - skip + ask_part * LS_COLUMNS, bytes, &full[b]);
         ++asked;
         if (++ask_part == slices) { ask_part = 0; ++ask_r; }
     };
@@ -220,11 +193,15 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
     int said[LS_AHEAD], drafted = -1, bias_id = -1;            // this thread's first tokens of the history, its drafted one, its
     float bias_of = 0.f;                                       // first biased one
     uint32_t next_word[GROUPS];                                // of the mask, for the next slice
-    auto read_mask = [&](int first) {                          // the words of the columns from there on
+    uint32_t next_more[GROUPS];                                // the words behind them, where four columns lie in two
+    int skip = 0;
+    auto read_mask = [&](int first) {                          // of the columns from there on, four a group
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
-            const int c = first + (i * LS_THREADS + tid) * 4;
-            next_word[i] = mask && c < a.vocab ? mask[c >> 5] : 0xffffffffu;
+            const int c = first + (i * LS_THREADS + tid) * 4, at = c >> 5;
+            next_word[i] = next_more[i] = 0xffffffffu;
+            if (mask && c >= 0 && c < a.vocab) next_word[i] = mask[at];
+            if (mask && skip && (c & 31) > 28 && at + 1 < (a.vocab + 31) >> 5) next_more[i] = mask[at + 1];
         }
     };
     for (int k = 0, b = 0, phase = 0; k < todo; ++k) {
@@ -234,7 +211,8 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
             asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
             ask();
         }
-        const int col0 = part * LS_COLUMNS, n_cols = min(LS_COLUMNS, a.vocab - col0);
+        if (k == 0 || part == 0) skip = (int)((uintptr_t)(a.logits + r * a.in_stride) >> 2 & 3);
+        const int col0 = part * LS_COLUMNS - skip, n_cols = min(LS_COLUMNS, a.vocab - col0);       // to the slice's first place
         if (k == 0 || part == 0) {                             // another row
             const int q = a.owner ? a.owner[r] : r;
             mask = nullptr;
@@ -275,12 +253,12 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
         }
         uint32_t word[GROUPS];
 #pragma unroll
-        for (int i = 0; i < GROUPS; ++i) word[i] = next_word[i];
+        for (int i = 0; i < GROUPS; ++i) word[i] = __funnelshift_r(next_word[i], next_more[i], col0 + (i * LS_THREADS + tid) * 4 & 31) & 0xfu;
         if (part + 1 < slices) read_mask(col0 + LS_COLUMNS);
         if (counts) {
             auto count_in = [&](int token) {
                 const uint32_t c = (uint32_t)(token - col0);
-                if (token >= 0 && c < (uint32_t)n_cols) atomicAdd(&count[c], 1u);
+                if (token >= 0 && c < (uint32_t)max(n_cols, 0)) atomicAdd(&count[c], 1u);
             };
             count_in(drafted);
 #pragma unroll
@@ -289,27 +267,23 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
             for (int i = h_lo + LS_AHEAD * LS_THREADS + tid; i < h_hi; i += LS_THREADS) count_in(a.history[i]);
         }
         if (ok) ok = tg_wait(&full[b], phase, &drafts_error_flag, 1);
-        if (tid < (n_cols & 3)) {                              // behind the last whole 16 bytes
-            const int c = (n_cols & ~3) + tid;
-            buf[c] = a.logits[(long long)r * a.in_stride + col0 + c];
-        }
         if (__syncthreads_or(!ok)) break;
         if (b_hi > b_lo) {
             const uint32_t mine = (uint32_t)(bias_id - col0);
-            if (bias_id >= 0 && mine < (uint32_t)n_cols) buf[mine] += bias_of;
+            if (bias_id >= 0 && mine < (uint32_t)max(n_cols, 0)) buf[mine] += bias_of;
             for (int i = b_lo + LS_THREADS + tid; i < b_hi; i += LS_THREADS) {
                 const int id = a.bias_ids[i];
                 const uint32_t c = (uint32_t)(id - col0);
-                if (id >= 0 && c < (uint32_t)n_cols) buf[c] += a.bias[i];
+                if (id >= 0 && c < (uint32_t)max(n_cols, 0)) buf[c] += a.bias[i];
             }
             __syncthreads();
         }
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
             const int g = i * LS_THREADS + tid;
-            const uint32_t bits = word[i] >> (4 * g & 31);
+            const uint32_t bits = word[i];
             const uint4 n = ((const uint4*)count)[g];
-            if ((bits & 0xfu) == 0xfu && !(n.x | n.y | n.z | n.w)) continue;
+            if (bits == 0xfu && !(n.x | n.y | n.z | n.w)) continue;
             float4 v = ((const float4*)buf)[g];
             if (n.x | n.y | n.z | n.w) {
                 ((uint4*)count)[g] = make_uint4(0u, 0u, 0u, 0u);
@@ -327,10 +301,15 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
         float* dst = a.out + (long long)r * a.out_stride + col0;
-        if (tid < (n_cols & 3)) dst[(n_cols & ~3) + tid] = buf[(n_cols & ~3) + tid];
+        // whole 16 bytes by a copy, what is before and behind them one by one
+        const int lo = part == 0 ? skip : 0, lo4 = lo + 3 & ~3, hi4 = max(n_cols, 0) & ~3;
         if (tid == 0) {
-            if (n_cols >= 4) ls_store(dst, buf, (uint32_t)(n_cols & ~3) * 4u);
+            if (hi4 > lo4) ls_store(dst + lo4, buf + lo4, (uint32_t)(hi4 - lo4) * 4u);
             else asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+        if (tid >= 32 && tid < 40) {
+            const int c = tid < 36 ? lo + tid - 32 : max(hi4, lo4) + tid - 36;
+            if (tid < 36 ? c < min(lo4, n_cols) : c < n_cols) dst[c] = buf[c];
         }
         if (++part == slices) { part = 0; ++r; }
         if (++b == LS_RING) { b = 0; phase ^= 1; }
@@ -355,8 +334,8 @@ TGO_API int tgo_logits_constrain(const float* logits, long long in_stride, float
     Constrain a = {logits, out, in_stride, out_stride, rows, vocab, requests, owner, bias_start, bias_ids, bias, history_start, history,
                    penalties, windows, draft_start, draft_tokens, (const unsigned long long*)seen, (const uint32_t*)allowed,
                    allowed_stride, allowed_rows_n, allowed_rows};
-    const bool vectors = ((uintptr_t)logits % 16 == 0 && (uintptr_t)out % 16 == 0) && (rows == 1 || (in_stride % 4 == 0 && out_stride % 4 == 0));
-    if (vectors && logits != out) {
+    if (logits != out && ((uintptr_t)logits - (uintptr_t)out) % 16 == 0 && (rows == 1 || (in_stride - out_stride) % 4 == 0) &&
+        (long long)rows * ((vocab + 3) / LS_COLUMNS + 1) <= 0x7fffffffll) {
         constexpr size_t smem = (LS_RING + 1) * LS_COLUMNS * sizeof(float) + LS_RING * 8;
         static bool set[64] = {};
         int dev = 0;
@@ -368,12 +347,13 @@ TGO_API int tgo_logits_constrain(const float* logits, long long in_stride, float
             if (e != cudaSuccess) return (int)e;
             set[dev] = true;
         }
-        const int cuts = (vocab + LS_COLUMNS - 1) / LS_COLUMNS;
-        const long long units = (long long)rows * cuts, blocks = (long long)LS_BLOCKS * tgo_multiprocessors();
-        return tgo_launch_pdl(constrain_stream_kernel, dim3((unsigned)(units < blocks ? units : blocks)), dim3(LS_THREADS), smem, stream, a, cuts);
+        // slices of the row that has most numbers before its first column
+        const bool even = (uintptr_t)logits % 16 == 0 && (rows == 1 || in_stride % 4 == 0);
+        const int cuts = (vocab + (even ? 0 : 3) + LS_COLUMNS - 1) / LS_COLUMNS;
+        const int units = rows * cuts, blocks = LS_BLOCKS * tgo_multiprocessors();
+        return tgo_launch_pdl(constrain_stream_kernel, dim3(units < blocks ? units : blocks), dim3(LS_THREADS), smem, stream, a, cuts);
     }
-    if (vectors) return tgo_launch_pdl(constrain_kernel<true>, dim3(slices, rows), dim3(LC_THREADS), 0, stream, a);
-    return tgo_launch_pdl(constrain_kernel<false>, dim3(slices, rows), dim3(LC_THREADS), 0, stream, a);
+    return tgo_launch_pdl(constrain_kernel, dim3(slices, rows), dim3(LC_THREADS), 0, stream, a);
 }
 
 // --------------------------------------------------------------------------- tree_accept
