@@ -36,10 +36,15 @@ def paths_of(parents):
     return bits
 
 
-@pytest.fixture(params=["chosen", "FMA units"])
+WAYS = ["chosen", "FMA units", "one tile whole", "one tile cut", "two tiles whole", "two tiles cut"]
+
+
+@pytest.fixture(params=WAYS)
 def way(request):
-    """The attention goes the way that the framework chooses, and by the kernel that takes every call."""
-    ops().attention_tree_force_way(["chosen", "FMA units"].index(request.param))
+    """The attention goes the way that the framework chooses, and all the others where they take the call."""
+    if request.param not in WAYS[:2] and request.node.callspec.params.get("dtype", torch.bfloat16) != torch.bfloat16:
+        pytest.skip("these ways are bfloat16's")
+    ops().attention_tree_force_way(WAYS.index(request.param))
     yield request.param
     ops().attention_tree_force_way(0)
     assert ops().attention_tree_error() == 0

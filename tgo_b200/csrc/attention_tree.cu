@@ -1162,7 +1162,7 @@ TGO_API int tgo_attention_tree_tc_supports(int dh, int group, int page_size) {
 // The code that a wait of that kernel left when it ran out (1 copies, 2 products, 3 softmax, 4 results), or 0. Synchronises.
 TGO_API int tgo_attention_tree_error(int* value) { return (int)cudaMemcpyFromSymbol(value, tree_error_flag, sizeof(int)); }
 
-static int tree_force = 0;                    // for tests: 1 plain products, 2 tensor cores where they take the call
+static int tree_force = 0;                    // for tests: 1 plain products; 2, 3 items of one row tile, whole and cut; 4, 5 of two
 TGO_API int tgo_attention_tree_force(int way) { tree_force = way; return 0; }
 
 // Floats of workspace that a call wants.
@@ -1266,10 +1266,45 @@ static int tree_tc_go(const CUtensorMap& mk, const CUtensorMap& mv, const CUtens
     return tree_join_go<bf16>(out, out_stride, DH, w, work, tree_ml(work, w, DH), tree_notes(work, w, DH), stream);
 }
 
-// Whether a call's items stay whole: where none has more than so many key tiles.
-static int tree_whole(const TreeWork& w, int max_context, int keys, int tiles) {
+// Most key tiles of an item.
+static int tree_tiles(const TreeWork& w, int max_context, int keys) {
     const int reach = w.window > 0 && max_context > w.window + w.max_nodes ? w.window + w.max_nodes + keys - 1 : max_context;
-    return (reach + keys - 1) / keys <= tiles;
+    return reach <= keys ? 1 : (reach + keys - 1) / keys;
+}
+
+// The tensor cores' four ways, by what they took where they were measured (us; 8 kv heads of 4 query heads, 128 wide, lengths up to 30 %
+// apart; "one" and "two": row tiles an item, "whole" and "cut"):
+//                                   one whole  one cut  two whole  two cut
+//    1 request of  4 nodes,    300       11.7     12.3
+//    1             4,         1000       18.1     13.0
+//   16             8,         2000       30.0     32.2
+//   40             8,         1500       62.8     52.7
+//    4            64,          500       15.1     19.6       21.5     22.8
+//    4            64,        16000      143.8     81.6      254.7     72.7
+//   32            64,         1000       67.7     74.5       60.5     75.9
+//    8            40,         1000       20.7     28.1       30.1     28.3
+// Whole items run in rounds of one an SM: a key tile takes 1.4 us, or 2.2 for two row tiles, an item's beginning and end 2 and 4 where they show
+// once, and 3.5 and 8 in every round of several. Cutting costs 5.5 more (the join) and shares all tiles out evenly, 1.5
+// and 2.3 us each beside the items' beginnings and ends. The cheapest by this count is within 8 % of the fastest measured.
+static void tree_choose(TreeWork& w, int max_context, int G, int sms) {
+    const int tokens = TT_ROWS / G, t = tree_tiles(w, max_context, TT_KEYS);
+    double best = 0;
+    int way = 0;
+    for (int rt = 1; rt <= 2; ++rt) {
+        if (rt == 2 && w.max_nodes <= tokens) break;
+        const double items = (double)w.B * w.Hkv * ((w.max_nodes + rt * tokens - 1) / (rt * tokens));
+        const double rounds = (double)(long long)((items + sms - 1) / sms);
+        const double whole = rounds * (t * (rt == 1 ? 1.4 : 2.2) + (rounds > 1 ? rt == 1 ? 3.5 : 8.0 : rt == 1 ? 2.0 : 4.0));
+        const double each = items * (t + TREE_OVERHEAD) / sms;
+        const double cut = 5.5 + (each > 1 ? each : 1) * (rt == 1 ? 1.5 : 2.3) + items / sms * (rt == 1 ? 3.0 : 8.0);
+        if (!way || whole < best) { best = whole; way = 2 * rt; }
+        if (cut < best) { best = cut; way = 2 * rt + 1; }
+    }
+    if (tree_force >= 2 && (tree_force < 4 || w.max_nodes > tokens)) way = tree_force;
+    w.tokens_per_tile = way / 2 * tokens;
+    w.rows_per_tile = (w.max_nodes < w.tokens_per_tile ? w.max_nodes : w.tokens_per_tile) * G;      // of a part
+    w.whole = way % 2 == 0;
+    w.min_units = w.whole ? 1 : 2;
 }
 
 template <typename T, int DP, int R>
@@ -1296,7 +1331,7 @@ static int tree_plain_go(const void* q, long long q_stride, void* out, long long
     if ((1 << shift) != page_size) shift = -1;
     w.rows_per_tile = ROWS;
     w.workers = held[dev] * tgo_multiprocessors();
-    w.whole = tree_whole(w, max_context, TP_KEYS, 2);
+    w.whole = tree_tiles(w, max_context, TP_KEYS) <= 2;
     if (w.whole) w.min_units = 1;
     int rc = tgo_launch_pdl(tree_plain_kernel<T, DP, R>, dim3(w.workers), dim3(TP_THREADS), smem, stream, (const T*)q, q_stride, (T*)out,
                             out_stride, (const T*)k, (const T*)v, n_pages, page_size, shift, tables, max_blocks,
@@ -1323,13 +1358,9 @@ TGO_API int tgo_attention_tree(const void* q, long long q_stride, void* out, lon
     if (dtype == TGO_BF16 && tree_force != 1 && tgo_attention_tree_tc_supports(dh, G, page_size) && q_stride % 8 == 0 && out_stride % 8 == 0 &&
         (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)k_cache % 128 == 0 && (uintptr_t)v_cache % 128 == 0 &&
         rows + page_size <= 0x7fffffffll) {
-        // trees of more rows than a tile's: two tiles an item
-        const bool two = max_nodes > TT_ROWS / G;
-        w.tokens_per_tile = (two ? 2 : 1) * (TT_ROWS / G);
-        w.rows_per_tile = (max_nodes < w.tokens_per_tile ? max_nodes : w.tokens_per_tile) * G;      // of a part
         w.workers = sms;
-        w.whole = tree_whole(w, max_context, TT_KEYS, two ? 8 : 12);
-        if (w.whole) w.min_units = 1;
+        tree_choose(w, max_context, G, sms);
+        const bool two = w.tokens_per_tile > TT_ROWS / G;
         const CUtensorMap* mk = tree_map_kv(k_cache, rows, page_size, dh);
         const CUtensorMap* mv = tree_map_kv(v_cache, rows, page_size, dh);
         const CUtensorMap* mq = tree_map_q(q, q_stride, T, H, G, dh);

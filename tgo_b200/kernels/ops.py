@@ -2293,8 +2293,9 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, num_heads: int, num_kv_he
 
 
 def attention_tree_force_way(way: int = 0) -> None:
-    """For tests and tuning: `attention_tree` takes the FMA units (1) or, where they take the call, the tensor cores (2)
-    instead of choosing; 0 gives the choice back."""
+    """For tests and tuning: `attention_tree` takes the FMA units (1) or, where the tensor cores take the call, them with one
+    tile of rows an item, left whole (2) or cut (3), or with two tiles, where a tree may have them (4, 5), instead of
+    choosing; 0 gives the choice back."""
     load_library("attention_tree").tgo_attention_tree_force(c_int(way))
 
 
