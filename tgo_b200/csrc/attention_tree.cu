@@ -73,11 +73,21 @@ template <int KT> struct TreeWalk {
         TreeRequest mine;
         mine.units = 0;
         if (lane < w.B) mine = tree_request<KT>(w, lane);
-        const int first_units = mine.units;
-        int total = first_units;
-        for (int c = lane + 32; c < w.B; c += 32) total += tree_request<KT>(w, c).units;
+        auto scan = [&](int x) {                   // the sum of the lanes up to this one
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+            for (int o = 1; o < 32; o <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += other;
+            }
+            return x;
+        };
+        int upto = scan(mine.units);
+        int total = __shfl_sync(0xffffffffu, upto, 31);
+        if (w.B > 32) {
+            int rest = 0;
+            for (int c = lane + 32; c < w.B; c += 32) rest += tree_request<KT>(w, c).units;
+            total += __shfl_sync(0xffffffffu, scan(rest), 31);
+        }
         const int most = total / w.min_units;
         cut.workers = total == 0 ? 0 : most < 1 ? 1 : min(most, w.workers);
         u = end = first = b = 0;
@@ -91,12 +101,7 @@ template <int KT> struct TreeWalk {
             if (b0) {
                 mine.units = 0;
                 if (b0 + lane < w.B) mine = tree_request<KT>(w, b0 + lane);
-            }
-            int upto = mine.units;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int other = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += other;
+                upto = scan(mine.units);
             }
             const uint32_t in = __ballot_sync(0xffffffffu, u < before + upto);
             if (in) {
@@ -585,6 +590,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = w.H / w.Hkv;
     const int tile_tokens = TT_ROWS / G, tile_rows = tile_tokens * G;       // of a row tile
+    const uint32_t by_g = (65535u + (uint32_t)G) / (uint32_t)G;             // r / G for r < 256
+    auto node_of = [&](int r) { return (int)((uint32_t)r * by_g >> 16); };
     int* const err = &tree_error_flag;
     // rows of the Q tiles that no box writes must not hold NaN by chance
     if (tile_rows != TT_ROWS) for (int i = tid; i < 2 * TT_TILE / 16; i += TT_THREADS) ((uint4*)sQ)[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -828,7 +835,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
             const TreeItem rec = ring[n & 3];
             const int n_rows = min(rec.n_rows - row_lo, tile_rows);
             const bool row_ok = row < n_rows;
-            const unsigned long long bits = rec.valid && row_ok ? s_bits[(n & 1u) * 64 + (row_lo + row) / G] : 0ull;
+            const unsigned long long bits = rec.valid && row_ok ? s_bits[(n & 1u) * 64 + node_of(row_lo + row)] : 0ull;
             if (!rec.valid) break;
             __syncwarp();
             if (lane == 0) tg_arrive(&q_empty[n & 1u]);
@@ -941,10 +948,13 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
             unsigned long long bits[RT];
 #pragma unroll
             for (int t = 0; t < RT; ++t)
-                bits[t] = row < min(rec.n_rows - t * tile_rows, tile_rows) ? s_bits[(n & 1u) * 64 + (t * tile_rows + row) / G] : 0ull;
+                bits[t] = row < min(rec.n_rows - t * tile_rows, tile_rows) ? s_bits[(n & 1u) * 64 + node_of(t * tile_rows + row)] : 0ull;
             __syncwarp();
             if (lane == 0) tg_arrive(&q_empty[n & 1u]);
-            auto result = [&](int r) { return out + (size_t)(rec.tok0 + r / G) * out_stride + (size_t)(rec.kvh * G + r % G) * DH; };
+            auto result = [&](int r) {
+                const int node = node_of(r);
+                return out + (size_t)(rec.tok0 + node) * out_stride + (size_t)(rec.kvh * G + r - node * G) * DH;
+            };
             if (rec.n_it == 0) {
                 for (int r = row; r < rec.n_rows; r += TT_ROWS) {
                     bf16* dst = result(r);
@@ -1019,57 +1029,63 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
                     *(float2*)(part_ml + ((size_t)rec.slot * w.rows_per_tile + item_row) * 2) = make_float2(m, l);
                 float4* po = (float4*)part_o + (size_t)rec.slot * (DH / 4) * w.rows_per_tile + item_row;
                 const uint32_t tm_o = tmem + 256u + (RT == 2 ? 128u * t : 0u) + lane_base;
+                // the rows that this lane stores: four lanes a row of 64 bytes
+                bf16* line_out[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) line_out[k] = result(t * tile_rows + quarter * 32 + 8 * k + (lane >> 2)) + (lane & 3) * 8;
+                auto emit = [&](bool odd) {
 #pragma unroll 1
-                for (int c = 0; c < DH / 32; ++c) {
-                    float o[32];
-                    if (RT == 2) {
-                        uint32_t r[32];
-                        tg_ld32(tm_o + 32u * c, r);
-                        tg_wait_ld();
+                    for (int c = 0; c < DH / 32; ++c) {
+                        float o[32];
+                        if (RT == 2) {
+                            uint32_t r[32];
+                            tg_ld32(tm_o + 32u * c, r);
+                            tg_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(r[i]) * f0;
-                    } else {
-                        uint32_t r[32], u[32];
-                        tg_ld32(tm_o + 32u * c, r);
-                        tg_ld32(tm_o + 128u + 32u * c, u);
-                        tg_wait_ld();
+                            for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(r[i]) * f0;
+                        } else {
+                            uint32_t r[32], u[32];
+                            tg_ld32(tm_o + 32u * c, r);
+                            tg_ld32(tm_o + 128u + 32u * c, u);
+                            tg_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            o[i] = fmaf(__uint_as_float(r[i]), f0, __uint_as_float(u[i]) * f1);
-                    }
-                    if (nodes | edge) {
-                        for (int k = 0; k < 128; ++k) {
-                            if (!((k < 64 ? nodes >> k : edge >> (k - 64)) & 1ull)) continue;
-                            const int key = k < 64 ? rec.base + k : rec.lo + k - 64;
-                            const int page = block_tables[(size_t)rec.seq * max_blocks + (key >> page_shift)];
-                            const bf16* v = v_cache + (((size_t)page * w.Hkv + rec.kvh) * page_size + (key & (page_size - 1))) * DH + 32 * c;
+                            for (int i = 0; i < 32; ++i) o[i] = fmaf(__uint_as_float(r[i]), f0, __uint_as_float(u[i]) * f1);
+                        }
+                        if (odd) {
+                            for (int k = 0; k < 128; ++k) {
+                                if (!((k < 64 ? nodes >> k : edge >> (k - 64)) & 1ull)) continue;
+                                const int key = k < 64 ? rec.base + k : rec.lo + k - 64;
+                                const int page = block_tables[(size_t)rec.seq * max_blocks + (key >> page_shift)];
+                                const bf16* v = v_cache + (((size_t)page * w.Hkv + rec.kvh) * page_size + (key & (page_size - 1))) * DH + 32 * c;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                const float y = __bfloat162float(v[i]);
-                                if (!isfinite(y)) o[i] += y;
+                                for (int i = 0; i < 32; ++i) {
+                                    const float y = __bfloat162float(v[i]);
+                                    if (!isfinite(y)) o[i] += y;
+                                }
                             }
                         }
-                    }
-                    if (rec.whole) {
-                        // by way of shared memory, so that four lanes store a row's 64 bytes
+                        if (rec.whole) {
+                            // by way of shared memory
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            stage[lane * 4 + ((i ^ (lane >> 1)) & 3)] = make_uint4(tg_pack(o[8 * i], o[8 * i + 1]), tg_pack(o[8 * i + 2], o[8 * i + 3]),
-                                                                         tg_pack(o[8 * i + 4], o[8 * i + 5]), tg_pack(o[8 * i + 6], o[8 * i + 7]));
-                        __syncwarp();
+                            for (int i = 0; i < 4; ++i)
+                                stage[lane * 4 + ((i ^ (lane >> 1)) & 3)] = make_uint4(tg_pack(o[8 * i], o[8 * i + 1]), tg_pack(o[8 * i + 2], o[8 * i + 3]),
+                                                                             tg_pack(o[8 * i + 4], o[8 * i + 5]), tg_pack(o[8 * i + 6], o[8 * i + 7]));
+                            __syncwarp();
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const int line = 8 * k + (lane >> 2), r_out = quarter * 32 + line;
-                            if (r_out < n_rows)
-                                *(uint4*)(result(t * tile_rows + r_out) + 32 * c + (lane & 3) * 8) = stage[line * 4 + ((lane ^ (line >> 1)) & 3)];
+                            for (int k = 0; k < 4; ++k) {
+                                const int line = 8 * k + (lane >> 2);
+                                if (quarter * 32 + line < n_rows) *(uint4*)(line_out[k] + 32 * c) = stage[line * 4 + ((lane ^ (line >> 1)) & 3)];
+                            }
+                            __syncwarp();
+                        } else if (row_ok) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                po[(8 * c + i) * w.rows_per_tile] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                         }
-                        __syncwarp();
-                    } else if (row_ok) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            po[(8 * c + i) * w.rows_per_tile] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
-                }
+                };
+                if (__any_sync(0xffffffffu, (nodes | edge) != 0)) emit(true);
+                else emit(false);
             }
             // these warps are at most two items apart: nobody reads the last item's but three any more, or writes them yet
             if (quarter == 0 && lane == 0) odd_nodes[(walked + 4u) & 7u] = odd_edge[(walked + 4u) & 7u] = 0;
