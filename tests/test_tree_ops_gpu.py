@@ -699,3 +699,9 @@ def test_every_call_runs_on_the_device_of_the_current_stream():
 
 def test_sizes_are_those_the_kernels_state():
     assert ops().TREE_NODES == 64 and math.log2(ops().TREE_NODES) == 6
+
+
+def test_no_wait_ran_out():
+    x, c = constrained(40, 70001, 4, seed=2, history=50)
+    ops().logits_constrain(x, out=torch.empty_like(x), **c)
+    assert not {"logits_constrain", "attention_tree"} & set(ops().kernel_wait_errors())

@@ -320,6 +320,8 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
     }
 }
 
+TGO_API int tgo_logits_constrain_error(int* value) { return (int)cudaMemcpyFromSymbol(value, drafts_error_flag, sizeof(int)); }
+
 // Addresses that are null leave their stage out. strides in elements (words for `allowed`).
 TGO_API int tgo_logits_constrain(const float* logits, long long in_stride, float* out, long long out_stride, int rows, int vocab,
                                  int requests, const int* owner, const int* bias_start, const int* bias_ids, const float* bias,

@@ -7,6 +7,7 @@ nothing falls back to it. A refused size raises with the kernel's name in the me
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from array import array
 from operator import index
@@ -2249,6 +2250,12 @@ _tc_err = {}
 TREE_NODES = 64          # drafted tokens of a request that the kernels take: what a node sees is a 64-bit number
 
 
+@functools.lru_cache(maxsize=256)
+def _tree_work(code: int, head_dim: int, group: int, page_size: int, max_nodes: int) -> int:
+    """Numbers of workspace that calls of these sizes want; a function of the sizes and of the GPU's kind."""
+    return entry_points("attention_tree").tgo_attention_tree_work(code, head_dim, group, page_size, max_nodes)
+
+
 def attention_tree(q: torch.Tensor, out: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int,
                    k_cache: torch.Tensor, v_cache: torch.Tensor, page_size: int, block_tables: torch.Tensor,
                    context_lens: torch.Tensor, q_start: torch.Tensor, seen: torch.Tensor, scale: float, window: int,
@@ -2263,32 +2270,30 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, num_heads: int, num_kv_he
     q, out [T, >= heads * head_dim] float32 or bfloat16, rows may be strided; k_cache, v_cache [pages, kv heads, page_size,
     head_dim] of that type; block_tables int32 [B, width], context_lens int32 [B], q_start int32 [B + 1], seen int64
     [T]. head_dim at most 256. max_nodes, max_context: the most that any request of the call has."""
-    if not (q.is_cuda and out.is_cuda and k_cache.is_cuda and v_cache.is_cuda and block_tables.is_cuda and
-            context_lens.is_cuda and q_start.is_cuda and seen.is_cuda):
-        _need_cuda(q, out, k_cache, v_cache, block_tables, context_lens, q_start, seen)
     T, kind, shape = q.shape[0], q.dtype, k_cache.shape
     B, width = block_tables.shape
     code = dtype_code(kind)
     (qs, q1), (os, o1) = q.stride(), out.stride()
-    assert out.dtype == k_cache.dtype == v_cache.dtype == kind and q1 == o1 == 1 and out.shape[0] == T
+    i32 = torch.int32
+    assert out.dtype is kind and k_cache.dtype is kind and v_cache.dtype is kind and q1 == o1 == 1 and out.shape[0] == T
     assert q.shape[1] >= num_heads * head_dim and out.shape[1] >= num_heads * head_dim
     assert shape[1:] == (num_kv_heads, page_size, head_dim) and v_cache.shape == shape
-    assert k_cache.is_contiguous() and v_cache.is_contiguous()
-    assert block_tables.dtype == context_lens.dtype == q_start.dtype == torch.int32 and seen.dtype == torch.int64
-    assert block_tables.is_contiguous() and context_lens.is_contiguous() and q_start.is_contiguous() and seen.is_contiguous()
-    assert context_lens.shape == (B,) and q_start.shape == (B + 1,) and seen.shape == (T,)
+    assert block_tables.dtype is i32 and context_lens.dtype is i32 and q_start.dtype is i32 and seen.dtype is torch.int64
+    assert context_lens.numel() == B and q_start.numel() == B + 1 and seen.numel() == T
+    if not (q.is_cuda and out.is_cuda):
+        _need_cuda(q, out)
+    tensors = (_flat(k_cache), _flat(v_cache), shape[0], page_size, _flat(block_tables), width, _flat(context_lens), _flat(q_start),
+               _flat(seen), B, num_heads, num_kv_heads, head_dim, window, max_nodes, max_context)
     if not 0 <= max_nodes <= TREE_NODES:
         raise KernelError(f"attention_tree: {max_nodes} drafted tokens of a request; at most {TREE_NODES}")
     if T == 0 or B == 0 or max_nodes == 0:
         return
     lib = entry_points("attention_tree")
-    work = q.new_empty(lib.tgo_attention_tree_work(code, head_dim, num_heads // num_kv_heads, page_size, max_nodes),
-                       dtype=torch.float32)
-    _check(lib.tgo_attention_tree(q.data_ptr(), qs, out.data_ptr(), os, code, T, k_cache.data_ptr(), v_cache.data_ptr(), shape[0],
-                                  page_size, block_tables.data_ptr(), width, context_lens.data_ptr(), q_start.data_ptr(),
-                                  seen.data_ptr(), B, num_heads, num_kv_heads, head_dim, window, max_nodes, max_context,
-                                  work.data_ptr(), _stream(), float(scale)), "attention_tree",
-           f"(head_dim={head_dim}, heads={num_heads}/{num_kv_heads}, page_size={page_size}, window={window})")
+    work = q.new_empty(_tree_work(code, head_dim, num_heads // num_kv_heads, page_size, max_nodes), dtype=torch.float32)
+    status = lib.tgo_attention_tree(q.data_ptr(), qs, out.data_ptr(), os, code, T, *tensors, work.data_ptr(), _stream(),
+                                    float(scale))
+    _check(status, "attention_tree", f"(head_dim={head_dim}, heads={num_heads}/{num_kv_heads}, page_size={page_size}, "
+                                     f"window={window})" if status else "")
     LAUNCHES[0] += 1
 
 
@@ -2305,6 +2310,14 @@ def attention_tree_error() -> int:
     value = ctypes.c_int(0)
     _check(entry_points("attention_tree").tgo_attention_tree_error(ctypes.addressof(value)), "attention_tree_error")
     return int(value.value)
+
+
+def _flat(t: torch.Tensor) -> int:
+    """The address of a contiguous tensor on the device."""
+    if not t.is_cuda:
+        _need_cuda(t)
+    assert t.is_contiguous()
+    return t.data_ptr()
 
 
 def logits_constrain(logits: torch.Tensor, owner: Optional[torch.Tensor] = None, bias=None, history=None,
@@ -2330,48 +2343,63 @@ def logits_constrain(logits: torch.Tensor, owner: Optional[torch.Tensor] = None,
         _need_cuda(logits, out)
     R, V = logits.shape
     (s_in, s1), (s_out, s2) = logits.stride(), out.stride()
-    assert logits.dtype == out.dtype == torch.float32 and out.shape == (R, V) and (V <= 1 or s1 == s2 == 1)
+    i32, f32 = torch.int32, torch.float32
+    assert logits.dtype is f32 and out.dtype is f32 and out.shape == (R, V) and (V <= 1 or s1 == s2 == 1)
     assert R <= 1 or (s_in >= V and s_out >= V)
     at, to = logits.data_ptr(), out.data_ptr()
     if R and V and (s_in != s_out if at == to else
                     at < to + 4 * ((R - 1) * s_out + V) and to < at + 4 * ((R - 1) * s_in + V)):
         raise KernelError("logits_constrain: `out` lies over other rows of the logits; the same rows, or rows of its own")
-    Q = R
-
-    def take(t, kind, shape=None):
-        if not t.is_cuda:
-            _need_cuda(t)
-        assert t.dtype == kind and t.is_contiguous() and (shape is None or t.shape == shape)
-        return t.data_ptr()
-
-    for t in (penalties, windows):
-        if t is not None:
-            Q = t.shape[0]
-    for t in (bias, history, drafts):
-        if t is not None:
-            Q = t[0].shape[0] - 1
-    i32, f32 = torch.int32, torch.float32
-    p_owner = take(owner, i32, (R,)) if owner is not None else 0
-    b0 = b1 = b2 = h0 = h1 = d0 = d1 = d2 = words = m = width = 0
+    # requests: as many as the first array that is given for each of them says
+    Q = penalties.shape[0] if penalties is not None else windows.shape[0] if windows is not None else \
+        history[0].numel() - 1 if history is not None else bias[0].numel() - 1 if bias is not None else \
+        drafts[0].numel() - 1 if drafts is not None else R
+    p_owner = b0 = b1 = b2 = h0 = h1 = d0 = d1 = d2 = p_pen = p_win = words = m = width = p_rows = 0
+    if owner is not None:
+        assert owner.dtype is i32 and owner.numel() == R
+        p_owner = _flat(owner)
     if bias is not None:
-        b0, b1, b2 = take(bias[0], i32, (Q + 1,)), take(bias[1], i32), take(bias[2], f32, bias[1].shape)
+        first, ids, values = bias
+        assert first.dtype is i32 and ids.dtype is i32 and values.dtype is f32 and first.numel() == Q + 1 and \
+            ids.numel() == values.numel()
+        b0, b1, b2 = _flat(first), _flat(ids), _flat(values)
     if history is not None:
-        h0, h1 = take(history[0], i32, (Q + 1,)), take(history[1], i32)
+        first, tokens = history
+        assert first.dtype is i32 and tokens.dtype is i32 and first.numel() == Q + 1
+        h0, h1 = _flat(first), _flat(tokens)
     if drafts is not None:
-        d0, d1, d2 = take(drafts[0], i32, (Q + 1,)), take(drafts[1], i32), take(drafts[2], torch.int64, (R,))
-    p_pen = take(penalties, f32, (Q, 3)) if penalties is not None else 0
-    p_win = take(windows, i32, (Q,)) if windows is not None else 0
+        first, tokens, seen = drafts
+        assert first.dtype is i32 and tokens.dtype is i32 and seen.dtype is torch.int64 and first.numel() == Q + 1 and \
+            seen.numel() == R
+        d0, d1, d2 = _flat(first), _flat(tokens), _flat(seen)
+    if penalties is not None:
+        assert penalties.dtype is f32 and penalties.shape == (Q, 3)
+        p_pen = _flat(penalties)
+    if windows is not None:
+        assert windows.dtype is i32 and windows.numel() == Q
+        p_win = _flat(windows)
     if allowed is not None:
         m, width = allowed.shape
-        words = take(allowed, i32)
+        assert allowed.dtype is i32
+        words = _flat(allowed)
         if width * 32 < V:
             raise KernelError(f"logits_constrain: masks of {width} words for {V} tokens")
-    p_rows = take(allowed_rows, i32, (R,)) if allowed_rows is not None else 0
+    if allowed_rows is not None:
+        assert allowed_rows.dtype is i32 and allowed_rows.numel() == R
+        p_rows = _flat(allowed_rows)
     if R == 0 or V == 0:
         return
-    _check(entry_points("drafts").tgo_logits_constrain(
+    status = entry_points("drafts").tgo_logits_constrain(
         at, s_in, to, s_out, R, V, Q, p_owner, b0, b1, b2, h0, h1, p_pen, p_win, d0, d1, d2, words, width, m, p_rows,
-        _stream()), "logits_constrain", f"(R={R}, V={V})")
+        _stream())
+    _check(status, "logits_constrain", f"(R={R}, V={V})" if status else "")
+
+
+def logits_constrain_error() -> int:
+    """1 if a wait of logits_constrain's copying kernel ran out, else 0. Synchronises with the device."""
+    value = ctypes.c_int(0)
+    _check(entry_points("drafts").tgo_logits_constrain_error(ctypes.addressof(value)), "logits_constrain_error")
+    return int(value.value)
 
 
 def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, chosen: torch.Tensor, q_start: torch.Tensor, path: torch.Tensor,
@@ -2383,19 +2411,16 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, chosen: torch.Tenso
 
     tokens, parents (a node's place in its request; below its own, or -1), chosen, path int32 [T]; q_start int32 [B + 1], at
     most 64 nodes a request; counts, following int32 [B]."""
-    if not (tokens.is_cuda and parents.is_cuda and chosen.is_cuda and q_start.is_cuda and path.is_cuda and counts.is_cuda and
-            following.is_cuda):
-        _need_cuda(tokens, parents, chosen, q_start, path, counts, following)
-    shape, each = tokens.shape, counts.shape
-    assert len(shape) == len(each) == 1 and parents.shape == chosen.shape == path.shape == shape and following.shape == each
-    assert q_start.shape == (each[0] + 1,)
-    for t in (tokens, parents, chosen, q_start, path, counts, following):
-        assert t.dtype == torch.int32 and t.is_contiguous()
-    if each[0] == 0:
+    i32 = torch.int32
+    assert tokens.dtype is i32 and parents.dtype is i32 and chosen.dtype is i32 and q_start.dtype is i32 and path.dtype is i32 \
+        and counts.dtype is i32 and following.dtype is i32
+    T, B = tokens.numel(), counts.numel()
+    assert parents.numel() == chosen.numel() == path.numel() == T and following.numel() == B and q_start.numel() == B + 1
+    args = (_flat(tokens), _flat(parents), _flat(chosen), _flat(q_start), B, _flat(path), _flat(counts), _flat(following))
+    if B == 0:
         return
-    _check(entry_points("drafts").tgo_tree_accept(tokens.data_ptr(), parents.data_ptr(), chosen.data_ptr(), q_start.data_ptr(),
-                                                  each[0], path.data_ptr(), counts.data_ptr(), following.data_ptr(), _stream()),
-           "tree_accept", f"(B={each[0]})")
+    status = entry_points("drafts").tgo_tree_accept(*args, _stream())
+    _check(status, "tree_accept", f"(B={B})" if status else "")
 
 
 def tree_keep(tensors, slots: torch.Tensor, q_start: torch.Tensor, path: torch.Tensor, counts: torch.Tensor, axis: int = 0) -> None:
@@ -2407,12 +2432,11 @@ def tree_keep(tensors, slots: torch.Tensor, q_start: torch.Tensor, path: torch.T
 
     tensors contiguous, all with pages of one size; slots, path int32 [T] (a request's slots distinct), q_start int32
     [B + 1], counts int32 [B]."""
-    if not (slots.is_cuda and q_start.is_cuda and path.is_cuda and counts.is_cuda):
-        _need_cuda(slots, q_start, path, counts)
-    shape, (B,) = slots.shape, counts.shape
-    assert path.shape == shape and q_start.shape == (B + 1,)
-    assert slots.dtype == q_start.dtype == path.dtype == counts.dtype == torch.int32
-    assert slots.is_contiguous() and q_start.is_contiguous() and path.is_contiguous() and counts.is_contiguous()
+    i32 = torch.int32
+    assert slots.dtype is i32 and q_start.dtype is i32 and path.dtype is i32 and counts.dtype is i32
+    B = counts.numel()
+    assert path.numel() == slots.numel() and q_start.numel() == B + 1
+    lists = (_flat(slots), _flat(q_start), B, _flat(path), _flat(counts))
     desc, page_size = array("q"), 0
     for t in tensors:
         if not t.is_cuda:
@@ -2427,9 +2451,8 @@ def tree_keep(tensors, slots: torch.Tensor, q_start: torch.Tensor, path: torch.T
             desc.extend((t.data_ptr(), math.prod(one[:axis]), one[axis], one[axis + 1] if rest == 4 else 1, one[-1] * size))
     if not desc or B == 0:
         return
-    _check(entry_points("drafts").tgo_tree_keep(desc.buffer_info()[0], len(desc) // 5, page_size, slots.data_ptr(),
-                                                q_start.data_ptr(), B, path.data_ptr(), counts.data_ptr(), _stream()),
-           "tree_keep", f"(B={B}, page_size={page_size})")
+    status = entry_points("drafts").tgo_tree_keep(desc.buffer_info()[0], len(desc) // 5, page_size, *lists, _stream())
+    _check(status, "tree_keep", f"(B={B}, page_size={page_size})" if status else "")
     LAUNCHES[0] += (len(desc) // 5 - 1) // 64
 
 
@@ -2525,6 +2548,10 @@ def kernel_wait_errors() -> dict:
         code = attention_tree_error()
         if code:
             out["attention_tree"] = code
+    if "drafts" in _loaded:
+        code = logits_constrain_error()
+        if code:
+            out["logits_constrain"] = code
     if "attention_decode_tma" in _loaded:
         code = attention_decode_tma_error()
         if code:
