@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(LC_THREADS) constrain_kernel(const Constrain a
 #ifndef LS_AHEAD
 #define LS_AHEAD 8                   // tokens of the history that a thread keeps for all the slices of a row
 #endif
+#define LS_NONE (int)0x80000000      // no token: far from every column
 
 __device__ int drafts_error_flag = 0;
 
@@ -190,18 +191,19 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
     float rep = 1.f, presence = 0.f, frequency = 0.f;
     bool counts = false, ok = true;
     const uint32_t* mask = nullptr;
-    int said[LS_AHEAD], drafted = -1, bias_id = -1;            // this thread's first tokens of the history, its drafted one, its
+    int said[LS_AHEAD], drafted = LS_NONE, bias_id = -1;            // this thread's first tokens of the history, its drafted one, its
     float bias_of = 0.f;                                       // first biased one
-    uint32_t next_word[GROUPS];                                // of the mask, for the next slice
-    uint32_t next_more[GROUPS];                                // the words behind them, where four columns lie in two
+    uint32_t next_word[GROUPS] = {};                           // of the mask, for the next slice; where four columns lie in two
+    uint32_t next_more[GROUPS] = {};                           // words, the second ones
     int skip = 0;
-    auto read_mask = [&](int first) {                          // of the columns from there on, four a group
+    const int last_word = a.vocab - 1 >> 5;
+    auto read_mask = [&](int first) {                          // of the columns from there on, four a group; nothing here waits
+        if (!mask) return;                                     // for what is read
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
-            const int c = first + (i * LS_THREADS + tid) * 4, at = c >> 5;
-            next_word[i] = next_more[i] = 0xffffffffu;
-            if (mask && c >= 0 && c < a.vocab) next_word[i] = mask[at];
-            if (mask && skip && (c & 31) > 28 && at + 1 < (a.vocab + 31) >> 5) next_more[i] = mask[at + 1];
+            const int at = first + (i * LS_THREADS + tid) * 4 >> 5;                 // columns outside the row: any word
+            next_word[i] = mask[max(0, min(at, last_word))];
+            if (skip) next_more[i] = mask[max(0, min(at + 1, last_word))];
         }
     };
     for (int k = 0, b = 0, phase = 0; k < todo; ++k) {
@@ -246,8 +248,11 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
                 }
             }
 #pragma unroll
-            for (int j = 0; j < LS_AHEAD; ++j) said[j] = h_lo + j * LS_THREADS + tid < h_hi ? a.history[h_lo + j * LS_THREADS + tid] : -1;
-            drafted = tid < DR_NODES && path >> tid & 1ull ? a.draft_tokens[d_lo + tid] : -1;
+            for (int j = 0; j < LS_AHEAD; ++j) said[j] = h_lo + j * LS_THREADS + tid < h_hi ? a.history[h_lo + j * LS_THREADS + tid] : LS_NONE;
+            drafted = tid < DR_NODES && path >> tid & 1ull ? a.draft_tokens[d_lo + tid] : LS_NONE;
+#pragma unroll
+            for (int j = 0; j < LS_AHEAD; ++j) said[j] = said[j] < 0 ? LS_NONE : said[j];
+            drafted = drafted < 0 ? LS_NONE : drafted;
             bias_id = b_lo + tid < b_hi ? a.bias_ids[b_lo + tid] : -1;
             bias_of = b_lo + tid < b_hi ? a.bias[b_lo + tid] : 0.f;
         }
@@ -255,48 +260,68 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) word[i] = __funnelshift_r(next_word[i], next_more[i], col0 + (i * LS_THREADS + tid) * 4 & 31) & 0xfu;
         if (part + 1 < slices) read_mask(col0 + LS_COLUMNS);
+        const uint32_t width = (uint32_t)max(n_cols, 0);
+        uint32_t here = 0;                                     // which of this thread's tokens the slice has
         if (counts) {
             auto count_in = [&](int token) {
                 const uint32_t c = (uint32_t)(token - col0);
-                if (token >= 0 && c < (uint32_t)max(n_cols, 0)) atomicAdd(&count[c], 1u);
+                if (c < width) atomicAdd(&count[c], 1u);
+                return c < width;
             };
-            count_in(drafted);
+            here = count_in(drafted) ? 1u << LS_AHEAD : 0u;
 #pragma unroll
-            for (int j = 0; j < LS_AHEAD; ++j)
-                if (h_lo + j * LS_THREADS < h_hi) count_in(said[j]);
-            for (int i = h_lo + LS_AHEAD * LS_THREADS + tid; i < h_hi; i += LS_THREADS) count_in(a.history[i]);
+            for (int j = 0; j < LS_AHEAD; ++j) {
+                if (h_lo + j * LS_THREADS >= h_hi) break;
+                if (count_in(said[j])) here |= 1u << j;
+            }
+            for (int i = h_lo + LS_AHEAD * LS_THREADS + tid; i < h_hi; i += LS_THREADS)
+                if (a.history[i] >= 0) count_in(a.history[i]);
         }
         if (ok) ok = tg_wait(&full[b], phase, &drafts_error_flag, 1);
         if (__syncthreads_or(!ok)) break;
         if (b_hi > b_lo) {
             const uint32_t mine = (uint32_t)(bias_id - col0);
-            if (bias_id >= 0 && mine < (uint32_t)max(n_cols, 0)) buf[mine] += bias_of;
+            if (bias_id >= 0 && mine < width) buf[mine] += bias_of;
             for (int i = b_lo + LS_THREADS + tid; i < b_hi; i += LS_THREADS) {
                 const int id = a.bias_ids[i];
                 const uint32_t c = (uint32_t)(id - col0);
-                if (id >= 0 && c < (uint32_t)max(n_cols, 0)) buf[c] += a.bias[i];
+                if (id >= 0 && c < width) buf[c] += a.bias[i];
             }
             __syncthreads();
         }
+        if (counts) {
+            auto edit = [&](int token) {                       // by the first thread that comes for the column
+                const uint32_t c = (uint32_t)(token - col0), n = atomicExch(&count[c], 0u);
+                if (n) buf[c] = lc_edit(buf[c], n, rep, presence, frequency);
+            };
+            for (; here; here &= here - 1) {
+                const int which = __ffs(here) - 1;
+                int token = drafted;
 #pragma unroll
-        for (int i = 0; i < GROUPS; ++i) {
-            const int g = i * LS_THREADS + tid;
-            const uint32_t bits = word[i];
-            const uint4 n = ((const uint4*)count)[g];
-            if (bits == 0xfu && !(n.x | n.y | n.z | n.w)) continue;
-            float4 v = ((const float4*)buf)[g];
-            if (n.x | n.y | n.z | n.w) {
-                ((uint4*)count)[g] = make_uint4(0u, 0u, 0u, 0u);
-                v.x = lc_edit(v.x, n.x, rep, presence, frequency);
-                v.y = lc_edit(v.y, n.y, rep, presence, frequency);
-                v.z = lc_edit(v.z, n.z, rep, presence, frequency);
-                v.w = lc_edit(v.w, n.w, rep, presence, frequency);
+                for (int j = 0; j < LS_AHEAD; ++j)
+                    if (j == which) token = said[j];
+                edit(token);
             }
-            if (!(bits & 1u)) v.x = -INFINITY;
-            if (!(bits & 2u)) v.y = -INFINITY;
-            if (!(bits & 4u)) v.z = -INFINITY;
-            if (!(bits & 8u)) v.w = -INFINITY;
-            ((float4*)buf)[g] = v;
+            for (int i = h_lo + LS_AHEAD * LS_THREADS + tid; i < h_hi; i += LS_THREADS) {
+                const int token = a.history[i];
+                if (token >= 0 && (uint32_t)(token - col0) < width) edit(token);
+            }
+            __syncthreads();                                   // the next slice counts there
+        }
+        if (mask) {
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i) {
+                const int g = i * LS_THREADS + tid;
+                const uint32_t bits = word[i];
+                if (bits == 0xfu) continue;
+                float4 v;
+                if (bits) v = ((const float4*)buf)[g];
+                if (!(bits & 1u)) v.x = -INFINITY;
+                if (!(bits & 2u)) v.y = -INFINITY;
+                if (!(bits & 4u)) v.z = -INFINITY;
+                if (!(bits & 8u)) v.w = -INFINITY;
+                ((float4*)buf)[g] = v;
+            }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
