@@ -446,39 +446,47 @@ template <typename V>
 __global__ void __launch_bounds__(TK_THREADS) keep_kernel(const __grid_constant__ KeepRows a, const int* __restrict__ slots,
                                                           const int* __restrict__ q_start, const int* __restrict__ path,
                                                           const int* __restrict__ counts) {
-    __shared__ int from[DR_NODES], to[DR_NODES];
+    __shared__ long long from[DR_NODES], to[DR_NODES];         // the rows that move, as offsets into a head's pages
+    __shared__ int moves;
     pdl_wait();
     const int b = blockIdx.y, t = blockIdx.z, tid = threadIdx.x;
     const int t0 = q_start[b], n = min(q_start[b + 1] - t0, DR_NODES);
     const int count = min(counts[b], n);
     if (count <= 1) return;
-    const long long rows = (long long)a.pages[t] * a.page_size;
-    if (tid < count) {
-        const int p = path[t0 + tid];
-        int s = p >= tid && p < n ? slots[t0 + p] : -1, d = slots[t0 + tid];
-        if (s < 0 || d < 0 || s >= rows || d >= rows || p == tid) s = d = -1;
-        from[tid] = s;
-        to[tid] = d;
+    if (tid < 32) {
+        const long long rows = (long long)a.pages[t] * a.page_size;
+        auto offset = [&](int slot) {
+            return slot / a.page_size * a.page_stride[t] + (long long)(slot % a.page_size) * a.row_bytes[t];
+        };
+        int kept = 0;
+        for (int j0 = 0; j0 < count; j0 += 32) {
+            const int j = j0 + tid, p = j < count ? path[t0 + j] : -1;
+            const int d = j < count ? slots[t0 + j] : -1, s = p > j && p < n ? slots[t0 + p] : -1;
+            const bool go = s >= 0 && d >= 0 && s < rows && d < rows;
+            const uint32_t going = __ballot_sync(0xffffffffu, go);
+            if (go) {
+                const int at = kept + __popc(going & (1u << tid) - 1u);
+                from[at] = offset(s);
+                to[at] = offset(d);
+            }
+            kept += __popc(going);
+        }
+        if (tid == 0) moves = kept;
     }
     __syncthreads();
-    const int pieces = a.row_bytes[t] / (int)sizeof(V);
-    const long long total = (long long)a.outer[t] * a.heads[t] * pieces;
-    const long long i = (long long)blockIdx.x * TK_THREADS + tid;
-    if (i >= total) return;
-    const int piece = (int)(i % pieces);
-    const long long oh = i / pieces;
-    char* base = a.base[t] + oh / a.heads[t] * a.outer_stride[t] + oh % a.heads[t] * a.head_stride[t] + (size_t)piece * sizeof(V);
-    auto at = [&](int slot) {
-        return (V*)(base + (long long)(slot / a.page_size) * a.page_stride[t] + (long long)(slot % a.page_size) * a.row_bytes[t]);
-    };
-    for (int j = 0; j < count; j += TK_AHEAD) {
+    const uint32_t pieces = (uint32_t)a.row_bytes[t] / (uint32_t)sizeof(V), heads = (uint32_t)a.heads[t];
+    const uint32_t i = blockIdx.x * TK_THREADS + tid, oh = i / pieces, o = oh / heads;
+    if (o >= (uint32_t)a.outer[t]) return;
+    char* base = a.base[t] + o * a.outer_stride[t] + (oh - o * heads) * a.head_stride[t] + (size_t)(i - oh * pieces) * sizeof(V);
+    const int all = moves;
+    for (int j = 0; j < all; j += TK_AHEAD) {
         V v[TK_AHEAD];
 #pragma unroll
         for (int k = 0; k < TK_AHEAD; ++k)
-            if (j + k < count && from[j + k] >= 0) v[k] = *at(from[j + k]);
+            if (j + k < all) v[k] = *(const V*)(base + from[j + k]);
 #pragma unroll
         for (int k = 0; k < TK_AHEAD; ++k)
-            if (j + k < count && from[j + k] >= 0) *at(to[j + k]) = v[k];
+            if (j + k < all) *(V*)(base + to[j + k]) = v[k];
     }
 }
 
@@ -519,7 +527,7 @@ TGO_API int tgo_tree_keep(const long long* desc, int tensors, int page_size, con
             const long long c = ((long long)a.outer[i] * a.heads[i] * (a.row_bytes[i] / width) + TK_THREADS - 1) / TK_THREADS;
             blocks = c > blocks ? c : blocks;
         }
-        if (blocks > 0x7fffff00) return TGO_E_BAD_ARG;
+        if (blocks > 0x7fffffff / TK_THREADS) return TGO_E_BAD_ARG;         // pieces are counted in 32 bits
         int rc;
         if (width == 16) rc = keep_launch<uint4>(a, n, requests, blocks, slots, q_start, path, counts, stream);
         else if (width == 8) rc = keep_launch<uint2>(a, n, requests, blocks, slots, q_start, path, counts, stream);
