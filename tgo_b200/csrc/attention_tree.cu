@@ -199,6 +199,15 @@ __device__ __forceinline__ void tp_copy4(float* dst, const bf16* src, bool there
                                 __uint_as_float(u.y & 0xffff0000u));
 }
 
+// The same, or one by one where four do not lie together; `left` of them belong to the row.
+template <typename T>
+__device__ __forceinline__ void tp_row4(float* dst, const T* src, bool there, bool vectors, int left) {
+    if (vectors) tp_copy4(dst, src, there);
+    else
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e) dst[e] = there && e < left ? to_f32(src[e]) : 0.f;
+}
+
 template <typename T, int DP, int R>
 __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
     const T* __restrict__ q, long long q_stride, T* __restrict__ out, long long out_stride, const T* __restrict__ k_cache,
@@ -226,6 +235,9 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
     __syncthreads();
     TreeWalk<TP_KEYS> walk = s_walk;
     const int G = w.H / w.Hkv;
+    // r / G: r < 64 G, and r G < 2^32
+    const uint32_t by_g = G > 1 ? (uint32_t)((0x100000000ull + G - 1) / G) : 0;
+    auto node_of = [&](int r) { return G > 1 ? (int)__umulhi((uint32_t)r, by_g) : r; };
     const float c = scale * TREE_LOG2E;
     const bool vectors = dh % 4 == 0 && ((uintptr_t)k_cache | (uintptr_t)v_cache) % (4 * sizeof(T)) == 0;
     const bool q_vectors = dh % 4 == 0 && q_stride % 4 == 0 && (uintptr_t)q % (4 * sizeof(T)) == 0;
@@ -236,49 +248,43 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
         const int kvh = walk.kvh;
         const int hi = r.base < 0 ? 0 : min(r.len, w.max_keys);
         const int* bt = block_tables + (size_t)walk.b * max_blocks;
-        // A tile of K or V, a thread the same four columns of every EACH-th row. 32-bit numbers are copied past the registers.
-        auto fill = [&](float* dst, const T* cache, int t) {
+        // A tile of K or V, a thread the same four columns of every EACH-th row: where its rows lie, and their copies. 32-bit
+        // numbers are copied past the registers.
+        int page[PASSES], place[PASSES];
+        auto look = [&](int t) {
             const int key0 = (r.t_lo + t) * TP_KEYS;
-            int page[PASSES], place[PASSES];
 #pragma unroll
             for (int i = 0; i < PASSES; ++i) {
                 const int key = key0 + my_row + i * EACH, nth = page_shift >= 0 ? key >> page_shift : key / page_size;
                 place[i] = key - nth * page_size;
                 page[i] = key < hi ? bt[nth] : -1;
             }
+        };
+        auto copy = [&](float* dst, const T* cache) {
 #pragma unroll
             for (int i = 0; i < PASSES; ++i) {
                 const bool there = page[i] >= 0 && page[i] < n_pages && my_d < dh;
                 const T* at = cache + (there ? (((size_t)page[i] * w.Hkv + kvh) * page_size + place[i]) * dh + my_d : 0);
-                float* to = dst + (my_row + i * EACH) * LD + my_d;
-                if (vectors) tp_copy4(to, at, there);
-                else
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) to[e] = there && my_d + e < dh ? to_f32(at[e]) : 0.f;
+                tp_row4(dst + (my_row + i * EACH) * LD + my_d, at, there, vectors, dh - my_d);
             }
+            asm volatile("cp.async.commit_group;" ::: "memory");
         };
         __syncthreads();                          // the last piece's rows have been read
-#pragma unroll
+        look(walk.from);
         for (int row = my_row; row < ROWS; row += EACH) {
-            const int f = row0 + row;
+            const int f = row0 + row, node = node_of(f);
             const bool there = row < n_rows && my_d < dh;
-            const T* at = q + (there ? (size_t)(r.tok0 + f / G) * q_stride + (size_t)(kvh * G + f % G) * dh + my_d : 0);
-            float* to = sq + row * LD + my_d;
-            if (q_vectors) tp_copy4(to, at, there);
-            else
-#pragma unroll
-                for (int e = 0; e < 4; ++e) to[e] = there && my_d + e < dh ? to_f32(at[e]) : 0.f;
+            const T* at = q + (there ? (size_t)(r.tok0 + node) * q_stride + (size_t)(kvh * G + f - node * G) * dh + my_d : 0);
+            tp_row4(sq + row * LD + my_d, at, there, q_vectors, dh - my_d);
         }
-        fill(sk, k_cache, walk.from);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        fill(sv, v_cache, walk.from);
-        asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) copy(i ? sv : sk, i ? v_cache : k_cache);
         TreeRow see[R];
         float m[R], l[R], o[R][J * 4];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int row = ty * R + i;
-            if (row < n_rows) see[i] = tree_row(w, r, seen, (row0 + row) / G);
+            if (row < n_rows) see[i] = tree_row(w, r, seen, node_of(row0 + row));
             else { see[i].lo = 0x7fffffff; see[i].bits = 0; }
             m[i] = -INFINITY;
             l[i] = 0.f;
@@ -308,8 +314,12 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
                     }
             }
             __syncthreads();                      // K has been read
-            if (t + 1 < walk.to) fill(sk, k_cache, t + 1);
-            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (t + 1 < walk.to) {
+                look(t + 1);
+                copy(sk, k_cache);
+            } else {
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            }
             // all of the tile's keys are seen by every row: cached, behind every window's beginning
             const bool whole = key0 + TP_KEYS <= min(hi, r.base) && (w.window <= 0 || key0 >= r.base + r.n - w.window);
 #pragma unroll
@@ -390,8 +400,12 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
                 }
             }
             __syncthreads();                      // V has been read
-            if (t + 1 < walk.to) fill(sv, v_cache, t + 1);
-            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (t + 1 < walk.to) {
+                look(t + 1);
+                copy(sv, v_cache);
+            } else {
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         const bool whole_item = walk.from == 0 && walk.to == r.tiles;
@@ -406,7 +420,8 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
             if (row >= n_rows) continue;
             if (whole_item) {
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                T* dst = out + (size_t)(r.tok0 + f / G) * out_stride + (size_t)(kvh * G + f % G) * dh;
+                const int node = node_of(f);
+                T* dst = out + (size_t)(r.tok0 + node) * out_stride + (size_t)(kvh * G + f - node * G) * dh;
 #pragma unroll
                 for (int d = 0; d < J * 4; ++d) {
                     const int col = tx * 4 + 64 * (d >> 2) + (d & 3);
