@@ -1306,17 +1306,18 @@ static int tree_tiles(const TreeWork& w, int max_context, int keys) {
 // The tensor cores' four ways, by what they took where they were measured (us; 8 kv heads of 4 query heads, 128 wide, lengths up to 30 %
 // apart; "one" and "two": row tiles an item, "whole" and "cut"):
 //                                   one whole  one cut  two whole  two cut
-//    1 request of  4 nodes,    300       11.7     12.3
-//    1             4,         1000       18.1     13.0
-//   16             8,         2000       30.0     32.2
-//   40             8,         1500       62.8     52.7
-//    4            64,          500       15.1     19.6       21.5     22.8
-//    4            64,        16000      143.8     81.6      254.7     72.7
-//   32            64,         1000       67.7     74.5       60.5     75.9
-//    8            40,         1000       20.7     28.1       30.1     28.3
-// Whole items run in rounds of one an SM: a key tile takes 1.4 us, or 2.2 for two row tiles, an item's beginning and end 2 and 4 where they show
-// once, and 3.5 and 8 in every round of several. Cutting costs 5.5 more (the join) and shares all tiles out evenly, 1.5
-// and 2.3 us each beside the items' beginnings and ends. The cheapest by this count is within 8 % of the fastest measured.
+//    1 request of  4 nodes,    300       10.6     12.1
+//    1             4,         1000       17.0     12.8
+//   16             8,         2000       28.2     31.0
+//   40             8,         1500       57.7     48.8
+//    1            64,         2000       24.8     16.6       41.5     22.1
+//    4            64,         1000       17.5     21.1       26.7     23.9
+//    4            64,        16000      135.4     81.7      258.8     73.2
+//   32            64,         1000       61.4     70.7       54.7     72.4
+//    8            40,         8000       73.6     74.5      129.3     69.3
+// Whole items run in rounds of one an SM; cutting costs a join and a beginning and an end for every piece, and shares all tiles out
+// evenly. Straight lines through 65 such measurements: us for a call, a round or an item of each SM, and a key tile. The cheapest by
+// them is within 11 % of the fastest measured (within 3 % in 63 of the 65).
 static void tree_choose(TreeWork& w, int max_context, int G, int sms) {
     const int tokens = TT_ROWS / G, t = tree_tiles(w, max_context, TT_KEYS);
     double best = 0;
@@ -1325,9 +1326,9 @@ static void tree_choose(TreeWork& w, int max_context, int G, int sms) {
         if (rt == 2 && w.max_nodes <= tokens) break;
         const double items = (double)w.B * w.Hkv * ((w.max_nodes + rt * tokens - 1) / (rt * tokens));
         const double rounds = (double)(long long)((items + sms - 1) / sms);
-        const double whole = rounds * (t * (rt == 1 ? 1.4 : 2.2) + (rounds > 1 ? rt == 1 ? 3.5 : 8.0 : rt == 1 ? 2.0 : 4.0));
-        const double each = items * (t + TREE_OVERHEAD) / sms;
-        const double cut = 5.5 + (each > 1 ? each : 1) * (rt == 1 ? 1.5 : 2.3) + items / sms * (rt == 1 ? 3.0 : 8.0);
+        const double whole = rt == 1 ? 3.2 + rounds * (4.5 + 1.1 * t) : rounds * (10.8 + 1.95 * t) - 1.8;
+        const double each = items * (t + TREE_OVERHEAD) / sms, tiles = each > 1 ? each : 1;
+        const double cut = rt == 1 ? 11.5 + items / sms * 2.5 + tiles * 1.3 : 18.3 + items / sms * 5.0 + tiles * 2.1;
         if (!way || whole < best) { best = whole; way = 2 * rt; }
         if (cut < best) { best = cut; way = 2 * rt + 1; }
     }
