@@ -14,8 +14,6 @@
 // and a captured call fits every step. What is cut leaves an unnormalised sum, a maximum and a sum of exponentials per
 // row in the workspace, at most two of them a worker, and a second kernel joins them, in the order of the keys: equal
 // calls give equal bits.
-#include <mutex>
-#include <unordered_map>
 
 #include "tcgen.cuh"
 
@@ -1207,59 +1205,16 @@ TGO_API int tgo_attention_tree_work(int dtype, int dh, int group, int page_size,
     return sms * 2 * rows * ((dh + 3) / 4 * 4 + 2) + 2 * sms * (int)(sizeof(TreeNote) / sizeof(float));
 }
 
-// The tensor map of a layer's K or V pages, kept by address, rows, page size and width.
-static const CUtensorMap* tree_map_kv(const void* pages, long long rows, int page_size, int dh) {
-    struct Key {
-        const void* pages; long long rows; int page_size, dh;
-        bool operator==(const Key& o) const { return pages == o.pages && rows == o.rows && page_size == o.page_size && dh == o.dh; }
-    };
-    struct Hash {
-        size_t operator()(const Key& k) const {
-            return (size_t)(uintptr_t)k.pages ^ ((size_t)k.rows * 0x9e3779b97f4a7c15ull) ^ ((size_t)k.page_size << 56) ^ ((size_t)k.dh << 48);
-        }
-    };
-    static std::mutex lock;
-    static std::unordered_map<Key, CUtensorMap, Hash> maps;
-    std::lock_guard<std::mutex> hold(lock);
-    const Key key{pages, rows, page_size, dh};
-    auto it = maps.find(key);
-    if (it != maps.end()) return &it->second;
-    CUtensorMap map;
-    if (!tg_map(&map, pages, rows, dh, dh, page_size)) return nullptr;
-    return &maps.emplace(key, map).first->second;
-}
-// ... of query rows [tokens][heads][dh], `stride` apart, in boxes of 64 columns of G heads of box_tokens tokens.
-static const CUtensorMap* tree_map_q(const void* q, long long stride, int tokens, int H, int G, int dh) {
-    struct Key {
-        const void* q; long long stride; int tokens, H, G, dh;
-        bool operator==(const Key& o) const {
-            return q == o.q && stride == o.stride && tokens == o.tokens && H == o.H && G == o.G && dh == o.dh;
-        }
-    };
-    struct Hash {
-        size_t operator()(const Key& k) const {
-            return (size_t)(uintptr_t)k.q * 0x9e3779b97f4a7c15ull ^ ((size_t)k.stride << 32) ^ ((size_t)k.tokens << 12) ^
-                   ((size_t)k.H << 6) ^ (size_t)k.G ^ ((size_t)k.dh << 56);
-        }
-    };
-    static std::mutex lock;
-    static std::unordered_map<Key, CUtensorMap, Hash> maps;
-    std::lock_guard<std::mutex> hold(lock);
-    const Key key{q, stride, tokens, H, G, dh};
-    auto it = maps.find(key);
-    if (it != maps.end()) return &it->second;
+// The tensor map of query rows [tokens][heads][dh], `stride` apart, in boxes of 64 columns of G heads of a row tile's tokens.
+static bool tree_map_q(CUtensorMap* map, const void* q, long long stride, int tokens, int H, int G, int dh) {
     const TgEncodeFn encode = tg_encode();
-    if (!encode) return nullptr;
-    CUtensorMap map;
+    if (!encode) return false;
     const cuuint64_t dims[3] = {(cuuint64_t)dh, (cuuint64_t)H, (cuuint64_t)tokens};
     const cuuint64_t strides[2] = {(cuuint64_t)dh * 2, (cuuint64_t)stride * 2};
     const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(TT_ROWS / G)};
     const cuuint32_t elem[3] = {1, 1, 1};
-    if (encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-        return nullptr;
-    if (maps.size() > 4096) maps.clear();
-    return &maps.emplace(key, map).first->second;
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T>
@@ -1387,17 +1342,17 @@ TGO_API int tgo_attention_tree(const void* q, long long q_stride, void* out, lon
     TreeWork w = {context_lens, q_start, B, T, H, Hkv, window, max_nodes, max_blocks * page_size, 0, 0, 2, 0, 0};
     // units are counted in 32 bits
     if ((double)B * Hkv * ((double)max_nodes * G / 16 + 1) * ((double)max_blocks * page_size / TP_KEYS + 2 + TREE_OVERHEAD) > 2e9) return TGO_E_BAD_ARG;
-    if (dtype == TGO_BF16 && tree_force != 1 && tgo_attention_tree_tc_supports(dh, G, page_size) && q_stride % 8 == 0 && out_stride % 8 == 0 &&
+    if (dtype == TGO_BF16 && tree_force != 1 && tgo_attention_tree_tc_supports(dh, G, page_size) && q_stride % 8 == 0 && q_stride >= (long long)H * dh && out_stride % 8 == 0 &&
         (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)k_cache % 128 == 0 && (uintptr_t)v_cache % 128 == 0 &&
         rows + page_size <= 0x7fffffffll) {
         w.workers = sms;
         tree_choose(w, max_context, G, sms);
         const bool two = w.tokens_per_tile > TT_ROWS / G;
-        const CUtensorMap* mk = tree_map_kv(k_cache, rows, page_size, dh);
-        const CUtensorMap* mv = tree_map_kv(v_cache, rows, page_size, dh);
-        const CUtensorMap* mq = tree_map_q(q, q_stride, T, H, G, dh);
-        if (!mk || !mv || !mq) return TGO_E_BAD_ARG;
-#define TT_GO(DH, RT) return tree_tc_go<DH, RT>(*mk, *mv, *mq, v_cache, n_pages, out, out_stride, page_size, block_tables, max_blocks, seen, scale, w, work, stream)
+        CUtensorMap mk, mv, mq;
+        if (!tg_map(&mk, k_cache, rows, dh, dh, page_size) || !tg_map(&mv, v_cache, rows, dh, dh, page_size) ||
+            !tree_map_q(&mq, q, q_stride, T, H, G, dh))
+            return TGO_E_BAD_ARG;
+#define TT_GO(DH, RT) return tree_tc_go<DH, RT>(mk, mv, mq, v_cache, n_pages, out, out_stride, page_size, block_tables, max_blocks, seen, scale, w, work, stream)
         if (dh == 128) { if (two) TT_GO(128, 2); TT_GO(128, 1); }
         if (two) TT_GO(64, 2);
         TT_GO(64, 1);
