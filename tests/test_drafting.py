@@ -187,6 +187,45 @@ def test_samples_are_drawn_as_without_drafts(emulated, tmp_path):
     assert all(t % 8 != 7 for t in masked)
 
 
+def test_a_grammar_that_ends_on_a_path_nobody_takes(emulated, tmp_path):
+    """What a grammar says behind drafts matters where the request comes there, and then as without drafts."""
+    d, cfg, run = tiny_model(tmp_path, "B")
+    V = cfg["vocab_size"]
+    prompts = prompts_of(V, [6, 7], seed=8)
+    model = cpu_model(d, cfg)
+    free = model.generate(prompts, Policy(max_tokens=12), page_size=8)
+    texts = [p + t for p, t in zip(prompts, free)]
+    asked = []
+
+    def along(out):                          # nothing comes next but on the texts' way
+        asked.append(list(out))
+        return list(range(V)) if any(t[:len(out)] == out for t in free) else []
+
+    pol = Policy(max_tokens=12, allowed=along)
+    assert model.generate_drafted(prompts, pol, nodes=20, drafter=Oracle(texts, 4, 3, V), page_size=8) == free
+    assert model.last_drafts.accepted > 0 and any(all(t[:len(o)] != o for t in free) for o in asked)
+    early = Policy(max_tokens=12, allowed=lambda out: list(range(V)) if len(out) < 5 else [])
+    with pytest.raises(ValueError, match="no token"):
+        model.generate(prompts[:1], early, page_size=8)
+    runner = DraftedGeneration(model.new_engine(page_size=8, num_pages=20, num_slots=1), Oracle(texts, 4, 3, V), nodes=20)
+    req = Request(prompts[0], early)
+    with pytest.raises(ValueError, match="no token"):
+        runner.run([req])
+    assert req.output == free[0][:5]
+
+
+def test_a_grammar_is_asked_once_a_node(emulated, tmp_path):
+    d, cfg, run = tiny_model(tmp_path, "A")
+    V = cfg["vocab_size"]
+    prompts = prompts_of(V, [6], seed=3)
+    model = cpu_model(d, cfg)
+    calls = []
+    pol = Policy(max_tokens=20, allowed=lambda out: calls.append(len(out)))
+    text = prompts[0] + model.generate(prompts, Policy(max_tokens=20), page_size=8)[0]
+    model.generate_drafted(prompts, pol, nodes=12, drafter=Oracle([text], 8, 1, V), page_size=8)
+    assert len(calls) <= 1 + model.last_drafts.steps + model.last_drafts.drafted
+
+
 def test_stop_ids_end_a_path(emulated, tmp_path):
     d, cfg, run = tiny_model(tmp_path, "B")
     V = cfg["vocab_size"]

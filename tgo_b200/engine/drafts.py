@@ -175,11 +175,11 @@ class DraftedGeneration:
 
     def _turn(self, waiting: List[Request], live: List[_Live]) -> None:
         longest = self.engine._longest_path()
-        entries, reports = self._trees(live, longest), []
+        entries, reports, stuck = self._trees(live, longest), [], {}
         while True:
             reqs = [one.request for one in live]
             try:
-                got = self.engine.draft_step(entries, lambda logits, ctx: self._choose(logits, ctx, reqs, entries, reports))
+                got = self.engine.draft_step(entries, lambda logits, ctx: self._choose(logits, ctx, reqs, entries, reports, stuck))
                 break
             except PagesExhausted:
                 if any(len(e.tokens) > 1 for e in entries):
@@ -201,37 +201,41 @@ class DraftedGeneration:
             self.accepted += len(a.path) - 1
             req.sampler.index += len(a.path)
             req.logprobs.extend(r for r in (reports[at + i] for i in a.path) if r is not None)
+            along = [e.tokens[i] for i in a.path[1:]]
+            if at + a.path[-1] in stuck:
+                req.output.extend(along)
+                raise stuck[at + a.path[-1]]
             at += len(e.tokens)
-            self._take(one, [e.tokens[i] for i in a.path[1:]] + [a.following], live)
+            self._take(one, along + [a.following], live)
 
-    def _choose(self, logits, ctx, reqs: Sequence[Request], entries: Sequence[DraftEntry], reports: list):
-        """A token behind every token of every tree, as its request's policy chooses it there."""
+    def _choose(self, logits, ctx, reqs: Sequence[Request], entries: Sequence[DraftEntry], reports: list, stuck: dict):
+        """A token behind every token of every tree, as its request's policy chooses it there. `stuck` gets the rows where a
+        grammar failed behind drafts, and how: that matters if the request comes there."""
         V = logits.shape[1]
         policies, draws, masks, owner = [], [], [], []
         for q, (req, e) in enumerate(zip(reqs, entries)):
             if req.sampler is None:
                 req.sampler = DrawStream(req.policy.seed)
+            first = len(masks)
             said: List[List[int]] = []                       # drafted tokens up to each one
-            for i, p in enumerate(e.parents):
-                said.append(said[p] + [e.tokens[i]] if i else [])
+            reached: List[bool] = []                         # not behind a token that is forbidden or ends the request,
+            for i, p in enumerate(e.parents):                # where a grammar cannot be asked: nobody comes there
+                t = e.tokens[i]
+                said.append(said[p] + [t] if i else [])
+                over = masks[first + p] if i else None
+                reached.append(i == 0 or reached[p] and first + p not in stuck and t not in self.stop_ids and
+                               (over is None or bool(int(over[t // 32]) >> t % 32 & 1)))
                 policies.append(req.policy)
                 draws.append(req.sampler.ahead(len(said[i])))
-                masks.append(req.policy.allowed_words(req.output + said[i], V) if self._may_be(req, said[i]) else None)
+                masks.append(None)
                 owner.append(q)
+                if reached[i] and req.policy.allowed is not None:
+                    try:
+                        masks[-1] = req.policy.allowed_words(req.output + said[i], V)
+                    except Exception as error:
+                        if i == 0:
+                            raise
+                        stuck[first + i] = error
         constrain(logits, [r.policy for r in reqs], [r.prompt + r.output[:-1] if r.policy.penalises else () for r in reqs],
                   masks, owner, (ctx.q_start, ctx.token_ids, ctx.seen))
         return sample_batch(logits, policies, draws, reports=reports, edited=True)
-
-    def _may_be(self, req: Request, said: Sequence[int]) -> bool:
-        """Whether a grammar can be asked what follows these drafts: not behind a token that it forbids or that ends the
-        request, which nobody will choose or go on from."""
-        if req.policy.allowed is None:
-            return False
-        V = self.engine.model.spec.vocab_size
-        for i, t in enumerate(said):
-            if t in self.stop_ids:
-                return False
-            words = req.policy.allowed_words(req.output + list(said[:i]), V)
-            if words is not None and not int(words[t // 32]) >> t % 32 & 1:
-                return False
-        return True
