@@ -509,6 +509,44 @@ def test_constrain_odd_values():
     assert bool((y == -INF).all())
 
 
+@pytest.mark.parametrize("V,first", [(5000, 0), (20003, 1), (151936, 3)])
+def test_constrain_long_histories(V, first):
+    """More tokens than a block's threads keep, many of them alike, others none at all, at every boundary."""
+    x, c = constrained(5, V, 3, seed=V, history=9001, windows=[0, 8000, 4500], nodes=12, bias=1400, allowed=3)
+    tokens = c["history"][1]
+    tokens[::7] = ints([-1, -V, V, 2 ** 31 - 1, -2 ** 31, 5, V - 1]).repeat(tokens.numel())[:tokens[::7].numel()]
+    c["drafts"][1][::5] = -3
+    want = plain_constrain(x, **c).to(DEV)
+    rows = torch.full((5, V + 8), 9.0, device=DEV)
+    src = rows[:, first:V + first]
+    src.copy_(x)
+    kept = torch.full((5, V + 8), 9.0, device=DEV)
+    dst = kept[:, first:V + first]
+    ops().logits_constrain(src, out=dst, **c)
+    assert torch.equal(src, x) and torch.equal(dst == -INF, want == -INF)
+    # 9012 times the frequency penalty's 0.2, and the roundings of `check_constrain`
+    size = x.abs().double() * 2 + 4 * 6 + 1900
+    fine = want != -INF
+    assert bool(((dst.double() - want).abs()[fine] <= 5 * 2.0 ** -24 * size[fine]).all())
+    assert bool((kept[:, :first] == 9).all()) and bool((kept[:, V + first:] == 9).all())
+    ops().logits_constrain(src, **c)
+    assert torch.equal(src, dst)
+
+
+def test_constrain_starts_outside_their_lists():
+    x, c = constrained(3, 700, 3, seed=3, history=30, bias=8, nodes=5, owner=False)
+    lists = {k: [t.clone() for t in c[k]] for k in ("history", "bias", "drafts")}
+    for k in lists:
+        n = c[k][1].numel()
+        c[k][0].copy_(ints([-4, min(3, n), n + 9, 2 ** 31 - 1]))   # -4..: from 0 on; 3..n + 9: to the end; n + 9..: nothing
+        lists[k][0].copy_(ints([0, min(3, n), n, n]))
+    want = plain_constrain(x, **dict(c, **lists)).to(DEV)
+    for out in (torch.empty_like(x), None):
+        got = x.clone()
+        ops().logits_constrain(got, out=out, **c)
+        assert float(((got if out is None else out).double() - want).abs().max()) <= 5 * 2.0 ** -24 * 100
+
+
 def test_constrain_owners_outside_are_left_alone():
     x, c = constrained(4, 777, 2, seed=8, bias=4, history=30)
     c["owner"] = ints([-1, 0, 2, 1])
@@ -599,6 +637,10 @@ def test_accept_a_chain_of_64_and_links_that_are_none():
     assert (path, counts, following) == ([0, 1, 2], [0, 3, 0], [-1, 1, -1])
 
 
+def test_accept_starts_outside():
+    assert run_accept([1] * 4, [-1, 0, 1, 2], [1] * 4, [-3, 2, 9, 12]) == ([0, 1, 0, -1], [2, 1, 0], [1, 1, -1])
+
+
 def test_accept_refusals():
     t, s, c = ints([1, 2]), ints([0, 2]), ints([0])
     with pytest.raises(AssertionError):
@@ -661,6 +703,14 @@ def test_keep_passes_over_what_is_outside():
     ops().tree_keep([], ints([0]), ints([0, 1]), ints([0]), ints([1]))
 
 
+def test_keep_starts_outside():
+    t = torch.randn((8, 4, 6), device=DEV)
+    want = t.clone()
+    want[0, 1] = t[0, 2]
+    ops().tree_keep([t], ints([0, 1, 2]), ints([-5, 3, 40, 2 ** 31 - 1]), ints([0, 2, -1]), ints([3, 3, 3]))
+    assert torch.equal(t, want)
+
+
 def test_keep_more_tensors_than_a_launch_takes():
     tensors = [torch.randn((6, 2, 8, 16), device=DEV) for _ in range(67)]
     want = [t.clone() for t in tensors]
@@ -705,3 +755,46 @@ def test_no_wait_ran_out():
     x, c = constrained(40, 70001, 4, seed=2, history=50)
     ops().logits_constrain(x, out=torch.empty_like(x), **c)
     assert not {"logits_constrain", "attention_tree"} & set(ops().kernel_wait_errors())
+
+
+def test_the_operators_of_a_step_captured_and_replayed():
+    """Constrained rows, the path that their tokens confirm, its rows of a cache moved: one graph, new inputs."""
+    n, V, rng = 9, 5000, random.Random(4)
+    x, c = constrained(2 * n, V, 2, seed=6, history=200, nodes=n, allowed=2 * n)
+    c["owner"] = ints([0] * n + [1] * n)
+    starts, slots = ints([0, n, 2 * n]), ints(rng.sample(range(80), 2 * n))
+    tokens, parents, picked = c["drafts"][1], ints([0] * 2 * n), ints([0] * 2 * n)
+    path, counts, following = ints([0] * 2 * n), ints([0] * 2), ints([0] * 2)
+    cache, out = torch.zeros((3, 5, 2, 16, 32), device=DEV), torch.empty_like(x)
+
+    def step():
+        ops().logits_constrain(x, out=out, **c)
+        picked.copy_(out.argmax(1))
+        ops().tree_accept(tokens, parents, picked, starts, path, counts, following)
+        ops().tree_keep([cache], slots, starts, path, counts, axis=1)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for turn in range(3):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator(device=DEV).manual_seed(turn), device=DEV))
+        trees = [random_parents(rng, n) for _ in range(2)]
+        parents.copy_(ints(sum(trees, [])))
+        c["drafts"][2].copy_(ints(signed(paths_of(trees[0]) + paths_of(trees[1])), torch.int64))
+        c["allowed"].copy_(torch.zeros_like(c["allowed"]))
+        for r in range(2 * n):                                 # a token each, mostly one that was drafted there
+            kids = [i for i, p in enumerate(trees[r // n]) if p == r % n]
+            t = int(tokens[r // n * n + kids[0]]) if kids and turn else rng.randrange(V)
+            c["allowed"][r, t // 32] = signed([1 << t % 32 | (0xffffffff00000000 if t % 32 == 31 else 0)])[0]
+        c["allowed_rows"].copy_(ints(list(range(2 * n))))
+        cache.normal_()
+        old = cache.clone()
+        graph.replay()
+        got = [t.clone() for t in (out, picked, path, counts, following, cache)]
+        assert torch.equal(got[0] == -INF, plain_constrain(x, **c).to(DEV) == -INF)
+        assert tuple(t.tolist() for t in got[2:5]) == plain_accept(tokens.tolist(), parents.tolist(), got[1].tolist(), [0, n, 2 * n])
+        cache.copy_(old)
+        step()
+        assert all(torch.equal(a, b) for a, b in zip(got, (out, picked, path, counts, following, cache)))

@@ -5,6 +5,12 @@
 
 #define DR_NODES 64               // most drafted tokens of a request: a path is a 64-bit number
 
+// Entries start[i] .. start[i + 1] - 1 of a list of n; none of what is outside it.
+__device__ __forceinline__ void dr_span(const int* start, int i, int n, int& lo, int& hi) {
+    lo = min(max(start[i], 0), n);
+    hi = min(max(start[i + 1], lo), n);
+}
+
 // ---------------------------------------------------------------------- logits_constrain
 // Row r of request q = owner[r], token i:
 //   x = logits[r, i] + bias_q(i)
@@ -27,7 +33,7 @@
 struct Constrain {
     const float* logits; float* out;
     long long in_stride, out_stride;
-    int rows, vocab, requests;
+    int rows, vocab, requests, n_bias, n_history, n_drafts;
     const int* owner;
     const int *bias_start, *bias_ids; const float* bias;
     const int *history_start, *history;
@@ -68,15 +74,16 @@ __global__ void __launch_bounds__(LC_THREADS) constrain_kernel(const Constrain a
     float rep = 1.f, presence = 0.f, frequency = 0.f;
     int b_lo = 0, b_hi = 0, h_lo = 0, h_hi = 0, room = 0, d_lo = 0, d_n = 0;
     unsigned long long path = 0;
-    if (owned && a.bias_start) { b_lo = a.bias_start[q]; b_hi = a.bias_start[q + 1]; }
+    if (owned && a.bias_start) dr_span(a.bias_start, q, a.n_bias, b_lo, b_hi);
     if (owned && a.penalties) {
         rep = a.penalties[3 * q]; presence = a.penalties[3 * q + 1]; frequency = a.penalties[3 * q + 2];
-        if (a.history_start) { h_lo = a.history_start[q]; h_hi = a.history_start[q + 1]; }
+        if (a.history_start) dr_span(a.history_start, q, a.n_history, h_lo, h_hi);
         if (a.windows) room = a.windows[q];
         if (a.seen) {
+            int d_hi;
             path = a.seen[r];
-            d_lo = a.draft_start[q];
-            d_n = min(a.draft_start[q + 1] - d_lo, DR_NODES);
+            dr_span(a.draft_start, q, a.n_drafts, d_lo, d_hi);
+            d_n = min(d_hi - d_lo, DR_NODES);
         }
     }
     const bool counts = (rep != 0.f && rep != 1.f) || presence != 0.f || frequency != 0.f;
@@ -229,16 +236,17 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
             int d_lo = 0;
             if (q >= 0 && q < a.requests) {
                 int room = 0;
-                if (a.bias_start) { b_lo = a.bias_start[q]; b_hi = a.bias_start[q + 1]; }
+                if (a.bias_start) dr_span(a.bias_start, q, a.n_bias, b_lo, b_hi);
                 if (a.penalties) {
                     rep = a.penalties[3 * q]; presence = a.penalties[3 * q + 1]; frequency = a.penalties[3 * q + 2];
                     counts = (rep != 0.f && rep != 1.f) || presence != 0.f || frequency != 0.f;
-                    if (a.history_start) { h_lo = a.history_start[q]; h_hi = a.history_start[q + 1]; }
+                    if (a.history_start) dr_span(a.history_start, q, a.n_history, h_lo, h_hi);
                     if (a.windows) room = a.windows[q];
                     if (room <= 0) room = 0x7fffffff;
                     if (a.seen) {
-                        d_lo = a.draft_start[q];
-                        const int n = min(a.draft_start[q + 1] - d_lo, DR_NODES);
+                        int d_hi;
+                        dr_span(a.draft_start, q, a.n_drafts, d_lo, d_hi);
+                        const int n = min(d_hi - d_lo, DR_NODES);
                         path = a.seen[r] & (n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull);
                         const int length = __popcll(path);
                         while (__popcll(path) > room) path &= path - 1;         // the last ones
@@ -350,15 +358,15 @@ TGO_API int tgo_logits_constrain_error(int* value) { return (int)cudaMemcpyFromS
 // Addresses that are null leave their stage out. strides in elements (words for `allowed`).
 TGO_API int tgo_logits_constrain(const float* logits, long long in_stride, float* out, long long out_stride, int rows, int vocab,
                                  int requests, const int* owner, const int* bias_start, const int* bias_ids, const float* bias,
-                                 const int* history_start, const int* history, const float* penalties, const int* windows,
-                                 const int* draft_start, const int* draft_tokens, const void* seen, const void* allowed,
+                                 int n_bias, const int* history_start, const int* history, int n_history, const float* penalties,
+                                 const int* windows, const int* draft_start, const int* draft_tokens, int n_drafts, const void* seen, const void* allowed,
                                  long long allowed_stride, int allowed_rows_n, const int* allowed_rows, cudaStream_t stream) {
     if (rows <= 0 || vocab <= 0) return 0;
     const int slices = (vocab + LC_COLUMNS - 1) / LC_COLUMNS;
     if (rows > 65535 || (rows > 1 && (in_stride < vocab || out_stride < vocab)) || requests < 0 ||
         (allowed && allowed_stride < (vocab + 31) / 32))
         return TGO_E_BAD_ARG;
-    Constrain a = {logits, out, in_stride, out_stride, rows, vocab, requests, owner, bias_start, bias_ids, bias, history_start, history,
+    Constrain a = {logits, out, in_stride, out_stride, rows, vocab, requests, n_bias, n_history, n_drafts, owner, bias_start, bias_ids, bias, history_start, history,
                    penalties, windows, draft_start, draft_tokens, (const unsigned long long*)seen, (const uint32_t*)allowed,
                    allowed_stride, allowed_rows_n, allowed_rows};
     if (logits != out && ((uintptr_t)logits - (uintptr_t)out) % 16 == 0 && (rows == 1 || (in_stride - out_stride) % 4 == 0) &&
@@ -388,11 +396,13 @@ TGO_API int tgo_logits_constrain(const float* logits, long long in_stride, float
 // later node that is its child and holds the token chosen at it.
 __global__ void __launch_bounds__(32) accept_kernel(const int* __restrict__ tokens, const int* __restrict__ parents,
                                                     const int* __restrict__ chosen, const int* __restrict__ q_start,
+                                                    int T,
                                                     int* __restrict__ path, int* __restrict__ counts, int* __restrict__ following) {
     pdl_wait();
     const int b = blockIdx.x, lane = threadIdx.x;
-    const int t0 = q_start[b], all = q_start[b + 1] - t0;
-    const int n = min(all, DR_NODES);
+    int t0, end;
+    dr_span(q_start, b, T, t0, end);
+    const int all = end - t0, n = min(all, DR_NODES);
     int token[2] = {-1, -1}, parent[2] = {-1, -1}, pick[2] = {-1, -1}, mine[2] = {-1, -1};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -421,9 +431,9 @@ __global__ void __launch_bounds__(32) accept_kernel(const int* __restrict__ toke
 }
 
 TGO_API int tgo_tree_accept(const int* tokens, const int* parents, const int* chosen, const int* q_start, int requests,
-                            int* path, int* counts, int* following, cudaStream_t stream) {
+                            int T, int* path, int* counts, int* following, cudaStream_t stream) {
     if (requests <= 0) return 0;
-    return tgo_launch_pdl(accept_kernel, dim3(requests), dim3(32), 0, stream, tokens, parents, chosen, q_start, path, counts, following);
+    return tgo_launch_pdl(accept_kernel, dim3(requests), dim3(32), 0, stream, tokens, parents, chosen, q_start, T, path, counts, following);
 }
 
 // ----------------------------------------------------------------------------- tree_keep
@@ -444,14 +454,15 @@ struct KeepRows {
 
 template <typename V>
 __global__ void __launch_bounds__(TK_THREADS) keep_kernel(const __grid_constant__ KeepRows a, const int* __restrict__ slots,
-                                                          const int* __restrict__ q_start, const int* __restrict__ path,
-                                                          const int* __restrict__ counts) {
+                                                          const int* __restrict__ q_start, int T,
+                                                          const int* __restrict__ path, const int* __restrict__ counts) {
     __shared__ long long from[DR_NODES], to[DR_NODES];         // the rows that move, as offsets into a head's pages
     __shared__ int moves;
     pdl_wait();
     const int b = blockIdx.y, t = blockIdx.z, tid = threadIdx.x;
-    const int t0 = q_start[b], n = min(q_start[b + 1] - t0, DR_NODES);
-    const int count = min(counts[b], n);
+    int t0, end;
+    dr_span(q_start, b, T, t0, end);
+    const int n = min(end - t0, DR_NODES), count = min(counts[b], n);
     if (count <= 1) return;
     if (tid < 32) {
         const long long rows = (long long)a.pages[t] * a.page_size;
@@ -492,14 +503,14 @@ __global__ void __launch_bounds__(TK_THREADS) keep_kernel(const __grid_constant_
 
 template <typename V>
 static int keep_launch(const KeepRows& a, int n, int requests, long long blocks, const int* slots, const int* q_start,
-                       const int* path, const int* counts, cudaStream_t stream) {
-    return tgo_launch_pdl(keep_kernel<V>, dim3((unsigned)blocks, requests, n), dim3(TK_THREADS), 0, stream, a, slots, q_start, path, counts);
+                       int T, const int* path, const int* counts, cudaStream_t stream) {
+    return tgo_launch_pdl(keep_kernel<V>, dim3((unsigned)blocks, requests, n), dim3(TK_THREADS), 0, stream, a, slots, q_start, T, path, counts);
 }
 
 // desc: per tensor five numbers: address, outer count, pages, heads, bytes of a row; all contiguous
 // [outer][pages][heads][page_size][row].
 TGO_API int tgo_tree_keep(const long long* desc, int tensors, int page_size, const int* slots, const int* q_start, int requests,
-                          const int* path, const int* counts, cudaStream_t stream) {
+                          int T, const int* path, const int* counts, cudaStream_t stream) {
     if (tensors <= 0 || requests <= 0) return 0;
     if (page_size <= 0 || requests > 65535) return TGO_E_BAD_ARG;
     for (int first = 0; first < tensors; first += TK_MAX_TENSORS) {
@@ -529,10 +540,10 @@ TGO_API int tgo_tree_keep(const long long* desc, int tensors, int page_size, con
         }
         if (blocks > 0x7fffffff / TK_THREADS) return TGO_E_BAD_ARG;         // pieces are counted in 32 bits
         int rc;
-        if (width == 16) rc = keep_launch<uint4>(a, n, requests, blocks, slots, q_start, path, counts, stream);
-        else if (width == 8) rc = keep_launch<uint2>(a, n, requests, blocks, slots, q_start, path, counts, stream);
-        else if (width == 4) rc = keep_launch<uint32_t>(a, n, requests, blocks, slots, q_start, path, counts, stream);
-        else if (width == 2) rc = keep_launch<uint16_t>(a, n, requests, blocks, slots, q_start, path, counts, stream);
+        if (width == 16) rc = keep_launch<uint4>(a, n, requests, blocks, slots, q_start, T, path, counts, stream);
+        else if (width == 8) rc = keep_launch<uint2>(a, n, requests, blocks, slots, q_start, T, path, counts, stream);
+        else if (width == 4) rc = keep_launch<uint32_t>(a, n, requests, blocks, slots, q_start, T, path, counts, stream);
+        else if (width == 2) rc = keep_launch<uint16_t>(a, n, requests, blocks, slots, q_start, T, path, counts, stream);
         else return TGO_E_BAD_ARG;
         if (rc) return rc;
     }

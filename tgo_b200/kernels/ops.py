@@ -2329,7 +2329,7 @@ def logits_constrain(logits: torch.Tensor, owner: Optional[torch.Tensor] = None,
     added; then, for a token that stands c > 0 times in the last windows[q] tokens (0 or None: all) of its history, and a
     repetition penalty that is neither 0 nor 1, a positive logit is divided by it and another multiplied, and
     presence + frequency * c is taken off; then tokens that row allowed_rows[r] (None: r; outside: no mask) of `allowed`
-    does not name become -inf.
+    does not name become -inf. What of a list lies outside its entries is passed over.
 
     logits, out float32 [R, V], rows may be strided; owner int32 [R]. bias: (int32 starts [Q + 1], int32 ids, float32
     values), a request's ids distinct. history: (int32 starts [Q + 1], int32 tokens). penalties float32 [Q, 3]: repetition,
@@ -2354,7 +2354,7 @@ def logits_constrain(logits: torch.Tensor, owner: Optional[torch.Tensor] = None,
     Q = penalties.shape[0] if penalties is not None else windows.shape[0] if windows is not None else \
         history[0].numel() - 1 if history is not None else bias[0].numel() - 1 if bias is not None else \
         drafts[0].numel() - 1 if drafts is not None else R
-    p_owner = b0 = b1 = b2 = h0 = h1 = d0 = d1 = d2 = p_pen = p_win = words = m = width = p_rows = 0
+    n_bias = n_history = n_drafts = p_owner = b0 = b1 = b2 = h0 = h1 = d0 = d1 = d2 = p_pen = p_win = words = m = width = p_rows = 0
     if owner is not None:
         assert owner.dtype is i32 and owner.numel() == R
         p_owner = _flat(owner)
@@ -2362,16 +2362,16 @@ def logits_constrain(logits: torch.Tensor, owner: Optional[torch.Tensor] = None,
         first, ids, values = bias
         assert first.dtype is i32 and ids.dtype is i32 and values.dtype is f32 and first.numel() == Q + 1 and \
             ids.numel() == values.numel()
-        b0, b1, b2 = _flat(first), _flat(ids), _flat(values)
+        b0, b1, b2, n_bias = _flat(first), _flat(ids), _flat(values), ids.numel()
     if history is not None:
         first, tokens = history
         assert first.dtype is i32 and tokens.dtype is i32 and first.numel() == Q + 1
-        h0, h1 = _flat(first), _flat(tokens)
+        h0, h1, n_history = _flat(first), _flat(tokens), tokens.numel()
     if drafts is not None:
         first, tokens, seen = drafts
         assert first.dtype is i32 and tokens.dtype is i32 and seen.dtype is torch.int64 and first.numel() == Q + 1 and \
             seen.numel() == R
-        d0, d1, d2 = _flat(first), _flat(tokens), _flat(seen)
+        d0, d1, d2, n_drafts = _flat(first), _flat(tokens), _flat(seen), tokens.numel()
     if penalties is not None:
         assert penalties.dtype is f32 and penalties.shape == (Q, 3)
         p_pen = _flat(penalties)
@@ -2390,7 +2390,7 @@ def logits_constrain(logits: torch.Tensor, owner: Optional[torch.Tensor] = None,
     if R == 0 or V == 0:
         return
     status = entry_points("drafts").tgo_logits_constrain(
-        at, s_in, to, s_out, R, V, Q, p_owner, b0, b1, b2, h0, h1, p_pen, p_win, d0, d1, d2, words, width, m, p_rows,
+        at, s_in, to, s_out, R, V, Q, p_owner, b0, b1, b2, n_bias, h0, h1, n_history, p_pen, p_win, d0, d1, n_drafts, d2, words, width, m, p_rows,
         _stream())
     _check(status, "logits_constrain", f"(R={R}, V={V})" if status else "")
 
@@ -2416,7 +2416,7 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, chosen: torch.Tenso
         and counts.dtype is i32 and following.dtype is i32
     T, B = tokens.numel(), counts.numel()
     assert parents.numel() == chosen.numel() == path.numel() == T and following.numel() == B and q_start.numel() == B + 1
-    args = (_flat(tokens), _flat(parents), _flat(chosen), _flat(q_start), B, _flat(path), _flat(counts), _flat(following))
+    args = (_flat(tokens), _flat(parents), _flat(chosen), _flat(q_start), B, T, _flat(path), _flat(counts), _flat(following))
     if B == 0:
         return
     status = entry_points("drafts").tgo_tree_accept(*args, _stream())
@@ -2430,13 +2430,13 @@ def tree_keep(tensors, slots: torch.Tensor, q_start: torch.Tensor, path: torch.T
     page * page_size + offset, and what lies before `axis` is gone through page by page. A path ascends
     (`tree_accept`'s do); an entry of it outside its request or below j, or a place outside the tensor, is passed over.
 
-    tensors contiguous, all with pages of one size; slots, path int32 [T] (a request's slots distinct), q_start int32
+    tensors contiguous and apart, all with pages of one size; slots, path int32 [T] (a request's slots distinct), q_start int32
     [B + 1], counts int32 [B]."""
     i32 = torch.int32
     assert slots.dtype is i32 and q_start.dtype is i32 and path.dtype is i32 and counts.dtype is i32
     B = counts.numel()
     assert path.numel() == slots.numel() and q_start.numel() == B + 1
-    lists = (_flat(slots), _flat(q_start), B, _flat(path), _flat(counts))
+    lists = (_flat(slots), _flat(q_start), B, slots.numel(), _flat(path), _flat(counts))
     desc, page_size = array("q"), 0
     for t in tensors:
         if not t.is_cuda:
