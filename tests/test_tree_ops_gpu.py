@@ -531,6 +531,11 @@ def test_constrain_long_histories(V, first):
     assert bool((kept[:, :first] == 9).all()) and bool((kept[:, V + first:] == 9).all())
     ops().logits_constrain(src, **c)
     assert torch.equal(src, dst)
+    c["allowed"] = c["allowed_rows"] = None                    # in place without masks: only what changes is written
+    src.copy_(x)
+    ops().logits_constrain(src, out=dst, **c)
+    ops().logits_constrain(src, **c)
+    assert torch.equal(src, dst) and bool((rows[:, :first] == 9).all()) and bool((rows[:, V + first:] == 9).all())
 
 
 def test_constrain_starts_outside_their_lists():

@@ -18,15 +18,14 @@ __device__ __forceinline__ void dr_span(const int* start, int i, int n, int& lo,
 //   c > 0:  x = x > 0 ? x / repetition : x * repetition;  x -= presence + frequency * c
 //   not allowed: x = -inf
 // the order and the arithmetic of the sampler's single rows (adjust_kernel of sampling.cu), so that both give the same bits.
-//
-// In place, and where the two matrices' rows lie differently to 16-byte boundaries, a block takes a slice of 8192 columns of a
-// row: it counts the history's tokens that fall into its slice in shared memory (integers: the order of the additions
-// changes nothing), and then edits and stores, a thread a column at a time, in place only what changes. A biased token is left
-// to a second look, when everything else of the slice is done.
+// (Counts are integers: the order of the additions changes nothing.)
 #define LC_THREADS 256
 #define LC_COLUMNS 8192
 #define LC_AHEAD 8                // tokens of the history that a thread reads at once
 #define LC_BIASED 0x80000000u
+#define LC_NONE (int)0x80000000   // no token: far from every column
+#define LI_THREADS 512
+#define LI_COLUMNS 16384
 
 struct Constrain {
     const float* logits; float* out;
@@ -52,83 +51,141 @@ __device__ __forceinline__ float lc_edit(float x, uint32_t count, float rep, flo
     return x;
 }
 
+// What is done to a row beside its mask.
+struct ConstrainRow {
+    int b_lo, b_hi, h_lo, h_hi, d_lo;         // its biases, the history's tokens and the drafted ones that are counted
+    unsigned long long path;                  // (these by bits)
+    float rep, presence, frequency;
+    bool counts;
+    __device__ __forceinline__ void find(const Constrain& a, int r, int q) {           // q: its request
+        b_lo = b_hi = h_lo = h_hi = d_lo = 0;
+        path = 0;
+        counts = false;
+        if (q < 0 || q >= a.requests) return;
+        if (a.bias_start) dr_span(a.bias_start, q, a.n_bias, b_lo, b_hi);
+        if (!a.penalties) return;
+        int room = 0;
+        rep = a.penalties[3 * q]; presence = a.penalties[3 * q + 1]; frequency = a.penalties[3 * q + 2];
+        counts = (rep != 0.f && rep != 1.f) || presence != 0.f || frequency != 0.f;
+        if (a.history_start) dr_span(a.history_start, q, a.n_history, h_lo, h_hi);
+        if (a.windows) room = a.windows[q];
+        if (room <= 0) room = 0x7fffffff;
+        if (a.seen) {
+            int d_hi;
+            dr_span(a.draft_start, q, a.n_drafts, d_lo, d_hi);
+            const int n = min(d_hi - d_lo, DR_NODES);
+            path = a.seen[r] & (n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull);
+            const int length = __popcll(path);
+            while (__popcll(path) > room) path &= path - 1;         // the last ones
+            room -= min(room, length);
+        }
+        if (h_hi - h_lo > room) h_lo = h_hi - room;
+    }
+    // Token `tid` of the path, or none.
+    __device__ __forceinline__ int drafted(const Constrain& a, int tid) const {
+        const int t = tid < DR_NODES && path >> tid & 1ull ? a.draft_tokens[d_lo + tid] : LC_NONE;
+        return t < 0 ? LC_NONE : t;
+    }
+};
+
+__device__ __forceinline__ const uint32_t* lc_mask(const Constrain& a, int r) {
+    if (!a.allowed) return nullptr;
+    const int w = a.allowed_rows ? a.allowed_rows[r] : r;
+    return w >= 0 && w < a.allowed_rows_n ? a.allowed + (size_t)w * a.allowed_stride : nullptr;
+}
+
+// In place and without masks: only columns that change are touched. A block takes a slice of a row. It adds the biases, counts
+// the tokens that fall into its slice in shared memory, and after a barrier a thread comes for each of the tokens it counted,
+// takes the count out, and, if it was the first to come, edits the column.
+//   MEASURED, in a graph of calls: 64 rows of 151936 with histories of 4001 tokens 13.5 us (18.7 by the copying kernel below, which
+// takes the rows over in place where there are masks: 14.9 with masks alone), of 300 5.9; 128 rows, 600 tokens 10.7 (28.2);
+// one row, 700 tokens 2.8. Bound by latency and by every slice's look at the row's whole history: slices of 8192 17.6 and
+// 16.7 us for 13.5 and 10.7, of 32768 17.8 and 14.1.
+__global__ void __launch_bounds__(LI_THREADS) constrain_in_place_kernel(const Constrain a) {
+    extern __shared__ __align__(16) uint32_t li_count[];
+    pdl_wait();
+    const int tid = threadIdx.x, r = blockIdx.y, col0 = blockIdx.x * LI_COLUMNS;
+    const uint32_t width = (uint32_t)min(LI_COLUMNS, a.vocab - col0);
+    float* x = a.out + (long long)r * a.out_stride + col0;
+    ConstrainRow row;
+    row.find(a, r, a.owner ? a.owner[r] : r);
+    for (int i = row.b_lo + tid; i < row.b_hi; i += LI_THREADS) {
+        const int id = a.bias_ids[i];
+        if (id >= 0 && (uint32_t)(id - col0) < width) x[id - col0] += a.bias[i];
+    }
+    if (!row.counts) return;
+    int said[LC_AHEAD];                       // this thread's first tokens
+    const int drafted = row.drafted(a, tid);
+#pragma unroll
+    for (int j = 0; j < LC_AHEAD; ++j) said[j] = row.h_lo + j * LI_THREADS + tid < row.h_hi ? a.history[row.h_lo + j * LI_THREADS + tid] : LC_NONE;
+    for (int i = tid; i < LI_COLUMNS / 4; i += LI_THREADS) ((uint4*)li_count)[i] = make_uint4(0u, 0u, 0u, 0u);
+    __syncthreads();
+    auto all = [&](auto&& each) {             // the tokens of this thread that the slice has, each with its column
+        auto one = [&](int token) {
+            const uint32_t c = (uint32_t)(token - col0);
+            if (token >= 0 && c < width) each(c);
+        };
+        one(drafted);
+#pragma unroll
+        for (int j = 0; j < LC_AHEAD; ++j) one(said[j]);
+        for (int i = row.h_lo + LC_AHEAD * LI_THREADS + tid; i < row.h_hi; i += LI_THREADS) one(a.history[i]);
+    };
+    all([&](uint32_t c) { atomicAdd(&li_count[c], 1u); });
+    __syncthreads();
+    all([&](uint32_t c) {
+        const uint32_t n = atomicExch(&li_count[c], 0u);
+        if (n) x[c] = lc_edit(x[c], n, row.rep, row.presence, row.frequency);
+    });
+}
+
+// Where the two matrices' rows lie differently to 16-byte boundaries: a block copies a slice of a row, a thread a column at a
+// time, with its counts beside it. A biased token is left to a second look, when everything else of the slice is done.
 __global__ void __launch_bounds__(LC_THREADS) constrain_kernel(const Constrain a) {
     __shared__ __align__(16) uint32_t count[LC_COLUMNS];
     pdl_wait();
-    const int tid = threadIdx.x, r = blockIdx.y;
-    const int col0 = blockIdx.x * LC_COLUMNS;
+    const int tid = threadIdx.x, r = blockIdx.y, col0 = blockIdx.x * LC_COLUMNS;
     const int n_cols = min(LC_COLUMNS, a.vocab - col0);
-    const float* src = a.logits + (size_t)r * a.in_stride + col0;
-    float* dst = a.out + (size_t)r * a.out_stride + col0;
-    const bool in_place = a.logits == a.out;
-    const int q = a.owner ? a.owner[r] : r;
-    const uint32_t* words = nullptr;
-    if (a.allowed) {
-        const int w = a.allowed_rows ? a.allowed_rows[r] : r;
-        if (w >= 0 && w < a.allowed_rows_n) words = a.allowed + (size_t)w * a.allowed_stride + (col0 >> 5);
-    }
-    const bool owned = q >= 0 && q < a.requests;
-    if (in_place && !owned && !words) return;
-    float rep = 1.f, presence = 0.f, frequency = 0.f;
-    int b_lo = 0, b_hi = 0, h_lo = 0, h_hi = 0, room = 0, d_lo = 0, d_n = 0;
-    unsigned long long path = 0;
-    if (owned && a.bias_start) dr_span(a.bias_start, q, a.n_bias, b_lo, b_hi);
-    if (owned && a.penalties) {
-        rep = a.penalties[3 * q]; presence = a.penalties[3 * q + 1]; frequency = a.penalties[3 * q + 2];
-        if (a.history_start) dr_span(a.history_start, q, a.n_history, h_lo, h_hi);
-        if (a.windows) room = a.windows[q];
-        if (a.seen) {
-            int d_hi;
-            path = a.seen[r];
-            dr_span(a.draft_start, q, a.n_drafts, d_lo, d_hi);
-            d_n = min(d_hi - d_lo, DR_NODES);
-        }
-    }
-    const bool counts = (rep != 0.f && rep != 1.f) || presence != 0.f || frequency != 0.f;
-    if (in_place && !counts && !words && b_hi <= b_lo) return;
+    const float* src = a.logits + (long long)r * a.in_stride + col0;
+    float* dst = a.out + (long long)r * a.out_stride + col0;
+    ConstrainRow row;
+    row.find(a, r, a.owner ? a.owner[r] : r);
+    const uint32_t* words = lc_mask(a, r);
+    if (words) words += col0 >> 5;
     for (int i = tid; i < LC_COLUMNS / 4; i += LC_THREADS) ((uint4*)count)[i] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
-    if (counts) {
-        if (room <= 0) room = 0x7fffffff;
-        path &= d_n >= 64 ? ~0ull : d_n <= 0 ? 0ull : (1ull << d_n) - 1ull;
-        if (tid < DR_NODES && path >> tid & 1ull && __popcll(path >> tid) <= room) {
-            const int c = a.draft_tokens[d_lo + tid] - col0;
-            if (c >= 0 && c < n_cols) atomicAdd(&count[c], 1u);
-        }
-        room -= min(room, __popcll(path));
-        if (h_hi - h_lo > room) h_lo = h_hi - room;
-        for (int i = h_lo + tid; i < h_hi; i += LC_AHEAD * LC_THREADS) {
+    if (row.counts) {
+        const int d = row.drafted(a, tid) - col0;
+        if (d >= 0 && d < n_cols) atomicAdd(&count[d], 1u);
+        for (int i = row.h_lo + tid; i < row.h_hi; i += LC_AHEAD * LC_THREADS) {
             int c[LC_AHEAD];
 #pragma unroll
-            for (int k = 0; k < LC_AHEAD; ++k) c[k] = i + k * LC_THREADS < h_hi ? a.history[i + k * LC_THREADS] - col0 : -1;
+            for (int k = 0; k < LC_AHEAD; ++k) c[k] = i + k * LC_THREADS < row.h_hi ? a.history[i + k * LC_THREADS] : -1;
 #pragma unroll
             for (int k = 0; k < LC_AHEAD; ++k)
-                if (c[k] >= 0 && c[k] < n_cols) atomicAdd(&count[c[k]], 1u);
+                if (c[k] >= col0 && c[k] - col0 < n_cols) atomicAdd(&count[c[k] - col0], 1u);
         }
     }
-    for (int i = b_lo + tid; i < b_hi; i += LC_THREADS) {
-        const int c = a.bias_ids[i] - col0;
-        if (c >= 0 && c < n_cols) atomicOr(&count[c], LC_BIASED);
+    for (int i = row.b_lo + tid; i < row.b_hi; i += LC_THREADS) {
+        const int id = a.bias_ids[i];
+        if (id >= col0 && id - col0 < n_cols) atomicOr(&count[id - col0], LC_BIASED);
     }
     __syncthreads();
 #pragma unroll 4
     for (int c = tid; c < n_cols; c += LC_THREADS) {
         const bool ok = !words || words[c >> 5] >> (c & 31) & 1u;
         const uint32_t n = count[c];
-        if (n & LC_BIASED) continue;
-        if (!ok) dst[c] = -INFINITY;
-        else if (n || !in_place) dst[c] = lc_edit(src[c], n, rep, presence, frequency);
+        if (!(n & LC_BIASED)) dst[c] = ok ? lc_edit(src[c], n, row.rep, row.presence, row.frequency) : -INFINITY;
     }
-    for (int i = b_lo + tid; i < b_hi; i += LC_THREADS) {
-        const int c = a.bias_ids[i] - col0;
-        if (c < 0 || c >= n_cols) continue;
+    for (int i = row.b_lo + tid; i < row.b_hi; i += LC_THREADS) {
+        const int id = a.bias_ids[i], c = id - col0;
+        if (id < col0 || c >= n_cols) continue;
         const bool ok = !words || words[c >> 5] >> (c & 31) & 1u;
-        dst[c] = ok ? lc_edit(src[c] + a.bias[i], count[c] & ~LC_BIASED, rep, presence, frequency) : -INFINITY;
+        dst[c] = ok ? lc_edit(src[c] + a.bias[i], count[c] & ~LC_BIASED, row.rep, row.presence, row.frequency) : -INFINITY;
     }
 }
 
-// Out of place: persistent blocks take slices one after the other, each a run of them, mostly of one row, whose numbers then
-// stay in registers. A slice comes into shared memory by one bulk copy, asked for while the slice before it is edited, is
+// Out of place, and in place with masks: persistent blocks take slices one after the other, each a run of them, mostly of one row,
+// whose numbers then stay in registers. A slice comes into shared memory by one bulk copy, asked for while the slice before it is edited, is
 // edited there where there is something to edit, and leaves by another: the copies wait for nothing but each other. They go
 // by 16 bytes: a slice begins at a boundary, and what of a first or last 16 bytes belongs to another row is read but not
 // stored. (Both matrices' rows lie alike to the boundaries.)
@@ -144,7 +201,6 @@ __global__ void __launch_bounds__(LC_THREADS) constrain_kernel(const Constrain a
 #define LS_RING 3
 #define LS_COLUMNS 6144              // a slice: a whole number of four columns a thread
 #define LS_AHEAD 8                   // tokens of the history that a thread keeps for all the slices of a row
-#define LS_NONE (int)0x80000000      // no token: far from every column
 
 __device__ int drafts_error_flag = 0;
 
@@ -189,11 +245,11 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
     if (tid == 0)
         while (asked < todo && asked < LS_RING - 2) ask();
     __syncthreads();
-    int b_lo = 0, b_hi = 0, h_lo = 0, h_hi = 0;
-    float rep = 1.f, presence = 0.f, frequency = 0.f;
-    bool counts = false, ok = true;
+    ConstrainRow row;
+    bool ok = true;
+    const bool in_place = a.logits == a.out;
     const uint32_t* mask = nullptr;
-    int said[LS_AHEAD], drafted = LS_NONE, bias_id = -1;            // this thread's first tokens of the history, its drafted one, its
+    int said[LS_AHEAD], drafted = LC_NONE, bias_id = -1;            // this thread's first tokens of the history, its drafted one, its
     float bias_of = 0.f;                                       // first biased one
     uint32_t next_word[GROUPS] = {};                           // of the mask, for the next slice; where four columns lie in two
     uint32_t next_more[GROUPS] = {};                           // words, the second ones
@@ -219,45 +275,16 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
         const int col0 = part * LS_COLUMNS - skip, n_cols = min(LS_COLUMNS, a.vocab - col0);       // to the slice's first place
         if (k == 0 || part == 0) {                             // another row
             const int q = a.owner ? a.owner[r] : r;
-            mask = nullptr;
-            if (a.allowed) {
-                const int w = a.allowed_rows ? a.allowed_rows[r] : r;
-                if (w >= 0 && w < a.allowed_rows_n) mask = a.allowed + (size_t)w * a.allowed_stride;
-            }
+            mask = lc_mask(a, r);
             read_mask(col0);
-            b_lo = b_hi = h_lo = h_hi = 0;
-            counts = false;
-            unsigned long long path = 0;                       // drafted tokens of the row's history
-            int d_lo = 0;
-            if (q >= 0 && q < a.requests) {
-                int room = 0;
-                if (a.bias_start) dr_span(a.bias_start, q, a.n_bias, b_lo, b_hi);
-                if (a.penalties) {
-                    rep = a.penalties[3 * q]; presence = a.penalties[3 * q + 1]; frequency = a.penalties[3 * q + 2];
-                    counts = (rep != 0.f && rep != 1.f) || presence != 0.f || frequency != 0.f;
-                    if (a.history_start) dr_span(a.history_start, q, a.n_history, h_lo, h_hi);
-                    if (a.windows) room = a.windows[q];
-                    if (room <= 0) room = 0x7fffffff;
-                    if (a.seen) {
-                        int d_hi;
-                        dr_span(a.draft_start, q, a.n_drafts, d_lo, d_hi);
-                        const int n = min(d_hi - d_lo, DR_NODES);
-                        path = a.seen[r] & (n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull);
-                        const int length = __popcll(path);
-                        while (__popcll(path) > room) path &= path - 1;         // the last ones
-                        room -= min(room, length);
-                    }
-                    if (h_hi - h_lo > room) h_lo = h_hi - room;
-                }
-            }
+            row.find(a, r, q);
 #pragma unroll
-            for (int j = 0; j < LS_AHEAD; ++j) said[j] = h_lo + j * LS_THREADS + tid < h_hi ? a.history[h_lo + j * LS_THREADS + tid] : LS_NONE;
-            drafted = tid < DR_NODES && path >> tid & 1ull ? a.draft_tokens[d_lo + tid] : LS_NONE;
+            for (int j = 0; j < LS_AHEAD; ++j) said[j] = row.h_lo + j * LS_THREADS + tid < row.h_hi ? a.history[row.h_lo + j * LS_THREADS + tid] : LC_NONE;
+            drafted = row.drafted(a, tid);
 #pragma unroll
-            for (int j = 0; j < LS_AHEAD; ++j) said[j] = said[j] < 0 ? LS_NONE : said[j];
-            drafted = drafted < 0 ? LS_NONE : drafted;
-            bias_id = b_lo + tid < b_hi ? a.bias_ids[b_lo + tid] : -1;
-            bias_of = b_lo + tid < b_hi ? a.bias[b_lo + tid] : 0.f;
+            for (int j = 0; j < LS_AHEAD; ++j) said[j] = said[j] < 0 ? LC_NONE : said[j];
+            bias_id = row.b_lo + tid < row.b_hi ? a.bias_ids[row.b_lo + tid] : -1;
+            bias_of = row.b_lo + tid < row.b_hi ? a.bias[row.b_lo + tid] : 0.f;
         }
         uint32_t word[GROUPS];
 #pragma unroll
@@ -265,7 +292,7 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
         if (part + 1 < slices) read_mask(col0 + LS_COLUMNS);
         const uint32_t width = (uint32_t)max(n_cols, 0);
         uint32_t here = 0;                                     // which of this thread's tokens the slice has
-        if (counts) {
+        if (row.counts) {
             auto count_in = [&](int token) {
                 const uint32_t c = (uint32_t)(token - col0);
                 if (c < width) atomicAdd(&count[c], 1u);
@@ -274,28 +301,28 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
             here = count_in(drafted) ? 1u << LS_AHEAD : 0u;
 #pragma unroll
             for (int j = 0; j < LS_AHEAD; ++j) {
-                if (h_lo + j * LS_THREADS >= h_hi) break;
+                if (row.h_lo + j * LS_THREADS >= row.h_hi) break;
                 if (count_in(said[j])) here |= 1u << j;
             }
-            for (int i = h_lo + LS_AHEAD * LS_THREADS + tid; i < h_hi; i += LS_THREADS)
+            for (int i = row.h_lo + LS_AHEAD * LS_THREADS + tid; i < row.h_hi; i += LS_THREADS)
                 if (a.history[i] >= 0) count_in(a.history[i]);
         }
         if (ok) ok = tg_wait(&full[b], phase, &drafts_error_flag, 1);
         if (__syncthreads_or(!ok)) break;
-        if (b_hi > b_lo) {
+        if (row.b_hi > row.b_lo) {
             const uint32_t mine = (uint32_t)(bias_id - col0);
             if (bias_id >= 0 && mine < width) buf[mine] += bias_of;
-            for (int i = b_lo + LS_THREADS + tid; i < b_hi; i += LS_THREADS) {
+            for (int i = row.b_lo + LS_THREADS + tid; i < row.b_hi; i += LS_THREADS) {
                 const int id = a.bias_ids[i];
                 const uint32_t c = (uint32_t)(id - col0);
                 if (id >= 0 && c < width) buf[c] += a.bias[i];
             }
             __syncthreads();
         }
-        if (counts) {
+        if (row.counts) {
             auto edit = [&](int token) {                       // by the first thread that comes for the column
                 const uint32_t c = (uint32_t)(token - col0), n = atomicExch(&count[c], 0u);
-                if (n) buf[c] = lc_edit(buf[c], n, rep, presence, frequency);
+                if (n) buf[c] = lc_edit(buf[c], n, row.rep, row.presence, row.frequency);
             };
             for (; here; here &= here - 1) {
                 const int which = __ffs(here) - 1;
@@ -305,11 +332,11 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
                     if (j == which) token = said[j];
                 edit(token);
             }
-            for (int i = h_lo + LS_AHEAD * LS_THREADS + tid; i < h_hi; i += LS_THREADS) {
+            for (int i = row.h_lo + LS_AHEAD * LS_THREADS + tid; i < row.h_hi; i += LS_THREADS) {
                 const int token = a.history[i];
                 if (token >= 0 && (uint32_t)(token - col0) < width) edit(token);
             }
-            __syncthreads();                                   // the next slice counts there
+            __syncthreads();                                   // the next slice row.counts there
         }
         if (mask) {
 #pragma unroll
@@ -331,11 +358,12 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
         float* dst = a.out + (long long)r * a.out_stride + col0;
         // whole 16 bytes by a copy, what is before and behind them one by one
         const int lo = part == 0 ? skip : 0, lo4 = lo + 3 & ~3, hi4 = max(n_cols, 0) & ~3;
+        const bool same = in_place && !mask && !row.counts && row.b_hi <= row.b_lo;                       // as it lies there
         if (tid == 0) {
-            if (hi4 > lo4) ls_store(dst + lo4, buf + lo4, (uint32_t)(hi4 - lo4) * 4u);
+            if (hi4 > lo4 && !same) ls_store(dst + lo4, buf + lo4, (uint32_t)(hi4 - lo4) * 4u);
             else asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
-        if (tid >= 32 && tid < 40) {
+        if (tid >= 32 && tid < 40 && !same) {
             const int c = tid < 36 ? lo + tid - 32 : max(hi4, lo4) + tid - 36;
             if (tid < 36 ? c < min(lo4, n_cols) : c < n_cols) dst[c] = buf[c];
         }
@@ -358,13 +386,13 @@ TGO_API int tgo_logits_constrain(const float* logits, long long in_stride, float
                                  long long allowed_stride, int allowed_rows_n, const int* allowed_rows, cudaStream_t stream) {
     if (rows <= 0 || vocab <= 0) return 0;
     const int slices = (vocab + LC_COLUMNS - 1) / LC_COLUMNS;
-    if (rows > 65535 || (rows > 1 && (in_stride < vocab || out_stride < vocab)) || requests < 0 ||
+    if (rows > 65535 || (rows > 1 && (in_stride < vocab || out_stride < vocab || (logits == out && in_stride != out_stride))) || requests < 0 ||
         (allowed && allowed_stride < (vocab + 31) / 32))
         return TGO_E_BAD_ARG;
     Constrain a = {logits, out, in_stride, out_stride, rows, vocab, requests, n_bias, n_history, n_drafts, owner, bias_start, bias_ids, bias, history_start, history,
                    penalties, windows, draft_start, draft_tokens, (const unsigned long long*)seen, (const uint32_t*)allowed,
                    allowed_stride, allowed_rows_n, allowed_rows};
-    if (logits != out && ((uintptr_t)logits - (uintptr_t)out) % 16 == 0 && (rows == 1 || (in_stride - out_stride) % 4 == 0) &&
+    if ((logits != out || allowed) && ((uintptr_t)logits - (uintptr_t)out) % 16 == 0 && (rows == 1 || (in_stride - out_stride) % 4 == 0) &&
         (long long)rows * ((vocab + 3) / LS_COLUMNS + 1) <= 0x7fffffffll) {
         constexpr size_t smem = (LS_RING + 1) * LS_COLUMNS * sizeof(float) + LS_RING * 8;
         static bool set[64] = {};
@@ -382,6 +410,21 @@ TGO_API int tgo_logits_constrain(const float* logits, long long in_stride, float
         const int cuts = (vocab + (even ? 0 : 3) + LS_COLUMNS - 1) / LS_COLUMNS;
         const int units = rows * cuts, blocks = LS_BLOCKS * tgo_multiprocessors();
         return tgo_launch_pdl(constrain_stream_kernel, dim3(units < blocks ? units : blocks), dim3(LS_THREADS), smem, stream, a, cuts);
+    }
+    if (logits == out && !allowed) {
+        constexpr size_t smem = LI_COLUMNS * sizeof(uint32_t);
+        static bool set[64] = {};
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return (int)e;
+        if (dev < 0 || dev >= 64) return TGO_E_BAD_ARG;
+        if (!set[dev]) {
+            e = cudaFuncSetAttribute(constrain_in_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e != cudaSuccess) return (int)e;
+            set[dev] = true;
+        }
+        if (!bias_start && !penalties) return 0;
+        return tgo_launch_pdl(constrain_in_place_kernel, dim3((vocab + LI_COLUMNS - 1) / LI_COLUMNS, rows), dim3(LI_THREADS), smem, stream, a);
     }
     return tgo_launch_pdl(constrain_kernel, dim3(slices, rows), dim3(LC_THREADS), 0, stream, a);
 }
