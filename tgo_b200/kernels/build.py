@@ -13,6 +13,9 @@ from __future__ import annotations
 
 import ctypes
 import hashlib
+import importlib.machinery
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -26,6 +29,20 @@ CSRC = os.path.normpath(os.path.join(os.path.dirname(__file__), "..", "csrc"))
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--shared", "-Xcompiler", "-fPIC",
               "-Xcompiler", "-fvisibility=hidden"] + os.environ.get("TGO_NVCC_DEFS", "").split()
+
+
+
+def _torch_flags():
+    """Against torch's own headers and libraries, and named by its version."""
+    try:
+        root = importlib.util.find_spec("torch").submodule_search_locations[0]
+        version = importlib.metadata.version("torch")
+    except (AttributeError, ValueError, importlib.metadata.PackageNotFoundError):
+        return []
+    lib = os.path.join(root, "lib")
+    return ["-I", os.path.join(root, "include"), "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+            f'-DTGO_TORCH="{version}"', "-L", lib, f"-Wl,-rpath,{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+
 
 # library name -> (sources, extra link flags)
 LIBRARIES = {
@@ -56,9 +73,11 @@ LIBRARIES = {
     "host_runtime": (["host_runtime.cpp"], []),
     # calls of the other libraries' entry points (a Python extension; see `entry_points`)
     "fastcall": (["fastcall.cpp"], []),
+    # what a wrapper asks of its tensors (a Python extension; see `tensor_reader`)
+    "tensors": (["tensors.cpp"], _torch_flags()),
 }
-OPTIONAL = ("fastcall",)         # the package runs without, a little slower
-PYTHON_LIBRARIES = ("fastcall",)  # compiled against the Python headers: good for one binary interface
+OPTIONAL = ("fastcall", "tensors")         # the package runs without, a little slower
+PYTHON_LIBRARIES = ("fastcall", "tensors")  # compiled against the Python headers: good for one binary interface
 HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"]
 PYTHON_INCLUDE = sysconfig.get_paths()["include"]
 
@@ -244,6 +263,25 @@ def _bind_ctypes(fn):
     return call
 
 
+def _extension(name: str):
+    """A library that is a Python extension, as a module."""
+    loader = importlib.machinery.ExtensionFileLoader(f"tgo_{name}", compile_library(name))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader(f"tgo_{name}", loader))
+    loader.exec_module(module)
+    return module
+
+
+def tensor_reader():
+    """The extension that reads what wrappers ask of their tensors (`look`, `rows`), or None where it does not build or
+    load."""
+    try:
+        with _lock:
+            return _extension("tensors")
+    except (KernelBuildError, ImportError, OSError) as e:
+        _say(f"[tgo_b200] tensors are read from Python: {str(e)[:500]}")
+        return None
+
+
 _binder = None
 _entries = {}
 
@@ -255,13 +293,8 @@ def _find_binder():
     if platform.machine() != "x86_64" or not sys.platform.startswith("linux") or \
             not os.path.exists(os.path.join(PYTHON_INCLUDE, "Python.h")):
         return _bind_ctypes
-    import importlib.machinery
-    import importlib.util
     try:
-        path = compile_library("fastcall")
-        loader = importlib.machinery.ExtensionFileLoader("tgo_fastcall", path)
-        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("tgo_fastcall", loader))
-        loader.exec_module(module)
+        module = _extension("fastcall")
     except (KernelBuildError, ImportError, OSError) as e:
         _say(f"[tgo_b200] the kernels are called by ctypes: {str(e)[:500]}")
         return _bind_ctypes

@@ -15,7 +15,7 @@ from typing import Optional
 
 import torch
 
-from .build import entry_points, load_library
+from .build import entry_points, load_library, tensor_reader
 
 F32, BF16 = 0, 1
 _CODES = {torch.float32: F32, torch.bfloat16: BF16}
@@ -53,6 +53,64 @@ def _need_cuda(*tensors) -> None:
         if t is not None and not t.is_cuda:
             raise KernelError("the kernels run on a CUDA device only; got a tensor on "
                               f"{t.device}. There is no CPU path.")
+
+
+_KINDS = {"i": torch.int32, "l": torch.int64, "f": torch.float32, "b": torch.bfloat16}
+
+
+def _look(kinds: str, *tensors):
+    """[addresses..., counts of numbers...] of contiguous tensors on the device, each of the type that its letter
+    of `kinds` names (_KINDS); 0 and 0 for None. None instead if one is not such a tensor (`_refuse` says which)."""
+    _find_reader()
+    return _look(kinds, *tensors)
+
+
+def _rows(t: torch.Tensor):
+    """(rows, columns, stride of a row, stride of a column, address) of a matrix on the device, or None."""
+    _find_reader()
+    return _rows(t)
+
+
+def _pages(t: torch.Tensor, axis: int):
+    """(places of a page, numbers, address, what lies before the pages, pages, heads, bytes of a row) of a contiguous
+    tensor on the device whose pages lie along `axis`, or None."""
+    _find_reader()
+    return _pages(t, axis)
+
+
+def _find_reader() -> None:
+    """From the first call on, the extension reads tensors, or, where there is none, Python."""
+    global _look, _rows, _pages
+    reader = tensor_reader()
+    _look, _rows, _pages = (reader.look, reader.rows, reader.pages) if reader else (_look_plain, _rows_plain, _pages_plain)
+
+
+def _look_plain(kinds: str, *tensors):
+    if any(t is not None and not (t.is_cuda and t.dtype is _KINDS[k] and t.is_contiguous()) for k, t in zip(kinds, tensors)):
+        return None
+    return [0 if t is None else t.data_ptr() for t in tensors] + [0 if t is None else t.numel() for t in tensors]
+
+
+def _rows_plain(t: torch.Tensor):
+    return (*t.shape, *t.stride(), t.data_ptr()) if t.is_cuda and t.dim() == 2 else None
+
+
+def _pages_plain(t: torch.Tensor, axis: int):
+    size = t.shape
+    rest = len(size) - axis
+    if axis < 0 or rest not in (3, 4) or not t.is_cuda or not t.is_contiguous():
+        return None
+    return (size[-2], t.numel(), t.data_ptr(), math.prod(size[:axis]), size[axis], size[axis + 1] if rest == 4 else 1,
+            size[-1] * t.element_size())
+
+
+def _refuse(kinds: str, *tensors) -> None:
+    """Why `_look` or `_rows` gave None."""
+    _need_cuda(*tensors)
+    for k, t in zip(kinds, tensors):
+        assert t is None or t.dtype is _KINDS[k], f"a tensor of {t.dtype} for one of {_KINDS[k]}"
+        assert t is None or t.is_contiguous(), "a tensor is not contiguous"
+    raise AssertionError("a tensor is no matrix")
 
 
 LAUNCHES = [0]        # kernels of this package launched so far (graph replays add theirs)
@@ -2270,28 +2328,30 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, num_heads: int, num_kv_he
     q, out [T, >= heads * head_dim] float32 or bfloat16, rows may be strided; k_cache, v_cache [pages, kv heads, page_size,
     head_dim] of that type; block_tables int32 [B, width], context_lens int32 [B], q_start int32 [B + 1], seen int64
     [T]. head_dim at most 256. max_nodes, max_context: the most that any request of the call has."""
-    T, kind, shape = q.shape[0], q.dtype, k_cache.shape
-    B, width = block_tables.shape
+    kind, shape = q.dtype, k_cache.shape
     code = dtype_code(kind)
-    (qs, q1), (os, o1) = q.stride(), out.stride()
-    i32 = torch.int32
-    assert out.dtype is kind and k_cache.dtype is kind and v_cache.dtype is kind and q1 == o1 == 1 and out.shape[0] == T
-    assert q.shape[1] >= num_heads * head_dim and out.shape[1] >= num_heads * head_dim
-    assert shape[1:] == (num_kv_heads, page_size, head_dim) and v_cache.shape == shape
-    assert block_tables.dtype is i32 and context_lens.dtype is i32 and q_start.dtype is i32 and seen.dtype is torch.int64
-    assert context_lens.numel() == B and q_start.numel() == B + 1 and seen.numel() == T
-    if not (q.is_cuda and out.is_cuda):
+    kinds = "ffiiil" if code == F32 else "bbiiil"
+    got = _look(kinds, k_cache, v_cache, block_tables, context_lens, q_start, seen)
+    q_rows, out_rows = _rows(q), _rows(out)
+    if got is None or q_rows is None or out_rows is None:
         _need_cuda(q, out)
-    tensors = (_flat(k_cache), _flat(v_cache), shape[0], page_size, _flat(block_tables), width, _flat(context_lens), _flat(q_start),
-               _flat(seen), B, num_heads, num_kv_heads, head_dim, window, max_nodes, max_context)
+        _refuse(kinds, k_cache, v_cache, block_tables, context_lens, q_start, seen)
+    (T, q_width, qs, q1, p_q), (o_T, o_width, os, o1, p_out) = q_rows, out_rows
+    k, v, tables, lens, first, bits, _, _, _, n_lens, n_first, n_bits = got
+    B, width = block_tables.shape
+    assert out.dtype is kind and q1 == o1 == 1 and o_T == T
+    assert q_width >= num_heads * head_dim and o_width >= num_heads * head_dim
+    assert shape[1:] == (num_kv_heads, page_size, head_dim) and v_cache.shape == shape
+    assert n_lens == B and n_first == B + 1 and n_bits == T
     if not 0 <= max_nodes <= TREE_NODES:
         raise KernelError(f"attention_tree: {max_nodes} drafted tokens of a request; at most {TREE_NODES}")
     if T == 0 or B == 0 or max_nodes == 0:
         return
     lib = entry_points("attention_tree")
     work = q.new_empty(_tree_work(code, head_dim, num_heads // num_kv_heads, page_size, max_nodes), dtype=torch.float32)
-    status = lib.tgo_attention_tree(q.data_ptr(), qs, out.data_ptr(), os, code, T, *tensors, work.data_ptr(), _stream(),
-                                    float(scale))
+    status = lib.tgo_attention_tree(p_q, qs, p_out, os, code, T, k, v, shape[0], page_size, tables, width, lens, first, bits, B,
+                                    num_heads, num_kv_heads, head_dim, window, max_nodes, max_context, work.data_ptr(),
+                                    _stream(), float(scale))
     _check(status, "attention_tree", f"(head_dim={head_dim}, heads={num_heads}/{num_kv_heads}, page_size={page_size}, "
                                      f"window={window})" if status else "")
     LAUNCHES[0] += 1
@@ -2310,14 +2370,6 @@ def attention_tree_error() -> int:
     value = ctypes.c_int(0)
     _check(entry_points("attention_tree").tgo_attention_tree_error(ctypes.addressof(value)), "attention_tree_error")
     return int(value.value)
-
-
-def _flat(t: torch.Tensor) -> int:
-    """The address of a contiguous tensor on the device."""
-    if not t.is_cuda:
-        _need_cuda(t)
-    assert t.is_contiguous()
-    return t.data_ptr()
 
 
 def logits_constrain(logits: torch.Tensor, owner: Optional[torch.Tensor] = None, bias=None, history=None,
@@ -2339,59 +2391,46 @@ def logits_constrain(logits: torch.Tensor, owner: Optional[torch.Tensor] = None,
     vocabulary are passed over."""
     if out is None:
         out = logits
-    if not (logits.is_cuda and out.is_cuda):
-        _need_cuda(logits, out)
-    R, V = logits.shape
-    (s_in, s1), (s_out, s2) = logits.stride(), out.stride()
-    i32, f32 = torch.int32, torch.float32
-    assert logits.dtype is f32 and out.dtype is f32 and out.shape == (R, V) and (V <= 1 or s1 == s2 == 1)
+    matrix = _rows(logits)
+    into = matrix if out is logits else _rows(out)
+    if matrix is None or into is None:
+        _refuse("ff", logits, out)
+    (R, V, s_in, s1, at), (o_R, o_V, s_out, s2, to) = matrix, into
+    f32 = torch.float32
+    assert logits.dtype is f32 and out.dtype is f32 and o_R == R and o_V == V and (V <= 1 or s1 == s2 == 1)
     assert R <= 1 or (s_in >= V and s_out >= V)
-    at, to = logits.data_ptr(), out.data_ptr()
     if R and V and (s_in != s_out if at == to else
                     at < to + 4 * ((R - 1) * s_out + V) and to < at + 4 * ((R - 1) * s_in + V)):
         raise KernelError("logits_constrain: `out` lies over other rows of the logits; the same rows, or rows of its own")
+    b_first, ids, values = bias if bias is not None else (None, None, None)
+    h_first, said = history if history is not None else (None, None)
+    d_first, drafted, seen = drafts if drafts is not None else (None, None, None)
+    tensors = (owner, b_first, ids, values, h_first, said, penalties, windows, d_first, drafted, seen, allowed, allowed_rows)
+    got = _look("iiifiifiiilii", *tensors)
+    if got is None:
+        _refuse("iiifiifiiilii", *tensors)
+    (p_owner, b0, b1, b2, h0, h1, p_pen, p_win, d0, d1, d2, words, p_rows, n_owner, n_b0, n_bias, n_values, n_h0, n_history, n_pen,
+     n_win, n_d0, n_drafts, n_seen, _, n_rows) = got
     # requests: as many as the first array that is given for each of them says
-    Q = penalties.shape[0] if penalties is not None else windows.shape[0] if windows is not None else \
-        history[0].numel() - 1 if history is not None else bias[0].numel() - 1 if bias is not None else \
-        drafts[0].numel() - 1 if drafts is not None else R
-    n_bias = n_history = n_drafts = p_owner = b0 = b1 = b2 = h0 = h1 = d0 = d1 = d2 = p_pen = p_win = words = m = width = p_rows = 0
-    if owner is not None:
-        assert owner.dtype is i32 and owner.numel() == R
-        p_owner = _flat(owner)
-    if bias is not None:
-        first, ids, values = bias
-        assert first.dtype is i32 and ids.dtype is i32 and values.dtype is f32 and first.numel() == Q + 1 and \
-            ids.numel() == values.numel()
-        b0, b1, b2, n_bias = _flat(first), _flat(ids), _flat(values), ids.numel()
-    if history is not None:
-        first, tokens = history
-        assert first.dtype is i32 and tokens.dtype is i32 and first.numel() == Q + 1
-        h0, h1, n_history = _flat(first), _flat(tokens), tokens.numel()
-    if drafts is not None:
-        first, tokens, seen = drafts
-        assert first.dtype is i32 and tokens.dtype is i32 and seen.dtype is torch.int64 and first.numel() == Q + 1 and \
-            seen.numel() == R
-        d0, d1, d2, n_drafts = _flat(first), _flat(tokens), _flat(seen), tokens.numel()
-    if penalties is not None:
-        assert penalties.dtype is f32 and penalties.shape == (Q, 3)
-        p_pen = _flat(penalties)
-    if windows is not None:
-        assert windows.dtype is i32 and windows.numel() == Q
-        p_win = _flat(windows)
+    Q = penalties.shape[0] if penalties is not None else n_win if windows is not None else n_h0 - 1 if history is not None else \
+        n_b0 - 1 if bias is not None else n_d0 - 1 if drafts is not None else R
+    assert owner is None or n_owner == R
+    assert bias is None or n_b0 == Q + 1 and n_bias == n_values
+    assert history is None or n_h0 == Q + 1
+    assert drafts is None or n_d0 == Q + 1 and n_seen == R
+    assert penalties is None or penalties.dim() == 2 and n_pen == 3 * Q
+    assert windows is None or n_win == Q
+    assert allowed_rows is None or n_rows == R
+    m = width = 0
     if allowed is not None:
         m, width = allowed.shape
-        assert allowed.dtype is i32
-        words = _flat(allowed)
         if width * 32 < V:
             raise KernelError(f"logits_constrain: masks of {width} words for {V} tokens")
-    if allowed_rows is not None:
-        assert allowed_rows.dtype is i32 and allowed_rows.numel() == R
-        p_rows = _flat(allowed_rows)
     if R == 0 or V == 0:
         return
     status = entry_points("drafts").tgo_logits_constrain(
-        at, s_in, to, s_out, R, V, Q, p_owner, b0, b1, b2, n_bias, h0, h1, n_history, p_pen, p_win, d0, d1, n_drafts, d2, words, width, m, p_rows,
-        _stream())
+        at, s_in, to, s_out, R, V, Q, p_owner, b0, b1, b2, n_bias, h0, h1, n_history, p_pen, p_win, d0, d1, n_drafts, d2, words, width, m,
+        p_rows, _stream())
     _check(status, "logits_constrain", f"(R={R}, V={V})" if status else "")
 
 
@@ -2411,15 +2450,15 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, chosen: torch.Tenso
 
     tokens, parents (a node's place in its request; below its own, or -1), chosen, path int32 [T]; q_start int32 [B + 1], at
     most 64 nodes a request; counts, following int32 [B]."""
-    i32 = torch.int32
-    assert tokens.dtype is i32 and parents.dtype is i32 and chosen.dtype is i32 and q_start.dtype is i32 and path.dtype is i32 \
-        and counts.dtype is i32 and following.dtype is i32
-    T, B = tokens.numel(), counts.numel()
-    assert parents.numel() == chosen.numel() == path.numel() == T and following.numel() == B and q_start.numel() == B + 1
-    args = (_flat(tokens), _flat(parents), _flat(chosen), _flat(q_start), B, T, _flat(path), _flat(counts), _flat(following))
+    tensors = (tokens, parents, chosen, q_start, path, counts, following)
+    got = _look("iiiiiii", *tensors)
+    if got is None:
+        _refuse("iiiiiii", *tensors)
+    p_tokens, p_parents, p_chosen, first, to, n, last, T, T1, T2, starts, T3, B, B1 = got
+    assert T == T1 == T2 == T3 and B == B1 == starts - 1
     if B == 0:
         return
-    status = entry_points("drafts").tgo_tree_accept(*args, _stream())
+    status = entry_points("drafts").tgo_tree_accept(p_tokens, p_parents, p_chosen, first, B, T, to, n, last, _stream())
     _check(status, "tree_accept", f"(B={B})" if status else "")
 
 
@@ -2432,26 +2471,25 @@ def tree_keep(tensors, slots: torch.Tensor, q_start: torch.Tensor, path: torch.T
 
     tensors contiguous and apart, all with pages of one size; slots, path int32 [T] (a request's slots distinct), q_start int32
     [B + 1], counts int32 [B]."""
-    i32 = torch.int32
-    assert slots.dtype is i32 and q_start.dtype is i32 and path.dtype is i32 and counts.dtype is i32
-    B = counts.numel()
-    assert path.numel() == slots.numel() and q_start.numel() == B + 1
-    lists = (_flat(slots), _flat(q_start), B, slots.numel(), _flat(path), _flat(counts))
+    got = _look("iiii", slots, q_start, path, counts)
+    if got is None:
+        _refuse("iiii", slots, q_start, path, counts)
+    places, first, along, n, T, starts, T1, B = got
+    assert T == T1 and starts == B + 1
     desc, page_size = array("q"), 0
     for t in tensors:
-        if not t.is_cuda:
+        one = _pages(t, axis)
+        if one is None:
             _need_cuda(t)
-        one, size = t.shape, t.element_size()
-        rest = len(one) - axis
-        assert 0 <= axis and rest in (3, 4) and t.is_contiguous() and size >= 2
-        if page_size and one[-2] != page_size:
-            raise KernelError(f"tree_keep: pages of {one[-2]} places beside pages of {page_size}")
-        page_size = one[-2]
-        if t.numel():
-            desc.extend((t.data_ptr(), math.prod(one[:axis]), one[axis], one[axis + 1] if rest == 4 else 1, one[-1] * size))
+            raise AssertionError("tree_keep: a tensor is not contiguous, or has no pages along that axis")
+        if page_size and one[0] != page_size:
+            raise KernelError(f"tree_keep: pages of {one[0]} places beside pages of {page_size}")
+        page_size = one[0]
+        if one[1]:
+            desc.extend(one[2:])
     if not desc or B == 0:
         return
-    status = entry_points("drafts").tgo_tree_keep(desc.buffer_info()[0], len(desc) // 5, page_size, *lists, _stream())
+    status = entry_points("drafts").tgo_tree_keep(desc.buffer_info()[0], len(desc) // 5, page_size, places, first, B, T, along, n, _stream())
     _check(status, "tree_keep", f"(B={B}, page_size={page_size})" if status else "")
     LAUNCHES[0] += (len(desc) // 5 - 1) // 64
 
