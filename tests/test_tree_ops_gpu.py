@@ -288,6 +288,23 @@ def test_pages_that_nobody_has(way, dtype):
     assert torch.equal(c.run(bad)[:4], want[:4])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_pages_far_into_a_cache(way, dtype):
+    """Numbers of a cache beyond 2^31, bytes beyond 2^32; rows kept there move too."""
+    c = Trees(dtype, 16, 8, 128, [300, 40], [9, 3], seed=14)
+    far, own = 140000, c.k.shape[0]                            # 16384 numbers a page
+    for name in ("k", "v"):
+        big = torch.empty((far, 8, 16, 128), dtype=dtype, device=DEV)
+        big[far - own:] = getattr(c, name)
+        setattr(c, name, big)
+    c.tables += far - own
+    c.check()
+    old, at = c.k[far - own:].clone(), (far - 2) * 16
+    ops().tree_keep([c.k], ints([at, at + 1, at + 17]), ints([0, 3]), ints([0, 2, -1]), ints([2]))
+    old[own - 2, :, 1] = old[own - 1, :, 1]
+    assert torch.equal(torch.nan_to_num(c.k[far - own:]), torch.nan_to_num(old))
+
+
 def test_attention_captured_beside_another_stream(way):
     """A captured call follows what its inputs hold; two graphs and an eager call on another stream share nothing."""
     cases = [Trees(BF, 16, 4, 128, [2000, 77], [16, 5], seed=s) for s in range(3)]
@@ -536,6 +553,25 @@ def test_constrain_long_histories(V, first):
     ops().logits_constrain(src, out=dst, **c)
     ops().logits_constrain(src, **c)
     assert torch.equal(src, dst) and bool((rows[:, :first] == 9).all()) and bool((rows[:, V + first:] == 9).all())
+
+
+@pytest.mark.parametrize("masked", [True, False])
+def test_constrain_rows_far_into_a_matrix(masked):
+    """Numbers beyond 2^31; of all rows only the last has anything to edit."""
+    R, V = 15000, 151936
+    x, c = constrained(1, V, 1, seed=8, history=400, bias=20, allowed=1)
+    c["allowed_rows"] = ints([0])
+    if not masked:
+        c["allowed"] = c["allowed_rows"] = None
+    want = x.clone()
+    ops().logits_constrain(want, **c)
+    rows = torch.full((R, V), 2.5, device=DEV)
+    rows[-1] = x[0]
+    c["owner"] = ints([-1] * (R - 1) + [0])
+    if masked:
+        c["allowed_rows"] = ints([-1] * (R - 1) + [0])
+    ops().logits_constrain(rows, **c)
+    assert torch.equal(rows[-1:], want) and bool((rows[:-1] == 2.5).all())
 
 
 def test_constrain_starts_outside_their_lists():
