@@ -289,6 +289,17 @@ def test_pages_that_nobody_has(way, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("lens", [[300, 40], [900, 7, 0, 131]])
+def test_queries_off_every_boundary(way, dtype, lens):
+    """Where the tensor cores do not take the rows, whatever a call of these sizes would have kept whole or cut."""
+    c = Trees(dtype, 16, 4, 128, lens, [8] * len(lens), seed=15)
+    wide = torch.zeros((c.qkv.shape[0], c.qkv.shape[1] + 1), dtype=dtype, device=DEV)
+    wide[:, 1:] = c.qkv
+    c.qkv = wide[:, 1:]
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
 def test_pages_far_into_a_cache(way, dtype):
     """Numbers of a cache beyond 2^31, bytes beyond 2^32; rows kept there move too."""
     c = Trees(dtype, 16, 8, 128, [300, 40], [9, 3], seed=14)

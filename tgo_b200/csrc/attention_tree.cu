@@ -18,6 +18,7 @@
 #include "tcgen.cuh"
 
 #define TREE_NODES 64
+#define TREE_E_WORK 1001                      // returned, nothing done: the call wants a workspace
 #define TREE_OVERHEAD 1
 
 struct TreeWork {
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
         k.find(w, blockIdx.x);
         if (tid == 0) {
             s_walk = k;
-            notes[blockIdx.x].n_rows = 0;
+            if (!w.whole) notes[blockIdx.x].n_rows = 0;
         }
     }
     __syncthreads();
@@ -645,7 +646,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
         TreeWalk<TT_KEYS> walk;
         walk.find(w, blockIdx.x);
         TreeNote note = {0, 0, 0, 0, 0};
-        if (lane == 0) notes[blockIdx.x] = note;
+        if (lane == 0 && !w.whole) notes[blockIdx.x] = note;
         uint32_t sent = 0, g = 0;                               // items whose Q was asked for, key tiles
         bool ok = true;
         for (uint32_t n = 0;; ++n) {
@@ -673,7 +674,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
                     rec->valid = 0;
                     tg_arrive(&told[qb]);
                     tg_arrive(&bits_told[qb]);
-                    notes[blockIdx.x] = note;
+                    if (!w.whole) notes[blockIdx.x] = note;
                 }
                 break;
             }
@@ -1205,17 +1206,6 @@ TGO_API int tgo_attention_tree_error(int* value) { return (int)cudaMemcpyFromSym
 static int tree_force = 0;                    // for tests: 1 plain products; 2, 3 items of one row tile, whole and cut; 4, 5 of two
 TGO_API int tgo_attention_tree_force(int way) { tree_force = way; return 0; }
 
-// Floats of workspace that a call wants.
-TGO_API int tgo_attention_tree_work(int dtype, int dh, int group, int page_size, int max_nodes) {
-    const int sms = tgo_multiprocessors();
-    int rows = 2 * 64;                        // two blocks an SM with 64 rows a tile
-    if (dtype == TGO_BF16 && tgo_attention_tree_tc_supports(dh, group, page_size)) {
-        const int mine = max_nodes * group < 2 * TT_ROWS ? max_nodes * group : 2 * TT_ROWS;
-        rows = mine > rows ? mine : rows;
-    }
-    return sms * 2 * rows * ((dh + 3) / 4 * 4 + 2) + 2 * sms * (int)(sizeof(TreeNote) / sizeof(float));
-}
-
 // The tensor map of query rows [tokens][heads][dh], `stride` apart, in boxes of 64 columns of G heads of a row tile's tokens.
 static bool tree_map_q(CUtensorMap* map, const void* q, long long stride, int tokens, int H, int G, int dh) {
     const TgEncodeFn encode = tg_encode();
@@ -1237,8 +1227,8 @@ static int tree_join_go(void* out, long long out_stride, int dh, const TreeWork&
                           (T*)out, out_stride, dh, w.H / w.Hkv, w.rows_per_tile, strips, notes, part_o, part_ml);
 }
 // The workspace's parts: sums, (maximum, sum of exponentials) pairs, notes.
-static float* tree_ml(float* work, const TreeWork& w, int dh) { return work + (size_t)w.workers * 2 * w.rows_per_tile * ((dh + 3) / 4 * 4); }
-static TreeNote* tree_notes(float* work, const TreeWork& w, int dh) { return (TreeNote*)(tree_ml(work, w, dh) + (size_t)w.workers * 4 * w.rows_per_tile); }
+static float* tree_ml(float* work, const TreeWork& w, int dh) { return work ? work + (size_t)w.workers * 2 * w.rows_per_tile * ((dh + 3) / 4 * 4) : nullptr; }
+static TreeNote* tree_notes(float* work, const TreeWork& w, int dh) { return work ? (TreeNote*)(tree_ml(work, w, dh) + (size_t)w.workers * 4 * w.rows_per_tile) : nullptr; }
 
 template <int DH, int RT>
 static int tree_tc_go(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, const void* v, int n_pages, void* out,
@@ -1305,6 +1295,8 @@ static void tree_choose(TreeWork& w, int max_context, int G, int sms) {
     w.min_units = w.whole ? 1 : 2;
 }
 
+static bool tree_plain_whole(const TreeWork& w, int max_context) { return tree_tiles(w, max_context, TP_KEYS) <= 2; }
+
 template <typename T, int DP, int R>
 static int tree_plain_go(const void* q, long long q_stride, void* out, long long out_stride, const void* k, const void* v,
                          int n_pages, int page_size, const int* tables, int max_blocks, const void* seen, int dh, float scale,
@@ -1329,8 +1321,9 @@ static int tree_plain_go(const void* q, long long q_stride, void* out, long long
     if ((1 << shift) != page_size) shift = -1;
     w.rows_per_tile = ROWS;
     w.workers = held[dev] * tgo_multiprocessors();
-    w.whole = tree_tiles(w, max_context, TP_KEYS) <= 2;
+    w.whole = tree_plain_whole(w, max_context);
     if (w.whole) w.min_units = 1;
+    else if (!work) return TREE_E_WORK;
     int rc = tgo_launch_pdl(tree_plain_kernel<T, DP, R>, dim3(w.workers), dim3(TP_THREADS), smem, stream, (const T*)q, q_stride, (T*)out,
                             out_stride, (const T*)k, (const T*)v, n_pages, page_size, shift, tables, max_blocks,
                             (const unsigned long long*)seen, dh, scale, w, work, tree_ml(work, w, dh), tree_notes(work, w, dh));
@@ -1338,7 +1331,27 @@ static int tree_plain_go(const void* q, long long q_stride, void* out, long long
     return tree_join_go<T>(out, out_stride, dh, w, work, tree_ml(work, w, dh), tree_notes(work, w, dh), stream);
 }
 
-// work: tgo_attention_tree_work() floats. scale > 0.
+// Floats of workspace that a call of these sizes wants: none where items stay whole. max_context -1: that any call wants.
+TGO_API int tgo_attention_tree_work(int dtype, int B, int H, int Hkv, int dh, int page_size, int window, int max_nodes, int max_context) {
+    if (B <= 0 || Hkv <= 0 || H % Hkv || max_nodes <= 0) return 0;
+    const int sms = tgo_multiprocessors(), G = H / Hkv;
+    const bool tc = dtype == TGO_BF16 && tgo_attention_tree_tc_supports(dh, G, page_size);
+    if (max_context >= 0) {
+        TreeWork w = {nullptr, nullptr, B, 0, H, Hkv, window, max_nodes, 0, 0, 0, 2, sms, 0};
+        if (tc) tree_choose(w, max_context, G, sms);
+        else w.whole = tree_plain_whole(w, max_context);
+        if (w.whole) return 0;
+    }
+    int rows = 2 * 64;                        // two blocks an SM with 64 rows a tile
+    if (tc) {
+        const int mine = max_nodes * G < 2 * TT_ROWS ? max_nodes * G : 2 * TT_ROWS;
+        rows = mine > rows ? mine : rows;
+    }
+    return sms * 2 * rows * ((dh + 3) / 4 * 4 + 2) + 2 * sms * (int)(sizeof(TreeNote) / sizeof(float));
+}
+
+// work: tgo_attention_tree_work() floats, or null. TREE_E_WORK, and nothing is done, where it is null and items are cut, as they may be
+// although that said none: by the FMA units for want of alignment. scale > 0.
 TGO_API int tgo_attention_tree(const void* q, long long q_stride, void* out, long long out_stride, int dtype, int T, const void* k_cache,
                                const void* v_cache, int n_pages, int page_size, const int* block_tables, int max_blocks,
                                const int* context_lens, const int* q_start, const void* seen, int B, int H, int Hkv, int dh,
@@ -1354,10 +1367,12 @@ TGO_API int tgo_attention_tree(const void* q, long long q_stride, void* out, lon
     // units are counted in 32 bits
     if ((double)B * Hkv * ((double)max_nodes * G / 16 + 1) * ((double)max_blocks * page_size / TP_KEYS + 2 + TREE_OVERHEAD) > 2e9) return TGO_E_BAD_ARG;
     if (dtype == TGO_BF16 && tree_force != 1 && tgo_attention_tree_tc_supports(dh, G, page_size) && q_stride % 8 == 0 &&
-        q_stride >= (long long)H * dh && out_stride % 8 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)k_cache % 128 == 0 && (uintptr_t)v_cache % 128 == 0 &&
+        q_stride >= (long long)H * dh && out_stride % 8 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0 &&
+        (uintptr_t)k_cache % 128 == 0 && (uintptr_t)v_cache % 128 == 0 &&
         rows + page_size <= 0x7fffffffll) {
         w.workers = sms;
         tree_choose(w, max_context, G, sms);
+        if (!w.whole && !work) return TREE_E_WORK;
         const bool two = w.tokens_per_tile > TT_ROWS / G;
         CUtensorMap mk, mv, mq;
         if (!tg_map(&mk, k_cache, rows, dh, dh, page_size) || !tg_map(&mv, v_cache, rows, dh, dh, page_size) ||

@@ -2309,9 +2309,9 @@ TREE_NODES = 64          # drafted tokens of a request that the kernels take: wh
 
 
 @functools.lru_cache(maxsize=256)
-def _tree_work(code: int, head_dim: int, group: int, page_size: int, max_nodes: int) -> int:
-    """Numbers of workspace that calls of these sizes want; a function of the sizes and of the GPU's kind."""
-    return entry_points("attention_tree").tgo_attention_tree_work(code, head_dim, group, page_size, max_nodes)
+def _tree_work(*sizes: int) -> int:
+    """Numbers of workspace that a call of these sizes wants, by the library's rule."""
+    return entry_points("attention_tree").tgo_attention_tree_work(*sizes)
 
 
 def attention_tree(q: torch.Tensor, out: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int,
@@ -2348,13 +2348,19 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, num_heads: int, num_kv_he
     if T == 0 or B == 0 or max_nodes == 0:
         return
     lib = entry_points("attention_tree")
-    work = q.new_empty(_tree_work(code, head_dim, num_heads // num_kv_heads, page_size, max_nodes), dtype=torch.float32)
-    status = lib.tgo_attention_tree(p_q, qs, p_out, os, code, T, k, v, shape[0], page_size, tables, width, lens, first, bits, B,
-                                    num_heads, num_kv_heads, head_dim, window, max_nodes, max_context, work.data_ptr(),
-                                    _stream(), float(scale))
+    args = (p_q, qs, p_out, os, code, T, k, v, shape[0], page_size, tables, width, lens, first, bits, B, num_heads, num_kv_heads,
+            head_dim, window, max_nodes, max_context)
+    floats = _tree_work(code, B, num_heads, num_kv_heads, head_dim, page_size, window, max_nodes, max_context)
+    work = q.new_empty(floats, dtype=torch.float32) if floats else None
+    status = lib.tgo_attention_tree(*args, work.data_ptr() if floats else 0, _stream(), float(scale))
+    if status == E_WORK:                      # items are cut all the same
+        work = q.new_empty(_tree_work(code, B, num_heads, num_kv_heads, head_dim, page_size, window, max_nodes, -1),
+                           dtype=torch.float32)
+        status = lib.tgo_attention_tree(*args, work.data_ptr(), _stream(), float(scale))
     _check(status, "attention_tree", f"(head_dim={head_dim}, heads={num_heads}/{num_kv_heads}, page_size={page_size}, "
                                      f"window={window})" if status else "")
-    LAUNCHES[0] += 1
+    if work is not None:
+        LAUNCHES[0] += 1                      # the join
 
 
 def attention_tree_force_way(way: int = 0) -> None:
