@@ -620,7 +620,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
     // rows of the Q tiles that no box writes must not hold NaN by chance
     if (tile_rows != TT_ROWS) for (int i = tid; i < 2 * TT_TILE / 16; i += TT_THREADS) ((uint4*)sQ)[i] = make_uint4(0u, 0u, 0u, 0u);
     if (tid < 16) odd_nodes[tid] = 0;
-    if (tid == 0) {
+    if (tid == 64) {
         for (int i = 0; i < 2; ++i) {
             tg_init(&q_full[i], 1); tg_init(&q_empty[i], 14);   // products 1 + 1, softmax 8, results 4
             tg_init(&k_full[i], 1); tg_init(&k_empty[i], 1);
@@ -635,16 +635,24 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
     }
     tg_init_done();
     if (warp == 1) tg_alloc512(tmem_slot);
-    tg_before();
-    __syncthreads();
+    pdl_wait();
+    // The two warps that ask for copies find their pieces first; they wait for what the others have laid out, and nobody for them.
+    TreeWalk<TT_KEYS> walk;
+    if (warp == 0 || warp == 3) {
+        walk.find(w, blockIdx.x);
+        __syncwarp();
+        asm volatile("barrier.cta.sync.aligned 1, %0;" ::"n"(TT_THREADS) : "memory");
+    } else {
+        __syncwarp();
+        tg_before();
+        asm volatile("barrier.cta.arrive.aligned 1, %0;" ::"n"(TT_THREADS) : "memory");
+        asm volatile("barrier.cta.sync.aligned 2, %0;" ::"n"(TT_THREADS - 64) : "memory");
+    }
     tg_after();
     const uint32_t tmem = *tmem_slot;
-    pdl_wait();
 
     if (warp == 0) {
         // ------------------------------------------------------------- records and Q
-        TreeWalk<TT_KEYS> walk;
-        walk.find(w, blockIdx.x);
         TreeNote note = {0, 0, 0, 0, 0};
         if (lane == 0 && !w.whole) notes[blockIdx.x] = note;
         uint32_t sent = 0, g = 0;                               // items whose Q was asked for, key tiles
@@ -730,8 +738,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(
         // ------------------------------------------------------------- V
         bool ok = true;
         uint32_t g = 0, mixed = 0, plain0 = 0, plain1 = 0;      // tiles; mixed ones, the others by stage
-        TreeWalk<TT_KEYS> walk;
-        walk.find(w, blockIdx.x);
         while (ok && walk.next(w)) {
             TreePages pages(w, walk, block_tables, max_blocks, page_shift);
             for (int it = 0; it < pages.n_it; ++it, ++g) {
