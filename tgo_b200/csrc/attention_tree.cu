@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
 // Waits have a limit of about two seconds, after which a code is left, what is under way is waited for, and the CTA ends.
 //   MEASURED, in a graph of calls, with the join: 8 requests of 16 nodes, 4099 to 1230 keys, 8 kv heads of 4 query heads of 128: 27.5 us (90
 // MB of K and V; 1.3 us a tile of 128 keys, which is the copy rate, beside 11.5 of beginnings, ends and the join); 2 requests of
-// 64 nodes over 32703 keys: 79 us, 0.84 PFLOP/s, the softmax threads; one request of 8 nodes over 497 keys 11.2 us: a chain of
+// 64 nodes over 32703 keys: 78 us, 0.85 PFLOP/s, the softmax threads; one request of 8 nodes over 497 keys 11.4 us: a chain of
 // reads (lengths, pages, K), a masked tile, its result. Taken back: the four softmax warps of a stream as eight with two threads a row
 // (29 and 92 us for 27.5 and 79), a quarter of the exponentials as cubics on the FMA units (the same), K and V asked for by
 // one warp (a copy every 80 cycles, 32 a tile), pages into the L2 ahead of them (33 and 92).
