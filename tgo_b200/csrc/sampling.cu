@@ -6,7 +6,8 @@
 // the temperature -> top-k on the softmax weights by (weight, lower id) -> top-p (smallest
 // prefix of the descending candidates whose weight reaches p of the total; at most 128
 // candidates) -> walk the kept ids in ascending order and return the first whose running
-// sum exceeds u * total, or the last kept id if rounding never gets there.
+// sum exceeds u * total, or the last kept id with weight if rounding never gets there. An id
+// without weight (masked, or too small for exp) is never drawn.
 //
 // Sums over the vocabulary are formed per thread over a contiguous range and then over the
 // threads in order, which is not the reference's single ascending sum: totals can differ
@@ -256,6 +257,7 @@ sample_kernel(const float* __restrict__ logits, long long stride, int V,
     __shared__ int cid[SM_MAXC], sid[SM_MAXC];
     __shared__ int n_cand, n_kept;
     __shared__ int single_s;
+    __shared__ int first_s, last_s;           // of the ranges
 
     const int r = blockIdx.x, t = threadIdx.x;
     const float* row = logits + (size_t)r * stride;
@@ -295,17 +297,31 @@ sample_kernel(const float* __restrict__ logits, long long stride, int V,
 
     const bool all_kept = k_req <= 0 && p_req <= 0.f;
     if (all_kept) {
-        if (t == 0) result_s = V - 1;
+        // The first range that has weight and ends above the target; the last that has weight if none
+        // does. Ends are sums of 32 bits, made one way inside 32 ranges and another way between them: they
+        // may go down from one range to the next, and up over a range without weight.
+        if (t == 0) { result_s = V - 1; first_s = SM_THREADS; last_s = -1; }
         __syncthreads();
         const float target = u * total_all;
-        const float before = part[t];
         const float after = t + 1 < SM_THREADS ? part[t + 1] : total_all;
-        if (c0 < c1 && before <= target && after > target) {
-            float acc = before;
+        const unsigned above = __ballot_sync(0xffffffffu, mine > 0.f && after > target);
+        const unsigned some = __ballot_sync(0xffffffffu, mine > 0.f);
+        if ((t & 31) == 0) {
+            if (above) atomicMin(&first_s, t + __ffs(above) - 1);
+            if (some) atomicMax(&last_s, t + 31 - __clz(some));
+        }
+        __syncthreads();
+        if (t == (first_s < SM_THREADS ? first_s : last_s)) {
+            // the running sum may end below the range's: then it is the last id with weight
+            float acc = part[t];
             int pick = c1 - 1;
             for (int i = c0; i < c1; ++i) {
-                acc += expf(row[i] / T - m);
-                if (acc > target) { pick = i; break; }
+                const float w = expf(row[i] / T - m);
+                acc += w;
+                if (w > 0.f) {
+                    pick = i;
+                    if (acc > target) break;
+                }
             }
             result_s = pick;
         }
@@ -428,8 +444,11 @@ sample_kernel(const float* __restrict__ logits, long long stride, int V,
         int pick = kept > 0 ? cid[kept - 1] : 0;
         float w_pick = kept > 0 ? cw[kept - 1] : 0.f;
         for (int j = 0; j < kept; ++j) {
+            if (!(cw[j] > 0.f)) continue;                     // kept for want of others
             acc += cw[j];
-            if (acc > target) { pick = cid[j]; w_pick = cw[j]; break; }
+            pick = cid[j];
+            w_pick = cw[j];
+            if (acc > target) break;
         }
         out[r] = pick;
         if (want >= 0) lp_out[r] = logf(w_pick / total_s);
