@@ -197,14 +197,20 @@ class DraftedGeneration:
         at = 0
         for one, e, a in zip(list(live), entries, got):
             req = one.request
+            path = a.path
+            # a grammar's failure counts where the request comes first; what was chosen from there on had no mask
+            failed = next((k for k, i in enumerate(path) if at + i in stuck), None)
+            if failed is not None:
+                path = path[:failed + 1]
+            along = [e.tokens[i] for i in path[1:]]
+            chosen = path if failed is None else path[:-1]   # where a token was chosen that the request gets
             self.drafted += len(e.tokens) - 1
-            self.accepted += len(a.path) - 1
-            req.sampler.index += len(a.path)
-            req.logprobs.extend(r for r in (reports[at + i] for i in a.path) if r is not None)
-            along = [e.tokens[i] for i in a.path[1:]]
-            if at + a.path[-1] in stuck:
+            self.accepted += len(along)
+            req.sampler.index += len(chosen)
+            req.logprobs.extend(r for r in (reports[at + i] for i in chosen) if r is not None)
+            if failed is not None:
                 req.output.extend(along)
-                raise stuck[at + a.path[-1]]
+                raise stuck[at + path[-1]]
             at += len(e.tokens)
             self._take(one, along + [a.following], live)
 
