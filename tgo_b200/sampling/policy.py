@@ -16,6 +16,7 @@ from typing import Callable, Dict, List, Optional
 import numpy as np
 
 TOP_MAX = 128                 # most candidates either truncation keeps (sample/sample.go:47)
+FLOAT32_MAX = 3.4028234663852886e38
 MAX_DRAW = 0.99999994         # the largest float32 below one (sample/sample.go:194)
 
 
@@ -75,7 +76,8 @@ class Policy:
                              f"a {type(self.allowed).__name__}")
 
     def allowed_words(self, generated: List[int], vocab: int):
-        """The mask of the tokens that may follow `generated`, uint32 [vocab / 32, rounded up], or None: any may."""
+        """The mask of the tokens that may follow `generated`, uint32 [vocab / 32, rounded up], or None: any may. A token
+        that a bias of -inf takes out is none of them."""
         got = self.allowed(list(generated)) if self.allowed is not None else None
         if got is None:
             return None
@@ -92,6 +94,9 @@ class Policy:
                 raise ValueError(f"policy: an allowed id is outside the vocabulary of {vocab}")
             words = np.zeros(n, dtype=np.uint32)
             np.bitwise_or.at(words, ids // 32, np.uint32(1) << (ids % 32).astype(np.uint32))
+        for i, b in self.logit_bias.items():
+            if b < -FLOAT32_MAX:
+                words[int(i) // 32] &= ~np.uint32(1 << int(i) % 32)
         if not words.any():
             raise ValueError("policy: no token is allowed to come next")
         return words
