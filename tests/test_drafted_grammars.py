@@ -1,6 +1,7 @@
 """Grammars that fail on a request's way, with and without drafts, and through a session; no GPU."""
 import copy
 
+import numpy as np
 import pytest
 
 from emulated_drafts import Oracle
@@ -86,3 +87,11 @@ def test_a_session_under_a_grammar(emulated, tmp_path):        # noqa: F811
         session = model.new_session(64, page_size=8)
         session.stop_ids = {5}
         assert list(session.complete([1, 2, 3], pol)) == want[:next(i for i, t in enumerate(want) if t == 5)]
+
+
+@pytest.mark.parametrize("got", [[True, False, True], np.array([True, False]), (np.bool_(True),)])
+def test_truth_values_are_no_ids(got):
+    with pytest.raises(ValueError, match="truth values"):
+        Policy(allowed=lambda done: got).allowed_words([], 70)
+    assert Policy(allowed=lambda done: range(2)).allowed_words([], 70).tolist() == [3, 0, 0]
+    assert Policy(allowed=lambda done: np.array([1, 64])).allowed_words([], 70).tolist() == [2, 0, 1]

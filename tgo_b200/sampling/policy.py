@@ -89,7 +89,10 @@ class Policy:
             if vocab % 32:
                 words[-1] &= np.uint32((1 << vocab % 32) - 1)
         else:
-            ids = np.fromiter((int(i) for i in got), dtype=np.int64)
+            ids = list(got)
+            if not {bool, np.bool_}.isdisjoint(map(type, ids)):
+                raise ValueError("policy: `allowed` names ids, or gives 32 of them a number; it gave truth values")
+            ids = np.fromiter(map(int, ids), dtype=np.int64, count=len(ids))
             if ids.size and (ids.min() < 0 or ids.max() >= vocab):
                 raise ValueError(f"policy: an allowed id is outside the vocabulary of {vocab}")
             words = np.zeros(n, dtype=np.uint32)
