@@ -27,6 +27,7 @@ def _library():
         P, I, L = c_void_p, c_int, c_longlong
         lib.tgo_step_grow.argtypes = [P, I, P, P, P, P]
         lib.tgo_step_commit.argtypes = [P, I, P, P]
+        lib.tgo_cache_trim.argtypes = [P, I, P]
         lib.tgo_step_pack.argtypes = [P, I, P, P, P, P, P, I, I, I, P, L, P]
         lib.tgo_cache_last_error.restype = ctypes.c_char_p
         for name in ("tgo_cache_request", "tgo_cache_pool", "tgo_cache_slot_of"):
@@ -219,6 +220,15 @@ class NativeCacheManager:
             self._raise(rc)
         self._sharing = True
         return pages
+
+    def trim(self, request_ids) -> None:
+        """Pages at the requests' ends that neither what they hold nor what they were admitted with
+        needs go back: those of drafted tokens that were not kept, or of a step that failed."""
+        n = len(request_ids)
+        handles = np.fromiter((self.requests[r].handle for r in request_ids), dtype=np.int64, count=n)
+        rc = self._lib.tgo_cache_trim(self._h, n, handles.ctypes.data)
+        if rc:
+            self._raise(rc)
 
     def finish(self, request_id) -> List[tuple]:
         req = self.requests[request_id]

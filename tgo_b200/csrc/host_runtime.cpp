@@ -86,6 +86,7 @@ struct Pool {
 struct Request {
     int slot = -1;
     long long length = 0, version = 0;
+    long long reserved = 0;          // tokens it was admitted with pages for
     std::vector<std::vector<int>> tables;
 };
 
@@ -217,6 +218,7 @@ TGO_HOST_API int tgo_cache_admit(void* p, long long handle, long long reserve_to
         return m->fail(SLOTS_EXHAUSTED, "cache: all " + std::to_string(m->num_slots) + " request slots are taken");
     Request r;
     r.slot = m->free_slots.back();
+    r.reserved = std::max(reserve_tokens, 0ll);
     r.tables.resize(m->kind.size());
     if (reserve_tokens > 0) {
         const int rc = m->grow(r, reserve_tokens, true);
@@ -275,6 +277,31 @@ TGO_HOST_API int tgo_cache_commit(void* p, long long handle, long long new_lengt
         ++r.version;
     }
     if (n_released) *n_released = n;
+    return OK;
+}
+
+// Pages at the requests' ends that neither what they hold nor what they were admitted with needs go back: those
+// of drafted tokens that were not kept, or of a step that failed.
+TGO_HOST_API int tgo_cache_trim(void* p, int n, const long long* handles) {
+    Manager* m = M(p);
+    std::vector<int> gone;
+    for (int i = 0; i < n; ++i) {
+        auto it = m->requests.find(handles[i]);
+        if (it == m->requests.end()) return m->fail(NOT_LIVE, "cache: the request is not live", i);
+        Request& r = it->second;
+        for (int g = 0; g < (int)m->kind.size(); ++g) {
+            std::vector<int>& t = r.tables[g];
+            const long long keep = m->pages_for(m->kind[g] == KIND_FULL ? std::max(r.length, r.reserved) : r.length);
+            if ((long long)t.size() <= keep) continue;
+            gone.clear();
+            for (size_t j = (size_t)keep; j < t.size(); ++j)
+                if (t[j] != NULL_PAGE) gone.push_back(t[j]);
+            t.resize((size_t)keep);
+            ++r.version;
+            const int bad = gone.empty() ? 0 : m->pools[g].give(gone);
+            if (bad) return m->fail(PAGE_MISUSE, "cache: page " + std::to_string(bad) + " cannot be given back", g, bad);
+        }
+    }
     return OK;
 }
 

@@ -350,7 +350,8 @@ class Engine:
         the choice confirms. `choose(logits, ctx)` gets float32 logits [tokens of the step, vocabulary], the entries' one
         after the other, and returns int32 token ids [tokens] on the device. From its first token on, a request then goes
         along the drafts that were chosen: their cache rows are moved together, its length grows by the
-        path's. A step that fails leaves every request where it was."""
+        path's, and pages beyond it and beyond what the request was admitted with go back. A step that fails leaves every
+        request where it was."""
         entries = [e if isinstance(e, DraftEntry) else DraftEntry(*e) for e in entries]
         if not entries:
             raise ValueError("draft_step: an empty batch carries nothing")
@@ -358,6 +359,12 @@ class Engine:
         if self.device.type == "cuda":
             compile_together(["attention_tree", "drafts"])
         ids = [e.request_id for e in entries]
+        try:
+            return self._draft_step(entries, paths, ids, choose)
+        finally:
+            self.cache.trim(ids)                          # places that nobody keeps, of a failed step all
+
+    def _draft_step(self, entries: List[DraftEntry], paths: List[List[int]], ids: list, choose) -> List[Accepted]:
         begun = self.cache.step_begin(ids, [len(e.tokens) for e in entries])
         self._begun = (ids, begun)
         try:
