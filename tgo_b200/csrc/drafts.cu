@@ -308,7 +308,8 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
                 if (a.history[i] >= 0) count_in(a.history[i]);
         }
         if (ok) ok = tg_wait(&full[b], phase, &drafts_error_flag, 1);
-        if (__syncthreads_or(!ok)) break;
+        ok = __syncthreads_and(ok);                            // each thread times its own wait: all leave, and know why
+        if (!ok) break;
         if (row.b_hi > row.b_lo) {
             const uint32_t mine = (uint32_t)(bias_id - col0);
             if (bias_id >= 0 && mine < width) buf[mine] += bias_of;
