@@ -15,7 +15,7 @@ def source(name):
 def kernel(name, file):
     text = source(file)
     start = text.index(f" {name}(")
-    return text[start:text.index("\n}\n", start)]
+    return re.sub(r"//.*", "", text[start:text.index("\n}\n", start)])
 
 
 def test_a_wait_that_ran_out_in_one_thread_is_known_to_all():
