@@ -72,7 +72,7 @@ def constrain(logits: torch.Tensor, policies: Sequence[Policy], histories: Seque
     which = np.cumsum([m is not None for m in masks]) - 1
     parts = [np.array([q if edits[q] else -1 for q in (owner if owner is not None else range(R))], dtype=np.int32),
              np.array([-1 if m is None else w for m, w in zip(masks, which)], dtype=np.int32),
-             np.array([p.penalty_window for p in policies], dtype=np.int32), first_bias, first_said, np.concatenate(said),
+             np.array([min(p.penalty_window, 2 ** 31 - 1) for p in policies], dtype=np.int32), first_bias, first_said, np.concatenate(said),
              np.array([i for b in biases for i, _ in b], dtype=np.int32),
              np.array([v for b in biases for _, v in b], dtype=np.float32),
              np.array([[p.repetition_penalty, p.presence_penalty, p.frequency_penalty] for p in policies], dtype=np.float32),
