@@ -2378,6 +2378,17 @@ def attention_tree_error() -> int:
     return int(value.value)
 
 
+def _over_each_other(rows: int, columns: int, a: int, a_stride: int, b: int, b_stride: int) -> bool:
+    """Whether rows of 32-bit numbers at addresses a and b lie over other rows of each other. Rows that alternate do not."""
+    if a == b:
+        return rows > 1 and a_stride != b_stride
+    if a >= b + 4 * ((rows - 1) * b_stride + columns) or b >= a + 4 * ((rows - 1) * a_stride + columns):
+        return False
+    if rows > 1 and a_stride == b_stride:
+        return not columns <= (b - a) / 4 % a_stride <= a_stride - columns
+    return True
+
+
 def logits_constrain(logits: torch.Tensor, owner: Optional[torch.Tensor] = None, bias=None, history=None,
                      penalties: Optional[torch.Tensor] = None, windows: Optional[torch.Tensor] = None, drafts=None,
                      allowed: Optional[torch.Tensor] = None, allowed_rows: Optional[torch.Tensor] = None,
@@ -2405,8 +2416,7 @@ def logits_constrain(logits: torch.Tensor, owner: Optional[torch.Tensor] = None,
     f32 = torch.float32
     assert logits.dtype is f32 and out.dtype is f32 and o_R == R and o_V == V and (V <= 1 or s1 == s2 == 1)
     assert R <= 1 or (s_in >= V and s_out >= V)
-    if R and V and (s_in != s_out if at == to else
-                    at < to + 4 * ((R - 1) * s_out + V) and to < at + 4 * ((R - 1) * s_in + V)):
+    if R and V and _over_each_other(R, V, at, s_in, to, s_out):
         raise KernelError("logits_constrain: `out` lies over other rows of the logits; the same rows, or rows of its own")
     b_first, ids, values = bias if bias is not None else (None, None, None)
     h_first, said = history if history is not None else (None, None)
