@@ -50,3 +50,42 @@ def test_one_row_has_no_stride():
     a.copy_(x)
     ops().logits_constrain(a, out=b, **c)
     close(a, plain_constrain(x, **c).to(DEV), x)
+
+
+@pytest.mark.parametrize("form", ["in place", "apart", "apart, at another boundary", "masked", "no owners"])
+def test_more_rows_than_a_grids_second_extent(form):
+    R, V = 65535 + 700, 37
+    many = lambda t: t.repeat(-(-R // 300), *[1] * (t.dim() - 1))[:R].contiguous()       # noqa: E731
+    x, c = constrained(300, V, 300 if form == "no owners" else 5, seed=3, owner=form != "no owners", bias=3,
+                       history=4 if form == "no owners" else 30, allowed=4 if form == "masked" else 0)
+    rows = many(x)
+    for name in ("owner", "allowed_rows"):
+        if c[name] is not None:
+            c[name] = many(c[name])
+    if form == "no owners":                                    # as many requests as rows
+        c["penalties"] = many(c["penalties"])
+        for name in ("bias", "history"):
+            first, *lists = c[name]
+            ends = many(first.diff()).cumsum(0).to(torch.int32)
+            c[name] = (torch.cat([first[:1], ends]), *[t.repeat(-(-R // 300)).contiguous() for t in lists])
+    small = slice(R - 300, R)
+    want = rows[small].clone()
+    part = dict(c, owner=torch.arange(R - 300, R, dtype=torch.int32, device=DEV) if c["owner"] is None else c["owner"][small].contiguous(),
+                allowed_rows=None if c["allowed_rows"] is None else c["allowed_rows"][small].contiguous())
+    ops().logits_constrain(want, **part)
+    out = None
+    if form.startswith("apart"):
+        shift = 1 if "another" in form else 0
+        out = torch.full((R * V + 4,), 5.0, device=DEV)[shift:shift + R * V].view(R, V)
+    start = rows.clone()
+    n = ops().LAUNCHES[0]
+    ops().logits_constrain(rows, out=out, **c)
+    got = rows if out is None else out
+    assert torch.equal(got[small], want)
+    first = slice(0, 300)
+    head = start[first].clone()
+    ops().logits_constrain(head, **dict(c, owner=torch.arange(300, dtype=torch.int32, device=DEV) if c["owner"] is None else c["owner"][first].contiguous(),
+                                        allowed_rows=None if c["allowed_rows"] is None else c["allowed_rows"][first].contiguous()))
+    assert torch.equal(got[first], head)
+    # (each of the other two counted one)
+    assert ops().LAUNCHES[0] - n == 1 + (2 if form in ("in place", "no owners", "apart, at another boundary") else 1)

@@ -39,6 +39,7 @@ struct Constrain {
     const int *draft_start, *draft_tokens; const unsigned long long* seen;
     const uint32_t* allowed; long long allowed_stride; int allowed_rows_n;
     const int* allowed_rows;
+    int row0;                                // of a launch whose blocks take a row each
 };
 
 __device__ __forceinline__ float lc_edit(float x, uint32_t count, float rep, float presence, float frequency) {
@@ -104,7 +105,7 @@ __device__ __forceinline__ const uint32_t* lc_mask(const Constrain& a, int r) {
 __global__ void __launch_bounds__(LI_THREADS) constrain_in_place_kernel(const Constrain a) {
     extern __shared__ __align__(16) uint32_t li_count[];
     pdl_wait();
-    const int tid = threadIdx.x, r = blockIdx.y, col0 = blockIdx.x * LI_COLUMNS;
+    const int tid = threadIdx.x, r = a.row0 + blockIdx.y, col0 = blockIdx.x * LI_COLUMNS;
     const uint32_t width = (uint32_t)min(LI_COLUMNS, a.vocab - col0);
     float* x = a.out + (long long)r * a.out_stride + col0;
     ConstrainRow row;
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(LI_THREADS) constrain_in_place_kernel(const Co
 __global__ void __launch_bounds__(LC_THREADS) constrain_kernel(const Constrain a) {
     __shared__ __align__(16) uint32_t count[LC_COLUMNS];
     pdl_wait();
-    const int tid = threadIdx.x, r = blockIdx.y, col0 = blockIdx.x * LC_COLUMNS;
+    const int tid = threadIdx.x, r = a.row0 + blockIdx.y, col0 = blockIdx.x * LC_COLUMNS;
     const int n_cols = min(LC_COLUMNS, a.vocab - col0);
     const float* src = a.logits + (long long)r * a.in_stride + col0;
     float* dst = a.out + (long long)r * a.out_stride + col0;
@@ -379,6 +380,17 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
 
 TGO_API int tgo_logits_constrain_error(int* value) { return (int)cudaMemcpyFromSymbol(value, drafts_error_flag, sizeof(int)); }
 
+// Launches of as many rows as a grid's second extent takes, mostly one.
+#define LC_ROWS 65535
+template <typename Launch> static int by_rows(Constrain& a, Launch&& launch) {
+    for (long long r = 0; r < a.rows; r += LC_ROWS) {
+        a.row0 = (int)r;
+        const int rc = launch(a.rows - a.row0 < LC_ROWS ? a.rows - a.row0 : LC_ROWS);
+        if (rc) return rc;
+    }
+    return 0;
+}
+
 // Addresses that are null leave their stage out. strides in elements (words for `allowed`).
 TGO_API int tgo_logits_constrain(const float* logits, long long in_stride, float* out, long long out_stride, int rows, int vocab,
                                  int requests, const int* owner, const int* bias_start, const int* bias_ids, const float* bias,
@@ -387,12 +399,12 @@ TGO_API int tgo_logits_constrain(const float* logits, long long in_stride, float
                                  long long allowed_stride, int allowed_rows_n, const int* allowed_rows, cudaStream_t stream) {
     if (rows <= 0 || vocab <= 0) return 0;
     const int slices = (vocab + LC_COLUMNS - 1) / LC_COLUMNS;
-    if (rows > 65535 || (rows > 1 && (in_stride < vocab || out_stride < vocab || (logits == out && in_stride != out_stride))) || requests < 0 ||
+    if ((rows > 1 && (in_stride < vocab || out_stride < vocab || (logits == out && in_stride != out_stride))) || requests < 0 ||
         (allowed && allowed_stride < (vocab + 31) / 32))
         return TGO_E_BAD_ARG;
     Constrain a = {logits, out, in_stride, out_stride, rows, vocab, requests, n_bias, n_history, n_drafts, owner, bias_start, bias_ids, bias, history_start, history,
                    penalties, windows, draft_start, draft_tokens, (const unsigned long long*)seen, (const uint32_t*)allowed,
-                   allowed_stride, allowed_rows_n, allowed_rows};
+                   allowed_stride, allowed_rows_n, allowed_rows, 0};
     if ((logits != out || allowed) && ((uintptr_t)logits - (uintptr_t)out) % 16 == 0 && (rows == 1 || (in_stride - out_stride) % 4 == 0) &&
         (long long)rows * ((vocab + 3) / LS_COLUMNS + 1) <= 0x7fffffffll) {
         constexpr size_t smem = (LS_RING + 1) * LS_COLUMNS * sizeof(float) + LS_RING * 8;
@@ -425,9 +437,11 @@ TGO_API int tgo_logits_constrain(const float* logits, long long in_stride, float
             set[dev] = true;
         }
         if (!bias_start && !penalties) return 0;
-        return tgo_launch_pdl(constrain_in_place_kernel, dim3((vocab + LI_COLUMNS - 1) / LI_COLUMNS, rows), dim3(LI_THREADS), smem, stream, a);
+        return by_rows(a, [&](int n) {
+            return tgo_launch_pdl(constrain_in_place_kernel, dim3((vocab + LI_COLUMNS - 1) / LI_COLUMNS, n), dim3(LI_THREADS), smem, stream, a);
+        });
     }
-    return tgo_launch_pdl(constrain_kernel, dim3(slices, rows), dim3(LC_THREADS), 0, stream, a);
+    return by_rows(a, [&](int n) { return tgo_launch_pdl(constrain_kernel, dim3(slices, n), dim3(LC_THREADS), 0, stream, a); });
 }
 
 // --------------------------------------------------------------------------- tree_accept

@@ -2448,6 +2448,8 @@ def logits_constrain(logits: torch.Tensor, owner: Optional[torch.Tensor] = None,
         at, s_in, to, s_out, R, V, Q, p_owner, b0, b1, b2, n_bias, h0, h1, n_history, p_pen, p_win, d0, d1, n_drafts, d2, words, width, m,
         p_rows, _stream())
     _check(status, "logits_constrain", f"(R={R}, V={V})" if status else "")
+    if R > 65535 and (at == to and not words or (to - at) % 16 or (s_out - s_in) % 4):
+        LAUNCHES[0] += (R - 1) // 65535       # by the kernels that go a row a block
 
 
 def logits_constrain_error() -> int:
