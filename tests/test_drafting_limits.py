@@ -1,0 +1,30 @@
+"""Models that drafted steps do not take are refused by name before anything runs; no GPU."""
+import pytest
+
+import tiny
+from test_beam_search import cpu_model
+from test_drafting import emulated                                # noqa: F401  (a fixture)
+from tgo_b200.engine.drafts import DraftedGeneration
+from tgo_b200.engine.step import DraftEntry
+from tgo_b200.sampling.policy import Policy
+
+
+@pytest.mark.parametrize("dim,taken", [(64, True), (256, True), (258, False), (320, False), (512, False)])
+def test_heads_wider_than_the_attention_of_trees_takes(emulated, tmp_path, dim, taken):        # noqa: F811
+    cfg = dict(tiny.TINIES["A"][0], head_dim=dim)
+    d = tiny.make_model_dir(tmp_path / "m", cfg, 1, 0.05)
+    model = cpu_model(d, cfg)
+    eng = model.new_engine(page_size=8, max_tokens=100, num_slots=1)
+    if taken:
+        assert eng.takes_drafts() is None
+        return
+    assert str(dim) in eng.takes_drafts()
+    with pytest.raises(ValueError, match=f"heads of {dim}"):
+        DraftedGeneration(eng)
+    with pytest.raises(ValueError, match=f"heads of {dim}"):
+        model.generate_drafted([[1, 2]], Policy(max_tokens=3))
+    eng.admit("a")
+    with pytest.raises(ValueError, match=f"heads of {dim}"):
+        eng.draft_step([DraftEntry("a", [1], [-1])], None)
+    assert eng.cache.requests["a"].held(0) == []
+    assert len(model.generate([[1, 2]], Policy(max_tokens=3))[0]) == 3

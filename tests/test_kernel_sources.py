@@ -28,3 +28,12 @@ def test_a_wait_that_ran_out_in_one_thread_is_known_to_all():
     assert re.search(r"if \(!ok\) tg_settle_copies\(full", body[leave:])
     # nobody's own answer between the two
     assert "__syncthreads_or(!ok)" not in "".join(source(f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh")))
+
+
+def test_limits_are_those_of_the_sources():
+    from tgo_b200.kernels import ops
+    tree, drafts = source("attention_tree.cu"), source("drafts.cu")
+    assert [int(re.search(rf"#define {name} (\d+)", text).group(1)) for name, text in (("TREE_NODES", tree), ("DR_NODES", drafts))] == \
+        [ops.TREE_NODES] * 2
+    assert f"dh > {ops.TREE_HEAD} " in tree[tree.index("TGO_API int tgo_attention_tree(const"):]
+    assert int(re.search(r"#define LC_ROWS (\d+)", drafts).group(1)) == 65535

@@ -313,6 +313,8 @@ class Engine:
             mixer = self.model.blocks[call.layer].mixer
             if not getattr(mixer, "takes_drafts", False):
                 return f"its mixer {type(mixer).__name__} takes no trees of tokens"
+            if getattr(mixer, "refuses_drafts", None):
+                return f"its mixer {type(mixer).__name__} takes no trees of tokens with {mixer.refuses_drafts}"
         if self.storage.state:
             return "it keeps a state per request, which cannot go back to the token before a draft"
         return None

@@ -2306,6 +2306,7 @@ _tc_err = {}
 
 
 TREE_NODES = 64          # drafted tokens of a request that the kernels take: what a node sees is a 64-bit number
+TREE_HEAD = 256          # widest heads that attention_tree takes
 
 
 @functools.lru_cache(maxsize=256)
@@ -2327,7 +2328,11 @@ def attention_tree(q: torch.Tensor, out: torch.Tensor, num_heads: int, num_kv_he
 
     q, out [T, >= heads * head_dim] float32 or bfloat16, rows may be strided; k_cache, v_cache [pages, kv heads, page_size,
     head_dim] of that type; block_tables int32 [B, width], context_lens int32 [B], q_start int32 [B + 1], seen int64
-    [T]. head_dim at most 256. max_nodes, max_context: the most that any request of the call has."""
+    [T]. head_dim at most 256, scale positive. max_nodes, max_context: the most that any request of the call has.
+
+    Among the nodes `window` says nothing: a path that is longer than the window has to leave the bits of the nodes outside it
+    out (Engine.draft_step takes none that is). bfloat16 calls on the tensor cores round the weights to bfloat16
+    for their product with V (at most 2^-8 of a weight; their sum is of 32 bits)."""
     kind, shape = q.dtype, k_cache.shape
     code = dtype_code(kind)
     kinds = "ffiiil" if code == F32 else "bbiiil"

@@ -281,6 +281,12 @@ class GQAAttention(Part):
     lazy_rows = True        # x may come as ops.NormedRows; its first product folds the norm in
     takes_drafts = True     # steps whose tokens are trees of drafts
 
+    @property
+    def refuses_drafts(self):
+        if self.dh > ops.TREE_HEAD:
+            return f"heads of {self.dh}: at most {ops.TREE_HEAD}"
+        return None if self.scale > 0 else f"scores times {self.scale}"
+
     def forward(self, x, ctx, cache: LayerCache, residual=None):
         """With `residual` (the float32 stream) the result may be added to it, and None is
         then returned; otherwise the result is returned for the caller to add."""

@@ -43,7 +43,8 @@ that offers none of them still runs):
                   would otherwise make on the host during the step (lists derived from the
                   step's shape), leaving it in ctx.aux under a key that starts with "tiles";
   takes_drafts = True (a mixer's class): its forward takes a step of drafted tokens (`ctx.seen`), whose
-                  requests' tokens are trees; an engine refuses drafted steps of a model with other mixers;
+                  requests' tokens are trees; an engine refuses drafted steps of a model with other mixers,
+                  and of one whose mixer's `refuses_drafts` is not None but says why;
   adapter_sites() -> the products whose results a request's low-rank adapter may add to
                   (`AdapterSite`), and bind_adapters(banks) -> take {site's key: AdapterBank}: the
                   forward then calls `bank.add(rows, result, ctx)` behind the product;
