@@ -2,6 +2,7 @@
 import pytest
 
 import tiny
+from emulated_drafts import Oracle
 from test_beam_search import cpu_model
 from test_drafting import emulated                                # noqa: F401  (a fixture)
 from tgo_b200.engine.drafts import DraftedGeneration
@@ -28,3 +29,16 @@ def test_heads_wider_than_the_attention_of_trees_takes(emulated, tmp_path, dim, 
         eng.draft_step([DraftEntry("a", [1], [-1])], None)
     assert eng.cache.requests["a"].held(0) == []
     assert len(model.generate([[1, 2]], Policy(max_tokens=3))[0]) == 3
+
+
+@pytest.mark.parametrize("nodes,wrong,steps", [(1, 0, 19), (2, 0, 10), (2, 1, 19), (5, 0, 4), (4, 1, 10), (64, 0, 1)])
+def test_steps_that_right_drafts_take(emulated, tmp_path, nodes, wrong, steps):        # noqa: F811
+    """20 tokens, the first of them from the prompt: a step gives as many as its path has. Beside a right draft `wrong`
+    others come first, with one behind the last of them."""
+    d = tiny.make_model_dir(tmp_path / "m", tiny.TINIES["A"][0], 1, 0.2)
+    model = cpu_model(d, tiny.TINIES["A"][0])
+    prompt = [5, 9, 11, 3]
+    text = prompt + model.generate([prompt], Policy(max_tokens=20), page_size=4)[0]
+    got = model.generate_drafted([prompt], Policy(max_tokens=20), nodes=nodes, page_size=4,
+                                 drafter=Oracle([text], 30, wrong, tiny.TINIES["A"][0]["vocab_size"]))
+    assert prompt + got[0] == text and model.last_drafts.steps == steps
