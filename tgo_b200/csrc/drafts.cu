@@ -17,7 +17,8 @@ __device__ __forceinline__ void dr_span(const int* start, int i, int n, int& lo,
 //   c = how often i stands in the last `window` tokens of (q's history, then the drafted tokens of r's own path)
 //   c > 0:  x = x > 0 ? x / repetition : x * repetition;  x -= presence + frequency * c
 //   not allowed: x = -inf
-// the order and the arithmetic of the sampler's single rows (adjust_kernel of sampling.cu), so that both give the same bits.
+// the order and the arithmetic of adjust_kernel (sampling.cu), which edits one row from counts made on the host and which the tests
+// hold this to: both give the same bits.
 // (Counts are integers: the order of the additions changes nothing.)
 #define LC_THREADS 256
 #define LC_COLUMNS 8192
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(LS_THREADS, LS_BLOCKS) constrain_stream_kernel
                 const int token = a.history[i];
                 if (token >= 0 && (uint32_t)(token - col0) < width) edit(token);
             }
-            __syncthreads();                                   // the next slice row.counts there
+            __syncthreads();                                   // the next slice's tokens are counted in the same places
         }
         if (mask) {
 #pragma unroll

@@ -20,7 +20,9 @@
 // ---------------------------------------------------------------- bias and penalties
 // Sparse edits of one row: logits[bias_ids[i]] += bias[i]; then for each distinct history
 // token (ids, counts): repetition (divide a positive logit, multiply otherwise), then
-// subtract presence + frequency * count (sample/stages.go:152-190).
+// subtract presence + frequency * count (sample/stages.go:152-190). Rows are edited by
+// logits_constrain (drafts.cu), all of a batch at once; this plain form of one row is what
+// the tests compare it with, bit for bit.
 __global__ void adjust_kernel(float* __restrict__ row, const int* __restrict__ bias_ids,
                               const float* __restrict__ bias, int n_bias,
                               const int* __restrict__ ids, const int* __restrict__ counts, int n_ids,

@@ -2145,7 +2145,8 @@ def logits_adjust(row: torch.Tensor, bias_ids: Optional[torch.Tensor],
                   counts: Optional[torch.Tensor], repetition: float, presence: float,
                   frequency: float) -> None:
     """Edit one row of logits in place: add the biases, then apply the penalties to the
-    distinct history tokens `ids` with their `counts`."""
+    distinct history tokens `ids` with their `counts`. The sampler edits all rows of a batch by
+    `logits_constrain`; this is the plain form that the tests hold it to."""
     _need_cuda(row, bias_ids, bias, ids, counts)
     assert row.dtype == torch.float32 and row.dim() == 1 and row.is_contiguous()
     nb = 0 if bias_ids is None else bias_ids.numel()

@@ -21,7 +21,7 @@ from .policy import DrawStream, Policy, TokenProb
 
 
 def penalty_counts(history: Sequence[int], window: int):
-    """Distinct tokens of the last `window` tokens of history (0: all) with their counts."""
+    """Distinct tokens of the last `window` tokens of history (0: all) with their counts: for `adjust_row`."""
     h = list(history)
     if window > 0 and len(h) > window:
         h = h[-window:]
@@ -31,6 +31,7 @@ def penalty_counts(history: Sequence[int], window: int):
 
 
 def adjust_row(row: torch.Tensor, policy: Policy, history: Sequence[int]) -> None:
+    """One row edited from counts made on the host: the plain form that the tests hold `constrain` to."""
     dev = row.device
     bias_ids = bias = ids = counts = None
     if policy.logit_bias:
