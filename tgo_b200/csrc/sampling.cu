@@ -314,16 +314,19 @@ sample_kernel(const float* __restrict__ logits, long long stride, int V,
         }
         __syncthreads();
         if (t == (first_s < SM_THREADS ? first_s : last_s)) {
-            // the running sum may end below the range's: then it is the last id with weight
             float acc = part[t];
-            int pick = c1 - 1;
-            for (int i = c0; i < c1; ++i) {
-                const float w = expf(row[i] / T - m);
-                acc += w;
-                if (w > 0.f) {
-                    pick = i;
-                    if (acc > target) break;
+            int pick = -1;
+            if (acc <= target)
+                for (int i = c0; i < c1; ++i) {
+                    acc += expf(row[i] / T - m);
+                    if (acc > target) { pick = i; break; }
                 }
+            // a range that begins above the target: its first id with weight; a running sum that ends below the
+            // range's: its last
+            const bool first = acc > target;
+            for (int i = c0; i < c1 && pick < 0; ++i) {
+                const int j = first ? i : c1 - 1 - (i - c0);
+                if (expf(row[j] / T - m) > 0.f) pick = j;
             }
             result_s = pick;
         }
