@@ -70,8 +70,8 @@ class _Live:
 
 class DraftedGeneration:
     """Requests through an engine with drafted tokens: a prompt is run when its request is admitted, then every turn is one
-    step of all live requests' trees. When pages run out, a turn goes without drafts, and if that does not help the request
-    that was admitted last gives its pages back and is run again later."""
+    step of all live requests' trees, or a decode step where no request has a draft. When pages run out, a turn goes
+    without drafts, and if that does not help the request that was admitted last gives its pages back and is run again later."""
 
     def __init__(self, engine: Engine, drafter=None, nodes: int = 16, chunk: int = 2048, stop_ids: Sequence[int] = ()):
         why = engine.takes_drafts()
@@ -179,7 +179,10 @@ class DraftedGeneration:
         while True:
             reqs = [one.request for one in live]
             try:
-                got = self.engine.draft_step(entries, lambda logits, ctx: self._choose(logits, ctx, reqs, entries, reports, stuck))
+                if any(len(e.tokens) > 1 for e in entries):
+                    got = self.engine.draft_step(entries, lambda logits, ctx: self._choose(logits, ctx, reqs, entries, reports, stuck))
+                else:                                         # a decode step as any other, from a graph where there is one
+                    got, logits = None, self.engine.step([StepEntry(e.request_id, e.tokens, [0]) for e in entries])
                 break
             except PagesExhausted:
                 if any(len(e.tokens) > 1 for e in entries):
@@ -194,6 +197,10 @@ class DraftedGeneration:
                 waiting.insert(0, gone.request)
                 entries.pop()
         self.steps += 1
+        if got is None:
+            for one, t in zip(list(live), sample_rows(logits, reqs)):
+                self._take(one, [int(t)], live)
+            return
         at = 0
         for one, e, a in zip(list(live), entries, got):
             req = one.request
