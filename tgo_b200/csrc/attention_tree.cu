@@ -448,8 +448,8 @@ __global__ void __launch_bounds__(TP_THREADS) tree_plain_kernel(
 // r / G, head r % G) make one tile of 128 rows or, for wide trees, two, which share the item's K and V. One persistent CTA an
 // SM walks its pieces.
 //
-// The softmax of a tile takes longer than its two products, most of it in the special-function unit, which idles while
-// scores are read, maxima found and products waited for. So there are two streams, each with scores S, sums O, a running
+// The softmax of a tile takes longer than its two products: a warp's line of scores read, maxima found, exponentials, sums and
+// weights stored, each behind the other (fewer exponentials for the special-function unit changed nothing). So there are two streams, each with scores S, sums O, a running
 // maximum and a sum of exponentials of its own, and four softmax warps, a thread a row, that need nothing of each other:
 // two row tiles, or, where there is one, the first and the second half of every key tile, put together at the item's end. A
 // step of a stream is 64 keys, and its scores have two buffers: the next step's are made while this one's exponentials run.
@@ -1279,7 +1279,12 @@ static int tree_tiles(const TreeWork& w, int max_context, int keys) {
 //    8            40,         8000       73.6     74.5      129.3     69.3
 // Whole items run in rounds of one an SM; cutting costs a join and a beginning and an end for every piece, and shares all tiles out
 // evenly. Straight lines through 65 such measurements: us for a call, a round or an item of each SM, and a key tile. The cheapest by
-// them is within 11 % of the fastest measured (within 3 % in 63 of the 65).
+// them is within 11 % of the fastest measured (within 3 % in 63 of the 65). The lines know nothing of other layouts and of windows beyond
+// the count of items and tiles; they hold for them: in 54 calls (heads of 64, groups of 1, 5 and 8, a window of 1024; 1 to 32 requests of 4 to
+// 64 nodes over 300 to 8000 keys) the chosen way is within 3 % of the fastest, e.g.
+//   16 over 2 of  64,  8 requests of 16, 4000   35.1     15.6
+//   40 over 8 of 128, 16             8,  2000   31.1     33.2
+//   64 over 8 of 128, 12            23,  window 35.4     40.8      30.5     39.8
 static void tree_choose(TreeWork& w, int max_context, int G, int sms) {
     const int tokens = TT_ROWS / G, t = tree_tiles(w, max_context, TT_KEYS);
     double best = 0;

@@ -101,8 +101,8 @@ __device__ __forceinline__ const uint32_t* lc_mask(const Constrain& a, int r) {
 // takes the count out, and, if it was the first to come, edits the column.
 //   MEASURED, in a graph of calls: 64 rows of 151936 with histories of 4001 tokens 13.5 us (18.7 by the copying kernel below, which
 // takes the rows over in place where there are masks: 14.9 with masks alone), of 300 5.9; 128 rows, 600 tokens 10.7 (28.2);
-// one row, 700 tokens 2.8. Bound by latency and by every slice's look at the row's whole history: slices of 8192 17.6 and
-// 16.7 us for 13.5 and 10.7, of 32768 17.8 and 14.1.
+// one row, 700 tokens 2.8. What changes, by 32 bytes, and the histories are 10 and 3 MB (1.4 and 0.5 us): bound by latency and by
+// every slice's look at the row's whole history: slices of 8192 17.6 and 16.7 us for 13.5 and 10.7, of 32768 17.8 and 14.1.
 __global__ void __launch_bounds__(LI_THREADS) constrain_in_place_kernel(const Constrain a) {
     extern __shared__ __align__(16) uint32_t li_count[];
     pdl_wait();
